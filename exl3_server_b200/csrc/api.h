@@ -456,4 +456,23 @@ int exl3_embed_sinusoid(const int* ids, const int* tok_pos, const void* table, i
 // type, K and the pitch of x multiples of 16 bytes.
 int exl3_gemm_few_out(const void* x, int64_t ldx, const void* w, const void* bias, float* y, int in_dtype, int M, int N,
                       int K, cudaStream_t stream);
+// The 4-bit key/value cache (format: cache4.cuh).  Bytes of a page of 64 tokens of one key/value head; 0 for heads it does not take.
+int exl3_kv4_page_bytes(int hd);
+// q, k, v [T, (nh + 2 nkv) * hd] bfloat16: q rotated into q_out [T, nh * hd], k (rotated) and v into the pages of the tokens' positions.  freq: hd / 2
+// frequencies (null: no rotation), freq_lo: what float32 lost of them, or null.
+int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float* freq, const float* freq_lo, const int* tok_pos,
+                   const int* tok_seq, const int* block_table, int bt_stride, void* pool, int64_t n_pages, int T, int nh, int nkv, int hd,
+                   cudaStream_t stream);
+// What the listed pages stand for, [n, nkv, 64, hd] bfloat16 each (zeros for a number that is no page's).  table_out (or null): entry i becomes i
+// where there is a page, else -1, and nothing is written for it.
+int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
+                  int* table_out, cudaStream_t stream);
+// Attention of one token or a few per row over the 4-bit cache.  Row r has tokens row_start[r] .. row_start[r + 1] - 1 (null: token r) at positions
+// row_pos0[r] ...; chunk: tiles of 4096 / hd keys that a block walks, max_chunks: chunks of the longest row (window's reach).
+long long exl3_kv4_attn_scratch(int rows, int max_new, int nh, int nkv, int hd, int max_chunks);
+int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
+                  const int* row_start, const int* row_pos0, int rows, int max_new, int nh, int nkv, int hd, int window, float scale,
+                  int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream);
+// Code left by a bounded wait that ran out (0: none); cleared by the call.
+int exl3_kv4_attn_status();
 }

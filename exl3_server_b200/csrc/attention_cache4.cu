@@ -1,0 +1,581 @@
+// Attention of a step's new tokens over the 4-bit key/value cache (cache4.cuh), for one token or a few per sequence:
+//
+//   s[j] = (q . K[j]) * scale,   j in [max(0, p - window + 1), p] for the token at position p
+//   out  = sum_j softmax(s)[j] * V[j],   K[j] = mn + sc * code by groups of 32 features, V likewise
+//
+// The codes go to the tensor cores as they are.  A code of 4 bits in the low bits of a 16-bit float is a subnormal of fp16, code * 2^-24
+// (or, one nibble up, 16 times that), so one AND makes two operands out of a word and no conversion is done at all; the groups'
+// numbers come in where there is less to multiply.  With q' the query in fp16, scaled by a power of two so that its largest value lies in
+// [1024, 2048), and odd pairs of features divided by 16:
+//
+//   q . K[j] = sum_groups (sc_g * C_g + mn_g * Q_g),   C_g = the product of codes and q' (mma.m16n8k16, keys x features the 16-row operand,
+//   the queries its 8 columns), Q_g = the sum of the group's q'
+//
+// and for the values, with p the softmax's terms, P_g = p * sc_g * F in fp16 (F a power of two that keeps the largest scale seen so far at 2^14:
+// the probabilities keep their 11 bits down to 2^-28 of the largest) as the second product's operand, the codes of 16 tokens the 16-row one, and
+// sum p mn_g beside it in float32.  Scores, maximum, sums and outputs are float32; q is exact in fp16 (bfloat16 has fewer bits) unless it is
+// 2^-20 of the row's largest.
+//
+// A column is a (new token, query head) of one key/value head: up to 8 or 16 columns share a walk over the codes, each with its own causal limit.
+// A block of four warps takes one (row, key/value head, group of columns, chunk of keys); its warps take every fourth tile of 5,120
+// bytes, through a ring each that bulk copies fill ahead.  The warps' results meet in shared memory.  Where a row has several chunks their
+// records go to scratch memory and a second kernel joins them, in the chunks' order.
+#include "api.h"
+#include "cache4.cuh"
+
+#include <cuda_fp16.h>
+#include <type_traits>
+
+namespace exl3 {
+
+using namespace kv4;
+
+constexpr int A4_WARPS = 4;
+constexpr int A4_STAGES = 3;
+constexpr int A4_MAX_CHUNK = 32 * A4_WARPS;               // tiles: a warp keeps its page numbers one a lane
+constexpr uint32_t A4_WAIT_LIMIT = 1u << 22;              // polls of some tens of cycles: a fraction of a second
+
+static __device__ int g_a4_error = 0;
+
+__device__ inline uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ inline bool a4_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = a4_smem(bar);
+  for (uint32_t i = 0; i < A4_WAIT_LIMIT; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+// fp16 x fp16 -> float32, 16 x 8 x 16.
+__device__ inline void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ inline uint32_t a4_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ inline float a4_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ inline uint32_t a4_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ inline float a4_pow2(int e) { return __int_as_float((e + 127) << 23); }       // e in -126 .. 127
+
+struct A4Args {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  __nv_bfloat16* out;
+  const unsigned char* pool;
+  int n_pages;
+  const int* block_table;
+  int bt_stride;
+  const int* row_start;      // null: row r is token r
+  const int* row_pos0;
+  int nh, nkv, window;
+  float scale_log2;          // softmax scale * log2(e)
+  int chunk;                 // tiles of a chunk, aligned to absolute positions
+  int max_chunks;            // chunks that the grid (and the scratch) has room for
+  int n_ct;                  // groups of columns the grid has room for
+  float* scratch;            // [rows][nkv][n_ct][max_chunks][columns][HD + 2] where max_chunks > 1
+};
+
+// What a (row, group of columns) sees: tiles t_lo .. t_hi, and the chunks that hold them.  Both kernels ask.
+template <int HD> struct A4Range {
+  int start, n_new, G, col0, cols, pos0, t_lo, t_hi, c_first, n_chunks;
+  __device__ inline A4Range(const A4Args& a, int row, int ct, int columns) {
+    start = a.row_start ? __ldcg(a.row_start + row) : row;
+    n_new = a.row_start ? __ldcg(a.row_start + row + 1) - start : 1;
+    pos0 = __ldcg(a.row_pos0 + row);
+    G = a.nh / a.nkv;
+    col0 = ct * columns;
+    cols = min(columns, n_new * G - col0);
+    t_lo = 0; t_hi = -1; c_first = 0; n_chunks = 0;
+    if (cols <= 0) return;
+    const int p_lo = pos0 + col0 / G, p_hi = pos0 + (col0 + cols - 1) / G;
+    if (p_hi < 0) return;
+    t_lo = a.window > 0 ? max(0, p_lo - a.window + 1) / tile_tokens(HD) : 0;
+    t_hi = p_hi / tile_tokens(HD);
+    c_first = t_lo / a.chunk;
+    n_chunks = min(t_hi / a.chunk - c_first + 1, a.max_chunks);
+  }
+};
+
+template <int HD, int NC>
+__global__ void __launch_bounds__(A4_WARPS * 32, NC == 1 ? 3 : 2)
+kv4_attn_kernel(const A4Args a) {
+  constexpr int COLS = 8 * NC, TT = tile_tokens(HD), NT = TT / 16, NG = HD / 32, SPP = HD / 64;
+  constexpr int RING = A4_STAGES * TILE;
+  static_assert(COLS * HD * 4 <= RING, "a warp's results take the place of its ring");
+  extern __shared__ __align__(128) unsigned char a4_smem_raw[];
+  __shared__ uint64_t full[A4_WARPS][A4_STAGES];
+  __shared__ __align__(16) uint32_t s_q[COLS][HD / 2];      // q' in fp16 pairs
+  __shared__ float s_qsum[COLS][NG], s_f[COLS];
+  __shared__ float s_m[A4_WARPS][COLS], s_l[A4_WARPS][COLS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int row = blockIdx.z, kvh = blockIdx.y / a.n_ct, ct = blockIdx.y % a.n_ct;
+  pdl_trigger();
+  pdl_wait();
+  const A4Range<HD> r(a, row, ct, COLS);
+  if (r.cols <= 0 || (int)blockIdx.x >= max(r.n_chunks, 1)) return;
+  const int chunk0 = (r.c_first + (int)blockIdx.x) * a.chunk;
+  const int tile_a = max(r.t_lo, chunk0), tile_b = min(r.t_hi + 1, chunk0 + a.chunk);      // none where the row sees nothing
+
+  // this warp's tiles, one a lane: tile_a + warp + 4 * lane; tiles without a page are left out
+  int my_page = -1;
+  {
+    const int tile = tile_a + warp + A4_WARPS * lane;
+    if (tile < tile_b && tile / SPP < a.bt_stride) my_page = __ldcg(a.block_table + (int64_t)row * a.bt_stride + tile / SPP);
+    if (my_page >= a.n_pages) my_page = -1;
+  }
+  uint32_t todo = __ballot_sync(0xffffffffu, my_page >= 0), ask = todo;
+  unsigned char* ring = a4_smem_raw + warp * RING;
+  uint64_t* bars = full[warp];
+  if (lane == 0) {
+    for (int s = 0; s < A4_STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(a4_smem(bars + s)));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncwarp();
+  auto request = [&](int stage) {                           // the next tile of `ask` into a stage
+    const int i = __ffs(ask) - 1;
+    ask &= ask - 1;
+    const int page = __shfl_sync(0xffffffffu, my_page, i);
+    if (lane == 0) {
+      const int tile = tile_a + warp + A4_WARPS * i;
+      const unsigned char* src = a.pool + ((int64_t)page * a.nkv + kvh) * page_bytes(HD) + tile % SPP * TILE;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a4_smem(bars + stage)), "r"(TILE) : "memory");
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   ::"r"(a4_smem(ring + stage * TILE)), "l"(src), "r"(TILE), "r"(a4_smem(bars + stage)) : "memory");
+    }
+  };
+  for (int s = 0; s < A4_STAGES; ++s)
+    if (ask) request(s);
+
+  // the queries: a warp takes every fourth column
+  for (int c = warp; c < COLS; c += A4_WARPS) {
+    float x[NG];
+    float top = 0.0f;
+    const int col = r.col0 + c;
+    const __nv_bfloat16* src = a.q + (int64_t)(r.start + col / r.G) * a.q_stride + (int64_t)(kvh * r.G + col % r.G) * HD;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      x[i] = c < r.cols ? __bfloat162float(src[i * 32 + lane]) : 0.0f;
+      top = fmaxf(top, fabsf(x[i]));
+    }
+    top = warp_max(top);
+    // the exponent that brings the largest value to [2^10, 2^11); a row of zeros, or one that is not finite, stays as it is
+    int e = 0;
+    if (top > 0.0f && top < __int_as_float(0x7f800000)) e = min(max(10 - (int)((__float_as_uint(top) >> 23) & 255) + 127, -100), 100);
+    const float up = a4_pow2(e);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const __half h = __float2half_rn(x[i] * up);
+      const float sum = warp_sum(__half2float(h));
+      if (lane == 0) s_qsum[c][i] = sum * 0x1p-24f;
+      // pairs 1 and 3 of eight features meet codes 16 times as large
+      reinterpret_cast<__half*>(s_q[c])[i * 32 + lane] = (lane & 2) ? __float2half_rn(x[i] * up * 0.0625f) : h;
+    }
+    if (lane == 0) s_f[c] = a.scale_log2 * a4_pow2(24 - e > 127 ? 127 : 24 - e);
+  }
+  __syncthreads();
+
+  uint32_t qf[NC][NG][4];                                   // this lane's part of q': features 32 group + 8 t .. + 7 of column g
+  float qs[NC][NG][2], fac[NC][2];
+  int limit[NC][2];                                         // the positions of columns 2 t, 2 t + 1
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(&s_q[8 * n + g][i * 16 + 4 * t]);
+      qf[n][i][0] = v.x; qf[n][i][1] = v.y; qf[n][i][2] = v.z; qf[n][i][3] = v.w;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = 8 * n + 2 * t + h;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) qs[n][i][h] = s_qsum[c][i];
+      fac[n][h] = s_f[c];
+      limit[n][h] = c < r.cols ? r.pos0 + (r.col0 + c) / r.G : -1;
+    }
+  }
+  // keys that every column sees: full_lo .. full_hi
+  const int full_hi = r.pos0 + r.col0 / r.G;
+  const int full_lo = a.window > 0 ? r.pos0 + (r.col0 + r.cols - 1) / r.G - a.window + 1 : 0;
+
+  float o[NC][NG][2][4] = {};                               // [column block][group][features 4 g + 2 k (+ 1)] x columns 2 t, 2 t + 1, in units of 2^-24 F
+  float om[NC][NG][2] = {};                                 // sum p mn, this lane's tokens
+  float m[NC][2], l[NC][2] = {};
+#pragma unroll
+  for (int n = 0; n < NC; ++n) m[n][0] = m[n][1] = __int_as_float(0xff800000);
+  uint32_t sc_top = 0;                                      // the largest value scale met, rounded up to a power of two (as its exponent bits)
+  float F = 1.0f;
+
+  auto walk = [&](const unsigned char* buf, int key0, auto masked_t) {
+    constexpr bool MASKED = decltype(masked_t)::value;
+    float x[NT][NC][4];
+#pragma unroll
+    for (int mt = 0; mt < NT; ++mt) {
+      uint32_t kw[2][NG], pw[2][NG];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tok = mt * 16 + g + 8 * h;
+        const unsigned char* kp = buf + tok * (HD / 2) + t * (NG * 4);
+        const unsigned char* pp = buf + K_WORDS + tok * (NG * 4);
+        if constexpr (NG == 2) {
+          const uint2 u = *reinterpret_cast<const uint2*>(kp), v = *reinterpret_cast<const uint2*>(pp);
+          kw[h][0] = u.x; kw[h][1] = u.y; pw[h][0] = v.x; pw[h][1] = v.y;
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(kp), v = *reinterpret_cast<const uint4*>(pp);
+          kw[h][0] = u.x; kw[h][1] = u.y; kw[h][2] = u.z; kw[h][3] = u.w;
+          pw[h][0] = v.x; pw[h][1] = v.y; pw[h][2] = v.z; pw[h][3] = v.w;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[mt][n][e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const uint32_t u0 = kw[0][i], u1 = kw[1][i], s0 = u0 >> 8, s1 = u1 >> 8;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          float c[4] = {};
+          a4_mma(c, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[n][i][0], qf[n][i][1]);
+          a4_mma(c, s0 & 0x000f000fu, s1 & 0x000f000fu, s0 & 0x00f000f0u, s1 & 0x00f000f0u, qf[n][i][2], qf[n][i][3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[mt][n][e] = fmaf(word_sc(pw[e >> 1][i]), c[e], fmaf(word_mn(pw[e >> 1][i]), qs[n][i][e & 1], x[mt][n][e]));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[mt][n][e] *= fac[n][e & 1];
+          if (MASKED) {
+            const int key = key0 + mt * 16 + g + 8 * (e >> 1), lim = limit[n][e & 1];
+            if (key > lim || (a.window > 0 && lim - key >= a.window)) x[mt][n][e] = __int_as_float(0xff800000);
+          }
+        }
+    }
+    // the running maximum of a column, over the lanes that share it
+    float alpha[NC][2], mm[NC][2];
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v = x[0][n][h];
+#pragma unroll
+        for (int mt = 0; mt < NT; ++mt) v = fmaxf(v, fmaxf(x[mt][n][h], x[mt][n][h + 2]));
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+        const float next = fmaxf(m[n][h], v);
+        mm[n][h] = next == __int_as_float(0xff800000) ? 0.0f : next;
+        alpha[n][h] = a4_exp2(m[n][h] - mm[n][h]);
+        moved = moved || next != m[n][h];
+        m[n][h] = next;
+      }
+    // the values' numbers, and the power of two that keeps the largest scale in fp16's range
+    uint32_t vw[NT][2][NG];
+    uint32_t top = 0;
+#pragma unroll
+    for (int mt = 0; mt < NT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char* pp = buf + V_WORDS + (mt * 16 + g + 8 * h) * (NG * 4);
+        if constexpr (NG == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(pp);
+          vw[mt][h][0] = v.x; vw[mt][h][1] = v.y;
+        } else {
+          const uint4 v = *reinterpret_cast<const uint4*>(pp);
+          vw[mt][h][0] = v.x; vw[mt][h][1] = v.y; vw[mt][h][2] = v.z; vw[mt][h][3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i] < 0x7f800000u ? vw[mt][h][i] : 0u);      // (NaN groups do not count)
+      }
+    top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
+    float keep = 1.0f;
+    if (top > sc_top) {                                     // (the same for the whole warp)
+      const float old = F;
+      sc_top = top;
+      F = a4_pow2(min(max(13 - ((int)(top >> 23) - 127), -100), 100));
+      keep = F / old;
+      moved = true;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float f = alpha[n][h] * keep;
+          l[n][h] *= alpha[n][h];
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            om[n][i][h] *= alpha[n][h];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) { o[n][i][k][h] *= f; o[n][i][k][h + 2] *= f; }
+          }
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < NT; ++mt) {
+      uint32_t pb[NC][NG][2];                               // P_g, tokens x columns, transposed
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = a4_exp2(x[mt][n][e] - mm[n][e & 1]);
+          l[n][e & 1] += p[e];
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float sc = word_sc(vw[mt][e >> 1][i]) * F, mn = word_mn(vw[mt][e >> 1][i]);
+            if (MASKED && x[mt][n][e] == __int_as_float(0xff800000)) {       // what is hidden may hold anything
+              w[e] = 0.0f;
+            } else {
+              w[e] = p[e] * sc;
+              om[n][i][e & 1] = fmaf(p[e], mn, om[n][i][e & 1]);
+            }
+          }
+          pb[n][i][0] = a4_transpose(a4_pack(w[0], w[1]));
+          pb[n][i][1] = a4_transpose(a4_pack(w[2], w[3]));
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < NG / 2; ++half) {
+        const uint4 v = *reinterpret_cast<const uint4*>(buf + V_CODES + ((mt * (NG / 2) + half) * 32 + lane) * 16);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const uint32_t lo = __byte_perm(v.x, v.y, part ? 0x7632 : 0x5410), hi = __byte_perm(v.z, v.w, part ? 0x7632 : 0x5410);
+          const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+          const int i = half * 2 + part;
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            a4_mma(o[n][i][0], lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u, pb[n][i][0], pb[n][i][1]);
+            a4_mma(o[n][i][1], lo8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x000f000fu, hi8 & 0x00f000f0u, pb[n][i][0], pb[n][i][1]);
+          }
+        }
+      }
+    }
+  };
+
+  bool ok = true;
+  int k = 0;
+  while (todo) {
+    const int i = __ffs(todo) - 1, stage = k % A4_STAGES;
+    todo &= todo - 1;
+    ok = __all_sync(0xffffffffu, a4_wait(bars + stage, (k / A4_STAGES) & 1));
+    if (!ok) break;
+    const int key0 = (tile_a + warp + A4_WARPS * i) * TT;
+    const unsigned char* buf = ring + stage * TILE;
+    if (key0 + TT - 1 <= full_hi && key0 >= full_lo && r.cols == COLS) walk(buf, key0, std::false_type());
+    else walk(buf, key0, std::true_type());
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // this lane's reads come before the copy that follows
+    __syncwarp();
+    if (ask) request(stage);
+    ++k;
+  }
+  if (!ok) {
+    // copies still on their way get the time to land before this shared memory is used again
+    if (lane == 0) atomicExch(&g_a4_error, 1);
+    for (int i = 0; i < 1000; ++i) __nanosleep(100);
+  }
+  __syncwarp();
+
+  // this warp's sums over its lanes, then its results [column][feature] in the ring's place
+  float* mine = reinterpret_cast<float*>(ring);
+  const float unit = 0x1p24f / F;
+#pragma unroll
+  for (int n = 0; n < NC; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = 8 * n + 2 * t + h;
+      float v = l[n][h];
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      if (g == 0) { s_m[warp][c] = m[n][h]; s_l[warp][c] = v; }
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        float s = om[n][i][h];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        float4 y;
+        y.x = fmaf(o[n][i][0][h], unit, s);
+        y.y = fmaf(o[n][i][0][h + 2], unit * 0.0625f, s);
+        y.z = fmaf(o[n][i][1][h], unit, s);
+        y.w = fmaf(o[n][i][1][h + 2], unit * 0.0625f, s);
+        *reinterpret_cast<float4*>(mine + c * HD + i * 32 + 4 * g) = y;
+      }
+    }
+  __syncthreads();
+  // the four warps' results: one record, or the output
+  const bool last = a.max_chunks == 1 || r.n_chunks <= 1;
+  const int64_t rec = (((int64_t)row * a.nkv + kvh) * a.n_ct + ct) * a.max_chunks + blockIdx.x;
+  for (int i = threadIdx.x; i < r.cols * (HD / 4); i += A4_WARPS * 32) {
+    const int c = i / (HD / 4), d = i % (HD / 4) * 4;
+    float top = s_m[0][c];
+#pragma unroll
+    for (int w = 1; w < A4_WARPS; ++w) top = fmaxf(top, s_m[w][c]);
+    const float safe = top == __int_as_float(0xff800000) ? 0.0f : top;
+    float sum = 0.0f, acc[4] = {};
+#pragma unroll
+    for (int w = 0; w < A4_WARPS; ++w) {
+      const float f = a4_exp2(s_m[w][c] - safe);
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a4_smem_raw + w * RING) + c * HD + d);
+      sum = fmaf(s_l[w][c], f, sum);
+      acc[0] = fmaf(y.x, f, acc[0]); acc[1] = fmaf(y.y, f, acc[1]); acc[2] = fmaf(y.z, f, acc[2]); acc[3] = fmaf(y.w, f, acc[3]);
+    }
+    const int col = r.col0 + c;
+    if (last) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint2 w;
+      __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv), hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+      w.x = *reinterpret_cast<uint32_t*>(&lo);
+      w.y = *reinterpret_cast<uint32_t*>(&hi);
+      *reinterpret_cast<uint2*>(a.out + ((int64_t)(r.start + col / r.G) * a.nh + kvh * r.G + col % r.G) * HD + d) = w;
+    } else {
+      float* to = a.scratch + (rec * COLS + c) * (HD + 4);
+      *reinterpret_cast<float4*>(to + 4 + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (d == 0) { to[0] = top; to[1] = sum; }
+    }
+  }
+}
+
+// Joins the chunks of a (row, key/value head, column): a block each, its warps over the chunks, then the warps' sums.
+constexpr int A4_JOIN_WARPS = 8;
+template <int HD>
+__global__ void __launch_bounds__(A4_JOIN_WARPS * 32)
+kv4_join_kernel(const A4Args a, int columns) {
+  constexpr int V = HD / 32;                                // features a lane
+  __shared__ float s_acc[A4_JOIN_WARPS][HD], s_m[A4_JOIN_WARPS], s_l[A4_JOIN_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y / a.n_ct, ct = blockIdx.y % a.n_ct, c = blockIdx.x, row = blockIdx.z;
+  pdl_trigger();
+  pdl_wait();
+  const A4Range<HD> r(a, row, ct, columns);
+  if (c >= r.cols || r.n_chunks <= 1) return;               // (a single chunk wrote the output itself)
+  const float* base = a.scratch + ((((int64_t)row * a.nkv + kvh) * a.n_ct + ct) * a.max_chunks * columns + c) * (HD + 4);
+  const int64_t step = (int64_t)columns * (HD + 4);
+  float m = __int_as_float(0xff800000), l = 0.0f, acc[V] = {};
+  for (int k0 = warp; k0 < r.n_chunks; k0 += 4 * A4_JOIN_WARPS) {
+    float mk[4], lk[4], y[4][V];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + u * A4_JOIN_WARPS;
+      const float* p = base + (k < r.n_chunks ? k : 0) * step;
+      mk[u] = k < r.n_chunks ? __ldcg(p) : __int_as_float(0xff800000);
+      lk[u] = __ldcg(p + 1);
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[u][i] = __ldcg(p + 4 + i * 32 + lane);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (k0 + u * A4_JOIN_WARPS >= r.n_chunks) break;
+      const float top = fmaxf(m, mk[u]), safe = top == __int_as_float(0xff800000) ? 0.0f : top;
+      const float f0 = a4_exp2(m - safe), f1 = a4_exp2(mk[u] - safe);
+      l = l * f0 + lk[u] * f1;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = acc[i] * f0 + y[u][i] * f1;
+      m = top;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) s_acc[warp][i * 32 + lane] = acc[i];
+  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+  __syncthreads();
+  if (threadIdx.x < HD) {
+    float top = s_m[0];
+#pragma unroll
+    for (int w = 1; w < A4_JOIN_WARPS; ++w) top = fmaxf(top, s_m[w]);
+    const float safe = top == __int_as_float(0xff800000) ? 0.0f : top;
+    float sum = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < A4_JOIN_WARPS; ++w) {
+      const float f = a4_exp2(s_m[w] - safe);
+      sum = fmaf(s_l[w], f, sum);
+      y = fmaf(s_acc[w][threadIdx.x], f, y);
+    }
+    const int col = r.col0 + c;
+    a.out[((int64_t)(r.start + col / r.G) * a.nh + kvh * r.G + col % r.G) * HD + threadIdx.x] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : y / sum);
+  }
+}
+
+constexpr uint32_t A4_SMEM = A4_WARPS * A4_STAGES * TILE;
+
+}  // namespace exl3
+
+using namespace exl3;
+
+extern "C" int exl3_kv4_attn_status() {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_a4_error, sizeof(int));
+  if (v) { int z = 0; cudaMemcpyToSymbol(g_a4_error, &z, sizeof(int)); }
+  return v;
+}
+
+// Floats of scratch that a call with these sizes wants (0 with one chunk).
+extern "C" long long exl3_kv4_attn_scratch(int rows, int max_new, int nh, int nkv, int hd, int max_chunks) {
+  if (max_chunks <= 1 || nkv < 1) return 0;
+  const int ncol = max_new * (nh / nkv), columns = ncol <= 8 ? 8 : 16;
+  return (long long)rows * nkv * ceil_div(ncol, columns) * max_chunks * columns * (hd + 4);
+}
+
+extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const void* pool, int64_t n_pages, const int* block_table,
+                             int bt_stride, const int* row_start, const int* row_pos0, int rows, int max_new, int nh, int nkv, int hd,
+                             int window, float scale, int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream) {
+  if (rows == 0 || max_new == 0) return 0;
+  if (rows < 0 || rows > 65535 || max_new < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || window < 0 || chunk < 1 ||
+      chunk > A4_MAX_CHUNK || max_chunks < 1 || n_pages < 1 || n_pages > INT32_MAX || bt_stride < 1 || !q || !out || !pool || !block_table ||
+      !row_pos0 || (!row_start && max_new != 1)) {
+    set_error("kv4_attn: needs heads of 64 or 128, chunks of 1 to %d tiles and all of its arrays, got rows=%d max_new=%d heads=%d kv_heads=%d "
+              "head_dim=%d chunk=%d max_chunks=%d", A4_MAX_CHUNK, rows, max_new, nh, nkv, hd, chunk, max_chunks);
+    return ERR_BAD_ARGUMENT;
+  }
+  if (!aligned16(q) || !aligned16(out) || !aligned16(pool) || q_stride % 8) { set_error("kv4_attn: q, its rows, out and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  if (max_chunks > 1 && (!scratch || scratch_floats < exl3_kv4_attn_scratch(rows, max_new, nh, nkv, hd, max_chunks))) {
+    set_error("kv4_attn: %lld floats of scratch wanted", exl3_kv4_attn_scratch(rows, max_new, nh, nkv, hd, max_chunks));
+    return ERR_SCRATCH;
+  }
+  const int ncol = max_new * (nh / nkv), columns = ncol <= 8 ? 8 : 16;
+  A4Args a = {};
+  a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.out = static_cast<__nv_bfloat16*>(out);
+  a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.block_table = block_table; a.bt_stride = bt_stride;
+  a.row_start = row_start; a.row_pos0 = row_pos0; a.nh = nh; a.nkv = nkv; a.window = window; a.scale_log2 = scale * 1.4426950408889634f;
+  a.chunk = chunk; a.max_chunks = max_chunks; a.n_ct = ceil_div(ncol, columns); a.scratch = scratch;
+  if ((int64_t)a.nkv * a.n_ct > 65535) { set_error("kv4_attn: too many new tokens for this kernel"); return ERR_UNSUPPORTED; }
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaSuccess;
+    for (const void* f : {(const void*)kv4_attn_kernel<64, 1>, (const void*)kv4_attn_kernel<64, 2>, (const void*)kv4_attn_kernel<128, 1>, (const void*)kv4_attn_kernel<128, 2>})
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)A4_SMEM);
+    if (e != cudaSuccess) { set_error("kv4_attn: cannot get %u bytes of shared memory: %s", A4_SMEM, cudaGetErrorString(e)); return (int)e; }
+    configured = true;
+  }
+  const dim3 grid(max_chunks, nkv * a.n_ct, rows), block(A4_WARPS * 32);
+  auto go = [&](auto kernel) { launch_pdl(kernel, grid, block, A4_SMEM, stream, a); };
+  if (hd == 64) { if (columns == 8) go(kv4_attn_kernel<64, 1>); else go(kv4_attn_kernel<64, 2>); }
+  else { if (columns == 8) go(kv4_attn_kernel<128, 1>); else go(kv4_attn_kernel<128, 2>); }
+  int rc = launch_status("kv4_attn");
+  if (rc || max_chunks == 1) return rc;
+  const dim3 jgrid(columns < ncol ? columns : ncol, nkv * a.n_ct, rows), jblock(A4_JOIN_WARPS * 32);
+  if (hd == 64) launch_pdl(kv4_join_kernel<64>, jgrid, jblock, 0, stream, a, columns);
+  else launch_pdl(kv4_join_kernel<128>, jgrid, jblock, 0, stream, a, columns);
+  return launch_status("kv4_attn join");
+}

@@ -1,0 +1,200 @@
+// The 4-bit key/value cache's two ways: a step's keys and values into its pages (with the rotary encoding of queries and keys), and
+// pages back into bfloat16.  The format is in cache4.cuh.
+//
+//   store  q, k rotated in float32 (pairs d, d + HD / 2), q rounded to bfloat16; per group of 32 features mn = bfloat16(min),
+//          sc = bfloat16((max - mn) / 15), code = clamp(rint((x - mn) * (1 / sc)), 0, 15) on the float32 values.  A group that holds a
+//          value that is not finite, or whose range is not, becomes NaN as a whole.
+//   load   mn + sc * code (exact in float32: 8 x 4 bits) rounded to bfloat16.
+//
+// Both are bound by memory, or by their launch in a decode step.
+#include "api.h"
+#include "cache4.cuh"
+
+namespace exl3 {
+
+using namespace kv4;
+
+constexpr int C4_THREADS = 256;
+
+// A lane has features 8 j .. 8 j + 7 of a head (j = 0 .. HD / 8 - 1); four neighbouring lanes have a group.  Returns the group's word and
+// the lane's eight codes, feature e's in bits 4 e ...
+__device__ inline uint32_t c4_quantize(const float (&x)[8], uint32_t& codes) {
+  float lo = x[0], hi = x[0];
+  bool finite = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    lo = fminf(lo, x[e]);
+    hi = fmaxf(hi, x[e]);
+    finite = finite && fabsf(x[e]) < __int_as_float(0x7f800000);
+  }
+  if (!finite) { lo = __int_as_float(0xff800000); hi = __int_as_float(0x7f800000); }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  const __nv_bfloat16 mnb = __float2bfloat16_rn(lo);
+  const float mn = __bfloat162float(mnb);
+  const float range = fmaxf(hi - mn, 0.0f);
+  const __nv_bfloat16 scb = __float2bfloat16_rn(__fdiv_rn(range, 15.0f));
+  const float sc = __bfloat162float(scb);
+  codes = 0;
+  if (!(sc < __int_as_float(0x7f800000)) || !(fabsf(mn) < __int_as_float(0x7f800000))) return 0x7fc07fc0u;
+  const float inv = sc > SC_MIN ? __frcp_rn(sc) : 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], mn), inv)), 0.0f), 15.0f);
+    codes |= (uint32_t)(int)c << (4 * e);
+  }
+  return (uint32_t)__bfloat16_as_ushort(scb) << 16 | __bfloat16_as_ushort(mnb);
+}
+
+// A block takes one token and the heads blockIdx.y, + gridDim.y, ... in steps of as many as its threads cover; the token's sines and cosines
+// are worked out once for all of them.
+template <int HD>
+__global__ void __launch_bounds__(C4_THREADS)
+kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv_bfloat16* __restrict__ q_out,
+                 const float* __restrict__ freq, const float* __restrict__ freq_lo, const int* __restrict__ tok_pos,
+                 const int* __restrict__ tok_seq, const int* __restrict__ block_table, int bt_stride, unsigned char* __restrict__ pool,
+                 int n_pages, int nh, int nkv) {
+  constexpr int LANES = HD / 8, HEADS = C4_THREADS / LANES;           // heads that the block works on side by side
+  __shared__ float s_cos[HD / 2], s_sin[HD / 2];
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x;
+  const int pos = __ldcg(tok_pos + t), seq = __ldcg(tok_seq + t);
+  if (freq) {
+    for (int d = threadIdx.x; d < HD / 2; d += C4_THREADS)
+      rope_sincos((float)pos, __ldg(freq + d), freq_lo ? __ldg(freq_lo + d) : 0.0f, s_sin + d, s_cos + d);
+    __syncthreads();
+  }
+  const int page = pos >= 0 ? __ldcg(block_table + (int64_t)seq * bt_stride + pos / PAGE) : -1;
+  const int j = threadIdx.x % LANES;
+  const int total = nh + 2 * nkv;
+  for (int first = blockIdx.y * HEADS; first < total; first += gridDim.y * HEADS) {
+    const int head = first + threadIdx.x / LANES;
+    const bool live = head < total;                                    // (the whole group of lanes; the shuffles need everybody)
+    const __nv_bfloat16* src = qkv + (int64_t)t * qkv_stride + (int64_t)(live ? head : 0) * HD;
+    float x[8];
+    load_vec_cg(src + 8 * j, x);
+    if (freq && head < nh + nkv) {
+      const int jp = j ^ (LANES / 2);
+      float y[8];
+      load_vec_cg(src + 8 * jp, y);
+      const int d0 = 8 * (j & (LANES / 2 - 1));
+      const float sign = j < LANES / 2 ? -1.0f : 1.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * s_cos[d0 + e] + sign * (y[e] * s_sin[d0 + e]);
+    }
+    if (live && head < nh) store_vec(q_out + ((int64_t)t * nh + head) * HD + 8 * j, x);
+    // (warps that hold queries only skip the rest; a warp's heads are neighbours)
+    if (__all_sync(0xffffffffu, head < nh || !live)) continue;
+    uint32_t codes;
+    const uint32_t word = c4_quantize(x, codes);
+    // values: a word has four features of one group below and four of the next above: lanes j and j ^ 4 trade halves
+    const uint32_t give = (j & 4) ? codes & 0xffffu : codes >> 16;
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 4);
+    if (!live || head < nh || page < 0 || page >= n_pages) continue;
+    const bool key = head < nh + nkv;
+    const int kv = key ? head - nh : head - nh - nkv;
+    const int slot = pos % PAGE, tok = slot % tile_tokens(HD);
+    unsigned char* tile = pool + ((int64_t)page * nkv + kv) * page_bytes(HD) + slot / tile_tokens(HD) * TILE;
+    if (key) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w |= ((codes >> (4 * e)) & 15u) << (4 * (e / 2 + 4 * (e % 2)));
+      *reinterpret_cast<uint32_t*>(tile + k_word<HD>(tok, j & 3, j >> 2)) = w;
+    } else {
+      const int half = j >> 3, jj = j & 7;
+      const uint32_t w = jj < 4 ? (codes & 0xffffu) | got << 16 : got | (codes & 0xffff0000u);
+      *reinterpret_cast<uint32_t*>(tile + v_word<HD>(tok, half, jj < 4 ? 2 * jj : 2 * (jj - 4) + 1)) = w;
+    }
+    if ((j & 3) == 0)
+      *reinterpret_cast<uint32_t*>(tile + (key ? K_WORDS : V_WORDS) + (tok * (HD / 32) + (j >> 2)) * 4) = word;
+  }
+}
+
+// Pages listed in `pages` to bfloat16 [n, nkv, 64, HD]: a block per (page, kv head), a thread per eight features of a key or value.
+template <int HD>
+__global__ void __launch_bounds__(C4_THREADS)
+kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n_pages, int nkv,
+                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ table_out) {
+  constexpr int LANES = HD / 8;
+  pdl_trigger();
+  pdl_wait();
+  const int page = __ldcg(pages + blockIdx.x), kv = blockIdx.y;
+  const bool there = page >= 0 && page < n_pages;
+  if (table_out) {                                                      // the unpacked pages' own table: no values where there is no page
+    if (kv == 0 && threadIdx.x == 0) table_out[blockIdx.x] = there ? (int)blockIdx.x : -1;
+    if (!there) return;
+  }
+  const unsigned char* base = pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD);
+  const int64_t out0 = ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD;
+  for (int i = threadIdx.x; i < 2 * PAGE * LANES; i += C4_THREADS) {
+    const bool key = i < PAGE * LANES;
+    const int r = key ? i : i - PAGE * LANES, slot = r / LANES, j = r % LANES;
+    const unsigned char* tile = base + slot / tile_tokens(HD) * TILE;
+    const int tok = slot % tile_tokens(HD);
+    const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(tile + (key ? K_WORDS : V_WORDS) + (tok * (HD / 32) + (j >> 2)) * 4));
+    uint32_t code[8];
+    if (key) {
+      const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(tile + k_word<HD>(tok, j & 3, j >> 2)));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) code[e] = (w >> (4 * (e / 2 + 4 * (e % 2)))) & 15u;
+    } else {
+      const int half = j >> 3, jj = j & 7;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(tile + v_word<HD>(tok, half, 2 * (jj & 3) + p))) >> (jj < 4 ? 0 : 16);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) code[4 * p + n] = (w >> (4 * n)) & 15u;
+      }
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = there ? fmaf(word_sc(word), (float)code[e], word_mn(word)) : 0.0f;
+    store_vec((key ? k_out : v_out) + out0 + (int64_t)slot * HD + 8 * j, v);
+  }
+}
+
+}  // namespace exl3
+
+using namespace exl3;
+
+extern "C" int exl3_kv4_page_bytes(int hd) { return hd == 64 || hd == 128 ? kv4::page_bytes(hd) : 0; }
+
+extern "C" int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float* freq, const float* freq_lo, const int* tok_pos,
+                              const int* tok_seq, const int* block_table, int bt_stride, void* pool, int64_t n_pages, int T, int nh, int nkv,
+                              int hd, cudaStream_t stream) {
+  if (T == 0) return 0;
+  if (T < 0 || nh < 1 || nkv < 1 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || bt_stride < 1 || !qkv || !q_out ||
+      !tok_pos || !tok_seq || !block_table || !pool) {
+    set_error("kv4_store: needs heads of 64 or 128 and all of its arrays, got T=%d heads=%d kv_heads=%d head_dim=%d", T, nh, nkv, hd);
+    return ERR_BAD_ARGUMENT;
+  }
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(pool) || qkv_stride % 8) { set_error("kv4_store: qkv, its rows, q and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  const int per = C4_THREADS / (hd / 8), rounds = ceil_div(nh + 2 * nkv, per);
+  const int gy = T >= 296 ? 1 : rounds < 32 ? rounds : 32;             // few tokens: a token's heads over several blocks
+  auto go = [&](auto kernel) {
+    launch_pdl(kernel, dim3(T, gy), dim3(C4_THREADS), 0, stream, static_cast<const __nv_bfloat16*>(qkv), qkv_stride, static_cast<__nv_bfloat16*>(q_out), freq,
+               freq_lo, tok_pos, tok_seq, block_table, bt_stride, static_cast<unsigned char*>(pool), (int)n_pages, nh, nkv);
+  };
+  if (hd == 64) go(kv4_store_kernel<64>); else go(kv4_store_kernel<128>);
+  return launch_status("kv4_store");
+}
+
+extern "C" int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
+                             int* table_out, cudaStream_t stream) {
+  if (n == 0) return 0;
+  if (n < 0 || nkv < 1 || nkv > 65535 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || !pool || !pages || !k_out || !v_out) {
+    set_error("kv4_load: needs heads of 64 or 128 and all of its arrays, got %d pages, kv_heads=%d head_dim=%d", n, nkv, hd);
+    return ERR_BAD_ARGUMENT;
+  }
+  if (!aligned16(pool) || !aligned16(k_out) || !aligned16(v_out)) { set_error("kv4_load: the pool and the results must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  auto go = [&](auto kernel) {
+    launch_pdl(kernel, dim3(n, nkv), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, (int)n_pages, nkv,
+               static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), table_out);
+  };
+  if (hd == 64) go(kv4_load_kernel<64>); else go(kv4_load_kernel<128>);
+  return launch_status("kv4_load");
+}

@@ -1139,7 +1139,8 @@ def check_status() -> None:
                                      ("gemm_pair", gemm_pair_status),
                                      ("attn_prefill_tc", attn_prefill_tc_status),
                                      ("attn_decode", attn_decode_status),
-                                     ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status)) if fn()]
+                                     ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status),
+                                     ("kv4_attn", kv4_attn_status)) if fn()]
     if gave_up:
         raise KernelLibraryError("a bounded wait ran out in " + ", ".join(gave_up) +
                                  ": a copy or a tensor-core product did not complete in time")
@@ -1809,3 +1810,168 @@ def residual_step(h: torch.Tensor, a: Optional[torch.Tensor] = None, b: Optional
         code(emb), _ptr(ids), _c_float(emb_scale), _ptr(vec), _ptr(w), code(w), _c_float(eps), _ptr(x), code(x), _c_int(T),
         _c_int(W), _stream()), "residual_step")
     return x
+
+
+# ---- the 4-bit key/value cache (format: cache4.cuh) ----------------------------------------------------------
+
+KV4_PAGE = 64
+
+
+def kv4_page_bytes(head_dim: int) -> int:
+    """Bytes of a page of 64 tokens of one key/value head, keys and values together (head sizes 64 and 128)."""
+    n = int(library().exl3_kv4_page_bytes(_c_int(head_dim)))
+    if n == 0:
+        raise KernelLibraryError(f"the 4-bit cache takes heads of 64 or 128, got {head_dim}")
+    return n
+
+
+def kv4_pool(pages: int, kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """An empty pool: uint8 ``[pages, kv_heads, bytes]``."""
+    return torch.zeros((pages, kv_heads, kv4_page_bytes(head_dim)), dtype=torch.uint8, device=device)
+
+
+def _kv4_check_pool(pool: torch.Tensor, kv_heads: Optional[int], head_dim: int, what: str) -> None:
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != kv4_page_bytes(head_dim) or \
+            (kv_heads is not None and pool.shape[1] != kv_heads):
+        raise KernelLibraryError(f"{what}: the pool must be uint8 [pages, kv_heads, {kv4_page_bytes(head_dim)}], got "
+                                 f"{pool.dtype} {tuple(pool.shape)}")
+    _contig(pool, "pool")
+
+
+def _int32(t: torch.Tensor, name: str, what: str) -> None:
+    if t.dtype != torch.int32:
+        raise KernelLibraryError(f"{what}: {name} must be int32, got {t.dtype}")
+    _contig(t, name)
+
+
+def _table(t: torch.Tensor, rows: Optional[int], what: str) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (rows is not None and t.shape[0] < rows):
+        raise KernelLibraryError(f"{what}: the block table must be int32 [rows, pages]")
+
+
+def kv4_store(qkv: torch.Tensor, inv_freq: Optional[torch.Tensor], tok_pos: torch.Tensor, tok_seq: torch.Tensor,
+              block_table: torch.Tensor, pool: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates the queries and keys of ``qkv`` bfloat16 ``[T, (heads + 2 kv_heads) * head_dim]`` (pairs d, d + head_dim / 2;
+    ``inv_freq`` as in ``rotary_table``, None: no rotation), rounds the rotated keys and the values to 4 bits into the
+    tokens' places in ``pool`` and returns the rotated queries ``[T, heads * head_dim]``.  ``qkv`` stays as it is.  A token whose position is
+    negative or whose page is not there is not stored."""
+    T = qkv.shape[0]
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * kv_heads) * head_dim or qkv.stride(1) != 1:
+        raise KernelLibraryError(f"kv4_store: qkv must be bfloat16 [tokens, {(heads + 2 * kv_heads) * head_dim}], got {qkv.dtype} {tuple(qkv.shape)}")
+    _kv4_check_pool(pool, kv_heads, head_dim, "kv4_store")
+    _table(block_table, None, "kv4_store")
+    for n, t in (("tok_pos", tok_pos), ("tok_seq", tok_seq)):
+        _int32(t, n, "kv4_store")
+        if t.numel() < T:
+            raise KernelLibraryError(f"kv4_store: {n} has {t.numel()} entries for {T} tokens")
+    hi, lo = _rotary_rows(inv_freq, head_dim, "kv4_store") if inv_freq is not None else (_c_void_p(0), _c_void_p(0))
+    if out is None:
+        out = torch.empty((T, heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
+        raise KernelLibraryError(f"kv4_store: out must be contiguous bfloat16 {(T, heads * head_dim)}")
+    _check(library().exl3_kv4_store(
+        _ptr(qkv), _c_int64(qkv.stride(0)), _ptr(out), hi, lo, _ptr(tok_pos), _ptr(tok_seq), _ptr(block_table),
+        _c_int(block_table.stride(0)), _ptr(pool), _c_int64(pool.shape[0]), _c_int(T), _c_int(heads), _c_int(kv_heads),
+        _c_int(head_dim), _stream()), "kv4_store")
+    return out
+
+
+def kv4_load(pool: torch.Tensor, pages: torch.Tensor, head_dim: int):
+    """The keys and values that the listed pages stand for: bfloat16 ``[n, kv_heads, 64, head_dim]`` each (zeros for a number
+    that is no page's)."""
+    _kv4_check_pool(pool, None, head_dim, "kv4_load")
+    _int32(pages, "pages", "kv4_load")
+    n, kv_heads = pages.numel(), pool.shape[1]
+    k, v = (torch.empty((n, kv_heads, KV4_PAGE, head_dim), dtype=torch.bfloat16, device=pool.device) for _ in range(2))
+    _check(library().exl3_kv4_load(_ptr(pool), _c_int64(pool.shape[0]), _ptr(pages), _c_int(n), _c_int(kv_heads),
+                                   _c_int(head_dim), _ptr(k), _ptr(v), _ptr(None), _stream()), "kv4_load")
+    return k, v
+
+
+def kv4_attn_status() -> int:
+    """0, or the code the 4-bit cache's attention left when a bounded wait ran out (cleared by this call)."""
+    return int(library().exl3_kv4_attn_status())
+
+
+KV4_FEW_COLUMNS = 64        # new tokens times query heads per key/value head up to which the keys are walked as codes
+
+
+def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: int, span: int, window: int, sms: int):
+    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys."""
+    tiles = max(1, -(-span * head_dim // 4096))
+    slots = sms * (3 if columns == 8 else 2)
+    total = rows * kv_heads * groups * tiles
+    chunk = -(-total // slots) if total <= 16 * slots else max(16, min(64, total // (4 * slots)))
+    chunk = max(4, min(128, -(-chunk // 4) * 4))
+    return chunk, (tiles - 1) // chunk + 1 + (1 if window > 0 and tiles > 1 else 0)
+
+
+def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row_start: Optional[torch.Tensor],
+             row_pos0: torch.Tensor, tiles: Optional[tuple], max_new: int, max_len: int, heads: int, kv_heads: int,
+             head_dim: int, scale: float, window: int = 0, workspace=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of a step's new tokens over the 4-bit cache, which already holds them: ``softmax(q K^T * scale) V`` with K and V
+    as the pages stand for them.  Row r has tokens ``row_start[r] .. row_start[r + 1] - 1`` of ``q`` bfloat16 ``[T, heads * head_dim]`` at positions
+    ``row_pos0[r] ...`` (``row_start`` None: row r is token r); ``max_new``: the most tokens of a row, ``max_len``: the most keys of one.
+    ``window`` > 0: a query sees the last ``window`` keys, its own among them.  A query that sees nothing gets zeros.
+    ``tiles``: ``(row, first new token, count)`` of the tiles of 128 queries, as ``attn_prefill_tc`` takes them, for rows of many new
+    tokens (None: never more than a few).  ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's).
+
+    A few tokens a row (``KV4_FEW_COLUMNS``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
+    unpacked to bfloat16 and go through the tcgen05 attention."""
+    T = q.shape[0]
+    if q.dtype != torch.bfloat16 or q.dim() != 2 or q.shape[1] != heads * head_dim or q.stride(1) != 1:
+        raise KernelLibraryError(f"kv4_attn: q must be bfloat16 [tokens, {heads * head_dim}], got {q.dtype} {tuple(q.shape)}")
+    if kv_heads < 1 or heads % kv_heads or window < 0 or max_new < 0 or max_len < 0:
+        raise KernelLibraryError(f"kv4_attn: {heads} heads on {kv_heads}, window {window}, max_new {max_new}, max_len {max_len}")
+    _kv4_check_pool(pool, kv_heads, head_dim, "kv4_attn")
+    _int32(row_pos0, "row_pos0", "kv4_attn")
+    rows = row_pos0.numel()
+    if row_start is not None:
+        _int32(row_start, "row_start", "kv4_attn")
+        if row_start.numel() != rows + 1:
+            raise KernelLibraryError(f"kv4_attn: row_start has {row_start.numel()} entries for {rows} rows")
+    elif max_new != 1 or T != rows:
+        raise KernelLibraryError("kv4_attn: without row_start every row has one token")
+    _table(block_table, rows, "kv4_attn")
+    if out is None:
+        out = torch.empty((T, heads * head_dim), dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
+        raise KernelLibraryError(f"kv4_attn: out must be contiguous bfloat16 {(T, heads * head_dim)}")
+    if T == 0 or rows == 0:
+        return out
+    lib = library()
+    columns_wanted = max_new * (heads // kv_heads)
+    if tiles is not None and columns_wanted > KV4_FEW_COLUMNS:
+        return _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window,
+                                workspace, out)
+    columns = 8 if columns_wanted <= 8 else 16
+    span = min(max_len, window + max_new - 1) if window > 0 else max_len
+    chunk, chunks = _kv4_chunks(rows, kv_heads, -(-columns_wanted // columns), columns, head_dim, max(1, span), window, sm_count(q.device))
+    lib.exl3_kv4_attn_scratch.restype = _c_int64
+    need = int(lib.exl3_kv4_attn_scratch(_c_int(rows), _c_int(max_new), _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_int(chunks)))
+    scratch = None
+    if need:
+        scratch = workspace.plain(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
+    _check(lib.exl3_kv4_attn(
+        _ptr(q), _c_int64(q.stride(0)), _ptr(out), _ptr(pool), _c_int64(pool.shape[0]), _ptr(block_table), _c_int(block_table.stride(0)),
+        _ptr(row_start), _ptr(row_pos0), _c_int(rows), _c_int(max_new), _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_int(window),
+        _c_float(scale), _c_int(chunk), _c_int(chunks), _ptr(scratch), _c_int64(need), _stream()), "kv4_attn")
+    return out
+
+
+def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window, workspace, out):
+    """Prompts: the rows' pages in bfloat16 in scratch memory, page i of row r at r * width + i, and the tcgen05 attention over them."""
+    rows, width = row_pos0.numel(), block_table.shape[1]
+    n = rows * width
+    floats = n * kv_heads * KV4_PAGE * head_dim // 2
+    need = 2 * floats + n
+    scratch = workspace.plain(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
+    shape = (n, kv_heads, KV4_PAGE, head_dim)
+    k, v = (scratch[i * floats:(i + 1) * floats].view(torch.bfloat16).view(shape) for i in range(2))
+    table = scratch[2 * floats:2 * floats + n].view(torch.int32).view(rows, width)
+    pages = block_table[:rows] if block_table.stride(0) == width else block_table[:rows].contiguous()
+    _check(library().exl3_kv4_load(_ptr(pool), _c_int64(pool.shape[0]), _ptr(pages), _c_int(n), _c_int(kv_heads), _c_int(head_dim),
+                                   _ptr(k), _ptr(v), _ptr(table), _stream()), "kv4_load")
+    return attn_prefill_tc(q, q.stride(0), out, k, v, table, row_start, row_pos0, tiles[0], tiles[1], tiles[2], heads, kv_heads,
+                           head_dim, KV4_PAGE, window, scale)
