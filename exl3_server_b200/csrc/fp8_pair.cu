@@ -1,0 +1,346 @@
+// Products of many rows in 8-bit floating point (fp8.cuh): the activations' rounding, and the product on pairs of SMs.
+//
+//   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} cx[m, k] cw[n, k]  (+ bias, or silu(gate) * up)
+//
+// Two blocks of a cluster are one tensor core (tcgen05.mma.cta_group::2, kind::f8f6f4, M 256, N 256, K 32) on tiles of 256 x 256; each copies its
+// 128 rows of codes of x and of w per 128 of K (16 KB + 16 KB, a ring of five stages).  The scales differ from block to block of K, so
+// every block's 128-long product is an accumulator of its own: two of 256 columns take turns in tensor memory, and eight
+// warps add them, times sx * sw, to 128 float32 registers a thread (lane = row, a warp's half of the columns has one sw).  Per block the
+// products take 512 cycles of the tensor core, the accumulator's way out 256 of tensor memory's and 64 packed fma a thread, so the tensor core
+// stays the bound.
+//
+//   warp 0    TMA producer (both blocks)     warp 1    even block: issues the MMAs; both: tensor memory
+//   warps 2-9 accumulators and results (both blocks)
+//
+// Every wait is bounded; when one runs out the kernel records a code, leaves its loops, waits (bounded) for its copies, meets its partner at
+// the cluster barrier, frees its tensor memory and returns.
+#include "api.h"
+#include "fp8.cuh"
+
+namespace exl3 {
+
+using namespace tc5;
+
+// ---- activations to codes -------------------------------------------------------------------------------------------
+
+// Eight lanes take a block of 128 features of a row, 16 features a lane.  Codes [M, K]; scales [M, blocks], or [blocks, M] (transposed).
+__global__ void __launch_bounds__(256)
+fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int M, int K, int kblocks, unsigned char* __restrict__ codes,
+                    float* __restrict__ sx, int transposed) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t item = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int j = threadIdx.x & 7;
+  const bool live = item < (int64_t)M * kblocks;
+  const int row = live ? (int)(item / kblocks) : 0, b = live ? (int)(item % kblocks) : 0, k = b * fp8::KB + j * 16;
+  uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+  if (live && k < K) {
+    const uint4* p = reinterpret_cast<const uint4*>(x + (int64_t)row * ldx + k);
+    v0 = __ldcg(p);
+    v1 = __ldcg(p + 1);
+  }
+  float v[16];
+  fp8::widen16(v0, v1, v);
+  float top = fp8::amax16(v);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (!live) return;
+  if (k < K) *reinterpret_cast<uint4*>(codes + (int64_t)row * K + k) = fp8::codes16(v, fp8::multiplier(top));
+  if (j == 0) sx[transposed ? (int64_t)b * M + row : (int64_t)row * kblocks + b] = fp8::scale_of(top);
+}
+
+// ---- the product ------------------------------------------------------------------------------------------------------
+
+constexpr int F8P_BM = 256, F8P_BN = 256, F8P_STAGES = 6, F8P_EPI = 8;
+constexpr int F8P_THREADS = 64 + 32 * F8P_EPI;
+constexpr uint32_t F8P_HALF = 128 * 128;                  // bytes of a block's 128 rows of either operand
+constexpr uint32_t F8P_SMEM = 1024 + F8P_STAGES * 2 * F8P_HALF;
+
+static __device__ int g_f8p_error = 0;
+
+struct F8pArgs {
+  const float* sx;           // [blocks of K, M]
+  const float* sw;           // [ceil(N / 128), blocks of K]
+  const __nv_bfloat16* bias;
+  void* y;
+  int M, N, K, group, gated, y_f32, vec;
+};
+
+__device__ inline void f8p_fma2(float2& acc, uint32_t d0, uint32_t d1, float s) {
+  uint64_t c, d, f;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(c) : "f"(acc.x), "f"(acc.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "f"(s));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(d), "l"(f));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(c));
+}
+
+__global__ void __launch_bounds__(F8P_THREADS, 1)
+fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const F8pArgs a) {
+  constexpr int STAGES = F8P_STAGES;
+  extern __shared__ unsigned char f8p_raw[];
+  // (the two blocks' offsets have to agree: the same kernel, the same alignment)
+  unsigned char* base = f8p_raw + ((1024u - (smem_u32(f8p_raw) & 1023u)) & 1023u);
+  unsigned char* sA = base;
+  unsigned char* sB = base + STAGES * F8P_HALF;
+  __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    prefetch_map(&map_x);
+    prefetch_map(&map_w);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 2 * F8P_EPI); }
+    mbar_init_fence();
+  }
+  if (warp == 1) tmem_alloc_pair<512>(&tmem_slot);
+  fence_before();
+  cluster_sync_all();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+  const int n_m = (a.M + F8P_BM - 1) / F8P_BM, n_n = (a.N + F8P_BN - 1) / F8P_BN, n_tiles = n_m * n_n;
+  const int kblocks = (a.K + fp8::KB - 1) / fp8::KB;
+  auto place = [&](int tile, int& m, int& n) {              // groups of rows of tiles, within them rows fastest
+    const int first = tile / (a.group * n_n) * a.group, rows = min(a.group, n_m - first), r = tile - first * n_n;
+    m = first + r % rows;
+    n = r / rows;
+  };
+  bool ok = true;
+
+  if (warp == 0) {
+    uint32_t it = 0;
+    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+      int tm, tn;
+      place(tile, tm, tn);
+      const int m0 = tm * F8P_BM + (int)rank * 128, n0 = tn * F8P_BN + (int)rank * 128;
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int s = it % STAGES;
+        ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((it / STAGES) & 1) ^ 1));
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t bar = cluster_addr(full + s, 0);
+          if (rank == 0) mbar_expect_tx(full + s, 4 * F8P_HALF);
+          tma_load_2d_pair(sA + s * F8P_HALF, &map_x, bar, kb * fp8::KB, m0);
+          tma_load_2d_pair(sB + s * F8P_HALF, &map_w, bar, kb * fp8::KB, n0);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicExch(&g_f8p_error, 1);
+      if (rank == 0)
+        for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= it; ++back) mbar_wait(full + (it - back) % STAGES, ((it - back) / STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      uint32_t it = 0;
+      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % STAGES, buf = it & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1) && mbar_wait(full + s, (it / STAGES) & 1));
+          if (!ok) break;
+          fence_after();
+          if (lane == 0) {
+            const uint64_t da = smem_desc_k128(smem_u32(sA + s * F8P_HALF)), db = smem_desc_k128(smem_u32(sB + s * F8P_HALF));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) fp8::mma_ss_pair(tmem + buf * F8P_BN, da + 2 * k, db + 2 * k, fp8::idesc_e4m3(F8P_BM, F8P_BN), k > 0);
+            mma_commit_pair(empty + s);
+            mma_commit_pair(acc_full + buf);
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok && lane == 0) atomicExch(&g_f8p_error, 2);
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lane_taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
+    const uint32_t acc_empty_addr[2] = {cluster_addr(acc_empty, 0), cluster_addr(acc_empty + 1, 0)};
+    uint32_t it = 0;
+    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+      int tm, tn;
+      place(tile, tm, tn);
+      const int row = tm * F8P_BM + (int)rank * 128 + q * 32 + lane, n0 = tn * F8P_BN + half * 128;
+      const bool live = row < a.M, inside = n0 < a.N;
+      float2 acc[64];
+#pragma unroll
+      for (int c = 0; c < 64; ++c) acc[c] = make_float2(0.0f, 0.0f);
+      const float* sw = a.sw + (int64_t)(inside ? n0 / 128 : 0) * kblocks;
+      auto factor = [&](int kb) { return live && inside && kb < kblocks ? __ldcg(a.sx + (int64_t)kb * a.M + row) * __ldg(sw + kb) : 0.0f; };
+      float f_next = factor(0);
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const uint32_t buf = it & 1;
+        const float f = f_next;
+        f_next = factor(kb + 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (it >> 1) & 1));
+        if (!ok) break;
+        fence_after();
+        uint32_t d[2][32];
+        tmem_ld32_issue(lane_taddr + buf * F8P_BN, d[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait(d[c & 1]);
+          if (c < 3) {
+            tmem_ld32_issue(lane_taddr + buf * F8P_BN + (c + 1) * 32, d[(c + 1) & 1]);
+          } else {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty_addr[buf]);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) f8p_fma2(acc[c * 16 + e], d[c & 1][2 * e], d[c & 1][2 * e + 1], f);
+        }
+      }
+      if (!ok) break;
+      if (!live || !inside) continue;
+      const int n_out = a.gated ? a.N / 2 : a.N;
+      if (a.gated) {
+        const int64_t at = (int64_t)row * n_out + n0 / 2;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {                       // eight gates, then the eight ups of the same features
+          if (n0 + 16 * g >= a.N) break;
+          float o[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 gate = acc[g * 8 + e], up = acc[g * 8 + 4 + e];
+            o[2 * e] = __fdividef(gate.x, 1.0f + __expf(-gate.x)) * up.x;
+            o[2 * e + 1] = __fdividef(gate.y, 1.0f + __expf(-gate.y)) * up.y;
+          }
+          if (a.y_f32) {
+            float* y = static_cast<float*>(a.y) + at + 8 * g;
+            reinterpret_cast<float4*>(y)[0] = make_float4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<float4*>(y)[1] = make_float4(o[4], o[5], o[6], o[7]);
+          } else {
+            store_vec(static_cast<__nv_bfloat16*>(a.y) + at + 8 * g, o);
+          }
+        }
+      } else {
+        const int64_t at = (int64_t)row * n_out + n0;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+          float o[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { o[2 * e] = acc[g * 4 + e].x; o[2 * e + 1] = acc[g * 4 + e].y; }
+          const int n = n0 + 8 * g;
+          if (a.bias) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] += n + e < a.N ? __bfloat162float(a.bias[n + e]) : 0.0f;
+          }
+          if (a.vec && n + 8 <= a.N) {
+            if (a.y_f32) {
+              float* y = static_cast<float*>(a.y) + at + 8 * g;
+              reinterpret_cast<float4*>(y)[0] = make_float4(o[0], o[1], o[2], o[3]);
+              reinterpret_cast<float4*>(y)[1] = make_float4(o[4], o[5], o[6], o[7]);
+            } else {
+              store_vec(static_cast<__nv_bfloat16*>(a.y) + at + 8 * g, o);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < a.N) {
+                if (a.y_f32) static_cast<float*>(a.y)[at + 8 * g + e] = o[e];
+                else static_cast<__nv_bfloat16*>(a.y)[at + 8 * g + e] = __float2bfloat16_rn(o[e]);
+              }
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) atomicExch(&g_f8p_error, 3);
+  }
+  fence_before();
+  cluster_sync_all();                                       // nobody reads the partner's shared or tensor memory after this
+  fence_after();
+  if (warp == 1) tmem_free_pair<512>(tmem);
+}
+
+static void f8p_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int blocks, cudaStream_t stream) {
+  *cfg = cudaLaunchConfig_t{};
+  cfg->gridDim = dim3(blocks);
+  cfg->blockDim = dim3(F8P_THREADS);
+  cfg->dynamicSmemBytes = F8P_SMEM;
+  cfg->stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = pdl_enabled() ? 2 : 1;
+}
+
+// Pairs that the GPU runs at once; 0 when the kernel cannot have its shared memory.
+static int f8p_pairs() {
+  static int pairs = 0;
+  if (pairs) return pairs;
+  if (cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8P_SMEM) != cudaSuccess) return 0;
+  int dev = 0, sms = 0, clusters = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int n = sms / 2;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  f8p_config(&cfg, attr, sms & ~1, nullptr);
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&clusters, fp8_pair_kernel, &cfg) == cudaSuccess && clusters > 0 && clusters < n) n = clusters;
+  cudaGetLastError();
+  pairs = n > 0 ? n : 1;
+  return pairs;
+}
+
+}  // namespace exl3
+
+using namespace exl3;
+
+extern "C" int exl3_fp8_pair_status() {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_f8p_error, sizeof(int));
+  if (v) { int z = 0; cudaMemcpyToSymbol(g_f8p_error, &z, sizeof(int)); }
+  return v;
+}
+
+extern "C" int exl3_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, float* sx, int transposed, cudaStream_t stream) {
+  if (M == 0) return 0;
+  if (M < 0 || K < 16 || K % 16 || !x || !codes || !sx) { set_error("fp8_quantize: needs K a multiple of 16 and its arrays, got M=%d K=%d", M, K); return ERR_BAD_ARGUMENT; }
+  if (!aligned16(x) || !aligned16(codes) || ldx % 8) { set_error("fp8_quantize: x, its rows and the codes must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  const int kblocks = ceil_div(K, fp8::KB);
+  const int64_t blocks = ((int64_t)M * kblocks + 31) / 32;
+  if (blocks > INT32_MAX) { set_error("fp8_quantize: too many rows"); return ERR_UNSUPPORTED; }
+  launch_pdl(fp8_quantize_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const __nv_bfloat16*>(x), ldx, M, K, kblocks,
+             static_cast<unsigned char*>(codes), sx, transposed);
+  return launch_status("fp8_quantize");
+}
+
+// codes and sx as exl3_fp8_quantize leaves them with `transposed`.
+extern "C" int exl3_fp8_pair(const void* codes, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype,
+                             int M, int N, int K, int gated, cudaStream_t stream) {
+  if (M == 0 || N == 0) return 0;
+  if (M < 0 || N < 0 || K < 16 || K % 16 || (out_dtype != DT_F32 && out_dtype != DT_BF16) || (gated && (N % 16 || bias)) || !codes || !sx || !w || !sw || !y) {
+    set_error("fp8_pair: needs K a multiple of 16, N of 16 and no bias where gated, a bfloat16 or float32 result and its arrays, got M=%d N=%d K=%d", M, N, K);
+    return ERR_BAD_ARGUMENT;
+  }
+  if (!aligned16(codes) || !aligned16(w) || !aligned16(y)) { set_error("fp8_pair: the codes, w and y must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  const int max_pairs = f8p_pairs();
+  if (!max_pairs) { set_error("fp8_pair: cannot get %u bytes of shared memory", F8P_SMEM); return ERR_UNSUPPORTED; }
+  CUtensorMap map_x, map_w;
+  int rc = fp8::make_map(&map_x, codes, M, K, 128, "fp8_pair");
+  if (rc) return rc;
+  rc = fp8::make_map(&map_w, w, N, K, 128, "fp8_pair");
+  if (rc) return rc;
+  const int n_m = ceil_div(M, F8P_BM), tiles = n_m * ceil_div(N, F8P_BN);
+  F8pArgs a = {};
+  a.sx = sx; a.sw = sw; a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
+  a.M = M; a.N = N; a.K = K; a.gated = gated; a.y_f32 = out_dtype == DT_F32; a.vec = N % 8 == 0;
+  // all rows of tiles together while x's codes stay in L2, else in groups (as gemm_pair.cu has it for bfloat16)
+  a.group = (int64_t)M * K <= (40 << 20) ? n_m : n_m < 8 ? n_m : 8;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  f8p_config(&cfg, attr, 2 * (tiles < max_pairs ? tiles : max_pairs), stream);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_pair_kernel, map_x, map_w, a);
+  if (e != cudaSuccess) { set_error("fp8_pair: launch failed: %s", cudaGetErrorString(e)); return (int)e; }
+  return launch_status("fp8_pair");
+}

@@ -1,0 +1,287 @@
+// Products of few rows with weights in 8-bit floating point (fp8.cuh) on the 5th-generation tensor cores:
+//
+//   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} cx[m, k] cw[n, k]  (+ bias, or silu(gate) * up)
+//
+// A decode step's product reads every weight once and is bound by that.  The weights are the 128-row operand of tcgen05.mma
+// (kind::f8f6f4), one tile of 128 x 128 codes = 16 KB per copy; the batch is the narrow operand (16, 32 or 64 columns).  x comes in
+// bfloat16 and is rounded to codes by the block itself, straight into the swizzled operand, so that there is no kernel ahead of this one;
+// a block does that for its own range of K, once for 128 features.
+//
+// The scales differ from block to block of K, so each block's 128-long product is an accumulator of its own (two in turn in tensor memory), and
+// four warps add it to float32 registers times sx * sw while the next one is formed.
+//
+//   warp 0     TMA producer of weight tiles          warp 1      issues the MMAs; allocates and frees tensor memory
+//   warps 2-5  take accumulators, thread = feature    warps 6-9   x to codes, eight lanes a row of 128
+//
+// K is cut over the S blocks of a cluster; their sums meet through distributed shared memory, block r adding up columns r, r + S, ... in the
+// blocks' order.  Every wait is bounded; when one runs out the kernel records a code, waits (bounded) for its copies, meets the cluster
+// barriers, frees its tensor memory and returns.
+#include "api.h"
+#include "fp8.cuh"
+
+namespace exl3 {
+
+using namespace tc5;
+
+constexpr int F8S_THREADS = 320;
+constexpr int F8S_MAX_SPLIT = 8;
+constexpr int F8S_SLOTS = 8;                              // scales of the last blocks of K: more than the stages and the two accumulators
+
+__host__ __device__ constexpr int f8s_stages(int nb) { return nb <= 32 ? 5 : 6; }
+__host__ __device__ constexpr uint32_t f8s_smem(int nb) { return 1024 + f8s_stages(nb) * (16384 + nb * 128); }
+
+static __device__ int g_f8s_error = 0;
+
+struct F8sArgs {
+  const __nv_bfloat16* x;
+  int64_t ldx;
+  const float* sw;           // [ceil(N / 128), blocks of K]
+  const __nv_bfloat16* bias;
+  void* y;
+  int M, N, K, S, gated, y_f32;
+};
+
+__device__ inline float f8s_ld_peer(const float* mine, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(mine, rank)) : "memory");
+  return v;
+}
+
+template <int NB>
+__global__ void __launch_bounds__(F8S_THREADS, 1)
+fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
+  constexpr int STAGES = f8s_stages(NB);
+  constexpr uint32_t W_BYTES = 16384, X_BYTES = NB * 128;
+  static_assert(STAGES * W_BYTES >= NB * 128 * 4, "the sums take the place of the weight tiles");
+  static_assert(STAGES + 2 <= F8S_SLOTS, "scales live until their accumulator has been taken");
+  extern __shared__ unsigned char f8s_raw[];
+  unsigned char* base = f8s_raw + ((1024u - (smem_u32(f8s_raw) & 1023u)) & 1023u);
+  unsigned char* sW = base;
+  unsigned char* sX = base + STAGES * W_BYTES;
+  __shared__ uint64_t wfull[STAGES], xfull[STAGES], empty[STAGES], acc_full[2], acc_empty[2], sfull[F8S_SLOTS];
+  __shared__ __align__(16) float s_sx[F8S_SLOTS][NB];
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = a.S > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / a.S, n0 = tile * 128, m0 = blockIdx.y * NB;
+  const int kblocks = (a.K + fp8::KB - 1) / fp8::KB;
+  const int kb0 = (int)((int64_t)kblocks * rank / a.S), kb1 = (int)((int64_t)kblocks * (rank + 1) / a.S), n_kb = kb1 - kb0;
+  constexpr int TM_COLS = 2 * NB < 32 ? 32 : 2 * NB;
+  if (threadIdx.x == 0) {
+    prefetch_map(&map_w);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(wfull + s, 1); mbar_init(xfull + s, 4); mbar_init(empty + s, 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 4); }
+    for (int s = 0; s < F8S_SLOTS; ++s) mbar_init(sfull + s, 4);
+    mbar_init_fence();
+  }
+  if (warp == 1) tmem_alloc<TM_COLS>(&tmem_slot);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_trigger();
+  bool ok = true;
+
+  if (warp == 0) {
+    // ---- weights: no kernel writes them, so the first tiles are asked for before the kernel ahead has ended -----------
+    uint32_t asked = 0;
+    for (int i = 0; i < n_kb && ok; ++i, ++asked) {
+      const int s = i % STAGES;
+      ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(wfull + s, W_BYTES);
+        tma_load_2d(sW + s * W_BYTES, &map_w, wfull + s, (kb0 + i) * fp8::KB, n0);
+      }
+      __syncwarp();
+    }
+    if (!ok) {
+      if (lane == 0) atomicExch(&g_f8s_error, 1);
+      for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= asked; ++back) mbar_wait(wfull + (asked - back) % STAGES, ((asked - back) / STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    for (int i = 0; i < n_kb; ++i) {
+      const int s = i % STAGES, buf = i & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((i >> 1) & 1) ^ 1) && mbar_wait(wfull + s, (i / STAGES) & 1) &&
+                                       mbar_wait(xfull + s, (i / STAGES) & 1));
+      if (!ok) break;
+      fence_after();
+      if (lane == 0) {
+        const uint64_t da = smem_desc_k128(smem_u32(sW + s * W_BYTES)), db = smem_desc_k128(smem_u32(sX + s * X_BYTES));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) fp8::mma_ss(tmem + buf * NB, da + 2 * k, db + 2 * k, fp8::idesc_e4m3(128, NB), k > 0);
+        mma_commit(empty + s);
+        mma_commit(acc_full + buf);
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) atomicExch(&g_f8s_error, 2);
+  } else if (warp < 6) {
+    // ---- accumulators: lane = feature of this warp's 32, registers over the columns ----------------------------------
+    const int q = warp & 3;
+    float acc[NB];
+#pragma unroll
+    for (int c = 0; c < NB; ++c) acc[c] = 0.0f;
+    const float* sw = a.sw + (int64_t)tile * kblocks + kb0;
+    float w_next = n_kb > 0 ? __ldg(sw) : 0.0f;
+    for (int i = 0; i < n_kb; ++i) {
+      const int buf = i & 1, slot = i % F8S_SLOTS;
+      const float w = w_next;
+      if (i + 1 < n_kb) w_next = __ldg(sw + i + 1);
+      ok = __all_sync(0xffffffffu, mbar_wait(sfull + slot, (i / F8S_SLOTS) & 1) && mbar_wait(acc_full + buf, (i >> 1) & 1));
+      if (!ok) break;
+      fence_after();
+#pragma unroll
+      for (int c0 = 0; c0 < NB; c0 += 16) {
+        uint32_t d[16];
+        tmem_ld16(tmem + buf * NB + c0 + ((uint32_t)(q * 32) << 16), d);
+#pragma unroll
+        for (int c = 0; c < 16; c += 4) {
+          const float4 sx = *reinterpret_cast<const float4*>(&s_sx[slot][c0 + c]);
+          acc[c0 + c] = fmaf(__uint_as_float(d[c]), sx.x * w, acc[c0 + c]);
+          acc[c0 + c + 1] = fmaf(__uint_as_float(d[c + 1]), sx.y * w, acc[c0 + c + 1]);
+          acc[c0 + c + 2] = fmaf(__uint_as_float(d[c + 2]), sx.z * w, acc[c0 + c + 2]);
+          acc[c0 + c + 3] = fmaf(__uint_as_float(d[c + 3]), sx.w * w, acc[c0 + c + 3]);
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + buf);
+    }
+    if (!ok && lane == 0) atomicExch(&g_f8s_error, 3);
+    // (after a failed wait copies may still be landing in the tiles' place: the sums are not to be trusted, nor written there)
+    if (ok) {
+      float* part = reinterpret_cast<float*>(sW);
+#pragma unroll
+      for (int c = 0; c < NB; ++c) part[c * 128 + q * 32 + lane] = acc[c];
+    }
+  } else {
+    // ---- x to codes: four rows a warp at a time, eight lanes a row, 16 features a lane --------------------------------
+    pdl_wait();
+    constexpr int ROUNDS = NB / 16;
+    const int j = lane & 7, r0 = (warp - 6) * 4 + (lane >> 3);
+    auto fetch = [&](int i, int u, uint4& v0, uint4& v1) {
+      const int row = m0 + u * 16 + r0, k = (kb0 + i) * fp8::KB + j * 16;
+      v0 = v1 = make_uint4(0, 0, 0, 0);
+      if (i < n_kb && row < a.M && k < a.K) {
+        const uint4* p = reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.ldx + k);
+        v0 = __ldcg(p);
+        v1 = __ldcg(p + 1);
+      }
+    };
+    // a block of K ahead of the one that is rounded
+    uint4 cur[ROUNDS][2], nxt[ROUNDS][2];
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) fetch(0, u, cur[u][0], cur[u][1]);
+    for (int i = 0; i < n_kb; ++i) {
+      const int s = i % STAGES, slot = i % F8S_SLOTS;
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) fetch(i + 1, u, nxt[u][0], nxt[u][1]);
+      ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1));
+      if (!ok) break;
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) {
+        float v[16];
+        fp8::widen16(cur[u][0], cur[u][1], v);
+        float top = fp8::amax16(v);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int r = u * 16 + r0;
+        *reinterpret_cast<uint4*>(sX + s * X_BYTES + r * 128 + ((j ^ (r & 7)) << 4)) = fp8::codes16(v, fp8::multiplier(top));
+        if (j == 0) s_sx[slot][r] = fp8::scale_of(top);
+      }
+      fence_smem_to_tma();                                 // the codes are read through the async proxy
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(xfull + s); mbar_arrive(sfull + slot); }
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) { cur[u][0] = nxt[u][0]; cur[u][1] = nxt[u][1]; }
+    }
+    if (!ok && lane == 0) atomicExch(&g_f8s_error, 4);
+  }
+
+  // ---- the cluster's sums ---------------------------------------------------------------------------------------------
+  pdl_wait();                                              // (y may be what an earlier kernel still reads)
+  if (a.S > 1) cluster_sync_all(); else __syncthreads();
+  {
+    const float* part = reinterpret_cast<const float*>(sW);
+    const int per = a.gated ? 64 : 128, n_out = a.gated ? a.N / 2 : a.N, o0 = a.gated ? n0 / 2 : n0;
+    const int rows = min(NB, a.M - m0), mine = rows > rank ? (rows - rank + a.S - 1) / a.S : 0;
+    for (int i = threadIdx.x; i < mine * per; i += F8S_THREADS) {
+      const int c = rank + i / per * a.S, f = i % per;
+      auto total = [&](int feature) {
+        if (a.S == 1) return part[c * 128 + feature];
+        float v[F8S_MAX_SPLIT];
+#pragma unroll
+        for (int b = 0; b < F8S_MAX_SPLIT; ++b) v[b] = b < a.S ? f8s_ld_peer(part + c * 128 + feature, b) : 0.0f;
+        float sum = v[0];
+#pragma unroll
+        for (int b = 1; b < F8S_MAX_SPLIT; ++b) if (b < a.S) sum += v[b];
+        return sum;
+      };
+      float out;
+      if (o0 + f >= n_out) continue;
+      if (a.gated) {
+        const float gate = total(f / 8 * 16 + f % 8), up = total(f / 8 * 16 + 8 + f % 8);
+        out = __fdividef(gate, 1.0f + __expf(-gate)) * up;
+      } else {
+        out = total(f) + (a.bias ? __bfloat162float(a.bias[n0 + f]) : 0.0f);
+      }
+      const int64_t at = (int64_t)(m0 + c) * n_out + o0 + f;
+      if (a.y_f32) static_cast<float*>(a.y)[at] = out;
+      else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(out);
+    }
+  }
+  fence_before();
+  if (a.S > 1) cluster_sync_all(); else __syncthreads();   // nobody reads a block's shared memory after it has gone
+  fence_after();
+  if (warp == 1) tmem_free<TM_COLS>(tmem);
+}
+
+}  // namespace exl3
+
+using namespace exl3;
+
+extern "C" int exl3_fp8_skinny_status() {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_f8s_error, sizeof(int));
+  if (v) { int z = 0; cudaMemcpyToSymbol(g_f8s_error, &z, sizeof(int)); }
+  return v;
+}
+
+extern "C" int exl3_fp8_skinny(const void* x, int64_t ldx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M,
+                               int N, int K, int gated, cudaStream_t stream) {
+  if (M == 0 || N == 0) return 0;
+  if (M < 0 || N < 0 || K < 16 || K % 16 || (out_dtype != DT_F32 && out_dtype != DT_BF16) || (gated && (N % 16 || bias)) || !x || !w || !sw || !y) {
+    set_error("fp8_skinny: needs K a multiple of 16, N of 16 and no bias where gated, a bfloat16 or float32 result and its arrays, got M=%d N=%d K=%d", M, N, K);
+    return ERR_BAD_ARGUMENT;
+  }
+  if (!aligned16(x) || !aligned16(w) || ldx % 8) { set_error("fp8_skinny: x, its rows and w must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  const int nb = M <= 16 ? 16 : M <= 32 ? 32 : 64, groups = ceil_div(M, nb), tiles = ceil_div(N, 128), kblocks = ceil_div(K, 128);
+  if (groups > 65535) { set_error("fp8_skinny: %d rows are too many", M); return ERR_UNSUPPORTED; }
+  static int sms = 0;
+  if (!sms) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaError_t e = cudaSuccess;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(16));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(32));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(64));
+    if (e != cudaSuccess) { sms = 0; set_error("fp8_skinny: cannot get its shared memory: %s", cudaGetErrorString(e)); return (int)e; }
+  }
+  // as many blocks a tile as still run side by side, one an SM
+  int S = sms / (tiles * groups);
+  S = S < 1 ? 1 : S > F8S_MAX_SPLIT ? F8S_MAX_SPLIT : S;
+  if (S > kblocks) S = kblocks;
+  CUtensorMap map;
+  int rc = fp8::make_map(&map, w, N, K, 128, "fp8_skinny");
+  if (rc) return rc;
+  F8sArgs a = {};
+  a.x = static_cast<const __nv_bfloat16*>(x); a.ldx = ldx; a.sw = sw; a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
+  a.M = M; a.N = N; a.K = K; a.S = S; a.gated = gated; a.y_f32 = out_dtype == DT_F32;
+  auto go = [&](auto kernel) {
+    launch_pdl_clusters(kernel, dim3(tiles * S, groups), dim3(F8S_THREADS), S, f8s_smem(nb), stream, map, a);
+  };
+  if (nb == 16) go(fp8_skinny_kernel<16>); else if (nb == 32) go(fp8_skinny_kernel<32>); else go(fp8_skinny_kernel<64>);
+  return launch_status("fp8_skinny");
+}

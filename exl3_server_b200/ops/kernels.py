@@ -1140,7 +1140,8 @@ def check_status() -> None:
                                      ("attn_prefill_tc", attn_prefill_tc_status),
                                      ("attn_decode", attn_decode_status),
                                      ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status),
-                                     ("kv4_attn", kv4_attn_status)) if fn()]
+                                     ("kv4_attn", kv4_attn_status), ("fp8_skinny", fp8_skinny_status),
+                                     ("fp8_pair", fp8_pair_status)) if fn()]
     if gave_up:
         raise KernelLibraryError("a bounded wait ran out in " + ", ".join(gave_up) +
                                  ": a copy or a tensor-core product did not complete in time")
@@ -1975,3 +1976,108 @@ def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv
                                    _ptr(k), _ptr(v), _ptr(table), _stream()), "kv4_load")
     return attn_prefill_tc(q, q.stride(0), out, k, v, table, row_start, row_pos0, tiles[0], tiles[1], tiles[2], heads, kv_heads,
                            head_dim, KV4_PAGE, window, scale)
+
+
+# ---- products in 8-bit floating point (fp8.cuh) ---------------------------------------------------------------
+
+FP8_BLOCK = 128
+FP8_SKINNY_ROWS = 64        # rows up to which the weight-streaming kernel runs in one group
+
+
+def fp8_skinny_status() -> int:
+    return int(library().exl3_fp8_skinny_status())
+
+
+def fp8_pair_status() -> int:
+    return int(library().exl3_fp8_pair_status())
+
+
+def _fp8_check_x(x: torch.Tensor, what: str) -> None:
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
+        raise KernelLibraryError(f"{what}: x must be bfloat16 [rows, features], got {x.dtype} {tuple(x.shape)}")
+    if x.shape[1] < 16 or x.shape[1] % 16:
+        raise KernelLibraryError(f"{what}: the features must be a multiple of 16, got {x.shape[1]}")
+
+
+def fp8_quantize(x: torch.Tensor):
+    """``(codes, scales)`` of x bfloat16 ``[M, K]``: float8_e4m3fn ``[M, K]`` and float32 ``[M, ceil(K / 128)]``: per row and 128 features
+    ``a = max |x|`` (at least 1e-30), scale ``a / 448``, codes ``e4m3(x * (448 / a))`` in float32."""
+    _fp8_check_x(x, "fp8_quantize")
+    M, Kd = x.shape
+    codes = torch.empty((M, Kd), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((M, -(-Kd // FP8_BLOCK)), dtype=torch.float32, device=x.device)
+    _check(library().exl3_fp8_quantize(_ptr(x), _c_int64(x.stride(0)), _c_int(M), _c_int(Kd), _ptr(codes), _ptr(scales), _c_int(0),
+                                       _stream()), "fp8_quantize")
+    return codes, scales
+
+
+def fp8_quantize_weight(w: torch.Tensor):
+    """``(codes, scales)`` of a weight ``[N, K]``: float8_e4m3fn ``[N, K]`` and float32 ``[ceil(N / 128), ceil(K / 128)]``, a scale for
+    each block of 128 x 128, by the rule of ``fp8_quantize``.  Done once when a model is loaded, with torch's own operations (any device)."""
+    if w.dim() != 2:
+        raise KernelLibraryError(f"fp8_quantize_weight: a weight is 2-dimensional, got {tuple(w.shape)}")
+    N, Kd = w.shape
+    nb, kb = -(-N // FP8_BLOCK), -(-Kd // FP8_BLOCK)
+    codes = torch.empty((N, Kd), dtype=torch.float8_e4m3fn, device=w.device)
+    scales = torch.empty((nb, kb), dtype=torch.float32, device=w.device)
+    step = 64                                               # blocks of rows at a time: float32 copies of a part only
+    for b0 in range(0, nb, step):
+        n0, n1 = b0 * FP8_BLOCK, min(N, (b0 + step) * FP8_BLOCK)
+        rows = -(-(n1 - n0) // FP8_BLOCK)
+        x = torch.zeros((rows * FP8_BLOCK, kb * FP8_BLOCK), dtype=torch.float32, device=w.device)
+        x[:n1 - n0, :Kd] = w[n0:n1].float()
+        x = x.view(rows, FP8_BLOCK, kb, FP8_BLOCK)
+        amax = x.abs().amax(dim=(1, 3)).clamp(min=1e-30)
+        top = torch.full_like(amax, 448.0)
+        y = (x * (top / amax)[:, None, :, None]).to(torch.float8_e4m3fn).view(rows * FP8_BLOCK, kb * FP8_BLOCK)
+        codes[n0:n1] = y[:n1 - n0, :Kd]
+        scales[b0:b0 + rows] = amax / top
+    return codes, scales
+
+
+def _fp8_few(M: int, N: int, sms: int) -> bool:
+    """Whether the weight-streaming kernel takes M rows: always up to 64, and in groups of 64 while the paired one's tiles of 256 x 256 would leave
+    most of the GPU idle."""
+    if M <= FP8_SKINNY_ROWS:
+        return True
+    tiles = -(-M // 256) * -(-N // 256)
+    return M <= 256 and tiles < sms // 4
+
+
+def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               out_dtype: torch.dtype = torch.bfloat16, gated: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ W.T (+ bias)`` with W as ``fp8_quantize_weight`` gives it and x bfloat16 ``[M, K]`` rounded as ``fp8_quantize`` rounds it; sums in
+    float32, the result in ``out_dtype`` (bfloat16 or float32).  ``gated``: W's rows are eight gate rows, then the eight up rows of the same
+    features, and so on, and ``silu(gate) * up`` comes out (N / 2 wide, no bias)."""
+    _fp8_check_x(x, "fp8_linear")
+    M, Kd = x.shape
+    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.shape[1] != Kd:
+        raise KernelLibraryError(f"fp8_linear: w must be float8_e4m3fn [features out, {Kd}], got {w.dtype} {tuple(w.shape)}")
+    N = w.shape[0]
+    _contig(w, "w")
+    blocks = -(-Kd // FP8_BLOCK)
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != (-(-N // FP8_BLOCK), blocks):
+        raise KernelLibraryError(f"fp8_linear: the scales must be float32 {(-(-N // FP8_BLOCK), blocks)}, got {w_scale.dtype} {tuple(w_scale.shape)}")
+    _contig(w_scale, "w_scale")
+    if gated and (N % 16 or bias is not None):
+        raise KernelLibraryError("fp8_linear: the gated product takes rows in sixteens and no bias")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != N):
+        raise KernelLibraryError(f"fp8_linear: bias must be bfloat16 [{N}]")
+    shape = (M, N // 2 if gated else N)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=x.device)
+    elif tuple(out.shape) != shape or not out.is_contiguous():
+        raise KernelLibraryError(f"fp8_linear: out must be contiguous {shape}")
+    code = _c_int(dtype_code(out.dtype))
+    if M == 0:
+        return out
+    if _fp8_few(M, N, sm_count(x.device)):
+        _check(library().exl3_fp8_skinny(_ptr(x), _c_int64(x.stride(0)), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(out), code, _c_int(M), _c_int(N),
+                                         _c_int(Kd), _c_int(1 if gated else 0), _stream()), "fp8_skinny")
+        return out
+    codes = torch.empty((M, Kd), dtype=torch.uint8, device=x.device)
+    sx = torch.empty((blocks, M), dtype=torch.float32, device=x.device)
+    _check(library().exl3_fp8_quantize(_ptr(x), _c_int64(x.stride(0)), _c_int(M), _c_int(Kd), _ptr(codes), _ptr(sx), _c_int(1), _stream()), "fp8_quantize")
+    _check(library().exl3_fp8_pair(_ptr(codes), _ptr(sx), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(out), code, _c_int(M), _c_int(N), _c_int(Kd),
+                                   _c_int(1 if gated else 0), _stream()), "fp8_pair")
+    return out
