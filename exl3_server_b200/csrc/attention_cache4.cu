@@ -165,13 +165,20 @@ kv4_attn_kernel(const A4Args a) {
 
   // the queries: a warp takes every fourth column
   for (int c = warp; c < COLS; c += A4_WARPS) {
+    if (c >= r.cols) {
+      if (lane < NG) s_qsum[c][lane] = 0.0f;
+      if (lane == 0) s_f[c] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NG / 2; ++i) s_q[c][i * 32 + lane] = 0;
+      continue;
+    }
     float x[NG];
     float top = 0.0f;
     const int col = r.col0 + c;
     const __nv_bfloat16* src = a.q + (int64_t)(r.start + col / r.G) * a.q_stride + (int64_t)(kvh * r.G + col % r.G) * HD;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      x[i] = c < r.cols ? __bfloat162float(src[i * 32 + lane]) : 0.0f;
+      x[i] = __bfloat162float(src[i * 32 + lane]);
       top = fmaxf(top, fabsf(x[i]));
     }
     top = warp_max(top);
@@ -304,9 +311,19 @@ kv4_attn_kernel(const A4Args a) {
           vw[mt][h][0] = v.x; vw[mt][h][1] = v.y; vw[mt][h][2] = v.z; vw[mt][h][3] = v.w;
         }
 #pragma unroll
-        for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i] < 0x7f800000u ? vw[mt][h][i] : 0u);      // (NaN groups do not count)
+        for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i]);
       }
     top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
+    if (top == 0x7f800000u) {                               // NaN groups do not count (nor does what lies behind the last token)
+      top = 0;
+#pragma unroll
+      for (int mt = 0; mt < NT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i] < 0x7f800000u ? vw[mt][h][i] : 0u);
+      top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
+    }
     float keep = 1.0f;
     if (top > sc_top) {                                     // (the same for the whole warp)
       const float old = F;
@@ -385,7 +402,7 @@ kv4_attn_kernel(const A4Args a) {
     if (!ok) break;
     const int key0 = (tile_a + warp + A4_WARPS * i) * TT;
     const unsigned char* buf = ring + stage * TILE;
-    if (key0 + TT - 1 <= full_hi && key0 >= full_lo && r.cols == COLS) walk(buf, key0, std::false_type());
+    if (key0 + TT - 1 <= full_hi && key0 >= full_lo) walk(buf, key0, std::false_type());
     else walk(buf, key0, std::true_type());
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // this lane's reads come before the copy that follows
     __syncwarp();

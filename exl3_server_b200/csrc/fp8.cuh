@@ -17,10 +17,6 @@ __device__ inline uint32_t pack4(float a, float b, float c, float d) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return (uint32_t)hi << 16 | lo;
 }
-// The largest magnitude of a block from its lanes' maxima, and what its values are multiplied by.
-__device__ inline float multiplier(float amax) { return __fdiv_rn(TOP, fmaxf(amax, TINY)); }
-__device__ inline float scale_of(float amax) { return __fdiv_rn(fmaxf(amax, TINY), TOP); }
-
 // 16 bfloat16 (two vectors of 16 bytes) as floats.
 __device__ inline void widen16(const uint4& a, const uint4& b, float (&v)[16]) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};

@@ -4,13 +4,13 @@
 //
 // Two blocks of a cluster are one tensor core (tcgen05.mma.cta_group::2, kind::f8f6f4, M 256, N 256, K 32) on tiles of 256 x 256; each copies its
 // 128 rows of codes of x and of w per 128 of K (16 KB + 16 KB, a ring of five stages).  The scales differ from block to block of K, so
-// every block's 128-long product is an accumulator of its own: two of 256 columns take turns in tensor memory, and eight
+// every block's 128-long product is an accumulator of its own: two times two of 128 columns take turns in tensor memory (four, so that the
+// way from a product's end to its accumulator's next use, two signals and a read, is covered by the three others), and eight
 // warps add them, times sx * sw, to 128 float32 registers a thread (lane = row, a warp's half of the columns has one sw).  Per block the
-// products take 512 cycles of the tensor core, the accumulator's way out 256 of tensor memory's and 64 packed fma a thread, so the tensor core
-// stays the bound.
+// products take 512 cycles of the tensor core, the accumulators' way out 256 of tensor memory's and 64 packed fma a thread.
 //
 //   warp 0    TMA producer (both blocks)     warp 1    even block: issues the MMAs; both: tensor memory
-//   warps 2-9 accumulators and results (both blocks)
+//   warps 4-11 accumulators and results (both blocks); the first four warps leave them their registers
 //
 // Every wait is bounded; when one runs out the kernel records a code, leaves its loops, waits (bounded) for its copies, meets its partner at
 // the cluster barrier, frees its tensor memory and returns.
@@ -44,15 +44,22 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int M, int
   float top = fp8::amax16(v);
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // one division a lane: even lanes the multiplier, odd lanes the scale
+  top = fmaxf(top, fp8::TINY);
+  const float quot = __fdiv_rn((j & 1) ? top : fp8::TOP, (j & 1) ? fp8::TOP : top);
+  const float mul = __shfl_sync(0xffffffffu, quot, threadIdx.x & 24);
   if (!live) return;
-  if (k < K) *reinterpret_cast<uint4*>(codes + (int64_t)row * K + k) = fp8::codes16(v, fp8::multiplier(top));
-  if (j == 0) sx[transposed ? (int64_t)b * M + row : (int64_t)row * kblocks + b] = fp8::scale_of(top);
+  if (k < K) *reinterpret_cast<uint4*>(codes + (int64_t)row * K + k) = fp8::codes16(v, mul);
+  if (j == 1) sx[transposed ? (int64_t)b * M + row : (int64_t)row * kblocks + b] = quot;
 }
 
 // ---- the product ------------------------------------------------------------------------------------------------------
 
 constexpr int F8P_BM = 256, F8P_BN = 256, F8P_STAGES = 6, F8P_EPI = 8;
-constexpr int F8P_THREADS = 64 + 32 * F8P_EPI;
+constexpr int F8P_THREADS = 128 + 32 * F8P_EPI;
+// Registers a thread after the split: 128 x 40 + 256 x 208 is less than what the block is launched with, 384 x 168.
+constexpr int F8P_REGS_LOW = 40, F8P_REGS_HIGH = 208;
+static_assert(128 * F8P_REGS_LOW + 256 * F8P_REGS_HIGH <= 384 * 168, "a split that the launch does not cover waits for good");
 constexpr uint32_t F8P_HALF = 128 * 128;                  // bytes of a block's 128 rows of either operand
 constexpr uint32_t F8P_SMEM = 1024 + F8P_STAGES * 2 * F8P_HALF;
 
@@ -75,6 +82,12 @@ __device__ inline void f8p_fma2(float2& acc, uint32_t d0, uint32_t d1, float s) 
   asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(c));
 }
 
+// One arrival on an mbarrier of the pair's even block.  What it orders is tensor memory's reads, complete when tcgen05.wait::ld has passed: with
+// a release over the cluster the warp would wait here for its global loads too (the factors ahead), which took as long as all the rest.
+__device__ inline void f8p_arrive(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+
 __global__ void __launch_bounds__(F8P_THREADS, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const F8pArgs a) {
   constexpr int STAGES = F8P_STAGES;
@@ -83,7 +96,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   unsigned char* base = f8p_raw + ((1024u - (smem_u32(f8p_raw) & 1023u)) & 1023u);
   unsigned char* sA = base;
   unsigned char* sB = base + STAGES * F8P_HALF;
-  __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[4], acc_empty[4];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -92,7 +105,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     prefetch_map(&map_x);
     prefetch_map(&map_w);
     for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 2 * F8P_EPI); }
+    for (int b = 0; b < 4; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 2 * F8P_EPI); }
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc_pair<512>(&tmem_slot);
@@ -110,56 +123,67 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     n = r / rows;
   };
   bool ok = true;
-
-  if (warp == 0) {
-    uint32_t it = 0;
-    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
-      int tm, tn;
-      place(tile, tm, tn);
-      const int m0 = tm * F8P_BM + (int)rank * 128, n0 = tn * F8P_BN + (int)rank * 128;
-      for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const int s = it % STAGES;
-        ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((it / STAGES) & 1) ^ 1));
-        if (!ok) break;
-        if (lane == 0) {
-          const uint32_t bar = cluster_addr(full + s, 0);
-          if (rank == 0) mbar_expect_tx(full + s, 4 * F8P_HALF);
-          tma_load_2d_pair(sA + s * F8P_HALF, &map_x, bar, kb * fp8::KB, m0);
-          tma_load_2d_pair(sB + s * F8P_HALF, &map_w, bar, kb * fp8::KB, n0);
-        }
-        __syncwarp();
-      }
-    }
-    if (!ok) {
-      if (lane == 0) atomicExch(&g_f8p_error, 1);
-      if (rank == 0)
-        for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= it; ++back) mbar_wait(full + (it - back) % STAGES, ((it - back) / STAGES) & 1);
-    }
-  } else if (warp == 1) {
-    if (rank == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8P_REGS_LOW));
+    if (warp == 0) {
       uint32_t it = 0;
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+        int tm, tn;
+        place(tile, tm, tn);
+        const int m0 = tm * F8P_BM + (int)rank * 128, n0 = tn * F8P_BN + (int)rank * 128;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          const int s = it % STAGES, buf = it & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1) && mbar_wait(full + s, (it / STAGES) & 1));
+          const int s = it % STAGES;
+          ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((it / STAGES) & 1) ^ 1));
           if (!ok) break;
-          fence_after();
           if (lane == 0) {
-            const uint64_t da = smem_desc_k128(smem_u32(sA + s * F8P_HALF)), db = smem_desc_k128(smem_u32(sB + s * F8P_HALF));
-#pragma unroll
-            for (int k = 0; k < 4; ++k) fp8::mma_ss_pair(tmem + buf * F8P_BN, da + 2 * k, db + 2 * k, fp8::idesc_e4m3(F8P_BM, F8P_BN), k > 0);
-            mma_commit_pair(empty + s);
-            mma_commit_pair(acc_full + buf);
+            const uint32_t bar = cluster_addr(full + s, 0);
+            if (rank == 0) mbar_expect_tx(full + s, 4 * F8P_HALF);
+            tma_load_2d_pair(sA + s * F8P_HALF, &map_x, bar, kb * fp8::KB, m0);
+            tma_load_2d_pair(sB + s * F8P_HALF, &map_w, bar, kb * fp8::KB, n0);
           }
           __syncwarp();
         }
       }
-      if (!ok && lane == 0) atomicExch(&g_f8p_error, 2);
+      if (!ok) {
+        if (lane == 0) atomicExch(&g_f8p_error, 1);
+        if (rank == 0)
+          for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= it; ++back) mbar_wait(full + (it - back) % STAGES, ((it - back) / STAGES) & 1);
+      }
+    } else if (warp == 1) {
+      if (rank == 0) {
+        uint32_t it = 0;
+        for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+          for (int kb = 0; kb < kblocks; ++kb, ++it) {
+            const int s = it % STAGES;
+            ok = __all_sync(0xffffffffu, mbar_wait(full + s, (it / STAGES) & 1));
+            if (!ok) break;
+            const uint64_t da = smem_desc_k128(smem_u32(sA + s * F8P_HALF));
+  #pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {                // rows 64 h .. of both blocks' halves of w
+              const uint32_t buf = (it & 1) * 2 + h;
+              ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1));
+              if (!ok) break;
+              fence_after();
+              if (lane == 0) {
+                const uint64_t db = smem_desc_k128(smem_u32(sB + s * F8P_HALF + h * (F8P_HALF / 2)));
+  #pragma unroll
+                for (int k = 0; k < 4; ++k) fp8::mma_ss_pair(tmem + buf * 128, da + 2 * k, db + 2 * k, fp8::idesc_e4m3(F8P_BM, 128), k > 0);
+                if (h == 1) mma_commit_pair(empty + s);
+                mma_commit_pair(acc_full + buf);
+              }
+              __syncwarp();
+            }
+            if (!ok) break;
+          }
+        }
+        if (!ok && lane == 0) atomicExch(&g_f8p_error, 2);
+      }
     }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t lane_taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
-    const uint32_t acc_empty_addr[2] = {cluster_addr(acc_empty, 0), cluster_addr(acc_empty + 1, 0)};
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8P_REGS_HIGH));
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t lane_taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 64;
+    const uint32_t acc_empty_addr = cluster_addr(acc_empty, 0);
     uint32_t it = 0;
     for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
       int tm, tn;
@@ -173,27 +197,28 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       auto factor = [&](int kb) { return live && inside && kb < kblocks ? __ldcg(a.sx + (int64_t)kb * a.M + row) * __ldg(sw + kb) : 0.0f; };
       float f_next = factor(0);
       for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const uint32_t buf = it & 1;
         const float f = f_next;
         f_next = factor(kb + 1);
-        ok = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (it >> 1) & 1));
-        if (!ok) break;
-        fence_after();
-        uint32_t d[2][32];
-        tmem_ld32_issue(lane_taddr + buf * F8P_BN, d[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait(d[c & 1]);
-          if (c < 3) {
-            tmem_ld32_issue(lane_taddr + buf * F8P_BN + (c + 1) * 32, d[(c + 1) & 1]);
-          } else {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty_addr[buf]);
-          }
+        for (uint32_t h = 0; h < 2; ++h) {                  // this warp's columns 64 h .. 64 h + 63
+          const uint32_t buf = (it & 1) * 2 + h;
+          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (it >> 1) & 1));
+          if (!ok) break;
+          fence_after();
+          uint32_t d0[32], d1[32];
+          tmem_ld32_issue(lane_taddr + buf * 128, d0);
+          tmem_ld32_issue(lane_taddr + buf * 128 + 32, d1);
+          tmem_ld_wait(d0);
+          tmem_ld_wait(d1);
+          fence_before();
+          __syncwarp();
+          if (lane == 0) f8p_arrive(acc_empty_addr + buf * 8);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) f8p_fma2(acc[c * 16 + e], d[c & 1][2 * e], d[c & 1][2 * e + 1], f);
+          for (int e = 0; e < 16; ++e) f8p_fma2(acc[h * 32 + e], d0[2 * e], d0[2 * e + 1], f);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) f8p_fma2(acc[h * 32 + 16 + e], d1[2 * e], d1[2 * e + 1], f);
         }
+        if (!ok) break;
       }
       if (!ok) break;
       if (!live || !inside) continue;

@@ -11,7 +11,7 @@
 // four warps add it to float32 registers times sx * sw while the next one is formed.
 //
 //   warp 0     TMA producer of weight tiles          warp 1      issues the MMAs; allocates and frees tensor memory
-//   warps 2-5  take accumulators, thread = feature    warps 6-9   x to codes, eight lanes a row of 128
+//   warps 2-5  take accumulators, thread = feature    the rest    x to codes, eight lanes a row of 128
 //
 // K is cut over the S blocks of a cluster; their sums meet through distributed shared memory, block r adding up columns r, r + S, ... in the
 // blocks' order.  Every wait is bounded; when one runs out the kernel records a code, waits (bounded) for its copies, meets the cluster
@@ -23,9 +23,11 @@ namespace exl3 {
 
 using namespace tc5;
 
-constexpr int F8S_THREADS = 320;
+// Warps that round x: four rows a warp at a time, so that a block's columns are one round (16) or two (32, 64).
+__host__ __device__ constexpr int f8s_xwarps(int nb) { return nb == 64 ? 8 : 4; }
+__host__ __device__ constexpr int f8s_threads(int nb) { return 192 + 32 * f8s_xwarps(nb); }
 constexpr int F8S_MAX_SPLIT = 8;
-constexpr int F8S_SLOTS = 8;                              // scales of the last blocks of K: more than the stages and the two accumulators
+constexpr int F8S_SLOTS = 16;                             // scales of the last blocks of K: more than the stages and the two accumulators
 
 __host__ __device__ constexpr int f8s_stages(int nb) { return nb <= 32 ? 5 : 6; }
 __host__ __device__ constexpr uint32_t f8s_smem(int nb) { return 1024 + f8s_stages(nb) * (16384 + nb * 128); }
@@ -48,12 +50,12 @@ __device__ inline float f8s_ld_peer(const float* mine, uint32_t rank) {
 }
 
 template <int NB>
-__global__ void __launch_bounds__(F8S_THREADS, 1)
+__global__ void __launch_bounds__(f8s_threads(NB), 1)
 fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
-  constexpr int STAGES = f8s_stages(NB);
+  constexpr int STAGES = f8s_stages(NB), XW = f8s_xwarps(NB), THREADS = f8s_threads(NB);
   constexpr uint32_t W_BYTES = 16384, X_BYTES = NB * 128;
   static_assert(STAGES * W_BYTES >= NB * 128 * 4, "the sums take the place of the weight tiles");
-  static_assert(STAGES + 2 <= F8S_SLOTS, "scales live until their accumulator has been taken");
+  static_assert(STAGES + 3 <= F8S_SLOTS, "scales live until their accumulator has been added up");
   extern __shared__ unsigned char f8s_raw[];
   unsigned char* base = f8s_raw + ((1024u - (smem_u32(f8s_raw) & 1023u)) & 1023u);
   unsigned char* sW = base;
@@ -69,9 +71,9 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
   constexpr int TM_COLS = 2 * NB < 32 ? 32 : 2 * NB;
   if (threadIdx.x == 0) {
     prefetch_map(&map_w);
-    for (int s = 0; s < STAGES; ++s) { mbar_init(wfull + s, 1); mbar_init(xfull + s, 4); mbar_init(empty + s, 1); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(wfull + s, 1); mbar_init(xfull + s, XW); mbar_init(empty + s, 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 4); }
-    for (int s = 0; s < F8S_SLOTS; ++s) mbar_init(sfull + s, 4);
+    for (int s = 0; s < F8S_SLOTS; ++s) mbar_init(sfull + s, XW);
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc<TM_COLS>(&tmem_slot);
@@ -131,12 +133,23 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
       ok = __all_sync(0xffffffffu, mbar_wait(sfull + slot, (i / F8S_SLOTS) & 1) && mbar_wait(acc_full + buf, (i >> 1) & 1));
       if (!ok) break;
       fence_after();
+      constexpr int CH = NB < 32 ? NB : 32;
 #pragma unroll
-      for (int c0 = 0; c0 < NB; c0 += 16) {
-        uint32_t d[16];
-        tmem_ld16(tmem + buf * NB + c0 + ((uint32_t)(q * 32) << 16), d);
+      for (int c0 = 0; c0 < NB; c0 += CH) {
+        uint32_t d[CH];
+        const uint32_t at = tmem + buf * NB + c0 + ((uint32_t)(q * 32) << 16);
+        if constexpr (CH == 16) {
+          tmem_ld16(at, d);
+        } else {
+          tmem_ld32(at, d);
+        }
+        if (c0 + CH == NB) {                               // the accumulator is free, its last part in registers
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + buf);
+        }
 #pragma unroll
-        for (int c = 0; c < 16; c += 4) {
+        for (int c = 0; c < CH; c += 4) {
           const float4 sx = *reinterpret_cast<const float4*>(&s_sx[slot][c0 + c]);
           acc[c0 + c] = fmaf(__uint_as_float(d[c]), sx.x * w, acc[c0 + c]);
           acc[c0 + c + 1] = fmaf(__uint_as_float(d[c + 1]), sx.y * w, acc[c0 + c + 1]);
@@ -144,9 +157,6 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
           acc[c0 + c + 3] = fmaf(__uint_as_float(d[c + 3]), sx.w * w, acc[c0 + c + 3]);
         }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + buf);
     }
     if (!ok && lane == 0) atomicExch(&g_f8s_error, 3);
     // (after a failed wait copies may still be landing in the tiles' place: the sums are not to be trusted, nor written there)
@@ -158,10 +168,11 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
   } else {
     // ---- x to codes: four rows a warp at a time, eight lanes a row, 16 features a lane --------------------------------
     pdl_wait();
-    constexpr int ROUNDS = NB / 16;
+    constexpr int STEP = 4 * XW, ROUNDS = NB / STEP;
+    static_assert(ROUNDS <= 2, "a lane's division is a multiplier or a scale of one round");
     const int j = lane & 7, r0 = (warp - 6) * 4 + (lane >> 3);
     auto fetch = [&](int i, int u, uint4& v0, uint4& v1) {
-      const int row = m0 + u * 16 + r0, k = (kb0 + i) * fp8::KB + j * 16;
+      const int row = m0 + u * STEP + r0, k = (kb0 + i) * fp8::KB + j * 16;
       v0 = v1 = make_uint4(0, 0, 0, 0);
       if (i < n_kb && row < a.M && k < a.K) {
         const uint4* p = reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.ldx + k);
@@ -169,32 +180,49 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
         v1 = __ldcg(p + 1);
       }
     };
-    // a block of K ahead of the one that is rounded
-    uint4 cur[ROUNDS][2], nxt[ROUNDS][2];
+    // two blocks of K ahead of the one that is rounded
+    uint4 v[3][ROUNDS][2];
 #pragma unroll
-    for (int u = 0; u < ROUNDS; ++u) fetch(0, u, cur[u][0], cur[u][1]);
-    for (int i = 0; i < n_kb; ++i) {
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) fetch(d, u, v[d][u][0], v[d][u][1]);
+    auto round = [&](int i, uint4 (&cur)[ROUNDS][2], uint4 (&far)[ROUNDS][2]) -> bool {
       const int s = i % STAGES, slot = i % F8S_SLOTS;
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) fetch(i + 1, u, nxt[u][0], nxt[u][1]);
-      ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1));
-      if (!ok) break;
+      for (int u = 0; u < ROUNDS; ++u) fetch(i + 2, u, far[u][0], far[u][1]);
+      float top[ROUNDS];
 #pragma unroll
       for (int u = 0; u < ROUNDS; ++u) {
-        float v[16];
-        fp8::widen16(cur[u][0], cur[u][1], v);
-        float top = fp8::amax16(v);
+        float f[16];
+        fp8::widen16(cur[u][0], cur[u][1], f);
+        top[u] = fp8::amax16(f);
+      }
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int r = u * 16 + r0;
-        *reinterpret_cast<uint4*>(sX + s * X_BYTES + r * 128 + ((j ^ (r & 7)) << 4)) = fp8::codes16(v, fp8::multiplier(top));
-        if (j == 0) s_sx[slot][r] = fp8::scale_of(top);
+      for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+        for (int u = 0; u < ROUNDS; ++u) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+      // one division a lane: even lanes the multipliers, odd lanes the scales, of the rounds in turn
+      const float mine = fmaxf(ROUNDS == 2 && (j & 2) ? top[ROUNDS - 1] : top[0], fp8::TINY);
+      const float quot = __fdiv_rn((j & 1) ? mine : fp8::TOP, (j & 1) ? fp8::TOP : mine);
+      if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1))) return false;
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) {
+        const float mul = __shfl_sync(0xffffffffu, quot, (lane & 24) + 2 * u);
+        float f[16];
+        fp8::widen16(cur[u][0], cur[u][1], f);
+        const int r = u * STEP + r0;
+        *reinterpret_cast<uint4*>(sX + s * X_BYTES + r * 128 + ((j ^ (r & 7)) << 4)) = fp8::codes16(f, mul);
+        if (j == 2 * u + 1) s_sx[slot][r] = quot;
       }
       fence_smem_to_tma();                                 // the codes are read through the async proxy
       __syncwarp();
       if (lane == 0) { mbar_arrive(xfull + s); mbar_arrive(sfull + slot); }
-#pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) { cur[u][0] = nxt[u][0]; cur[u][1] = nxt[u][1]; }
+      return true;
+    };
+    for (int i = 0; i < n_kb && ok; i += 3) {
+      ok = round(i, v[0], v[2]);
+      if (ok && i + 1 < n_kb) ok = round(i + 1, v[1], v[0]);
+      if (ok && i + 2 < n_kb) ok = round(i + 2, v[2], v[1]);
     }
     if (!ok && lane == 0) atomicExch(&g_f8s_error, 4);
   }
@@ -206,7 +234,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
     const float* part = reinterpret_cast<const float*>(sW);
     const int per = a.gated ? 64 : 128, n_out = a.gated ? a.N / 2 : a.N, o0 = a.gated ? n0 / 2 : n0;
     const int rows = min(NB, a.M - m0), mine = rows > rank ? (rows - rank + a.S - 1) / a.S : 0;
-    for (int i = threadIdx.x; i < mine * per; i += F8S_THREADS) {
+    for (int i = threadIdx.x; i < mine * per; i += THREADS) {
       const int c = rank + i / per * a.S, f = i % per;
       auto total = [&](int feature) {
         if (a.S == 1) return part[c * 128 + feature];
@@ -280,7 +308,7 @@ extern "C" int exl3_fp8_skinny(const void* x, int64_t ldx, const void* w, const 
   a.x = static_cast<const __nv_bfloat16*>(x); a.ldx = ldx; a.sw = sw; a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
   a.M = M; a.N = N; a.K = K; a.S = S; a.gated = gated; a.y_f32 = out_dtype == DT_F32;
   auto go = [&](auto kernel) {
-    launch_pdl_clusters(kernel, dim3(tiles * S, groups), dim3(F8S_THREADS), S, f8s_smem(nb), stream, map, a);
+    launch_pdl_clusters(kernel, dim3(tiles * S, groups), dim3(f8s_threads(nb)), S, f8s_smem(nb), stream, map, a);
   };
   if (nb == 16) go(fp8_skinny_kernel<16>); else if (nb == 32) go(fp8_skinny_kernel<32>); else go(fp8_skinny_kernel<64>);
   return launch_status("fp8_skinny");

@@ -8,6 +8,7 @@ these names: a tensor that is not on a CUDA device is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -1813,6 +1814,37 @@ def residual_step(h: torch.Tensor, a: Optional[torch.Tensor] = None, b: Optional
     return x
 
 
+# ---- entry points that a step calls often: argument types declared once, so that plain numbers go through ----------
+
+_ENTRIES: dict = {}
+_ARG_TYPES = {"p": _c_void_p, "i": _c_int, "l": _c_int64, "f": _c_float}
+
+
+def _entry(name: str, args: str):
+    """The entry point ``name`` with its arguments' types (``p`` pointer, ``i`` int, ``l`` int64, ``f`` float) declared; the last
+    one, the stream, is added here."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = getattr(library(), name)
+        fn.argtypes = [_ARG_TYPES[a] for a in args] + [_c_void_p]
+        fn.restype = _c_int
+        _ENTRIES[name] = fn
+    return fn
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    if t is None:
+        return 0
+    if not t.is_cuda:
+        raise KernelLibraryError("kernel called with a tensor that is not on a CUDA device; "
+                                 "there is no CPU implementation of the product path")
+    return t.data_ptr()
+
+
+def _raw_stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 # ---- the 4-bit key/value cache (format: cache4.cuh) ----------------------------------------------------------
 
 KV4_PAGE = 64
@@ -1820,10 +1852,9 @@ KV4_PAGE = 64
 
 def kv4_page_bytes(head_dim: int) -> int:
     """Bytes of a page of 64 tokens of one key/value head, keys and values together (head sizes 64 and 128)."""
-    n = int(library().exl3_kv4_page_bytes(_c_int(head_dim)))
-    if n == 0:
+    if head_dim not in (64, 128):
         raise KernelLibraryError(f"the 4-bit cache takes heads of 64 or 128, got {head_dim}")
-    return n
+    return 80 * head_dim          # 64 tokens of head_dim / 2 bytes of codes and head_dim / 8 of numbers, keys and values
 
 
 def kv4_pool(pages: int, kv_heads: int, head_dim: int, device) -> torch.Tensor:
@@ -1866,15 +1897,22 @@ def kv4_store(qkv: torch.Tensor, inv_freq: Optional[torch.Tensor], tok_pos: torc
         _int32(t, n, "kv4_store")
         if t.numel() < T:
             raise KernelLibraryError(f"kv4_store: {n} has {t.numel()} entries for {T} tokens")
-    hi, lo = _rotary_rows(inv_freq, head_dim, "kv4_store") if inv_freq is not None else (_c_void_p(0), _c_void_p(0))
+    hi = lo = 0
+    if inv_freq is not None:
+        half = head_dim // 2
+        if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or tuple(inv_freq.shape) not in ((half,), (2, half)):
+            raise KernelLibraryError(f"kv4_store: inv_freq must be float32 [{half}], or [2, {half}] (see rotary_table)")
+        hi = _addr(inv_freq)
+        lo = hi + 4 * half if inv_freq.dim() == 2 else 0
     if out is None:
         out = torch.empty((T, heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
         raise KernelLibraryError(f"kv4_store: out must be contiguous bfloat16 {(T, heads * head_dim)}")
-    _check(library().exl3_kv4_store(
-        _ptr(qkv), _c_int64(qkv.stride(0)), _ptr(out), hi, lo, _ptr(tok_pos), _ptr(tok_seq), _ptr(block_table),
-        _c_int(block_table.stride(0)), _ptr(pool), _c_int64(pool.shape[0]), _c_int(T), _c_int(heads), _c_int(kv_heads),
-        _c_int(head_dim), _stream()), "kv4_store")
+    rc = _entry("exl3_kv4_store", "plppppppipliiii")(
+        _addr(qkv), qkv.stride(0), _addr(out), hi, lo, _addr(tok_pos), _addr(tok_seq), _addr(block_table), block_table.stride(0),
+        _addr(pool), pool.shape[0], T, heads, kv_heads, head_dim, _raw_stream())
+    if rc:
+        _check(rc, "kv4_store")
     return out
 
 
@@ -1884,10 +1922,15 @@ def kv4_load(pool: torch.Tensor, pages: torch.Tensor, head_dim: int):
     _kv4_check_pool(pool, None, head_dim, "kv4_load")
     _int32(pages, "pages", "kv4_load")
     n, kv_heads = pages.numel(), pool.shape[1]
-    k, v = (torch.empty((n, kv_heads, KV4_PAGE, head_dim), dtype=torch.bfloat16, device=pool.device) for _ in range(2))
-    _check(library().exl3_kv4_load(_ptr(pool), _c_int64(pool.shape[0]), _ptr(pages), _c_int(n), _c_int(kv_heads),
-                                   _c_int(head_dim), _ptr(k), _ptr(v), _ptr(None), _stream()), "kv4_load")
+    k, v = torch.empty((2, n, kv_heads, KV4_PAGE, head_dim), dtype=torch.bfloat16, device=pool.device).unbind(0)
+    _kv4_unpack(pool, pages, n, head_dim, k.data_ptr(), v.data_ptr(), 0)
     return k, v
+
+
+def _kv4_unpack(pool: torch.Tensor, pages: torch.Tensor, n: int, head_dim: int, k: int, v: int, table: int) -> None:
+    rc = _entry("exl3_kv4_load", "plpiiippp")(_addr(pool), pool.shape[0], _addr(pages), n, pool.shape[1], head_dim, k, v, table, _raw_stream())
+    if rc:
+        _check(rc, "kv4_load")
 
 
 def kv4_attn_status() -> int:
@@ -1898,14 +1941,29 @@ def kv4_attn_status() -> int:
 KV4_FEW_COLUMNS = 64        # new tokens times query heads per key/value head up to which the keys are walked as codes
 
 
+@functools.lru_cache(maxsize=4096)
 def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: int, span: int, window: int, sms: int):
-    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys."""
+    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys, by a small model of the kernel's time: a block takes 3 us and its
+    tiles, at 0.23 us each while it is alone and at 0.11 us (0.17 us with 16 columns) times the blocks that share its SM when these are more;
+    joining chunks takes 3 us."""
     tiles = max(1, -(-span * head_dim // 4096))
-    slots = sms * (3 if columns == 8 else 2)
-    total = rows * kv_heads * groups * tiles
-    chunk = -(-total // slots) if total <= 16 * slots else max(16, min(64, total // (4 * slots)))
-    chunk = max(4, min(128, -(-chunk // 4) * 4))
-    return chunk, (tiles - 1) // chunk + 1 + (1 if window > 0 and tiles > 1 else 0)
+    per_sm = 3 if columns == 8 else 2
+    each = 0.11 if columns == 8 else 0.17
+    items = rows * kv_heads * groups
+    best = None
+    for n in range(1, min(tiles, 1024) + 1):
+        chunk = -(-tiles // n)
+        if chunk > 128 or (n > 1 and chunk < 4):
+            continue
+        n = -(-tiles // chunk)
+        blocks = items * n
+        waves = -(-blocks // (per_sm * sms))
+        here = min(per_sm, -(-blocks // sms))
+        cost = waves * (3.0 + chunk * max(0.23, each * here)) + (3.0 if n > 1 else 0.0)
+        if best is None or cost < best[0] - 1e-9:
+            best = (cost, chunk, n)
+    _, chunk, n = best
+    return chunk, n + (1 if window > 0 and tiles > 1 else 0)
 
 
 def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row_start: Optional[torch.Tensor],
@@ -1941,23 +1999,23 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         raise KernelLibraryError(f"kv4_attn: out must be contiguous bfloat16 {(T, heads * head_dim)}")
     if T == 0 or rows == 0:
         return out
-    lib = library()
     columns_wanted = max_new * (heads // kv_heads)
     if tiles is not None and columns_wanted > KV4_FEW_COLUMNS:
         return _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window,
                                 workspace, out)
     columns = 8 if columns_wanted <= 8 else 16
+    groups = -(-columns_wanted // columns)
     span = min(max_len, window + max_new - 1) if window > 0 else max_len
-    chunk, chunks = _kv4_chunks(rows, kv_heads, -(-columns_wanted // columns), columns, head_dim, max(1, span), window, sm_count(q.device))
-    lib.exl3_kv4_attn_scratch.restype = _c_int64
-    need = int(lib.exl3_kv4_attn_scratch(_c_int(rows), _c_int(max_new), _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_int(chunks)))
-    scratch = None
-    if need:
+    chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, sm_count(q.device))
+    need, scratch = 0, None
+    if chunks > 1:
+        need = rows * kv_heads * groups * chunks * columns * (head_dim + 4)
         scratch = workspace.plain(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
-    _check(lib.exl3_kv4_attn(
-        _ptr(q), _c_int64(q.stride(0)), _ptr(out), _ptr(pool), _c_int64(pool.shape[0]), _ptr(block_table), _c_int(block_table.stride(0)),
-        _ptr(row_start), _ptr(row_pos0), _c_int(rows), _c_int(max_new), _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_int(window),
-        _c_float(scale), _c_int(chunk), _c_int(chunks), _ptr(scratch), _c_int64(need), _stream()), "kv4_attn")
+    rc = _entry("exl3_kv4_attn", "plpplpippiiiiiifiipl")(
+        _addr(q), q.stride(0), _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), _addr(row_start),
+        _addr(row_pos0), rows, max_new, heads, kv_heads, head_dim, window, scale, chunk, chunks, _addr(scratch), need, _raw_stream())
+    if rc:
+        _check(rc, "kv4_attn")
     return out
 
 
@@ -1972,8 +2030,7 @@ def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv
     k, v = (scratch[i * floats:(i + 1) * floats].view(torch.bfloat16).view(shape) for i in range(2))
     table = scratch[2 * floats:2 * floats + n].view(torch.int32).view(rows, width)
     pages = block_table[:rows] if block_table.stride(0) == width else block_table[:rows].contiguous()
-    _check(library().exl3_kv4_load(_ptr(pool), _c_int64(pool.shape[0]), _ptr(pages), _c_int(n), _c_int(kv_heads), _c_int(head_dim),
-                                   _ptr(k), _ptr(v), _ptr(table), _stream()), "kv4_load")
+    _kv4_unpack(pool, pages, n, head_dim, k.data_ptr(), v.data_ptr(), table.data_ptr())
     return attn_prefill_tc(q, q.stride(0), out, k, v, table, row_start, row_pos0, tiles[0], tiles[1], tiles[2], heads, kv_heads,
                            head_dim, KV4_PAGE, window, scale)
 
@@ -2006,9 +2063,14 @@ def fp8_quantize(x: torch.Tensor):
     M, Kd = x.shape
     codes = torch.empty((M, Kd), dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty((M, -(-Kd // FP8_BLOCK)), dtype=torch.float32, device=x.device)
-    _check(library().exl3_fp8_quantize(_ptr(x), _c_int64(x.stride(0)), _c_int(M), _c_int(Kd), _ptr(codes), _ptr(scales), _c_int(0),
-                                       _stream()), "fp8_quantize")
+    _fp8_round(x, codes, scales, 0)
     return codes, scales
+
+
+def _fp8_round(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, transposed: int) -> None:
+    rc = _entry("exl3_fp8_quantize", "pliippi")(_addr(x), x.stride(0), x.shape[0], x.shape[1], _addr(codes), _addr(scales), transposed, _raw_stream())
+    if rc:
+        _check(rc, "fp8_quantize")
 
 
 def fp8_quantize_weight(w: torch.Tensor):
@@ -2068,16 +2130,20 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
         out = torch.empty(shape, dtype=out_dtype, device=x.device)
     elif tuple(out.shape) != shape or not out.is_contiguous():
         raise KernelLibraryError(f"fp8_linear: out must be contiguous {shape}")
-    code = _c_int(dtype_code(out.dtype))
+    code = dtype_code(out.dtype)
     if M == 0:
         return out
     if _fp8_few(M, N, sm_count(x.device)):
-        _check(library().exl3_fp8_skinny(_ptr(x), _c_int64(x.stride(0)), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(out), code, _c_int(M), _c_int(N),
-                                         _c_int(Kd), _c_int(1 if gated else 0), _stream()), "fp8_skinny")
+        rc = _entry("exl3_fp8_skinny", "plppppiiiii")(_addr(x), x.stride(0), _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
+                                                      1 if gated else 0, _raw_stream())
+        if rc:
+            _check(rc, "fp8_skinny")
         return out
     codes = torch.empty((M, Kd), dtype=torch.uint8, device=x.device)
     sx = torch.empty((blocks, M), dtype=torch.float32, device=x.device)
-    _check(library().exl3_fp8_quantize(_ptr(x), _c_int64(x.stride(0)), _c_int(M), _c_int(Kd), _ptr(codes), _ptr(sx), _c_int(1), _stream()), "fp8_quantize")
-    _check(library().exl3_fp8_pair(_ptr(codes), _ptr(sx), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(out), code, _c_int(M), _c_int(N), _c_int(Kd),
-                                   _c_int(1 if gated else 0), _stream()), "fp8_pair")
+    _fp8_round(x, codes, sx, 1)
+    rc = _entry("exl3_fp8_pair", "ppppppiiiii")(_addr(codes), _addr(sx), _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
+                                                1 if gated else 0, _raw_stream())
+    if rc:
+        _check(rc, "fp8_pair")
     return out
