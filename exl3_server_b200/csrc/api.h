@@ -477,13 +477,14 @@ int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const void* pool, 
 int exl3_kv4_attn_status();
 // 8-bit floating point (e4m3, fp8.cuh): w codes [N, K] with scales sw [ceil(N / 128), ceil(K / 128)], x bfloat16 rounded to codes with a scale per row
 // and 128 features; y = x w^T (+ bias), or with `gated` silu(gate) * up for rows of w in eights (N / 2 wide).  K a multiple of 16.
-// exl3_fp8_quantize: codes [M, K] and scales [M, blocks], or [blocks, M] with `transposed`, which exl3_fp8_pair takes.
+// exl3_fp8_quantize: codes [M, K] and scales [M, blocks], or [blocks, M] with `transposed`, which exl3_fp8_wide takes.
 int exl3_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, float* sx, int transposed, cudaStream_t stream);
-int exl3_fp8_skinny(const void* x, int64_t ldx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M, int N, int K,
-                    int gated, cudaStream_t stream);
-int exl3_fp8_pair(const void* codes, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M, int N,
+// exl3_fp8_skinny, a few rows: x in bfloat16 up to 16, else its codes with the transposed scales in sx.
+int exl3_fp8_skinny(const void* x, int64_t ldx, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M,
+                    int N, int K, int gated, cudaStream_t stream);
+int exl3_fp8_wide(const void* codes, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M, int N,
                   int K, int gated, cudaStream_t stream);
 // Codes left by bounded waits that ran out (0: none); cleared by the calls.
 int exl3_fp8_skinny_status();
-int exl3_fp8_pair_status();
+int exl3_fp8_wide_status();
 }

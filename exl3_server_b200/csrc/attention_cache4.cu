@@ -31,7 +31,7 @@ namespace exl3 {
 using namespace kv4;
 
 constexpr int A4_WARPS = 4;
-constexpr int A4_STAGES = 3;
+constexpr int A4_STAGES = 2;
 constexpr int A4_MAX_CHUNK = 32 * A4_WARPS;               // tiles: a warp keeps its page numbers one a lane
 constexpr uint32_t A4_WAIT_LIMIT = 1u << 22;              // polls of some tens of cycles: a fraction of a second
 
@@ -113,10 +113,10 @@ template <int HD> struct A4Range {
 };
 
 template <int HD, int NC>
-__global__ void __launch_bounds__(A4_WARPS * 32, NC == 1 ? 3 : 2)
+__global__ void __launch_bounds__(A4_WARPS * 32, NC == 1 ? 4 : 2)
 kv4_attn_kernel(const A4Args a) {
   constexpr int COLS = 8 * NC, TT = tile_tokens(HD), NT = TT / 16, NG = HD / 32, SPP = HD / 64;
-  constexpr int RING = A4_STAGES * TILE;
+  constexpr int RING = A4_STAGES * TILE;                    // (COLS * HD * 4 bytes of results fit)
   static_assert(COLS * HD * 4 <= RING, "a warp's results take the place of its ring");
   extern __shared__ __align__(128) unsigned char a4_smem_raw[];
   __shared__ uint64_t full[A4_WARPS][A4_STAGES];

@@ -51,14 +51,6 @@ __device__ inline void mma_ss(uint32_t d_tmem, uint64_t da, uint64_t db, uint32_
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
       ::"r"(d_tmem), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
 }
-__device__ inline void mma_ss_pair(uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
-      ::"r"(d_tmem), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
-}
-
 // A [rows, K] row-major matrix of codes in boxes of box_rows x 128 bytes, 128B swizzle, zeros outside.  K a multiple of 16.
 inline int make_map(CUtensorMap* map, const void* ptr, int64_t rows, int K, int box_rows, const char* who) {
   tc5::EncodeTiledFn fn = tc5::encode_fn();

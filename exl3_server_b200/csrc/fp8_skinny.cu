@@ -3,15 +3,16 @@
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} cx[m, k] cw[n, k]  (+ bias, or silu(gate) * up)
 //
 // A decode step's product reads every weight once and is bound by that.  The weights are the 128-row operand of tcgen05.mma
-// (kind::f8f6f4), one tile of 128 x 128 codes = 16 KB per copy; the batch is the narrow operand (16, 32 or 64 columns).  x comes in
-// bfloat16 and is rounded to codes by the block itself, straight into the swizzled operand, so that there is no kernel ahead of this one;
-// a block does that for its own range of K, once for 128 features.
+// (kind::f8f6f4), one tile of 128 x 128 codes = 16 KB per copy; the batch is the narrow operand (16, 32 or 64 columns).  Up to 16 rows
+// x comes in bfloat16 and is rounded to codes by the block itself, straight into the swizzled operand, so that there is no kernel ahead of this
+// one; a block does that for its own range of K, once for 128 features.  For more rows that is too much to do over again in every block
+// (64 rows x 6,144, K 4,096: 26 us), and x's codes come by TMA from the kernel ahead.
 //
 // The scales differ from block to block of K, so each block's 128-long product is an accumulator of its own (two in turn in tensor memory), and
 // four warps add it to float32 registers times sx * sw while the next one is formed.
 //
 //   warp 0     TMA producer of weight tiles          warp 1      issues the MMAs; allocates and frees tensor memory
-//   warps 2-5  take accumulators, thread = feature    the rest    x to codes, eight lanes a row of 128
+//   warps 2-5  take accumulators, thread = feature    the rest    x to codes, eight lanes a row of 128 (or its scales)
 //
 // K is cut over the S blocks of a cluster; their sums meet through distributed shared memory, block r adding up columns r, r + S, ... in the
 // blocks' order.  Every wait is bounded; when one runs out the kernel records a code, waits (bounded) for its copies, meets the cluster
@@ -23,20 +24,21 @@ namespace exl3 {
 
 using namespace tc5;
 
-// Warps that round x: four rows a warp at a time, so that a block's columns are one round (16) or two (32, 64).
-__host__ __device__ constexpr int f8s_xwarps(int nb) { return nb == 64 ? 8 : 4; }
+// Warps behind the first six: 16 columns, four that round x, four rows each; 32 and 64, one that brings the scales.
+__host__ __device__ constexpr int f8s_xwarps(int nb) { return nb == 16 ? 4 : 1; }
 __host__ __device__ constexpr int f8s_threads(int nb) { return 192 + 32 * f8s_xwarps(nb); }
 constexpr int F8S_MAX_SPLIT = 8;
 constexpr int F8S_SLOTS = 16;                             // scales of the last blocks of K: more than the stages and the two accumulators
 
-__host__ __device__ constexpr int f8s_stages(int nb) { return nb <= 32 ? 5 : 6; }
+__host__ __device__ constexpr int f8s_stages(int nb) { return nb <= 32 ? 5 : 4; }      // two blocks an SM
 __host__ __device__ constexpr uint32_t f8s_smem(int nb) { return 1024 + f8s_stages(nb) * (16384 + nb * 128); }
 
 static __device__ int g_f8s_error = 0;
 
 struct F8sArgs {
-  const __nv_bfloat16* x;
+  const __nv_bfloat16* x;    // 16 columns
   int64_t ldx;
+  const float* sx;           // 32 and 64 columns: [blocks of K, M], beside x's codes in map_x
   const float* sw;           // [ceil(N / 128), blocks of K]
   const __nv_bfloat16* bias;
   void* y;
@@ -50,17 +52,18 @@ __device__ inline float f8s_ld_peer(const float* mine, uint32_t rank) {
 }
 
 template <int NB>
-__global__ void __launch_bounds__(f8s_threads(NB), 1)
-fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
+__global__ void __launch_bounds__(f8s_threads(NB), 2)
+fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8sArgs a) {
   constexpr int STAGES = f8s_stages(NB), XW = f8s_xwarps(NB), THREADS = f8s_threads(NB);
+  constexpr bool ROUNDS_X = NB == 16;                       // x comes in bfloat16 and is rounded here
   constexpr uint32_t W_BYTES = 16384, X_BYTES = NB * 128;
   static_assert(STAGES * W_BYTES >= NB * 128 * 4, "the sums take the place of the weight tiles");
-  static_assert(STAGES + 3 <= F8S_SLOTS, "scales live until their accumulator has been added up");
+  static_assert(STAGES + 3 <= F8S_SLOTS, "scales of the rounding warps live until their accumulator has been added up: they follow the tiles' ring");
   extern __shared__ unsigned char f8s_raw[];
   unsigned char* base = f8s_raw + ((1024u - (smem_u32(f8s_raw) & 1023u)) & 1023u);
   unsigned char* sW = base;
   unsigned char* sX = base + STAGES * W_BYTES;
-  __shared__ uint64_t wfull[STAGES], xfull[STAGES], empty[STAGES], acc_full[2], acc_empty[2], sfull[F8S_SLOTS];
+  __shared__ uint64_t wfull[STAGES], xfull[STAGES], empty[STAGES], acc_full[2], acc_empty[2], sfull[F8S_SLOTS], sempty[F8S_SLOTS];
   __shared__ __align__(16) float s_sx[F8S_SLOTS][NB];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -71,9 +74,10 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
   constexpr int TM_COLS = 2 * NB < 32 ? 32 : 2 * NB;
   if (threadIdx.x == 0) {
     prefetch_map(&map_w);
+    if (!ROUNDS_X) prefetch_map(&map_x);
     for (int s = 0; s < STAGES; ++s) { mbar_init(wfull + s, 1); mbar_init(xfull + s, XW); mbar_init(empty + s, 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 4); }
-    for (int s = 0; s < F8S_SLOTS; ++s) mbar_init(sfull + s, XW);
+    for (int s = 0; s < F8S_SLOTS; ++s) { mbar_init(sfull + s, XW); mbar_init(sempty + s, 4); }
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc<TM_COLS>(&tmem_slot);
@@ -85,15 +89,29 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
   bool ok = true;
 
   if (warp == 0) {
-    // ---- weights: no kernel writes them, so the first tiles are asked for before the kernel ahead has ended -----------
-    uint32_t asked = 0;
-    for (int i = 0; i < n_kb && ok; ++i, ++asked) {
+    // ---- weights: no kernel writes them, so the first tiles are asked for before the kernel ahead has ended; x's codes are its work --------
+    const int early = n_kb < STAGES ? n_kb : STAGES;
+    if (lane == 0)
+      for (int i = 0; i < early; ++i) {
+        mbar_expect_tx(wfull + i, W_BYTES + (ROUNDS_X ? 0 : X_BYTES));
+        tma_load_2d(sW + i * W_BYTES, &map_w, wfull + i, (kb0 + i) * fp8::KB, n0);
+      }
+    __syncwarp();
+    if (!ROUNDS_X) {
+      pdl_wait();
+      if (lane == 0)
+        for (int i = 0; i < early; ++i) tma_load_2d(sX + i * X_BYTES, &map_x, wfull + i, (kb0 + i) * fp8::KB, m0);
+      __syncwarp();
+    }
+    uint32_t asked = early;
+    for (int i = early; i < n_kb && ok; ++i, ++asked) {
       const int s = i % STAGES;
       ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1));
       if (!ok) break;
       if (lane == 0) {
-        mbar_expect_tx(wfull + s, W_BYTES);
+        mbar_expect_tx(wfull + s, W_BYTES + (ROUNDS_X ? 0 : X_BYTES));
         tma_load_2d(sW + s * W_BYTES, &map_w, wfull + s, (kb0 + i) * fp8::KB, n0);
+        if (!ROUNDS_X) tma_load_2d(sX + s * X_BYTES, &map_x, wfull + s, (kb0 + i) * fp8::KB, m0);
       }
       __syncwarp();
     }
@@ -102,10 +120,11 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
       for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= asked; ++back) mbar_wait(wfull + (asked - back) % STAGES, ((asked - back) / STAGES) & 1);
     }
   } else if (warp == 1) {
+    pdl_wait();                                             // (not on a barrier, whose wait is bounded)
     for (int i = 0; i < n_kb; ++i) {
       const int s = i % STAGES, buf = i & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((i >> 1) & 1) ^ 1) && mbar_wait(wfull + s, (i / STAGES) & 1) &&
-                                       mbar_wait(xfull + s, (i / STAGES) & 1));
+                                       (!ROUNDS_X || mbar_wait(xfull + s, (i / STAGES) & 1)));
       if (!ok) break;
       fence_after();
       if (lane == 0) {
@@ -120,6 +139,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
     if (!ok && lane == 0) atomicExch(&g_f8s_error, 2);
   } else if (warp < 6) {
     // ---- accumulators: lane = feature of this warp's 32, registers over the columns ----------------------------------
+    pdl_wait();
     const int q = warp & 3;
     float acc[NB];
 #pragma unroll
@@ -157,6 +177,10 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
           acc[c0 + c + 3] = fmaf(__uint_as_float(d[c + 3]), sx.w * w, acc[c0 + c + 3]);
         }
       }
+      if (!ROUNDS_X) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sempty + slot);
+      }
     }
     if (!ok && lane == 0) atomicExch(&g_f8s_error, 3);
     // (after a failed wait copies may still be landing in the tiles' place: the sums are not to be trusted, nor written there)
@@ -165,55 +189,66 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const F8sArgs a) {
 #pragma unroll
       for (int c = 0; c < NB; ++c) part[c * 128 + q * 32 + lane] = acc[c];
     }
-  } else {
-    // ---- x to codes: four rows a warp at a time, eight lanes a row, 16 features a lane --------------------------------
+  } else if constexpr (!ROUNDS_X) {
+    // ---- scales of x, a block of K after the other ----------------------------------------------------------------------
     pdl_wait();
-    constexpr int STEP = 4 * XW, ROUNDS = NB / STEP;
-    static_assert(ROUNDS <= 2, "a lane's division is a multiplier or a scale of one round");
-    const int j = lane & 7, r0 = (warp - 6) * 4 + (lane >> 3);
-    auto fetch = [&](int i, int u, uint4& v0, uint4& v1) {
-      const int row = m0 + u * STEP + r0, k = (kb0 + i) * fp8::KB + j * 16;
-      v0 = v1 = make_uint4(0, 0, 0, 0);
-      if (i < n_kb && row < a.M && k < a.K) {
-        const uint4* p = reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.ldx + k);
-        v0 = __ldcg(p);
-        v1 = __ldcg(p + 1);
-      }
+    constexpr int PER = NB / 32;
+    auto fetch = [&](int i, int u) {
+      const int row = m0 + u * 32 + lane;
+      return i < n_kb && row < a.M ? __ldcg(a.sx + (int64_t)(kb0 + i) * a.M + row) : 0.0f;
     };
-    // two blocks of K ahead of the one that is rounded
-    uint4 v[3][ROUNDS][2];
+    float nxt[2][PER];
 #pragma unroll
     for (int d = 0; d < 2; ++d)
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) fetch(d, u, v[d][u][0], v[d][u][1]);
-    auto round = [&](int i, uint4 (&cur)[ROUNDS][2], uint4 (&far)[ROUNDS][2]) -> bool {
+      for (int u = 0; u < PER; ++u) nxt[d][u] = fetch(d, u);
+    for (int i = 0; i < n_kb; ++i) {
+      // the slots are a ring of their own: the tiles' barriers may be two phases on when this warp looks, since the MMAs do not wait for it
+      const int slot = i % F8S_SLOTS;
+      ok = __all_sync(0xffffffffu, mbar_wait(sempty + slot, ((i / F8S_SLOTS) & 1) ^ 1));
+      if (!ok) break;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        s_sx[slot][u * 32 + lane] = nxt[0][u];
+        nxt[0][u] = nxt[1][u];
+        nxt[1][u] = fetch(i + 2, u);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sfull + slot);
+    }
+    if (!ok && lane == 0) atomicExch(&g_f8s_error, 5);
+  } else {
+    // ---- x to codes: four rows a warp at a time, eight lanes a row, 16 features a lane --------------------------------
+    pdl_wait();
+    const int j = lane & 7, r = (warp - 6) * 4 + (lane >> 3);
+    auto fetch = [&](int i, uint4 (&v)[2]) {
+      const int row = m0 + r, k = (kb0 + i) * fp8::KB + j * 16;
+      v[0] = v[1] = make_uint4(0, 0, 0, 0);
+      if (i < n_kb && row < a.M && k < a.K) {
+        const uint4* p = reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.ldx + k);
+        v[0] = __ldcg(p);
+        v[1] = __ldcg(p + 1);
+      }
+    };
+    // two blocks of K ahead of the one that is rounded
+    uint4 v[3][2];
+    fetch(0, v[0]);
+    fetch(1, v[1]);
+    auto round = [&](int i, uint4 (&cur)[2], uint4 (&far)[2]) -> bool {
       const int s = i % STAGES, slot = i % F8S_SLOTS;
+      fetch(i + 2, far);
+      float f[16];
+      fp8::widen16(cur[0], cur[1], f);
+      float top = fp8::amax16(f);
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) fetch(i + 2, u, far[u][0], far[u][1]);
-      float top[ROUNDS];
-#pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) {
-        float f[16];
-        fp8::widen16(cur[u][0], cur[u][1], f);
-        top[u] = fp8::amax16(f);
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1)
-#pragma unroll
-        for (int u = 0; u < ROUNDS; ++u) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
-      // one division a lane: even lanes the multipliers, odd lanes the scales, of the rounds in turn
-      const float mine = fmaxf(ROUNDS == 2 && (j & 2) ? top[ROUNDS - 1] : top[0], fp8::TINY);
-      const float quot = __fdiv_rn((j & 1) ? mine : fp8::TOP, (j & 1) ? fp8::TOP : mine);
+      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // one division a lane: even lanes the multiplier, odd lanes the scale
+      top = fmaxf(top, fp8::TINY);
+      const float quot = __fdiv_rn((j & 1) ? top : fp8::TOP, (j & 1) ? fp8::TOP : top);
+      const uint4 codes = fp8::codes16(f, __shfl_sync(0xffffffffu, quot, lane & 24));
       if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1))) return false;
-#pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) {
-        const float mul = __shfl_sync(0xffffffffu, quot, (lane & 24) + 2 * u);
-        float f[16];
-        fp8::widen16(cur[u][0], cur[u][1], f);
-        const int r = u * STEP + r0;
-        *reinterpret_cast<uint4*>(sX + s * X_BYTES + r * 128 + ((j ^ (r & 7)) << 4)) = fp8::codes16(f, mul);
-        if (j == 2 * u + 1) s_sx[slot][r] = quot;
-      }
+      *reinterpret_cast<uint4*>(sX + s * X_BYTES + r * 128 + ((j ^ (r & 7)) << 4)) = codes;
+      if (j == 1) s_sx[slot][r] = quot;
       fence_smem_to_tma();                                 // the codes are read through the async proxy
       __syncwarp();
       if (lane == 0) { mbar_arrive(xfull + s); mbar_arrive(sfull + slot); }
@@ -276,39 +311,57 @@ extern "C" int exl3_fp8_skinny_status() {
   return v;
 }
 
-extern "C" int exl3_fp8_skinny(const void* x, int64_t ldx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M,
-                               int N, int K, int gated, cudaStream_t stream) {
+// x: bfloat16 [M, K] up to 16 rows; else its codes [M, K] with sx [blocks, M] as exl3_fp8_quantize leaves them with `transposed` (ldx is not used).
+extern "C" int exl3_fp8_skinny(const void* x, int64_t ldx, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype,
+                               int M, int N, int K, int gated, cudaStream_t stream) {
   if (M == 0 || N == 0) return 0;
-  if (M < 0 || N < 0 || K < 16 || K % 16 || (out_dtype != DT_F32 && out_dtype != DT_BF16) || (gated && (N % 16 || bias)) || !x || !w || !sw || !y) {
+  if (M < 0 || N < 0 || K < 16 || K % 16 || (out_dtype != DT_F32 && out_dtype != DT_BF16) || (gated && (N % 16 || bias)) || !x || !w || !sw || !y ||
+      (M > 16 && !sx)) {
     set_error("fp8_skinny: needs K a multiple of 16, N of 16 and no bias where gated, a bfloat16 or float32 result and its arrays, got M=%d N=%d K=%d", M, N, K);
     return ERR_BAD_ARGUMENT;
   }
-  if (!aligned16(x) || !aligned16(w) || ldx % 8) { set_error("fp8_skinny: x, its rows and w must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  if (!aligned16(x) || !aligned16(w) || (M <= 16 && ldx % 8)) { set_error("fp8_skinny: x, its rows and w must be 16-byte aligned"); return ERR_ALIGNMENT; }
   const int nb = M <= 16 ? 16 : M <= 32 ? 32 : 64, groups = ceil_div(M, nb), tiles = ceil_div(N, 128), kblocks = ceil_div(K, 128);
   if (groups > 65535) { set_error("fp8_skinny: %d rows are too many", M); return ERR_UNSUPPORTED; }
-  static int sms = 0;
-  if (!sms) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    cudaError_t e = cudaSuccess;
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(16));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(32));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(64));
-    if (e != cudaSuccess) { sms = 0; set_error("fp8_skinny: cannot get its shared memory: %s", cudaGetErrorString(e)); return (int)e; }
+  const void* fn = nb == 16 ? (const void*)fp8_skinny_kernel<16> : nb == 32 ? (const void*)fp8_skinny_kernel<32> : (const void*)fp8_skinny_kernel<64>;
+  // clusters of 1, 2, 4 and 8 blocks that the GPU runs at once, for each width
+  static int slots[3][4];
+  int (&mine)[4] = slots[nb == 16 ? 0 : nb == 32 ? 1 : 2];
+  if (!mine[0]) {
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(nb));
+    if (e != cudaSuccess) { set_error("fp8_skinny: cannot get its shared memory: %s", cudaGetErrorString(e)); return (int)e; }
+    for (int i = 3; i >= 0; --i) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      cfg.gridDim = dim3(8 * 1024);
+      cfg.blockDim = dim3(f8s_threads(nb));
+      cfg.dynamicSmemBytes = f8s_smem(nb);
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << i;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      mine[i] = cudaOccupancyMaxActiveClusters(&n, fn, &cfg) == cudaSuccess && n > 0 ? n : 1;
+    }
+    cudaGetLastError();
   }
-  // as many blocks a tile as still run side by side, one an SM
-  int S = sms / (tiles * groups);
-  S = S < 1 ? 1 : S > F8S_MAX_SPLIT ? F8S_MAX_SPLIT : S;
-  if (S > kblocks) S = kblocks;
-  CUtensorMap map;
-  int rc = fp8::make_map(&map, w, N, K, 128, "fp8_skinny");
+  // as many blocks a tile as still run side by side
+  int S = 1;
+  for (int i = 1; i < 4 && (1 << i) <= kblocks && tiles * groups <= mine[i]; ++i) S = 1 << i;
+  CUtensorMap map_w, map_x;
+  int rc = fp8::make_map(&map_w, w, N, K, 128, "fp8_skinny");
   if (rc) return rc;
+  map_x = map_w;
+  if (nb > 16) {
+    rc = fp8::make_map(&map_x, x, M, K, nb, "fp8_skinny");
+    if (rc) return rc;
+  }
   F8sArgs a = {};
-  a.x = static_cast<const __nv_bfloat16*>(x); a.ldx = ldx; a.sw = sw; a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
+  a.x = static_cast<const __nv_bfloat16*>(x); a.ldx = ldx; a.sx = sx; a.sw = sw; a.bias = static_cast<const __nv_bfloat16*>(bias); a.y = y;
   a.M = M; a.N = N; a.K = K; a.S = S; a.gated = gated; a.y_f32 = out_dtype == DT_F32;
   auto go = [&](auto kernel) {
-    launch_pdl_clusters(kernel, dim3(tiles * S, groups), dim3(f8s_threads(nb)), S, f8s_smem(nb), stream, map, a);
+    launch_pdl_clusters(kernel, dim3(tiles * S, groups), dim3(f8s_threads(nb)), S, f8s_smem(nb), stream, map_w, map_x, a);
   };
   if (nb == 16) go(fp8_skinny_kernel<16>); else if (nb == 32) go(fp8_skinny_kernel<32>); else go(fp8_skinny_kernel<64>);
   return launch_status("fp8_skinny");

@@ -1142,7 +1142,7 @@ def check_status() -> None:
                                      ("attn_decode", attn_decode_status),
                                      ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status),
                                      ("kv4_attn", kv4_attn_status), ("fp8_skinny", fp8_skinny_status),
-                                     ("fp8_pair", fp8_pair_status)) if fn()]
+                                     ("fp8_wide", fp8_wide_status)) if fn()]
     if gave_up:
         raise KernelLibraryError("a bounded wait ran out in " + ", ".join(gave_up) +
                                  ": a copy or a tensor-core product did not complete in time")
@@ -1947,7 +1947,7 @@ def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: i
     tiles, at 0.23 us each while it is alone and at 0.11 us (0.17 us with 16 columns) times the blocks that share its SM when these are more;
     joining chunks takes 3 us."""
     tiles = max(1, -(-span * head_dim // 4096))
-    per_sm = 3 if columns == 8 else 2
+    per_sm = 4 if columns == 8 else 2
     each = 0.11 if columns == 8 else 0.17
     items = rows * kv_heads * groups
     best = None
@@ -2038,15 +2038,16 @@ def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv
 # ---- products in 8-bit floating point (fp8.cuh) ---------------------------------------------------------------
 
 FP8_BLOCK = 128
-FP8_SKINNY_ROWS = 64        # rows up to which the weight-streaming kernel runs in one group
+FP8_ROUNDED_ROWS = 16       # rows up to which the weight-streaming kernel rounds x itself
+FP8_SKINNY_ROWS = 64        # rows up to which it runs in one group
 
 
 def fp8_skinny_status() -> int:
     return int(library().exl3_fp8_skinny_status())
 
 
-def fp8_pair_status() -> int:
-    return int(library().exl3_fp8_pair_status())
+def fp8_wide_status() -> int:
+    return int(library().exl3_fp8_wide_status())
 
 
 def _fp8_check_x(x: torch.Tensor, what: str) -> None:
@@ -2098,12 +2099,12 @@ def fp8_quantize_weight(w: torch.Tensor):
 
 
 def _fp8_few(M: int, N: int, sms: int) -> bool:
-    """Whether the weight-streaming kernel takes M rows: always up to 64, and in groups of 64 while the paired one's tiles of 256 x 256 would leave
+    """Whether the weight-streaming kernel takes M rows: always up to 64, and in groups of 64 while the other one's tiles of 128 x 256 would leave
     most of the GPU idle."""
     if M <= FP8_SKINNY_ROWS:
         return True
-    tiles = -(-M // 256) * -(-N // 256)
-    return M <= 256 and tiles < sms // 4
+    tiles = -(-M // 128) * -(-N // 256)
+    return M <= 256 and tiles < sms // 2
 
 
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -2133,17 +2134,20 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     code = dtype_code(out.dtype)
     if M == 0:
         return out
-    if _fp8_few(M, N, sm_count(x.device)):
-        rc = _entry("exl3_fp8_skinny", "plppppiiiii")(_addr(x), x.stride(0), _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
-                                                      1 if gated else 0, _raw_stream())
+    few = _fp8_few(M, N, sm_count(x.device))
+    codes = sx = None
+    if M > FP8_ROUNDED_ROWS:
+        codes = torch.empty((M, Kd), dtype=torch.uint8, device=x.device)
+        sx = torch.empty((blocks, M), dtype=torch.float32, device=x.device)
+        _fp8_round(x, codes, sx, 1)
+    if few:
+        rc = _entry("exl3_fp8_skinny", "plpppppiiiii")(_addr(x if codes is None else codes), x.stride(0), _addr(sx), _addr(w), _addr(w_scale), _addr(bias),
+                                                       _addr(out), code, M, N, Kd, 1 if gated else 0, _raw_stream())
         if rc:
             _check(rc, "fp8_skinny")
         return out
-    codes = torch.empty((M, Kd), dtype=torch.uint8, device=x.device)
-    sx = torch.empty((blocks, M), dtype=torch.float32, device=x.device)
-    _fp8_round(x, codes, sx, 1)
-    rc = _entry("exl3_fp8_pair", "ppppppiiiii")(_addr(codes), _addr(sx), _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
+    rc = _entry("exl3_fp8_wide", "ppppppiiiii")(_addr(codes), _addr(sx), _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
                                                 1 if gated else 0, _raw_stream())
     if rc:
-        _check(rc, "fp8_pair")
+        _check(rc, "fp8_wide")
     return out
