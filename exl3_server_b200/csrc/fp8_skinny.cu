@@ -8,7 +8,7 @@
 // one; a block does that for its own range of K, once for 128 features.  For more rows that is too much to do over again in every block
 // (64 rows x 6,144, K 4,096: 26 us), and x's codes come by TMA from the kernel ahead.
 //
-// The scales differ from block to block of K, so each block's 128-long product is an accumulator of its own (two in turn in tensor memory), and
+// The scales differ from block to block of K, so each block's 128-long product is an accumulator of its own (four in turn in tensor memory), and
 // four warps add it to float32 registers times sx * sw while the next one is formed.
 //
 //   warp 0     TMA producer of weight tiles          warp 1      issues the MMAs; allocates and frees tensor memory
@@ -28,7 +28,7 @@ using namespace tc5;
 __host__ __device__ constexpr int f8s_xwarps(int nb) { return nb == 16 ? 4 : 1; }
 __host__ __device__ constexpr int f8s_threads(int nb) { return 192 + 32 * f8s_xwarps(nb); }
 constexpr int F8S_MAX_SPLIT = 8;
-constexpr int F8S_SLOTS = 16;                             // scales of the last blocks of K: more than the stages and the two accumulators
+constexpr int F8S_SLOTS = 16;                             // scales of the last blocks of K: more than the stages and the accumulators
 
 __host__ __device__ constexpr int f8s_stages(int nb) { return nb <= 32 ? 5 : 4; }      // two blocks an SM
 __host__ __device__ constexpr uint32_t f8s_smem(int nb) { return 1024 + f8s_stages(nb) * (16384 + nb * 128); }
@@ -55,15 +55,16 @@ template <int NB>
 __global__ void __launch_bounds__(f8s_threads(NB), 2)
 fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8sArgs a) {
   constexpr int STAGES = f8s_stages(NB), XW = f8s_xwarps(NB), THREADS = f8s_threads(NB);
+  constexpr int ACCS = 4;                                   // accumulators in turn: the way round one is longer than a tile takes to come
   constexpr bool ROUNDS_X = NB == 16;                       // x comes in bfloat16 and is rounded here
   constexpr uint32_t W_BYTES = 16384, X_BYTES = NB * 128;
   static_assert(STAGES * W_BYTES >= NB * 128 * 4, "the sums take the place of the weight tiles");
-  static_assert(STAGES + 3 <= F8S_SLOTS, "scales of the rounding warps live until their accumulator has been added up: they follow the tiles' ring");
+  static_assert(STAGES + ACCS + 1 <= F8S_SLOTS, "scales of the rounding warps live until their accumulator has been added up: they follow the tiles' ring");
   extern __shared__ unsigned char f8s_raw[];
   unsigned char* base = f8s_raw + ((1024u - (smem_u32(f8s_raw) & 1023u)) & 1023u);
   unsigned char* sW = base;
   unsigned char* sX = base + STAGES * W_BYTES;
-  __shared__ uint64_t wfull[STAGES], xfull[STAGES], empty[STAGES], acc_full[2], acc_empty[2], sfull[F8S_SLOTS], sempty[F8S_SLOTS];
+  __shared__ uint64_t wfull[STAGES], xfull[STAGES], empty[STAGES], acc_full[ACCS], acc_empty[ACCS], sfull[F8S_SLOTS], sempty[F8S_SLOTS];
   __shared__ __align__(16) float s_sx[F8S_SLOTS][NB];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -71,12 +72,12 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   const int tile = blockIdx.x / a.S, n0 = tile * 128, m0 = blockIdx.y * NB;
   const int kblocks = (a.K + fp8::KB - 1) / fp8::KB;
   const int kb0 = (int)((int64_t)kblocks * rank / a.S), kb1 = (int)((int64_t)kblocks * (rank + 1) / a.S), n_kb = kb1 - kb0;
-  constexpr int TM_COLS = 2 * NB < 32 ? 32 : 2 * NB;
+  constexpr int TM_COLS = ACCS * NB;
   if (threadIdx.x == 0) {
     prefetch_map(&map_w);
     if (!ROUNDS_X) prefetch_map(&map_x);
     for (int s = 0; s < STAGES; ++s) { mbar_init(wfull + s, 1); mbar_init(xfull + s, XW); mbar_init(empty + s, 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 4); }
+    for (int b = 0; b < ACCS; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 4); }
     for (int s = 0; s < F8S_SLOTS; ++s) { mbar_init(sfull + s, XW); mbar_init(sempty + s, 4); }
     mbar_init_fence();
   }
@@ -106,7 +107,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     uint32_t asked = early;
     for (int i = early; i < n_kb && ok; ++i, ++asked) {
       const int s = i % STAGES;
-      ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1));
+      ok = __all_sync(0xffffffffu, fp8::wait(empty + s, ((i / STAGES) & 1) ^ 1));
       if (!ok) break;
       if (lane == 0) {
         mbar_expect_tx(wfull + s, W_BYTES + (ROUNDS_X ? 0 : X_BYTES));
@@ -117,14 +118,14 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     }
     if (!ok) {
       if (lane == 0) atomicExch(&g_f8s_error, 1);
-      for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= asked; ++back) mbar_wait(wfull + (asked - back) % STAGES, ((asked - back) / STAGES) & 1);
+      for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= asked; ++back) fp8::wait(wfull + (asked - back) % STAGES, ((asked - back) / STAGES) & 1);
     }
   } else if (warp == 1) {
     pdl_wait();                                             // (not on a barrier, whose wait is bounded)
     for (int i = 0; i < n_kb; ++i) {
-      const int s = i % STAGES, buf = i & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((i >> 1) & 1) ^ 1) && mbar_wait(wfull + s, (i / STAGES) & 1) &&
-                                       (!ROUNDS_X || mbar_wait(xfull + s, (i / STAGES) & 1)));
+      const int s = i % STAGES, buf = i % ACCS;
+      ok = __all_sync(0xffffffffu, fp8::wait(acc_empty + buf, ((i / ACCS) & 1) ^ 1) && fp8::wait(wfull + s, (i / STAGES) & 1) &&
+                                       (!ROUNDS_X || fp8::wait(xfull + s, (i / STAGES) & 1)));
       if (!ok) break;
       fence_after();
       if (lane == 0) {
@@ -141,80 +142,102 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     // ---- accumulators: lane = feature of this warp's 32, registers over the columns ----------------------------------
     pdl_wait();
     const int q = warp & 3;
-    float acc[NB];
+    float2 acc[NB / 2];
 #pragma unroll
-    for (int c = 0; c < NB; ++c) acc[c] = 0.0f;
+    for (int c = 0; c < NB / 2; ++c) acc[c] = make_float2(0.0f, 0.0f);
     const float* sw = a.sw + (int64_t)tile * kblocks + kb0;
-    float w_next = n_kb > 0 ? __ldg(sw) : 0.0f;
-    for (int i = 0; i < n_kb; ++i) {
-      const int buf = i & 1, slot = i % F8S_SLOTS;
-      const float w = w_next;
-      if (i + 1 < n_kb) w_next = __ldg(sw + i + 1);
-      ok = __all_sync(0xffffffffu, mbar_wait(sfull + slot, (i / F8S_SLOTS) & 1) && mbar_wait(acc_full + buf, (i >> 1) & 1));
-      if (!ok) break;
+    const uint32_t at = tmem + ((uint32_t)(q * 32) << 16);
+    uint32_t d[2][16];
+    float w0 = 0.0f, w1 = 0.0f;
+    if (ROUNDS_X && n_kb > 0) { w0 = __ldg(sw); w1 = __ldg(sw + min(1, n_kb - 1)); }
+    auto open = [&](int i, uint32_t (&r)[16]) -> bool {    // the first 16 columns of step i's accumulator
+      if (!__all_sync(0xffffffffu, fp8::wait(acc_full + i % ACCS, (i / ACCS) & 1))) return false;
       fence_after();
-      constexpr int CH = NB < 32 ? NB : 32;
+      fp8::ld16_issue(at + i % ACCS * NB, r);
+      return true;
+    };
+    constexpr int P = NB / 16;
+    auto step = [&](int i, int first) -> bool {            // d[first] is on its way; leaves the next step's in d[first ^ (P & 1)]
+      const int slot = i % F8S_SLOTS;
+      float w = 1.0f;                                       // (else the scales come with it)
+      if (ROUNDS_X) {                                       // asked for two steps ahead
+        w = w0;
+        w0 = w1;
+        w1 = __ldg(sw + min(i + 2, n_kb - 1));
+      }
+      if (!__all_sync(0xffffffffu, fp8::wait(sfull + slot, (i / F8S_SLOTS) & 1))) return false;
+      bool good = true;
 #pragma unroll
-      for (int c0 = 0; c0 < NB; c0 += CH) {
-        uint32_t d[CH];
-        const uint32_t at = tmem + buf * NB + c0 + ((uint32_t)(q * 32) << 16);
-        if constexpr (CH == 16) {
-          tmem_ld16(at, d);
-        } else {
-          tmem_ld32(at, d);
-        }
-        if (c0 + CH == NB) {                               // the accumulator is free, its last part in registers
+      for (int p = 0; p < P; ++p) {
+        uint32_t (&now)[16] = d[(first + p) & 1];
+        uint32_t (&next)[16] = d[(first + p + 1) & 1];
+        fp8::ld16_wait(now);
+        if (p + 1 < P) {
+          fp8::ld16_issue(at + i % ACCS * NB + (p + 1) * 16, next);
+        } else {                                           // the accumulator is free, its last part in registers
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + buf);
+          if (lane == 0) mbar_arrive(acc_empty + i % ACCS);
+          if (i + 1 < n_kb) good = open(i + 1, next);
         }
 #pragma unroll
-        for (int c = 0; c < CH; c += 4) {
-          const float4 sx = *reinterpret_cast<const float4*>(&s_sx[slot][c0 + c]);
-          acc[c0 + c] = fmaf(__uint_as_float(d[c]), sx.x * w, acc[c0 + c]);
-          acc[c0 + c + 1] = fmaf(__uint_as_float(d[c + 1]), sx.y * w, acc[c0 + c + 1]);
-          acc[c0 + c + 2] = fmaf(__uint_as_float(d[c + 2]), sx.z * w, acc[c0 + c + 2]);
-          acc[c0 + c + 3] = fmaf(__uint_as_float(d[c + 3]), sx.w * w, acc[c0 + c + 3]);
+        for (int c = 0; c < 16; c += 4) {
+          float4 sx = *reinterpret_cast<const float4*>(&s_sx[slot][p * 16 + c]);
+          if (ROUNDS_X) { sx.x *= w; sx.y *= w; sx.z *= w; sx.w *= w; }
+          fp8::fma2(acc[(p * 16 + c) / 2], now[c], now[c + 1], sx.x, sx.y);
+          fp8::fma2(acc[(p * 16 + c) / 2 + 1], now[c + 2], now[c + 3], sx.z, sx.w);
         }
       }
       if (!ROUNDS_X) {
         __syncwarp();
         if (lane == 0) mbar_arrive(sempty + slot);
       }
+      return good;
+    };
+    if (n_kb > 0) ok = open(0, d[0]);
+    for (int i = 0; i < n_kb && ok; i += 2) {
+      ok = step(i, 0);
+      if (ok && i + 1 < n_kb) ok = step(i + 1, P & 1);
     }
     if (!ok && lane == 0) atomicExch(&g_f8s_error, 3);
     // (after a failed wait copies may still be landing in the tiles' place: the sums are not to be trusted, nor written there)
     if (ok) {
       float* part = reinterpret_cast<float*>(sW);
 #pragma unroll
-      for (int c = 0; c < NB; ++c) part[c * 128 + q * 32 + lane] = acc[c];
+      for (int c = 0; c < NB; ++c) part[c * 128 + q * 32 + lane] = c & 1 ? acc[c / 2].y : acc[c / 2].x;
     }
   } else if constexpr (!ROUNDS_X) {
     // ---- scales of x, a block of K after the other ----------------------------------------------------------------------
     pdl_wait();
     constexpr int PER = NB / 32;
-    auto fetch = [&](int i, int u) {
-      const int row = m0 + u * 32 + lane;
-      return i < n_kb && row < a.M ? __ldcg(a.sx + (int64_t)(kb0 + i) * a.M + row) : 0.0f;
-    };
-    float nxt[2][PER];
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-#pragma unroll
-      for (int u = 0; u < PER; ++u) nxt[d][u] = fetch(d, u);
-    for (int i = 0; i < n_kb; ++i) {
-      // the slots are a ring of their own: the tiles' barriers may be two phases on when this warp looks, since the MMAs do not wait for it
-      const int slot = i % F8S_SLOTS;
-      ok = __all_sync(0xffffffffu, mbar_wait(sempty + slot, ((i / F8S_SLOTS) & 1) ^ 1));
-      if (!ok) break;
+    constexpr int AHEAD = 4;                                // steps; multiplied only when they are put down (a product at the load would wait for it)
+    float x[AHEAD][PER], w[AHEAD];
+    auto fetch = [&](int i, float (&v)[PER], float& ws) {
+      if (i >= n_kb) return;
+      ws = __ldg(a.sw + (int64_t)tile * kblocks + kb0 + i);
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
-        s_sx[slot][u * 32 + lane] = nxt[0][u];
-        nxt[0][u] = nxt[1][u];
-        nxt[1][u] = fetch(i + 2, u);
+        const int row = m0 + u * 32 + lane;
+        v[u] = row < a.M ? __ldcg(a.sx + (int64_t)(kb0 + i) * a.M + row) : 0.0f;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sfull + slot);
+    };
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) fetch(d, x[d], w[d]);
+    for (int i0 = 0; i0 < n_kb && ok; i0 += AHEAD) {
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        const int i = i0 + d;
+        if (i >= n_kb) break;
+        // the slots are a ring of their own: the tiles' barriers may be two phases on when this warp looks, since the MMAs do not wait for it
+        const int slot = i % F8S_SLOTS;
+        ok = __all_sync(0xffffffffu, fp8::wait(sempty + slot, ((i / F8S_SLOTS) & 1) ^ 1));
+        if (!ok) break;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) s_sx[slot][u * 32 + lane] = x[d][u] * w[d];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sfull + slot);
+        fetch(i + AHEAD, x[d], w[d]);
+      }
     }
     if (!ok && lane == 0) atomicExch(&g_f8s_error, 5);
   } else {
@@ -246,7 +269,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       top = fmaxf(top, fp8::TINY);
       const float quot = __fdiv_rn((j & 1) ? top : fp8::TOP, (j & 1) ? fp8::TOP : top);
       const uint4 codes = fp8::codes16(f, __shfl_sync(0xffffffffu, quot, lane & 24));
-      if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / STAGES) & 1) ^ 1))) return false;
+      if (!__all_sync(0xffffffffu, fp8::wait(empty + s, ((i / STAGES) & 1) ^ 1))) return false;
       *reinterpret_cast<uint4*>(sX + s * X_BYTES + r * 128 + ((j ^ (r & 7)) << 4)) = codes;
       if (j == 1) s_sx[slot][r] = quot;
       fence_smem_to_tma();                                 // the codes are read through the async proxy
@@ -300,6 +323,35 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   if (warp == 1) tmem_free<TM_COLS>(tmem);
 }
 
+// Never launched: a block of this kernel's shape for the driver's count of clusters, which for a kernel that allocates tensor memory says one block
+// an SM, while two run (as gemm_skinny.cu found by timing).
+__global__ void __launch_bounds__(f8s_threads(16)) f8s_block_shape_kernel() {}
+
+// Clusters of s blocks that run at once, two blocks an SM.
+static int f8s_max_clusters(int s) {
+  static int count[F8S_MAX_SPLIT + 1] = {};
+  if (count[s]) return count[s];
+  const int smem = (int)f8s_smem(32) + 5 * 1024;
+  int n = 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(1024 * s);
+  cfg.blockDim = dim3(f8s_threads(16));
+  cfg.dynamicSmemBytes = smem;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = s;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(f8s_block_shape_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, f8s_block_shape_kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 1;
+  }
+  count[s] = n;
+  return n;
+}
+
 }  // namespace exl3
 
 using namespace exl3;
@@ -323,32 +375,18 @@ extern "C" int exl3_fp8_skinny(const void* x, int64_t ldx, const float* sx, cons
   if (!aligned16(x) || !aligned16(w) || (M <= 16 && ldx % 8)) { set_error("fp8_skinny: x, its rows and w must be 16-byte aligned"); return ERR_ALIGNMENT; }
   const int nb = M <= 16 ? 16 : M <= 32 ? 32 : 64, groups = ceil_div(M, nb), tiles = ceil_div(N, 128), kblocks = ceil_div(K, 128);
   if (groups > 65535) { set_error("fp8_skinny: %d rows are too many", M); return ERR_UNSUPPORTED; }
-  const void* fn = nb == 16 ? (const void*)fp8_skinny_kernel<16> : nb == 32 ? (const void*)fp8_skinny_kernel<32> : (const void*)fp8_skinny_kernel<64>;
-  // clusters of 1, 2, 4 and 8 blocks that the GPU runs at once, for each width
-  static int slots[3][4];
-  int (&mine)[4] = slots[nb == 16 ? 0 : nb == 32 ? 1 : 2];
-  if (!mine[0]) {
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(nb));
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(fp8_skinny_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(16));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(32));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_skinny_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)f8s_smem(64));
     if (e != cudaSuccess) { set_error("fp8_skinny: cannot get its shared memory: %s", cudaGetErrorString(e)); return (int)e; }
-    for (int i = 3; i >= 0; --i) {
-      cudaLaunchConfig_t cfg = {};
-      cudaLaunchAttribute attr[1];
-      cfg.gridDim = dim3(8 * 1024);
-      cfg.blockDim = dim3(f8s_threads(nb));
-      cfg.dynamicSmemBytes = f8s_smem(nb);
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 1u << i;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      int n = 0;
-      mine[i] = cudaOccupancyMaxActiveClusters(&n, fn, &cfg) == cudaSuccess && n > 0 ? n : 1;
-    }
-    cudaGetLastError();
+    configured = true;
   }
-  // as many blocks a tile as still run side by side
-  int S = 1;
-  for (int i = 1; i < 4 && (1 << i) <= kblocks && tiles * groups <= mine[i]; ++i) S = 1 << i;
+  // As many cuts of K as still let all clusters run at once, with two blocks of K a block at least.  From N and K only, so that a row's result
+  // does not depend on the rows beside it.
+  int S = F8S_MAX_SPLIT;
+  while (S > 1 && (kblocks / S < 2 || tiles > f8s_max_clusters(S))) --S;
   CUtensorMap map_w, map_x;
   int rc = fp8::make_map(&map_w, w, N, K, 128, "fp8_skinny");
   if (rc) return rc;

@@ -74,30 +74,6 @@ struct F8wArgs {
   int M, N, K, group, gated, y_f32, vec;
 };
 
-__device__ inline void f8w_fma2(float2& acc, uint32_t d0, uint32_t d1, float s) {
-  uint64_t c, d, f;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(c) : "f"(acc.x), "f"(acc.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "f"(s));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(d), "l"(f));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(c));
-}
-
-// A bounded wait that suspends the thread for up to a microsecond at a time: polls without a pause would hold up what they wait for.
-__device__ inline bool f8w_wait(uint64_t* bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t i = 0; i < (1u << 20); ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(addr), "r"(parity), "r"(1000u) : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
-
 __global__ void __launch_bounds__(F8W_THREADS, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const F8wArgs a) {
   constexpr int STAGES = F8W_STAGES;
@@ -139,7 +115,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         place(tile, tm, tn);
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
-          ok = __all_sync(0xffffffffu, f8w_wait(empty + s, ((it / STAGES) & 1) ^ 1));
+          ok = __all_sync(0xffffffffu, fp8::wait(empty + s, ((it / STAGES) & 1) ^ 1));
           if (!ok) break;
           if (lane == 0) {
             mbar_expect_tx(full + s, F8W_A + F8W_B);
@@ -158,13 +134,13 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
-          ok = __all_sync(0xffffffffu, f8w_wait(full + s, (it / STAGES) & 1));
+          ok = __all_sync(0xffffffffu, fp8::wait(full + s, (it / STAGES) & 1));
           if (!ok) break;
           const uint64_t da = smem_desc_k128(smem_u32(sA + s * F8W_A));
 #pragma unroll
           for (uint32_t h = 0; h < 2; ++h) {
             const uint32_t buf = (it & 1) * 2 + h;
-            ok = __all_sync(0xffffffffu, f8w_wait(acc_empty + buf, ((it >> 1) & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, fp8::wait(acc_empty + buf, ((it >> 1) & 1) ^ 1));
             if (!ok) break;
             fence_after();
             if (lane == 0) {
@@ -188,7 +164,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     uint32_t it = 0;
     // the first 32 columns of this half's accumulator of step i
     auto open = [&](uint32_t i, uint32_t (&d)[32]) -> bool {
-      if (!__all_sync(0xffffffffu, f8w_wait(acc_full + (i & 1) * 2 + half, (i >> 1) & 1))) return false;
+      if (!__all_sync(0xffffffffu, fp8::wait(acc_full + (i & 1) * 2 + half, (i >> 1) & 1))) return false;
       fence_after();
       tmem_ld32_issue(lane_taddr + (i & 1) * 256, d);
       return true;
@@ -202,13 +178,17 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll
       for (int c = 0; c < 64; ++c) acc[c] = make_float2(0.0f, 0.0f);
       const float* sw = a.sw + (int64_t)(inside ? n0 / 128 : 0) * kblocks;
-      auto factor = [&](int kb) { return live && inside && kb < kblocks ? __ldcg(a.sx + (int64_t)kb * a.M + row) * __ldg(sw + kb) : 0.0f; };
-      float f_next = factor(0);
+      // the scales of the block at hand and of the two after it, multiplied only when they are used (a product at the load would wait for it)
+      const float* sx = a.sx + (live ? row : 0);
+      const int last = kblocks - 1;
+      float x0 = __ldcg(sx), w0 = __ldg(sw), x1 = __ldcg(sx + (int64_t)min(1, last) * a.M), w1 = __ldg(sw + min(1, last));
       uint32_t d[2][32];
       ok = open(it, d[0]);
       for (int kb = 0; kb < kblocks && ok; ++kb, ++it) {
-        const float f = f_next;
-        f_next = factor(kb + 1);
+        const float f = x0 * w0;
+        x0 = x1; w0 = w1;
+        x1 = __ldcg(sx + (int64_t)min(kb + 2, last) * a.M);
+        w1 = __ldg(sw + min(kb + 2, last));
         // four pieces of 32 columns; the next one is asked for before this one is added up
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -222,7 +202,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             if (kb + 1 < kblocks) ok = open(it + 1, d[0]);
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) f8w_fma2(acc[c * 16 + e], d[c & 1][2 * e], d[c & 1][2 * e + 1], f);
+          for (int e = 0; e < 16; ++e) fp8::fma2(acc[c * 16 + e], d[c & 1][2 * e], d[c & 1][2 * e + 1], f, f);
         }
       }
       if (!ok) break;
