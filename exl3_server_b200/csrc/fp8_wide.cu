@@ -162,11 +162,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const int q = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
     uint32_t it = 0;
-    // the first 32 columns of this half's accumulator of step i
-    auto open = [&](uint32_t i, uint32_t (&d)[32]) -> bool {
+    auto opened = [&](uint32_t i) -> bool {                 // this half's accumulator of step i is complete
       if (!__all_sync(0xffffffffu, fp8::wait(acc_full + (i & 1) * 2 + half, (i >> 1) & 1))) return false;
       fence_after();
-      tmem_ld32_issue(lane_taddr + (i & 1) * 256, d);
       return true;
     };
     for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
@@ -183,27 +181,42 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const int last = kblocks - 1;
       float x0 = __ldcg(sx), w0 = __ldg(sw), x1 = __ldcg(sx + (int64_t)min(1, last) * a.M), w1 = __ldg(sw + min(1, last));
       uint32_t d[2][32];
-      ok = open(it, d[0]);
-      for (int kb = 0; kb < kblocks && ok; ++kb, ++it) {
+      ok = opened(it);
+      if (!ok) break;
+      tmem_ld32_issue(lane_taddr + (it & 1) * 256, d[0]);
+      tmem_ld32_issue(lane_taddr + (it & 1) * 256 + 32, d[1]);
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
         const float f = x0 * w0;
         x0 = x1; w0 = w1;
         x1 = __ldcg(sx + (int64_t)min(kb + 2, last) * a.M);
         w1 = __ldg(sw + min(kb + 2, last));
-        // four pieces of 32 columns; the next one is asked for before this one is added up
+        // 64 columns at a time: a wait is for all loads on their way, so two travel together, and each half's successor is asked for as soon as it
+        // has been added up
+        auto add = [&](int c, const uint32_t (&r)[32]) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait(d[c & 1]);
-          if (c < 3) {
-            tmem_ld32_issue(lane_taddr + (it & 1) * 256 + (c + 1) * 32, d[(c + 1) & 1]);
-          } else {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + (it & 1) * 2 + half);
-            if (kb + 1 < kblocks) ok = open(it + 1, d[0]);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) fp8::fma2(acc[c * 16 + e], d[c & 1][2 * e], d[c & 1][2 * e + 1], f, f);
+          for (int e = 0; e < 16; ++e) fp8::fma2(acc[c * 16 + e], r[2 * e], r[2 * e + 1], f, f);
+        };
+        const uint32_t at = lane_taddr + (it & 1) * 256, nx = lane_taddr + ((it + 1) & 1) * 256;
+        tmem_ld_wait(d[0]);
+        tmem_ld_wait(d[1]);
+        add(0, d[0]);
+        tmem_ld32_issue(at + 64, d[0]);
+        add(1, d[1]);
+        tmem_ld32_issue(at + 96, d[1]);
+        tmem_ld_wait(d[0]);
+        tmem_ld_wait(d[1]);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + (it & 1) * 2 + half);
+        add(2, d[0]);
+        const bool more = kb + 1 < kblocks;
+        if (more) {
+          ok = opened(it + 1);
+          if (!ok) break;
+          tmem_ld32_issue(nx, d[0]);
         }
+        add(3, d[1]);
+        if (more) tmem_ld32_issue(nx + 32, d[1]);
       }
       if (!ok) break;
       if (!live || !inside) continue;
