@@ -65,6 +65,10 @@ __device__ inline bool wait(uint64_t* bar, uint32_t parity) {
   }
   return false;
 }
+// One arrival a warp, by its first lane: a predicated instruction, not a branch that the warp has to come together after.
+__device__ inline void arrive_first(uint64_t* bar, int lane) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(tc5::smem_u32(bar)), "r"(lane) : "memory");
+}
 // 16 columns of tensor memory, the registers valid after ld16_wait.
 __device__ inline void ld16_issue(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(

@@ -91,53 +91,51 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 
   if (warp == 0) {
     // ---- weights: no kernel writes them, so the first tiles are asked for before the kernel ahead has ended; x's codes are its work --------
-    const int early = n_kb < STAGES ? n_kb : STAGES;
-    if (lane == 0)
+    // (one thread from end to end, as in fp8_wide.cu)
+    if (lane == 0) {
+      const int early = n_kb < STAGES ? n_kb : STAGES;
       for (int i = 0; i < early; ++i) {
         mbar_expect_tx(wfull + i, W_BYTES + (ROUNDS_X ? 0 : X_BYTES));
         tma_load_2d(sW + i * W_BYTES, &map_w, wfull + i, (kb0 + i) * fp8::KB, n0);
       }
-    __syncwarp();
-    if (!ROUNDS_X) {
-      pdl_wait();
-      if (lane == 0)
+      if (!ROUNDS_X) {
+        pdl_wait();
         for (int i = 0; i < early; ++i) tma_load_2d(sX + i * X_BYTES, &map_x, wfull + i, (kb0 + i) * fp8::KB, m0);
-      __syncwarp();
-    }
-    uint32_t asked = early;
-    for (int i = early; i < n_kb && ok; ++i, ++asked) {
-      const int s = i % STAGES;
-      ok = __all_sync(0xffffffffu, fp8::wait(empty + s, ((i / STAGES) & 1) ^ 1));
-      if (!ok) break;
-      if (lane == 0) {
+      }
+      uint32_t asked = early;
+      for (int i = early; i < n_kb && ok; ++i) {
+        const int s = i % STAGES;
+        ok = fp8::wait(empty + s, ((i / STAGES) & 1) ^ 1);
+        if (!ok) break;
         mbar_expect_tx(wfull + s, W_BYTES + (ROUNDS_X ? 0 : X_BYTES));
         tma_load_2d(sW + s * W_BYTES, &map_w, wfull + s, (kb0 + i) * fp8::KB, n0);
         if (!ROUNDS_X) tma_load_2d(sX + s * X_BYTES, &map_x, wfull + s, (kb0 + i) * fp8::KB, m0);
+        ++asked;
       }
-      __syncwarp();
+      if (!ok) {
+        atomicExch(&g_f8s_error, 1);
+        for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= asked; ++back) fp8::wait(wfull + (asked - back) % STAGES, ((asked - back) / STAGES) & 1);
+      }
     }
-    if (!ok) {
-      if (lane == 0) atomicExch(&g_f8s_error, 1);
-      for (uint32_t back = 1; back <= (uint32_t)STAGES && back <= asked; ++back) fp8::wait(wfull + (asked - back) % STAGES, ((asked - back) / STAGES) & 1);
-    }
+    __syncwarp();
   } else if (warp == 1) {
-    pdl_wait();                                             // (not on a barrier, whose wait is bounded)
-    for (int i = 0; i < n_kb; ++i) {
-      const int s = i % STAGES, buf = i % ACCS;
-      ok = __all_sync(0xffffffffu, fp8::wait(acc_empty + buf, ((i / ACCS) & 1) ^ 1) && fp8::wait(wfull + s, (i / STAGES) & 1) &&
-                                       (!ROUNDS_X || fp8::wait(xfull + s, (i / STAGES) & 1)));
-      if (!ok) break;
-      fence_after();
-      if (lane == 0) {
+    if (lane == 0) {
+      pdl_wait();                                           // (not on a barrier, whose wait is bounded)
+      for (int i = 0; i < n_kb && ok; ++i) {
+        const int s = i % STAGES, buf = i % ACCS;
+        ok = fp8::wait(acc_empty + buf, ((i / ACCS) & 1) ^ 1) && fp8::wait(wfull + s, (i / STAGES) & 1) &&
+             (!ROUNDS_X || fp8::wait(xfull + s, (i / STAGES) & 1));
+        if (!ok) break;
+        fence_after();
         const uint64_t da = smem_desc_k128(smem_u32(sW + s * W_BYTES)), db = smem_desc_k128(smem_u32(sX + s * X_BYTES));
 #pragma unroll
         for (int k = 0; k < 4; ++k) fp8::mma_ss(tmem + buf * NB, da + 2 * k, db + 2 * k, fp8::idesc_e4m3(128, NB), k > 0);
-        mma_commit(empty + s);
         mma_commit(acc_full + buf);
+        mma_commit(empty + s);
       }
-      __syncwarp();
+      if (!ok) atomicExch(&g_f8s_error, 2);
     }
-    if (!ok && lane == 0) atomicExch(&g_f8s_error, 2);
+    __syncwarp();
   } else if (warp < 6) {
     // ---- accumulators: lane = feature of this warp's 32, registers over the columns ----------------------------------
     pdl_wait();
@@ -177,7 +175,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         } else {                                           // the accumulator is free, its last part in registers
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + i % ACCS);
+          fp8::arrive_first(acc_empty + i % ACCS, lane);
           if (i + 1 < n_kb) good = open(i + 1, next);
         }
 #pragma unroll
@@ -190,7 +188,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       }
       if (!ROUNDS_X) {
         __syncwarp();
-        if (lane == 0) mbar_arrive(sempty + slot);
+        fp8::arrive_first(sempty + slot, lane);
       }
       return good;
     };
@@ -235,7 +233,7 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 #pragma unroll
         for (int u = 0; u < PER; ++u) s_sx[slot][u * 32 + lane] = x[d][u] * w[d];
         __syncwarp();
-        if (lane == 0) mbar_arrive(sfull + slot);
+        fp8::arrive_first(sfull + slot, lane);
         fetch(i + AHEAD, x[d], w[d]);
       }
     }
@@ -274,7 +272,8 @@ fp8_skinny_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       if (j == 1) s_sx[slot][r] = quot;
       fence_smem_to_tma();                                 // the codes are read through the async proxy
       __syncwarp();
-      if (lane == 0) { mbar_arrive(xfull + s); mbar_arrive(sfull + slot); }
+      fp8::arrive_first(xfull + s, lane);
+      fp8::arrive_first(sfull + slot, lane);
       return true;
     };
     for (int i = 0; i < n_kb && ok; i += 3) {
