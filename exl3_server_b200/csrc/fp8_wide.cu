@@ -3,12 +3,13 @@
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} cx[m, k] cw[n, k]  (+ bias, or silu(gate) * up)
 //
 // Tiles of 128 x 256 (kind::f8f6f4), persistent blocks, one an SM, 48 KB of codes per 128 of K in a ring of four stages.  The scales differ
-// from block to block of K, so every block's 128-long product is an accumulator of its own, and there is room in tensor memory for two blocks' only
-// (two times two of 128 x 128).  What bounds such a kernel is therefore the way round: product, signal, tensor memory to registers, signal, next
-// product.  It is kept short: the halves of a tile have accumulators, signals and warps of their own (four warps a half, lane = row, 128
-// float32 sums a thread, one sw a block), a warp has the next 32 columns on their way while it adds up the last (packed fma), and gives the
-// accumulator back before it does; waits suspend in hardware (polling held up the signals).  Pairs of SMs on one tile, which read a third less
-// from L2, took longer: their signals cross between the SMs (2,048 x 28,672, K 4,096: 349 us).
+// from block to block of K, so every block's 128-long product is an accumulator of its own, and tensor memory has room for two of 128 x 256.
+// What bounds such a kernel is therefore the way round: product, signal, tensor memory to registers, signal, next product.  It is kept
+// short: eight warps read an accumulator (lane = row, 128 float32 sums a thread, one sw a block of K), 64 columns at a time, the next ones on their way
+// while the last are added up (packed fma), and give it back before they have added up its end; waits suspend in hardware; the copies and the
+// products are issued by one thread each from end to end.  2,048 x 28,672, K 4,096 with the gate 228 us (2.1 PFLOP/s); what was measured on the
+// way: pairs of SMs on one tile 349 (a third less from L2, but the signals cross between SMs), two accumulators of 128 x 128 per block of K
+// 288 (the instruction reads x's rows again), without the sums 179, copies alone 125.
 //
 //   warp 0    TMA producer     warp 1    issues the MMAs; tensor memory     warps 4-11    sums and results
 //   (the first four warps leave the others their registers)
@@ -81,14 +82,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   unsigned char* base = f8w_raw + ((1024u - (smem_u32(f8w_raw) & 1023u)) & 1023u);
   unsigned char* sA = base;
   unsigned char* sB = base + STAGES * F8W_A;
-  __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[4], acc_empty[4];
+  __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     prefetch_map(&map_x);
     prefetch_map(&map_w);
     for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-    for (int b = 0; b < 4; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, 4); }
+    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + b, 1); mbar_init(acc_empty + b, F8W_EPI); }
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc<512>(&tmem_slot);
@@ -108,8 +109,8 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   bool ok = true;
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8W_REGS_LOW));
-    // One thread each runs these loops from end to end: a warp that parts for its first lane and comes together again at every step took 0.7 us
-    // of it (567 us instead of 311 with the waits by the first lane alone).
+    // One thread each runs these loops from end to end: a warp that parts for its first lane and comes together again at every step loses time
+    // each time (318 us instead of 296).
     if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
@@ -135,18 +136,15 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           const int s = it % STAGES;
           ok = fp8::wait(full + s, (it / STAGES) & 1);
           const uint64_t da = smem_desc_k128(smem_u32(sA + s * F8W_A));
+          const uint32_t buf = it & 1;
+          ok = ok && fp8::wait(acc_empty + buf, ((it >> 1) & 1) ^ 1);
+          if (!ok) break;
+          fence_after();
+          const uint64_t db = smem_desc_k128(smem_u32(sB + s * F8W_B));
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
-            const uint32_t buf = (it & 1) * 2 + h;
-            ok = ok && fp8::wait(acc_empty + buf, ((it >> 1) & 1) ^ 1);
-            if (!ok) break;
-            fence_after();
-            const uint64_t db = smem_desc_k128(smem_u32(sB + s * F8W_B + h * (F8W_B / 2)));
-#pragma unroll
-            for (int k = 0; k < 4; ++k) fp8::mma_ss(tmem + buf * 128, da + 2 * k, db + 2 * k, fp8::idesc_e4m3(F8W_BM, 128), k > 0);
-            mma_commit(acc_full + buf);
-            if (h == 1) mma_commit(empty + s);
-          }
+          for (int k = 0; k < 4; ++k) fp8::mma_ss(tmem + buf * 256, da + 2 * k, db + 2 * k, fp8::idesc_e4m3(F8W_BM, 256), k > 0);
+          mma_commit(acc_full + buf);
+          mma_commit(empty + s);
         }
       }
       if (!ok) atomicExch(&g_f8w_error, 2);
@@ -157,8 +155,8 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const int q = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
     uint32_t it = 0;
-    auto opened = [&](uint32_t i) -> bool {                 // this half's accumulator of step i is complete
-      if (!__all_sync(0xffffffffu, fp8::wait(acc_full + (i & 1) * 2 + half, (i >> 1) & 1))) return false;
+    auto opened = [&](uint32_t i) -> bool {                 // the accumulator of step i is complete
+      if (!__all_sync(0xffffffffu, fp8::wait(acc_full + (i & 1), (i >> 1) & 1))) return false;
       fence_after();
       return true;
     };
@@ -202,7 +200,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         tmem_ld_wait(d[1]);
         fence_before();
         __syncwarp();
-        fp8::arrive_first(acc_empty + (it & 1) * 2 + half, lane);
+        fp8::arrive_first(acc_empty + (it & 1), lane);
         add(2, d[0]);
         const bool more = kb + 1 < kblocks;
         if (more) {
