@@ -3,18 +3,22 @@
 //   s[j] = (q . K[j]) * scale,   j in [max(0, p - window + 1), p] for the token at position p
 //   out  = sum_j softmax(s)[j] * V[j],   K[j] = mn + sc * code by groups of 32 features, V likewise
 //
-// The codes go to the tensor cores as they are.  A code of 4 bits in the low bits of a 16-bit float is a subnormal of fp16, code * 2^-24
-// (or, one nibble up, 16 times that), so one AND makes two operands out of a word and no conversion is done at all; the groups'
-// numbers come in where there is less to multiply.  With q' the query in fp16, scaled by a power of two so that its largest value lies in
-// [1024, 2048), and odd pairs of features divided by 16:
+// The codes go to the tensor cores as they are.  A code of 4 bits in the low half of a byte is an 8-bit float (e4m3), code * 2^-9, and in the
+// low bits of a 16-bit float a subnormal of fp16, code * 2^-24 (or, one nibble up, 16 times that): one AND makes four or two operands
+// out of a word, and no conversion is done at all.  The groups' numbers come in where there is less to multiply.
 //
-//   q . K[j] = sum_groups (sc_g * C_g + mn_g * Q_g),   C_g = the product of codes and q' (mma.m16n8k16, keys x features the 16-row operand,
-//   the queries its 8 columns), Q_g = the sum of the group's q'
+// Keys: q is taken apart into two e4m3 numbers, q' = hi + lo, scaled by a power of two so that its largest value lies in [128, 256); for
+// bfloat16 q (8 bits) that is exact down to 2^-9 of the row's largest, and never off by more than 2^-17 of it.
 //
-// and for the values, with p the softmax's terms, P_g = p * sc_g * F in fp16 (F a power of two that keeps the largest scale seen so far at 2^14:
-// the probabilities keep their 11 bits down to 2^-28 of the largest) as the second product's operand, the codes of 16 tokens the 16-row one, and
-// sum p mn_g beside it in float32.  Scores, maximum, sums and outputs are float32; q is exact in fp16 (bfloat16 has fewer bits) unless it is
-// 2^-20 of the row's largest.
+//   q . K[j] = sum_groups (sc_g * C_g + mn_g * Q_g),   C_g = the product of codes and q' (mma.m16n8k32, keys x features the 16-row operand,
+//   the queries its 8 columns), Q_g = the sum of the group's q', in three bfloat16 parts the operand of one more product with the mn_g
+//
+// Up to four columns, hi and lo stand side by side in the 8 columns of one instruction and meet in the thread that gets both; more columns
+// take an instruction each.
+//
+// Values: with p the softmax's terms, P_g = p * sc_g * F in fp16 (F a power of two that keeps the largest scale seen so far at 2^14, carried by p's
+// exponent: the probabilities keep their 11 bits down to 2^-28 of the largest) is the second product's operand, the codes of 16 tokens the 16-row
+// one, and sum p mn_g goes beside it in float32.  Scores, maximum, sums and outputs are float32.
 //
 // A column is a (new token, query head) of one key/value head: up to 8 or 16 columns share a walk over the codes, each with its own causal limit.
 // A block of four warps takes one (row, key/value head, group of columns, chunk of keys); its warps take every fourth tile of 5,120
@@ -24,6 +28,7 @@
 #include "cache4.cuh"
 
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 #include <type_traits>
 
 namespace exl3 {
@@ -54,6 +59,15 @@ __device__ inline bool a4_wait(uint64_t* bar, uint32_t parity) {
 // fp16 x fp16 -> float32, 16 x 8 x 16.
 __device__ inline void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// e4m3 x e4m3 -> float32, 16 x 8 x 32.
+__device__ inline void a4_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ inline void a4_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ inline uint32_t a4_transpose(uint32_t x) {
@@ -112,15 +126,19 @@ template <int HD> struct A4Range {
   }
 };
 
-template <int HD, int NC>
-__global__ void __launch_bounds__(A4_WARPS * 32, NC == 1 ? 4 : 2)
+// COLS: columns of a block, 4 (hi and lo side by side), 8 or 16.
+template <int HD, int COLS>
+__global__ void __launch_bounds__(A4_WARPS * 32, COLS == 16 ? 2 : COLS == 8 && HD == 128 ? 3 : 4)
 kv4_attn_kernel(const A4Args a) {
-  constexpr int COLS = 8 * NC, TT = tile_tokens(HD), NT = TT / 16, NG = HD / 32, SPP = HD / 64;
-  constexpr int RING = A4_STAGES * TILE;                    // (COLS * HD * 4 bytes of results fit)
+  constexpr bool SIDE = COLS == 4;
+  constexpr int NC = SIDE ? 1 : COLS / 8;                   // column blocks of an instruction
+  constexpr int CP = SIDE ? 1 : 2;                          // columns of a thread in one: t, or 2 t and 2 t + 1
+  constexpr int TT = tile_tokens(HD), NT = TT / 16, NG = HD / 32, SPP = HD / 64;
+  constexpr int RING = A4_STAGES * TILE;
   static_assert(COLS * HD * 4 <= RING, "a warp's results take the place of its ring");
   extern __shared__ __align__(128) unsigned char a4_smem_raw[];
   __shared__ uint64_t full[A4_WARPS][A4_STAGES];
-  __shared__ __align__(16) uint32_t s_q[COLS][HD / 2];      // q' in fp16 pairs
+  __shared__ __align__(16) unsigned char s_q[2][COLS][HD];  // hi and lo, a lane's eight features in the order of its operand's bytes
   __shared__ float s_qsum[COLS][NG], s_f[COLS];
   __shared__ float s_m[A4_WARPS][COLS], s_l[A4_WARPS][COLS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -152,67 +170,75 @@ kv4_attn_kernel(const A4Args a) {
     const int i = __ffs(ask) - 1;
     ask &= ask - 1;
     const int page = __shfl_sync(0xffffffffu, my_page, i);
-    if (lane == 0) {
-      const int tile = tile_a + warp + A4_WARPS * i;
-      const unsigned char* src = a.pool + ((int64_t)page * a.nkv + kvh) * page_bytes(HD) + tile % SPP * TILE;
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a4_smem(bars + stage)), "r"(TILE) : "memory");
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                   ::"r"(a4_smem(ring + stage * TILE)), "l"(src), "r"(TILE), "r"(a4_smem(bars + stage)) : "memory");
-    }
+    const int tile = tile_a + warp + A4_WARPS * i;
+    const unsigned char* src = a.pool + ((int64_t)page * a.nkv + kvh) * page_bytes(HD) + tile % SPP * TILE;
+    asm volatile(                                           // (predicated for the first lane: no branch for the warp to come together after)
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.s32 p, %4, 0;\n\t"
+        "@p mbarrier.arrive.expect_tx.shared::cta.b64 _, [%3], %2;\n\t"
+        "@p cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
+        ::"r"(a4_smem(ring + stage * TILE)), "l"(src), "r"(TILE), "r"(a4_smem(bars + stage)), "r"(lane) : "memory");
   };
   for (int s = 0; s < A4_STAGES; ++s)
     if (ask) request(s);
 
   // the queries: a warp takes every fourth column
   for (int c = warp; c < COLS; c += A4_WARPS) {
-    if (c >= r.cols) {
-      if (lane < NG) s_qsum[c][lane] = 0.0f;
-      if (lane == 0) s_f[c] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NG / 2; ++i) s_q[c][i * 32 + lane] = 0;
-      continue;
-    }
+    const int col = r.col0 + c;
+    const bool there = c < r.cols;                          // columns that are not there are zeros, computed and dropped
+    const __nv_bfloat16* src = a.q + (int64_t)(r.start + (there ? col / r.G : 0)) * a.q_stride + (int64_t)(kvh * r.G + (there ? col % r.G : 0)) * HD;
     float x[NG];
     float top = 0.0f;
-    const int col = r.col0 + c;
-    const __nv_bfloat16* src = a.q + (int64_t)(r.start + col / r.G) * a.q_stride + (int64_t)(kvh * r.G + col % r.G) * HD;
+    bool finite = true;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      x[i] = __bfloat162float(src[i * 32 + lane]);
+      x[i] = there ? __bfloat162float(src[i * 32 + lane]) : 0.0f;
       top = fmaxf(top, fabsf(x[i]));
+      finite = finite && fabsf(x[i]) < __int_as_float(0x7f800000);
     }
     top = warp_max(top);
-    // the exponent that brings the largest value to [2^10, 2^11); a row of zeros, or one that is not finite, stays as it is
-    int e = 0;
-    if (top > 0.0f && top < __int_as_float(0x7f800000)) e = min(max(10 - (int)((__float_as_uint(top) >> 23) & 255) + 127, -100), 100);
+    finite = __all_sync(0xffffffffu, finite);
+    const int e = finite && top > 0.0f ? min(max(7 + 127 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
     const float up = a4_pow2(e);
+    const int place = (lane & 24) + ((lane >> 1) & 1) * 4 + (lane & 1) * 2 + ((lane >> 2) & 1);
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      const __half h = __float2half_rn(x[i] * up);
-      const float sum = warp_sum(__half2float(h));
-      if (lane == 0) s_qsum[c][i] = sum * 0x1p-24f;
-      // pairs 1 and 3 of eight features meet codes 16 times as large
-      reinterpret_cast<__half*>(s_q[c])[i * 32 + lane] = (lane & 2) ? __float2half_rn(x[i] * up * 0.0625f) : h;
+      const float v = x[i] * up;
+      const __nv_fp8_e4m3 hi(v);
+      const __nv_fp8_e4m3 lo(v - (float)hi);
+      const float sum = warp_sum((float)hi + (float)lo);
+      if (lane == 0) s_qsum[c][i] = sum * 0x1p-9f;
+      s_q[0][c][i * 32 + place] = hi.__x;
+      s_q[1][c][i * 32 + place] = lo.__x;
     }
-    if (lane == 0) s_f[c] = a.scale_log2 * a4_pow2(24 - e > 127 ? 127 : 24 - e);
+    if (lane == 0) s_f[c] = finite ? a.scale_log2 * a4_pow2(9 - e) : __int_as_float(0x7fc00000);      // (a row that is not finite: NaN)
   }
   __syncthreads();
 
-  uint32_t qf[NC][NG][4];                                   // this lane's part of q': features 32 group + 8 t .. + 7 of column g
-  float qs[NC][NG][2], fac[NC][2];
-  int limit[NC][2];                                         // the positions of columns 2 t, 2 t + 1
+  constexpr int PARTS = SIDE ? 1 : 2;
+  uint32_t qf[NC][PARTS][NG][2];                            // this lane's part of q': features 32 group + 8 t .. + 7
+  uint32_t qsum[NC][2];                                     // Q_t in three bfloat16 parts, for the product with the keys' mn
+  float fac[NC][CP];
+  int limit[NC][CP];                                        // the positions of this thread's columns
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
+    const int qc = SIDE ? g >> 1 : 8 * n + g;               // the operand's column g: a column's hi or lo, or both in turn
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const uint4 v = *reinterpret_cast<const uint4*>(&s_q[8 * n + g][i * 16 + 4 * t]);
-      qf[n][i][0] = v.x; qf[n][i][1] = v.y; qf[n][i][2] = v.z; qf[n][i][3] = v.w;
-    }
+    for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = 8 * n + 2 * t + h;
+      for (int i = 0; i < NG; ++i) {
+        const uint2 v = *reinterpret_cast<const uint2*>(&s_q[SIDE ? g & 1 : part][qc][i * 32 + 8 * t]);
+        qf[n][part][i][0] = v.x; qf[n][part][i][1] = v.y;
+      }
+    const float v = t < NG && !(SIDE && (g & 1)) ? s_qsum[qc][t] : 0.0f;
+    const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+    const float rest = v - __bfloat162float(hi);
+    const __nv_bfloat16 mid = __float2bfloat16_rn(rest), lo = __float2bfloat16_rn(rest - __bfloat162float(mid));
+    qsum[n][0] = (uint32_t)__bfloat16_as_ushort(mid) << 16 | __bfloat16_as_ushort(hi);
+    qsum[n][1] = __bfloat16_as_ushort(lo);
 #pragma unroll
-      for (int i = 0; i < NG; ++i) qs[n][i][h] = s_qsum[c][i];
+    for (int h = 0; h < CP; ++h) {
+      const int c = SIDE ? t : 8 * n + 2 * t + h;
       fac[n][h] = s_f[c];
       limit[n][h] = c < r.cols ? r.pos0 + (r.col0 + c) / r.G : -1;
     }
@@ -221,25 +247,29 @@ kv4_attn_kernel(const A4Args a) {
   const int full_hi = r.pos0 + r.col0 / r.G;
   const int full_lo = a.window > 0 ? r.pos0 + (r.col0 + r.cols - 1) / r.G - a.window + 1 : 0;
 
-  float o[NC][NG][2][4] = {};                               // [column block][group][features 4 g + 2 k (+ 1)] x columns 2 t, 2 t + 1, in units of 2^-24 F
-  float om[NC][NG][2] = {};                                 // sum p mn, this lane's tokens
-  float m[NC][2], l[NC][2] = {};
+  float o[NC][NG][2][4] = {};                               // [column block][group][features 4 g + 2 k (+ 1)] x columns 2 t, 2 t + 1, in units of 2^-24
+  float om[NC][NG][CP] = {};                                // sum p mn, this lane's tokens
+  float m[NC][CP], ref[NC][CP], l[NC][CP] = {};
 #pragma unroll
-  for (int n = 0; n < NC; ++n) m[n][0] = m[n][1] = __int_as_float(0xff800000);
+  for (int n = 0; n < NC; ++n)
+#pragma unroll
+    for (int h = 0; h < CP; ++h) m[n][h] = ref[n][h] = __int_as_float(0xff800000);
   uint32_t sc_top = 0;                                      // the largest value scale met, rounded up to a power of two (as its exponent bits)
-  float F = 1.0f;
+  float up = 0.0f;                                          // log2 F
 
   auto walk = [&](const unsigned char* buf, int key0, auto masked_t) {
     constexpr bool MASKED = decltype(masked_t)::value;
-    float x[NT][NC][4];
+    float x[NT][NC][2][CP];                                 // keys g and g + 8 of 16, this thread's columns
 #pragma unroll
     for (int mt = 0; mt < NT; ++mt) {
-      uint32_t kw[2][NG], pw[2][NG];
+      uint32_t kw[2][NG], pw[2][NG], mn[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int tok = mt * 16 + g + 8 * h;
         const unsigned char* kp = buf + tok * (HD / 2) + t * (NG * 4);
         const unsigned char* pp = buf + K_WORDS + tok * (NG * 4);
+        const uint32_t own = *reinterpret_cast<const uint32_t*>(pp + (t % NG) * 4);
+        mn[h] = __byte_perm(own, own, 0x1010);              // group t's mn twice
         if constexpr (NG == 2) {
           const uint2 u = *reinterpret_cast<const uint2*>(kp), v = *reinterpret_cast<const uint2*>(pp);
           kw[h][0] = u.x; kw[h][1] = u.y; pw[h][0] = v.x; pw[h][1] = v.y;
@@ -249,51 +279,51 @@ kv4_attn_kernel(const A4Args a) {
           pw[h][0] = v.x; pw[h][1] = v.y; pw[h][2] = v.z; pw[h][3] = v.w;
         }
       }
+      float y[NC][4] = {};
 #pragma unroll
-      for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[mt][n][e] = 0.0f;
+      for (int n = 0; n < NC; ++n) a4_mma_bf16(y[n], mn[0], mn[1], mn[0], mn[1], qsum[n][0], qsum[n][1]);      // sum_g mn_g Q_g
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        const uint32_t u0 = kw[0][i], u1 = kw[1][i], s0 = u0 >> 8, s1 = u1 >> 8;
+        const uint32_t a0 = kw[0][i] & 0x0f0f0f0fu, a1 = kw[1][i] & 0x0f0f0f0fu, a2 = (kw[0][i] >> 4) & 0x0f0f0f0fu, a3 = (kw[1][i] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
           float c[4] = {};
-          a4_mma(c, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[n][i][0], qf[n][i][1]);
-          a4_mma(c, s0 & 0x000f000fu, s1 & 0x000f000fu, s0 & 0x00f000f0u, s1 & 0x00f000f0u, qf[n][i][2], qf[n][i][3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[mt][n][e] = fmaf(word_sc(pw[e >> 1][i]), c[e], fmaf(word_mn(pw[e >> 1][i]), qs[n][i][e & 1], x[mt][n][e]));
+          for (int part = 0; part < PARTS; ++part) a4_mma8(c, a0, a1, a2, a3, qf[n][part][i][0], qf[n][part][i][1]);
+          if constexpr (SIDE) {
+            y[n][0] = fmaf(word_sc(pw[0][i]), c[0] + c[1], y[n][0]);
+            y[n][2] = fmaf(word_sc(pw[1][i]), c[2] + c[3], y[n][2]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[n][e] = fmaf(word_sc(pw[e >> 1][i]), c[e], y[n][e]);
+          }
         }
       }
 #pragma unroll
       for (int n = 0; n < NC; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[mt][n][e] *= fac[n][e & 1];
-          if (MASKED) {
-            const int key = key0 + mt * 16 + g + 8 * (e >> 1), lim = limit[n][e & 1];
-            if (key > lim || (a.window > 0 && lim - key >= a.window)) x[mt][n][e] = __int_as_float(0xff800000);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < CP; ++c) {
+            x[mt][n][h][c] = y[n][2 * h + c] * fac[n][c];
+            if (MASKED) {
+              const int key = key0 + mt * 16 + g + 8 * h, lim = limit[n][c];
+              if (key > lim || (a.window > 0 && lim - key >= a.window)) x[mt][n][h][c] = __int_as_float(0xff800000);
+            }
           }
-        }
     }
     // the running maximum of a column, over the lanes that share it
-    float alpha[NC][2], mm[NC][2];
-    bool moved = false;
+    float next[NC][CP];
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v = x[0][n][h];
+      for (int h = 0; h < CP; ++h) {
+        float v = x[0][n][0][h];
 #pragma unroll
-        for (int mt = 0; mt < NT; ++mt) v = fmaxf(v, fmaxf(x[mt][n][h], x[mt][n][h + 2]));
+        for (int mt = 0; mt < NT; ++mt) v = fmaxf(v, fmaxf(x[mt][n][0][h], x[mt][n][1][h]));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-        const float next = fmaxf(m[n][h], v);
-        mm[n][h] = next == __int_as_float(0xff800000) ? 0.0f : next;
-        alpha[n][h] = a4_exp2(m[n][h] - mm[n][h]);
-        moved = moved || next != m[n][h];
-        m[n][h] = next;
+        next[n][h] = fmaxf(m[n][h], v);
       }
     // the values' numbers, and the power of two that keeps the largest scale in fp16's range
     uint32_t vw[NT][2][NG];
@@ -324,55 +354,68 @@ kv4_attn_kernel(const A4Args a) {
           for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i] < 0x7f800000u ? vw[mt][h][i] : 0u);
       top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
     }
-    float keep = 1.0f;
     if (top > sc_top) {                                     // (the same for the whole warp)
-      const float old = F;
       sc_top = top;
-      F = a4_pow2(min(max(13 - ((int)(top >> 23) - 127), -100), 100));
-      keep = F / old;
-      moved = true;
+      up = (float)min(max(13 - ((int)(top >> 23) - 127), -100), 100);
     }
+    // p = 2^(x - ref): ref is the maximum less the exponent that the values' scales want, so p carries F and nothing else has to
+    float mm[NC][CP];
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int h = 0; h < CP; ++h) {
+        m[n][h] = next[n][h];
+        mm[n][h] = next[n][h] - up;                         // (-inf stays)
+        moved = moved || mm[n][h] != ref[n][h];
+      }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int n = 0; n < NC; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float f = alpha[n][h] * keep;
-          l[n][h] *= alpha[n][h];
+        for (int h = 0; h < CP; ++h) {
+          const float f = ref[n][h] == mm[n][h] ? 1.0f : a4_exp2(ref[n][h] - mm[n][h]);
+          ref[n][h] = mm[n][h];
+          l[n][h] *= f;
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
-            om[n][i][h] *= alpha[n][h];
+            om[n][i][h] *= f;
 #pragma unroll
             for (int k = 0; k < 2; ++k) { o[n][i][k][h] *= f; o[n][i][k][h + 2] *= f; }
           }
         }
     }
 #pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int h = 0; h < CP; ++h) mm[n][h] = ref[n][h] == __int_as_float(0xff800000) ? 0.0f : ref[n][h];
+#pragma unroll
     for (int mt = 0; mt < NT; ++mt) {
       uint32_t pb[NC][NG][2];                               // P_g, tokens x columns, transposed
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        float p[4];
+        float p[2][CP];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = a4_exp2(x[mt][n][e] - mm[n][e & 1]);
-          l[n][e & 1] += p[e];
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < CP; ++c) {
+            p[h][c] = a4_exp2(x[mt][n][h][c] - mm[n][c]);
+            l[n][c] += p[h][c];
+          }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          float w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float sc = word_sc(vw[mt][e >> 1][i]) * F, mn = word_mn(vw[mt][e >> 1][i]);
-            if (MASKED && x[mt][n][e] == __int_as_float(0xff800000)) {       // what is hidden may hold anything
-              w[e] = 0.0f;
-            } else {
-              w[e] = p[e] * sc;
-              om[n][i][e & 1] = fmaf(p[e], mn, om[n][i][e & 1]);
+          for (int h = 0; h < 2; ++h) {
+            const float sc = word_sc(vw[mt][h][i]), mn = word_mn(vw[mt][h][i]);
+            float w[2] = {};                                // (side by side: the odd columns stay empty)
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+              if (MASKED && x[mt][n][h][c] == __int_as_float(0xff800000)) continue;       // what is hidden may hold anything
+              w[c] = p[h][c] * sc;
+              om[n][i][c] = fmaf(p[h][c], mn, om[n][i][c]);
             }
+            pb[n][i][h] = a4_transpose(a4_pack(w[0], w[1]));
           }
-          pb[n][i][0] = a4_transpose(a4_pack(w[0], w[1]));
-          pb[n][i][1] = a4_transpose(a4_pack(w[2], w[3]));
         }
       }
 #pragma unroll
@@ -418,16 +461,16 @@ kv4_attn_kernel(const A4Args a) {
 
   // this warp's sums over its lanes, then its results [column][feature] in the ring's place
   float* mine = reinterpret_cast<float*>(ring);
-  const float unit = 0x1p24f / F;
+  const float unit = 0x1p24f;
 #pragma unroll
   for (int n = 0; n < NC; ++n)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = 8 * n + 2 * t + h;
+    for (int h = 0; h < CP; ++h) {
+      const int c = SIDE ? t : 8 * n + 2 * t + h;
       float v = l[n][h];
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-      if (g == 0) { s_m[warp][c] = m[n][h]; s_l[warp][c] = v; }
+      if (g == 0) { s_m[warp][c] = ref[n][h]; s_l[warp][c] = v; }
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         float s = om[n][i][h];
@@ -476,7 +519,7 @@ kv4_attn_kernel(const A4Args a) {
 }
 
 // Joins the chunks of a (row, key/value head, column): a block each, its warps over the chunks, then the warps' sums.
-constexpr int A4_JOIN_WARPS = 8;
+constexpr int A4_JOIN_WARPS = 16;
 template <int HD>
 __global__ void __launch_bounds__(A4_JOIN_WARPS * 32)
 kv4_join_kernel(const A4Args a, int columns) {
@@ -536,6 +579,8 @@ kv4_join_kernel(const A4Args a, int columns) {
 
 constexpr uint32_t A4_SMEM = A4_WARPS * A4_STAGES * TILE;
 
+static int a4_columns(int wanted) { return wanted <= 4 ? 4 : wanted <= 8 ? 8 : 16; }
+
 }  // namespace exl3
 
 using namespace exl3;
@@ -550,7 +595,7 @@ extern "C" int exl3_kv4_attn_status() {
 // Floats of scratch that a call with these sizes wants (0 with one chunk).
 extern "C" long long exl3_kv4_attn_scratch(int rows, int max_new, int nh, int nkv, int hd, int max_chunks) {
   if (max_chunks <= 1 || nkv < 1) return 0;
-  const int ncol = max_new * (nh / nkv), columns = ncol <= 8 ? 8 : 16;
+  const int ncol = max_new * (nh / nkv), columns = a4_columns(ncol);
   return (long long)rows * nkv * ceil_div(ncol, columns) * max_chunks * columns * (hd + 4);
 }
 
@@ -570,7 +615,7 @@ extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const v
     set_error("kv4_attn: %lld floats of scratch wanted", exl3_kv4_attn_scratch(rows, max_new, nh, nkv, hd, max_chunks));
     return ERR_SCRATCH;
   }
-  const int ncol = max_new * (nh / nkv), columns = ncol <= 8 ? 8 : 16;
+  const int ncol = max_new * (nh / nkv), columns = a4_columns(ncol);
   A4Args a = {};
   a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.out = static_cast<__nv_bfloat16*>(out);
   a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.block_table = block_table; a.bt_stride = bt_stride;
@@ -580,15 +625,16 @@ extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const v
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaSuccess;
-    for (const void* f : {(const void*)kv4_attn_kernel<64, 1>, (const void*)kv4_attn_kernel<64, 2>, (const void*)kv4_attn_kernel<128, 1>, (const void*)kv4_attn_kernel<128, 2>})
+    for (const void* f : {(const void*)kv4_attn_kernel<64, 4>, (const void*)kv4_attn_kernel<64, 8>, (const void*)kv4_attn_kernel<64, 16>,
+                          (const void*)kv4_attn_kernel<128, 4>, (const void*)kv4_attn_kernel<128, 8>, (const void*)kv4_attn_kernel<128, 16>})
       if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)A4_SMEM);
     if (e != cudaSuccess) { set_error("kv4_attn: cannot get %u bytes of shared memory: %s", A4_SMEM, cudaGetErrorString(e)); return (int)e; }
     configured = true;
   }
   const dim3 grid(max_chunks, nkv * a.n_ct, rows), block(A4_WARPS * 32);
   auto go = [&](auto kernel) { launch_pdl(kernel, grid, block, A4_SMEM, stream, a); };
-  if (hd == 64) { if (columns == 8) go(kv4_attn_kernel<64, 1>); else go(kv4_attn_kernel<64, 2>); }
-  else { if (columns == 8) go(kv4_attn_kernel<128, 1>); else go(kv4_attn_kernel<128, 2>); }
+  if (hd == 64) { if (columns == 4) go(kv4_attn_kernel<64, 4>); else if (columns == 8) go(kv4_attn_kernel<64, 8>); else go(kv4_attn_kernel<64, 16>); }
+  else { if (columns == 4) go(kv4_attn_kernel<128, 4>); else if (columns == 8) go(kv4_attn_kernel<128, 8>); else go(kv4_attn_kernel<128, 16>); }
   int rc = launch_status("kv4_attn");
   if (rc || max_chunks == 1) return rc;
   const dim3 jgrid(columns < ncol ? columns : ncol, nkv * a.n_ct, rows), jblock(A4_JOIN_WARPS * 32);

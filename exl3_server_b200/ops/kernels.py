@@ -1947,8 +1947,8 @@ def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: i
     tiles, at 0.23 us each while it is alone and at 0.11 us (0.17 us with 16 columns) times the blocks that share its SM when these are more;
     joining chunks takes 3 us."""
     tiles = max(1, -(-span * head_dim // 4096))
-    per_sm = 4 if columns == 8 else 2
-    each = 0.11 if columns == 8 else 0.17
+    per_sm = 2 if columns == 16 else 3 if columns == 8 and head_dim == 128 else 4
+    each = 0.11 if columns <= 8 else 0.17
     items = rows * kv_heads * groups
     best = None
     for n in range(1, min(tiles, 1024) + 1):
@@ -2003,7 +2003,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     if tiles is not None and columns_wanted > KV4_FEW_COLUMNS:
         return _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window,
                                 workspace, out)
-    columns = 8 if columns_wanted <= 8 else 16
+    columns = 4 if columns_wanted <= 4 else 8 if columns_wanted <= 8 else 16
     groups = -(-columns_wanted // columns)
     span = min(max_len, window + max_new - 1) if window > 0 else max_len
     chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, sm_count(q.device))
