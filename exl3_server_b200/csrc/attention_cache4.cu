@@ -38,20 +38,21 @@ using namespace kv4;
 constexpr int A4_WARPS = 4;
 constexpr int A4_STAGES = 2;
 constexpr int A4_MAX_CHUNK = 32 * A4_WARPS;               // tiles: a warp keeps its page numbers one a lane
-constexpr uint32_t A4_WAIT_LIMIT = 1u << 22;              // polls of some tens of cycles: a fraction of a second
+constexpr uint32_t A4_WAIT_LIMIT = 1u << 20;              // looks of up to a microsecond each: a second
 
 static __device__ int g_a4_error = 0;
 
 __device__ inline uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// Suspends the warp for up to a microsecond at a time: a warp that polls takes issue slots from those that compute.
 __device__ inline bool a4_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = a4_smem(bar);
   for (uint32_t i = 0; i < A4_WAIT_LIMIT; ++i) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+        : "=r"(ok) : "r"(addr), "r"(parity), "r"(1000u) : "memory");
     if (ok) return true;
   }
   return false;
@@ -66,9 +67,14 @@ __device__ inline void a4_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ inline void a4_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// The same onto zeros (which take no registers), and bfloat16 onto zeros.
+__device__ inline void a4_mma8_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ inline void a4_mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ inline uint32_t a4_transpose(uint32_t x) {
   uint32_t y;
@@ -279,17 +285,17 @@ kv4_attn_kernel(const A4Args a) {
           pw[h][0] = v.x; pw[h][1] = v.y; pw[h][2] = v.z; pw[h][3] = v.w;
         }
       }
-      float y[NC][4] = {};
+      float y[NC][4];
 #pragma unroll
-      for (int n = 0; n < NC; ++n) a4_mma_bf16(y[n], mn[0], mn[1], mn[0], mn[1], qsum[n][0], qsum[n][1]);      // sum_g mn_g Q_g
+      for (int n = 0; n < NC; ++n) a4_mma_bf16_first(y[n], mn[0], mn[1], mn[0], mn[1], qsum[n][0], qsum[n][1]);      // sum_g mn_g Q_g
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         const uint32_t a0 = kw[0][i] & 0x0f0f0f0fu, a1 = kw[1][i] & 0x0f0f0f0fu, a2 = (kw[0][i] >> 4) & 0x0f0f0f0fu, a3 = (kw[1][i] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-          float c[4] = {};
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) a4_mma8(c, a0, a1, a2, a3, qf[n][part][i][0], qf[n][part][i][1]);
+          float c[4];
+          a4_mma8_first(c, a0, a1, a2, a3, qf[n][0][i][0], qf[n][0][i][1]);
+          if constexpr (!SIDE) a4_mma8(c, a0, a1, a2, a3, qf[n][1][i][0], qf[n][1][i][1]);
           if constexpr (SIDE) {
             y[n][0] = fmaf(word_sc(pw[0][i]), c[0] + c[1], y[n][0]);
             y[n][2] = fmaf(word_sc(pw[1][i]), c[2] + c[3], y[n][2]);

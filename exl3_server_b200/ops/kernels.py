@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from typing import Optional
 
 import torch
@@ -1943,12 +1944,12 @@ KV4_FEW_COLUMNS = 64        # new tokens times query heads per key/value head up
 
 @functools.lru_cache(maxsize=4096)
 def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: int, span: int, window: int, sms: int):
-    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys, by a small model of the kernel's time: a block takes 3 us and its
-    tiles, at 0.23 us each while it is alone and at 0.11 us (0.17 us with 16 columns) times the blocks that share its SM when these are more;
-    joining chunks takes 3 us."""
+    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys, by a small model of the kernel's time: a block takes 3 us and for
+    each of its tiles 0.15 us and 0.14 us times the blocks that share its SM (a third more with 8 columns, as much again with 16); rows of a batch are
+    taken to be unequal, seven tenths of the longest in the mean; joining chunks takes 3 us."""
     tiles = max(1, -(-span * head_dim // 4096))
     per_sm = 2 if columns == 16 else 3 if columns == 8 and head_dim == 128 else 4
-    each = 0.11 if columns <= 8 else 0.17
+    wide = {4: 1.0, 8: 1.33, 16: 2.0}[columns]
     items = rows * kv_heads * groups
     best = None
     for n in range(1, min(tiles, 1024) + 1):
@@ -1956,10 +1957,10 @@ def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: i
         if chunk > 128 or (n > 1 and chunk < 4):
             continue
         n = -(-tiles // chunk)
-        blocks = items * n
-        waves = -(-blocks // (per_sm * sms))
-        here = min(per_sm, -(-blocks // sms))
-        cost = waves * (3.0 + chunk * max(0.23, each * here)) + (3.0 if n > 1 else 0.0)
+        blocks = items * n if rows == 1 else items * (0.7 * n + 0.3)
+        waves = math.ceil(blocks / (per_sm * sms))
+        here = min(per_sm, math.ceil(blocks / sms))
+        cost = waves * (3.0 + chunk * wide * (0.15 + 0.14 * here)) + (3.0 if n > 1 else 0.0)
         if best is None or cost < best[0] - 1e-9:
             best = (cost, chunk, n)
     _, chunk, n = best
