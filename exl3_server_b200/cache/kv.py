@@ -33,7 +33,7 @@ PAGE_SIZE = 64
 @dataclass
 class KVLayerView:
     """What a mixer sees of the cache during one step."""
-    k: torch.Tensor               # [pages, kv_heads, page_size, head_dim] of this layer
+    k: torch.Tensor               # [pages, kv_heads, page_size, head_dim] of this layer; 4-bit: uint8 [pages, kv_heads, bytes], keys and values
     v: torch.Tensor               # [pages, kv_heads, page_size, value_dim or head_dim]
     block_table: torch.Tensor     # int32 [batch rows, pages per row] for this step; -1: no page
     page_size: int
@@ -55,6 +55,14 @@ class KVGroup:
     def allocate(self, dtype: torch.dtype, device) -> None:
         r = self.request
         # one page more than the pool hands out: rows that only pad a batch write there
+        if r.codes:
+            from ..ops import kernels as K
+            if self.page_size != K.KV4_PAGE:
+                raise CacheError(f"the 4-bit cache has pages of {K.KV4_PAGE}, not {self.page_size}")
+            self.k, self._k_store = self._guarded((len(self.owners), self.pool.n_pages + 1, r.kv_heads, K.kv4_page_bytes(r.head_dim)),
+                                                  torch.uint8, device)
+            self.v = self.k
+            return
         shape = (len(self.owners), self.pool.n_pages + 1, r.kv_heads, self.page_size)
         self.k, self._k_store = self._guarded(shape + (r.head_dim,), dtype, device)
         if r.values_in_keys:
@@ -74,21 +82,27 @@ class KVGroup:
         for d in shape:
             n *= d
         store = torch.zeros(n + 2 * cls.GUARD, dtype=dtype, device=device)
-        store[:cls.GUARD] = cls.PATTERN
-        store[-cls.GUARD:] = cls.PATTERN
+        store[:cls.GUARD] = cls._pattern(dtype)
+        store[-cls.GUARD:] = cls._pattern(dtype)
         return store[cls.GUARD:cls.GUARD + n].view(shape), store
+
+    @classmethod
+    def _pattern(cls, dtype: torch.dtype):
+        return cls.PATTERN if dtype.is_floating_point else 0xA5
 
     def guards_intact(self) -> bool:
         for store in (self._k_store, self._v_store):
             if store is None:
                 continue
             edge = torch.cat([store[:self.GUARD], store[-self.GUARD:]])
-            if not bool((edge == self.PATTERN).all()):
+            if not bool((edge == self._pattern(store.dtype)).all()):
                 return False
         return True
 
     def bytes_per_token(self, itemsize: int) -> int:
         r = self.request
+        if r.codes:
+            return len(self.owners) * r.kv_heads * r.head_dim * 5 // 4       # half a byte a feature and four bytes a group of 32, twice
         per_head = r.head_dim if r.values_in_keys else r.head_dim + (r.value_dim or r.head_dim)
         return len(self.owners) * r.kv_heads * per_head * itemsize
 
@@ -138,9 +152,9 @@ class SequenceCache:
                     raise CacheError(f"schedule entry {i} reads the cache of entry {src}, which owns none")
                 if kv is not None:
                     src_req = self.groups[self.entry_group[src][0]].request
-                    if (kv.kv_heads, kv.head_dim, kv.value_dim or kv.head_dim, kv.values_in_keys) != (
+                    if (kv.kv_heads, kv.head_dim, kv.value_dim or kv.head_dim, kv.values_in_keys, kv.codes) != (
                             src_req.kv_heads, src_req.head_dim, src_req.value_dim or src_req.head_dim,
-                            src_req.values_in_keys):
+                            src_req.values_in_keys, src_req.codes):
                         raise CacheError(f"schedule entry {i} cannot read entry {src}'s cache: head shapes differ")
                     # the owner gives back the pages its own window no longer reaches: a reader that looks
                     # further back would find them gone (the kernels skip pages that are not there)

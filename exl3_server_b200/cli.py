@@ -54,6 +54,9 @@ def build_parser() -> argparse.ArgumentParser:
     o = ap.add_argument_group("other")
     o.add_argument("--batch", type=int, default=64, metavar="N", help="most prompts that run as one batch (default 64)")
     o.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16", help="(default bfloat16)")
+    o.add_argument("--weight-type", choices=["fp8"], default=None,
+                   help="keep the layers' matrices in 8-bit floating point (default: as --dtype)")
+    o.add_argument("--cache-type", choices=["int4"], default=None, help="keep keys and values in 4 bits (default: as --dtype)")
     o.add_argument("--cache-tokens", type=int, default=0, metavar="N",
                    help="tokens the cache holds (default: enough for one batch)")
     o.add_argument("--device", default="cuda:0")
@@ -82,7 +85,7 @@ def main(argv=None) -> int:
     need = sum((len(p) + args.max_tokens + 63) // 64 * 64 for p in prompts[:max(1, args.batch)])
     try:
         engine = Engine.from_folder(args.model, dtype=args.dtype, max_tokens=args.cache_tokens or need,
-                                    device=args.device)
+                                    device=args.device, weight_type=args.weight_type, cache_type=args.cache_type)
     except Exception as e:                            # config, weights or kernel library
         print(f"exl3-server-b200: {e}", file=sys.stderr)
         return 1

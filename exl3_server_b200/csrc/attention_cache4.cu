@@ -188,35 +188,48 @@ kv4_attn_kernel(const A4Args a) {
   for (int s = 0; s < A4_STAGES; ++s)
     if (ask) request(s);
 
-  // the queries: a warp takes every fourth column
+  // the queries: a warp takes every fourth column, a lane HD / 32 neighbouring features of it
+#pragma unroll
   for (int c = warp; c < COLS; c += A4_WARPS) {
     const int col = r.col0 + c;
     const bool there = c < r.cols;                          // columns that are not there are zeros, computed and dropped
     const __nv_bfloat16* src = a.q + (int64_t)(r.start + (there ? col / r.G : 0)) * a.q_stride + (int64_t)(kvh * r.G + (there ? col % r.G : 0)) * HD;
     float x[NG];
+    if constexpr (NG == 2) {
+      const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(src) + lane);
+      x[0] = __uint_as_float(w << 16); x[1] = __uint_as_float(w & 0xffff0000u);
+    } else {
+      const uint2 w = __ldcg(reinterpret_cast<const uint2*>(src) + lane);
+      x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u);
+      x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
+    }
     float top = 0.0f;
     bool finite = true;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      x[i] = there ? __bfloat162float(src[i * 32 + lane]) : 0.0f;
+      if (!there) x[i] = 0.0f;
       top = fmaxf(top, fabsf(x[i]));
       finite = finite && fabsf(x[i]) < __int_as_float(0x7f800000);
     }
-    top = warp_max(top);
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     finite = __all_sync(0xffffffffu, finite);
     const int e = finite && top > 0.0f ? min(max(7 + 127 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
     const float up = a4_pow2(e);
-    const int place = (lane & 24) + ((lane >> 1) & 1) * 4 + (lane & 1) * 2 + ((lane >> 2) & 1);
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
+      const int f = lane * NG + i;                          // the feature, and its byte among the operand's eight
+      const int place = (f & ~7) + ((f >> 1) & 1) * 4 + (f & 1) * 2 + ((f >> 2) & 1);
       const float v = x[i] * up;
       const __nv_fp8_e4m3 hi(v);
       const __nv_fp8_e4m3 lo(v - (float)hi);
-      const float sum = warp_sum((float)hi + (float)lo);
-      if (lane == 0) s_qsum[c][i] = sum * 0x1p-9f;
-      s_q[0][c][i * 32 + place] = hi.__x;
-      s_q[1][c][i * 32 + place] = lo.__x;
+      sum += (float)hi + (float)lo;
+      s_q[0][c][place] = hi.__x;
+      s_q[1][c][place] = lo.__x;
     }
+#pragma unroll
+    for (int off = 1; off < 32 / NG; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane % (32 / NG) == 0) s_qsum[c][lane / (32 / NG)] = sum * 0x1p-9f;
     if (lane == 0) s_f[c] = finite ? a.scale_log2 * a4_pow2(9 - e) : __int_as_float(0x7fc00000);      // (a row that is not finite: NaN)
   }
   __syncthreads();
@@ -525,8 +538,8 @@ kv4_attn_kernel(const A4Args a) {
 }
 
 // Joins the chunks of a (row, key/value head, column): a block each, its warps over the chunks, then the warps' sums.
-constexpr int A4_JOIN_WARPS = 16;
-template <int HD>
+// As many warps as leave each four chunks, up to 16: all of a warp's records are on their way at once.
+template <int HD, int A4_JOIN_WARPS>
 __global__ void __launch_bounds__(A4_JOIN_WARPS * 32)
 kv4_join_kernel(const A4Args a, int columns) {
   constexpr int V = HD / 32;                                // features a lane
@@ -566,7 +579,7 @@ kv4_join_kernel(const A4Args a, int columns) {
   for (int i = 0; i < V; ++i) s_acc[warp][i * 32 + lane] = acc[i];
   if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
   __syncthreads();
-  if (threadIdx.x < HD) {
+  for (int d = threadIdx.x; d < HD; d += A4_JOIN_WARPS * 32) {
     float top = s_m[0];
 #pragma unroll
     for (int w = 1; w < A4_JOIN_WARPS; ++w) top = fmaxf(top, s_m[w]);
@@ -576,10 +589,10 @@ kv4_join_kernel(const A4Args a, int columns) {
     for (int w = 0; w < A4_JOIN_WARPS; ++w) {
       const float f = a4_exp2(s_m[w] - safe);
       sum = fmaf(s_l[w], f, sum);
-      y = fmaf(s_acc[w][threadIdx.x], f, y);
+      y = fmaf(s_acc[w][d], f, y);
     }
     const int col = r.col0 + c;
-    a.out[((int64_t)(r.start + col / r.G) * a.nh + kvh * r.G + col % r.G) * HD + threadIdx.x] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : y / sum);
+    a.out[((int64_t)(r.start + col / r.G) * a.nh + kvh * r.G + col % r.G) * HD + d] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : y / sum);
   }
 }
 
@@ -643,8 +656,10 @@ extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const v
   else { if (columns == 4) go(kv4_attn_kernel<128, 4>); else if (columns == 8) go(kv4_attn_kernel<128, 8>); else go(kv4_attn_kernel<128, 16>); }
   int rc = launch_status("kv4_attn");
   if (rc || max_chunks == 1) return rc;
-  const dim3 jgrid(columns < ncol ? columns : ncol, nkv * a.n_ct, rows), jblock(A4_JOIN_WARPS * 32);
-  if (hd == 64) launch_pdl(kv4_join_kernel<64>, jgrid, jblock, 0, stream, a, columns);
-  else launch_pdl(kv4_join_kernel<128>, jgrid, jblock, 0, stream, a, columns);
+  const dim3 jgrid(columns < ncol ? columns : ncol, nkv * a.n_ct, rows);
+  auto join = [&](auto kernel, int warps) { launch_pdl(kernel, jgrid, dim3(warps * 32), 0, stream, a, columns); };
+  if (max_chunks <= 8) { if (hd == 64) join(kv4_join_kernel<64, 2>, 2); else join(kv4_join_kernel<128, 2>, 2); }
+  else if (max_chunks <= 24) { if (hd == 64) join(kv4_join_kernel<64, 6>, 6); else join(kv4_join_kernel<128, 6>, 6); }
+  else { if (hd == 64) join(kv4_join_kernel<64, 16>, 16); else join(kv4_join_kernel<128, 16>, 16); }
   return launch_status("kv4_attn join");
 }

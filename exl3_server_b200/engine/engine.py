@@ -76,17 +76,19 @@ def resolve_dtype(dtype: Union[str, torch.dtype]) -> torch.dtype:
         raise ValueError(f"dtype must be one of {sorted(DTYPES)}, got {dtype!r}") from None
 
 
-def load_model(model_dir: str, dtype: Union[str, torch.dtype] = "bfloat16", device="cuda:0") -> Model:
+def load_model(model_dir: str, dtype: Union[str, torch.dtype] = "bfloat16", device="cuda:0", weight_type: Optional[str] = None,
+               cache_type: Optional[str] = None) -> Model:
     """Reads config.json, finds the architecture in the registry, checks the
-    checkpoint against the plan's tensor list and builds the model."""
+    checkpoint against the plan's tensor list and builds the model.  ``weight_type`` and ``cache_type``: see ``Model``."""
     from .. import models  # noqa: F401  (registers the architectures)
     dt = resolve_dtype(dtype)
     obj = read_config_json(model_dir)
     arch = resolve_architecture(obj)
     cfg = arch.config_class.from_dict(obj)
     plan = arch.build_plan(cfg)
+    Model._check_types(plan, dt, weight_type, cache_type)      # before the checkpoint is read
     tensors = load_tensors(model_dir, plan_manifest(plan), dt, device, ignorable=plan.ignorable)
-    model = Model(plan, tensors, dt, device)
+    model = Model(plan, tensors, dt, device, weight_type=weight_type, cache_type=cache_type)
     model.config = cfg
     return model
 
@@ -108,7 +110,7 @@ class Engine:
         self.stats = Stats()
         self.last_generate_stats: Optional[Stats] = None
         itemsize = 4 if model.dtype == torch.float32 else 2
-        self._body_params = (model.weight_bytes() - model.head.read_bytes()) // itemsize
+        self._body_params = model.body_params()
         self._head_params = model.head.read_bytes() // itemsize
         self._cache_bytes_per_token = sum(g.bytes_per_token(itemsize) for g in self.cache.groups)
         self._score_flops_per_key = sum(4.0 * m.spec.heads * m.spec.head_dim
@@ -132,8 +134,10 @@ class Engine:
 
     @classmethod
     def from_folder(cls, model_dir: str, dtype="bfloat16", max_tokens: int = 4096, device="cuda:0",
-                    max_slots: Optional[int] = None) -> "Engine":
-        return cls(load_model(model_dir, dtype, device), max_tokens, max_slots)
+                    max_slots: Optional[int] = None, weight_type: Optional[str] = None, cache_type: Optional[str] = None) -> "Engine":
+        """``weight_type`` "fp8": the layers' matrices in 8-bit floating point with scales for blocks of 128 (rounded here, from the
+        checkpoint's).  ``cache_type`` "int4": keys and values in 4 bits.  Both for the Llama-family decoder in bfloat16."""
+        return cls(load_model(model_dir, dtype, device, weight_type, cache_type), max_tokens, max_slots)
 
     @property
     def stop_token_ids(self) -> List[int]:

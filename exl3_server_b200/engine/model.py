@@ -15,6 +15,7 @@ import torch
 from ..cache.kv import SequenceCache
 from ..ops import kernels as K
 from ..parts.base import BuildContext, KVRequest, StateRequest
+from ..parts.linear import LinearFP8
 from ..parts.registry import (arrangement_class, embedding_class, feed_forward_class, head_class, mixer_class,
                               norm_class)
 from ..parts.spec import ModelPlan
@@ -64,12 +65,17 @@ def enter(stream, entry, block) -> None:
 
 
 class Model:
-    def __init__(self, plan: ModelPlan, tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device):
+    def __init__(self, plan: ModelPlan, tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device,
+                 weight_type: Optional[str] = None, cache_type: Optional[str] = None):
+        """``weight_type`` "fp8" and ``cache_type`` "int4" keep the layers' matrices and the keys and values in fewer bits than ``dtype`` (which is
+        then bfloat16); embeddings, norms and the head stay as they are."""
         plan.validate()
         self.plan = plan
         self.dtype = dtype
         self.device = torch.device(device)
-        ctx = BuildContext(dtype=dtype, device=self.device)
+        self.weight_type, self.cache_type = weight_type, cache_type
+        self._check_types(plan, dtype, weight_type, cache_type)
+        ctx = BuildContext(dtype=dtype, device=self.device, weight_type=weight_type, cache_type=cache_type)
         self.embedding = embedding_class(plan.embedding.kind)(plan.embedding, tensors, ctx)
         self.blocks = []
         for layer in plan.layers:
@@ -102,6 +108,35 @@ class Model:
         if plan.entry_vectors is not None:
             self.entry_vectors = tensors[plan.entry_vectors[0]].float().contiguous()
         self._adds_embedding = any(e.add_embedding for e in plan.schedule)
+
+    @staticmethod
+    def _check_types(plan: ModelPlan, dtype: torch.dtype, weight_type: Optional[str], cache_type: Optional[str]) -> None:
+        """Refuses types of weights and caches that the plan's parts do not keep, before anything is built."""
+        if weight_type not in (None, "fp8") or cache_type not in (None, "int4"):
+            raise ValueError(f"weight_type is None or 'fp8' and cache_type None or 'int4', got {weight_type!r} and {cache_type!r}")
+        if (weight_type or cache_type) and dtype != torch.bfloat16:
+            raise ValueError("weights in 8 bits and caches in 4 go with bfloat16 activations")
+        for i, layer in enumerate(plan.layers):
+            for kind, part in ((layer.mixer.kind, mixer_class(layer.mixer.kind)),
+                               (layer.feed_forward.kind, feed_forward_class(layer.feed_forward.kind)) if layer.feed_forward is not None else (None, None)):
+                if part is not None and weight_type is not None and weight_type not in getattr(part, "weight_types", ()):
+                    raise ValueError(f"layer {i}: {kind!r} does not keep its weights as {weight_type!r}")
+            if cache_type is not None and cache_type not in getattr(mixer_class(layer.mixer.kind), "cache_types", ()):
+                raise ValueError(f"layer {i}: {layer.mixer.kind!r} does not keep its cache as {cache_type!r}")
+        if cache_type is not None and any(e.cache_from is not None for e in plan.schedule):
+            raise ValueError(f"layers that read other layers' keys and values do not take a cache kept as {cache_type!r}")
+
+    def body_params(self) -> int:
+        """Parameters that a step's layers use, whatever bytes they are kept in."""
+        itemsize = 4 if self.dtype == torch.float32 else 2
+        n = (self.weight_bytes() - self.head.read_bytes()) // itemsize
+        if self.weight_type is not None:
+            for e in self.plan.schedule:
+                for part in (self.blocks[e.layer].mixer, self.blocks[e.layer].feed_forward):
+                    for lin in vars(part).values() if part is not None else ():
+                        if isinstance(lin, LinearFP8):
+                            n += lin.weight.numel() - (lin.weight.numel() + 4 * lin.scales.numel()) // itemsize
+        return n
 
     def cache_requests(self) -> List[Tuple[Optional[KVRequest], Optional[StateRequest], Optional[int]]]:
         out = []

@@ -1944,23 +1944,24 @@ KV4_FEW_COLUMNS = 64        # new tokens times query heads per key/value head up
 
 @functools.lru_cache(maxsize=4096)
 def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: int, span: int, window: int, sms: int):
-    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys, by a small model of the kernel's time: a block takes 3 us and for
-    each of its tiles 0.15 us and 0.14 us times the blocks that share its SM (a third more with 8 columns, as much again with 16); rows of a batch are
-    taken to be unequal, seven tenths of the longest in the mean; joining chunks takes 3 us."""
+    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys, by a small model of the kernel's time with constants fitted to 104
+    shapes (what it picks is 5 % slower in the mean than the best of a shape): a wave of blocks takes 10 us and for each of a block's tiles 0.13 us and
+    0.21 us times the blocks that share its SM (a fifth less for heads of 128, a fifth more with 16 columns); rows of a batch are taken to be
+    unequal; joining chunks takes 4.5 us."""
     tiles = max(1, -(-span * head_dim // 4096))
     per_sm = 2 if columns == 16 else 3 if columns == 8 and head_dim == 128 else 4
-    wide = {4: 1.0, 8: 1.33, 16: 2.0}[columns]
+    wide = (1.2 if columns == 16 else 1.0) * (0.8 if head_dim == 128 else 1.0)
     items = rows * kv_heads * groups
     best = None
     for n in range(1, min(tiles, 1024) + 1):
         chunk = -(-tiles // n)
-        if chunk > 128 or (n > 1 and chunk < 4):
+        if chunk > 128 or (n > 1 and chunk < 2):
             continue
         n = -(-tiles // chunk)
-        blocks = items * n if rows == 1 else items * (0.7 * n + 0.3)
-        waves = math.ceil(blocks / (per_sm * sms))
+        blocks = items * n if rows == 1 else items * (0.83 * n + 0.17)
+        waves = max(1.0, blocks / (per_sm * sms) + (0.5 if blocks > per_sm * sms else 0.0))
         here = min(per_sm, math.ceil(blocks / sms))
-        cost = waves * (3.0 + chunk * wide * (0.15 + 0.14 * here)) + (3.0 if n > 1 else 0.0)
+        cost = waves * (10.0 + chunk * wide * (0.13 + 0.21 * here)) + (4.5 if n > 1 else 0.0)
         if best is None or cost < best[0] - 1e-9:
             best = (cost, chunk, n)
     _, chunk, n = best

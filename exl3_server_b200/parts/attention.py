@@ -17,6 +17,8 @@ bfloat16 with heads of 64 or 128, are one kernel: it rotates the queries and the
 value from the projection's output, adds them to the softmax and writes them to the cache (``_decode_fused``;
 the position part must offer ``fused_rotation``).  Everything else (float32, other head sizes) takes the
 position step and the CUDA-core attention kernel.
+
+With the 4-bit cache (``BuildContext.cache_type``) a step is ``kernels.kv4_store`` and ``kernels.kv4_attn``, for every kind of step.
 """
 from __future__ import annotations
 
@@ -31,7 +33,7 @@ import torch
 from ..ops import kernels as K
 from ..weights.loader import TensorSpec
 from .base import BuildContext, KVRequest, StateRequest
-from .linear import Linear
+from .linear import make_linear
 from .registry import position_class, register_mixer
 from .spec import MixerSpec, PositionSpec
 
@@ -97,14 +99,21 @@ class Attention:
             sizes = (spec.heads * spec.head_dim, spec.kv_heads * spec.head_dim, spec.kv_heads * spec.head_dim)
             b = torch.cat([(x.to(ctx.dtype) if x is not None else torch.zeros(n, dtype=ctx.dtype, device=w.device))
                            for x, n in zip(biases, sizes)])
-        self.qkv = Linear(w, b, ctx.dtype)
-        self.o = Linear(tensors[prefix + "o_proj.weight"], tensors.get(prefix + "o_proj.bias"), ctx.dtype)
+        self.qkv = make_linear(w, b, ctx)
+        self.o = make_linear(tensors[prefix + "o_proj.weight"], tensors.get(prefix + "o_proj.bias"), ctx)
         pos = spec.position or PositionSpec(kind="none", dims=0)
         self.position = position_class(pos.kind)(pos, spec.head_dim, ctx)
         self.scale = spec.softmax_scale if spec.softmax_scale is not None else spec.head_dim ** -0.5
+        if ctx.cache_type == "int4":
+            fused = getattr(self.position, "fused_rotation", None)
+            if spec.head_dim not in (64, 128) or fused is None or fused(spec.head_dim) is None:
+                raise ValueError(f"attention: the 4-bit cache takes heads of 64 or 128 that are rotated as a whole or not at all, got {spec.head_dim}")
+
+    weight_types = ("fp8",)  # the types of weights and of caches that this part keeps beside the model's own
+    cache_types = ("int4",)
 
     def cache_request(self) -> Optional[KVRequest]:
-        return KVRequest(self.spec.kv_heads, self.spec.head_dim, self.spec.window)
+        return KVRequest(self.spec.kv_heads, self.spec.head_dim, self.spec.window, codes=4 if self.ctx.cache_type == "int4" else 0)
 
     def state_request(self) -> Optional[StateRequest]:
         return None
@@ -116,6 +125,8 @@ class Attention:
         s = self.spec
         if kv is None:
             raise RuntimeError("attention needs a cache view")
+        if self.ctx.cache_type == "int4":
+            return self.o(self._attend4(self.qkv(x), batch, kv), then=then)
         qkv = self._prompt_fused(x, batch, kv)
         if qkv is not None:
             # prompts: the projection has rotated the queries and put the rotated keys and the values into the
@@ -130,6 +141,15 @@ class Attention:
             self.position.rotate_and_store(qkv, batch, kv, s.heads, s.kv_heads, s.head_dim)
             self.attend(qkv, out, batch, kv)
         return self.o(out, then=then)
+
+    def _attend4(self, qkv: torch.Tensor, batch, kv) -> torch.Tensor:
+        """The step with the 4-bit cache: every token's key and value go there first, and the attention reads all of them from there, so a
+        prompt's tokens see each other as later tokens will see them, however the prompt is cut into steps."""
+        s = self.spec
+        inv_freq = self.position.fused_rotation(s.head_dim)[0]
+        q = K.kv4_store(qkv, inv_freq, batch.tok_pos, batch.tok_seq, kv.block_table, kv.k, s.heads, s.kv_heads, s.head_dim)
+        return K.kv4_attn(q, kv.k, kv.block_table, batch.row_start, batch.row_pos0, batch.tiles.get(128), batch.max_new, batch.max_kv_len,
+                          s.heads, s.kv_heads, s.head_dim, self.scale, window=s.window, workspace=batch.workspace)
 
     def _prompt_fused(self, x, batch, kv):
         """Prompts in bfloat16 with heads and pages of 64, enough rows for the paired GEMM and an attention kernel

@@ -35,6 +35,10 @@ import torch
 class BuildContext:
     dtype: torch.dtype            # activations and matrix weights: bfloat16 or float32
     device: torch.device
+    # matrix weights kept in fewer bits than ``dtype``: "fp8" (8-bit floating point with scales for blocks of 128), or None
+    weight_type: Optional[str] = None
+    # keys and values kept in fewer bits than ``dtype``: "int4" (the 4-bit cache), or None
+    cache_type: Optional[str] = None
     # what parts of one model keep together (keyed as they like), such as tables that one kernel reads for all of them
     shared: Dict[Any, Any] = field(default_factory=dict, compare=False)
 
@@ -47,7 +51,8 @@ class KVRequest:
     keeps as keys (one latent row per token) gets the key pool as both.  ``chunk`` > 0: a query sees only the keys
     of its own block of ``chunk`` positions (counted from the sequence's start), so the cache gives back the pages
     that lie wholly before the block of the next position.  ``keep_first`` > 0 (with a window): the keys at positions
-    below it stay visible to every later query, so their pages are never given back."""
+    below it stay visible to every later query, so their pages are never given back.  ``codes`` = 4: keys and values are kept in
+    the 4-bit format of ``kernels.kv4_store`` (one pool of bytes for both)."""
     kv_heads: int
     head_dim: int
     window: int = 0
@@ -55,6 +60,7 @@ class KVRequest:
     values_in_keys: bool = False
     chunk: int = 0
     keep_first: int = 0
+    codes: int = 0
 
 
 @dataclass(frozen=True)

@@ -29,7 +29,7 @@ import torch
 from ..ops import kernels as K
 from ..weights.loader import TensorSpec
 from .base import BuildContext
-from .linear import Linear
+from .linear import Linear, make_linear
 from .registry import register_feed_forward
 from .spec import FeedForwardSpec
 
@@ -66,9 +66,10 @@ class SwiGLU:
         else:
             w = torch.cat([wg, wu], dim=0)
             b = torch.cat([bg, bu]) if has_bias else None
-        self.gate_up = Linear(w, b, ctx.dtype)
-        self.down = Linear(tensors[prefix + "down_proj.weight"], tensors.get(prefix + "down_proj.bias"), ctx.dtype)
+        self.gate_up = make_linear(w, b, ctx)
+        self.down = make_linear(tensors[prefix + "down_proj.weight"], tensors.get(prefix + "down_proj.bias"), ctx)
 
+    weight_types = ("fp8",)  # the types of weights that this part keeps beside the model's own
     takes_then = True       # the last projection may fold its output into the residual (NormAfter)
     takes_raw = True        # the first projection takes a norm's output in two pieces (RawNormed)
 

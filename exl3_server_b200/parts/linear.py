@@ -16,6 +16,9 @@ position encoding.  Products in between (some hundred rows, or a narrow output)
 are the library's (cuBLAS through ``torch``), as the reference's are MLX's
 (src/model.cpp:549); the gated feed-forward projection, whose epilogue is fused,
 never goes to the library.
+
+``LinearFP8`` keeps the weight in 8-bit floating point with scales for blocks of 128 and rounds the activations likewise; one
+kernel up to 16 rows, the rounding and the product beyond (``kernels.fp8_linear``).
 """
 from __future__ import annotations
 
@@ -24,7 +27,7 @@ from typing import Optional
 import torch
 
 from ..ops import kernels as K
-from .base import RawNormed
+from .base import BuildContext, RawNormed
 
 
 import os
@@ -185,3 +188,58 @@ class Linear:
         if self.bias is not None:
             n += self.bias.numel() * self.bias.element_size()
         return n
+
+
+class LinearFP8:
+    """``Linear`` with the weight in 8-bit floating point, a scale for each block of 128 x 128, rounded once when the model is built
+    (``kernels.fp8_quantize_weight``).  Activations are rounded per row and 128 features inside the product; the results are bfloat16 (or
+    float32).  It takes a norm's output whole and leaves the residual to the next norm's kernel."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor], dtype: torch.dtype):
+        if weight.dim() != 2:
+            raise ValueError(f"LinearFP8: weight must be 2-dimensional, got {tuple(weight.shape)}")
+        if dtype != torch.bfloat16:
+            raise ValueError(f"weights in 8 bits go with bfloat16 activations, not {dtype}")
+        if weight.shape[1] % 16:
+            raise ValueError(f"weights in 8 bits want input features in multiples of 16, got {weight.shape[1]}")
+        self.weight, self.scales = K.fp8_quantize_weight(weight.to(dtype))
+        self.bias = None if bias is None else bias.to(dtype).contiguous()
+        self.out_features, self.in_features = self.weight.shape
+        self.dtype = dtype
+
+    def __call__(self, x, out_dtype: Optional[torch.dtype] = None, then=None) -> torch.Tensor:
+        if isinstance(x, RawNormed):
+            x = x.materialize()
+        return K.fp8_linear(x, self.weight, self.scales, self.bias, out_dtype or self.dtype)
+
+    def heads_rotated_and_cached(self, *args, **kwargs):
+        return None
+
+    def wide_dtype(self, rows: int) -> torch.dtype:
+        return torch.float32 if rows <= SKINNY_ROWS else self.dtype
+
+    def xielu(self, x, act_p, act_n, out_dtype):
+        return None
+
+    def gelu(self, x, out_dtype, tanh: bool = False, relu2: bool = False):
+        return None
+
+    def streams_weights(self, rows: int) -> bool:
+        return True
+
+    def fuses_gate(self) -> bool:
+        return self.bias is None and self.out_features % 16 == 0
+
+    def gated(self, x: torch.Tensor) -> torch.Tensor:
+        if isinstance(x, RawNormed):
+            x = x.materialize()
+        return K.fp8_linear(x, self.weight, self.scales, None, self.dtype, gated=True)
+
+    def weight_bytes(self) -> int:
+        n = self.weight.numel() + self.scales.numel() * 4
+        return n + (self.bias.numel() * self.bias.element_size() if self.bias is not None else 0)
+
+
+def make_linear(weight: torch.Tensor, bias: Optional[torch.Tensor], ctx: BuildContext):
+    """A projection whose weight is kept as the context says."""
+    return (LinearFP8 if ctx.weight_type == "fp8" else Linear)(weight, bias, ctx.dtype)
