@@ -1,0 +1,43 @@
+// Prompts over the 4-bit cache: the rows' pages come out of it in fp16 (cache4.cu), and the prompt attention of
+// attention_prefill_tc.cuh, compiled for fp16, runs over them.
+//
+// Why fp16: it is what tcgen05.mma takes at this rate beside bfloat16, and its 11 bits hold mn + sc * code to 2^-12, where bfloat16's 8
+// moved the scores so far that results were 0.005 off (relative to 64 bits; fp16 0.0017, the bfloat16 result's own rounding).  A query row is
+// scaled by a power of two into fp16's range, and its factor travels with it; keys and values beyond 65,504 count as 65,504.
+#define EXL3_PREFILL_F16
+#include "attention_prefill_tc.cuh"
+
+extern "C" int exl3_kv4_prompt_status() { return fa_status(); }
+
+static long long kv4_up16(long long n) { return (n + 15) / 16 * 16; }
+
+// Bytes of scratch: the pages' keys and values, the queries, their factors, the pages' own table.
+extern "C" long long exl3_kv4_prompt_scratch(int T, int pages, int nh, int nkv, int hd) {
+  return 2 * (long long)pages * nkv * 64 * hd * 2 + kv4_up16((long long)T * nh * hd * 2) + kv4_up16((long long)T * nh * 4) + kv4_up16((long long)pages * 4);
+}
+
+extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table,
+                               int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0,
+                               int n_tiles, int nh, int nkv, int hd, int window, float scale, void* scratch, long long scratch_bytes,
+                               cudaStream_t stream) {
+  if (T == 0 || n_tiles == 0) return 0;
+  if (T < 0 || rows < 1 || width < 1 || nkv < 1 || nh < 1 || nh % nkv || !fa_supported(hd, 64) || (int64_t)rows * width > INT32_MAX || !q || !out ||
+      !pool || !block_table || !row_start || !row_pos0 || !tile_seq || !tile_q0 || !scratch) {
+    set_error("kv4_prompt: needs heads of 64 or 128 and all of its arrays, got T=%d rows=%d heads=%d kv_heads=%d head_dim=%d", T, rows, nh, nkv, hd);
+    return ERR_BAD_ARGUMENT;
+  }
+  const int pages = rows * width;
+  if (!aligned16(scratch) || scratch_bytes < exl3_kv4_prompt_scratch(T, pages, nh, nkv, hd)) {
+    set_error("kv4_prompt: %lld bytes of scratch wanted, 16-byte aligned", exl3_kv4_prompt_scratch(T, pages, nh, nkv, hd));
+    return ERR_SCRATCH;
+  }
+  unsigned char* k = static_cast<unsigned char*>(scratch);
+  unsigned char* v = k + (long long)pages * nkv * 64 * hd * 2;
+  unsigned char* q16 = v + (long long)pages * nkv * 64 * hd * 2;
+  float* q_scale = reinterpret_cast<float*>(q16 + kv4_up16((long long)T * nh * hd * 2));
+  int* table = reinterpret_cast<int*>(reinterpret_cast<unsigned char*>(q_scale) + kv4_up16((long long)T * nh * 4));
+  const int rc = exl3_kv4_unpack16(pool, n_pages, block_table, pages, nkv, hd, k, v, table, q, q_stride, T, nh, q16, q_scale, stream);
+  if (rc) return rc;
+  return fa_run(q16, (int64_t)nh * hd, T, out, k, v, (int64_t)pages * nkv * 64, table, width, row_start, row_pos0, tile_seq, tile_q0, n_tiles,
+                nh, nkv, hd, 64, window, 0, 0, scale, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr, q_scale, stream);
+}

@@ -4,11 +4,13 @@
 //   store  q, k rotated in float32 (pairs d, d + HD / 2), q rounded to bfloat16; per group of 32 features mn = bfloat16(min),
 //          sc = bfloat16((max - mn) / 15), code = clamp(rint((x - mn) * (1 / sc)), 0, 15) on the float32 values.  A group that holds a
 //          value that is not finite, or whose range is not, becomes NaN as a whole.
-//   load   mn + sc * code (exact in float32: 8 x 4 bits) rounded to bfloat16.
+//   load   mn + sc * code (exact in float32: 8 x 4 bits) rounded to bfloat16, or to fp16 for the prompt attention.
 //
 // Both are bound by memory, or by their launch in a decode step.
 #include "api.h"
 #include "cache4.cuh"
+
+#include <cuda_fp16.h>
 
 namespace exl3 {
 
@@ -114,25 +116,18 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv
   }
 }
 
-// Pages listed in `pages` to bfloat16 [n, nkv, 64, HD]: a block per (page, kv head), a thread per eight features of a key or value.
-template <int HD>
-__global__ void __launch_bounds__(C4_THREADS)
-kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n_pages, int nkv,
-                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ table_out) {
+// fp16 holds up to 65,504; NaN stays.
+template <typename T> __device__ inline T c4_out(float v);
+template <> __device__ inline __nv_bfloat16 c4_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ inline __half c4_out<__half>(float v) { return __float2half_rn(fabsf(v) > 65504.0f ? copysignf(65504.0f, v) : v); }
+
+// Half of a page of a kv head, keys or values, to T [64][HD]: a thread per eight features.
+template <int HD, typename T>
+__device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool key, bool there, T* __restrict__ out) {
   constexpr int LANES = HD / 8;
-  pdl_trigger();
-  pdl_wait();
-  const int page = __ldcg(pages + blockIdx.x), kv = blockIdx.y;
-  const bool there = page >= 0 && page < n_pages;
-  if (table_out) {                                                      // the unpacked pages' own table: no values where there is no page
-    if (kv == 0 && threadIdx.x == 0) table_out[blockIdx.x] = there ? (int)blockIdx.x : -1;
-    if (!there) return;
-  }
-  const unsigned char* base = pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD);
-  const int64_t out0 = ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD;
-  for (int i = threadIdx.x; i < 2 * PAGE * LANES; i += C4_THREADS) {
-    const bool key = i < PAGE * LANES;
-    const int r = key ? i : i - PAGE * LANES, slot = r / LANES, j = r % LANES;
+#pragma unroll
+  for (int r = threadIdx.x; r < PAGE * LANES; r += C4_THREADS) {
+    const int slot = r / LANES, j = r % LANES;
     const unsigned char* tile = base + slot / tile_tokens(HD) * TILE;
     const int tok = slot % tile_tokens(HD);
     const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(tile + (key ? K_WORDS : V_WORDS) + (tok * (HD / 32) + (j >> 2)) * 4));
@@ -150,11 +145,72 @@ kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
         for (int n = 0; n < 4; ++n) code[4 * p + n] = (w >> (4 * n)) & 15u;
       }
     }
-    float v[8];
+    __align__(16) T v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = there ? fmaf(word_sc(word), (float)code[e], word_mn(word)) : 0.0f;
-    store_vec((key ? k_out : v_out) + out0 + (int64_t)slot * HD + 8 * j, v);
+    for (int e = 0; e < 8; ++e) v[e] = c4_out<T>(there ? fmaf(word_sc(word), (float)code[e], word_mn(word)) : 0.0f);
+    *reinterpret_cast<uint4*>(out + slot * HD + 8 * j) = *reinterpret_cast<const uint4*>(v);
   }
+}
+
+// Pages listed in `pages` to bfloat16 [n, nkv, 64, HD]: a block per (page, kv head) and keys or values.
+template <int HD>
+__global__ void __launch_bounds__(C4_THREADS)
+kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n_pages, int nkv,
+                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out) {
+  pdl_trigger();
+  pdl_wait();
+  const int page = __ldcg(pages + blockIdx.x), kv = blockIdx.y >> 1;
+  const bool key = !(blockIdx.y & 1), there = page >= 0 && page < n_pages;
+  c4_unpack<HD>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), key, there,
+                (key ? k_out : v_out) + ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD);
+}
+
+// The same to fp16 for the prompt attention, with the pages' own table (entry i: i, or -1 where there is no page, and nothing is written
+// for it), and the queries to fp16: a row of a head times a power of two that brings its largest value to [2^10, 2^11), whose inverse goes to
+// q_scale.  A query with a value that is not finite becomes NaN.
+template <int HD>
+__global__ void __launch_bounds__(C4_THREADS)
+kv4_unpack16_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n, int n_pages, int nkv, __half* __restrict__ k_out,
+                    __half* __restrict__ v_out, int* __restrict__ table, const __nv_bfloat16* __restrict__ q, int64_t q_stride, int T, int nh,
+                    __half* __restrict__ q_out, float* __restrict__ q_scale) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t page_blocks = (int64_t)n * nkv * 2;
+  if (blockIdx.x < page_blocks) {
+    const int i = (int)(blockIdx.x / (2 * nkv)), y = (int)(blockIdx.x % (2 * nkv)), kv = y >> 1;
+    const int page = __ldcg(pages + i);
+    const bool there = page >= 0 && page < n_pages;
+    if (y == 0 && threadIdx.x == 0) table[i] = there ? i : -1;
+    if (there) c4_unpack<HD>(pool + ((int64_t)page * nkv + kv) * page_bytes(HD), !(y & 1), true, ((y & 1) ? v_out : k_out) + ((int64_t)i * nkv + kv) * PAGE * HD);
+    return;
+  }
+  constexpr int LANES = HD / 8, GROUPS = C4_THREADS / LANES;           // eight features a lane
+  const int64_t item = (blockIdx.x - page_blocks) * GROUPS + threadIdx.x / LANES;
+  const int j = threadIdx.x % LANES;
+  const bool live = item < (int64_t)T * nh;
+  const int64_t t = live ? item / nh : 0;
+  const int head = live ? (int)(item % nh) : 0;
+  float x[8];
+  load_vec_cg(q + t * q_stride + (int64_t)head * HD + 8 * j, x);
+  float top = 0.0f;
+  bool finite = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top = fmaxf(top, fabsf(x[e]));
+    finite = finite && fabsf(x[e]) < __int_as_float(0x7f800000);
+  }
+  if (!finite) top = __int_as_float(0x7f800000);
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  finite = top < __int_as_float(0x7f800000);
+  const int e2 = finite && top > 0.0f ? min(max(10 + 127 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
+  const float up = __int_as_float((127 + e2) << 23), down = __int_as_float((127 - e2) << 23);
+  if (!live) return;
+  __align__(16) __half h[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = finite ? __float2half_rn(x[e] * up) : __ushort_as_half(0x7e00);
+  *reinterpret_cast<uint4*>(q_out + (t * nh + head) * HD + 8 * j) = *reinterpret_cast<const uint4*>(h);
+  if (j == 0) q_scale[t * nh + head] = down;
 }
 
 }  // namespace exl3
@@ -184,17 +240,32 @@ extern "C" int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, 
 }
 
 extern "C" int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
-                             int* table_out, cudaStream_t stream) {
+                             cudaStream_t stream) {
   if (n == 0) return 0;
-  if (n < 0 || nkv < 1 || nkv > 65535 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || !pool || !pages || !k_out || !v_out) {
+  if (n < 0 || nkv < 1 || nkv > 32767 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || !pool || !pages || !k_out || !v_out) {
     set_error("kv4_load: needs heads of 64 or 128 and all of its arrays, got %d pages, kv_heads=%d head_dim=%d", n, nkv, hd);
     return ERR_BAD_ARGUMENT;
   }
   if (!aligned16(pool) || !aligned16(k_out) || !aligned16(v_out)) { set_error("kv4_load: the pool and the results must be 16-byte aligned"); return ERR_ALIGNMENT; }
   auto go = [&](auto kernel) {
-    launch_pdl(kernel, dim3(n, nkv), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, (int)n_pages, nkv,
-               static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), table_out);
+    launch_pdl(kernel, dim3(n, 2 * nkv), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, (int)n_pages, nkv,
+               static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out));
   };
   if (hd == 64) go(kv4_load_kernel<64>); else go(kv4_load_kernel<128>);
   return launch_status("kv4_load");
+}
+
+extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
+                                 int* table, const void* q, int64_t q_stride, int T, int nh, void* q_out, float* q_scale, cudaStream_t stream) {
+  if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  const int per = C4_THREADS / (hd / 8);
+  const int64_t blocks = (int64_t)n * nkv * 2 + ((int64_t)T * nh + per - 1) / per;
+  if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
+  auto go = [&](auto kernel) {
+    launch_pdl(kernel, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, n, (int)n_pages, nkv,
+               static_cast<__half*>(k_out), static_cast<__half*>(v_out), table, static_cast<const __nv_bfloat16*>(q), q_stride, T, nh,
+               static_cast<__half*>(q_out), q_scale);
+  };
+  if (hd == 64) go(kv4_unpack16_kernel<64>); else go(kv4_unpack16_kernel<128>);
+  return launch_status("kv4_unpack16");
 }

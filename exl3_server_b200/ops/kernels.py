@@ -1142,7 +1142,7 @@ def check_status() -> None:
                                      ("attn_prefill_tc", attn_prefill_tc_status),
                                      ("attn_decode", attn_decode_status),
                                      ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status),
-                                     ("kv4_attn", kv4_attn_status), ("fp8_skinny", fp8_skinny_status),
+                                     ("kv4_attn", kv4_attn_status), ("kv4_prompt", kv4_prompt_status), ("fp8_skinny", fp8_skinny_status),
                                      ("fp8_wide", fp8_wide_status)) if fn()]
     if gave_up:
         raise KernelLibraryError("a bounded wait ran out in " + ", ".join(gave_up) +
@@ -1924,14 +1924,10 @@ def kv4_load(pool: torch.Tensor, pages: torch.Tensor, head_dim: int):
     _int32(pages, "pages", "kv4_load")
     n, kv_heads = pages.numel(), pool.shape[1]
     k, v = torch.empty((2, n, kv_heads, KV4_PAGE, head_dim), dtype=torch.bfloat16, device=pool.device).unbind(0)
-    _kv4_unpack(pool, pages, n, head_dim, k.data_ptr(), v.data_ptr(), 0)
-    return k, v
-
-
-def _kv4_unpack(pool: torch.Tensor, pages: torch.Tensor, n: int, head_dim: int, k: int, v: int, table: int) -> None:
-    rc = _entry("exl3_kv4_load", "plpiiippp")(_addr(pool), pool.shape[0], _addr(pages), n, pool.shape[1], head_dim, k, v, table, _raw_stream())
+    rc = _entry("exl3_kv4_load", "plpiiipp")(_addr(pool), pool.shape[0], _addr(pages), n, kv_heads, head_dim, k.data_ptr(), v.data_ptr(), _raw_stream())
     if rc:
         _check(rc, "kv4_load")
+    return k, v
 
 
 def kv4_attn_status() -> int:
@@ -1979,7 +1975,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     tokens (None: never more than a few).  ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's).
 
     A few tokens a row (``KV4_FEW_COLUMNS``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
-    unpacked to bfloat16 and go through the tcgen05 attention."""
+    unpacked to fp16 (values beyond 65,504 count as that) and go through the tcgen05 attention."""
     T = q.shape[0]
     if q.dtype != torch.bfloat16 or q.dim() != 2 or q.shape[1] != heads * head_dim or q.stride(1) != 1:
         raise KernelLibraryError(f"kv4_attn: q must be bfloat16 [tokens, {heads * head_dim}], got {q.dtype} {tuple(q.shape)}")
@@ -2021,20 +2017,23 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     return out
 
 
+def kv4_prompt_status() -> int:
+    return int(library().exl3_kv4_prompt_status())
+
+
 def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window, workspace, out):
-    """Prompts: the rows' pages in bfloat16 in scratch memory, page i of row r at r * width + i, and the tcgen05 attention over them."""
-    rows, width = row_pos0.numel(), block_table.shape[1]
-    n = rows * width
-    floats = n * kv_heads * KV4_PAGE * head_dim // 2
-    need = 2 * floats + n
-    scratch = workspace.plain(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
-    shape = (n, kv_heads, KV4_PAGE, head_dim)
-    k, v = (scratch[i * floats:(i + 1) * floats].view(torch.bfloat16).view(shape) for i in range(2))
-    table = scratch[2 * floats:2 * floats + n].view(torch.int32).view(rows, width)
+    """Prompts: the rows' pages and the queries in fp16 in scratch memory, and the tcgen05 attention over them (attention_prefill_f16.cu)."""
+    T, rows, width = q.shape[0], row_pos0.numel(), block_table.shape[1]
+    up = lambda n: -(-n // 16) * 16
+    need = 4 * rows * width * kv_heads * KV4_PAGE * head_dim + up(2 * T * heads * head_dim) + up(4 * T * heads) + up(4 * rows * width)
+    scratch = workspace.plain(need // 4) if workspace is not None else torch.empty(need // 4, dtype=torch.float32, device=q.device)
     pages = block_table[:rows] if block_table.stride(0) == width else block_table[:rows].contiguous()
-    _kv4_unpack(pool, pages, n, head_dim, k.data_ptr(), v.data_ptr(), table.data_ptr())
-    return attn_prefill_tc(q, q.stride(0), out, k, v, table, row_start, row_pos0, tiles[0], tiles[1], tiles[2], heads, kv_heads,
-                           head_dim, KV4_PAGE, window, scale)
+    rc = _entry("exl3_kv4_prompt", "plipplpiippppiiiiifpl")(
+        _addr(q), q.stride(0), T, _addr(out), _addr(pool), pool.shape[0], _addr(pages), rows, width, _addr(row_start), _addr(row_pos0),
+        _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, _addr(scratch), need, _raw_stream())
+    if rc:
+        _check(rc, "kv4_attn")
+    return out
 
 
 # ---- products in 8-bit floating point (fp8.cuh) ---------------------------------------------------------------
