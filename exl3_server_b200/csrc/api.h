@@ -467,7 +467,8 @@ int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float
 int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
                   cudaStream_t stream);
 // Pages and queries in fp16 for the prompt attention (see cache4.cu), and the attention of prompts over a table [rows, width] of pages.
-int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out, int* table,
+int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* pages, int rows, int width, const int* row_start, const int* row_pos0, int nkv,
+                      int hd, void* k_out, void* v_out, int* table,
                       const void* q, int64_t q_stride, int T, int nh, void* q_out, float* q_scale, cudaStream_t stream);
 long long exl3_kv4_prompt_scratch(int T, int pages, int nh, int nkv, int hd);
 int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table, int rows,

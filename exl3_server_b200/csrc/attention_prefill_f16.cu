@@ -3,7 +3,9 @@
 //
 // Why fp16: it is what tcgen05.mma takes at this rate beside bfloat16, and its 11 bits hold mn + sc * code to 2^-12, where bfloat16's 8
 // moved the scores so far that results were 0.005 off (relative to 64 bits; fp16 0.0017, the bfloat16 result's own rounding).  A query row is
-// scaled by a power of two into fp16's range, and its factor travels with it; keys and values beyond 65,504 count as 65,504.
+// scaled by a power of two into fp16's range, and its factor travels with it; keys and values beyond 65,504 count as 65,504.  The second
+// product multiplies hidden values by zero, so a token with a NaN among its values is given as a NaN key and values of zero: who sees it gets NaN (in
+// all features), who does not is not touched.
 #define EXL3_PREFILL_F16
 #include "attention_prefill_tc.cuh"
 
@@ -36,7 +38,7 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
   unsigned char* q16 = v + (long long)pages * nkv * 64 * hd * 2;
   float* q_scale = reinterpret_cast<float*>(q16 + kv4_up16((long long)T * nh * hd * 2));
   int* table = reinterpret_cast<int*>(reinterpret_cast<unsigned char*>(q_scale) + kv4_up16((long long)T * nh * 4));
-  const int rc = exl3_kv4_unpack16(pool, n_pages, block_table, pages, nkv, hd, k, v, table, q, q_stride, T, nh, q16, q_scale, stream);
+  const int rc = exl3_kv4_unpack16(pool, n_pages, block_table, rows, width, row_start, row_pos0, nkv, hd, k, v, table, q, q_stride, T, nh, q16, q_scale, stream);
   if (rc) return rc;
   return fa_run(q16, (int64_t)nh * hd, T, out, k, v, (int64_t)pages * nkv * 64, table, width, row_start, row_pos0, tile_seq, tile_q0, n_tiles,
                 nh, nkv, hd, 64, window, 0, 0, scale, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr, q_scale, stream);

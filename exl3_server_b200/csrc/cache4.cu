@@ -51,55 +51,74 @@ __device__ inline uint32_t c4_quantize(const float (&x)[8], uint32_t& codes) {
   return (uint32_t)__bfloat16_as_ushort(scb) << 16 | __bfloat16_as_ushort(mnb);
 }
 
-// A block takes one token and the heads blockIdx.y, + gridDim.y, ... in steps of as many as its threads cover; the token's sines and cosines
-// are worked out once for all of them.
-template <int HD>
+// A block takes TOK tokens (their positions, pages and sines at once: three trips to memory that stand in a row for each block) and the
+// (token, head) pairs blockIdx.y, + gridDim.y, ... in steps of as many as its threads cover; the next pair's features are asked for
+// before this one's are worked on.
+template <int HD, int TOK>
 __global__ void __launch_bounds__(C4_THREADS)
 kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv_bfloat16* __restrict__ q_out,
                  const float* __restrict__ freq, const float* __restrict__ freq_lo, const int* __restrict__ tok_pos,
                  const int* __restrict__ tok_seq, const int* __restrict__ block_table, int bt_stride, unsigned char* __restrict__ pool,
-                 int n_pages, int nh, int nkv) {
-  constexpr int LANES = HD / 8, HEADS = C4_THREADS / LANES;           // heads that the block works on side by side
-  __shared__ float s_cos[HD / 2], s_sin[HD / 2];
+                 int n_pages, int T, int nh, int nkv) {
+  constexpr int LANES = HD / 8, HEADS = C4_THREADS / LANES;           // pairs that the block works on side by side
+  __shared__ float s_cos[TOK][HD / 2], s_sin[TOK][HD / 2];
+  __shared__ int s_pos[TOK], s_page[TOK];
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x;
-  const int pos = __ldcg(tok_pos + t), seq = __ldcg(tok_seq + t);
-  if (freq) {
-    for (int d = threadIdx.x; d < HD / 2; d += C4_THREADS)
-      rope_sincos((float)pos, __ldg(freq + d), freq_lo ? __ldg(freq_lo + d) : 0.0f, s_sin + d, s_cos + d);
-    __syncthreads();
+  const int t0 = blockIdx.x * TOK, n_tok = min(TOK, T - t0);
+  const int j = threadIdx.x % LANES, jp = j ^ (LANES / 2);
+  const int total = nh + 2 * nkv, pairs = n_tok * total;
+  auto ask = [&](int i, uint4& own, uint4& other) {
+    own = other = make_uint4(0, 0, 0, 0);
+    if (i >= pairs) return;
+    const __nv_bfloat16* src = qkv + (int64_t)(t0 + i / total) * qkv_stride + (int64_t)(i % total) * HD;
+    own = load_raw_cg(src + 8 * j);
+    if (freq && i % total < nh + nkv) other = load_raw_cg(src + 8 * jp);
+  };
+  const int step = gridDim.y * HEADS;
+  int i = blockIdx.y * HEADS + threadIdx.x / LANES;
+  uint4 own, other;
+  ask(i, own, other);
+  if (threadIdx.x < n_tok) {
+    const int pos = __ldcg(tok_pos + t0 + threadIdx.x);
+    s_pos[threadIdx.x] = pos;
+    s_page[threadIdx.x] = pos >= 0 ? __ldcg(block_table + (int64_t)__ldcg(tok_seq + t0 + threadIdx.x) * bt_stride + pos / PAGE) : -1;
   }
-  const int page = pos >= 0 ? __ldcg(block_table + (int64_t)seq * bt_stride + pos / PAGE) : -1;
-  const int j = threadIdx.x % LANES;
-  const int total = nh + 2 * nkv;
-  for (int first = blockIdx.y * HEADS; first < total; first += gridDim.y * HEADS) {
-    const int head = first + threadIdx.x / LANES;
-    const bool live = head < total;                                    // (the whole group of lanes; the shuffles need everybody)
-    const __nv_bfloat16* src = qkv + (int64_t)t * qkv_stride + (int64_t)(live ? head : 0) * HD;
+  if (freq)
+    for (int d = threadIdx.x; d < n_tok * (HD / 2); d += C4_THREADS)
+      rope_sincos((float)__ldcg(tok_pos + t0 + d / (HD / 2)), __ldg(freq + d % (HD / 2)), freq_lo ? __ldg(freq_lo + d % (HD / 2)) : 0.0f,
+                  &s_sin[0][0] + d, &s_cos[0][0] + d);
+  __syncthreads();
+  for (int first = blockIdx.y * HEADS; first < pairs; first += step, i += step) {
+    const bool live = i < pairs;                                       // (the whole group of lanes; the shuffles need everybody)
+    const int tk = live ? i / total : 0, head = live ? i - tk * total : 0, t = t0 + tk;
+    uint4 next_own, next_other;
+    ask(i + step, next_own, next_other);
     float x[8];
-    load_vec_cg(src + 8 * j, x);
+    unpack_raw(own, x, static_cast<const __nv_bfloat16*>(nullptr));
     if (freq && head < nh + nkv) {
-      const int jp = j ^ (LANES / 2);
       float y[8];
-      load_vec_cg(src + 8 * jp, y);
+      unpack_raw(other, y, static_cast<const __nv_bfloat16*>(nullptr));
       const int d0 = 8 * (j & (LANES / 2 - 1));
       const float sign = j < LANES / 2 ? -1.0f : 1.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * s_cos[d0 + e] + sign * (y[e] * s_sin[d0 + e]);
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * s_cos[tk][d0 + e] + sign * (y[e] * s_sin[tk][d0 + e]);
     }
+    own = next_own;
+    other = next_other;
     if (live && head < nh) store_vec(q_out + ((int64_t)t * nh + head) * HD + 8 * j, x);
-    // (warps that hold queries only skip the rest; a warp's heads are neighbours)
+    // (warps that hold queries only skip the rest)
     if (__all_sync(0xffffffffu, head < nh || !live)) continue;
     uint32_t codes;
     const uint32_t word = c4_quantize(x, codes);
     // values: a word has four features of one group below and four of the next above: lanes j and j ^ 4 trade halves
     const uint32_t give = (j & 4) ? codes & 0xffffu : codes >> 16;
     const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 4);
+    const int page = s_page[tk];
     if (!live || head < nh || page < 0 || page >= n_pages) continue;
     const bool key = head < nh + nkv;
     const int kv = key ? head - nh : head - nh - nkv;
-    const int slot = pos % PAGE, tok = slot % tile_tokens(HD);
+    const int slot = s_pos[tk] % PAGE, tok = slot % tile_tokens(HD);
     unsigned char* tile = pool + ((int64_t)page * nkv + kv) * page_bytes(HD) + slot / tile_tokens(HD) * TILE;
     if (key) {
       uint32_t w = 0;
@@ -121,9 +140,10 @@ template <typename T> __device__ inline T c4_out(float v);
 template <> __device__ inline __nv_bfloat16 c4_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ inline __half c4_out<__half>(float v) { return __float2half_rn(fabsf(v) > 65504.0f ? copysignf(65504.0f, v) : v); }
 
-// Half of a page of a kv head, keys or values, to T [64][HD]: a thread per eight features.
-template <int HD, typename T>
-__device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool key, bool there, T* __restrict__ out) {
+// Half of a page of a kv head, keys or values, to T [64][HD]: a thread per eight features.  CLEAN, for a product that multiplies hidden values by
+// zero: places from `held` on are zeros, and a token with a NaN among its values has zeros there and NaN in all of its key, which a mask can hide.
+template <int HD, bool CLEAN, typename T>
+__device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool key, bool there, int held, T* __restrict__ out) {
   constexpr int LANES = HD / 8;
 #pragma unroll
   for (int r = threadIdx.x; r < PAGE * LANES; r += C4_THREADS) {
@@ -145,9 +165,27 @@ __device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool ke
         for (int n = 0; n < 4; ++n) code[4 * p + n] = (w >> (4 * n)) & 15u;
       }
     }
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = there ? fmaf(word_sc(word), (float)code[e], word_mn(word)) : 0.0f;
+    if (CLEAN) {
+      if (key) {
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+          const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(tile + V_WORDS + (tok * (HD / 32) + i) * 4));
+          nan = nan || !(fabsf(word_sc(w)) < __int_as_float(0x7f800000)) || !(fabsf(word_mn(w)) < __int_as_float(0x7f800000));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = slot >= held ? 0.0f : nan ? __int_as_float(0x7fc00000) : f[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = slot >= held || !(fabsf(f[e]) < __int_as_float(0x7f800000)) ? 0.0f : f[e];
+      }
+    }
     __align__(16) T v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c4_out<T>(there ? fmaf(word_sc(word), (float)code[e], word_mn(word)) : 0.0f);
+    for (int e = 0; e < 8; ++e) v[e] = c4_out<T>(f[e]);
     *reinterpret_cast<uint4*>(out + slot * HD + 8 * j) = *reinterpret_cast<const uint4*>(v);
   }
 }
@@ -161,8 +199,8 @@ kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
   pdl_wait();
   const int page = __ldcg(pages + blockIdx.x), kv = blockIdx.y >> 1;
   const bool key = !(blockIdx.y & 1), there = page >= 0 && page < n_pages;
-  c4_unpack<HD>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), key, there,
-                (key ? k_out : v_out) + ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD);
+  c4_unpack<HD, false>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), key, there, PAGE,
+                       (key ? k_out : v_out) + ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD);
 }
 
 // The same to fp16 for the prompt attention, with the pages' own table (entry i: i, or -1 where there is no page, and nothing is written
@@ -170,7 +208,8 @@ kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
 // q_scale.  A query with a value that is not finite becomes NaN.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
-kv4_unpack16_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n, int n_pages, int nkv, __half* __restrict__ k_out,
+kv4_unpack16_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n, int width, const int* __restrict__ row_start,
+                    const int* __restrict__ row_pos0, int n_pages, int nkv, __half* __restrict__ k_out,
                     __half* __restrict__ v_out, int* __restrict__ table, const __nv_bfloat16* __restrict__ q, int64_t q_stride, int T, int nh,
                     __half* __restrict__ q_out, float* __restrict__ q_scale) {
   pdl_trigger();
@@ -181,7 +220,10 @@ kv4_unpack16_kernel(const unsigned char* __restrict__ pool, const int* __restric
     const int page = __ldcg(pages + i);
     const bool there = page >= 0 && page < n_pages;
     if (y == 0 && threadIdx.x == 0) table[i] = there ? i : -1;
-    if (there) c4_unpack<HD>(pool + ((int64_t)page * nkv + kv) * page_bytes(HD), !(y & 1), true, ((y & 1) ? v_out : k_out) + ((int64_t)i * nkv + kv) * PAGE * HD);
+    if (there) {
+      const int row = i / width, held = __ldcg(row_pos0 + row) + __ldcg(row_start + row + 1) - __ldcg(row_start + row) - i % width * PAGE;
+      c4_unpack<HD, true>(pool + ((int64_t)page * nkv + kv) * page_bytes(HD), !(y & 1), true, held, ((y & 1) ? v_out : k_out) + ((int64_t)i * nkv + kv) * PAGE * HD);
+    }
     return;
   }
   constexpr int LANES = HD / 8, GROUPS = C4_THREADS / LANES;           // eight features a lane
@@ -229,13 +271,17 @@ extern "C" int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, 
     return ERR_BAD_ARGUMENT;
   }
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(pool) || qkv_stride % 8) { set_error("kv4_store: qkv, its rows, q and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  // Few tokens: one a block, its heads over several blocks; many: four a block.
   const int per = C4_THREADS / (hd / 8), rounds = ceil_div(nh + 2 * nkv, per);
-  const int gy = T >= 296 ? 1 : rounds < 32 ? rounds : 32;             // few tokens: a token's heads over several blocks
+  const bool many = T >= 1024;
+  const int gy = many ? 1 : T >= 296 ? 1 : rounds < 32 ? rounds : 32;
   auto go = [&](auto kernel) {
-    launch_pdl(kernel, dim3(T, gy), dim3(C4_THREADS), 0, stream, static_cast<const __nv_bfloat16*>(qkv), qkv_stride, static_cast<__nv_bfloat16*>(q_out), freq,
-               freq_lo, tok_pos, tok_seq, block_table, bt_stride, static_cast<unsigned char*>(pool), (int)n_pages, nh, nkv);
+    launch_pdl(kernel, dim3(many ? ceil_div(T, 4) : T, gy), dim3(C4_THREADS), 0, stream, static_cast<const __nv_bfloat16*>(qkv), qkv_stride,
+               static_cast<__nv_bfloat16*>(q_out), freq, freq_lo, tok_pos, tok_seq, block_table, bt_stride, static_cast<unsigned char*>(pool),
+               (int)n_pages, T, nh, nkv);
   };
-  if (hd == 64) go(kv4_store_kernel<64>); else go(kv4_store_kernel<128>);
+  if (hd == 64) { if (many) go(kv4_store_kernel<64, 4>); else go(kv4_store_kernel<64, 1>); }
+  else { if (many) go(kv4_store_kernel<128, 4>); else go(kv4_store_kernel<128, 1>); }
   return launch_status("kv4_store");
 }
 
@@ -255,15 +301,16 @@ extern "C" int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages
   return launch_status("kv4_load");
 }
 
-extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
+extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* pages, int rows, int width, const int* row_start, const int* row_pos0,
+                                 int nkv, int hd, void* k_out, void* v_out,
                                  int* table, const void* q, int64_t q_stride, int T, int nh, void* q_out, float* q_scale, cudaStream_t stream) {
   if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
-  const int per = C4_THREADS / (hd / 8);
+  const int per = C4_THREADS / (hd / 8), n = rows * width;
   const int64_t blocks = (int64_t)n * nkv * 2 + ((int64_t)T * nh + per - 1) / per;
   if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
   auto go = [&](auto kernel) {
-    launch_pdl(kernel, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, n, (int)n_pages, nkv,
-               static_cast<__half*>(k_out), static_cast<__half*>(v_out), table, static_cast<const __nv_bfloat16*>(q), q_stride, T, nh,
+    launch_pdl(kernel, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, n, width, row_start, row_pos0, (int)n_pages,
+               nkv, static_cast<__half*>(k_out), static_cast<__half*>(v_out), table, static_cast<const __nv_bfloat16*>(q), q_stride, T, nh,
                static_cast<__half*>(q_out), q_scale);
   };
   if (hd == 64) go(kv4_unpack16_kernel<64>); else go(kv4_unpack16_kernel<128>);

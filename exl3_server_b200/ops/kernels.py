@@ -1944,7 +1944,8 @@ def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: i
     shapes (what it picks is 5 % slower in the mean than the best of a shape): a wave of blocks takes 10 us and for each of a block's tiles 0.13 us and
     0.21 us times the blocks that share its SM (a fifth less for heads of 128, a fifth more with 16 columns); rows of a batch are taken to be
     unequal; joining chunks takes 4.5 us."""
-    tiles = max(1, -(-span * head_dim // 4096))
+    per = 4096 // head_dim
+    tiles = (span + per - 2) // per + 1 if window > 0 else max(1, -(-span // per))       # a window may begin anywhere in a tile
     per_sm = 2 if columns == 16 else 3 if columns == 8 and head_dim == 128 else 4
     wide = (1.2 if columns == 16 else 1.0) * (0.8 if head_dim == 128 else 1.0)
     items = rows * kv_heads * groups
@@ -1961,7 +1962,7 @@ def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: i
         if best is None or cost < best[0] - 1e-9:
             best = (cost, chunk, n)
     _, chunk, n = best
-    return chunk, n + (1 if window > 0 and tiles > 1 else 0)
+    return chunk, (tiles + chunk - 2) // chunk + 1 if window > 0 else n                  # and in a chunk
 
 
 def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row_start: Optional[torch.Tensor],
