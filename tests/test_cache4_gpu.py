@@ -254,6 +254,20 @@ def test_values_that_a_query_does_not_see_may_be_nan(heads, kv_heads, d):
     assert torch.equal(out[:2], clean[:2]) and bool(out[2].isnan().all())
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 2, 64), (8, 1, 128)])
+def test_prompts_do_not_see_later_nan(heads, kv_heads, d):
+    """The 61st of 150 new tokens has a NaN value: queries before it are as without it, the others NaN."""
+    c = Case([(50, 150)], heads, kv_heads, d, seed=15)
+    clean = c.run()
+    bad = c.qkv[110:111].clone()
+    bad[:, (heads + kv_heads) * d + 3] = math.nan                         # the first value head only
+    K().kv4_store(bad, None, ints([110]), ints([0]), c.table, c.pool, heads, kv_heads, d)
+    out = c.run().view(150, heads, d)
+    clean = clean.view(150, heads, d)
+    g = heads // kv_heads
+    assert torch.equal(out[:60], clean[:60]) and bool(out[60:, :g].isnan().all()) and torch.equal(out[:, g:], clean[:, g:])
+
+
 def test_a_group_of_values_that_is_nan_stays_in_its_features():
     c = Case([(80, 1)], 4, 4, 64, seed=9)
     bad = c.qkv[10:11].clone()
