@@ -18,18 +18,30 @@ using namespace kv4;
 
 constexpr int C4_THREADS = 256;
 
+__device__ inline float c4_min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ inline float c4_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // A lane has features 8 j .. 8 j + 7 of a head (j = 0 .. HD / 8 - 1); four neighbouring lanes have a group.  Returns the group's word and
-// the lane's eight codes, feature e's in bits 4 e ...
-__device__ inline uint32_t c4_quantize(const float (&x)[8], uint32_t& codes) {
-  float lo = x[0], hi = x[0];
-  bool finite = true;
+// the lane's eight codes as the low bits of floats around 1.5 * 2^23: adding that number rounds to an integer, ties to even, and leaves it there
+// (conversions have a pipe of a quarter of the others' rate: they and the shifts that put the codes together were half of the kernel's time).
+__device__ inline uint32_t c4_quantize(const float (&x)[8], uint32_t (&bits)[8]) {
+  constexpr float ROUND = 12582912.0f;
+  float lo = c4_min3(x[0], x[1], x[2]), hi = c4_max3(x[0], x[1], x[2]);
+  lo = c4_min3(lo, x[3], x[4]); hi = c4_max3(hi, x[3], x[4]);
+  lo = c4_min3(lo, x[5], x[6]); hi = c4_max3(hi, x[5], x[6]);
+  lo = fminf(lo, x[7]); hi = fmaxf(hi, x[7]);
+  float odd = 0.0f;                                                    // 0, or NaN where a value is not finite
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    finite = finite && fabsf(x[e]) < __int_as_float(0x7f800000);
-  }
-  if (!finite) { lo = __int_as_float(0xff800000); hi = __int_as_float(0x7f800000); }
+  for (int e = 0; e < 8; ++e) odd = fmaf(x[e], 0.0f, odd);
+  if (odd != 0.0f) { lo = __int_as_float(0xff800000); hi = __int_as_float(0x7f800000); }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -40,16 +52,25 @@ __device__ inline uint32_t c4_quantize(const float (&x)[8], uint32_t& codes) {
   const float range = fmaxf(hi - mn, 0.0f);
   const __nv_bfloat16 scb = __float2bfloat16_rn(__fdiv_rn(range, 15.0f));
   const float sc = __bfloat162float(scb);
-  codes = 0;
-  if (!(sc < __int_as_float(0x7f800000)) || !(fabsf(mn) < __int_as_float(0x7f800000))) return 0x7fc07fc0u;
-  const float inv = sc > SC_MIN ? __frcp_rn(sc) : 0.0f;
+  const bool fine = sc < __int_as_float(0x7f800000) && fabsf(mn) < __int_as_float(0x7f800000);
+  const float inv = fine && sc > SC_MIN ? __frcp_rn(sc) : 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], mn), inv)), 0.0f), 15.0f);
-    codes |= (uint32_t)(int)c << (4 * e);
+    const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[e], mn), inv), 0.0f), 15.0f);        // (NaN becomes 0)
+    bits[e] = __float_as_uint(__fadd_rn(c, ROUND));
   }
-  return (uint32_t)__bfloat16_as_ushort(scb) << 16 | __bfloat16_as_ushort(mnb);
+  return fine ? (uint32_t)__bfloat16_as_ushort(scb) << 16 | __bfloat16_as_ushort(mnb) : 0x7fc07fc0u;
 }
+// The codes as a word: feature e's in nibble e, or (keys) in nibble e / 2 + 4 (e % 2).  Multiply-adds modulo 2^32; what the floats have above their
+// codes adds up to a constant.
+template <bool KEY> __device__ inline uint32_t c4_word(const uint32_t (&bits)[8]) {
+  uint32_t w = 0u - 0x4b400000u * 0x11111111u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w += bits[e] * (1u << (4 * (KEY ? e / 2 + 4 * (e % 2) : e)));
+  return w;
+}
+// Code e of a word as a float.
+__device__ inline float c4_code(uint32_t w, int shift) { return __uint_as_float(((w >> shift) & 15u) | 0x4b000000u) - 8388608.0f; }
 
 // A block takes TOK tokens (their positions, pages and sines at once: three trips to memory that stand in a row for each block) and the
 // (token, head) pairs blockIdx.y, + gridDim.y, ... in steps of as many as its threads cover; the next pair's features are asked for
@@ -61,24 +82,25 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv
                  const int* __restrict__ tok_seq, const int* __restrict__ block_table, int bt_stride, unsigned char* __restrict__ pool,
                  int n_pages, int T, int nh, int nkv) {
   constexpr int LANES = HD / 8, HEADS = C4_THREADS / LANES;           // pairs that the block works on side by side
-  __shared__ float s_cos[TOK][HD / 2], s_sin[TOK][HD / 2];
+  __shared__ __align__(16) float s_cos[TOK][HD / 2], s_sin[TOK][HD / 2];
   __shared__ int s_pos[TOK], s_page[TOK];
   pdl_trigger();
   pdl_wait();
   const int t0 = blockIdx.x * TOK, n_tok = min(TOK, T - t0);
   const int j = threadIdx.x % LANES, jp = j ^ (LANES / 2);
   const int total = nh + 2 * nkv, pairs = n_tok * total;
-  auto ask = [&](int i, uint4& own, uint4& other) {
+  auto ask = [&](int tk, int head, uint4& own, uint4& other) {
     own = other = make_uint4(0, 0, 0, 0);
-    if (i >= pairs) return;
-    const __nv_bfloat16* src = qkv + (int64_t)(t0 + i / total) * qkv_stride + (int64_t)(i % total) * HD;
+    if (tk >= n_tok) return;
+    const __nv_bfloat16* src = qkv + (int64_t)(t0 + tk) * qkv_stride + head * HD;
     own = load_raw_cg(src + 8 * j);
-    if (freq && i % total < nh + nkv) other = load_raw_cg(src + 8 * jp);
+    if (freq && head < nh + nkv) other = load_raw_cg(src + 8 * jp);
   };
-  const int step = gridDim.y * HEADS;
-  int i = blockIdx.y * HEADS + threadIdx.x / LANES;
+  const int step = gridDim.y * HEADS, step_t = step / total, step_h = step % total;
+  const int i = blockIdx.y * HEADS + threadIdx.x / LANES;
+  int tk = i / total, head = i % total;                               // this pair; the next one is step_t tokens and step_h heads on
   uint4 own, other;
-  ask(i, own, other);
+  ask(tk, head, own, other);
   if (threadIdx.x < n_tok) {
     const int pos = __ldcg(tok_pos + t0 + threadIdx.x);
     s_pos[threadIdx.x] = pos;
@@ -89,42 +111,49 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv
       rope_sincos((float)__ldcg(tok_pos + t0 + d / (HD / 2)), __ldg(freq + d % (HD / 2)), freq_lo ? __ldg(freq_lo + d % (HD / 2)) : 0.0f,
                   &s_sin[0][0] + d, &s_cos[0][0] + d);
   __syncthreads();
-  for (int first = blockIdx.y * HEADS; first < pairs; first += step, i += step) {
-    const bool live = i < pairs;                                       // (the whole group of lanes; the shuffles need everybody)
-    const int tk = live ? i / total : 0, head = live ? i - tk * total : 0, t = t0 + tk;
+  const uint32_t flip = j < LANES / 2 ? 0x80008000u : 0u;             // the lower half of a head subtracts its partner's sines
+  for (int first = blockIdx.y * HEADS; first < pairs; first += step) {
+    const bool live = tk < n_tok;                                      // (the whole group of lanes; the shuffles need everybody)
+    const int now = live ? tk : 0, hd_now = live ? head : 0, t = t0 + now;
+    tk += step_t;
+    head += step_h;
+    if (head >= total) { head -= total; ++tk; }
     uint4 next_own, next_other;
-    ask(i + step, next_own, next_other);
+    ask(tk, head, next_own, next_other);
     float x[8];
     unpack_raw(own, x, static_cast<const __nv_bfloat16*>(nullptr));
-    if (freq && head < nh + nkv) {
+    if (freq && hd_now < nh + nkv) {
       float y[8];
+      other.x ^= flip; other.y ^= flip; other.z ^= flip; other.w ^= flip;
       unpack_raw(other, y, static_cast<const __nv_bfloat16*>(nullptr));
       const int d0 = 8 * (j & (LANES / 2 - 1));
-      const float sign = j < LANES / 2 ? -1.0f : 1.0f;
+      float c[8], sn[8];
+      *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(&s_cos[now][d0]);
+      *reinterpret_cast<float4*>(c + 4) = *reinterpret_cast<const float4*>(&s_cos[now][d0 + 4]);
+      *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(&s_sin[now][d0]);
+      *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(&s_sin[now][d0 + 4]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * s_cos[tk][d0 + e] + sign * (y[e] * s_sin[tk][d0 + e]);
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], c[e], y[e] * sn[e]);
     }
     own = next_own;
     other = next_other;
-    if (live && head < nh) store_vec(q_out + ((int64_t)t * nh + head) * HD + 8 * j, x);
+    if (live && hd_now < nh) store_vec(q_out + ((int64_t)t * nh + hd_now) * HD + 8 * j, x);
     // (warps that hold queries only skip the rest)
-    if (__all_sync(0xffffffffu, head < nh || !live)) continue;
-    uint32_t codes;
-    const uint32_t word = c4_quantize(x, codes);
+    if (__all_sync(0xffffffffu, hd_now < nh || !live)) continue;
+    uint32_t bits[8];
+    const uint32_t word = c4_quantize(x, bits);
+    const bool key = hd_now < nh + nkv;
+    const uint32_t codes = key ? c4_word<true>(bits) : c4_word<false>(bits);
     // values: a word has four features of one group below and four of the next above: lanes j and j ^ 4 trade halves
     const uint32_t give = (j & 4) ? codes & 0xffffu : codes >> 16;
     const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 4);
-    const int page = s_page[tk];
-    if (!live || head < nh || page < 0 || page >= n_pages) continue;
-    const bool key = head < nh + nkv;
-    const int kv = key ? head - nh : head - nh - nkv;
-    const int slot = s_pos[tk] % PAGE, tok = slot % tile_tokens(HD);
+    const int page = s_page[now];
+    if (!live || hd_now < nh || page < 0 || page >= n_pages) continue;
+    const int kv = key ? hd_now - nh : hd_now - nh - nkv;
+    const int slot = s_pos[now] % PAGE, tok = slot % tile_tokens(HD);
     unsigned char* tile = pool + ((int64_t)page * nkv + kv) * page_bytes(HD) + slot / tile_tokens(HD) * TILE;
     if (key) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w |= ((codes >> (4 * e)) & 15u) << (4 * (e / 2 + 4 * (e % 2)));
-      *reinterpret_cast<uint32_t*>(tile + k_word<HD>(tok, j & 3, j >> 2)) = w;
+      *reinterpret_cast<uint32_t*>(tile + k_word<HD>(tok, j & 3, j >> 2)) = codes;
     } else {
       const int half = j >> 3, jj = j & 7;
       const uint32_t w = jj < 4 ? (codes & 0xffffu) | got << 16 : got | (codes & 0xffff0000u);
@@ -140,67 +169,60 @@ template <typename T> __device__ inline T c4_out(float v);
 template <> __device__ inline __nv_bfloat16 c4_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ inline __half c4_out<__half>(float v) { return __float2half_rn(fabsf(v) > 65504.0f ? copysignf(65504.0f, v) : v); }
 
-// Half of a page of a kv head, keys or values, to T [64][HD]: a thread per eight features.  CLEAN, for a product that multiplies hidden values by
-// zero: places from `held` on are zeros, and a token with a NaN among its values has zeros there and NaN in all of its key, which a mask can hide.
+// A page of a kv head, keys and values, to T [64][HD] each: a thread has eight features of both of a few tokens, and asks for all of their words
+// before it uses the first.  CLEAN, for a product that multiplies hidden values by zero: places from `held` on are zeros, and a token with a NaN
+// among its values has zeros there and NaN in all of its key, which a mask can hide.
 template <int HD, bool CLEAN, typename T>
-__device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool key, bool there, int held, T* __restrict__ out) {
-  constexpr int LANES = HD / 8;
+__device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool there, int held, T* __restrict__ k_out, T* __restrict__ v_out) {
+  constexpr int LANES = HD / 8, N = PAGE * LANES / C4_THREADS;
+  uint32_t kw[N], kc[N], vw[N], vc[N][2];
+  const int j = threadIdx.x % LANES, half = j >> 3, jj = j & 7;
 #pragma unroll
-  for (int r = threadIdx.x; r < PAGE * LANES; r += C4_THREADS) {
-    const int slot = r / LANES, j = r % LANES;
+  for (int i = 0; i < N; ++i) {
+    const int slot = (i * C4_THREADS + threadIdx.x) / LANES, tok = slot % tile_tokens(HD);
     const unsigned char* tile = base + slot / tile_tokens(HD) * TILE;
-    const int tok = slot % tile_tokens(HD);
-    const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(tile + (key ? K_WORDS : V_WORDS) + (tok * (HD / 32) + (j >> 2)) * 4));
-    uint32_t code[8];
-    if (key) {
-      const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(tile + k_word<HD>(tok, j & 3, j >> 2)));
+    auto word = [&](int at) { return __ldcg(reinterpret_cast<const uint32_t*>(tile + at)); };
+    kw[i] = word(K_WORDS + (tok * (HD / 32) + (j >> 2)) * 4);
+    vw[i] = word(V_WORDS + (tok * (HD / 32) + (j >> 2)) * 4);
+    kc[i] = word(k_word<HD>(tok, j & 3, j >> 2));
+    vc[i][0] = word(v_word<HD>(tok, half, 2 * (jj & 3)));
+    vc[i][1] = word(v_word<HD>(tok, half, 2 * (jj & 3) + 1));
+  }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) code[e] = (w >> (4 * (e / 2 + 4 * (e % 2)))) & 15u;
-    } else {
-      const int half = j >> 3, jj = j & 7;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(tile + v_word<HD>(tok, half, 2 * (jj & 3) + p))) >> (jj < 4 ? 0 : 16);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) code[4 * p + n] = (w >> (4 * n)) & 15u;
-      }
-    }
-    float f[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = there ? fmaf(word_sc(word), (float)code[e], word_mn(word)) : 0.0f;
+  for (int i = 0; i < N; ++i) {
+    const int slot = (i * C4_THREADS + threadIdx.x) / LANES;
+    bool hide_key = false, zero = !there;
     if (CLEAN) {
-      if (key) {
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(tile + V_WORDS + (tok * (HD / 32) + i) * 4));
-          nan = nan || !(fabsf(word_sc(w)) < __int_as_float(0x7f800000)) || !(fabsf(word_mn(w)) < __int_as_float(0x7f800000));
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = slot >= held ? 0.0f : nan ? __int_as_float(0x7fc00000) : f[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = slot >= held || !(fabsf(f[e]) < __int_as_float(0x7f800000)) ? 0.0f : f[e];
-      }
+      const bool nan = !(fabsf(word_sc(vw[i])) < __int_as_float(0x7f800000)) || !(fabsf(word_mn(vw[i])) < __int_as_float(0x7f800000));
+      const uint32_t of_token = ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
+      hide_key = (__ballot_sync(0xffffffffu, nan) & of_token) != 0;
+      zero = zero || slot >= held;
+      if (nan) vw[i] = vc[i][0] = vc[i][1] = 0;
     }
-    __align__(16) T v[8];
+    __align__(16) T k[8], v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c4_out<T>(f[e]);
-    *reinterpret_cast<uint4*>(out + slot * HD + 8 * j) = *reinterpret_cast<const uint4*>(v);
+    for (int e = 0; e < 8; ++e) {
+      const float x = fmaf(word_sc(kw[i]), c4_code(kc[i], 4 * (e / 2 + 4 * (e % 2))), word_mn(kw[i]));
+      const float y = fmaf(word_sc(vw[i]), c4_code(jj < 4 ? vc[i][e >> 2] : vc[i][e >> 2] >> 16, 4 * (e & 3)), word_mn(vw[i]));
+      k[e] = c4_out<T>(zero ? 0.0f : hide_key ? __int_as_float(0x7fc00000) : x);
+      v[e] = c4_out<T>(zero ? 0.0f : y);
+    }
+    *reinterpret_cast<uint4*>(k_out + slot * HD + 8 * j) = *reinterpret_cast<const uint4*>(k);
+    *reinterpret_cast<uint4*>(v_out + slot * HD + 8 * j) = *reinterpret_cast<const uint4*>(v);
   }
 }
 
-// Pages listed in `pages` to bfloat16 [n, nkv, 64, HD]: a block per (page, kv head) and keys or values.
+// Pages listed in `pages` to bfloat16 [n, nkv, 64, HD]: a block per (page, kv head).
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
 kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n_pages, int nkv,
                 __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out) {
   pdl_trigger();
   pdl_wait();
-  const int page = __ldcg(pages + blockIdx.x), kv = blockIdx.y >> 1;
-  const bool key = !(blockIdx.y & 1), there = page >= 0 && page < n_pages;
-  c4_unpack<HD, false>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), key, there, PAGE,
-                       (key ? k_out : v_out) + ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD);
+  const int page = __ldcg(pages + blockIdx.x), kv = blockIdx.y;
+  const bool there = page >= 0 && page < n_pages;
+  const int64_t at = ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD;
+  c4_unpack<HD, false>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), there, PAGE, k_out + at, v_out + at);
 }
 
 // The same to fp16 for the prompt attention, with the pages' own table (entry i: i, or -1 where there is no page, and nothing is written
@@ -214,15 +236,16 @@ kv4_unpack16_kernel(const unsigned char* __restrict__ pool, const int* __restric
                     __half* __restrict__ q_out, float* __restrict__ q_scale) {
   pdl_trigger();
   pdl_wait();
-  const int64_t page_blocks = (int64_t)n * nkv * 2;
+  const int64_t page_blocks = (int64_t)n * nkv;
   if (blockIdx.x < page_blocks) {
-    const int i = (int)(blockIdx.x / (2 * nkv)), y = (int)(blockIdx.x % (2 * nkv)), kv = y >> 1;
+    const int i = (int)(blockIdx.x / nkv), kv = (int)(blockIdx.x % nkv);
     const int page = __ldcg(pages + i);
     const bool there = page >= 0 && page < n_pages;
-    if (y == 0 && threadIdx.x == 0) table[i] = there ? i : -1;
+    if (kv == 0 && threadIdx.x == 0) table[i] = there ? i : -1;
     if (there) {
       const int row = i / width, held = __ldcg(row_pos0 + row) + __ldcg(row_start + row + 1) - __ldcg(row_start + row) - i % width * PAGE;
-      c4_unpack<HD, true>(pool + ((int64_t)page * nkv + kv) * page_bytes(HD), !(y & 1), true, held, ((y & 1) ? v_out : k_out) + ((int64_t)i * nkv + kv) * PAGE * HD);
+      const int64_t at = ((int64_t)i * nkv + kv) * PAGE * HD;
+      c4_unpack<HD, true>(pool + ((int64_t)page * nkv + kv) * page_bytes(HD), true, held, k_out + at, v_out + at);
     }
     return;
   }
@@ -288,13 +311,13 @@ extern "C" int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, 
 extern "C" int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
                              cudaStream_t stream) {
   if (n == 0) return 0;
-  if (n < 0 || nkv < 1 || nkv > 32767 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || !pool || !pages || !k_out || !v_out) {
+  if (n < 0 || nkv < 1 || nkv > 65535 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || !pool || !pages || !k_out || !v_out) {
     set_error("kv4_load: needs heads of 64 or 128 and all of its arrays, got %d pages, kv_heads=%d head_dim=%d", n, nkv, hd);
     return ERR_BAD_ARGUMENT;
   }
   if (!aligned16(pool) || !aligned16(k_out) || !aligned16(v_out)) { set_error("kv4_load: the pool and the results must be 16-byte aligned"); return ERR_ALIGNMENT; }
   auto go = [&](auto kernel) {
-    launch_pdl(kernel, dim3(n, 2 * nkv), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, (int)n_pages, nkv,
+    launch_pdl(kernel, dim3(n, nkv), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, (int)n_pages, nkv,
                static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out));
   };
   if (hd == 64) go(kv4_load_kernel<64>); else go(kv4_load_kernel<128>);
@@ -306,7 +329,7 @@ extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* p
                                  int* table, const void* q, int64_t q_stride, int T, int nh, void* q_out, float* q_scale, cudaStream_t stream) {
   if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
   const int per = C4_THREADS / (hd / 8), n = rows * width;
-  const int64_t blocks = (int64_t)n * nkv * 2 + ((int64_t)T * nh + per - 1) / per;
+  const int64_t blocks = (int64_t)n * nkv + ((int64_t)T * nh + per - 1) / per;
   if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
   auto go = [&](auto kernel) {
     launch_pdl(kernel, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, n, width, row_start, row_pos0, (int)n_pages,
