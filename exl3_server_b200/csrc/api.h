@@ -461,8 +461,8 @@ int exl3_kv4_page_bytes(int hd);
 // q, k, v [T, (nh + 2 nkv) * hd] bfloat16: q rotated into q_out [T, nh * hd], k (rotated) and v into the pages of the tokens' positions.  freq: hd / 2
 // frequencies (null: no rotation), freq_lo: what float32 lost of them, or null.
 int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float* freq, const float* freq_lo, const int* tok_pos,
-                   const int* tok_seq, const int* block_table, int bt_stride, void* pool, int64_t n_pages, int T, int nh, int nkv, int hd,
-                   cudaStream_t stream);
+                   const int* tok_seq, const int* block_table, int bt_stride, int bt_rows, int bt_width, void* pool, int64_t n_pages, int T, int nh,
+                   int nkv, int hd, cudaStream_t stream);
 // What the listed pages stand for, [n, nkv, 64, hd] bfloat16 each (zeros for a number that is no page's).
 int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
                   cudaStream_t stream);
@@ -479,8 +479,8 @@ int exl3_kv4_prompt_status();
 // row_pos0[r] ...; chunk: tiles of 4096 / hd keys that a block walks, max_chunks: chunks of the longest row (window's reach).
 long long exl3_kv4_attn_scratch(int rows, int max_new, int nh, int nkv, int hd, int max_chunks);
 int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
-                  const int* row_start, const int* row_pos0, int rows, int max_new, int nh, int nkv, int hd, int window, float scale,
-                  int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream);
+                  int bt_width, const int* row_start, const int* row_pos0, int rows, int T, int max_new, int nh, int nkv, int hd, int window,
+                  float scale, int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream);
 // Code left by a bounded wait that ran out (0: none); cleared by the call.
 int exl3_kv4_attn_status();
 // 8-bit floating point (e4m3, fp8.cuh): w codes [N, K] with scales sw [ceil(N / 128), ceil(K / 128)], x bfloat16 rounded to codes with a scale per row
@@ -492,6 +492,9 @@ int exl3_fp8_skinny(const void* x, int64_t ldx, const float* sx, const void* w, 
                     int N, int K, int gated, cudaStream_t stream);
 int exl3_fp8_wide(const void* codes, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M, int N,
                   int K, int gated, cudaStream_t stream);
+// Any number of rows; codes and sx: scratch for the rounding from 17 rows on.
+int exl3_fp8_linear(const void* x, int64_t ldx, void* codes, float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype,
+                    int M, int N, int K, int gated, int few, cudaStream_t stream);
 // Codes left by bounded waits that ran out (0: none); cleared by the calls.
 int exl3_fp8_skinny_status();
 int exl3_fp8_wide_status();

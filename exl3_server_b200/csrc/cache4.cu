@@ -79,8 +79,8 @@ template <int HD, int TOK>
 __global__ void __launch_bounds__(C4_THREADS)
 kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv_bfloat16* __restrict__ q_out,
                  const float* __restrict__ freq, const float* __restrict__ freq_lo, const int* __restrict__ tok_pos,
-                 const int* __restrict__ tok_seq, const int* __restrict__ block_table, int bt_stride, unsigned char* __restrict__ pool,
-                 int n_pages, int T, int nh, int nkv) {
+                 const int* __restrict__ tok_seq, const int* __restrict__ block_table, int bt_stride, int bt_rows, int bt_width,
+                 unsigned char* __restrict__ pool, int n_pages, int T, int nh, int nkv) {
   constexpr int LANES = HD / 8, HEADS = C4_THREADS / LANES;           // pairs that the block works on side by side
   __shared__ __align__(16) float s_cos[TOK][HD / 2], s_sin[TOK][HD / 2];
   __shared__ int s_pos[TOK], s_page[TOK];
@@ -102,9 +102,10 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv
   uint4 own, other;
   ask(tk, head, own, other);
   if (threadIdx.x < n_tok) {
-    const int pos = __ldcg(tok_pos + t0 + threadIdx.x);
+    const int pos = __ldcg(tok_pos + t0 + threadIdx.x), seq = __ldcg(tok_seq + t0 + threadIdx.x);
     s_pos[threadIdx.x] = pos;
-    s_page[threadIdx.x] = pos >= 0 ? __ldcg(block_table + (int64_t)__ldcg(tok_seq + t0 + threadIdx.x) * bt_stride + pos / PAGE) : -1;
+    const bool there = pos >= 0 && pos / PAGE < bt_width && seq >= 0 && seq < bt_rows;
+    s_page[threadIdx.x] = there ? __ldcg(block_table + (int64_t)seq * bt_stride + pos / PAGE) : -1;
   }
   if (freq)
     for (int d = threadIdx.x; d < n_tok * (HD / 2); d += C4_THREADS)
@@ -285,10 +286,10 @@ using namespace exl3;
 extern "C" int exl3_kv4_page_bytes(int hd) { return hd == 64 || hd == 128 ? kv4::page_bytes(hd) : 0; }
 
 extern "C" int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float* freq, const float* freq_lo, const int* tok_pos,
-                              const int* tok_seq, const int* block_table, int bt_stride, void* pool, int64_t n_pages, int T, int nh, int nkv,
-                              int hd, cudaStream_t stream) {
+                              const int* tok_seq, const int* block_table, int bt_stride, int bt_rows, int bt_width, void* pool, int64_t n_pages, int T,
+                              int nh, int nkv, int hd, cudaStream_t stream) {
   if (T == 0) return 0;
-  if (T < 0 || nh < 1 || nkv < 1 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || bt_stride < 1 || !qkv || !q_out ||
+  if (T < 0 || nh < 1 || nkv < 1 || (hd != 64 && hd != 128) || n_pages < 1 || n_pages > INT32_MAX || bt_rows < 1 || bt_width < 1 || !qkv || !q_out ||
       !tok_pos || !tok_seq || !block_table || !pool) {
     set_error("kv4_store: needs heads of 64 or 128 and all of its arrays, got T=%d heads=%d kv_heads=%d head_dim=%d", T, nh, nkv, hd);
     return ERR_BAD_ARGUMENT;
@@ -300,7 +301,7 @@ extern "C" int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, 
   const int gy = many ? 1 : T >= 296 ? 1 : rounds < 32 ? rounds : 32;
   auto go = [&](auto kernel) {
     launch_pdl(kernel, dim3(many ? ceil_div(T, 4) : T, gy), dim3(C4_THREADS), 0, stream, static_cast<const __nv_bfloat16*>(qkv), qkv_stride,
-               static_cast<__nv_bfloat16*>(q_out), freq, freq_lo, tok_pos, tok_seq, block_table, bt_stride, static_cast<unsigned char*>(pool),
+               static_cast<__nv_bfloat16*>(q_out), freq, freq_lo, tok_pos, tok_seq, block_table, bt_stride, bt_rows, bt_width, static_cast<unsigned char*>(pool),
                (int)n_pages, T, nh, nkv);
   };
   if (hd == 64) { if (many) go(kv4_store_kernel<64, 4>); else go(kv4_store_kernel<64, 1>); }

@@ -327,3 +327,13 @@ extern "C" int exl3_fp8_wide(const void* codes, const float* sx, const void* w, 
   launch_pdl(fp8_wide_kernel, dim3(tiles < sms ? tiles : sms), dim3(F8W_THREADS), F8W_SMEM, stream, map_x, map_w, a);
   return launch_status("fp8_wide");
 }
+
+// The product of any number of rows: `few` picks the weight-streaming kernel; from 17 rows on x is rounded into codes [M, K] and sx [blocks, M] first.
+extern "C" int exl3_fp8_linear(const void* x, int64_t ldx, void* codes, float* sx, const void* w, const float* sw, const void* bias, void* y,
+                               int out_dtype, int M, int N, int K, int gated, int few, cudaStream_t stream) {
+  if (few && M <= 16) return exl3_fp8_skinny(x, ldx, nullptr, w, sw, bias, y, out_dtype, M, N, K, gated, stream);
+  const int rc = exl3_fp8_quantize(x, ldx, M, K, codes, sx, 1, stream);
+  if (rc) return rc;
+  return few ? exl3_fp8_skinny(codes, K, sx, w, sw, bias, y, out_dtype, M, N, K, gated, stream)
+             : exl3_fp8_wide(codes, sx, w, sw, bias, y, out_dtype, M, N, K, gated, stream);
+}

@@ -1864,6 +1864,9 @@ def kv4_pool(pages: int, kv_heads: int, head_dim: int, device) -> torch.Tensor:
 
 
 def _kv4_check_pool(pool: torch.Tensor, kv_heads: Optional[int], head_dim: int, what: str) -> None:
+    if pool.dtype is torch.uint8 and head_dim in (64, 128) and pool.shape[1:] == (pool.shape[1] if kv_heads is None else kv_heads, 80 * head_dim) \
+            and pool.is_contiguous():
+        return
     if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != kv4_page_bytes(head_dim) or \
             (kv_heads is not None and pool.shape[1] != kv_heads):
         raise KernelLibraryError(f"{what}: the pool must be uint8 [pages, kv_heads, {kv4_page_bytes(head_dim)}], got "
@@ -1872,12 +1875,15 @@ def _kv4_check_pool(pool: torch.Tensor, kv_heads: Optional[int], head_dim: int, 
 
 
 def _int32(t: torch.Tensor, name: str, what: str) -> None:
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise KernelLibraryError(f"{what}: {name} must be int32, got {t.dtype}")
-    _contig(t, name)
+    if not t.is_contiguous():
+        raise KernelLibraryError(f"{what}: {name} must be contiguous")
 
 
 def _table(t: torch.Tensor, rows: Optional[int], what: str) -> None:
+    if t.dtype is torch.int32 and t.is_contiguous() and t.dim() == 2 and (rows is None or t.shape[0] >= rows):
+        return
     if t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (rows is not None and t.shape[0] < rows):
         raise KernelLibraryError(f"{what}: the block table must be int32 [rows, pages]")
 
@@ -1889,7 +1895,7 @@ def kv4_store(qkv: torch.Tensor, inv_freq: Optional[torch.Tensor], tok_pos: torc
     ``inv_freq`` as in ``rotary_table``, None: no rotation), rounds the rotated keys and the values to 4 bits into the
     tokens' places in ``pool`` and returns the rotated queries ``[T, heads * head_dim]``.  ``qkv`` stays as it is.  A token whose position is
     negative or whose page is not there is not stored."""
-    T = qkv.shape[0]
+    T = qkv.shape[0] if qkv.dim() else 0
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * kv_heads) * head_dim or qkv.stride(1) != 1:
         raise KernelLibraryError(f"kv4_store: qkv must be bfloat16 [tokens, {(heads + 2 * kv_heads) * head_dim}], got {qkv.dtype} {tuple(qkv.shape)}")
     _kv4_check_pool(pool, kv_heads, head_dim, "kv4_store")
@@ -1906,12 +1912,12 @@ def kv4_store(qkv: torch.Tensor, inv_freq: Optional[torch.Tensor], tok_pos: torc
         hi = _addr(inv_freq)
         lo = hi + 4 * half if inv_freq.dim() == 2 else 0
     if out is None:
-        out = torch.empty((T, heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
+        out = qkv.new_empty((T, heads * head_dim))
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
         raise KernelLibraryError(f"kv4_store: out must be contiguous bfloat16 {(T, heads * head_dim)}")
-    rc = _entry("exl3_kv4_store", "plppppppipliiii")(
-        _addr(qkv), qkv.stride(0), _addr(out), hi, lo, _addr(tok_pos), _addr(tok_seq), _addr(block_table), block_table.stride(0),
-        _addr(pool), pool.shape[0], T, heads, kv_heads, head_dim, _raw_stream())
+    rc = _entry("exl3_kv4_store", "plppppppiiipliiii")(
+        _addr(qkv), qkv.stride(0), out.data_ptr(), hi, lo, _addr(tok_pos), _addr(tok_seq), _addr(block_table), block_table.stride(0),
+        *block_table.shape, _addr(pool), pool.shape[0], T, heads, kv_heads, head_dim, _raw_stream())
     if rc:
         _check(rc, "kv4_store")
     return out
@@ -1977,8 +1983,8 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
 
     A few tokens a row (``KV4_FEW_COLUMNS``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
     unpacked to fp16 (values beyond 65,504 count as that) and go through the tcgen05 attention."""
-    T = q.shape[0]
-    if q.dtype != torch.bfloat16 or q.dim() != 2 or q.shape[1] != heads * head_dim or q.stride(1) != 1:
+    T = q.shape[0] if q.dim() else 0
+    if q.dtype is not torch.bfloat16 or q.dim() != 2 or q.shape[1] != heads * head_dim or q.stride(1) != 1:
         raise KernelLibraryError(f"kv4_attn: q must be bfloat16 [tokens, {heads * head_dim}], got {q.dtype} {tuple(q.shape)}")
     if kv_heads < 1 or heads % kv_heads or window < 0 or max_new < 0 or max_len < 0:
         raise KernelLibraryError(f"kv4_attn: {heads} heads on {kv_heads}, window {window}, max_new {max_new}, max_len {max_len}")
@@ -1993,7 +1999,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         raise KernelLibraryError("kv4_attn: without row_start every row has one token")
     _table(block_table, rows, "kv4_attn")
     if out is None:
-        out = torch.empty((T, heads * head_dim), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, heads * head_dim))
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
         raise KernelLibraryError(f"kv4_attn: out must be contiguous bfloat16 {(T, heads * head_dim)}")
     if T == 0 or rows == 0:
@@ -2010,9 +2016,9 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     if chunks > 1:
         need = rows * kv_heads * groups * chunks * columns * (head_dim + 4)
         scratch = workspace.plain(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
-    rc = _entry("exl3_kv4_attn", "plpplpippiiiiiifiipl")(
-        _addr(q), q.stride(0), _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), _addr(row_start),
-        _addr(row_pos0), rows, max_new, heads, kv_heads, head_dim, window, scale, chunk, chunks, _addr(scratch), need, _raw_stream())
+    rc = _entry("exl3_kv4_attn", "plpplpiippiiiiiiifiipl")(
+        _addr(q), q.stride(0), _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), block_table.shape[1],
+        _addr(row_start), _addr(row_pos0), rows, T, max_new, heads, kv_heads, head_dim, window, scale, chunk, chunks, _addr(scratch), need, _raw_stream())
     if rc:
         _check(rc, "kv4_attn")
     return out
@@ -2116,7 +2122,7 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     features, and so on, and ``silu(gate) * up`` comes out (N / 2 wide, no bias)."""
     _fp8_check_x(x, "fp8_linear")
     M, Kd = x.shape
-    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.shape[1] != Kd:
+    if w.dtype is not torch.float8_e4m3fn or w.dim() != 2 or w.shape[1] != Kd:
         raise KernelLibraryError(f"fp8_linear: w must be float8_e4m3fn [features out, {Kd}], got {w.dtype} {tuple(w.shape)}")
     N = w.shape[0]
     _contig(w, "w")
@@ -2130,26 +2136,20 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
         raise KernelLibraryError(f"fp8_linear: bias must be bfloat16 [{N}]")
     shape = (M, N // 2 if gated else N)
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=x.device)
+        out = x.new_empty(shape) if out_dtype is torch.bfloat16 else torch.empty(shape, dtype=out_dtype, device=x.device)
     elif tuple(out.shape) != shape or not out.is_contiguous():
         raise KernelLibraryError(f"fp8_linear: out must be contiguous {shape}")
     code = dtype_code(out.dtype)
     if M == 0:
         return out
     few = _fp8_few(M, N, sm_count(x.device))
-    codes = sx = None
-    if M > FP8_ROUNDED_ROWS:
-        codes = torch.empty((M, Kd), dtype=torch.uint8, device=x.device)
-        sx = torch.empty((blocks, M), dtype=torch.float32, device=x.device)
-        _fp8_round(x, codes, sx, 1)
-    if few:
-        rc = _entry("exl3_fp8_skinny", "plpppppiiiii")(_addr(x if codes is None else codes), x.stride(0), _addr(sx), _addr(w), _addr(w_scale), _addr(bias),
-                                                       _addr(out), code, M, N, Kd, 1 if gated else 0, _raw_stream())
-        if rc:
-            _check(rc, "fp8_skinny")
-        return out
-    rc = _entry("exl3_fp8_wide", "ppppppiiiii")(_addr(codes), _addr(sx), _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
-                                                1 if gated else 0, _raw_stream())
+    codes = sx = 0
+    if M > FP8_ROUNDED_ROWS or not few:
+        room = x.new_empty(M * Kd // 2 + 2 * blocks * M + 8)               # codes, then (16-byte aligned) scales
+        codes = room.data_ptr()
+        sx = codes + -(-M * Kd // 16) * 16
+    rc = _entry("exl3_fp8_linear", "plppppppiiiiii")(_addr(x), x.stride(0), codes, sx, _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
+                                                     1 if gated else 0, 1 if few else 0, _raw_stream())
     if rc:
-        _check(rc, "fp8_wide")
+        _check(rc, "fp8_linear")
     return out
