@@ -16,8 +16,8 @@
 // Up to four columns, hi and lo stand side by side in the 8 columns of one instruction and meet in the thread that gets both; more columns
 // take an instruction each.
 //
-// Values: with p the softmax's terms, P_g = p * sc_g * F in fp16 (F a power of two that keeps the largest scale seen so far at 2^14, carried by p's
-// exponent: the probabilities keep their 11 bits down to 2^-28 of the largest) is the second product's operand, the codes of 16 tokens the 16-row
+// Values: with p the softmax's terms against a reference that follows the maximum lazily (p at most 2^8), P_g = p * sc_g * F in fp16 (F a power of two
+// that keeps the largest scale seen so far below 2^6, carried by p's exponent: the probabilities keep their 11 bits down to 2^-20 of the largest) is the second product's operand, the codes of 16 tokens the 16-row
 // one, and sum p mn_g goes beside it in float32.  Scores, maximum, sums and outputs are float32.
 //
 // A column is a (new token, query head) of one key/value head: up to 8 or 16 columns share a walk over the codes, each with its own causal limit.
@@ -39,6 +39,8 @@ constexpr int A4_WARPS = 4;
 constexpr int A4_STAGES = 2;
 constexpr int A4_MAX_CHUNK = 32 * A4_WARPS;               // tiles: a warp keeps its page numbers one a lane
 constexpr uint32_t A4_WAIT_LIMIT = 1u << 20;              // looks of up to a microsecond each: a second
+
+constexpr float A4_SLACK = 8.0f;                          // base-2 units that a score may lie above its column's reference
 
 static __device__ int g_a4_error = 0;
 
@@ -269,7 +271,7 @@ kv4_attn_kernel(const A4Args a) {
 
   float o[NC][NG][2][4] = {};                               // [column block][group][features 4 g + 2 k (+ 1)] x columns 2 t, 2 t + 1, in units of 2^-24
   float om[NC][NG][CP] = {};                                // sum p mn, this lane's tokens
-  float m[NC][CP], ref[NC][CP], l[NC][CP] = {};
+  float m[NC][CP], ref[NC][CP], mm[NC][CP] = {}, l[NC][CP] = {};       // mm: ref, or 0 while nothing was seen
 #pragma unroll
   for (int n = 0; n < NC; ++n)
 #pragma unroll
@@ -332,20 +334,7 @@ kv4_attn_kernel(const A4Args a) {
             }
           }
     }
-    // the running maximum of a column, over the lanes that share it
-    float next[NC][CP];
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-      for (int h = 0; h < CP; ++h) {
-        float v = x[0][n][0][h];
-#pragma unroll
-        for (int mt = 0; mt < NT; ++mt) v = fmaxf(v, fmaxf(x[mt][n][0][h], x[mt][n][1][h]));
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-        next[n][h] = fmaxf(m[n][h], v);
-      }
-    // the values' numbers, and the power of two that keeps the largest scale in fp16's range
+    // the values' numbers
     uint32_t vw[NT][2][NG];
     uint32_t top = 0;
 #pragma unroll
@@ -363,39 +352,49 @@ kv4_attn_kernel(const A4Args a) {
 #pragma unroll
         for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i]);
       }
-    top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
-    if (top == 0x7f800000u) {                               // NaN groups do not count (nor does what lies behind the last token)
-      top = 0;
-#pragma unroll
-      for (int mt = 0; mt < NT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i] < 0x7f800000u ? vw[mt][h][i] : 0u);
-      top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
-    }
-    if (top > sc_top) {                                     // (the same for the whole warp)
-      sc_top = top;
-      up = (float)min(max(13 - ((int)(top >> 23) - 127), -100), 100);
-    }
-    // p = 2^(x - ref): ref is the maximum less the exponent that the values' scales want, so p carries F and nothing else has to
-    float mm[NC][CP];
-    bool moved = false;
+    // A column's reference moves only when one of its scores is more than 2^8 above it, the scales' power of two only when a larger scale comes:
+    // each lane looks at what it has, one vote tells, and nothing is exchanged otherwise.
+    float best[NC][CP];                                     // this lane's largest score of a column
+    bool behind = (top & 0x7f800000u) > sc_top;
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int h = 0; h < CP; ++h) {
-        m[n][h] = next[n][h];
-        mm[n][h] = next[n][h] - up;                         // (-inf stays)
-        moved = moved || mm[n][h] != ref[n][h];
+        float v = x[0][n][0][h];
+#pragma unroll
+        for (int mt = 0; mt < NT; ++mt) v = fmaxf(v, fmaxf(x[mt][n][0][h], x[mt][n][1][h]));
+        best[n][h] = v;
+        behind = behind || v > ref[n][h] + (up + A4_SLACK);
       }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, behind)) {
+      top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
+      if (top == 0x7f800000u) {                             // NaN groups do not count (nor does what lies behind the last token)
+        top = 0;
+#pragma unroll
+        for (int mt = 0; mt < NT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i] < 0x7f800000u ? vw[mt][h][i] : 0u);
+        top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
+      }
+      if (top > sc_top) {
+        sc_top = top;
+        up = (float)min(max(5 - ((int)(top >> 23) - 127), -100), 100);
+      }
+      // p = 2^(x - ref): ref is the maximum less the exponent that the values' scales want, so p carries F and nothing else has to
 #pragma unroll
       for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int h = 0; h < CP; ++h) {
-          const float f = ref[n][h] == mm[n][h] ? 1.0f : a4_exp2(ref[n][h] - mm[n][h]);
-          ref[n][h] = mm[n][h];
+          float v = best[n][h];
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+          m[n][h] = fmaxf(m[n][h], v);
+          const float now = m[n][h] - up;                   // (-inf stays)
+          const float f = ref[n][h] == now ? 1.0f : a4_exp2(ref[n][h] - now);
+          ref[n][h] = now;
+          mm[n][h] = now == __int_as_float(0xff800000) ? 0.0f : now;
           l[n][h] *= f;
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
@@ -405,10 +404,6 @@ kv4_attn_kernel(const A4Args a) {
           }
         }
     }
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-      for (int h = 0; h < CP; ++h) mm[n][h] = ref[n][h] == __int_as_float(0xff800000) ? 0.0f : ref[n][h];
 #pragma unroll
     for (int mt = 0; mt < NT; ++mt) {
       uint32_t pb[NC][NG][2];                               // P_g, tokens x columns, transposed
