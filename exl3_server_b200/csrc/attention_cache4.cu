@@ -175,9 +175,15 @@ kv4_attn_kernel(const A4Args a) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   __syncwarp();
+  // Tiles that every column sees as a whole come first, then those that a limit cuts: the two kinds have code of their own, and going to and fro
+  // between them costs a tile some eighty moves of registers.
+  const int full_hi = r.pos0 + r.col0 / r.G;                // keys that every column sees: full_lo .. full_hi
+  const int full_lo = a.window > 0 ? r.pos0 + (r.col0 + r.cols - 1) / r.G - a.window + 1 : 0;
+  const int key_lane = (tile_a + warp + A4_WARPS * lane) * TT;
+  const uint32_t whole = __ballot_sync(0xffffffffu, my_page >= 0 && key_lane + TT - 1 <= full_hi && key_lane >= full_lo);
   auto request = [&](int stage) {                           // the next tile of `ask` into a stage
-    const int i = __ffs(ask) - 1;
-    ask &= ask - 1;
+    const int i = __ffs((ask & whole) ? ask & whole : ask) - 1;
+    ask &= ~(1u << i);
     const int page = __shfl_sync(0xffffffffu, my_page, i);
     const int tile = tile_a + warp + A4_WARPS * i;
     const unsigned char* src = a.pool + ((int64_t)page * a.nkv + kvh) * page_bytes(HD) + tile % SPP * TILE;
@@ -265,10 +271,6 @@ kv4_attn_kernel(const A4Args a) {
       limit[n][h] = c < r.cols ? r.pos0 + (r.col0 + c) / r.G : -1;
     }
   }
-  // keys that every column sees: full_lo .. full_hi
-  const int full_hi = r.pos0 + r.col0 / r.G;
-  const int full_lo = a.window > 0 ? r.pos0 + (r.col0 + r.cols - 1) / r.G - a.window + 1 : 0;
-
   float o[NC][NG][2][4] = {};                               // [column block][group][features 4 g + 2 k (+ 1)] x columns 2 t, 2 t + 1, in units of 2^-24
   float om[NC][NG][CP] = {};                                // sum p mn, this lane's tokens
   float m[NC][CP], ref[NC][CP], mm[NC][CP] = {}, l[NC][CP] = {};       // mm: ref, or 0 while nothing was seen
@@ -453,20 +455,21 @@ kv4_attn_kernel(const A4Args a) {
 
   bool ok = true;
   int k = 0;
-  while (todo) {
-    const int i = __ffs(todo) - 1, stage = k % A4_STAGES;
-    todo &= todo - 1;
-    ok = __all_sync(0xffffffffu, a4_wait(bars + stage, (k / A4_STAGES) & 1));
-    if (!ok) break;
-    const int key0 = (tile_a + warp + A4_WARPS * i) * TT;
-    const unsigned char* buf = ring + stage * TILE;
-    if (key0 + TT - 1 <= full_hi && key0 >= full_lo) walk(buf, key0, std::false_type());
-    else walk(buf, key0, std::true_type());
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // this lane's reads come before the copy that follows
-    __syncwarp();
-    if (ask) request(stage);
-    ++k;
-  }
+  auto tiles = [&](uint32_t todo, auto masked_t) {
+    while (todo && ok) {
+      const int i = __ffs(todo) - 1, stage = k % A4_STAGES;
+      todo &= todo - 1;
+      ok = __all_sync(0xffffffffu, a4_wait(bars + stage, (k / A4_STAGES) & 1));
+      if (!ok) break;
+      walk(ring + stage * TILE, (tile_a + warp + A4_WARPS * i) * TT, masked_t);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // this lane's reads come before the copy that follows
+      __syncwarp();
+      if (ask) request(stage);
+      ++k;
+    }
+  };
+  tiles(todo & whole, std::false_type());
+  tiles(todo & ~whole, std::true_type());
   if (!ok) {
     // copies still on their way get the time to land before this shared memory is used again
     if (lane == 0) atomicExch(&g_a4_error, 1);
