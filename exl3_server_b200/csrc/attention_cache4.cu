@@ -17,7 +17,7 @@
 // take an instruction each.
 //
 // Values: with p the softmax's terms against a reference that follows the maximum lazily (p at most 2^8), P_g = p * sc_g * F in fp16 (F a power of two
-// that keeps the largest scale seen so far below 2^6, carried by p's exponent: the probabilities keep their 11 bits down to 2^-20 of the largest) is the second product's operand, the codes of 16 tokens the 16-row
+// that keeps the largest scale seen so far below 2^6, carried by p's exponent: p sc keeps its 11 bits down to 2^-20 of the largest) is the second product's operand, the codes of 16 tokens the 16-row
 // one, and sum p mn_g goes beside it in float32.  Scores, maximum, sums and outputs are float32.
 //
 // A column is a (new token, query head) of one key/value head: up to 8 or 16 columns share a walk over the codes, each with its own causal limit.
@@ -87,6 +87,11 @@ __device__ inline float a4_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ inline float a4_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ inline uint32_t a4_pack(float lo, float hi) {
   uint32_t r;
@@ -179,6 +184,8 @@ kv4_attn_kernel(const A4Args a) {
   // between them costs a tile some eighty moves of registers.
   const int full_hi = r.pos0 + r.col0 / r.G;                // keys that every column sees: full_lo .. full_hi
   const int full_lo = a.window > 0 ? r.pos0 + (r.col0 + r.cols - 1) / r.G - a.window + 1 : 0;
+  const int seen_hi = r.pos0 + (r.col0 + r.cols - 1) / r.G;              // keys that any column sees
+  const int seen_lo = a.window > 0 ? r.pos0 + r.col0 / r.G - a.window + 1 : 0;
   const int key_lane = (tile_a + warp + A4_WARPS * lane) * TT;
   const uint32_t whole = __ballot_sync(0xffffffffu, my_page >= 0 && key_lane + TT - 1 <= full_hi && key_lane >= full_lo);
   auto request = [&](int stage) {                           // the next tile of `ask` into a stage
@@ -338,7 +345,7 @@ kv4_attn_kernel(const A4Args a) {
     }
     // the values' numbers
     uint32_t vw[NT][2][NG];
-    uint32_t top = 0;
+    float top_word = 0.0f;                                  // the largest word, as the float it is: its scale (NaN groups do not count)
 #pragma unroll
     for (int mt = 0; mt < NT; ++mt)
 #pragma unroll
@@ -351,35 +358,33 @@ kv4_attn_kernel(const A4Args a) {
           const uint4 v = *reinterpret_cast<const uint4*>(pp);
           vw[mt][h][0] = v.x; vw[mt][h][1] = v.y; vw[mt][h][2] = v.z; vw[mt][h][3] = v.w;
         }
+        if (MASKED) {                                       // what no column sees has no say in the scales' power of two
+          const int key = key0 + mt * 16 + g + 8 * h;
+          if (key > seen_hi || key < seen_lo) {
 #pragma unroll
-        for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i]);
+            for (int i = 0; i < NG; ++i) vw[mt][h][i] = 0;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NG; i += 2) top_word = a4_max3(top_word, __uint_as_float(vw[mt][h][i]), __uint_as_float(vw[mt][h][i + 1]));
       }
     // A column's reference moves only when one of its scores is more than 2^8 above it, the scales' power of two only when a larger scale comes:
     // each lane looks at what it has, one vote tells, and nothing is exchanged otherwise.
     float best[NC][CP];                                     // this lane's largest score of a column
-    bool behind = (top & 0x7f800000u) > sc_top;
+    uint32_t top = __float_as_uint(top_word) & 0x7f800000u;
+    bool behind = top > sc_top;
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int h = 0; h < CP; ++h) {
-        float v = x[0][n][0][h];
+        float v = __int_as_float(0xff800000);
 #pragma unroll
-        for (int mt = 0; mt < NT; ++mt) v = fmaxf(v, fmaxf(x[mt][n][0][h], x[mt][n][1][h]));
+        for (int mt = 0; mt < NT; ++mt) v = a4_max3(v, x[mt][n][0][h], x[mt][n][1][h]);
         best[n][h] = v;
         behind = behind || v > ref[n][h] + (up + A4_SLACK);
       }
     if (__any_sync(0xffffffffu, behind)) {
-      top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
-      if (top == 0x7f800000u) {                             // NaN groups do not count (nor does what lies behind the last token)
-        top = 0;
-#pragma unroll
-        for (int mt = 0; mt < NT; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < NG; ++i) top = max(top, vw[mt][h][i] < 0x7f800000u ? vw[mt][h][i] : 0u);
-        top = __reduce_max_sync(0xffffffffu, top) & 0x7f800000u;
-      }
+      top = __reduce_max_sync(0xffffffffu, top);
       if (top > sc_top) {
         sc_top = top;
         up = (float)min(max(5 - ((int)(top >> 23) - 127), -100), 100);
@@ -402,13 +407,17 @@ kv4_attn_kernel(const A4Args a) {
           for (int i = 0; i < NG; ++i) {
             om[n][i][h] *= f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) { o[n][i][k][h] *= f; o[n][i][k][h + 2] *= f; }
+            for (int k = 0; k < 2; ++k) {
+              const int at = SIDE ? i & 1 : h;              // where this column's values of the group are
+              o[n][i][k][at] *= f;
+              o[n][i][k][at + 2] *= f;
+            }
           }
         }
     }
 #pragma unroll
     for (int mt = 0; mt < NT; ++mt) {
-      uint32_t pb[NC][NG][2];                               // P_g, tokens x columns, transposed
+      uint32_t pb[NC][SIDE ? NG / 2 : NG][2];               // P_g, tokens x columns, transposed
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         float p[2][CP];
@@ -419,21 +428,23 @@ kv4_attn_kernel(const A4Args a) {
             p[h][c] = a4_exp2(x[mt][n][h][c] - mm[n][c]);
             l[n][c] += p[h][c];
           }
+        // Side by side the 8 columns have room for two groups' P: the even ones the first group's, the odd ones the second's; of a group's product
+        // the other's columns are dropped.
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
+        for (int i = 0; i < NG; i += SIDE ? 2 : 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float sc = word_sc(vw[mt][h][i]), mn = word_mn(vw[mt][h][i]);
-            float w[2] = {};                                // (side by side: the odd columns stay empty)
+            float w[2];
 #pragma unroll
-            for (int c = 0; c < CP; ++c) {
-              if (MASKED && x[mt][n][h][c] == __int_as_float(0xff800000)) continue;       // what is hidden may hold anything
-              w[c] = p[h][c] * sc;
-              om[n][i][c] = fmaf(p[h][c], mn, om[n][i][c]);
+            for (int c = 0; c < 2; ++c) {
+              const int gi = SIDE ? i + c : i, col = SIDE ? 0 : c;
+              const float sc = word_sc(vw[mt][h][gi]), mn = word_mn(vw[mt][h][gi]);
+              const bool hidden = MASKED && x[mt][n][h][col] == __int_as_float(0xff800000);        // what is hidden may hold anything
+              w[c] = hidden ? 0.0f : p[h][col] * sc;
+              if (!hidden) om[n][gi][col] = fmaf(p[h][col], mn, om[n][gi][col]);
             }
-            pb[n][i][h] = a4_transpose(a4_pack(w[0], w[1]));
+            pb[n][SIDE ? i / 2 : i][h] = a4_transpose(a4_pack(w[0], w[1]));
           }
-        }
       }
 #pragma unroll
       for (int half = 0; half < NG / 2; ++half) {
@@ -442,11 +453,11 @@ kv4_attn_kernel(const A4Args a) {
         for (int part = 0; part < 2; ++part) {
           const uint32_t lo = __byte_perm(v.x, v.y, part ? 0x7632 : 0x5410), hi = __byte_perm(v.z, v.w, part ? 0x7632 : 0x5410);
           const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
-          const int i = half * 2 + part;
+          const int i = half * 2 + part, ip = SIDE ? half : i;
 #pragma unroll
           for (int n = 0; n < NC; ++n) {
-            a4_mma(o[n][i][0], lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u, pb[n][i][0], pb[n][i][1]);
-            a4_mma(o[n][i][1], lo8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x000f000fu, hi8 & 0x00f000f0u, pb[n][i][0], pb[n][i][1]);
+            a4_mma(o[n][i][0], lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u, pb[n][ip][0], pb[n][ip][1]);
+            a4_mma(o[n][i][1], lo8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x000f000fu, hi8 & 0x00f000f0u, pb[n][ip][0], pb[n][ip][1]);
           }
         }
       }
@@ -495,10 +506,11 @@ kv4_attn_kernel(const A4Args a) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
         float4 y;
-        y.x = fmaf(o[n][i][0][h], unit, s);
-        y.y = fmaf(o[n][i][0][h + 2], unit * 0.0625f, s);
-        y.z = fmaf(o[n][i][1][h], unit, s);
-        y.w = fmaf(o[n][i][1][h + 2], unit * 0.0625f, s);
+        const int at = SIDE ? i & 1 : h;
+        y.x = fmaf(o[n][i][0][at], unit, s);
+        y.y = fmaf(o[n][i][0][at + 2], unit * 0.0625f, s);
+        y.z = fmaf(o[n][i][1][at], unit, s);
+        y.w = fmaf(o[n][i][1][at + 2], unit * 0.0625f, s);
         *reinterpret_cast<float4*>(mine + c * HD + i * 32 + 4 * g) = y;
       }
     }

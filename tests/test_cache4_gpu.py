@@ -282,6 +282,20 @@ def test_a_group_of_values_that_is_nan_stays_in_its_features():
     assert float(err.max()) <= 2.0 ** -7 * float(c.v[0].abs().max())
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (8, 1, 128), (32, 2, 64)])
+@pytest.mark.parametrize("new,window", [(1, 0), (2, 30), (90, 0)])
+def test_what_lies_in_unused_places_does_not_matter(heads, kv_heads, d, new, window):
+    """Places behind the last token, and before the window, hold keys and values of 1e30."""
+    c = Case([(100, new)], heads, kv_heads, d, seed=16)
+    want = c.run(window)
+    n = 100 + new
+    width = (heads + 2 * kv_heads) * d
+    places = list(range(n, c.table.shape[1] * 64)) + (list(range(0, 100 - 30 + 1 - 1)) if window else [])
+    huge = (torch.randn(len(places), width, device=DEV) * 1e30).bfloat16()
+    K().kv4_store(huge, None, ints(places), ints([0] * len(places)), c.table, c.pool, heads, kv_heads, d)
+    assert torch.equal(c.run(window), want)
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 @pytest.mark.parametrize("new", [1, 80])
 def test_queries_that_are_not_finite(value, new):
