@@ -1842,6 +1842,11 @@ def _addr(t: Optional[torch.Tensor]) -> int:
     return t.data_ptr()
 
 
+def _sms(t: torch.Tensor) -> int:
+    """``sm_count`` of a tensor's device."""
+    return _SM_COUNT.get(t.get_device()) or sm_count(t.device)
+
+
 def _raw_stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
@@ -1863,15 +1868,16 @@ def kv4_pool(pages: int, kv_heads: int, head_dim: int, device) -> torch.Tensor:
     return torch.zeros((pages, kv_heads, kv4_page_bytes(head_dim)), dtype=torch.uint8, device=device)
 
 
-def _kv4_check_pool(pool: torch.Tensor, kv_heads: Optional[int], head_dim: int, what: str) -> None:
-    if pool.dtype is torch.uint8 and head_dim in (64, 128) and pool.shape[1:] == (pool.shape[1] if kv_heads is None else kv_heads, 80 * head_dim) \
-            and pool.is_contiguous():
-        return
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != kv4_page_bytes(head_dim) or \
-            (kv_heads is not None and pool.shape[1] != kv_heads):
-        raise KernelLibraryError(f"{what}: the pool must be uint8 [pages, kv_heads, {kv4_page_bytes(head_dim)}], got "
-                                 f"{pool.dtype} {tuple(pool.shape)}")
-    _contig(pool, "pool")
+def _kv4_check_pool(pool: torch.Tensor, kv_heads: Optional[int], head_dim: int, what: str) -> tuple:
+    """The pool's pages and key/value heads, after its checks."""
+    page = kv4_page_bytes(head_dim)
+    if pool.dtype is torch.uint8 and pool.ndim == 3:
+        pages, held, size = pool.shape
+        if size == page and (kv_heads is None or held == kv_heads):
+            if pool.is_contiguous():
+                return pages, held
+            raise KernelLibraryError(f"{what}: pool must be contiguous")
+    raise KernelLibraryError(f"{what}: the pool must be uint8 [pages, kv_heads, {page}], got {pool.dtype} {tuple(pool.shape)}")
 
 
 def _int32(t: torch.Tensor, name: str, what: str) -> None:
@@ -1882,9 +1888,8 @@ def _int32(t: torch.Tensor, name: str, what: str) -> None:
 
 
 def _table(t: torch.Tensor, rows: Optional[int], what: str) -> None:
-    if t.dtype is torch.int32 and t.is_contiguous() and t.dim() == 2 and (rows is None or t.shape[0] >= rows):
-        return
-    if t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (rows is not None and t.shape[0] < rows):
+    if t.dtype is not torch.int32 or t.ndim != 2 or (t.shape[1] > 1 and not t.is_contiguous() and t.stride(1) != 1) or \
+            (rows is not None and t.shape[0] < rows):
         raise KernelLibraryError(f"{what}: the block table must be int32 [rows, pages]")
 
 
@@ -1895,29 +1900,30 @@ def kv4_store(qkv: torch.Tensor, inv_freq: Optional[torch.Tensor], tok_pos: torc
     ``inv_freq`` as in ``rotary_table``, None: no rotation), rounds the rotated keys and the values to 4 bits into the
     tokens' places in ``pool`` and returns the rotated queries ``[T, heads * head_dim]``.  ``qkv`` stays as it is.  A token whose position is
     negative or whose page is not there is not stored."""
-    T = qkv.shape[0] if qkv.dim() else 0
-    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * kv_heads) * head_dim or qkv.stride(1) != 1:
-        raise KernelLibraryError(f"kv4_store: qkv must be bfloat16 [tokens, {(heads + 2 * kv_heads) * head_dim}], got {qkv.dtype} {tuple(qkv.shape)}")
-    _kv4_check_pool(pool, kv_heads, head_dim, "kv4_store")
+    width = (heads + 2 * kv_heads) * head_dim
+    if qkv.dtype is not torch.bfloat16 or qkv.ndim != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
+        raise KernelLibraryError(f"kv4_store: qkv must be bfloat16 [tokens, {width}], got {qkv.dtype} {tuple(qkv.shape)}")
+    T = qkv.shape[0]
+    pages, _ = _kv4_check_pool(pool, kv_heads, head_dim, "kv4_store")
     _table(block_table, None, "kv4_store")
-    for n, t in (("tok_pos", tok_pos), ("tok_seq", tok_seq)):
-        _int32(t, n, "kv4_store")
-        if t.numel() < T:
-            raise KernelLibraryError(f"kv4_store: {n} has {t.numel()} entries for {T} tokens")
+    _int32(tok_pos, "tok_pos", "kv4_store")
+    _int32(tok_seq, "tok_seq", "kv4_store")
+    if tok_pos.numel() < T or tok_seq.numel() < T:
+        raise KernelLibraryError(f"kv4_store: tok_pos has {tok_pos.numel()} and tok_seq {tok_seq.numel()} entries for {T} tokens")
     hi = lo = 0
     if inv_freq is not None:
-        half = head_dim // 2
-        if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or tuple(inv_freq.shape) not in ((half,), (2, half)):
+        half, parts = head_dim // 2, inv_freq.ndim
+        if inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous() or inv_freq.shape != ((2, half) if parts == 2 else (half,)):
             raise KernelLibraryError(f"kv4_store: inv_freq must be float32 [{half}], or [2, {half}] (see rotary_table)")
         hi = _addr(inv_freq)
-        lo = hi + 4 * half if inv_freq.dim() == 2 else 0
+        lo = hi + 4 * half if parts == 2 else 0
     if out is None:
         out = qkv.new_empty((T, heads * head_dim))
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
         raise KernelLibraryError(f"kv4_store: out must be contiguous bfloat16 {(T, heads * head_dim)}")
     rc = _entry("exl3_kv4_store", "plppppppiiipliiii")(
-        _addr(qkv), qkv.stride(0), out.data_ptr(), hi, lo, _addr(tok_pos), _addr(tok_seq), _addr(block_table), block_table.stride(0),
-        *block_table.shape, _addr(pool), pool.shape[0], T, heads, kv_heads, head_dim, _raw_stream())
+        _addr(qkv), qkv.stride(0), _addr(out), hi, lo, _addr(tok_pos), _addr(tok_seq), _addr(block_table), block_table.stride(0),
+        *block_table.shape, _addr(pool), pages, T, heads, kv_heads, head_dim, _raw_stream())
     if rc:
         _check(rc, "kv4_store")
     return out
@@ -1926,11 +1932,12 @@ def kv4_store(qkv: torch.Tensor, inv_freq: Optional[torch.Tensor], tok_pos: torc
 def kv4_load(pool: torch.Tensor, pages: torch.Tensor, head_dim: int):
     """The keys and values that the listed pages stand for: bfloat16 ``[n, kv_heads, 64, head_dim]`` each (zeros for a number
     that is no page's)."""
-    _kv4_check_pool(pool, None, head_dim, "kv4_load")
+    held, kv_heads = _kv4_check_pool(pool, None, head_dim, "kv4_load")
     _int32(pages, "pages", "kv4_load")
-    n, kv_heads = pages.numel(), pool.shape[1]
-    k, v = torch.empty((2, n, kv_heads, KV4_PAGE, head_dim), dtype=torch.bfloat16, device=pool.device).unbind(0)
-    rc = _entry("exl3_kv4_load", "plpiiipp")(_addr(pool), pool.shape[0], _addr(pages), n, kv_heads, head_dim, k.data_ptr(), v.data_ptr(), _raw_stream())
+    n = pages.numel()
+    k = pool.new_empty((n, kv_heads, KV4_PAGE, head_dim), dtype=torch.bfloat16)
+    v = torch.empty_like(k)
+    rc = _entry("exl3_kv4_load", "plpiiipp")(_addr(pool), held, _addr(pages), n, kv_heads, head_dim, k.data_ptr(), v.data_ptr(), _raw_stream())
     if rc:
         _check(rc, "kv4_load")
     return k, v
@@ -1983,12 +1990,13 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
 
     A few tokens a row (``KV4_FEW_COLUMNS``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
     unpacked to fp16 (values beyond 65,504 count as that) and go through the tcgen05 attention."""
-    T = q.shape[0] if q.dim() else 0
-    if q.dtype is not torch.bfloat16 or q.dim() != 2 or q.shape[1] != heads * head_dim or q.stride(1) != 1:
+    plain = q.is_contiguous()
+    if q.dtype is not torch.bfloat16 or q.ndim != 2 or q.shape[1] != heads * head_dim or not (plain or q.stride(1) == 1):
         raise KernelLibraryError(f"kv4_attn: q must be bfloat16 [tokens, {heads * head_dim}], got {q.dtype} {tuple(q.shape)}")
+    T = q.shape[0]
     if kv_heads < 1 or heads % kv_heads or window < 0 or max_new < 0 or max_len < 0:
         raise KernelLibraryError(f"kv4_attn: {heads} heads on {kv_heads}, window {window}, max_new {max_new}, max_len {max_len}")
-    _kv4_check_pool(pool, kv_heads, head_dim, "kv4_attn")
+    pages, _ = _kv4_check_pool(pool, kv_heads, head_dim, "kv4_attn")
     _int32(row_pos0, "row_pos0", "kv4_attn")
     rows = row_pos0.numel()
     if row_start is not None:
@@ -1999,7 +2007,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         raise KernelLibraryError("kv4_attn: without row_start every row has one token")
     _table(block_table, rows, "kv4_attn")
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, heads * head_dim))
+        out = torch.empty_like(q) if plain else q.new_empty((T, heads * head_dim))
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
         raise KernelLibraryError(f"kv4_attn: out must be contiguous bfloat16 {(T, heads * head_dim)}")
     if T == 0 or rows == 0:
@@ -2011,13 +2019,13 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     columns = 4 if columns_wanted <= 4 else 8 if columns_wanted <= 8 else 16
     groups = -(-columns_wanted // columns)
     span = min(max_len, window + max_new - 1) if window > 0 else max_len
-    chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, sm_count(q.device))
+    chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, _sms(q))
     need, scratch = 0, None
     if chunks > 1:
         need = rows * kv_heads * groups * chunks * columns * (head_dim + 4)
         scratch = workspace.plain(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
     rc = _entry("exl3_kv4_attn", "plpplpiippiiiiiiifiipl")(
-        _addr(q), q.stride(0), _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), block_table.shape[1],
+        _addr(q), heads * head_dim if plain else q.stride(0), _addr(out), _addr(pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1],
         _addr(row_start), _addr(row_pos0), rows, T, max_new, heads, kv_heads, head_dim, window, scale, chunk, chunks, _addr(scratch), need, _raw_stream())
     if rc:
         _check(rc, "kv4_attn")
@@ -2058,11 +2066,14 @@ def fp8_wide_status() -> int:
     return int(library().exl3_fp8_wide_status())
 
 
-def _fp8_check_x(x: torch.Tensor, what: str) -> None:
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
+def _fp8_check_x(x: torch.Tensor, what: str) -> tuple:
+    """x's rows and features, after its checks."""
+    if x.dtype is not torch.bfloat16 or x.ndim != 2 or x.stride(1) != 1:
         raise KernelLibraryError(f"{what}: x must be bfloat16 [rows, features], got {x.dtype} {tuple(x.shape)}")
-    if x.shape[1] < 16 or x.shape[1] % 16:
-        raise KernelLibraryError(f"{what}: the features must be a multiple of 16, got {x.shape[1]}")
+    M, Kd = x.shape
+    if Kd < 16 or Kd % 16:
+        raise KernelLibraryError(f"{what}: the features must be a multiple of 16, got {Kd}")
+    return M, Kd
 
 
 def fp8_quantize(x: torch.Tensor):
@@ -2120,20 +2131,19 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     """``x @ W.T (+ bias)`` with W as ``fp8_quantize_weight`` gives it and x bfloat16 ``[M, K]`` rounded as ``fp8_quantize`` rounds it; sums in
     float32, the result in ``out_dtype`` (bfloat16 or float32).  ``gated``: W's rows are eight gate rows, then the eight up rows of the same
     features, and so on, and ``silu(gate) * up`` comes out (N / 2 wide, no bias)."""
-    _fp8_check_x(x, "fp8_linear")
-    M, Kd = x.shape
-    if w.dtype is not torch.float8_e4m3fn or w.dim() != 2 or w.shape[1] != Kd:
+    M, Kd = _fp8_check_x(x, "fp8_linear")
+    if w.dtype is not torch.float8_e4m3fn or w.ndim != 2 or w.shape[1] != Kd:
         raise KernelLibraryError(f"fp8_linear: w must be float8_e4m3fn [features out, {Kd}], got {w.dtype} {tuple(w.shape)}")
     N = w.shape[0]
-    _contig(w, "w")
-    blocks = -(-Kd // FP8_BLOCK)
-    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != (-(-N // FP8_BLOCK), blocks):
+    blocks = (Kd + FP8_BLOCK - 1) // FP8_BLOCK
+    if w_scale.dtype is not torch.float32 or w_scale.shape != ((N + FP8_BLOCK - 1) // FP8_BLOCK, blocks):
         raise KernelLibraryError(f"fp8_linear: the scales must be float32 {(-(-N // FP8_BLOCK), blocks)}, got {w_scale.dtype} {tuple(w_scale.shape)}")
-    _contig(w_scale, "w_scale")
+    if not (w.is_contiguous() and w_scale.is_contiguous()):
+        raise KernelLibraryError("fp8_linear: w and its scales must be contiguous")
     if gated and (N % 16 or bias is not None):
         raise KernelLibraryError("fp8_linear: the gated product takes rows in sixteens and no bias")
-    if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != N):
-        raise KernelLibraryError(f"fp8_linear: bias must be bfloat16 [{N}]")
+    if bias is not None and (bias.dtype is not torch.bfloat16 or bias.shape != (N,) or not bias.is_contiguous()):
+        raise KernelLibraryError(f"fp8_linear: bias must be contiguous bfloat16 [{N}]")
     shape = (M, N // 2 if gated else N)
     if out is None:
         out = x.new_empty(shape) if out_dtype is torch.bfloat16 else torch.empty(shape, dtype=out_dtype, device=x.device)
@@ -2142,7 +2152,7 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     code = dtype_code(out.dtype)
     if M == 0:
         return out
-    few = _fp8_few(M, N, sm_count(x.device))
+    few = M <= FP8_SKINNY_ROWS or _fp8_few(M, N, _sms(x))
     codes = sx = 0
     if M > FP8_ROUNDED_ROWS or not few:
         room = x.new_empty(M * Kd // 2 + 2 * blocks * M + 8)               # codes, then (16-byte aligned) scales
