@@ -487,12 +487,17 @@ int exl3_kv4_attn_status();
 // and 128 features; y = x w^T (+ bias), or with `gated` silu(gate) * up for rows of w in eights (N / 2 wide).  K a multiple of 16.
 // exl3_fp8_quantize: codes [M, K] and scales [M, blocks], or [blocks, M] with `transposed`, which exl3_fp8_wide takes.
 int exl3_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, float* sx, int transposed, cudaStream_t stream);
+// exl3_fp8_gemv, up to 8 rows and K up to 8,192: x in bfloat16.  exl3_fp8_gemv_pays: whether it is faster there than exl3_fp8_skinny.
+int exl3_fp8_gemv_pays(int M, int N, int K);
+int exl3_fp8_gemv(const void* x, int64_t ldx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M, int N, int K, int gated,
+                  cudaStream_t stream);
 // exl3_fp8_skinny, a few rows: x in bfloat16 up to 16, else its codes with the transposed scales in sx.
 int exl3_fp8_skinny(const void* x, int64_t ldx, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M,
                     int N, int K, int gated, cudaStream_t stream);
 int exl3_fp8_wide(const void* codes, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype, int M, int N,
                   int K, int gated, cudaStream_t stream);
-// Any number of rows; codes and sx: scratch for the rounding from 17 rows on.
+// Any number of rows; codes and sx: scratch for the rounding from 17 rows on; few: 0 exl3_fp8_wide, 1 exl3_fp8_skinny, 2 exl3_fp8_gemv where it pays, else
+// exl3_fp8_skinny.
 int exl3_fp8_linear(const void* x, int64_t ldx, void* codes, float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype,
                     int M, int N, int K, int gated, int few, cudaStream_t stream);
 // Codes left by bounded waits that ran out (0: none); cleared by the calls.

@@ -328,9 +328,11 @@ extern "C" int exl3_fp8_wide(const void* codes, const float* sx, const void* w, 
   return launch_status("fp8_wide");
 }
 
-// The product of any number of rows: `few` picks the weight-streaming kernel; from 17 rows on x is rounded into codes [M, K] and sx [blocks, M] first.
+// The product of any number of rows.  `few`: 1 the weight-streaming kernel, in which a row's bits do not depend on the rows beside it, 2 that or, where
+// it is faster, the one for up to 8 rows, which adds up in another order, 0 the one for many rows; from 17 rows on x is rounded into codes [M, K] and sx [blocks, M] first.
 extern "C" int exl3_fp8_linear(const void* x, int64_t ldx, void* codes, float* sx, const void* w, const float* sw, const void* bias, void* y,
                                int out_dtype, int M, int N, int K, int gated, int few, cudaStream_t stream) {
+  if (few == 2 && exl3_fp8_gemv_pays(M, N, K)) return exl3_fp8_gemv(x, ldx, w, sw, bias, y, out_dtype, M, N, K, gated, stream);
   if (few && M <= 16) return exl3_fp8_skinny(x, ldx, nullptr, w, sw, bias, y, out_dtype, M, N, K, gated, stream);
   const int rc = exl3_fp8_quantize(x, ldx, M, K, codes, sx, 1, stream);
   if (rc) return rc;

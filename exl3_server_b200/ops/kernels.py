@@ -2127,10 +2127,14 @@ def _fp8_few(M: int, N: int, sms: int) -> bool:
 
 
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
-               out_dtype: torch.dtype = torch.bfloat16, gated: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               out_dtype: torch.dtype = torch.bfloat16, gated: bool = False, out: Optional[torch.Tensor] = None,
+               fixed_order: bool = True) -> torch.Tensor:
     """``x @ W.T (+ bias)`` with W as ``fp8_quantize_weight`` gives it and x bfloat16 ``[M, K]`` rounded as ``fp8_quantize`` rounds it; sums in
     float32, the result in ``out_dtype`` (bfloat16 or float32).  ``gated``: W's rows are eight gate rows, then the eight up rows of the same
-    features, and so on, and ``silu(gate) * up`` comes out (N / 2 wide, no bias)."""
+    features, and so on, and ``silu(gate) * up`` comes out (N / 2 wide, no bias).
+
+    A row's bits are the same in any batch of up to 64 rows; ``fixed_order=False`` lets small products of up to 8 rows be added up in another
+    order, which takes a fifth to two fifths less time (fp8_gemv.cu)."""
     M, Kd = _fp8_check_x(x, "fp8_linear")
     if w.dtype is not torch.float8_e4m3fn or w.ndim != 2 or w.shape[1] != Kd:
         raise KernelLibraryError(f"fp8_linear: w must be float8_e4m3fn [features out, {Kd}], got {w.dtype} {tuple(w.shape)}")
@@ -2159,7 +2163,7 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
         codes = room.data_ptr()
         sx = codes + -(-M * Kd // 16) * 16
     rc = _entry("exl3_fp8_linear", "plppppppiiiiii")(_addr(x), x.stride(0), codes, sx, _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
-                                                     1 if gated else 0, 1 if few else 0, _raw_stream())
+                                                     1 if gated else 0, 0 if not few else 1 if fixed_order else 2, _raw_stream())
     if rc:
         _check(rc, "fp8_linear")
     return out

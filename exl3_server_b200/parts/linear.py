@@ -210,7 +210,7 @@ class LinearFP8:
     def __call__(self, x, out_dtype: Optional[torch.dtype] = None, then=None) -> torch.Tensor:
         if isinstance(x, RawNormed):
             x = x.materialize()
-        return K.fp8_linear(x, self.weight, self.scales, self.bias, out_dtype or self.dtype)
+        return K.fp8_linear(x, self.weight, self.scales, self.bias, out_dtype or self.dtype, fixed_order=False)
 
     def heads_rotated_and_cached(self, *args, **kwargs):
         return None
@@ -233,7 +233,7 @@ class LinearFP8:
     def gated(self, x: torch.Tensor) -> torch.Tensor:
         if isinstance(x, RawNormed):
             x = x.materialize()
-        return K.fp8_linear(x, self.weight, self.scales, None, self.dtype, gated=True)
+        return K.fp8_linear(x, self.weight, self.scales, None, self.dtype, gated=True, fixed_order=False)
 
     def weight_bytes(self) -> int:
         n = self.weight.numel() + self.scales.numel() * 4
