@@ -5,7 +5,7 @@ Flags keep the reference's spelling and meaning where the feature exists here:
 ``--model``, ``-p/--prompt`` (repeatable), ``--max-tokens``, ``--temp``,
 ``--top-p``, ``--top-k``, ``--min-p``, ``--repetition-penalty``,
 ``--presence-penalty``, ``--frequency-penalty``, ``--seed``, ``--ignore-eos``,
-``--batch``, ``--quiet``; every value flag takes ``--k v`` and ``--k=v``; an
+``--batch``, ``--quiet``; ``--weight-type fp8`` and ``--cache-type int4`` are this library's own; every value flag takes ``--k v`` and ``--k=v``; an
 unknown flag exits with 2.  There is no tokenizer in this library, so a prompt
 is a list of token ids (``-p "1,15,27"`` or ``--prompt-file`` with one list per
 line) and the output is token ids, one line per request, followed by the

