@@ -167,18 +167,18 @@ kv4_attn_kernel(const A4Args a) {
   const int row = blockIdx.z, kvh = blockIdx.y / a.n_ct, ct = blockIdx.y % a.n_ct;
   pdl_trigger();
   pdl_wait();
+  // this warp's tiles, one a lane: tile_a + warp + 4 * lane; tiles without a page are left out.  Without a window the chunk's place says which they
+  // are, and the table is read beside the row's lengths, not after them.
+  auto page_of = [&](int tile) { return tile / SPP < a.bt_width ? __ldcg(a.block_table + (int64_t)row * a.bt_stride + tile / SPP) : -1; };
+  int my_page = -1;
+  if (a.window == 0 && warp + A4_WARPS * lane < a.chunk) my_page = page_of((int)blockIdx.x * a.chunk + warp + A4_WARPS * lane);
   const A4Range<HD> r(a, row, ct, COLS);
   if (r.cols <= 0 || (int)blockIdx.x >= max(r.n_chunks, 1)) return;
   const int chunk0 = (r.c_first + (int)blockIdx.x) * a.chunk;
   const int tile_a = max(r.t_lo, chunk0), tile_b = min(r.t_hi + 1, chunk0 + a.chunk);      // none where the row sees nothing
-
-  // this warp's tiles, one a lane: tile_a + warp + 4 * lane; tiles without a page are left out
-  int my_page = -1;
-  {
-    const int tile = tile_a + warp + A4_WARPS * lane;
-    if (tile < tile_b && tile / SPP < a.bt_width) my_page = __ldcg(a.block_table + (int64_t)row * a.bt_stride + tile / SPP);
-    if (my_page >= a.n_pages) my_page = -1;
-  }
+  const int my_tile = tile_a + warp + A4_WARPS * lane;
+  if (a.window > 0 && my_tile < tile_b) my_page = page_of(my_tile);
+  if (my_tile >= tile_b || my_page >= a.n_pages) my_page = -1;
   uint32_t todo = __ballot_sync(0xffffffffu, my_page >= 0), ask = todo;
   unsigned char* ring = a4_smem_raw + warp * RING;
   uint64_t* bars = full[warp];
@@ -567,22 +567,26 @@ kv4_join_kernel(const A4Args a, int columns) {
   const int kvh = blockIdx.y / a.n_ct, ct = blockIdx.y % a.n_ct, c = blockIdx.x, row = blockIdx.z;
   pdl_trigger();
   pdl_wait();
-  const A4Range<HD> r(a, row, ct, columns);
-  if (c >= r.cols || r.n_chunks <= 1) return;               // (a single chunk wrote the output itself)
   const float* base = a.scratch + ((((int64_t)row * a.nkv + kvh) * a.n_ct + ct) * a.max_chunks * columns + c) * (HD + 4);
   const int64_t step = (int64_t)columns * (HD + 4);
   float m = __int_as_float(0xff800000), l = 0.0f, acc[V] = {};
-  for (int k0 = warp; k0 < r.n_chunks; k0 += 4 * A4_JOIN_WARPS) {
-    float mk[4], lk[4], y[4][V];
+  float mk[4], lk[4], y[4][V];
+  auto ask = [&](int k0) {                                  // records, the row's or not: what is not is never used
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int k = k0 + u * A4_JOIN_WARPS;
-      const float* p = base + (k < r.n_chunks ? k : 0) * step;
-      mk[u] = k < r.n_chunks ? __ldcg(p) : __int_as_float(0xff800000);
+      const float* p = base + (k < a.max_chunks ? k : 0) * step;
+      mk[u] = __ldcg(p);
       lk[u] = __ldcg(p + 1);
 #pragma unroll
       for (int i = 0; i < V; ++i) y[u][i] = __ldcg(p + 4 + i * 32 + lane);
     }
+  };
+  ask(warp);                                                // (beside the row's lengths, not after them)
+  const A4Range<HD> r(a, row, ct, columns);
+  if (c >= r.cols || r.n_chunks <= 1) return;               // (a single chunk wrote the output itself)
+  for (int k0 = warp; k0 < r.n_chunks; k0 += 4 * A4_JOIN_WARPS) {
+    if (k0 > warp) ask(k0);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if (k0 + u * A4_JOIN_WARPS >= r.n_chunks) break;
