@@ -26,11 +26,12 @@
 // records go to scratch memory and a second kernel joins them, in the chunks' order.
 //
 // Measured: 8 rows of 4,096 keys, 36 heads of 64 with keys of their own 28.8 us (94 MB, 3.3 TB/s); 64 rows of 130 to 8,000 keys, 32 heads of 128 on 8
-// 80.8 us (339 MB, 4.2 TB/s); one row of 131,071 keys of these 40.3 us (168 MB, 4.2 TB/s); one row of 128 keys, 16 heads of 64 on 2 3.9 us.
+// 79.9 us (339 MB, 4.2 TB/s); one row of 131,071 keys of these 38.4 us (168 MB, 4.4 TB/s); one row of 128 keys, 16 heads of 64 on 2 3.9 us.
 // What bounds it is the instructions of a tile, some 650 for a warp, half of them integer ones (masks, byte permutes, minima and maxima) that a
 // scheduler takes every second cycle; more warps an SM, more stages of the ring or larger chunks change nothing.  What brought it here, for
 // the 64 rows: 127 us with every group's numbers multiplied in first, 98 with keys as e4m3, 87 with F in the reference, 81 with whole tiles
-// first, one vote a tile on the reference and two groups to an operand.  A join by a cluster through distributed shared memory takes 1 us less
+// first, one vote a tile on the reference and two groups to an operand.  A block's beginning and end are some 4 us that few blocks an SM do not hide, hence the page numbers beside
+// the lengths (and chunks no smaller than a wave wants).  A join by a cluster through distributed shared memory takes 1 us less
 // than the second kernel where all clusters run at once, and a tenth more than the whole where they do not (90 us); it was left out.
 #include "api.h"
 #include "cache4.cuh"
