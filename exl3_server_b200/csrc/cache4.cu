@@ -6,10 +6,10 @@
 //          value that is not finite, or whose range is not, becomes NaN as a whole.
 //   load   mn + sc * code (exact in float32: 8 x 4 bits) rounded to bfloat16, or to fp16 for the prompt attention.
 //
-// Measured, 4,096 tokens of 36 heads of 64 with 36 key and value heads: store 31 us (87 MB, 2.8 TB/s), load of its pages 13.0 us (49 MB, 3.8 TB/s);
-// a step of 64 tokens of 32 heads of 128 with 8 and 8: store 3.0 us, load of 64 pages 7.5 us.  The load is bound by memory, the store of many
-// tokens by its instructions (245 for the warp's four token and head pairs; issue slots 79 % busy; 29 us without a store to the pool, 28 without
-// its loads), that of a decode step by its launch.
+// Measured, 4,096 tokens of 36 heads of 64 with 36 key and value heads: store 29.6 us (87 MB, 2.9 TB/s), load of its pages 13.0 us (49 MB, 3.8 TB/s);
+// a step of 64 tokens of 32 heads of 128 with 8 and 8: store 2.9 us, load of 64 pages 7.5 us.  The load is bound by memory, the store of many
+// tokens by its instructions (some 220 for the warp's four token and head pairs; 245, 31 us and issue slots 79 % busy before pairs of floats; of these 31,
+// 29 without a store to the pool, 28 without loads), that of a decode step by its launch.
 #include "api.h"
 #include "cache4.cuh"
 
@@ -32,6 +32,13 @@ __device__ inline float c4_max3(float a, float b, float c) {
   return d;
 }
 
+// Two floats at a time; each rounds as the scalar instruction does.
+__device__ inline uint64_t c4_pair(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ inline void c4_unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ inline uint64_t c4_add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ inline uint64_t c4_mul2(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ inline uint64_t c4_fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
 // A lane has features 8 j .. 8 j + 7 of a head (j = 0 .. HD / 8 - 1); four neighbouring lanes have a group.  Returns the group's word and
 // the lane's eight codes as the low bits of floats around 1.5 * 2^23: adding that number rounds to an integer, ties to even, and leaves it there
 // (conversions have a pipe of a quarter of the others' rate: they and the shifts that put the codes together were half of the kernel's time).
@@ -41,10 +48,12 @@ __device__ inline uint32_t c4_quantize(const float (&x)[8], uint32_t (&bits)[8])
   lo = c4_min3(lo, x[3], x[4]); hi = c4_max3(hi, x[3], x[4]);
   lo = c4_min3(lo, x[5], x[6]); hi = c4_max3(hi, x[5], x[6]);
   lo = fminf(lo, x[7]); hi = fmaxf(hi, x[7]);
-  float odd = 0.0f;                                                    // 0, or NaN where a value is not finite
+  uint64_t odd2 = 0;                                                   // zeros, or NaN where a value is not finite
 #pragma unroll
-  for (int e = 0; e < 8; ++e) odd = fmaf(x[e], 0.0f, odd);
-  if (odd != 0.0f) { lo = __int_as_float(0xff800000); hi = __int_as_float(0x7f800000); }
+  for (int e = 0; e < 8; e += 2) odd2 = c4_fma2(c4_pair(x[e], x[e + 1]), 0, odd2);
+  float odd, odd_b;
+  c4_unpair(odd2, odd, odd_b);
+  if (odd + odd_b != 0.0f) { lo = __int_as_float(0xff800000); hi = __int_as_float(0x7f800000); }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -58,9 +67,14 @@ __device__ inline uint32_t c4_quantize(const float (&x)[8], uint32_t (&bits)[8])
   const bool fine = sc < __int_as_float(0x7f800000) && fabsf(mn) < __int_as_float(0x7f800000);
   const float inv = fine && sc > SC_MIN ? __frcp_rn(sc) : 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[e], mn), inv), 0.0f), 15.0f);        // (NaN becomes 0)
-    bits[e] = __float_as_uint(__fadd_rn(c, ROUND));
+  for (int e = 0; e < 8; e += 2) {
+    float a, b;
+    c4_unpair(c4_mul2(c4_add2(c4_pair(x[e], x[e + 1]), c4_pair(-mn, -mn)), c4_pair(inv, inv)), a, b);
+    a = fminf(fmaxf(a, 0.0f), 15.0f);                                  // (NaN becomes 0)
+    b = fminf(fmaxf(b, 0.0f), 15.0f);
+    c4_unpair(c4_add2(c4_pair(a, b), c4_pair(ROUND, ROUND)), a, b);
+    bits[e] = __float_as_uint(a);
+    bits[e + 1] = __float_as_uint(b);
   }
   return fine ? (uint32_t)__bfloat16_as_ushort(scb) << 16 | __bfloat16_as_ushort(mnb) : 0x7fc07fc0u;
 }
@@ -137,7 +151,8 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv
       *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(&s_sin[now][d0]);
       *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(&s_sin[now][d0 + 4]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], c[e], y[e] * sn[e]);
+      for (int e = 0; e < 8; e += 2)
+        c4_unpair(c4_fma2(c4_pair(x[e], x[e + 1]), c4_pair(c[e], c[e + 1]), c4_mul2(c4_pair(y[e], y[e + 1]), c4_pair(sn[e], sn[e + 1]))), x[e], x[e + 1]);
     }
     own = next_own;
     other = next_other;
