@@ -1948,7 +1948,20 @@ def kv4_attn_status() -> int:
     return int(library().exl3_kv4_attn_status())
 
 
-KV4_FEW_COLUMNS = 64        # new tokens times query heads per key/value head up to which the keys are walked as codes
+KV4_FEW_COLUMNS = 16        # new tokens times query heads per key/value head up to which the keys are walked as codes in any case
+
+
+def _kv4_walks(rows: int, tiles: int, heads: int, kv_heads: int, head_dim: int, max_new: int, max_len: int, span: int) -> bool:
+    """Whether walking the codes beats unpacking them for a prompt: the walk reads all keys again for every 16 columns (430 tiles a microsecond),
+    the other path unpacks every page (3 TB/s) and then takes a page's time (0.75 us) for each of a query tile's pages, with some 190 query tiles
+    and heads at a time.  Fitted to 315 shapes of 5 to 100 new tokens at 200 to 30,000 keys.  Both sides, us: 32 heads of 128 on 8, 16 rows of 4,000 keys,
+    24 new tokens 235 / 261, 32 new 297 / 260; 16 heads of 64 on 2, one row of 30,000 keys, 100 new 112 / 363."""
+    groups = -(-max_new * (heads // kv_heads) // 16)
+    if max_new > 128 or kv_heads * groups > 65535:         # (more than a tile of queries: those are full)
+        return False
+    walk = 10.0 + rows * kv_heads * groups * -(-span * head_dim // 4096) / 430.0
+    unpack = 5.25 * rows * max_len * kv_heads * head_dim / 3e6
+    return walk < 10.0 + unpack + 0.75 * -(-span // KV4_PAGE) * max(1.0, tiles * heads / 190.0)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1988,7 +2001,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     ``tiles``: ``(row, first new token, count)`` of the tiles of 128 queries, as ``attn_prefill_tc`` takes them, for rows of many new
     tokens (None: never more than a few).  ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's).
 
-    A few tokens a row (``KV4_FEW_COLUMNS``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
+    A few tokens a row (``_kv4_walks``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
     unpacked to fp16 (values beyond 65,504 count as that) and go through the tcgen05 attention."""
     plain = q.is_contiguous()
     if q.dtype is not torch.bfloat16 or q.ndim != 2 or q.shape[1] != heads * head_dim or not (plain or q.stride(1) == 1):
@@ -2013,12 +2026,12 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     if T == 0 or rows == 0:
         return out
     columns_wanted = max_new * (heads // kv_heads)
-    if tiles is not None and columns_wanted > KV4_FEW_COLUMNS:
+    span = min(max_len, window + max_new - 1) if window > 0 else max_len
+    if tiles is not None and columns_wanted > KV4_FEW_COLUMNS and not _kv4_walks(rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, span):
         return _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window,
                                 workspace, out)
     columns = 4 if columns_wanted <= 4 else 8 if columns_wanted <= 8 else 16
     groups = -(-columns_wanted // columns)
-    span = min(max_len, window + max_new - 1) if window > 0 else max_len
     chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, _sms(q))
     need, scratch = 0, None
     if chunks > 1:

@@ -202,6 +202,16 @@ def test_prompts(heads, kv_heads, d, window):
     c.check(c.run(window), window, only=(0, 1, 63, 64, 127, 128, 199))
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (16, 2, 64), (8, 2, 128), (7, 1, 128)])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("walks", [True, False])
+def test_some_new_tokens_either_way(heads, kv_heads, d, window, walks, monkeypatch):
+    """Rows of 1 to 128 new tokens, by the codes and by unpacked pages, whatever the model of both picks."""
+    monkeypatch.setattr(K(), "_kv4_walks", lambda *a: walks)
+    c = Case([(900, 128), (70, 33), (0, 1), (5, 0), (300, 64), (0, 17)], heads, kv_heads, d, seed=heads + d + 3)
+    c.check(c.run(window), window, only=(0, 1, 16, 32, 63, 64, 127))
+
+
 @pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (8, 2, 128), (16, 1, 128)])
 def test_chunks_are_joined(heads, kv_heads, d):
     """A long row in many chunks beside short ones, and the same row alone."""

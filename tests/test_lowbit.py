@@ -107,3 +107,12 @@ def test_the_plain_forms_agree_with_torch():
     assert float((r - y).abs().max()) <= 0.51 / 15 * float((y.amax() - y.amin())) + 2.0 ** -8 * float(y.abs().max())
     k, v = page_values(torch.zeros(5120, dtype=torch.uint8), 64)
     assert bool((k == 0).all()) and k.shape == (64, 64) and v.shape == (64, 64)
+
+
+def test_which_way_the_4_bit_attention_goes():
+    walks = K._kv4_walks
+    # rows, query tiles, heads, key/value heads, head size, new tokens, longest row, visible keys: measured on both sides, far from the edge
+    assert walks(1, 1, 32, 2, 128, 5, 30005, 30005) and walks(1, 1, 16, 2, 64, 100, 30100, 30100) and walks(16, 16, 32, 8, 128, 12, 4012, 4012)
+    assert not walks(16, 16, 32, 8, 128, 64, 4064, 4064) and not walks(1, 31, 32, 8, 128, 3900, 5100, 5100)
+    assert not walks(16, 16, 16, 2, 64, 100, 4100, 4100)
+    assert not walks(1, 1, 128 * 65536 // 64, 65536 // 4, 64, 128, 128, 128)              # more groups of columns than a grid has room for
