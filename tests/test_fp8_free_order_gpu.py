@@ -84,3 +84,15 @@ def test_products_in_a_chain(M, N, Kd):
         torch.cuda.synchronize()
     assert bool(y.isfinite().all()) and torch.equal(first, y)
     assert all(torch.equal(run(), first) for _ in range(20))
+
+
+def test_refusals():
+    from exl3_server_b200.ops.lib import KernelLibraryError
+    x, w, s = make(2, 64, 128, seed=7)
+    wide = torch.zeros(128, device=DEV).bfloat16()
+    for kw in (dict(bias=wide[::2]), dict(bias=wide), dict(bias=wide[:64].float()), dict(bias=wide[:64], gated=True)):
+        with pytest.raises(KernelLibraryError, match="bias"):
+            K().fp8_linear(x, w, s, fixed_order=False, **kw)
+    with pytest.raises(KernelLibraryError):
+        K().fp8_linear(x.cpu(), w, s, fixed_order=False)
+    assert K().fp8_linear(x[:0], w, s, fixed_order=False).shape == (0, 64)
