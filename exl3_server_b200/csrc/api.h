@@ -466,13 +466,14 @@ int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float
 // What the listed pages stand for, [n, nkv, 64, hd] bfloat16 each (zeros for a number that is no page's).
 int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
                   cudaStream_t stream);
-// Pages and queries in fp16 for the prompt attention (see cache4.cu), and the attention of prompts over a table [rows, width] of pages.
-int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* pages, int rows, int width, const int* row_start, const int* row_pos0, int nkv,
-                      int hd, void* k_out, void* v_out, int* table,
-                      const void* q, int64_t q_stride, int T, int nh, void* q_out, float* q_scale, cudaStream_t stream);
-long long exl3_kv4_prompt_scratch(int T, int pages, int nh, int nkv, int hd);
-int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table, int rows,
-                    int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0, int n_tiles, int nh,
+// Pages and queries in fp16 for the prompt attention and where each row's pages are (own [rows], see cache4_rows.cuh), and the attention of prompts over
+// a table [rows, width] of pages; pages that are not there, or beyond the table, are hidden.
+int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* block_table, int bt_stride, int rows, int width, const int* row_start,
+                      const int* row_pos0, int nkv, int hd, void* k_out, void* v_out, void* own, const void* q, int64_t q_stride, int T, int nh,
+                      void* q_out, float* q_scale, cudaStream_t stream);
+long long exl3_kv4_prompt_scratch(int T, int rows, int pages, int nh, int nkv, int hd);
+int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
+                    int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0, int n_tiles, int nh,
                     int nkv, int hd, int window, float scale, void* scratch, long long scratch_bytes, cudaStream_t stream);
 int exl3_kv4_prompt_status();
 // Attention of one token or a few per row over the 4-bit cache.  Row r has tokens row_start[r] .. row_start[r + 1] - 1 (null: token r) at positions

@@ -16,13 +16,13 @@ extern "C" int exl3_kv4_prompt_status() { return fa_status(); }
 
 static long long kv4_up16(long long n) { return (n + 15) / 16 * 16; }
 
-// Bytes of scratch: the pages' keys and values, the queries, their factors, the pages' own table.
-extern "C" long long exl3_kv4_prompt_scratch(int T, int pages, int nh, int nkv, int hd) {
-  return 2 * (long long)pages * nkv * 64 * hd * 2 + kv4_up16((long long)T * nh * hd * 2) + kv4_up16((long long)T * nh * 4) + kv4_up16((long long)pages * 4);
+// Bytes of scratch: the pages' keys and values, the queries, their factors, where each row's pages are.
+extern "C" long long exl3_kv4_prompt_scratch(int T, int rows, int pages, int nh, int nkv, int hd) {
+  return 2 * (long long)pages * nkv * 64 * hd * 2 + kv4_up16((long long)T * nh * hd * 2) + kv4_up16((long long)T * nh * 4) + 16ll * rows;
 }
 
 extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table,
-                               int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0,
+                               int bt_stride, int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0,
                                int n_tiles, int nh, int nkv, int hd, int window, float scale, void* scratch, long long scratch_bytes,
                                cudaStream_t stream) {
   if (T == 0 || n_tiles == 0) return 0;
@@ -32,17 +32,18 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
     return ERR_BAD_ARGUMENT;
   }
   const int pages = rows * width;
-  if (!aligned16(scratch) || scratch_bytes < exl3_kv4_prompt_scratch(T, pages, nh, nkv, hd)) {
-    set_error("kv4_prompt: %lld bytes of scratch wanted, 16-byte aligned", exl3_kv4_prompt_scratch(T, pages, nh, nkv, hd));
+  if (!aligned16(scratch) || scratch_bytes < exl3_kv4_prompt_scratch(T, rows, pages, nh, nkv, hd)) {
+    set_error("kv4_prompt: %lld bytes of scratch wanted, 16-byte aligned", exl3_kv4_prompt_scratch(T, rows, pages, nh, nkv, hd));
     return ERR_SCRATCH;
   }
   unsigned char* k = static_cast<unsigned char*>(scratch);
   unsigned char* v = k + (long long)pages * nkv * 64 * hd * 2;
   unsigned char* q16 = v + (long long)pages * nkv * 64 * hd * 2;
   float* q_scale = reinterpret_cast<float*>(q16 + kv4_up16((long long)T * nh * hd * 2));
-  int* table = reinterpret_cast<int*>(reinterpret_cast<unsigned char*>(q_scale) + kv4_up16((long long)T * nh * 4));
-  const int rc = exl3_kv4_unpack16(pool, n_pages, block_table, rows, width, row_start, row_pos0, nkv, hd, k, v, table, q, q_stride, T, nh, q16, q_scale, stream);
+  FaRow* own = reinterpret_cast<FaRow*>(reinterpret_cast<unsigned char*>(q_scale) + kv4_up16((long long)T * nh * 4));
+  const int rc = exl3_kv4_unpack16(pool, n_pages, block_table, bt_stride, rows, width, row_start, row_pos0, nkv, hd, k, v, own, q, q_stride, T, nh, q16,
+                                   q_scale, stream);
   if (rc) return rc;
-  return fa_run(q16, (int64_t)nh * hd, T, out, k, v, (int64_t)pages * nkv * 64, table, width, row_start, row_pos0, tile_seq, tile_q0, n_tiles,
-                nh, nkv, hd, 64, window, 0, 0, scale, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr, q_scale, stream);
+  return fa_run(q16, (int64_t)nh * hd, T, out, k, v, (int64_t)pages * nkv * 64, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, n_tiles,
+                nh, nkv, hd, 64, window, 0, 0, scale, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr, q_scale, own, (int)n_pages, stream);
 }

@@ -40,7 +40,8 @@
 // exl3_attn_prefill_tc_status() returns, frees its tensor memory and exits.
 //
 // Compiled twice: for bfloat16 (attention_prefill_tc.cu), and with EXL3_PREFILL_F16 for fp16 queries, keys, values and probabilities
-// (attention_prefill_f16.cu), where every (query, head) brings a factor of its own beside the scale (FaOpts::q_scale).
+// (attention_prefill_f16.cu), where every (query, head) brings a factor of its own beside the scale (FaOpts::q_scale), and keys and values are copies
+// of a row's pages that were made for this step (FaRow): pages that are not there, or beyond the table, are hidden.
 #pragma once
 #include "api.h"
 #include "common.cuh"
@@ -48,6 +49,11 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <math.h>
+#ifdef EXL3_PREFILL_F16
+#include "cache4_rows.cuh"
+#else
+namespace exl3 { struct FaRow {}; }
+#endif
 
 #ifdef EXL3_PREFILL_F16
 #define EXL3_FA_NS prefill_f16
@@ -216,6 +222,8 @@ struct FaOpts {
   float dist_mul;
   const float* gate;           // a factor per (token, query head) on the output; null: none
   const float* q_scale;        // fp16: what the scores of a (token, query head) are multiplied by beside the scale
+  const FaRow* own;            // fp16: where the copies of the rows' pages are
+  int table_pages;             // fp16: pages of the pool that the block table speaks of
 };
 // What the scores of row `row` of q are multiplied by (base-2 units).
 __device__ inline float fa_score_mul(const FaOpts& opts, float scale_log2, int64_t row, bool there, int nh, int head) {
@@ -246,10 +254,35 @@ struct FaTile {
   int kept;        // pages from the sequence's start that are walked before it (kept first keys)
   int n_pages;     // pages to walk
   const int* bt;   // the sequence's page table
+  FaRow own;       // fp16
 };
+// Page j of the sequence in the pools of keys and values (a copy of a page that is not there would be at -1: zeros, to be hidden).
+__device__ inline int fa_page(const int* bt, const FaRow& own, const FaOpts& opts, int j) {
+#ifdef EXL3_PREFILL_F16
+  return row_copy(own, bt, opts.table_pages, j);
+#else
+  return bt[j];
+#endif
+}
+// Whether the page of keys from key0 on is to be hidden from everyone.
+__device__ inline bool fa_missing(const int* bt, const FaRow& own, const FaOpts& opts, int key0) {
+#ifdef EXL3_PREFILL_F16
+  return own.holes && row_copy(own, bt, opts.table_pages, key0 / FA_BK) < 0;
+#else
+  return false;
+#endif
+}
+__device__ inline FaRow fa_row(const FaOpts& opts, int b) {
+#ifdef EXL3_PREFILL_F16
+  const int4 w = __ldcg(reinterpret_cast<const int4*>(opts.own + b));
+  return {w.x, w.y, w.z, w.w};
+#else
+  return {};
+#endif
+}
 __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride, const int* row_start,
                                  const int* row_pos0, const int* tile_seq, const int* tile_q0, int window,
-                                 int chunk, int keep_first) {
+                                 int chunk, const FaOpts& opts) {
   FaTile t;
   const int b = tile_seq[tile], q0 = tile_q0[tile];
   const int n_new = row_start[b + 1] - row_start[b];
@@ -260,9 +293,11 @@ __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride
   int k_lo = (window > 0 && t.p_first - window + 1 > 0) ? t.p_first - window + 1 : 0;
   if (chunk > 0) k_lo = max(k_lo, t.p_first / chunk * chunk);    // the block of positions of the tile's first query
   t.page_lo = k_lo / FA_BK;
-  t.kept = fa_kept_pages(window, keep_first, t.page_lo);
+  t.kept = fa_kept_pages(window, opts.keep_first, t.page_lo);
   t.n_pages = t.kept + t.p_last / FA_BK - t.page_lo + 1;
+  if (FA_F16) t.n_pages = max(t.n_pages, 1);              // (queries before position 0: one page, hidden from all)
   t.bt = block_table + (int64_t)b * bt_stride;
+  t.own = fa_row(opts, b);
   return t;
 }
 
@@ -299,6 +334,13 @@ __device__ inline void fa_adjust(uint32_t (&sr)[2][32], const FaOpts& opts, int 
         sr[h][c] = dead ? 0xff800000u : sr[h][c];            // -inf
       }
   }
+}
+// Nobody sees this page.
+__device__ inline void fa_hide(uint32_t (&sr)[2][32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int c = 0; c < 32; ++c) sr[h][c] = 0xff800000u;
 }
 // Four independent chains for the maximum (and below for the sum): the row is long and a single chain would make every
 // step wait for the one before.
@@ -384,6 +426,7 @@ __device__ inline void fa_rescale_slowly(uint32_t taddr, float corr) {
 // What a row of O is multiplied by at the end.  A sink is a key of score 0 without a value: one more term in the sum, in
 // the units of the reference maximum.
 __device__ inline float fa_inverse(float l_run, float m_used, int sink, const FaOpts& opts, int head, int row, int nh, bool in) {
+  if (FA_F16 && l_run == 0.0f) return 0.0f;                  // a query that sees nothing
   float inv = 1.0f / (sink ? l_run + fa_exp2((opts.sink_vals ? __ldg(opts.sink_vals + head) * 1.4426950408889634f : 0.0f) - m_used) : l_run);
   if (opts.gate && in) inv *= __ldcg(opts.gate + (int64_t)row * nh + head);
   return inv;
@@ -448,8 +491,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const int other = n_tiles - 1 - (int)blockIdx.y;
   const int n_own = (fold && other > (int)blockIdx.y) ? 2 : 1;
   auto tile_of = [&](int w) {                       // the block's first (w = 0) or second tile
-    return fa_tile(w ? other : (int)blockIdx.y, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk,
-                   opts.keep_first);
+    return fa_tile(w ? other : (int)blockIdx.y, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
   };
 
   if (threadIdx.x == 0) {
@@ -506,7 +548,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       if (c >= n_total) return 0;
       const FaTile& tc = c >= n0 ? tb : ta;
       const int jc = c >= n0 ? c - n0 : c;
-      return tc.bt[jc < tc.kept ? jc : tc.page_lo + jc - tc.kept];
+      return fa_page(tc.bt, tc.own, opts, jc < tc.kept ? jc : tc.page_lo + jc - tc.kept);
     };
     int pgs = numbers(0), pgs_next = numbers(32);
     int copied = 0;                                          // pages whose copies were asked for
@@ -624,6 +666,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       const bool s_there = j + 1 < n_blocks && fa_mbar_test(s_full + (st ^ 1), ((f + 1) >> 1) & 1);
       const int key0 = (j < kept ? j : page_lo + j - kept) * FA_BK;
       fa_adjust(sr, opts, head, key0, p, p_first, p_last, p_first + warp * 32, window, chunk);
+      if (fa_missing(tw.bt, tw.own, opts, key0)) fa_hide(sr);
       const float mx = fa_row_max(sr) * score_mul;           // scale > 0: max and scale commute
       // lazy rescale: move the reference maximum only when it is far behind
       const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
@@ -712,6 +755,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x, tile = blockIdx.y;
+  if (FA_F16) pdl_wait();                         // where the copies are is the work of the kernel ahead
   const int b = tile_seq[tile], q0 = tile_q0[tile];
   const int n_new = row_start[b + 1] - row_start[b];
   const int pos0 = row_pos0[b];
@@ -722,8 +766,9 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   if (chunk > 0) k_lo = max(k_lo, p_first / chunk * chunk);
   const int page_lo = k_lo / FA_BK, page_hi = p_last / FA_BK;
   const int kept = fa_kept_pages(window, opts.keep_first, page_lo);
-  const int n_blocks = kept + page_hi - page_lo + 1;
+  const int n_blocks = FA_F16 ? max(kept + page_hi - page_lo + 1, 1) : kept + page_hi - page_lo + 1;      // (as in fa_tile)
   const int* bt = block_table + (int64_t)b * bt_stride;
+  const FaRow own = fa_row(opts, b);
 
   if (threadIdx.x == 0) {
     fa_mbar_init(q_full, 1);
@@ -756,7 +801,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     }
     auto load_kv = [&](int j) {
       const int st = j % F4_STAGES;
-      const int pg = bt[j < kept ? j : page_lo + j - kept];
+      const int pg = fa_page(bt, own, opts, j < kept ? j : page_lo + j - kept);
       if (lane == 0) {
         fa_mbar_expect_tx(kv_full + st, 2 * KVB);
         fa_tma_2d(sK + st * KVB, &map_k, kv_full + st, 0, (pg * nkv + g) * FA_BK);
@@ -812,6 +857,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       fa_wait_ld();
       const int key0 = (j < kept ? j : page_lo + j - kept) * FA_BK;
       fa_adjust(sr, opts, head, key0, p, p_first, p_last, p_first + warp * 32, window, chunk);
+      if (fa_missing(bt, own, opts, key0)) fa_hide(sr);
       const float mx = fa_row_max(sr) * score_mul;
       const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
@@ -920,7 +966,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     return k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
   };
   auto tile_of = [&](int item) {
-    return fa_tile(item / n_pairs, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts.keep_first);
+    return fa_tile(item / n_pairs, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
   };
 
   if (threadIdx.x == 0) {
@@ -951,7 +997,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     FaTile t = tile_of(item);
     auto numbers = [&](const FaTile& u, int j0) {
       const int j = j0 + lane;
-      return j < u.n_pages ? u.bt[j < u.kept ? j : u.page_lo + j - u.kept] : 0;
+      return j < u.n_pages ? fa_page(u.bt, u.own, opts, j < u.kept ? j : u.page_lo + j - u.kept) : 0;
     };
     int pgs = numbers(t, 0);
     while (ok) {
@@ -1083,6 +1129,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const bool s_there = j + 1 < n_pages && fa_mbar_test(s_full + 2 * s + (sb ^ 1), ((f + 1) >> 1) & 1);
         const int key0 = (j < t.kept ? j : t.page_lo + j - t.kept) * FA_BK;
         fa_adjust(sr, opts, head, key0, p, t.p_first, t.p_last, t.p_first + q * 32, window, chunk);
+        if (fa_missing(t.bt, t.own, opts, key0)) fa_hide(sr);
         const float mx = fa_row_max(sr) * score_mul;         // scale > 0: max and scale commute
         const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
@@ -1190,7 +1237,7 @@ static int fa_run(const void* q, int64_t q_row_stride, int T, void* out, const v
                   const int* tile_q0, int n_tiles, int nh, int nkv, int hd, int page, int window,
                   int chunk, int sink, float scale, int variant, int keep_first, float softcap,
                   const float* sink_vals, const float* dist, int dist_len, const float* gate,
-                  const float* q_scale, cudaStream_t stream) {
+                  const float* q_scale, const FaRow* own, int table_pages, cudaStream_t stream) {
   if (n_tiles == 0) return 0;
   if (dist_len < 0 || (dist_len > 0 && dist == nullptr)) {
     set_error("attn_prefill_tc: a table of %d distance biases is missing", dist_len);
@@ -1210,6 +1257,8 @@ static int fa_run(const void* q, int64_t q_row_stride, int T, void* out, const v
   opts.dist_len = dist_len;
   opts.gate = gate;
   opts.q_scale = q_scale;
+  opts.own = own;
+  opts.table_pages = table_pages;
   opts.dist_mul = softcap > 0.0f ? 1.0f / softcap : 1.0f / scale;
   if (!fa_supported(hd, page)) {
     set_error("attn_prefill_tc: needs bfloat16, head_dim 64 or 128 and pages of 64, got head_dim %d page %d", hd, page);

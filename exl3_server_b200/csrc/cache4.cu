@@ -12,6 +12,7 @@
 // 29 without a store to the pool, 28 without loads), that of a decode step by its launch.
 #include "api.h"
 #include "cache4.cuh"
+#include "cache4_rows.cuh"
 
 #include <cuda_fp16.h>
 
@@ -244,38 +245,57 @@ kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
   c4_unpack<HD, false>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), there, PAGE, k_out + at, v_out + at);
 }
 
-// The same to fp16 for the prompt attention, with the pages' own table (entry i: i, or -1 where there is no page, and nothing is written
-// for it), and the queries to fp16: a row of a head times a power of two that brings its largest value to [2^10, 2^11), whose inverse goes to
+// ---- prompts: fp16 copies of the rows' pages and of the queries, for the prompt attention ------------------------------------------
+
+struct C4Prompt {
+  const unsigned char* pool;
+  int n_pages, nkv;
+  const int* block_table;
+  int bt_stride, width, rows;
+  const int *row_start, *row_pos0;
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  int T, nh;
+  __half *k_out, *v_out, *q_out;
+  float* q_scale;
+  FaRow* own;
+};
+
+// A warp per row: where the copies of its pages will be, and whether some page that its queries look for is not there.
+__device__ inline void c4_row(const C4Prompt& a, int row) {
+  const int lane = threadIdx.x & 31;
+  const int end = __ldcg(a.row_pos0 + row) + __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row);      // positions 0 .. end - 1
+  const int pages = end > 0 ? (end - 1) / PAGE + 1 : 0, count = min(pages, a.width);
+  bool holes = pages > count;
+  for (int j = lane; j < count; j += 32) {
+    const int page = __ldcg(a.block_table + (int64_t)row * a.bt_stride + j);
+    holes = holes || page < 0 || page >= a.n_pages;
+  }
+  holes = __any_sync(0xffffffffu, holes);
+  if (lane == 0) a.own[row] = {0, count, row * a.width, holes ? 1 : 0};
+}
+
+// The rows, and the queries to fp16: a row of a head times a power of two that brings its largest value to [2^10, 2^11), whose inverse goes to
 // q_scale.  A query with a value that is not finite becomes NaN.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
-kv4_unpack16_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ pages, int n, int width, const int* __restrict__ row_start,
-                    const int* __restrict__ row_pos0, int n_pages, int nkv, __half* __restrict__ k_out,
-                    __half* __restrict__ v_out, int* __restrict__ table, const __nv_bfloat16* __restrict__ q, int64_t q_stride, int T, int nh,
-                    __half* __restrict__ q_out, float* __restrict__ q_scale) {
+kv4_prompt_rows_kernel(const C4Prompt a) {
   pdl_trigger();
   pdl_wait();
-  const int64_t page_blocks = (int64_t)n * nkv;
-  if (blockIdx.x < page_blocks) {
-    const int i = (int)(blockIdx.x / nkv), kv = (int)(blockIdx.x % nkv);
-    const int page = __ldcg(pages + i);
-    const bool there = page >= 0 && page < n_pages;
-    if (kv == 0 && threadIdx.x == 0) table[i] = there ? i : -1;
-    if (there) {
-      const int row = i / width, held = __ldcg(row_pos0 + row) + __ldcg(row_start + row + 1) - __ldcg(row_start + row) - i % width * PAGE;
-      const int64_t at = ((int64_t)i * nkv + kv) * PAGE * HD;
-      c4_unpack<HD, true>(pool + ((int64_t)page * nkv + kv) * page_bytes(HD), true, held, k_out + at, v_out + at);
-    }
+  const int row_blocks = (a.rows + C4_THREADS / 32 - 1) / (C4_THREADS / 32);
+  if ((int)blockIdx.x < row_blocks) {
+    const int row = blockIdx.x * (C4_THREADS / 32) + (threadIdx.x >> 5);
+    if (row < a.rows) c4_row(a, row);
     return;
   }
   constexpr int LANES = HD / 8, GROUPS = C4_THREADS / LANES;           // eight features a lane
-  const int64_t item = (blockIdx.x - page_blocks) * GROUPS + threadIdx.x / LANES;
+  const int64_t item = (int64_t)(blockIdx.x - row_blocks) * GROUPS + threadIdx.x / LANES;
   const int j = threadIdx.x % LANES;
-  const bool live = item < (int64_t)T * nh;
-  const int64_t t = live ? item / nh : 0;
-  const int head = live ? (int)(item % nh) : 0;
+  const bool live = item < (int64_t)a.T * a.nh;
+  const int64_t t = live ? item / a.nh : 0;
+  const int head = live ? (int)(item % a.nh) : 0;
   float x[8];
-  load_vec_cg(q + t * q_stride + (int64_t)head * HD + 8 * j, x);
+  load_vec_cg(a.q + t * a.q_stride + (int64_t)head * HD + 8 * j, x);
   float top = 0.0f;
   bool finite = true;
 #pragma unroll
@@ -293,8 +313,22 @@ kv4_unpack16_kernel(const unsigned char* __restrict__ pool, const int* __restric
   __align__(16) __half h[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) h[e] = finite ? __float2half_rn(x[e] * up) : __ushort_as_half(0x7e00);
-  *reinterpret_cast<uint4*>(q_out + (t * nh + head) * HD + 8 * j) = *reinterpret_cast<const uint4*>(h);
-  if (j == 0) q_scale[t * nh + head] = down;
+  *reinterpret_cast<uint4*>(a.q_out + (t * a.nh + head) * HD + 8 * j) = *reinterpret_cast<const uint4*>(h);
+  if (j == 0) a.q_scale[t * a.nh + head] = down;
+}
+
+// The pages of all rows: a block per (row, page, kv head).  Nothing is written for a page that is not there.
+template <int HD>
+__global__ void __launch_bounds__(C4_THREADS)
+kv4_unpack16_kernel(const C4Prompt a) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = (int)(blockIdx.x / a.nkv), kv = (int)(blockIdx.x % a.nkv), row = i / a.width, j = i % a.width;
+  const int page = __ldcg(a.block_table + (int64_t)row * a.bt_stride + j);
+  if (page < 0 || page >= a.n_pages) return;
+  const int held = __ldcg(a.row_pos0 + row) + __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row) - j * PAGE;
+  const int64_t at = ((int64_t)i * a.nkv + kv) * PAGE * HD;
+  c4_unpack<HD, true>(a.pool + ((int64_t)page * a.nkv + kv) * page_bytes(HD), true, held, a.k_out + at, a.v_out + at);
 }
 
 }  // namespace exl3
@@ -343,18 +377,24 @@ extern "C" int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages
   return launch_status("kv4_load");
 }
 
-extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* pages, int rows, int width, const int* row_start, const int* row_pos0,
-                                 int nkv, int hd, void* k_out, void* v_out,
-                                 int* table, const void* q, int64_t q_stride, int T, int nh, void* q_out, float* q_scale, cudaStream_t stream) {
+extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* block_table, int bt_stride, int rows, int width, const int* row_start,
+                                 const int* row_pos0, int nkv, int hd, void* k_out, void* v_out, void* own, const void* q, int64_t q_stride, int T, int nh,
+                                 void* q_out, float* q_scale, cudaStream_t stream) {
   if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
-  const int per = C4_THREADS / (hd / 8), n = rows * width;
-  const int64_t blocks = (int64_t)n * nkv + ((int64_t)T * nh + per - 1) / per;
-  if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
-  auto go = [&](auto kernel) {
-    launch_pdl(kernel, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, static_cast<const unsigned char*>(pool), pages, n, width, row_start, row_pos0, (int)n_pages,
-               nkv, static_cast<__half*>(k_out), static_cast<__half*>(v_out), table, static_cast<const __nv_bfloat16*>(q), q_stride, T, nh,
-               static_cast<__half*>(q_out), q_scale);
+  const int per = C4_THREADS / (hd / 8);
+  const int64_t blocks = (int64_t)rows * width * nkv, q_blocks = ceil_div(rows, C4_THREADS / 32) + ((int64_t)T * nh + per - 1) / per;
+  if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX || q_blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
+  C4Prompt a = {};
+  a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.nkv = nkv;
+  a.block_table = block_table; a.bt_stride = bt_stride; a.width = width; a.rows = rows;
+  a.row_start = row_start; a.row_pos0 = row_pos0;
+  a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.T = T; a.nh = nh;
+  a.k_out = static_cast<__half*>(k_out); a.v_out = static_cast<__half*>(v_out); a.q_out = static_cast<__half*>(q_out); a.q_scale = q_scale;
+  a.own = static_cast<FaRow*>(own);
+  auto go = [&](auto first, auto second) {
+    launch_pdl(first, dim3((unsigned)q_blocks), dim3(C4_THREADS), 0, stream, a);
+    launch_pdl(second, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, a);
   };
-  if (hd == 64) go(kv4_unpack16_kernel<64>); else go(kv4_unpack16_kernel<128>);
+  if (hd == 64) go(kv4_prompt_rows_kernel<64>, kv4_unpack16_kernel<64>); else go(kv4_prompt_rows_kernel<128>, kv4_unpack16_kernel<128>);
   return launch_status("kv4_unpack16");
 }

@@ -2053,11 +2053,10 @@ def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv
     """Prompts: the rows' pages and the queries in fp16 in scratch memory, and the tcgen05 attention over them (attention_prefill_f16.cu)."""
     T, rows, width = q.shape[0], row_pos0.numel(), block_table.shape[1]
     up = lambda n: -(-n // 16) * 16
-    need = 4 * rows * width * kv_heads * KV4_PAGE * head_dim + up(2 * T * heads * head_dim) + up(4 * T * heads) + up(4 * rows * width)
+    need = 4 * rows * width * kv_heads * KV4_PAGE * head_dim + up(2 * T * heads * head_dim) + up(4 * T * heads) + 16 * rows
     scratch = workspace.plain(need // 4) if workspace is not None else torch.empty(need // 4, dtype=torch.float32, device=q.device)
-    pages = block_table[:rows] if block_table.stride(0) == width else block_table[:rows].contiguous()
-    rc = _entry("exl3_kv4_prompt", "plipplpiippppiiiiifpl")(
-        _addr(q), q.stride(0), T, _addr(out), _addr(pool), pool.shape[0], _addr(pages), rows, width, _addr(row_start), _addr(row_pos0),
+    rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifpl")(
+        _addr(q), q.stride(0), T, _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), rows, width, _addr(row_start), _addr(row_pos0),
         _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, _addr(scratch), need, _raw_stream())
     if rc:
         _check(rc, "kv4_attn")
