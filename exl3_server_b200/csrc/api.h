@@ -467,11 +467,13 @@ int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float
 int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
                   cudaStream_t stream);
 // Pages and queries in fp16 for the prompt attention and where each row's pages are (own [rows], see cache4_rows.cuh), and the attention of prompts over
-// a table [rows, width] of pages; pages that are not there, or beyond the table, are hidden.
+// a table [rows, width] of pages; pages that are not there, or beyond the table, are hidden.  tops: float2 [rows, nkv, exl3_kv4_prompt_parts(width)],
+// undo: float2 [rows, nkv], the factors of the products with the keys and with the values.
+int exl3_kv4_prompt_parts(int width);
 int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* block_table, int bt_stride, int rows, int width, const int* row_start,
-                      const int* row_pos0, int nkv, int hd, void* k_out, void* v_out, void* own, const void* q, int64_t q_stride, int T, int nh,
+                      const int* row_pos0, int window, int nkv, int hd, void* k_out, void* v_out, void* own, void* tops, void* undo, const void* q, int64_t q_stride, int T, int nh,
                       void* q_out, float* q_scale, cudaStream_t stream);
-long long exl3_kv4_prompt_scratch(int T, int rows, int pages, int nh, int nkv, int hd);
+long long exl3_kv4_prompt_scratch(int T, int rows, int width, int nh, int nkv, int hd);
 int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
                     int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0, int n_tiles, int nh,
                     int nkv, int hd, int window, float scale, void* scratch, long long scratch_bytes, cudaStream_t stream);

@@ -222,13 +222,16 @@ struct FaOpts {
   float dist_mul;
   const float* gate;           // a factor per (token, query head) on the output; null: none
   const float* q_scale;        // fp16: what the scores of a (token, query head) are multiplied by beside the scale
+  const float2* undo;          // fp16: per (row, kv head), what its products with keys (scores) and with values are multiplied by
   const FaRow* own;            // fp16: where the copies of the rows' pages are
   int table_pages;             // fp16: pages of the pool that the block table speaks of
 };
-// What the scores of row `row` of q are multiplied by (base-2 units).
-__device__ inline float fa_score_mul(const FaOpts& opts, float scale_log2, int64_t row, bool there, int nh, int head) {
+// What the scores of row `row` of q, of the sequence b, are multiplied by (base-2 units); a positive number, so that a hidden score stays -inf.
+__device__ inline float fa_score_mul(const FaOpts& opts, float scale_log2, int64_t row, bool there, int nh, int head, int b, int nkv) {
   const float mul = opts.cap_in > 0.0f ? opts.cap_log2 : scale_log2;
-  return FA_F16 && there ? mul * __ldcg(opts.q_scale + row * nh + head) : mul;
+  if (!FA_F16) return mul;
+  const float f = there ? __ldcg(opts.q_scale + row * nh + head) * __ldcg(opts.undo + (int64_t)b * nkv + head / (nh / nkv)).x : 1.0f;
+  return fminf(fmaxf(mul * f, 1.1754944e-38f), 3.4028235e38f);
 }
 // Whether a page of keys from key0 on holds a key with a bias for one of a warp's 32 queries from position p0 on.
 __device__ inline bool fa_near(int key0, int p0, int dist_len) {
@@ -255,6 +258,7 @@ struct FaTile {
   int n_pages;     // pages to walk
   const int* bt;   // the sequence's page table
   FaRow own;       // fp16
+  int b;           // the sequence
 };
 // Page j of the sequence in the pools of keys and values (a copy of a page that is not there would be at -1: zeros, to be hidden).
 __device__ inline int fa_page(const int* bt, const FaRow& own, const FaOpts& opts, int j) {
@@ -298,6 +302,7 @@ __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride
   if (FA_F16) t.n_pages = max(t.n_pages, 1);              // (queries before position 0: one page, hidden from all)
   t.bt = block_table + (int64_t)b * bt_stride;
   t.own = fa_row(opts, b);
+  t.b = b;
   return t;
 }
 
@@ -425,8 +430,8 @@ __device__ inline void fa_rescale_slowly(uint32_t taddr, float corr) {
 }
 // What a row of O is multiplied by at the end.  A sink is a key of score 0 without a value: one more term in the sum, in
 // the units of the reference maximum.
-__device__ inline float fa_inverse(float l_run, float m_used, int sink, const FaOpts& opts, int head, int row, int nh, bool in) {
-  if (FA_F16 && l_run == 0.0f) return 0.0f;                  // a query that sees nothing
+__device__ inline float fa_inverse(float l_run, float m_used, int sink, const FaOpts& opts, int head, int row, int nh, bool in, int b, int nkv) {
+  if (FA_F16) return l_run == 0.0f ? 0.0f : __ldcg(opts.undo + (int64_t)b * nkv + head / (nh / nkv)).y / l_run;      // (0: a query that sees nothing)
   float inv = 1.0f / (sink ? l_run + fa_exp2((opts.sink_vals ? __ldg(opts.sink_vals + head) * 1.4426950408889634f : 0.0f) - m_used) : l_run);
   if (opts.gate && in) inv *= __ldcg(opts.gate + (int64_t)row * nh + head);
   return inv;
@@ -639,7 +644,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int p_first = tw.p_first, p_last = tw.p_last, n_blocks = tw.n_pages, page_lo = tw.page_lo, rows = tw.rows;
     const int kept = tw.kept;
     const int p = p_first + r;                               // this row's position
-    const float score_mul = fa_score_mul(opts, scale_log2, tw.row0 + r, r < rows, nh, head);
+    const float score_mul = fa_score_mul(opts, scale_log2, tw.row0 + r, r < rows, nh, head, tw.b, nkv);
     float m_used = -INFINITY, l_run = 0.0f;
     // The row of S_f is asked for as soon as the row of P_(f-1) is on its way into tensor memory (the first of a
     // tile: here), so that the load's latency and the store's pass together.
@@ -699,7 +704,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       ok = fa_mbar_wait(pv_done + (fl & 1), (fl >> 1) & 1);
       if (ok) {
         fa_fence_after();
-        const float inv = fa_inverse(l_run, m_used, sink, opts, head, tw.row0 + r, nh, r < rows);
+        const float inv = fa_inverse(l_run, m_used, sink, opts, head, tw.row0 + r, nh, r < rows, tw.b, nkv);
         fa_store_row<FA_HD>(tmem_o + lane_addr, inv, out + ((int64_t)(tw.row0 + r) * nh + head) * FA_HD, r < rows);
         fa_fence_before();                                 // O is read: the next tile's first product may write it
       }
@@ -846,7 +851,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const int r = threadIdx.x;
     const int p = p_first + r;
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
-    const float score_mul = fa_score_mul(opts, scale_log2, row_start[b] + q0 + r, r < rows, nh, head);
+    const float score_mul = fa_score_mul(opts, scale_log2, row_start[b] + q0 + r, r < rows, nh, head, b, nkv);
     float m_used = -INFINITY, l_run = 0.0f;
     for (int j = 0; j < n_blocks && ok; ++j) {
       if (!fa_mbar_wait(s_full, j & 1)) { ok = false; break; }
@@ -879,7 +884,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       ok = fa_mbar_wait(pv_done, jl & 1);
       if (ok) {
         fa_fence_after();
-        const float inv = fa_inverse(l_run, m_used, sink, opts, head, row_start[b] + q0 + r, nh, r < rows);
+        const float inv = fa_inverse(l_run, m_used, sink, opts, head, row_start[b] + q0 + r, nh, r < rows, b, nkv);
         __nv_bfloat16* dst = out + ((int64_t)(row_start[b] + q0 + r) * nh + head) * 64;
 #pragma unroll 1
         for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -1111,7 +1116,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const FaTile tn = next < n_items ? tile_of(next) : t;  // asked for an item ahead
       const int head = 2 * (item % n_pairs) + s;
       const int p = t.p_first + r, n_pages = t.n_pages;
-      const float score_mul = fa_score_mul(opts, scale_log2, t.row0 + r, r < t.rows, nh, head);
+      const float score_mul = fa_score_mul(opts, scale_log2, t.row0 + r, r < t.rows, nh, head, t.b, nkv);
       float m_used = -INFINITY, l_run = 0.0f;
       uint32_t sr[2][32];
       auto ask_s = [&](int f, bool there) -> bool {         // there: the barrier is known to have flipped
@@ -1159,7 +1164,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         if (ok) {
           fa_fence_after();
           const bool in = r < t.rows;
-          const float inv = fa_inverse(l_run, m_used, sink, opts, head, t.row0 + r, nh, in);
+          const float inv = fa_inverse(l_run, m_used, sink, opts, head, t.row0 + r, nh, in, t.b, nkv);
           fa_store_row<128>(tmem_o, inv, out + ((int64_t)(t.row0 + r) * nh + head) * 128, in);
           fa_fence_before();                                 // O is read: the next item's first product may write it
         }
@@ -1237,7 +1242,7 @@ static int fa_run(const void* q, int64_t q_row_stride, int T, void* out, const v
                   const int* tile_q0, int n_tiles, int nh, int nkv, int hd, int page, int window,
                   int chunk, int sink, float scale, int variant, int keep_first, float softcap,
                   const float* sink_vals, const float* dist, int dist_len, const float* gate,
-                  const float* q_scale, const FaRow* own, int table_pages, cudaStream_t stream) {
+                  const float* q_scale, const float2* undo, const FaRow* own, int table_pages, cudaStream_t stream) {
   if (n_tiles == 0) return 0;
   if (dist_len < 0 || (dist_len > 0 && dist == nullptr)) {
     set_error("attn_prefill_tc: a table of %d distance biases is missing", dist_len);
@@ -1257,6 +1262,7 @@ static int fa_run(const void* q, int64_t q_row_stride, int T, void* out, const v
   opts.dist_len = dist_len;
   opts.gate = gate;
   opts.q_scale = q_scale;
+  opts.undo = undo;
   opts.own = own;
   opts.table_pages = table_pages;
   opts.dist_mul = softcap > 0.0f ? 1.0f / softcap : 1.0f / scale;

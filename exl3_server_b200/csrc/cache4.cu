@@ -184,16 +184,16 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t qkv_stride, __nv
   }
 }
 
-// fp16 holds up to 65,504; NaN stays.
+// fp16 holds up to 65,504 (places that no query sees may hold more than a row's factor is made for); NaN stays.
 template <typename T> __device__ inline T c4_out(float v);
 template <> __device__ inline __nv_bfloat16 c4_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ inline __half c4_out<__half>(float v) { return __float2half_rn(fabsf(v) > 65504.0f ? copysignf(65504.0f, v) : v); }
 
 // A page of a kv head, keys and values, to T [64][HD] each: a thread has eight features of both of a few tokens, and asks for all of their words
 // before it uses the first.  CLEAN, for a product that multiplies hidden values by zero: places from `held` on are zeros, and a token with a NaN
-// among its values has zeros there and NaN in all of its key, which a mask can hide.
+// among its values has zeros there and NaN in all of its key, which a mask can hide; keys are multiplied by k_up, values by v_up (powers of two).
 template <int HD, bool CLEAN, typename T>
-__device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool there, int held, T* __restrict__ k_out, T* __restrict__ v_out) {
+__device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool there, int held, float k_up, float v_up, T* __restrict__ k_out, T* __restrict__ v_out) {
   constexpr int LANES = HD / 8, N = PAGE * LANES / C4_THREADS;
   uint32_t kw[N], kc[N], vw[N], vc[N][2];
   const int j = threadIdx.x % LANES, half = j >> 3, jj = j & 7;
@@ -222,8 +222,9 @@ __device__ inline void c4_unpack(const unsigned char* __restrict__ base, bool th
     __align__(16) T k[8], v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = fmaf(word_sc(kw[i]), c4_code(kc[i], 4 * (e / 2 + 4 * (e % 2))), word_mn(kw[i]));
-      const float y = fmaf(word_sc(vw[i]), c4_code(jj < 4 ? vc[i][e >> 2] : vc[i][e >> 2] >> 16, 4 * (e & 3)), word_mn(vw[i]));
+      float x = fmaf(word_sc(kw[i]), c4_code(kc[i], 4 * (e / 2 + 4 * (e % 2))), word_mn(kw[i]));
+      float y = fmaf(word_sc(vw[i]), c4_code(jj < 4 ? vc[i][e >> 2] : vc[i][e >> 2] >> 16, 4 * (e & 3)), word_mn(vw[i]));
+      if (CLEAN) { x *= k_up; y *= v_up; }
       k[e] = c4_out<T>(zero ? 0.0f : hide_key ? __int_as_float(0x7fc00000) : x);
       v[e] = c4_out<T>(zero ? 0.0f : y);
     }
@@ -242,7 +243,7 @@ kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
   const int page = __ldcg(pages + blockIdx.x), kv = blockIdx.y;
   const bool there = page >= 0 && page < n_pages;
   const int64_t at = ((int64_t)blockIdx.x * nkv + kv) * PAGE * HD;
-  c4_unpack<HD, false>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), there, PAGE, k_out + at, v_out + at);
+  c4_unpack<HD, false>(pool + ((int64_t)(there ? page : 0) * nkv + kv) * page_bytes(HD), there, PAGE, 1.0f, 1.0f, k_out + at, v_out + at);
 }
 
 // ---- prompts: fp16 copies of the rows' pages and of the queries, for the prompt attention ------------------------------------------
@@ -253,13 +254,73 @@ struct C4Prompt {
   const int* block_table;
   int bt_stride, width, rows;
   const int *row_start, *row_pos0;
+  int window, parts;
   const __nv_bfloat16* q;
   int64_t q_stride;
   int T, nh;
   __half *k_out, *v_out, *q_out;
   float* q_scale;
   FaRow* own;
+  float2* tops;          // [rows][nkv][parts]: the largest |key| and |value| of a part of a row's pages
+  float2* undo;          // [rows][nkv]: what the products of the copied keys and of the copied values are multiplied by
 };
+constexpr int C4_MAX_PARTS = 32;                                       // one a lane
+
+// The exponent of the power of two that brings numbers up to `top` below 2^15.  Down to 2^-110 that leaves all of fp16's bits to what is within 2^28
+// of the top.
+__device__ inline int c4_up(float top) { return top > 0.0f ? min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -113), 96) : 0; }
+__device__ inline float c4_pow2(int e) { return __int_as_float((127 + e) << 23); }
+
+// A warp per (row, kv head, part of the row's pages): the largest |key| and |value| among the places that some query of the row sees, from the
+// groups' words: a group's values lie between mn and mn + 15 sc.  NaN groups do not count.
+template <int HD> __device__ inline void c4_tops(const C4Prompt& a, int64_t item) {
+  constexpr int SPP = HD / 64, NG = HD / 32, AHEAD = 4;                // tiles of a page, groups of a token, pages asked for at a time
+  const int lane = threadIdx.x & 31, part = (int)(item % a.parts), kv = (int)(item / a.parts % a.nkv), row = (int)(item / a.parts / a.nkv);
+  const int pos0 = __ldcg(a.row_pos0 + row), end = pos0 + __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row);
+  const int first = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;    // places first .. end - 1 are seen
+  const int pages = end > 0 ? min((end - 1) / PAGE + 1, a.width) : 0;
+  float top[2] = {0.0f, 0.0f};
+  for (int j0 = first / PAGE + part * AHEAD; j0 < pages; j0 += a.parts * AHEAD) {
+    uint4 w[AHEAD][SPP][2];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int page = j0 + u < pages ? __ldcg(a.block_table + (int64_t)row * a.bt_stride + j0 + u) : -1;
+      const bool there = page >= 0 && page < a.n_pages;
+      const unsigned char* base = a.pool + ((int64_t)(there ? page : 0) * a.nkv + kv) * page_bytes(HD) + 16 * lane;
+#pragma unroll
+      for (int i = 0; i < SPP; ++i) {
+        w[u][i][0] = w[u][i][1] = make_uint4(0, 0, 0, 0);
+        if (there) {
+          w[u][i][0] = load_raw_cg(base + i * TILE + K_WORDS);
+          w[u][i][1] = load_raw_cg(base + i * TILE + V_WORDS);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int i = 0; i < SPP; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                                  // word 4 lane + e of the tile: its token and group
+          const int place = (j0 + u) * PAGE + i * tile_tokens(HD) + (4 * lane + e) / NG;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint4& v = w[u][i][x];
+            const uint32_t word = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+            if (place >= first && place < end) top[x] = c4_max3(top[x], fabsf(word_mn(word)), fabsf(fmaf(word_sc(word), 15.0f, word_mn(word))));
+          }
+        }
+  }
+  top[0] = warp_max(top[0]);
+  top[1] = warp_max(top[1]);
+  if (lane == 0) a.tops[item] = make_float2(top[0], top[1]);
+}
+// The exponents of a row's keys and values (every lane of the warp).
+__device__ inline int2 c4_row_up(const C4Prompt& a, int64_t row_and_head) {
+  const int lane = threadIdx.x & 31;
+  const float2 t = lane < a.parts ? __ldcg(a.tops + row_and_head * a.parts + lane) : make_float2(0.0f, 0.0f);
+  return make_int2(c4_up(warp_max(t.x)), c4_up(warp_max(t.y)));
+}
 
 // A warp per row: where the copies of its pages will be, and whether some page that its queries look for is not there.
 __device__ inline void c4_row(const C4Prompt& a, int row) {
@@ -275,7 +336,7 @@ __device__ inline void c4_row(const C4Prompt& a, int row) {
   if (lane == 0) a.own[row] = {0, count, row * a.width, holes ? 1 : 0};
 }
 
-// The rows, and the queries to fp16: a row of a head times a power of two that brings its largest value to [2^10, 2^11), whose inverse goes to
+// The rows, their keys' and values' sizes, and the queries to fp16: a row of a head times a power of two that brings its largest value to [2^10, 2^11), whose inverse goes to
 // q_scale.  A query with a value that is not finite becomes NaN.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
@@ -288,8 +349,15 @@ kv4_prompt_rows_kernel(const C4Prompt a) {
     if (row < a.rows) c4_row(a, row);
     return;
   }
+  const int64_t top_items = (int64_t)a.rows * a.nkv * a.parts;
+  const int top_blocks = (int)((top_items + C4_THREADS / 32 - 1) / (C4_THREADS / 32));
+  if ((int)blockIdx.x < row_blocks + top_blocks) {
+    const int64_t item = (int64_t)(blockIdx.x - row_blocks) * (C4_THREADS / 32) + (threadIdx.x >> 5);
+    if (item < top_items) c4_tops<HD>(a, item);
+    return;
+  }
   constexpr int LANES = HD / 8, GROUPS = C4_THREADS / LANES;           // eight features a lane
-  const int64_t item = (int64_t)(blockIdx.x - row_blocks) * GROUPS + threadIdx.x / LANES;
+  const int64_t item = (int64_t)(blockIdx.x - row_blocks - top_blocks) * GROUPS + threadIdx.x / LANES;
   const int j = threadIdx.x % LANES;
   const bool live = item < (int64_t)a.T * a.nh;
   const int64_t t = live ? item / a.nh : 0;
@@ -317,18 +385,21 @@ kv4_prompt_rows_kernel(const C4Prompt a) {
   if (j == 0) a.q_scale[t * a.nh + head] = down;
 }
 
-// The pages of all rows: a block per (row, page, kv head).  Nothing is written for a page that is not there.
+// The pages of all rows: a block per (row, page, kv head), times the powers of two that bring the row's keys and values of that head up to fp16's
+// largest; the block of a row's first page keeps what undoes them.  No copy is written of a page that is not there.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
 kv4_unpack16_kernel(const C4Prompt a) {
   pdl_trigger();
   pdl_wait();
   const int i = (int)(blockIdx.x / a.nkv), kv = (int)(blockIdx.x % a.nkv), row = i / a.width, j = i % a.width;
+  const int2 up = c4_row_up(a, (int64_t)row * a.nkv + kv);
+  if (j == 0 && threadIdx.x == 0) a.undo[row * a.nkv + kv] = make_float2(c4_pow2(-up.x), c4_pow2(-up.y));
   const int page = __ldcg(a.block_table + (int64_t)row * a.bt_stride + j);
   if (page < 0 || page >= a.n_pages) return;
   const int held = __ldcg(a.row_pos0 + row) + __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row) - j * PAGE;
   const int64_t at = ((int64_t)i * a.nkv + kv) * PAGE * HD;
-  c4_unpack<HD, true>(a.pool + ((int64_t)page * a.nkv + kv) * page_bytes(HD), true, held, a.k_out + at, a.v_out + at);
+  c4_unpack<HD, true>(a.pool + ((int64_t)page * a.nkv + kv) * page_bytes(HD), true, held, c4_pow2(up.x), c4_pow2(up.y), a.k_out + at, a.v_out + at);
 }
 
 }  // namespace exl3
@@ -377,12 +448,17 @@ extern "C" int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages
   return launch_status("kv4_load");
 }
 
+// Parts of a row's pages for the search of its largest values: a warp takes four pages at a time.
+extern "C" int exl3_kv4_prompt_parts(int width) { return width < 4 * C4_MAX_PARTS ? ceil_div(width, 4) : C4_MAX_PARTS; }
+
 extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* block_table, int bt_stride, int rows, int width, const int* row_start,
-                                 const int* row_pos0, int nkv, int hd, void* k_out, void* v_out, void* own, const void* q, int64_t q_stride, int T, int nh,
+                                 const int* row_pos0, int window, int nkv, int hd, void* k_out, void* v_out, void* own, void* tops, void* undo, const void* q, int64_t q_stride, int T, int nh,
                                  void* q_out, float* q_scale, cudaStream_t stream) {
   if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
   const int per = C4_THREADS / (hd / 8);
-  const int64_t blocks = (int64_t)rows * width * nkv, q_blocks = ceil_div(rows, C4_THREADS / 32) + ((int64_t)T * nh + per - 1) / per;
+  const int warps = C4_THREADS / 32, parts = exl3_kv4_prompt_parts(width);
+  const int64_t blocks = (int64_t)rows * width * nkv;
+  const int64_t q_blocks = ceil_div(rows, warps) + ((int64_t)rows * nkv * parts + warps - 1) / warps + ((int64_t)T * nh + per - 1) / per;
   if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX || q_blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
   C4Prompt a = {};
   a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.nkv = nkv;
@@ -390,7 +466,8 @@ extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* b
   a.row_start = row_start; a.row_pos0 = row_pos0;
   a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.T = T; a.nh = nh;
   a.k_out = static_cast<__half*>(k_out); a.v_out = static_cast<__half*>(v_out); a.q_out = static_cast<__half*>(q_out); a.q_scale = q_scale;
-  a.own = static_cast<FaRow*>(own);
+  a.own = static_cast<FaRow*>(own); a.tops = static_cast<float2*>(tops); a.undo = static_cast<float2*>(undo);
+  a.window = window; a.parts = parts;
   auto go = [&](auto first, auto second) {
     launch_pdl(first, dim3((unsigned)q_blocks), dim3(C4_THREADS), 0, stream, a);
     launch_pdl(second, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, a);

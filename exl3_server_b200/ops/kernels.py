@@ -2002,7 +2002,9 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     tokens (None: never more than a few).  ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's).
 
     A few tokens a row (``_kv4_walks``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
-    unpacked to fp16 (values beyond 65,504 count as that) and go through the tcgen05 attention."""
+    unpacked to fp16, times a power of two for a row's keys and one for its values of a head (what is 2^28 below the largest that the row's queries see
+    loses bits), and go through the tcgen05 attention.  A NaN among a token's values makes its group of 32 features NaN for those who see it, and
+    in the prompt form all features of its head."""
     plain = q.is_contiguous()
     if q.dtype is not torch.bfloat16 or q.ndim != 2 or q.shape[1] != heads * head_dim or not (plain or q.stride(1) == 1):
         raise KernelLibraryError(f"kv4_attn: q must be bfloat16 [tokens, {heads * head_dim}], got {q.dtype} {tuple(q.shape)}")
@@ -2053,7 +2055,8 @@ def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv
     """Prompts: the rows' pages and the queries in fp16 in scratch memory, and the tcgen05 attention over them (attention_prefill_f16.cu)."""
     T, rows, width = q.shape[0], row_pos0.numel(), block_table.shape[1]
     up = lambda n: -(-n // 16) * 16
-    need = 4 * rows * width * kv_heads * KV4_PAGE * head_dim + up(2 * T * heads * head_dim) + up(4 * T * heads) + 16 * rows
+    # copies of the pages, the queries and their factors, where rows' copies are, sizes by parts and what undoes their factors
+    need = 4 * rows * width * kv_heads * KV4_PAGE * head_dim + up(2 * T * heads * head_dim) + up(4 * T * heads) + 16 * rows + 8 * rows * kv_heads * (min(-(-width // 4), 32) + 1)
     scratch = workspace.plain(need // 4) if workspace is not None else torch.empty(need // 4, dtype=torch.float32, device=q.device)
     rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifpl")(
         _addr(q), q.stride(0), T, _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), rows, width, _addr(row_start), _addr(row_pos0),

@@ -2,11 +2,11 @@
 is a matter of time and must not show in its results.
 
 Tolerances are test_cache4_gpu.py's (``Case.check``): the result is rounded to bfloat16, the terms to fp16, in the unpacked form keys, values and
-queries to fp16 as well: 2^-7 of the largest value and what rounded keys move."""
+queries to fp16 as well, after a power of two that brings a row's largest near fp16's: 2^-7 of the largest value and what rounded keys move."""
 import pytest
 import torch
 
-from plain_lowbit import attend
+from plain_lowbit import attend, rounded4
 from test_cache4_gpu import DEV, Case, K, ints
 
 pytestmark = pytest.mark.gpu
@@ -16,6 +16,20 @@ pytestmark = pytest.mark.gpu
 def way(request, monkeypatch):
     monkeypatch.setattr(K(), "_kv4_walks", lambda *a: request.param)
     return request.param
+
+
+def refilled(c, f):
+    """The case's keys and values times f, a number or one for each key/value head, and its queries as they are."""
+    g, d = c.g, c.d
+    kv = c.qkv[:, c.h * d:].float().view(-1, 2, g, d) * torch.as_tensor(f, device=DEV).view(-1, 1)
+    qkv = torch.cat([c.qkv[:, :c.h * d], kv.reshape(-1, 2 * g * d).bfloat16()], 1)
+    lens = [a + n for a, n in c.rows]
+    K().kv4_store(qkv, None, ints([p for L in lens for p in range(L)]), ints([r for r, L in enumerate(lens) for _ in range(L)]), c.table, c.pool, c.h, g, d)
+    at = 0
+    for r, L in enumerate(lens):
+        x = qkv[at:at + L, c.h * d:].cpu().view(L, 2, g, d)
+        c.k[r], c.v[r] = rounded4(x[:, 0]), rounded4(x[:, 1])
+        at += L
 
 
 # ---- pages that are not there ---------------------------------------------------------------------------------------------------
@@ -71,3 +85,34 @@ def test_queries_before_the_first_position_get_zeros(way, first, heads, kv_heads
         want = attend(c.q[n:n + 1].cpu().view(1, heads, d), c.k[0], c.v[0], 0, d ** -0.5)[0]
         assert float((out[n] - want).abs().max()) <= 2.0 ** -7 * float(c.v[0].abs().max())
     K().check_status()
+
+
+# ---- sizes ----------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("exponent", [-60, -30, -22, -18, -12, 0, 12, 20, 60])
+@pytest.mark.parametrize("d,new", [(64, 70), (128, 150)])
+def test_sizes(way, exponent, d, new):
+    """Powers of two in q and in k and v move nothing but the result's size (k up, q down: the same scores)."""
+    c = Case([(90, new), (33, 20)], 4, 2, d, seed=11)
+    base = c.run()
+    f = 2.0 ** exponent
+    refilled(c, f)
+    out = c.run(q=(c.q.float() / f).bfloat16())
+    assert float((out.double() / f - base.double()).abs().max()) <= 2.0 ** -7 * max(float(v.abs().max()) for v in c.v) / f
+
+
+@pytest.mark.parametrize("d,new", [(64, 70), (128, 150)])
+def test_values_of_rows_and_heads_differ_in_size(way, d, new):
+    """A head's values 2^-25, its neighbour's 2^18: each result is as good as its own values allow."""
+    c = Case([(90, new), (33, 20)], 4, 2, d, seed=24, q_scale=2.0 ** -10)
+    refilled(c, [2.0 ** -25, 2.0 ** 18])
+    out, at = c.run().double().cpu().view(-1, 4, d), 0
+    for r, (ctx, n) in enumerate(c.rows):
+        for i in (0, n - 1):
+            q = c.q[at + i:at + i + 1].cpu().view(1, 4, d)
+            want = attend(q, c.k[r], c.v[r], ctx + i, d ** -0.5)[0]
+            for g in range(2):
+                moved = 2.0 ** -12 * d ** -0.5 * float(q[0, 2 * g:2 * g + 2].double().norm(dim=-1).max() * c.k[r][:, g].norm(dim=-1).max())
+                err = float((out[at + i, 2 * g:2 * g + 2] - want[2 * g:2 * g + 2]).abs().max())
+                assert err <= (2.0 ** -7 + 2 * moved) * float(c.v[r][:, g].abs().max()), (r, i, g)
+        at += n
