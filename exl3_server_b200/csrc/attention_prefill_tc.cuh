@@ -240,7 +240,7 @@ __device__ inline bool fa_near(int key0, int p0, int dist_len) {
 // Pages from the sequence's start that a tile walks before the pages of its window: those that hold kept first keys
 // and lie before the window's first page.
 __device__ inline int fa_kept_pages(int window, int keep_first, int page_lo) {
-  return (window > 0 && keep_first > 0) ? min((keep_first + FA_BK - 1) / FA_BK, page_lo) : 0;
+  return (!FA_F16 && window > 0 && keep_first > 0) ? min((keep_first + FA_BK - 1) / FA_BK, page_lo) : 0;
 }
 // tanh by one exponential and one reciprocal: 1 - 2 / (1 + e^(2x)); good to 1e-6 absolutely.
 __device__ inline float fa_tanh(float x) {
@@ -257,31 +257,30 @@ struct FaTile {
   int kept;        // pages from the sequence's start that are walked before it (kept first keys)
   int n_pages;     // pages to walk
   const int* bt;   // the sequence's page table
-  FaRow own;       // fp16
-  int b;           // the sequence
+  int mask_from;   // pages that reach beyond this position are masked: p_first, or (fp16) FA_HOLES where some page has to be hidden as a whole
 };
-// Page j of the sequence in the pools of keys and values (a copy of a page that is not there would be at -1: zeros, to be hidden).
-__device__ inline int fa_page(const int* bt, const FaRow& own, const FaOpts& opts, int j) {
-#ifdef EXL3_PREFILL_F16
-  return row_copy(own, bt, opts.table_pages, j);
-#else
-  return bt[j];
-#endif
-}
-// Whether the page of keys from key0 on is to be hidden from everyone.
-__device__ inline bool fa_missing(const int* bt, const FaRow& own, const FaOpts& opts, int key0) {
-#ifdef EXL3_PREFILL_F16
-  return own.holes && row_copy(own, bt, opts.table_pages, key0 / FA_BK) < 0;
-#else
-  return false;
-#endif
-}
+constexpr int FA_HOLES = INT32_MIN;
 __device__ inline FaRow fa_row(const FaOpts& opts, int b) {
 #ifdef EXL3_PREFILL_F16
   const int4 w = __ldcg(reinterpret_cast<const int4*>(opts.own + b));
   return {w.x, w.y, w.z, w.w};
 #else
   return {};
+#endif
+}
+__device__ inline bool fa_has_holes(const FaOpts& opts, int b) {
+#ifdef EXL3_PREFILL_F16
+  return __ldcg(&opts.own[b].holes) != 0;
+#else
+  return false;
+#endif
+}
+// Page j of the sequence in the pools of keys and values (a copy of a page that is not there would be at -1: zeros, to be hidden).
+__device__ inline int fa_page(const int* bt, const FaRow& own, const FaOpts& opts, int j) {
+#ifdef EXL3_PREFILL_F16
+  return row_copy(own, bt, opts.table_pages, j);
+#else
+  return bt[j];
 #endif
 }
 __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride, const int* row_start,
@@ -295,30 +294,32 @@ __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride
   t.p_first = row_pos0[b] + q0;
   t.p_last = t.p_first + t.rows - 1;
   int k_lo = (window > 0 && t.p_first - window + 1 > 0) ? t.p_first - window + 1 : 0;
-  if (chunk > 0) k_lo = max(k_lo, t.p_first / chunk * chunk);    // the block of positions of the tile's first query
+  if (!FA_F16 && chunk > 0) k_lo = max(k_lo, t.p_first / chunk * chunk);    // the block of positions of the tile's first query
   t.page_lo = k_lo / FA_BK;
   t.kept = fa_kept_pages(window, opts.keep_first, t.page_lo);
   t.n_pages = t.kept + t.p_last / FA_BK - t.page_lo + 1;
   if (FA_F16) t.n_pages = max(t.n_pages, 1);              // (queries before position 0: one page, hidden from all)
   t.bt = block_table + (int64_t)b * bt_stride;
-  t.own = fa_row(opts, b);
-  t.b = b;
+  t.mask_from = FA_F16 && fa_has_holes(opts, b) ? FA_HOLES : t.p_first;
   return t;
 }
 
 // ---- a row of 64 scores (thread = query row), for all kernels below ------------------------------------------------
-// Cap, distance biases and mask.  p0_warp: the position of the warp's first query.
-__device__ inline void fa_adjust(uint32_t (&sr)[2][32], const FaOpts& opts, int head, int key0, int p, int p_first,
-                                 int p_last, int p0_warp, int window, int chunk) {
-  const bool need_mask = (key0 + FA_BK - 1 > p_first) || (window > 0 && key0 <= p_last - window) ||
+// Cap, distance biases and mask (fp16: the mask alone).  p0_warp: the position of the warp's first query.  missing() says whether nobody sees this
+// page; it is asked where mask_from is FA_HOLES, and looks up all it needs: more registers in the loop over pages made it a tenth slower.
+template <typename Missing>
+__device__ inline void fa_adjust(uint32_t (&sr)[2][32], const FaOpts& opts, int head, int key0, int p, int mask_from,
+                                 int p_last, int p0_warp, int window, int chunk, Missing missing) {
+  if (FA_F16) chunk = 0;
+  const bool need_mask = (key0 + FA_BK - 1 > mask_from) || (window > 0 && key0 <= p_last - window) ||
                          (chunk > 0 && key0 < p_last / chunk * chunk);
-  if (opts.cap_in > 0.0f) {                                  // capped scores: tanh now, the cap with the scale below
+  if (!FA_F16 && opts.cap_in > 0.0f) {                       // capped scores: tanh now, the cap with the scale below
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int c = 0; c < 32; ++c) sr[h][c] = __float_as_uint(fa_tanh(__uint_as_float(sr[h][c]) * opts.cap_in));
   }
-  if (opts.dist_len > 0 && fa_near(key0, p0_warp, opts.dist_len)) {
+  if (!FA_F16 && opts.dist_len > 0 && fa_near(key0, p0_warp, opts.dist_len)) {
     // the biases of this row's distances p - key: neighbouring lanes read neighbouring entries
     const float* tab = dist_row(opts.dist, opts.dist_len, head) + (p - key0);
 #pragma unroll
@@ -330,22 +331,16 @@ __device__ inline void fa_adjust(uint32_t (&sr)[2][32], const FaOpts& opts, int 
   if (need_mask) {                                           // without branches: one test per page decides about the page
     int lo_key = (window > 0) ? p - window : -1;             // keys <= lo_key are out of the window
     if (chunk > 0) lo_key = max(lo_key, p / chunk * chunk - 1);   // or before the query's block of positions
+    const int hi_key = FA_F16 && mask_from == FA_HOLES && missing() ? -1 : p;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int c = 0; c < 32; ++c) {
         const int key = key0 + h * 32 + c;
-        const bool dead = (key > p) | ((key <= lo_key) & (key >= opts.keep_first));   // kept first keys stay
+        const bool dead = (key > hi_key) | ((key <= lo_key) & (FA_F16 || key >= opts.keep_first));   // kept first keys stay
         sr[h][c] = dead ? 0xff800000u : sr[h][c];            // -inf
       }
   }
-}
-// Nobody sees this page.
-__device__ inline void fa_hide(uint32_t (&sr)[2][32]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int c = 0; c < 32; ++c) sr[h][c] = 0xff800000u;
 }
 // Four independent chains for the maximum (and below for the sum): the row is long and a single chain would make every
 // step wait for the one before.
@@ -498,6 +493,11 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   auto tile_of = [&](int w) {                       // the block's first (w = 0) or second tile
     return fa_tile(w ? other : (int)blockIdx.y, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
   };
+  auto seq_of = [&](int w) { return !FA_F16 ? 0 : __ldcg(tile_seq + (w ? other : (int)blockIdx.y)); };
+  auto missing = [&](int w, int key0) {             // fp16: whether a page of that tile's sequence is not there
+    const int b = seq_of(w);
+    return fa_page(block_table + (int64_t)b * bt_stride, fa_row(opts, b), opts, key0 / FA_BK) < 0;
+  };
 
   if (threadIdx.x == 0) {
     fa_mbar_init(q_full, 1);
@@ -538,6 +538,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // for there delayed S by more than it cost here).  Page numbers come 32 at a time, lane i holding the number of
     // page c0 + i of the block's walk, a batch ahead.
     const FaTile ta = tile_of(0), tb = n_own == 2 ? tile_of(1) : ta;
+    const FaRow owna = fa_row(opts, seq_of(0)), ownb = fa_row(opts, seq_of(n_own - 1));
     const int n0 = ta.n_pages;
     const int n_total = n0 + (n_own == 2 ? tb.n_pages : 0);   // the block's pages, numbered through both tiles
     if (lane == 0) {
@@ -553,7 +554,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       if (c >= n_total) return 0;
       const FaTile& tc = c >= n0 ? tb : ta;
       const int jc = c >= n0 ? c - n0 : c;
-      return fa_page(tc.bt, tc.own, opts, jc < tc.kept ? jc : tc.page_lo + jc - tc.kept);
+      return fa_page(tc.bt, c >= n0 ? ownb : owna, opts, jc < tc.kept ? jc : tc.page_lo + jc - tc.kept);
     };
     int pgs = numbers(0), pgs_next = numbers(32);
     int copied = 0;                                          // pages whose copies were asked for
@@ -644,7 +645,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int p_first = tw.p_first, p_last = tw.p_last, n_blocks = tw.n_pages, page_lo = tw.page_lo, rows = tw.rows;
     const int kept = tw.kept;
     const int p = p_first + r;                               // this row's position
-    const float score_mul = fa_score_mul(opts, scale_log2, tw.row0 + r, r < rows, nh, head, tw.b, nkv);
+    const float score_mul = fa_score_mul(opts, scale_log2, tw.row0 + r, r < rows, nh, head, seq_of(w), nkv);
     float m_used = -INFINITY, l_run = 0.0f;
     // The row of S_f is asked for as soon as the row of P_(f-1) is on its way into tensor memory (the first of a
     // tile: here), so that the load's latency and the store's pass together.
@@ -670,8 +671,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       const bool p_free = f < 2 || fa_mbar_test(pv_done + st, ((f - 2) >> 1) & 1);
       const bool s_there = j + 1 < n_blocks && fa_mbar_test(s_full + (st ^ 1), ((f + 1) >> 1) & 1);
       const int key0 = (j < kept ? j : page_lo + j - kept) * FA_BK;
-      fa_adjust(sr, opts, head, key0, p, p_first, p_last, p_first + warp * 32, window, chunk);
-      if (fa_missing(tw.bt, tw.own, opts, key0)) fa_hide(sr);
+      fa_adjust(sr, opts, head, key0, p, tw.mask_from, p_last, p_first + warp * 32, window, chunk, [&] { return missing(w, key0); });
       const float mx = fa_row_max(sr) * score_mul;           // scale > 0: max and scale commute
       // lazy rescale: move the reference maximum only when it is far behind
       const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
@@ -704,7 +704,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       ok = fa_mbar_wait(pv_done + (fl & 1), (fl >> 1) & 1);
       if (ok) {
         fa_fence_after();
-        const float inv = fa_inverse(l_run, m_used, sink, opts, head, tw.row0 + r, nh, r < rows, tw.b, nkv);
+        const float inv = fa_inverse(l_run, m_used, sink, opts, head, tw.row0 + r, nh, r < rows, seq_of(w), nkv);
         fa_store_row<FA_HD>(tmem_o + lane_addr, inv, out + ((int64_t)(tw.row0 + r) * nh + head) * FA_HD, r < rows);
         fa_fence_before();                                 // O is read: the next tile's first product may write it
       }
@@ -768,12 +768,16 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   const int rows = min(FA_BQ, n_new - q0);
   const int p_first = pos0 + q0, p_last = pos0 + q0 + rows - 1;
   int k_lo = (window > 0 && p_first - window + 1 > 0) ? p_first - window + 1 : 0;
-  if (chunk > 0) k_lo = max(k_lo, p_first / chunk * chunk);
+  if (!FA_F16 && chunk > 0) k_lo = max(k_lo, p_first / chunk * chunk);
   const int page_lo = k_lo / FA_BK, page_hi = p_last / FA_BK;
   const int kept = fa_kept_pages(window, opts.keep_first, page_lo);
   const int n_blocks = FA_F16 ? max(kept + page_hi - page_lo + 1, 1) : kept + page_hi - page_lo + 1;      // (as in fa_tile)
   const int* bt = block_table + (int64_t)b * bt_stride;
-  const FaRow own = fa_row(opts, b);
+  const int mask_from = FA_F16 && fa_has_holes(opts, b) ? FA_HOLES : p_first;
+  auto missing = [&](int key0) {                  // as in the kernel above
+    const int again = __ldcg(tile_seq + tile);
+    return fa_page(block_table + (int64_t)again * bt_stride, fa_row(opts, again), opts, key0 / FA_BK) < 0;
+  };
 
   if (threadIdx.x == 0) {
     fa_mbar_init(q_full, 1);
@@ -806,7 +810,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     }
     auto load_kv = [&](int j) {
       const int st = j % F4_STAGES;
-      const int pg = fa_page(bt, own, opts, j < kept ? j : page_lo + j - kept);
+      const int pg = fa_page(bt, fa_row(opts, b), opts, j < kept ? j : page_lo + j - kept);
       if (lane == 0) {
         fa_mbar_expect_tx(kv_full + st, 2 * KVB);
         fa_tma_2d(sK + st * KVB, &map_k, kv_full + st, 0, (pg * nkv + g) * FA_BK);
@@ -861,8 +865,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       fa_ld32(tmem_base + lane_addr + 32, sr[1]);
       fa_wait_ld();
       const int key0 = (j < kept ? j : page_lo + j - kept) * FA_BK;
-      fa_adjust(sr, opts, head, key0, p, p_first, p_last, p_first + warp * 32, window, chunk);
-      if (fa_missing(bt, own, opts, key0)) fa_hide(sr);
+      fa_adjust(sr, opts, head, key0, p, mask_from, p_last, p_first + warp * 32, window, chunk, [&] { return missing(key0); });
       const float mx = fa_row_max(sr) * score_mul;
       const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
@@ -884,7 +887,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       ok = fa_mbar_wait(pv_done, jl & 1);
       if (ok) {
         fa_fence_after();
-        const float inv = fa_inverse(l_run, m_used, sink, opts, head, row_start[b] + q0 + r, nh, r < rows, b, nkv);
+        const float inv = fa_inverse(l_run, m_used, sink, opts, head, row_start[b] + q0 + r, nh, r < rows, FA_F16 ? __ldcg(tile_seq + tile) : 0, nkv);
         __nv_bfloat16* dst = out + ((int64_t)(row_start[b] + q0 + r) * nh + head) * 64;
 #pragma unroll 1
         for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -973,6 +976,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   auto tile_of = [&](int item) {
     return fa_tile(item / n_pairs, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
   };
+  auto seq_of = [&](int item) { return !FA_F16 ? 0 : __ldcg(tile_seq + item / n_pairs); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) { fa_mbar_init(q_full + i, 1); fa_mbar_init(q_free + i, 1); }
@@ -1000,19 +1004,19 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     // first batch) ahead.
     int c = 0, k = 0, item = item_of(0);                    // c: pages asked for
     FaTile t = tile_of(item);
-    auto numbers = [&](const FaTile& u, int j0) {
+    auto numbers = [&](const FaTile& u, int of, int j0) {
       const int j = j0 + lane;
-      return j < u.n_pages ? fa_page(u.bt, u.own, opts, j < u.kept ? j : u.page_lo + j - u.kept) : 0;
+      return j < u.n_pages ? fa_page(u.bt, fa_row(opts, seq_of(of)), opts, j < u.kept ? j : u.page_lo + j - u.kept) : 0;
     };
-    int pgs = numbers(t, 0);
+    int pgs = numbers(t, item, 0);
     while (ok) {
       const int next = item_of(k + 1);
       const FaTile tn = next < n_items ? tile_of(next) : t;
-      const int first_next = next < n_items ? numbers(tn, 0) : 0;
+      const int first_next = next < n_items ? numbers(tn, next, 0) : 0;
       const int hp = item % n_pairs, g = 2 * hp / (nh / nkv);
-      int ahead = numbers(t, 32);
+      int ahead = numbers(t, item, 32);
       for (int j = 0; j < t.n_pages; ++j, ++c) {
-        if ((j & 31) == 0 && j > 0) { pgs = ahead; ahead = numbers(t, j + 32); }
+        if ((j & 31) == 0 && j > 0) { pgs = ahead; ahead = numbers(t, item, j + 32); }
         const int st = c % FP_STAGES, pg = __shfl_sync(0xffffffffu, pgs, j & 31);
         if (c >= FP_STAGES && !fa_mbar_wait(kv_free + st, (c / FP_STAGES - 1) & 1)) { ok = false; break; }
         if (lane == 0) {
@@ -1116,7 +1120,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const FaTile tn = next < n_items ? tile_of(next) : t;  // asked for an item ahead
       const int head = 2 * (item % n_pairs) + s;
       const int p = t.p_first + r, n_pages = t.n_pages;
-      const float score_mul = fa_score_mul(opts, scale_log2, t.row0 + r, r < t.rows, nh, head, t.b, nkv);
+      const float score_mul = fa_score_mul(opts, scale_log2, t.row0 + r, r < t.rows, nh, head, seq_of(item), nkv);
       float m_used = -INFINITY, l_run = 0.0f;
       uint32_t sr[2][32];
       auto ask_s = [&](int f, bool there) -> bool {         // there: the barrier is known to have flipped
@@ -1133,8 +1137,10 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         // looked at early: see the kernel above
         const bool s_there = j + 1 < n_pages && fa_mbar_test(s_full + 2 * s + (sb ^ 1), ((f + 1) >> 1) & 1);
         const int key0 = (j < t.kept ? j : t.page_lo + j - t.kept) * FA_BK;
-        fa_adjust(sr, opts, head, key0, p, t.p_first, t.p_last, t.p_first + q * 32, window, chunk);
-        if (fa_missing(t.bt, t.own, opts, key0)) fa_hide(sr);
+        fa_adjust(sr, opts, head, key0, p, t.mask_from, t.p_last, t.p_first + q * 32, window, chunk, [&] {
+          const int b = seq_of(item);
+          return fa_page(block_table + (int64_t)b * bt_stride, fa_row(opts, b), opts, key0 / FA_BK) < 0;
+        });
         const float mx = fa_row_max(sr) * score_mul;         // scale > 0: max and scale commute
         const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
@@ -1164,7 +1170,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         if (ok) {
           fa_fence_after();
           const bool in = r < t.rows;
-          const float inv = fa_inverse(l_run, m_used, sink, opts, head, t.row0 + r, nh, in, t.b, nkv);
+          const float inv = fa_inverse(l_run, m_used, sink, opts, head, t.row0 + r, nh, in, seq_of(item), nkv);
           fa_store_row<128>(tmem_o, inv, out + ((int64_t)(t.row0 + r) * nh + head) * 128, in);
           fa_fence_before();                                 // O is read: the next item's first product may write it
         }

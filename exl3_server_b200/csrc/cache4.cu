@@ -336,28 +336,22 @@ __device__ inline void c4_row(const C4Prompt& a, int row) {
   if (lane == 0) a.own[row] = {0, count, row * a.width, holes ? 1 : 0};
 }
 
-// The rows, their keys' and values' sizes, and the queries to fp16: a row of a head times a power of two that brings its largest value to [2^10, 2^11), whose inverse goes to
-// q_scale.  A query with a value that is not finite becomes NaN.
+// The rows, and the sizes of their keys and values.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
 kv4_prompt_rows_kernel(const C4Prompt a) {
   pdl_trigger();
   pdl_wait();
-  const int row_blocks = (a.rows + C4_THREADS / 32 - 1) / (C4_THREADS / 32);
-  if ((int)blockIdx.x < row_blocks) {
-    const int row = blockIdx.x * (C4_THREADS / 32) + (threadIdx.x >> 5);
-    if (row < a.rows) c4_row(a, row);
-    return;
-  }
-  const int64_t top_items = (int64_t)a.rows * a.nkv * a.parts;
-  const int top_blocks = (int)((top_items + C4_THREADS / 32 - 1) / (C4_THREADS / 32));
-  if ((int)blockIdx.x < row_blocks + top_blocks) {
-    const int64_t item = (int64_t)(blockIdx.x - row_blocks) * (C4_THREADS / 32) + (threadIdx.x >> 5);
-    if (item < top_items) c4_tops<HD>(a, item);
-    return;
-  }
-  constexpr int LANES = HD / 8, GROUPS = C4_THREADS / LANES;           // eight features a lane
-  const int64_t item = (int64_t)(blockIdx.x - row_blocks - top_blocks) * GROUPS + threadIdx.x / LANES;
+  constexpr int WARPS = C4_THREADS / 32;
+  const int64_t item = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (item < a.rows) c4_row(a, (int)item);
+  else if (item - a.rows < (int64_t)a.rows * a.nkv * a.parts) c4_tops<HD>(a, item - a.rows);
+}
+
+// Eight lanes (sixteen for heads of 128) have a query of a head: to fp16, times a power of two that brings its largest value to [2^10, 2^11), whose
+// inverse goes to q_scale.  A query with a value that is not finite becomes NaN.
+template <int HD> __device__ inline void c4_query(const C4Prompt& a, int64_t item) {
+  constexpr int LANES = HD / 8;
   const int j = threadIdx.x % LANES;
   const bool live = item < (int64_t)a.T * a.nh;
   const int64_t t = live ? item / a.nh : 0;
@@ -376,22 +370,27 @@ kv4_prompt_rows_kernel(const C4Prompt a) {
   for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   finite = top < __int_as_float(0x7f800000);
   const int e2 = finite && top > 0.0f ? min(max(10 + 127 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
-  const float up = __int_as_float((127 + e2) << 23), down = __int_as_float((127 - e2) << 23);
+  const float up = c4_pow2(e2);
   if (!live) return;
   __align__(16) __half h[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) h[e] = finite ? __float2half_rn(x[e] * up) : __ushort_as_half(0x7e00);
   *reinterpret_cast<uint4*>(a.q_out + (t * a.nh + head) * HD + 8 * j) = *reinterpret_cast<const uint4*>(h);
-  if (j == 0) a.q_scale[t * a.nh + head] = down;
+  if (j == 0) a.q_scale[t * a.nh + head] = c4_pow2(-e2);
 }
 
-// The pages of all rows: a block per (row, page, kv head), times the powers of two that bring the row's keys and values of that head up to fp16's
-// largest; the block of a row's first page keeps what undoes them.  No copy is written of a page that is not there.
+// The pages of all rows, a block per (row, page, kv head), times the powers of two that bring the row's keys and values of that head up to fp16's
+// largest; the block of a row's first page keeps what undoes them.  No copy is written of a page that is not there.  The blocks behind have the queries.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
 kv4_unpack16_kernel(const C4Prompt a) {
   pdl_trigger();
   pdl_wait();
+  const int page_blocks = a.rows * a.width * a.nkv;
+  if ((int)blockIdx.x >= page_blocks) {
+    c4_query<HD>(a, (int64_t)(blockIdx.x - page_blocks) * (C4_THREADS * 8 / HD) + threadIdx.x / (HD / 8));
+    return;
+  }
   const int i = (int)(blockIdx.x / a.nkv), kv = (int)(blockIdx.x % a.nkv), row = i / a.width, j = i % a.width;
   const int2 up = c4_row_up(a, (int64_t)row * a.nkv + kv);
   if (j == 0 && threadIdx.x == 0) a.undo[row * a.nkv + kv] = make_float2(c4_pow2(-up.x), c4_pow2(-up.y));
@@ -457,9 +456,9 @@ extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* b
   if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
   const int per = C4_THREADS / (hd / 8);
   const int warps = C4_THREADS / 32, parts = exl3_kv4_prompt_parts(width);
-  const int64_t blocks = (int64_t)rows * width * nkv;
-  const int64_t q_blocks = ceil_div(rows, warps) + ((int64_t)rows * nkv * parts + warps - 1) / warps + ((int64_t)T * nh + per - 1) / per;
-  if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX || q_blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
+  const int64_t row_blocks = ((int64_t)rows * (1 + (int64_t)nkv * parts) + warps - 1) / warps;
+  const int64_t blocks = (int64_t)rows * width * nkv + ((int64_t)T * nh + per - 1) / per;
+  if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX || row_blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
   C4Prompt a = {};
   a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.nkv = nkv;
   a.block_table = block_table; a.bt_stride = bt_stride; a.width = width; a.rows = rows;
@@ -469,7 +468,7 @@ extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* b
   a.own = static_cast<FaRow*>(own); a.tops = static_cast<float2*>(tops); a.undo = static_cast<float2*>(undo);
   a.window = window; a.parts = parts;
   auto go = [&](auto first, auto second) {
-    launch_pdl(first, dim3((unsigned)q_blocks), dim3(C4_THREADS), 0, stream, a);
+    launch_pdl(first, dim3((unsigned)row_blocks), dim3(C4_THREADS), 0, stream, a);
     launch_pdl(second, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, a);
   };
   if (hd == 64) go(kv4_prompt_rows_kernel<64>, kv4_unpack16_kernel<64>); else go(kv4_prompt_rows_kernel<128>, kv4_unpack16_kernel<128>);
