@@ -466,17 +466,14 @@ int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float
 // What the listed pages stand for, [n, nkv, 64, hd] bfloat16 each (zeros for a number that is no page's).
 int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, int nkv, int hd, void* k_out, void* v_out,
                   cudaStream_t stream);
-// Pages and queries in fp16 for the prompt attention and where each row's pages are (own [rows], see cache4_rows.cuh), and the attention of prompts over
-// a table [rows, width] of pages; pages that are not there, or beyond the table, are hidden.  tops: float2 [rows, nkv, exl3_kv4_prompt_parts(width)],
-// undo: float2 [rows, nkv], the factors of the products with the keys and with the values.
-int exl3_kv4_prompt_parts(int width);
-int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* block_table, int bt_stride, int rows, int width, const int* row_start,
-                      const int* row_pos0, int window, int nkv, int hd, void* k_out, void* v_out, void* own, void* tops, void* undo, const void* q, int64_t q_stride, int T, int nh,
-                      void* q_out, float* q_scale, cudaStream_t stream);
-long long exl3_kv4_prompt_scratch(int T, int rows, int width, int nh, int nkv, int hd);
+// Attention of prompts over the 4-bit cache, by fp16 copies of the rows' pages in `slots` places of scratch memory.  row_pages, total: the most pages
+// of a row and of all rows that their queries see (what is beyond is hidden, as are pages that are not there, or beyond the table's width).  A
+// row's pages are copied in the pass (pages of the rows before it) / stride, so slots = total for one pass, else at least stride - 1 + row_pages.
+long long exl3_kv4_prompt_scratch(int T, int rows, int row_pages, int total, int slots, int passes, int n_tiles, int nh, int nkv, int hd);
 int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
                     int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0, int n_tiles, int nh,
-                    int nkv, int hd, int window, float scale, void* scratch, long long scratch_bytes, cudaStream_t stream);
+                    int nkv, int hd, int window, float scale, int row_pages, int total, int slots, int stride, int passes, void* scratch,
+                    long long scratch_bytes, cudaStream_t stream);
 int exl3_kv4_prompt_status();
 // Attention of one token or a few per row over the 4-bit cache.  Row r has tokens row_start[r] .. row_start[r + 1] - 1 (null: token r) at positions
 // row_pos0[r] ...; chunk: tiles of 4096 / hd keys that a block walks, max_chunks: chunks of the longest row (window's reach).

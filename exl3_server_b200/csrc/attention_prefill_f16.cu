@@ -17,38 +17,61 @@ extern "C" int exl3_kv4_prompt_status() { return fa_status(); }
 
 static long long kv4_up16(long long n) { return (n + 15) / 16 * 16; }
 
-// Bytes of scratch: the pages' keys and values, the queries, their factors, where each row's pages are, the
-// sizes of its keys and values by parts, and what undoes their factors.
-extern "C" long long exl3_kv4_prompt_scratch(int T, int rows, int width, int nh, int nkv, int hd) {
-  return 2 * (long long)rows * width * nkv * 64 * hd * 2 + kv4_up16((long long)T * nh * hd * 2) + kv4_up16((long long)T * nh * 4) + 16ll * rows +
-         8ll * rows * nkv * (exl3_kv4_prompt_parts(width) + 1);
+// Bytes of scratch: copies of `slots` pages, the queries, their factors, the plan (rows, passes, slots of all passes, tiles), the sizes of the rows' keys
+// and values by parts, and what undoes their factors.
+extern "C" long long exl3_kv4_prompt_scratch(int T, int rows, int row_pages, int total, int slots, int passes, int n_tiles, int nh, int nkv, int hd) {
+  return 2 * (long long)slots * nkv * 64 * hd * 2 + kv4_up16((long long)T * nh * hd * 2) + kv4_up16((long long)T * nh * 4) + 16ll * rows +
+         16ll * passes + 16ll * total + kv4_up16(4ll * rows) + 2 * kv4_up16(4ll * n_tiles) + kv4_up16(8ll * rows * nkv) +
+         8ll * rows * nkv * c4_prompt_parts(row_pages);
 }
 
 extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table,
                                int bt_stride, int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0,
-                               int n_tiles, int nh, int nkv, int hd, int window, float scale, void* scratch, long long scratch_bytes,
-                               cudaStream_t stream) {
+                               int n_tiles, int nh, int nkv, int hd, int window, float scale, int row_pages, int total, int slots, int stride,
+                               int passes, void* scratch, long long scratch_bytes, cudaStream_t stream) {
   if (T == 0 || n_tiles == 0) return 0;
-  if (T < 0 || rows < 1 || width < 1 || nkv < 1 || nh < 1 || nh % nkv || !fa_supported(hd, 64) || (int64_t)rows * width > INT32_MAX || !q || !out ||
-      !pool || !block_table || !row_start || !row_pos0 || !tile_seq || !tile_q0 || !scratch) {
-    set_error("kv4_prompt: needs heads of 64 or 128 and all of its arrays, got T=%d rows=%d heads=%d kv_heads=%d head_dim=%d", T, rows, nh, nkv, hd);
+  if (T < 0 || rows < 1 || width < 1 || nkv < 1 || nh < 1 || nh % nkv || !fa_supported(hd, 64) || n_tiles < 0 || window < 0 || n_pages < 1 ||
+      n_pages > INT32_MAX || row_pages < 1 || total < 1 || stride < 1 || passes < 1 || (total - 1) / stride >= passes ||
+      slots < (passes == 1 ? total : stride - 1 + row_pages) || !q || !out || !pool || !block_table || !row_start || !row_pos0 || !tile_seq || !tile_q0 ||
+      !scratch) {
+    set_error("kv4_prompt: needs heads of 64 or 128, passes that hold their rows' pages and all of its arrays, got T=%d rows=%d heads=%d kv_heads=%d "
+              "head_dim=%d pages=%d of %d slots=%d stride=%d passes=%d", T, rows, nh, nkv, hd, row_pages, total, slots, stride, passes);
     return ERR_BAD_ARGUMENT;
   }
-  const int pages = rows * width;
-  if (!aligned16(scratch) || scratch_bytes < exl3_kv4_prompt_scratch(T, rows, width, nh, nkv, hd)) {
-    set_error("kv4_prompt: %lld bytes of scratch wanted, 16-byte aligned", exl3_kv4_prompt_scratch(T, rows, width, nh, nkv, hd));
+  if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
+  const long long need = exl3_kv4_prompt_scratch(T, rows, row_pages, total, slots, passes, n_tiles, nh, nkv, hd);
+  if (!aligned16(scratch) || scratch_bytes < need) {
+    set_error("kv4_prompt: %lld bytes of scratch wanted, 16-byte aligned", need);
     return ERR_SCRATCH;
   }
-  unsigned char* k = static_cast<unsigned char*>(scratch);
-  unsigned char* v = k + (long long)pages * nkv * 64 * hd * 2;
-  unsigned char* q16 = v + (long long)pages * nkv * 64 * hd * 2;
-  float* q_scale = reinterpret_cast<float*>(q16 + kv4_up16((long long)T * nh * hd * 2));
-  FaRow* own = reinterpret_cast<FaRow*>(reinterpret_cast<unsigned char*>(q_scale) + kv4_up16((long long)T * nh * 4));
-  float2* undo = reinterpret_cast<float2*>(own + rows);
-  float2* tops = undo + (int64_t)rows * nkv;
-  const int rc = exl3_kv4_unpack16(pool, n_pages, block_table, bt_stride, rows, width, row_start, row_pos0, window, nkv, hd, k, v, own, tops, undo, q, q_stride,
-                                   T, nh, q16, q_scale, stream);
-  if (rc) return rc;
-  return fa_run(q16, (int64_t)nh * hd, T, out, k, v, (int64_t)pages * nkv * 64, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, n_tiles,
-                nh, nkv, hd, 64, window, 0, 0, scale, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr, q_scale, undo, own, (int)n_pages, stream);
+  unsigned char* at = static_cast<unsigned char*>(scratch);
+  auto take = [&](long long bytes) { unsigned char* p = at; at += kv4_up16(bytes); return p; };
+  C4Prompt a = {};
+  a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.nkv = nkv;
+  a.block_table = block_table; a.bt_stride = bt_stride; a.width = width; a.rows = rows;
+  a.row_start = row_start; a.row_pos0 = row_pos0; a.window = window; a.parts = c4_prompt_parts(row_pages);
+  a.tile_seq = tile_seq; a.tile_q0 = tile_q0; a.n_tiles = n_tiles;
+  a.row_pages = row_pages; a.total = total; a.stride = stride; a.passes = passes;
+  a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.T = T; a.nh = nh;
+  a.k_out = reinterpret_cast<__half*>(take((long long)slots * nkv * 64 * hd * 2));
+  a.v_out = reinterpret_cast<__half*>(take((long long)slots * nkv * 64 * hd * 2));
+  a.q_out = reinterpret_cast<__half*>(take((long long)T * nh * hd * 2));
+  a.q_scale = reinterpret_cast<float*>(take((long long)T * nh * 4));
+  a.own = reinterpret_cast<FaRow*>(take(16ll * rows));
+  a.pass = reinterpret_cast<PromptPass*>(take(16ll * passes));
+  a.slot = reinterpret_cast<int4*>(take(16ll * total));
+  a.pass_of = reinterpret_cast<int*>(take(4ll * rows));
+  a.seq_out = reinterpret_cast<int*>(take(4ll * n_tiles));
+  a.q0_out = reinterpret_cast<int*>(take(4ll * n_tiles));
+  a.undo = reinterpret_cast<float2*>(take(8ll * rows * nkv));
+  a.tops = reinterpret_cast<float2*>(at);
+  int rc = c4_prompt_plan(a, hd, stream);
+  for (int p = 0; p < passes && !rc; ++p) {
+    rc = c4_prompt_copies(a, hd, p, slots, stream);
+    if (!rc)
+      rc = fa_run(a.q_out, (int64_t)nh * hd, T, out, a.k_out, a.v_out, (int64_t)slots * nkv * 64, block_table, bt_stride, row_start, row_pos0, a.seq_out,
+                  a.q0_out, n_tiles, nh, nkv, hd, 64, window, 0, 0, scale, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr,
+                  FaCopies{a.q_scale, a.undo, a.own, a.pass + p, passes == 1, (int)n_pages}, stream);
+  }
+  return rc;
 }

@@ -13,7 +13,7 @@ extern "C" int exl3_attn_prefill_tc_opt(const void* q, int64_t q_row_stride, int
                                         cudaStream_t stream) {
   return fa_run(q, q_row_stride, T, out, k_pool, v_pool, n_pool_rows, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0,
                 n_tiles, nh, nkv, hd, page, window, chunk, sink, scale, variant, keep_first, softcap, sink_vals, dist, dist_len, gate,
-                nullptr, nullptr, nullptr, 0, stream);
+                FaCopies{}, stream);
 }
 
 extern "C" int exl3_attn_prefill_tc(const void* q, int64_t q_row_stride, int T, void* out, const void* k_pool,

@@ -52,13 +52,15 @@
 #ifdef EXL3_PREFILL_F16
 #include "cache4_rows.cuh"
 #else
-namespace exl3 { struct FaRow {}; }
+namespace exl3 { struct FaRow {}; struct PromptPass {}; }
 #endif
 
 #ifdef EXL3_PREFILL_F16
 #define EXL3_FA_NS prefill_f16
+#define EXL3_FA_LIST const int*                   // lists of tiles: a kernel's work here,
 #else
 #define EXL3_FA_NS prefill_bf16
+#define EXL3_FA_LIST const int* __restrict__      // the host's there
 #endif
 
 namespace exl3 {
@@ -207,6 +209,15 @@ __device__ inline uint32_t fa_pack(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// fp16: the copies that stand in for the cache.
+struct FaCopies {
+  const float* q_scale;        // what the scores of a (token, query head) are multiplied by beside the scale
+  const float2* undo;          // per (row, kv head): what its products with keys (scores) and with values are multiplied by
+  const FaRow* own;            // where the copies of the rows' pages are
+  const PromptPass* pass;      // the tiles of this launch, which
+  bool first;                  // begin the lists (known ahead of the pass where there is but one)
+  int table_pages;             // pages of the pool that the block table speaks of
+};
 // What a block needs to know of a tile of 128 queries.
 // Options beyond the plain causal softmax.  keep_first: with a window, the keys at positions below it stay visible.
 // cap_in > 0: a raw score s becomes tanh(s * cap_in) and is multiplied by cap_log2 (= cap * log2 e) instead of the
@@ -221,16 +232,13 @@ struct FaOpts {
   int dist_len;
   float dist_mul;
   const float* gate;           // a factor per (token, query head) on the output; null: none
-  const float* q_scale;        // fp16: what the scores of a (token, query head) are multiplied by beside the scale
-  const float2* undo;          // fp16: per (row, kv head), what its products with keys (scores) and with values are multiplied by
-  const FaRow* own;            // fp16: where the copies of the rows' pages are
-  int table_pages;             // fp16: pages of the pool that the block table speaks of
+  FaCopies copies;
 };
 // What the scores of row `row` of q, of the sequence b, are multiplied by (base-2 units); a positive number, so that a hidden score stays -inf.
 __device__ inline float fa_score_mul(const FaOpts& opts, float scale_log2, int64_t row, bool there, int nh, int head, int b, int nkv) {
   const float mul = opts.cap_in > 0.0f ? opts.cap_log2 : scale_log2;
   if (!FA_F16) return mul;
-  const float f = there ? __ldcg(opts.q_scale + row * nh + head) * __ldcg(opts.undo + (int64_t)b * nkv + head / (nh / nkv)).x : 1.0f;
+  const float f = there ? __ldcg(opts.copies.q_scale + row * nh + head) * __ldcg(opts.copies.undo + (int64_t)b * nkv + head / (nh / nkv)).x : 1.0f;
   return fminf(fmaxf(mul * f, 1.1754944e-38f), 3.4028235e38f);
 }
 // Whether a page of keys from key0 on holds a key with a bias for one of a warp's 32 queries from position p0 on.
@@ -262,15 +270,28 @@ struct FaTile {
 constexpr int FA_HOLES = INT32_MIN;
 __device__ inline FaRow fa_row(const FaOpts& opts, int b) {
 #ifdef EXL3_PREFILL_F16
-  const int4 w = __ldcg(reinterpret_cast<const int4*>(opts.own + b));
+  const int4 w = __ldcg(reinterpret_cast<const int4*>(opts.copies.own + b));
   return {w.x, w.y, w.z, w.w};
 #else
   return {};
 #endif
 }
+// fp16: the tiles of this launch, of which the host knows an upper bound only: moves the lists to their place and returns how many there are.
+template <typename List> __device__ inline int fa_tiles(const FaOpts& opts, int n_tiles, List& tile_seq, List& tile_q0) {
+#ifdef EXL3_PREFILL_F16
+  const int2 w = __ldcg(reinterpret_cast<const int2*>(&opts.copies.pass->tile0));
+  if (!opts.copies.first) {
+    tile_seq += w.x;
+    tile_q0 += w.x;
+  }
+  return w.y;
+#else
+  return n_tiles;
+#endif
+}
 __device__ inline bool fa_has_holes(const FaOpts& opts, int b) {
 #ifdef EXL3_PREFILL_F16
-  return __ldcg(&opts.own[b].holes) != 0;
+  return __ldcg(&opts.copies.own[b].holes) != 0;
 #else
   return false;
 #endif
@@ -278,7 +299,7 @@ __device__ inline bool fa_has_holes(const FaOpts& opts, int b) {
 // Page j of the sequence in the pools of keys and values (a copy of a page that is not there would be at -1: zeros, to be hidden).
 __device__ inline int fa_page(const int* bt, const FaRow& own, const FaOpts& opts, int j) {
 #ifdef EXL3_PREFILL_F16
-  return row_copy(own, bt, opts.table_pages, j);
+  return row_copy(own, bt, opts.copies.table_pages, j);
 #else
   return bt[j];
 #endif
@@ -426,7 +447,7 @@ __device__ inline void fa_rescale_slowly(uint32_t taddr, float corr) {
 // What a row of O is multiplied by at the end.  A sink is a key of score 0 without a value: one more term in the sum, in
 // the units of the reference maximum.
 __device__ inline float fa_inverse(float l_run, float m_used, int sink, const FaOpts& opts, int head, int row, int nh, bool in, int b, int nkv) {
-  if (FA_F16) return l_run == 0.0f ? 0.0f : __ldcg(opts.undo + (int64_t)b * nkv + head / (nh / nkv)).y / l_run;      // (0: a query that sees nothing)
+  if (FA_F16) return l_run == 0.0f ? 0.0f : __ldcg(opts.copies.undo + (int64_t)b * nkv + head / (nh / nkv)).y / l_run;      // (0: a query that sees nothing)
   float inv = 1.0f / (sink ? l_run + fa_exp2((opts.sink_vals ? __ldg(opts.sink_vals + head) * 1.4426950408889634f : 0.0f) - m_used) : l_run);
   if (opts.gate && in) inv *= __ldcg(opts.gate + (int64_t)row * nh + head);
   return inv;
@@ -463,8 +484,8 @@ __global__ void __launch_bounds__(FA_THREADS_MAIN, FA_HD == 64 ? 2 : 1)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out,
                        const int* __restrict__ block_table, int bt_stride, const int* __restrict__ row_start,
-                       const int* __restrict__ row_pos0, const int* __restrict__ tile_seq,
-                       const int* __restrict__ tile_q0, int n_tiles, int fold, int nh, int nkv, int window,
+                       const int* __restrict__ row_pos0, EXL3_FA_LIST tile_seq,
+                       EXL3_FA_LIST tile_q0, int n_tiles, int fold, int nh, int nkv, int window,
                        int chunk, int sink, float scale_log2, FaOpts opts) {
   extern __shared__ unsigned char fa_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fa_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -488,8 +509,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   // the caller lists the tiles with the most keys to visit first
   const int head = blockIdx.x;                      // blocks start in this order: all heads of y = 0, then y = 1, ...
   const int g = head / (nh / nkv);
-  const int other = n_tiles - 1 - (int)blockIdx.y;
-  const int n_own = (fold && other > (int)blockIdx.y) ? 2 : 1;
+  int other = n_tiles - 1 - (int)blockIdx.y;
+  int n_own = (fold && other > (int)blockIdx.y) ? 2 : 1;
   auto tile_of = [&](int w) {                       // the block's first (w = 0) or second tile
     return fa_tile(w ? other : (int)blockIdx.y, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
   };
@@ -525,12 +546,18 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   // so far nothing was touched that another kernel writes; the next kernel in the stream may be set up meanwhile
   pdl_trigger();
   pdl_wait();
+  if (FA_F16) {
+    other = fa_tiles(opts, n_tiles, tile_seq, tile_q0) - 1 - (int)blockIdx.y;
+    n_own = fold ? (other > (int)blockIdx.y ? 2 : other == (int)blockIdx.y ? 1 : 0) : other >= 0 ? 1 : 0;
+  }
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t tmem_o = tmem_base + 128;                  // columns: S0 0..63, S1 64..127, O from 128
   const uint32_t tmem_p = tmem_base + 128 + FA_HD;          // P0, then P1: 32 columns each (two bfloat16 per column)
   bool ok = true;
 
-  if (warp == 4) {
+  if (FA_F16 && n_own == 0) {
+    // no tile is left for this block
+  } else if (warp == 4) {
     // ---- copies and the second product ---------------------------------------------------
     // The Q tiles and the first pages' K and V at once; then O += P_f V_f as soon as the softmax threads hand P_f
     // over, and, once that product is done with its stage of the ring, the copy of the page that comes into the
@@ -740,8 +767,8 @@ __global__ void __launch_bounds__(FA_THREADS, 4)
 attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out,
                         const int* __restrict__ block_table, int bt_stride, const int* __restrict__ row_start,
-                        const int* __restrict__ row_pos0, const int* __restrict__ tile_seq,
-                        const int* __restrict__ tile_q0, int nh, int nkv, int window, int chunk, int sink,
+                        const int* __restrict__ row_pos0, EXL3_FA_LIST tile_seq,
+                        EXL3_FA_LIST tile_q0, int nh, int nkv, int window, int chunk, int sink,
                         float scale_log2, FaOpts opts) {
   extern __shared__ unsigned char fa_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fa_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -760,7 +787,10 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x, tile = blockIdx.y;
-  if (FA_F16) pdl_wait();                         // where the copies are is the work of the kernel ahead
+  if (FA_F16) {
+    pdl_wait();                                   // the list of tiles is the work of a kernel ahead
+    if (tile >= fa_tiles(opts, 0, tile_seq, tile_q0)) return;
+  }
   const int b = tile_seq[tile], q0 = tile_q0[tile];
   const int n_new = row_start[b + 1] - row_start[b];
   const int pos0 = row_pos0[b];
@@ -949,8 +979,8 @@ __global__ void __launch_bounds__(FP_THREADS, 1)
 attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                             const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out,
                             const int* __restrict__ block_table, int bt_stride, const int* __restrict__ row_start,
-                            const int* __restrict__ row_pos0, const int* __restrict__ tile_seq,
-                            const int* __restrict__ tile_q0, int n_tiles, int nh, int nkv, int window, int chunk, int sink,
+                            const int* __restrict__ row_pos0, EXL3_FA_LIST tile_seq,
+                            EXL3_FA_LIST tile_q0, int n_tiles, int nh, int nkv, int window, int chunk, int sink,
                             float scale_log2, FaOpts opts) {
   extern __shared__ unsigned char fa_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fa_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -969,7 +999,8 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_pairs = nh >> 1, n_items = n_tiles * n_pairs;
+  const int n_pairs = nh >> 1;
+  int n_items = n_tiles * n_pairs;
   auto item_of = [&](int k) {                               // the block's k-th item; n_items or more: none
     return k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
   };
@@ -995,10 +1026,13 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   // so far nothing was touched that another kernel writes; the next kernel in the stream may be set up meanwhile
   pdl_trigger();
   pdl_wait();
+  if (FA_F16) n_items = fa_tiles(opts, n_tiles, tile_seq, tile_q0) * n_pairs;
   const uint32_t tmem_base = *tmem_slot;                    // columns: S of head s at 128 s, O at 256 + 128 s
   bool ok = true;
 
-  if (warp == 10) {
+  if (FA_F16 && (int)blockIdx.x >= n_items) {
+    // no item is left for this block
+  } else if (warp == 10) {
     // ---- copies -------------------------------------------------------------------------------------------
     // Page numbers come 32 at a time, lane i holding that of page j0 + i of the item, a batch (or the next item's
     // first batch) ahead.
@@ -1248,7 +1282,7 @@ static int fa_run(const void* q, int64_t q_row_stride, int T, void* out, const v
                   const int* tile_q0, int n_tiles, int nh, int nkv, int hd, int page, int window,
                   int chunk, int sink, float scale, int variant, int keep_first, float softcap,
                   const float* sink_vals, const float* dist, int dist_len, const float* gate,
-                  const float* q_scale, const float2* undo, const FaRow* own, int table_pages, cudaStream_t stream) {
+                  const FaCopies& copies, cudaStream_t stream) {
   if (n_tiles == 0) return 0;
   if (dist_len < 0 || (dist_len > 0 && dist == nullptr)) {
     set_error("attn_prefill_tc: a table of %d distance biases is missing", dist_len);
@@ -1267,10 +1301,7 @@ static int fa_run(const void* q, int64_t q_row_stride, int T, void* out, const v
   opts.dist = dist;
   opts.dist_len = dist_len;
   opts.gate = gate;
-  opts.q_scale = q_scale;
-  opts.undo = undo;
-  opts.own = own;
-  opts.table_pages = table_pages;
+  opts.copies = copies;
   opts.dist_mul = softcap > 0.0f ? 1.0f / softcap : 1.0f / scale;
   if (!fa_supported(hd, page)) {
     set_error("attn_prefill_tc: needs bfloat16, head_dim 64 or 128 and pages of 64, got head_dim %d page %d", hd, page);

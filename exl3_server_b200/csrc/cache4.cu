@@ -14,8 +14,6 @@
 #include "cache4.cuh"
 #include "cache4_rows.cuh"
 
-#include <cuda_fp16.h>
-
 namespace exl3 {
 
 using namespace kv4;
@@ -248,24 +246,6 @@ kv4_load_kernel(const unsigned char* __restrict__ pool, const int* __restrict__ 
 
 // ---- prompts: fp16 copies of the rows' pages and of the queries, for the prompt attention ------------------------------------------
 
-struct C4Prompt {
-  const unsigned char* pool;
-  int n_pages, nkv;
-  const int* block_table;
-  int bt_stride, width, rows;
-  const int *row_start, *row_pos0;
-  int window, parts;
-  const __nv_bfloat16* q;
-  int64_t q_stride;
-  int T, nh;
-  __half *k_out, *v_out, *q_out;
-  float* q_scale;
-  FaRow* own;
-  float2* tops;          // [rows][nkv][parts]: the largest |key| and |value| of a part of a row's pages
-  float2* undo;          // [rows][nkv]: what the products of the copied keys and of the copied values are multiplied by
-};
-constexpr int C4_MAX_PARTS = 32;                                       // one a lane
-
 // The exponent of the power of two that brings numbers up to `top` below 2^15.  Down to 2^-110 that leaves all of fp16's bits to what is within 2^28
 // of the top.
 __device__ inline int c4_up(float top) { return top > 0.0f ? min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -113), 96) : 0; }
@@ -278,7 +258,7 @@ template <int HD> __device__ inline void c4_tops(const C4Prompt& a, int64_t item
   const int lane = threadIdx.x & 31, part = (int)(item % a.parts), kv = (int)(item / a.parts % a.nkv), row = (int)(item / a.parts / a.nkv);
   const int pos0 = __ldcg(a.row_pos0 + row), end = pos0 + __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row);
   const int first = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;    // places first .. end - 1 are seen
-  const int pages = end > 0 ? min((end - 1) / PAGE + 1, a.width) : 0;
+  const int pages = end > 0 ? min(min((end - 1) / PAGE + 1, a.width), first / PAGE + a.row_pages) : 0;
   float top[2] = {0.0f, 0.0f};
   for (int j0 = first / PAGE + part * AHEAD; j0 < pages; j0 += a.parts * AHEAD) {
     uint4 w[AHEAD][SPP][2];
@@ -336,16 +316,142 @@ __device__ inline void c4_row(const C4Prompt& a, int row) {
   if (lane == 0) a.own[row] = {0, count, row * a.width, holes ? 1 : 0};
 }
 
-// The rows, and the sizes of their keys and values.
+// Sum over the block's threads below this one, and (total) over all of them; warp_sums has room for 32 and one more.
+__device__ inline int c4_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();                                                     // (the sums of the call before have been read)
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < C4_THREADS / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  return before + x - v;
+}
+
+// One block: the pages that some query of a row sees, one row behind the other, and the passes they fall into.  What the sizes do not allow for (a row of
+// more pages than was said) is not copied, so nobody sees it.
+__device__ inline void c4_plan_rows(const C4Prompt& a) {
+  constexpr int N = C4_THREADS, WARPS = N / 32;
+  __shared__ int warp_sums[32], s_pass[N], s_holes[N], s_end[N];
+  __shared__ FaRow s_row[N];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int p = tid; p < a.passes; p += N) a.pass[p].slot0 = a.pass[p].slots = 0;
+  int base = 0, open = -1, open_slot0 = 0;                             // the pass of the last row so far, and its first slot
+  for (int r0 = 0; r0 < a.rows; r0 += N) {
+    const int row = r0 + tid, here = min(N, a.rows - r0);
+    int lo = 0, pages = 0, count = 0, end = 0;
+    if (row < a.rows) {
+      const int n_new = __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row), pos0 = __ldcg(a.row_pos0 + row);
+      end = pos0 + n_new;
+      if (n_new > 0 && end > 0) {
+        lo = a.window > 0 ? max(0, pos0 - a.window + 1) / PAGE : 0;
+        pages = (end - 1) / PAGE + 1 - lo;
+        count = max(0, min(min(pages, a.width - lo), a.row_pages));
+      }
+    }
+    int all;
+    const int at = min(base + c4_scan(count, warp_sums, all), a.total);
+    base += all;
+    count = min(count, a.total - at);
+    s_row[tid] = {lo, count, at, 0};
+    s_holes[tid] = pages > count;
+    s_end[tid] = end;
+    s_pass[tid] = min(at / a.stride, a.passes - 1);
+    __syncthreads();
+    const int per = here < WARPS ? WARPS / here : 1;                   // warps of a row
+    for (int r = warp / per; r < here && warp < WARPS / per * per; r += WARPS / per) {
+      const FaRow w = s_row[r];
+      bool holes = false;
+#pragma unroll 4
+      for (int k = warp % per * 32 + lane; k < w.count; k += 32 * per) {
+        const int page = __ldcg(a.block_table + (int64_t)(r0 + r) * a.bt_stride + w.lo + k);
+        const bool there = page >= 0 && page < a.n_pages;
+        holes = holes || !there;
+        a.slot[w.base + k] = make_int4(r0 + r, there ? page : -1, s_end[r] - (w.lo + k) * PAGE, k == 0);
+      }
+      if (holes) s_holes[r] = 1;
+    }
+    __syncthreads();
+    int slot0 = open_slot0, mine = s_pass[tid];
+    if (mine != open) {                                                // the first row of the pass is one of these
+      int x = 0, y = tid;
+      while (x < y) {
+        const int mid = (x + y) / 2;
+        if (s_pass[mid] < mine) x = mid + 1; else y = mid;
+      }
+      slot0 = s_row[x].base;
+    }
+    if (row < a.rows) {
+      a.own[row] = {lo, count, at - slot0, s_holes[tid]};
+      a.pass_of[row] = mine;
+      if (tid + 1 == here || s_pass[tid + 1] != mine) {                // the pass's last row so far
+        a.pass[mine].slot0 = slot0;
+        a.pass[mine].slots = at + count - slot0;
+      }
+    }
+    const int last = s_pass[here - 1];
+    if (last != open) {
+      int x = 0, y = here - 1;
+      while (x < y) {
+        const int mid = (x + y) / 2;
+        if (s_pass[mid] < last) x = mid + 1; else y = mid;
+      }
+      open = last;
+      open_slot0 = s_row[x].base;
+    }
+    __syncthreads();                                                   // (shared memory is the next rows')
+  }
+}
+
+// One block: the tiles of queries by passes, within one in the given order.
+__device__ inline void c4_plan_tiles(const C4Prompt& a) {
+  __shared__ int warp_sums[32];
+  int out = 0;
+  for (int p = 0; p < a.passes; ++p) {
+    const int first = out;
+    for (int t0 = 0; t0 < a.n_tiles; t0 += C4_THREADS) {
+      const int t = t0 + threadIdx.x, row = t < a.n_tiles ? __ldcg(a.tile_seq + t) : -1, q0 = t < a.n_tiles ? __ldcg(a.tile_q0 + t) : 0;
+      const bool mine = row >= 0 && row < a.rows && (a.passes == 1 || __ldcg(a.pass_of + row) == p);
+      int all;
+      const int at = out + c4_scan(mine ? 1 : 0, warp_sums, all);
+      if (mine) {
+        a.seq_out[at] = row;
+        a.q0_out[at] = q0;
+      }
+      out += all;
+    }
+    if (threadIdx.x == 0) { a.pass[p].tile0 = first; a.pass[p].tiles = out - first; }
+  }
+}
+
+// The plan, and the sizes of the rows' keys and values.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
-kv4_prompt_rows_kernel(const C4Prompt a) {
+kv4_prompt_plan_kernel(const C4Prompt a) {
   pdl_trigger();
   pdl_wait();
-  constexpr int WARPS = C4_THREADS / 32;
-  const int64_t item = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (item < a.rows) c4_row(a, (int)item);
-  else if (item - a.rows < (int64_t)a.rows * a.nkv * a.parts) c4_tops<HD>(a, item - a.rows);
+  if (blockIdx.x == 0) {
+    c4_plan_rows(a);
+    __syncthreads();
+    if (a.passes > 1) c4_plan_tiles(a);                                // (by the rows' passes)
+    return;
+  }
+  if (blockIdx.x == 1) {
+    if (a.passes == 1) c4_plan_tiles(a);
+    return;
+  }
+  const int64_t item = (int64_t)(blockIdx.x - 2) * (C4_THREADS / 32) + (threadIdx.x >> 5);
+  if (item < (int64_t)a.rows * a.nkv * a.parts) c4_tops<HD>(a, item);
 }
 
 // Eight lanes (sixteen for heads of 128) have a query of a head: to fp16, times a power of two that brings its largest value to [2^10, 2^11), whose
@@ -379,26 +485,45 @@ template <int HD> __device__ inline void c4_query(const C4Prompt& a, int64_t ite
   if (j == 0) a.q_scale[t * a.nh + head] = c4_pow2(-e2);
 }
 
-// The pages of all rows, a block per (row, page, kv head), times the powers of two that bring the row's keys and values of that head up to fp16's
+// A pass's pages, a block per (slot, kv head), times the powers of two that bring the row's keys and values of that head up to fp16's
 // largest; the block of a row's first page keeps what undoes them.  No copy is written of a page that is not there.  The blocks behind have the queries.
 template <int HD>
 __global__ void __launch_bounds__(C4_THREADS)
-kv4_unpack16_kernel(const C4Prompt a) {
+kv4_unpack16_kernel(const C4Prompt a, int pass, int page_blocks) {
   pdl_trigger();
   pdl_wait();
-  const int page_blocks = a.rows * a.width * a.nkv;
   if ((int)blockIdx.x >= page_blocks) {
     c4_query<HD>(a, (int64_t)(blockIdx.x - page_blocks) * (C4_THREADS * 8 / HD) + threadIdx.x / (HD / 8));
     return;
   }
-  const int i = (int)(blockIdx.x / a.nkv), kv = (int)(blockIdx.x % a.nkv), row = i / a.width, j = i % a.width;
+  const int i = (int)(blockIdx.x / a.nkv), kv = (int)(blockIdx.x % a.nkv);
+  const int2 of = __ldcg(reinterpret_cast<const int2*>(a.pass + pass));               // slot0, slots
+  const int4 slot = __ldcg(a.slot + (a.passes == 1 ? i : of.y > i ? of.x + i : 0));   // (beside the pass where there is but one)
+  if (i >= of.y) return;
+  const int row = slot.x, page = slot.y, held = slot.z;
   const int2 up = c4_row_up(a, (int64_t)row * a.nkv + kv);
-  if (j == 0 && threadIdx.x == 0) a.undo[row * a.nkv + kv] = make_float2(c4_pow2(-up.x), c4_pow2(-up.y));
-  const int page = __ldcg(a.block_table + (int64_t)row * a.bt_stride + j);
-  if (page < 0 || page >= a.n_pages) return;
-  const int held = __ldcg(a.row_pos0 + row) + __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row) - j * PAGE;
+  if (slot.w && threadIdx.x == 0) a.undo[row * a.nkv + kv] = make_float2(c4_pow2(-up.x), c4_pow2(-up.y));
+  if (page < 0) return;
   const int64_t at = ((int64_t)i * a.nkv + kv) * PAGE * HD;
   c4_unpack<HD, true>(a.pool + ((int64_t)page * a.nkv + kv) * page_bytes(HD), true, held, c4_pow2(up.x), c4_pow2(up.y), a.k_out + at, a.v_out + at);
+}
+
+int c4_prompt_plan(const C4Prompt& a, int hd, cudaStream_t stream) {
+  const int warps = C4_THREADS / 32;
+  const int64_t blocks = 2 + ((int64_t)a.rows * a.nkv * a.parts + warps - 1) / warps;
+  if (blocks > INT32_MAX) { set_error("kv4_prompt: too many rows"); return ERR_UNSUPPORTED; }
+  auto go = [&](auto kernel) { launch_pdl(kernel, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, a); };
+  if (hd == 64) go(kv4_prompt_plan_kernel<64>); else go(kv4_prompt_plan_kernel<128>);
+  return launch_status("kv4_prompt_plan");
+}
+
+int c4_prompt_copies(const C4Prompt& a, int hd, int pass, int slots, cudaStream_t stream) {
+  const int per = C4_THREADS / (hd / 8);
+  const int64_t page_blocks = (int64_t)slots * a.nkv, blocks = page_blocks + (pass == 0 ? ((int64_t)a.T * a.nh + per - 1) / per : 0);
+  if (blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
+  auto go = [&](auto kernel) { launch_pdl(kernel, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, a, pass, (int)page_blocks); };
+  if (hd == 64) go(kv4_unpack16_kernel<64>); else go(kv4_unpack16_kernel<128>);
+  return launch_status("kv4_unpack16");
 }
 
 }  // namespace exl3
@@ -445,32 +570,4 @@ extern "C" int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages
   };
   if (hd == 64) go(kv4_load_kernel<64>); else go(kv4_load_kernel<128>);
   return launch_status("kv4_load");
-}
-
-// Parts of a row's pages for the search of its largest values: a warp takes four pages at a time.
-extern "C" int exl3_kv4_prompt_parts(int width) { return width < 4 * C4_MAX_PARTS ? ceil_div(width, 4) : C4_MAX_PARTS; }
-
-extern "C" int exl3_kv4_unpack16(const void* pool, int64_t n_pages, const int* block_table, int bt_stride, int rows, int width, const int* row_start,
-                                 const int* row_pos0, int window, int nkv, int hd, void* k_out, void* v_out, void* own, void* tops, void* undo, const void* q, int64_t q_stride, int T, int nh,
-                                 void* q_out, float* q_scale, cudaStream_t stream) {
-  if (!aligned16(pool) || !aligned16(q) || q_stride % 8) { set_error("kv4_prompt: q, its rows and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }
-  const int per = C4_THREADS / (hd / 8);
-  const int warps = C4_THREADS / 32, parts = exl3_kv4_prompt_parts(width);
-  const int64_t row_blocks = ((int64_t)rows * (1 + (int64_t)nkv * parts) + warps - 1) / warps;
-  const int64_t blocks = (int64_t)rows * width * nkv + ((int64_t)T * nh + per - 1) / per;
-  if (n_pages < 1 || n_pages > INT32_MAX || blocks > INT32_MAX || row_blocks > INT32_MAX) { set_error("kv4_prompt: too many pages or tokens"); return ERR_UNSUPPORTED; }
-  C4Prompt a = {};
-  a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.nkv = nkv;
-  a.block_table = block_table; a.bt_stride = bt_stride; a.width = width; a.rows = rows;
-  a.row_start = row_start; a.row_pos0 = row_pos0;
-  a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.T = T; a.nh = nh;
-  a.k_out = static_cast<__half*>(k_out); a.v_out = static_cast<__half*>(v_out); a.q_out = static_cast<__half*>(q_out); a.q_scale = q_scale;
-  a.own = static_cast<FaRow*>(own); a.tops = static_cast<float2*>(tops); a.undo = static_cast<float2*>(undo);
-  a.window = window; a.parts = parts;
-  auto go = [&](auto first, auto second) {
-    launch_pdl(first, dim3((unsigned)row_blocks), dim3(C4_THREADS), 0, stream, a);
-    launch_pdl(second, dim3((unsigned)blocks), dim3(C4_THREADS), 0, stream, a);
-  };
-  if (hd == 64) go(kv4_prompt_rows_kernel<64>, kv4_unpack16_kernel<64>); else go(kv4_prompt_rows_kernel<128>, kv4_unpack16_kernel<128>);
-  return launch_status("kv4_unpack16");
 }

@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import Optional
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -1833,6 +1833,17 @@ def _entry(name: str, args: str):
     return fn
 
 
+def _long_entry(name: str, ints: int):
+    """The entry point ``name`` of so many ints that returns a long long and launches nothing."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = getattr(library(), name)
+        fn.argtypes = [_c_int] * ints
+        fn.restype = ctypes.c_longlong
+        _ENTRIES[name] = fn
+    return fn
+
+
 def _addr(t: Optional[torch.Tensor]) -> int:
     if t is None:
         return 0
@@ -1993,13 +2004,16 @@ def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: i
 
 def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row_start: Optional[torch.Tensor],
              row_pos0: torch.Tensor, tiles: Optional[tuple], max_new: int, max_len: int, heads: int, kv_heads: int,
-             head_dim: int, scale: float, window: int = 0, workspace=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+             head_dim: int, scale: float, window: int = 0, workspace=None, out: Optional[torch.Tensor] = None,
+             row_lens: Optional[Sequence[Tuple[int, int]]] = None) -> torch.Tensor:
     """Causal attention of a step's new tokens over the 4-bit cache, which already holds them: ``softmax(q K^T * scale) V`` with K and V
     as the pages stand for them.  Row r has tokens ``row_start[r] .. row_start[r + 1] - 1`` of ``q`` bfloat16 ``[T, heads * head_dim]`` at positions
     ``row_pos0[r] ...`` (``row_start`` None: row r is token r); ``max_new``: the most tokens of a row, ``max_len``: the most keys of one.
     ``window`` > 0: a query sees the last ``window`` keys, its own among them.  A query that sees nothing gets zeros.
     ``tiles``: ``(row, first new token, count)`` of the tiles of 128 queries, as ``attn_prefill_tc`` takes them, for rows of many new
     tokens (None: never more than a few).  ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's).
+    ``row_lens``: (tokens before the step, new tokens) of each row, as the device arrays have them, for callers that know them on the host: prompts of unequal
+    rows then take the scratch memory of the pages that they see, not of as many rows of ``max_len``.
 
     A few tokens a row (``_kv4_walks``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
     unpacked to fp16, times a power of two for a row's keys and one for its values of a head (what is 2^28 below the largest that the row's queries see
@@ -2025,13 +2039,15 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         out = torch.empty_like(q) if plain else q.new_empty((T, heads * head_dim))
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
         raise KernelLibraryError(f"kv4_attn: out must be contiguous bfloat16 {(T, heads * head_dim)}")
+    if row_lens is not None and len(row_lens) != rows:
+        raise KernelLibraryError(f"kv4_attn: row_lens has {len(row_lens)} entries for {rows} rows")
     if T == 0 or rows == 0:
         return out
     columns_wanted = max_new * (heads // kv_heads)
     span = min(max_len, window + max_new - 1) if window > 0 else max_len
     if tiles is not None and columns_wanted > KV4_FEW_COLUMNS and not _kv4_walks(rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, span):
-        return _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window,
-                                workspace, out)
+        return _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, max_new, max_len, heads, kv_heads, head_dim, scale, window,
+                                workspace, out, row_lens)
     columns = 4 if columns_wanted <= 4 else 8 if columns_wanted <= 8 else 16
     groups = -(-columns_wanted // columns)
     chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, _sms(q))
@@ -2051,16 +2067,44 @@ def kv4_prompt_status() -> int:
     return int(library().exl3_kv4_prompt_status())
 
 
-def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, heads, kv_heads, head_dim, scale, window, workspace, out):
+KV4_PROMPT_BYTES = 512 << 20      # scratch for fp16 copies of pages that a prompt step takes beyond what two of its longest rows need
+
+
+def _kv4_passes(row_pages: int, total: int, page_bytes: int) -> tuple:
+    """``(slots, stride, passes)`` for rows of up to ``row_pages`` pages each and ``total`` together: all at once where that fits into
+    ``KV4_PROMPT_BYTES`` (or two of the longest rows), else rows in turn: a row begins in the pass (pages before it) // stride."""
+    most = max(2 * row_pages, KV4_PROMPT_BYTES // page_bytes)
+    if total <= most:
+        return total, 1 << 30, 1
+    stride = most - row_pages + 1
+    return most, stride, (total - 1) // stride + 1
+
+
+def _kv4_row_pages(ctx: int, new: int, window: int, width: int) -> int:
+    """Pages that the queries of a row see."""
+    lo = max(0, ctx - window + 1) // KV4_PAGE if window else 0
+    return max(0, min(-(-(ctx + new) // KV4_PAGE), width) - lo) if new > 0 else 0
+
+
+def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, max_new, max_len, heads, kv_heads, head_dim, scale, window, workspace, out, row_lens):
     """Prompts: the rows' pages and the queries in fp16 in scratch memory, and the tcgen05 attention over them (attention_prefill_f16.cu)."""
     T, rows, width = q.shape[0], row_pos0.numel(), block_table.shape[1]
-    up = lambda n: -(-n // 16) * 16
-    # copies of the pages, the queries and their factors, where rows' copies are, sizes by parts and what undoes their factors
-    need = 4 * rows * width * kv_heads * KV4_PAGE * head_dim + up(2 * T * heads * head_dim) + up(4 * T * heads) + 16 * rows + 8 * rows * kv_heads * (min(-(-width // 4), 32) + 1)
+    if row_lens is not None:
+        sizes = [_kv4_row_pages(c, n, window, width) for c, n in row_lens]
+        row_pages, total = max(sizes), sum(sizes)
+    else:
+        row_pages = min(width, -(-max_len // KV4_PAGE))
+        if window:
+            row_pages = min(row_pages, (window + max_new - 2) // KV4_PAGE + 2)
+        total = min(rows, T) * row_pages
+    row_pages, total = max(1, row_pages), max(1, total)
+    slots, stride, passes = _kv4_passes(row_pages, total, 4 * kv_heads * KV4_PAGE * head_dim)
+    need = _long_entry("exl3_kv4_prompt_scratch", 10)(T, rows, row_pages, total, slots, passes, tiles[2], heads, kv_heads, head_dim)
     scratch = workspace.plain(need // 4) if workspace is not None else torch.empty(need // 4, dtype=torch.float32, device=q.device)
-    rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifpl")(
-        _addr(q), q.stride(0), T, _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), rows, width, _addr(row_start), _addr(row_pos0),
-        _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, _addr(scratch), need, _raw_stream())
+    rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifiiiiipl")(
+        _addr(q), q.stride(0), T, _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), rows, width, _addr(row_start),
+        _addr(row_pos0), _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, row_pages, total, slots, stride, passes,
+        _addr(scratch), need, _raw_stream())
     if rc:
         _check(rc, "kv4_attn")
     return out

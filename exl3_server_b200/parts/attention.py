@@ -149,7 +149,7 @@ class Attention:
         inv_freq = self.position.fused_rotation(s.head_dim)[0]
         q = K.kv4_store(qkv, inv_freq, batch.tok_pos, batch.tok_seq, kv.block_table, kv.k, s.heads, s.kv_heads, s.head_dim)
         return K.kv4_attn(q, kv.k, kv.block_table, batch.row_start, batch.row_pos0, batch.tiles.get(128), batch.max_new, batch.max_kv_len,
-                          s.heads, s.kv_heads, s.head_dim, self.scale, window=s.window, workspace=batch.workspace)
+                          s.heads, s.kv_heads, s.head_dim, self.scale, window=s.window, workspace=batch.workspace, row_lens=batch.row_lens)
 
     def _prompt_fused(self, x, batch, kv):
         """Prompts in bfloat16 with heads and pages of 64, enough rows for the paired GEMM and an attention kernel

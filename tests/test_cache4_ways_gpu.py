@@ -116,3 +116,66 @@ def test_values_of_rows_and_heads_differ_in_size(way, d, new):
                 err = float((out[at + i, 2 * g:2 * g + 2] - want[2 * g:2 * g + 2]).abs().max())
                 assert err <= (2.0 ** -7 + 2 * moved) * float(c.v[r][:, g].abs().max()), (r, i, g)
         at += n
+
+
+# ---- scratch memory -------------------------------------------------------------------------------------------------------------
+
+def peak(f):
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = f()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("window", [0, 200])
+def test_scratch_is_of_the_pages_that_are_seen(window):
+    """A long prompt among short ones, with the rows' lengths known on the host: copies of the pages that each row sees, not of as many as the longest
+    has; and the same bits without the lengths."""
+    rows = [(0, 6000)] + [(0, 200)] * 31
+    c = Case(rows, 8, 8, 64, seed=25)
+    c.row_lens = rows
+    known, took = peak(lambda: c.run(window, row_lens=rows))
+    pages = sum(-(-n // 64) for _, n in rows)
+    copies, queries = pages * 8 * 64 * 64 * 4, 2 * c.q.numel()
+    assert took <= copies + 2 * queries + (4 << 20), (took, copies)                 # the queries' copies, the result, the plan
+    assert torch.equal(c.run(window), known)
+    c.check(known, window, only=(0, 63, 64, 199, 4000, 5999))
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,window", [(4, 4, 64, 0), (40, 20, 64, 90), (8, 2, 128, 0), (7, 1, 128, 150)])
+@pytest.mark.parametrize("known", [True, False])
+def test_rows_in_several_passes(heads, kv_heads, d, window, known, monkeypatch):
+    """As many passes as two of the longest rows' pages at a time make of it: the same bits as in one."""
+    monkeypatch.setattr(K(), "_kv4_walks", lambda *a: False)
+    rows = [(300, 200), (0, 130), (0, 0), (700, 17), (64, 64), (5, 300), (0, 1), (600, 129), (130, 40)]
+    c = Case(rows, heads, kv_heads, d, seed=26)
+    c.table[1, 0], c.table[7, 9] = -1, -1
+    kw = dict(row_lens=rows) if known else {}
+    one = c.run(window, **kw)
+    monkeypatch.setattr(K(), "KV4_PROMPT_BYTES", 0)
+    assert torch.equal(c.run(window, **kw), one)
+    K().check_status()
+
+
+@pytest.mark.parametrize("said", [dict(max_len=100), dict(row_lens=[(90, 60), (0, 10)]), dict(row_lens=[(0, 1), (0, 1)])])
+def test_rows_longer_than_was_said(said, monkeypatch):
+    """What is beyond the sizes of the call is hidden; nothing is written or read out of place (the rows before stay right)."""
+    monkeypatch.setattr(K(), "_kv4_walks", lambda *a: False)
+    c = Case([(90, 60), (200, 150)], 4, 2, 64, seed=27)
+    want = c.run().view(210, 4, 64)
+    lens = said.pop("row_lens", None)
+    c.max_len = said.get("max_len", c.max_len)
+    out = c.run(row_lens=lens).view(210, 4, 64)
+    assert bool(out.isfinite().all())
+    if lens is None or lens[0] == (90, 60):
+        assert torch.equal(out[:10], want[:10])                                     # positions 90 .. 99, all of whose keys are within the sizes
+    K().check_status()
+
+
+def test_row_lens_of_another_number_of_rows_are_refused():
+    from exl3_server_b200.ops.lib import KernelLibraryError
+    c = Case([(90, 60)], 4, 2, 64, seed=28)
+    with pytest.raises(KernelLibraryError, match="row_lens"):
+        c.run(row_lens=[(90, 60), (0, 1)])
