@@ -468,19 +468,20 @@ int exl3_kv4_load(const void* pool, int64_t n_pages, const int* pages, int n, in
                   cudaStream_t stream);
 // Attention of prompts over the 4-bit cache, by fp16 copies of the rows' pages in `slots` places of scratch memory.  row_pages, total: the most pages
 // of a row and of all rows that their queries see (what is beyond is hidden, as are pages that are not there, or beyond the table's width).  A
-// row's pages are copied in the pass (pages of the rows before it) / stride, so slots = total for one pass, else at least stride - 1 + row_pages.
+// row's pages are copied in the pass (pages of the rows before it) / stride, so slots = total for one pass, else at least stride - 1 + row_pages.  Rows of
+// up to `few` new tokens are left out: neither their pages nor their results are touched.
 long long exl3_kv4_prompt_scratch(int T, int rows, int row_pages, int total, int slots, int passes, int n_tiles, int nh, int nkv, int hd);
 int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
                     int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0, int n_tiles, int nh,
-                    int nkv, int hd, int window, float scale, int row_pages, int total, int slots, int stride, int passes, void* scratch,
+                    int nkv, int hd, int window, float scale, int few, int row_pages, int total, int slots, int stride, int passes, void* scratch,
                     long long scratch_bytes, cudaStream_t stream);
 int exl3_kv4_prompt_status();
 // Attention of one token or a few per row over the 4-bit cache.  Row r has tokens row_start[r] .. row_start[r + 1] - 1 (null: token r) at positions
-// row_pos0[r] ...; chunk: tiles of 4096 / hd keys that a block walks, max_chunks: chunks of the longest row (window's reach).
+// row_pos0[r] ...; rows of more than `few` new tokens are left out where few > 0; chunk: tiles of 4096 / hd keys that a block walks, max_chunks: chunks of the longest row (window's reach).
 long long exl3_kv4_attn_scratch(int rows, int max_new, int nh, int nkv, int hd, int max_chunks);
 int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
                   int bt_width, const int* row_start, const int* row_pos0, int rows, int T, int max_new, int nh, int nkv, int hd, int window,
-                  float scale, int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream);
+                  float scale, int few, int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream);
 // Code left by a bounded wait that ran out (0: none); cleared by the call.
 int exl3_kv4_attn_status();
 // 8-bit floating point (e4m3, fp8.cuh): w codes [N, K] with scales sw [ceil(N / 128), ceil(K / 128)], x bfloat16 rounded to codes with a scale per row

@@ -120,6 +120,7 @@ struct A4Args {
   const int* row_start;      // null: row r is token r
   const int* row_pos0;
   int nh, nkv, window;
+  int few;                   // > 0: rows of more new tokens are not taken here
   float scale_log2;          // softmax scale * log2(e)
   int chunk;                 // tiles of a chunk, aligned to absolute positions
   int max_chunks;            // chunks that the grid (and the scratch) has room for
@@ -133,7 +134,7 @@ template <int HD> struct A4Range {
   __device__ inline A4Range(const A4Args& a, int row, int ct, int columns) {
     start = a.row_start ? __ldcg(a.row_start + row) : row;
     n_new = a.row_start ? __ldcg(a.row_start + row + 1) - start : 1;
-    if (start < 0 || start + n_new > a.T) n_new = 0;       // (rows that q does not have)
+    if (start < 0 || start + n_new > a.T || (a.few > 0 && n_new > a.few)) n_new = 0;       // (rows that q does not have, rows of another kernel)
     pos0 = __ldcg(a.row_pos0 + row);
     G = a.nh / a.nkv;
     col0 = ct * columns;
@@ -644,9 +645,9 @@ extern "C" long long exl3_kv4_attn_scratch(int rows, int max_new, int nh, int nk
 
 extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const void* pool, int64_t n_pages, const int* block_table,
                              int bt_stride, int bt_width, const int* row_start, const int* row_pos0, int rows, int T, int max_new, int nh, int nkv,
-                             int hd, int window, float scale, int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream) {
+                             int hd, int window, float scale, int few, int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream) {
   if (rows == 0 || max_new == 0) return 0;
-  if (rows < 0 || rows > 65535 || max_new < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || window < 0 || chunk < 1 ||
+  if (rows < 0 || rows > 65535 || max_new < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || window < 0 || few < 0 || chunk < 1 ||
       chunk > A4_MAX_CHUNK || max_chunks < 1 || n_pages < 1 || n_pages > INT32_MAX || bt_width < 1 || T < 0 || !q || !out || !pool || !block_table ||
       !row_pos0 || (!row_start && max_new != 1)) {
     set_error("kv4_attn: needs heads of 64 or 128, chunks of 1 to %d tiles and all of its arrays, got rows=%d max_new=%d heads=%d kv_heads=%d "
@@ -662,7 +663,7 @@ extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const v
   A4Args a = {};
   a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.out = static_cast<__nv_bfloat16*>(out);
   a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.block_table = block_table; a.bt_stride = bt_stride; a.bt_width = bt_width; a.T = T;
-  a.row_start = row_start; a.row_pos0 = row_pos0; a.nh = nh; a.nkv = nkv; a.window = window; a.scale_log2 = scale * 1.4426950408889634f;
+  a.row_start = row_start; a.row_pos0 = row_pos0; a.nh = nh; a.nkv = nkv; a.window = window; a.few = few; a.scale_log2 = scale * 1.4426950408889634f;
   a.chunk = chunk; a.max_chunks = max_chunks; a.n_ct = ceil_div(ncol, columns); a.scratch = scratch;
   if ((int64_t)a.nkv * a.n_ct > 65535) { set_error("kv4_attn: too many new tokens for this kernel"); return ERR_UNSUPPORTED; }
   static bool configured = false;

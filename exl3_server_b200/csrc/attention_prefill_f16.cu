@@ -22,15 +22,15 @@ static long long kv4_up16(long long n) { return (n + 15) / 16 * 16; }
 extern "C" long long exl3_kv4_prompt_scratch(int T, int rows, int row_pages, int total, int slots, int passes, int n_tiles, int nh, int nkv, int hd) {
   return 2 * (long long)slots * nkv * 64 * hd * 2 + kv4_up16((long long)T * nh * hd * 2) + kv4_up16((long long)T * nh * 4) + 16ll * rows +
          16ll * passes + 16ll * total + kv4_up16(4ll * rows) + 2 * kv4_up16(4ll * n_tiles) + kv4_up16(8ll * rows * nkv) +
-         8ll * rows * nkv * c4_prompt_parts(row_pages);
+         kv4_up16(8ll * rows * nkv * c4_prompt_parts(row_pages));
 }
 
 extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const void* pool, int64_t n_pages, const int* block_table,
                                int bt_stride, int rows, int width, const int* row_start, const int* row_pos0, const int* tile_seq, const int* tile_q0,
-                               int n_tiles, int nh, int nkv, int hd, int window, float scale, int row_pages, int total, int slots, int stride,
+                               int n_tiles, int nh, int nkv, int hd, int window, float scale, int few, int row_pages, int total, int slots, int stride,
                                int passes, void* scratch, long long scratch_bytes, cudaStream_t stream) {
   if (T == 0 || n_tiles == 0) return 0;
-  if (T < 0 || rows < 1 || width < 1 || nkv < 1 || nh < 1 || nh % nkv || !fa_supported(hd, 64) || n_tiles < 0 || window < 0 || n_pages < 1 ||
+  if (T < 0 || rows < 1 || width < 1 || nkv < 1 || nh < 1 || nh % nkv || !fa_supported(hd, 64) || n_tiles < 0 || window < 0 || few < 0 || n_pages < 1 ||
       n_pages > INT32_MAX || row_pages < 1 || total < 1 || stride < 1 || passes < 1 || (total - 1) / stride >= passes ||
       slots < (passes == 1 ? total : stride - 1 + row_pages) || !q || !out || !pool || !block_table || !row_start || !row_pos0 || !tile_seq || !tile_q0 ||
       !scratch) {
@@ -49,7 +49,7 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
   C4Prompt a = {};
   a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.nkv = nkv;
   a.block_table = block_table; a.bt_stride = bt_stride; a.width = width; a.rows = rows;
-  a.row_start = row_start; a.row_pos0 = row_pos0; a.window = window; a.parts = c4_prompt_parts(row_pages);
+  a.row_start = row_start; a.row_pos0 = row_pos0; a.window = window; a.few = few; a.parts = c4_prompt_parts(row_pages);
   a.tile_seq = tile_seq; a.tile_q0 = tile_q0; a.n_tiles = n_tiles;
   a.row_pages = row_pages; a.total = total; a.stride = stride; a.passes = passes;
   a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.T = T; a.nh = nh;

@@ -256,7 +256,8 @@ __device__ inline float c4_pow2(int e) { return __int_as_float((127 + e) << 23);
 template <int HD> __device__ inline void c4_tops(const C4Prompt& a, int64_t item) {
   constexpr int SPP = HD / 64, NG = HD / 32, AHEAD = 4;                // tiles of a page, groups of a token, pages asked for at a time
   const int lane = threadIdx.x & 31, part = (int)(item % a.parts), kv = (int)(item / a.parts % a.nkv), row = (int)(item / a.parts / a.nkv);
-  const int pos0 = __ldcg(a.row_pos0 + row), end = pos0 + __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row);
+  const int pos0 = __ldcg(a.row_pos0 + row), n_new = __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row), end = pos0 + n_new;
+  if (n_new <= a.few) return;
   const int first = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;    // places first .. end - 1 are seen
   const int pages = end > 0 ? min(min((end - 1) / PAGE + 1, a.width), first / PAGE + a.row_pages) : 0;
   float top[2] = {0.0f, 0.0f};
@@ -353,7 +354,7 @@ __device__ inline void c4_plan_rows(const C4Prompt& a) {
     if (row < a.rows) {
       const int n_new = __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row), pos0 = __ldcg(a.row_pos0 + row);
       end = pos0 + n_new;
-      if (n_new > 0 && end > 0) {
+      if (n_new > a.few && end > 0) {
         lo = a.window > 0 ? max(0, pos0 - a.window + 1) / PAGE : 0;
         pages = (end - 1) / PAGE + 1 - lo;
         count = max(0, min(min(pages, a.width - lo), a.row_pages));
@@ -421,7 +422,8 @@ __device__ inline void c4_plan_tiles(const C4Prompt& a) {
     const int first = out;
     for (int t0 = 0; t0 < a.n_tiles; t0 += C4_THREADS) {
       const int t = t0 + threadIdx.x, row = t < a.n_tiles ? __ldcg(a.tile_seq + t) : -1, q0 = t < a.n_tiles ? __ldcg(a.tile_q0 + t) : 0;
-      const bool mine = row >= 0 && row < a.rows && (a.passes == 1 || __ldcg(a.pass_of + row) == p);
+      bool mine = row >= 0 && row < a.rows && (a.passes == 1 || __ldcg(a.pass_of + row) == p);
+      if (mine && a.few > 0) mine = __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row) > a.few;
       int all;
       const int at = out + c4_scan(mine ? 1 : 0, warp_sums, all);
       if (mine) {

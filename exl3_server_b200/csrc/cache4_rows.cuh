@@ -33,6 +33,7 @@ struct C4Prompt {
   int bt_stride, width, rows;
   const int *row_start, *row_pos0;
   int window, parts;
+  int few;               // rows of up to so many new tokens are not taken here
   const int *tile_seq, *tile_q0;
   int n_tiles;
   int row_pages, total;  // pages at most of a row, and of all rows

@@ -2015,10 +2015,10 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     ``row_lens``: (tokens before the step, new tokens) of each row, as the device arrays have them, for callers that know them on the host: prompts of unequal
     rows then take the scratch memory of the pages that they see, not of as many rows of ``max_len``.
 
-    A few tokens a row (``_kv4_walks``) walk the codes themselves (attention_cache4.cu); prompts have their rows' pages
-    unpacked to fp16, times a power of two for a row's keys and one for its values of a head (what is 2^28 below the largest that the row's queries see
-    loses bits), and go through the tcgen05 attention.  A NaN among a token's values makes its group of 32 features NaN for those who see it, and
-    in the prompt form all features of its head."""
+    Rows of a few tokens (all of a step's by ``_kv4_walks``, else those of up to 16 columns) walk the codes themselves (attention_cache4.cu);
+    prompts have their rows' pages unpacked to fp16, times a power of two for a row's keys and one for its values of a head (what is 2^28 below the largest
+    that the row's queries see loses bits), and go through the tcgen05 attention.  A NaN among a token's values makes its group of 32 features NaN for
+    those who see it, and in the prompt form all features of its head."""
     plain = q.is_contiguous()
     if q.dtype is not torch.bfloat16 or q.ndim != 2 or q.shape[1] != heads * head_dim or not (plain or q.stride(1) == 1):
         raise KernelLibraryError(f"kv4_attn: q must be bfloat16 [tokens, {heads * head_dim}], got {q.dtype} {tuple(q.shape)}")
@@ -2043,21 +2043,47 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         raise KernelLibraryError(f"kv4_attn: row_lens has {len(row_lens)} entries for {rows} rows")
     if T == 0 or rows == 0:
         return out
-    columns_wanted = max_new * (heads // kv_heads)
+    group = heads // kv_heads
+    pitch = heads * head_dim if plain else q.stride(0)
+    rest = (heads, kv_heads, head_dim, window, scale)
+    if tiles is None or max_new * group <= KV4_FEW_COLUMNS or _kv4_walks(
+            rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, min(max_len, window + max_new - 1) if window > 0 else max_len):
+        return _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, max_new, max_len, *rest, 0, workspace, out)
+    # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000 keys
+    # beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 168 us and 5 MB this way).
+    few, few_len = 0, max_len
+    if row_lens is not None:
+        most = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1)
+        short = [(n, c + n) for c, n in row_lens if 0 < n <= most]
+        if short:
+            few, few_len = max(n for n, _ in short), max(k for _, k in short)
+    elif T < rows * max_new:
+        few = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1)
+    _kv4_attn_prompt(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, tiles, max_new, max_len, *rest, few, workspace, out, row_lens)
+    if few:
+        _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, few, few_len, *rest, few, workspace, out)
+    return out
+
+
+def _kv4_scratch(floats: int, workspace, q: torch.Tensor) -> torch.Tensor:
+    return workspace.plain(floats) if workspace is not None else torch.empty(floats, dtype=torch.float32, device=q.device)
+
+
+def _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, max_new, max_len, heads, kv_heads, head_dim, window, scale, few,
+                    workspace, out) -> torch.Tensor:
+    """Rows of up to ``max_new`` tokens walk the codes (attention_cache4.cu); with ``few`` > 0 those of more than so many are left out."""
+    wanted = max_new * (heads // kv_heads)
+    columns = 4 if wanted <= 4 else 8 if wanted <= 8 else 16
+    groups = -(-wanted // columns)
     span = min(max_len, window + max_new - 1) if window > 0 else max_len
-    if tiles is not None and columns_wanted > KV4_FEW_COLUMNS and not _kv4_walks(rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, span):
-        return _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, max_new, max_len, heads, kv_heads, head_dim, scale, window,
-                                workspace, out, row_lens)
-    columns = 4 if columns_wanted <= 4 else 8 if columns_wanted <= 8 else 16
-    groups = -(-columns_wanted // columns)
     chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, _sms(q))
     need, scratch = 0, None
     if chunks > 1:
         need = rows * kv_heads * groups * chunks * columns * (head_dim + 4)
-        scratch = workspace.plain(need) if workspace is not None else torch.empty(need, dtype=torch.float32, device=q.device)
-    rc = _entry("exl3_kv4_attn", "plpplpiippiiiiiiifiipl")(
-        _addr(q), heads * head_dim if plain else q.stride(0), _addr(out), _addr(pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1],
-        _addr(row_start), _addr(row_pos0), rows, T, max_new, heads, kv_heads, head_dim, window, scale, chunk, chunks, _addr(scratch), need, _raw_stream())
+        scratch = _kv4_scratch(need, workspace, q)
+    rc = _entry("exl3_kv4_attn", "plpplpiippiiiiiiifiiipl")(
+        _addr(q), pitch, _addr(out), _addr(pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], _addr(row_start),
+        _addr(row_pos0), rows, q.shape[0], max_new, heads, kv_heads, head_dim, window, scale, few, chunk, chunks, _addr(scratch), need, _raw_stream())
     if rc:
         _check(rc, "kv4_attn")
     return out
@@ -2086,28 +2112,29 @@ def _kv4_row_pages(ctx: int, new: int, window: int, width: int) -> int:
     return max(0, min(-(-(ctx + new) // KV4_PAGE), width) - lo) if new > 0 else 0
 
 
-def _kv4_attn_prompt(q, pool, block_table, row_start, row_pos0, tiles, max_new, max_len, heads, kv_heads, head_dim, scale, window, workspace, out, row_lens):
-    """Prompts: the rows' pages and the queries in fp16 in scratch memory, and the tcgen05 attention over them (attention_prefill_f16.cu)."""
-    T, rows, width = q.shape[0], row_pos0.numel(), block_table.shape[1]
+def _kv4_attn_prompt(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, tiles, max_new, max_len, heads, kv_heads, head_dim, window, scale, few,
+                     workspace, out, row_lens) -> None:
+    """Rows of more than ``few`` tokens: their pages and the queries in fp16 in scratch memory, and the tcgen05 attention over them
+    (attention_prefill_f16.cu)."""
+    T, width = q.shape[0], block_table.shape[1]
     if row_lens is not None:
-        sizes = [_kv4_row_pages(c, n, window, width) for c, n in row_lens]
+        sizes = [_kv4_row_pages(c, n, window, width) for c, n in row_lens if n > few] or [1]
         row_pages, total = max(sizes), sum(sizes)
     else:
         row_pages = min(width, -(-max_len // KV4_PAGE))
         if window:
             row_pages = min(row_pages, (window + max_new - 2) // KV4_PAGE + 2)
-        total = min(rows, T) * row_pages
+        total = max(1, min(rows, T // (few + 1))) * row_pages
     row_pages, total = max(1, row_pages), max(1, total)
     slots, stride, passes = _kv4_passes(row_pages, total, 4 * kv_heads * KV4_PAGE * head_dim)
     need = _long_entry("exl3_kv4_prompt_scratch", 10)(T, rows, row_pages, total, slots, passes, tiles[2], heads, kv_heads, head_dim)
-    scratch = workspace.plain(need // 4) if workspace is not None else torch.empty(need // 4, dtype=torch.float32, device=q.device)
-    rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifiiiiipl")(
-        _addr(q), q.stride(0), T, _addr(out), _addr(pool), pool.shape[0], _addr(block_table), block_table.stride(0), rows, width, _addr(row_start),
-        _addr(row_pos0), _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, row_pages, total, slots, stride, passes,
+    scratch = _kv4_scratch(need // 4, workspace, q)
+    rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifiiiiiipl")(
+        _addr(q), pitch, T, _addr(out), _addr(pool), pages, _addr(block_table), block_table.stride(0), rows, width, _addr(row_start), _addr(row_pos0),
+        _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, few, row_pages, total, slots, stride, passes,
         _addr(scratch), need, _raw_stream())
     if rc:
         _check(rc, "kv4_attn")
-    return out
 
 
 # ---- products in 8-bit floating point (fp8.cuh) ---------------------------------------------------------------

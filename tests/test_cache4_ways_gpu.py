@@ -3,6 +3,8 @@ is a matter of time and must not show in its results.
 
 Tolerances are test_cache4_gpu.py's (``Case.check``): the result is rounded to bfloat16, the terms to fp16, in the unpacked form keys, values and
 queries to fp16 as well, after a power of two that brings a row's largest near fp16's: 2^-7 of the largest value and what rounded keys move."""
+import math
+
 import pytest
 import torch
 
@@ -179,3 +181,31 @@ def test_row_lens_of_another_number_of_rows_are_refused():
     c = Case([(90, 60)], 4, 2, 64, seed=28)
     with pytest.raises(KernelLibraryError, match="row_lens"):
         c.run(row_lens=[(90, 60), (0, 1)])
+
+
+# ---- rows of a few tokens beside prompts ----------------------------------------------------------------------------------------
+
+MIXED = [(700, 1), (0, 200), (1300, 1), (64, 1), (90, 150), (0, 1), (0, 0), (513, 2), (40, 17)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (16, 2, 64), (40, 1, 64), (8, 2, 128), (7, 1, 128)])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("known", [True, False])
+def test_single_tokens_beside_prompts(heads, kv_heads, d, window, known, monkeypatch):
+    monkeypatch.setattr(K(), "_kv4_walks", lambda *a: False)
+    c = Case(MIXED, heads, kv_heads, d, seed=29)
+    out = c.run(window, row_lens=MIXED if known else None, out=torch.full_like(c.q, math.nan))
+    c.check(out, window, only=(0, 1, 16, 149, 199))
+    K().check_status()
+
+
+def test_single_tokens_beside_a_prompt_are_not_unpacked():
+    """Long rows that decode beside a short prompt take no scratch for their pages, with or without the lengths."""
+    rows = [(6000, 1)] * 15 + [(0, 300)]
+    c = Case(rows, 8, 2, 128, seed=30)
+    for lens in (rows, None):
+        _, took = peak(lambda: c.run(row_lens=lens))
+        one = 95 * 2 * 64 * 128 * 4                                    # copies of a long row's pages
+        chunks = 16 * 8 * 24 * 132 * 4 * 4                             # records of up to 24 chunks of 8 heads, 16 columns at most
+        assert took <= (0 if lens else 16) * one + 4 * 2 * c.q.numel() + chunks + (4 << 20), took
+    c.check(c.run(row_lens=rows), only=(0, 299))
