@@ -2046,7 +2046,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     group = heads // kv_heads
     pitch = heads * head_dim if plain else q.stride(0)
     rest = (heads, kv_heads, head_dim, window, scale)
-    if tiles is None or max_new * group <= KV4_FEW_COLUMNS or _kv4_walks(
+    if tiles is None or row_start is None or max_new * group <= KV4_FEW_COLUMNS or _kv4_walks(
             rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, min(max_len, window + max_new - 1) if window > 0 else max_len):
         return _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, max_new, max_len, *rest, 0, workspace, out)
     # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000 keys

@@ -209,3 +209,13 @@ def test_single_tokens_beside_a_prompt_are_not_unpacked():
         chunks = 16 * 8 * 24 * 132 * 4 * 4                             # records of up to 24 chunks of 8 heads, 16 columns at most
         assert took <= (0 if lens else 16) * one + 4 * 2 * c.q.numel() + chunks + (4 << 20), took
     c.check(c.run(row_lens=rows), only=(0, 299))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32, 1), (34, 2), (16, 16)])
+def test_one_token_a_row_without_starts(heads, kv_heads, monkeypatch):
+    """``row_start`` None goes with tiles too, and with more query heads a key/value head than 16."""
+    monkeypatch.setattr(K(), "_kv4_walks", lambda *a: False)
+    c = Case([(100, 1), (9, 1)], heads, kv_heads, 128, seed=5)
+    want = c.run(tiles=False)
+    c.check(want)
+    assert torch.equal(K().kv4_attn(c.q, c.pool, c.table, None, c.pos0, c.tiles, 1, c.max_len, heads, kv_heads, 128, 128 ** -0.5), want)
