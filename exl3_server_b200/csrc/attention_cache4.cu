@@ -647,11 +647,11 @@ extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const v
                              int bt_stride, int bt_width, const int* row_start, const int* row_pos0, int rows, int T, int max_new, int nh, int nkv,
                              int hd, int window, float scale, int few, int chunk, int max_chunks, float* scratch, long long scratch_floats, cudaStream_t stream) {
   if (rows == 0 || max_new == 0) return 0;
-  if (rows < 0 || rows > 65535 || max_new < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || window < 0 || few < 0 || chunk < 1 ||
+  if (rows < 0 || rows > 65535 || max_new < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || window < 0 || few < 0 || !isfinite(scale) || chunk < 1 ||
       chunk > A4_MAX_CHUNK || max_chunks < 1 || n_pages < 1 || n_pages > INT32_MAX || bt_width < 1 || T < 0 || !q || !out || !pool || !block_table ||
       !row_pos0 || (!row_start && max_new != 1)) {
-    set_error("kv4_attn: needs heads of 64 or 128, chunks of 1 to %d tiles and all of its arrays, got rows=%d max_new=%d heads=%d kv_heads=%d "
-              "head_dim=%d chunk=%d max_chunks=%d", A4_MAX_CHUNK, rows, max_new, nh, nkv, hd, chunk, max_chunks);
+    set_error("kv4_attn: needs heads of 64 or 128, chunks of 1 to %d tiles a finite scale and all of its arrays, got rows=%d max_new=%d heads=%d "
+              "kv_heads=%d head_dim=%d scale=%g chunk=%d max_chunks=%d", A4_MAX_CHUNK, rows, max_new, nh, nkv, hd, (double)scale, chunk, max_chunks);
     return ERR_BAD_ARGUMENT;
   }
   if (!aligned16(q) || !aligned16(out) || !aligned16(pool) || q_stride % 8) { set_error("kv4_attn: q, its rows, out and the pool must be 16-byte aligned"); return ERR_ALIGNMENT; }

@@ -44,6 +44,7 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
     set_error("kv4_prompt: %lld bytes of scratch wanted, 16-byte aligned", need);
     return ERR_SCRATCH;
   }
+  if (!isfinite(scale)) { set_error("kv4_prompt: the scale must be finite, got %g", (double)scale); return ERR_BAD_ARGUMENT; }
   unsigned char* at = static_cast<unsigned char*>(scratch);
   auto take = [&](long long bytes) { unsigned char* p = at; at += kv4_up16(bytes); return p; };
   C4Prompt a = {};
@@ -53,6 +54,7 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
   a.tile_seq = tile_seq; a.tile_q0 = tile_q0; a.n_tiles = n_tiles;
   a.row_pages = row_pages; a.total = total; a.stride = stride; a.passes = passes;
   a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.T = T; a.nh = nh;
+  a.q_sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;        // (the attention takes positive scales)
   a.k_out = reinterpret_cast<__half*>(take((long long)slots * nkv * 64 * hd * 2));
   a.v_out = reinterpret_cast<__half*>(take((long long)slots * nkv * 64 * hd * 2));
   a.q_out = reinterpret_cast<__half*>(take((long long)T * nh * hd * 2));
@@ -70,7 +72,7 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
     rc = c4_prompt_copies(a, hd, p, slots, stream);
     if (!rc)
       rc = fa_run(a.q_out, (int64_t)nh * hd, T, out, a.k_out, a.v_out, (int64_t)slots * nkv * 64, block_table, bt_stride, row_start, row_pos0, a.seq_out,
-                  a.q0_out, n_tiles, nh, nkv, hd, 64, window, 0, 0, scale, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr,
+                  a.q0_out, n_tiles, nh, nkv, hd, 64, window, 0, 0, scale != 0.0f ? fabsf(scale) : 1.0f, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr,
                   FaCopies{a.q_scale, a.undo, a.own, a.pass + p, passes == 1, (int)n_pages}, stream);
   }
   return rc;

@@ -457,7 +457,7 @@ kv4_prompt_plan_kernel(const C4Prompt a) {
 }
 
 // Eight lanes (sixteen for heads of 128) have a query of a head: to fp16, times a power of two that brings its largest value to [2^10, 2^11), whose
-// inverse goes to q_scale.  A query with a value that is not finite becomes NaN.
+// inverse goes to q_scale, and the sign of the scale.  A query with a value that is not finite becomes NaN.
 template <int HD> __device__ inline void c4_query(const C4Prompt& a, int64_t item) {
   constexpr int LANES = HD / 8;
   const int j = threadIdx.x % LANES;
@@ -478,7 +478,7 @@ template <int HD> __device__ inline void c4_query(const C4Prompt& a, int64_t ite
   for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   finite = top < __int_as_float(0x7f800000);
   const int e2 = finite && top > 0.0f ? min(max(10 + 127 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
-  const float up = c4_pow2(e2);
+  const float up = c4_pow2(e2) * a.q_sign;
   if (!live) return;
   __align__(16) __half h[8];
 #pragma unroll

@@ -41,6 +41,7 @@ struct C4Prompt {
   const __nv_bfloat16* q;
   int64_t q_stride;
   int T, nh;
+  float q_sign;          // 1, -1 or 0: what is left of the scale beside a positive one
   __half *k_out, *v_out, *q_out;
   float* q_scale;
   FaRow* own;            // [rows]

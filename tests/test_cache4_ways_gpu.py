@@ -219,3 +219,26 @@ def test_one_token_a_row_without_starts(heads, kv_heads, monkeypatch):
     want = c.run(tiles=False)
     c.check(want)
     assert torch.equal(K().kv4_attn(c.q, c.pool, c.table, None, c.pos0, c.tiles, 1, c.max_len, heads, kv_heads, 128, 128 ** -0.5), want)
+
+
+# ---- arguments ------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 3.0])
+@pytest.mark.parametrize("d,new", [(64, 70), (128, 150)])
+def test_scales(way, scale, d, new):
+    """Any finite scale: a negative one turns the order round, 0 gives the mean of what a query sees."""
+    c = Case([(90, new)], 4, 2, d, seed=31)
+    out = K().kv4_attn(c.q, c.pool, c.table, c.start, c.pos0, c.tiles, c.max_new, c.max_len, 4, 2, d, scale).double().cpu().view(new, 4, d)
+    for i in (0, 3, new - 1):
+        q = c.q[i:i + 1].cpu().view(1, 4, d)
+        want = attend(q, c.k[0], c.v[0], 90 + i, scale)[0]
+        moved = 2.0 ** -12 * abs(scale) * float(q.double().norm(dim=-1).max() * c.k[0].norm(dim=-1).max())
+        assert float((out[i] - want).abs().max()) <= (2.0 ** -7 + 2 * moved) * float(c.v[0].abs().max())
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_scales_that_are_not_finite_are_refused(way, scale):
+    from exl3_server_b200.ops.lib import KernelLibraryError
+    c = Case([(90, 70)], 4, 2, 64, seed=31)
+    with pytest.raises(KernelLibraryError, match="scale"):
+        K().kv4_attn(c.q, c.pool, c.table, c.start, c.pos0, c.tiles, c.max_new, c.max_len, 4, 2, 64, scale)
