@@ -1975,31 +1975,45 @@ def _kv4_walks(rows: int, tiles: int, heads: int, kv_heads: int, head_dim: int, 
     return walk < 10.0 + unpack + 0.75 * -(-span // KV4_PAGE) * max(1.0, tiles * heads / 190.0)
 
 
-@functools.lru_cache(maxsize=4096)
+KV4_MAX_CHUNK = 128         # tiles of a chunk, and
+KV4_MAX_CHUNKS = 1024       # chunks of a row that the plan considers
+
+
 def _kv4_chunks(rows: int, kv_heads: int, groups: int, columns: int, head_dim: int, span: int, window: int, sms: int):
-    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys, by a small model of the kernel's time with constants fitted to 104
-    shapes (what it picks is 5 % slower in the mean than the best of a shape): a wave of blocks takes 10 us and for each of a block's tiles 0.13 us and
-    0.21 us times the blocks that share its SM (a fifth less for heads of 128, a fifth more with 16 columns); rows of a batch are taken to be
-    unequal; joining chunks takes 4.5 us."""
+    """``(tiles of a chunk, chunks)`` for rows of up to ``span`` visible keys."""
     per = 4096 // head_dim
     tiles = (span + per - 2) // per + 1 if window > 0 else max(1, -(-span // per))       # a window may begin anywhere in a tile
+    return _kv4_tile_chunks(rows * kv_heads * groups, rows == 1, columns, head_dim, tiles, window > 0, sms)
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv4_tile_chunks(items: int, one_row: bool, columns: int, head_dim: int, tiles: int, window: bool, sms: int):
+    """By a small model of the kernel's time with constants fitted to 104
+    shapes (what it picks is 5 % slower in the mean than the best of a shape): a wave of blocks takes 10 us and for each of a block's tiles 0.13 us and
+    0.21 us times the blocks that share its SM (a fifth less for heads of 128, a fifth more with 16 columns); rows of a batch are taken to be
+    unequal; joining chunks takes 4.5 us.  Of the sizes that make the same number of chunks only the smallest is tried, at most 128 in all, and a
+    length asks once for every tile that it grows by (a row of 30,000 keys: 0.60 ms for every new length, now 0.05 for every 32nd)."""
     per_sm = 2 if columns == 16 else 3 if columns == 8 and head_dim == 128 else 4
     wide = (1.2 if columns == 16 else 1.0) * (0.8 if head_dim == 128 else 1.0)
-    items = rows * kv_heads * groups
-    best = None
-    for n in range(1, min(tiles, 1024) + 1):
-        chunk = -(-tiles // n)
-        if chunk > 128 or (n > 1 and chunk < 2):
-            continue
+    best, chunk = None, min(tiles, KV4_MAX_CHUNK)
+    while chunk >= 1:
         n = -(-tiles // chunk)
-        blocks = items * n if rows == 1 else items * (0.83 * n + 0.17)
+        if n > KV4_MAX_CHUNKS:
+            break
+        chunk = -(-tiles // n)                                # the smallest size that makes n chunks
+        if n > 1 and chunk < 2:
+            break
+        blocks = items * n if one_row else items * (0.83 * n + 0.17)
         waves = max(1.0, blocks / (per_sm * sms) + (0.5 if blocks > per_sm * sms else 0.0))
         here = min(per_sm, math.ceil(blocks / sms))
         cost = waves * (10.0 + chunk * wide * (0.13 + 0.21 * here)) + (4.5 if n > 1 else 0.0)
         if best is None or cost < best[0] - 1e-9:
             best = (cost, chunk, n)
+        chunk -= 1
+    if best is None:
+        raise KernelLibraryError(f"kv4_attn: a row of {tiles} tiles of {4096 // head_dim} keys is longer than {KV4_MAX_CHUNKS} chunks of {KV4_MAX_CHUNK} tiles")
     _, chunk, n = best
-    return chunk, (tiles + chunk - 2) // chunk + 1 if window > 0 else n                  # and in a chunk
+    return chunk, (tiles + chunk - 2) // chunk + 1 if window else n                      # a window may begin anywhere in a chunk, too
 
 
 def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row_start: Optional[torch.Tensor],
