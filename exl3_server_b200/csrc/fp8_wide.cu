@@ -25,12 +25,14 @@ using namespace tc5;
 
 // ---- activations to codes -------------------------------------------------------------------------------------------
 
-// Eight lanes take a block of 128 features of a row, 16 features a lane.  Codes [M, K]; scales [M, blocks], or [blocks, M] (transposed).
+// Eight lanes take a block of 128 features of a row, 16 features a lane.  Codes [M, K]; scales [M, blocks], or [blocks, M] (transposed: scratch of the
+// product behind, which waits for it).  What a caller gets may be the weights of a product, which reads those ahead of its wait: so the next kernel does
+// not start early then.
 // Bound by memory and, up to some hundred rows, by its launch (64 x 4,096: 2 us of the product's 12).
 __global__ void __launch_bounds__(256)
 fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int M, int K, int kblocks, unsigned char* __restrict__ codes,
                     float* __restrict__ sx, int transposed) {
-  pdl_trigger();
+  if (transposed) pdl_trigger();
   pdl_wait();
   const int64_t item = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
   const int j = threadIdx.x & 7;

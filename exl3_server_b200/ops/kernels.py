@@ -2233,6 +2233,9 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
     float32, the result in ``out_dtype`` (bfloat16 or float32).  ``gated``: W's rows are eight gate rows, then the eight up rows of the same
     features, and so on, and ``silu(gate) * up`` comes out (N / 2 wide, no bias).
 
+    ``w`` and ``w_scale`` are read before the kernels ahead in the stream have ended, where those let the next one start early: they may come from
+    copies, from torch's operations and from ``fp8_quantize`` and ``fp8_quantize_weight``, not from another kernel of this library that is still under way.
+
     A row's bits are the same in any batch of up to 64 rows; ``fixed_order=False`` lets small products of up to 8 rows be added up in another
     order, which takes a fifth to two fifths less time (fp8_gemv.cu)."""
     M, Kd = _fp8_check_x(x, "fp8_linear")
