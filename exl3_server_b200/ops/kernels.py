@@ -1853,6 +1853,11 @@ def _addr(t: Optional[torch.Tensor]) -> int:
     return t.data_ptr()
 
 
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from a matrix's row to the next (a matrix of one row has none, and any stride)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _sms(t: torch.Tensor) -> int:
     """``sm_count`` of a tensor's device."""
     return _SM_COUNT.get(t.get_device()) or sm_count(t.device)
@@ -1933,7 +1938,7 @@ def kv4_store(qkv: torch.Tensor, inv_freq: Optional[torch.Tensor], tok_pos: torc
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, heads * head_dim) or not out.is_contiguous():
         raise KernelLibraryError(f"kv4_store: out must be contiguous bfloat16 {(T, heads * head_dim)}")
     rc = _entry("exl3_kv4_store", "plppppppiiipliiii")(
-        _addr(qkv), qkv.stride(0), _addr(out), hi, lo, _addr(tok_pos), _addr(tok_seq), _addr(block_table), block_table.stride(0),
+        _addr(qkv), _pitch(qkv), _addr(out), hi, lo, _addr(tok_pos), _addr(tok_seq), _addr(block_table), block_table.stride(0),
         *block_table.shape, _addr(pool), pages, T, heads, kv_heads, head_dim, _raw_stream())
     if rc:
         _check(rc, "kv4_store")
@@ -2058,7 +2063,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     if T == 0 or rows == 0:
         return out
     group = heads // kv_heads
-    pitch = heads * head_dim if plain else q.stride(0)
+    pitch = heads * head_dim if plain else _pitch(q)
     rest = (heads, kv_heads, head_dim, window, scale)
     if tiles is None or row_start is None or max_new * group <= KV4_FEW_COLUMNS or _kv4_walks(
             rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, min(max_len, window + max_new - 1) if window > 0 else max_len):
@@ -2188,7 +2193,7 @@ def fp8_quantize(x: torch.Tensor):
 
 
 def _fp8_round(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, transposed: int) -> None:
-    rc = _entry("exl3_fp8_quantize", "pliippi")(_addr(x), x.stride(0), x.shape[0], x.shape[1], _addr(codes), _addr(scales), transposed, _raw_stream())
+    rc = _entry("exl3_fp8_quantize", "pliippi")(_addr(x), _pitch(x), x.shape[0], x.shape[1], _addr(codes), _addr(scales), transposed, _raw_stream())
     if rc:
         _check(rc, "fp8_quantize")
 
@@ -2265,7 +2270,7 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
         room = x.new_empty(M * Kd // 2 + 2 * blocks * M + 8)               # codes, then (16-byte aligned) scales
         codes = room.data_ptr()
         sx = codes + -(-M * Kd // 16) * 16
-    rc = _entry("exl3_fp8_linear", "plppppppiiiiii")(_addr(x), x.stride(0), codes, sx, _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
+    rc = _entry("exl3_fp8_linear", "plppppppiiiiii")(_addr(x), _pitch(x), codes, sx, _addr(w), _addr(w_scale), _addr(bias), _addr(out), code, M, N, Kd,
                                                      1 if gated else 0, 0 if not few else 1 if fixed_order else 2, _raw_stream())
     if rc:
         _check(rc, "fp8_linear")

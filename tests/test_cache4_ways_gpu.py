@@ -242,3 +242,16 @@ def test_scales_that_are_not_finite_are_refused(way, scale):
     c = Case([(90, 70)], 4, 2, 64, seed=31)
     with pytest.raises(KernelLibraryError, match="scale"):
         K().kv4_attn(c.q, c.pool, c.table, c.start, c.pos0, c.tiles, c.max_new, c.max_len, 4, 2, 64, scale)
+
+
+def test_one_token_of_a_matrix_with_any_stride():
+    """A step of one token has no distance between tokens, whatever the stride says."""
+    k = K()
+    c = Case([(10, 1)], 4, 2, 64, seed=14)
+    want = c.run()
+    odd = torch.zeros(1, 8 * 64 + 5, device=DEV).bfloat16()
+    odd[:, :512] = c.qkv[10:11]
+    odd[:, :256] = c.q
+    pool = c.pool.clone()
+    q = k.kv4_store(odd[:, :512], None, ints([10]), ints([0]), c.table, pool, 4, 2, 64)
+    assert torch.equal(q, c.q) and torch.equal(pool, c.pool) and torch.equal(c.run(q=odd[:, :256]), want)
