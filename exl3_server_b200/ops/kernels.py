@@ -2068,6 +2068,10 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
     if tiles is None or row_start is None or max_new * group <= KV4_FEW_COLUMNS or _kv4_walks(
             rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, min(max_len, window + max_new - 1) if window > 0 else max_len):
         return _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, max_new, max_len, *rest, 0, workspace, out)
+    for t in tiles[:2]:
+        _int32(t, "tiles", "kv4_attn")
+        if t.numel() < tiles[2]:
+            raise KernelLibraryError(f"kv4_attn: {tiles[2]} tiles, of which {t.numel()} are listed")
     # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000 keys
     # beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 168 us and 5 MB this way).
     few, few_len = 0, max_len

@@ -255,3 +255,13 @@ def test_one_token_of_a_matrix_with_any_stride():
     pool = c.pool.clone()
     q = k.kv4_store(odd[:, :512], None, ints([10]), ints([0]), c.table, pool, 4, 2, 64)
     assert torch.equal(q, c.q) and torch.equal(pool, c.pool) and torch.equal(c.run(q=odd[:, :256]), want)
+
+
+def test_lists_of_tiles_that_are_refused():
+    from exl3_server_b200.ops.lib import KernelLibraryError
+    c = Case([(90, 200)], 4, 2, 64, seed=32)
+    a, b, n = c.tiles
+    for tiles in ((a.long(), b, n), (a, b.long(), n), (a[:1], b, n), (a, b, n + 1)):
+        c.tiles = tiles
+        with pytest.raises(KernelLibraryError, match="tiles"):
+            c.run()
