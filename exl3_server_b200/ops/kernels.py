@@ -2062,6 +2062,8 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         raise KernelLibraryError(f"kv4_attn: row_lens has {len(row_lens)} entries for {rows} rows")
     if T == 0 or rows == 0:
         return out
+    if window >= max_len:                   # (positions less a window stay within 32 bits)
+        window = 0
     group = heads // kv_heads
     pitch = heads * head_dim if plain else _pitch(q)
     rest = (heads, kv_heads, head_dim, window, scale)

@@ -265,3 +265,11 @@ def test_lists_of_tiles_that_are_refused():
         c.tiles = tiles
         with pytest.raises(KernelLibraryError, match="tiles"):
             c.run()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 40])
+@pytest.mark.parametrize("first", [-3, 40])
+def test_windows_beyond_every_key(way, window, first):
+    c = Case([(40, 100)], 8, 2, 64, seed=33)
+    c.pos0[0] = first
+    assert torch.equal(c.run(window), c.run(0))
