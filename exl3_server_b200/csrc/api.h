@@ -456,8 +456,7 @@ int exl3_embed_sinusoid(const int* ids, const int* tok_pos, const void* table, i
 // type, K and the pitch of x multiples of 16 bytes.
 int exl3_gemm_few_out(const void* x, int64_t ldx, const void* w, const void* bias, float* y, int in_dtype, int M, int N,
                       int K, cudaStream_t stream);
-// The 4-bit key/value cache (format: cache4.cuh).  Bytes of a page of 64 tokens of one key/value head; 0 for heads it does not take.
-int exl3_kv4_page_bytes(int hd);
+// The 4-bit key/value cache (format: cache4.cuh).
 // q, k, v [T, (nh + 2 nkv) * hd] bfloat16: q rotated into q_out [T, nh * hd], k (rotated) and v into the pages of the tokens' positions.  freq: hd / 2
 // frequencies (null: no rotation), freq_lo: what float32 lost of them, or null.
 int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float* freq, const float* freq_lo, const int* tok_pos,
@@ -477,7 +476,8 @@ int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out, const voi
                     long long scratch_bytes, cudaStream_t stream);
 int exl3_kv4_prompt_status();
 // Attention of one token or a few per row over the 4-bit cache.  Row r has tokens row_start[r] .. row_start[r + 1] - 1 (null: token r) at positions
-// row_pos0[r] ...; rows of more than `few` new tokens are left out where few > 0; chunk: tiles of 4096 / hd keys that a block walks, max_chunks: chunks of the longest row (window's reach).
+// row_pos0[r] ...; rows of more than `few` new tokens are left out where few > 0; chunk: tiles of 4096 / hd keys that a block walks, max_chunks:
+// chunks of the longest row (window's reach).
 long long exl3_kv4_attn_scratch(int rows, int max_new, int nh, int nkv, int hd, int max_chunks);
 int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const void* pool, int64_t n_pages, const int* block_table, int bt_stride,
                   int bt_width, const int* row_start, const int* row_pos0, int rows, int T, int max_new, int nh, int nkv, int hd, int window,

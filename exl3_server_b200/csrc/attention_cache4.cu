@@ -20,7 +20,7 @@
 // that keeps the largest scale seen so far below 2^6, carried by p's exponent: p sc keeps its 11 bits down to 2^-20 of the largest) is the second product's operand, the codes of 16 tokens the 16-row
 // one, and sum p mn_g goes beside it in float32.  Scores, maximum, sums and outputs are float32.
 //
-// A column is a (new token, query head) of one key/value head: up to 8 or 16 columns share a walk over the codes, each with its own causal limit.
+// A column is a (new token, query head) of one key/value head: up to 4, 8 or 16 columns share a walk over the codes, each with its own causal limit.
 // A block of four warps takes one (row, key/value head, group of columns, chunk of keys); its warps take every fourth tile of 5,120
 // bytes, through a ring each that bulk copies fill ahead.  The warps' results meet in shared memory.  Where a row has several chunks their
 // records go to scratch memory and a second kernel joins them, in the chunks' order.
@@ -125,7 +125,7 @@ struct A4Args {
   int chunk;                 // tiles of a chunk, aligned to absolute positions
   int max_chunks;            // chunks that the grid (and the scratch) has room for
   int n_ct;                  // groups of columns the grid has room for
-  float* scratch;            // [rows][nkv][n_ct][max_chunks][columns][HD + 2] where max_chunks > 1
+  float* scratch;            // [rows][nkv][n_ct][max_chunks][columns][HD + 4] where max_chunks > 1
 };
 
 // What a (row, group of columns) sees: tiles t_lo .. t_hi, and the chunks that hold them.  Both kernels ask.

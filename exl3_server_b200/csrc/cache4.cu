@@ -532,8 +532,6 @@ int c4_prompt_copies(const C4Prompt& a, int hd, int pass, int slots, cudaStream_
 
 using namespace exl3;
 
-extern "C" int exl3_kv4_page_bytes(int hd) { return hd == 64 || hd == 128 ? kv4::page_bytes(hd) : 0; }
-
 extern "C" int exl3_kv4_store(const void* qkv, int64_t qkv_stride, void* q_out, const float* freq, const float* freq_lo, const int* tok_pos,
                               const int* tok_seq, const int* block_table, int bt_stride, int bt_rows, int bt_width, void* pool, int64_t n_pages, int T,
                               int nh, int nkv, int hd, cudaStream_t stream) {

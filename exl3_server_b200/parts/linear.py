@@ -215,18 +215,6 @@ class LinearFP8:
     def heads_rotated_and_cached(self, *args, **kwargs):
         return None
 
-    def wide_dtype(self, rows: int) -> torch.dtype:
-        return torch.float32 if rows <= SKINNY_ROWS else self.dtype
-
-    def xielu(self, x, act_p, act_n, out_dtype):
-        return None
-
-    def gelu(self, x, out_dtype, tanh: bool = False, relu2: bool = False):
-        return None
-
-    def streams_weights(self, rows: int) -> bool:
-        return True
-
     def fuses_gate(self) -> bool:
         return self.bias is None and self.out_features % 16 == 0
 
