@@ -273,3 +273,28 @@ def test_windows_beyond_every_key(way, window, first):
     c = Case([(40, 100)], 8, 2, 64, seed=33)
     c.pos0[0] = first
     assert torch.equal(c.run(window), c.run(0))
+
+
+# ---- what must not matter, in both forms ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (8, 1, 128), (32, 2, 64)])
+@pytest.mark.parametrize("new,window", [(90, 0), (90, 30), (150, 0), (150, 30)])
+def test_what_lies_in_unused_places_does_not_matter(way, heads, kv_heads, d, new, window):
+    """Places behind the last token, and before the window, hold keys and values of 1e30, then NaN."""
+    c = Case([(100, new)], heads, kv_heads, d, seed=16)
+    want = c.run(window)
+    width = (heads + 2 * kv_heads) * d
+    places = list(range(100 + new, c.table.shape[1] * 64)) + (list(range(0, 100 - 30 + 1)) if window else [])
+    for filler in (torch.randn(len(places), width, device=DEV) * 1e30, torch.full((len(places), width), math.nan, device=DEV)):
+        K().kv4_store(filler.bfloat16(), None, ints(places), ints([0] * len(places)), c.table, c.pool, heads, kv_heads, d)
+        assert torch.equal(c.run(window), want)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("d,new", [(64, 80), (128, 150)])
+def test_queries_that_are_not_finite(way, value, d, new):
+    c = Case([(70, new)], 4, 2, d, seed=10)
+    q = c.q.clone()
+    q[0, d + 6] = value                                                 # head 1 of the first token
+    out = c.run(q=q).view(new, 4, d)
+    assert bool(out[0, 1].isnan().all()) and bool(out[0, [0, 2, 3]].isfinite().all()) and bool(out[1:].isfinite().all())
