@@ -120,12 +120,12 @@ struct A4Args {
   const int* row_start;      // null: row r is token r
   const int* row_pos0;
   int nh, nkv, window;
-  int few;                   // > 0: rows of more new tokens are not taken here
   float scale_log2;          // softmax scale * log2(e)
   int chunk;                 // tiles of a chunk, aligned to absolute positions
   int max_chunks;            // chunks that the grid (and the scratch) has room for
   int n_ct;                  // groups of columns the grid has room for
   float* scratch;            // [rows][nkv][n_ct][max_chunks][columns][HD + 4] where max_chunks > 1
+  int few;                   // rows of more new tokens are not taken here (last: its place ahead of the others moved their loads about, 3 % for heads of 128)
 };
 
 // What a (row, group of columns) sees: tiles t_lo .. t_hi, and the chunks that hold them.  Both kernels ask.
@@ -134,7 +134,7 @@ template <int HD> struct A4Range {
   __device__ inline A4Range(const A4Args& a, int row, int ct, int columns) {
     start = a.row_start ? __ldcg(a.row_start + row) : row;
     n_new = a.row_start ? __ldcg(a.row_start + row + 1) - start : 1;
-    if (start < 0 || start + n_new > a.T || (a.few > 0 && n_new > a.few)) n_new = 0;       // (rows that q does not have, rows of another kernel)
+    if (start < 0 || start + n_new > a.T) n_new = 0;       // (rows that q does not have)
     pos0 = __ldcg(a.row_pos0 + row);
     G = a.nh / a.nkv;
     col0 = ct * columns;
@@ -150,8 +150,9 @@ template <int HD> struct A4Range {
   }
 };
 
-// COLS: columns of a block, 4 (hi and lo side by side), 8 or 16.
-template <int HD, int COLS>
+// COLS: columns of a block, 4 (hi and lo side by side), 8 or 16.  BESIDE: a step's rows of more than `few` new tokens are another kernel's (a kernel of its
+// own: the comparison takes 1.5 % of the time of heads of 128, 64 rows of 130 to 8,000 keys 81.6 -> 83.0 us).
+template <int HD, int COLS, bool BESIDE>
 __global__ void __launch_bounds__(A4_WARPS * 32, COLS == 16 ? 2 : COLS == 8 && HD == 128 ? 3 : 4)
 kv4_attn_kernel(const A4Args a) {
   constexpr bool SIDE = COLS == 4;
@@ -175,7 +176,7 @@ kv4_attn_kernel(const A4Args a) {
   int my_page = -1;
   if (a.window == 0 && warp + A4_WARPS * lane < a.chunk) my_page = page_of((int)blockIdx.x * a.chunk + warp + A4_WARPS * lane);
   const A4Range<HD> r(a, row, ct, COLS);
-  if (r.cols <= 0 || (int)blockIdx.x >= max(r.n_chunks, 1)) return;
+  if (r.cols <= 0 || (BESIDE && r.n_new > a.few) || (int)blockIdx.x >= max(r.n_chunks, 1)) return;
   const int chunk0 = (r.c_first + (int)blockIdx.x) * a.chunk;
   const int tile_a = max(r.t_lo, chunk0), tile_b = min(r.t_hi + 1, chunk0 + a.chunk);      // none where the row sees nothing
   const int my_tile = tile_a + warp + A4_WARPS * lane;
@@ -586,7 +587,7 @@ kv4_join_kernel(const A4Args a, int columns) {
   };
   ask(warp);                                                // (beside the row's lengths, not after them)
   const A4Range<HD> r(a, row, ct, columns);
-  if (c >= r.cols || r.n_chunks <= 1) return;               // (a single chunk wrote the output itself)
+  if (c >= r.cols || r.n_new > a.few || r.n_chunks <= 1) return;      // (a single chunk wrote the output itself)
   for (int k0 = warp; k0 < r.n_chunks; k0 += 4 * A4_JOIN_WARPS) {
     if (k0 > warp) ask(k0);
 #pragma unroll
@@ -663,22 +664,28 @@ extern "C" int exl3_kv4_attn(const void* q, int64_t q_stride, void* out, const v
   A4Args a = {};
   a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.out = static_cast<__nv_bfloat16*>(out);
   a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.block_table = block_table; a.bt_stride = bt_stride; a.bt_width = bt_width; a.T = T;
-  a.row_start = row_start; a.row_pos0 = row_pos0; a.nh = nh; a.nkv = nkv; a.window = window; a.few = few; a.scale_log2 = scale * 1.4426950408889634f;
+  a.row_start = row_start; a.row_pos0 = row_pos0; a.nh = nh; a.nkv = nkv; a.window = window; a.few = few > 0 ? few : INT32_MAX; a.scale_log2 = scale * 1.4426950408889634f;
   a.chunk = chunk; a.max_chunks = max_chunks; a.n_ct = ceil_div(ncol, columns); a.scratch = scratch;
   if ((int64_t)a.nkv * a.n_ct > 65535) { set_error("kv4_attn: too many new tokens for this kernel"); return ERR_UNSUPPORTED; }
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaSuccess;
-    for (const void* f : {(const void*)kv4_attn_kernel<64, 4>, (const void*)kv4_attn_kernel<64, 8>, (const void*)kv4_attn_kernel<64, 16>,
-                          (const void*)kv4_attn_kernel<128, 4>, (const void*)kv4_attn_kernel<128, 8>, (const void*)kv4_attn_kernel<128, 16>})
+    for (const void* f : {(const void*)kv4_attn_kernel<64, 4, false>, (const void*)kv4_attn_kernel<64, 8, false>, (const void*)kv4_attn_kernel<64, 16, false>,
+                          (const void*)kv4_attn_kernel<128, 4, false>, (const void*)kv4_attn_kernel<128, 8, false>, (const void*)kv4_attn_kernel<128, 16, false>,
+                          (const void*)kv4_attn_kernel<64, 4, true>, (const void*)kv4_attn_kernel<64, 8, true>, (const void*)kv4_attn_kernel<64, 16, true>,
+                          (const void*)kv4_attn_kernel<128, 4, true>, (const void*)kv4_attn_kernel<128, 8, true>, (const void*)kv4_attn_kernel<128, 16, true>})
       if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)A4_SMEM);
     if (e != cudaSuccess) { set_error("kv4_attn: cannot get %u bytes of shared memory: %s", A4_SMEM, cudaGetErrorString(e)); return (int)e; }
     configured = true;
   }
   const dim3 grid(max_chunks, nkv * a.n_ct, rows), block(A4_WARPS * 32);
   auto go = [&](auto kernel) { launch_pdl(kernel, grid, block, A4_SMEM, stream, a); };
-  if (hd == 64) { if (columns == 4) go(kv4_attn_kernel<64, 4>); else if (columns == 8) go(kv4_attn_kernel<64, 8>); else go(kv4_attn_kernel<64, 16>); }
-  else { if (columns == 4) go(kv4_attn_kernel<128, 4>); else if (columns == 8) go(kv4_attn_kernel<128, 8>); else go(kv4_attn_kernel<128, 16>); }
+  auto pick = [&](auto beside) {
+    constexpr bool B = decltype(beside)::value;
+    if (hd == 64) { if (columns == 4) go(kv4_attn_kernel<64, 4, B>); else if (columns == 8) go(kv4_attn_kernel<64, 8, B>); else go(kv4_attn_kernel<64, 16, B>); }
+    else { if (columns == 4) go(kv4_attn_kernel<128, 4, B>); else if (columns == 8) go(kv4_attn_kernel<128, 8, B>); else go(kv4_attn_kernel<128, 16, B>); }
+  };
+  if (few > 0) pick(std::true_type()); else pick(std::false_type());
   int rc = launch_status("kv4_attn");
   if (rc || max_chunks == 1) return rc;
   const dim3 jgrid(columns < ncol ? columns : ncol, nkv * a.n_ct, rows);

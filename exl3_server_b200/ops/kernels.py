@@ -2066,52 +2066,45 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         window = 0
     group = heads // kv_heads
     pitch = heads * head_dim if plain else _pitch(q)
-    rest = (heads, kv_heads, head_dim, window, scale)
-    if tiles is None or row_start is None or max_new * group <= KV4_FEW_COLUMNS or _kv4_walks(
+    few = 0                                  # > 0: only rows of up to so many new tokens walk, as prompts do not
+    if tiles is not None and row_start is not None and max_new * group > KV4_FEW_COLUMNS and not _kv4_walks(
             rows, tiles[2], heads, kv_heads, head_dim, max_new, max_len, min(max_len, window + max_new - 1) if window > 0 else max_len):
-        return _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, max_new, max_len, *rest, 0, workspace, out)
-    for t in tiles[:2]:
-        _int32(t, "tiles", "kv4_attn")
-        if t.numel() < tiles[2]:
-            raise KernelLibraryError(f"kv4_attn: {tiles[2]} tiles, of which {t.numel()} are listed")
-    # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000 keys
-    # beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 168 us and 5 MB this way).
-    few, few_len = 0, max_len
-    if row_lens is not None:
-        most = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1)
-        short = [(n, c + n) for c, n in row_lens if 0 < n <= most]
-        if short:
-            few, few_len = max(n for n, _ in short), max(k for _, k in short)
-    elif T < rows * max_new:
-        few = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1)
-    _kv4_attn_prompt(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, tiles, max_new, max_len, *rest, few, workspace, out, row_lens)
-    if few:
-        _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, few, few_len, *rest, few, workspace, out)
-    return out
-
-
-def _kv4_scratch(floats: int, workspace, q: torch.Tensor) -> torch.Tensor:
-    return workspace.plain(floats) if workspace is not None else torch.empty(floats, dtype=torch.float32, device=q.device)
-
-
-def _kv4_attn_codes(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, max_new, max_len, heads, kv_heads, head_dim, window, scale, few,
-                    workspace, out) -> torch.Tensor:
-    """Rows of up to ``max_new`` tokens walk the codes (attention_cache4.cu); with ``few`` > 0 those of more than so many are left out."""
-    wanted = max_new * (heads // kv_heads)
+        for t in tiles[:2]:
+            _int32(t, "tiles", "kv4_attn")
+            if t.numel() < tiles[2]:
+                raise KernelLibraryError(f"kv4_attn: {tiles[2]} tiles, of which {t.numel()} are listed")
+        # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000
+        # keys beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 168 us and 5 MB this way).
+        few_len, most = max_len, min(max(1, KV4_FEW_COLUMNS // group), max_new - 1)
+        if row_lens is not None:
+            short = [(n, c + n) for c, n in row_lens if 0 < n <= most]
+            if short:
+                few, few_len = max(n for n, _ in short), max(k for _, k in short)
+        elif T < rows * max_new:
+            few = most
+        _kv4_attn_prompt(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, tiles, max_new, max_len, heads, kv_heads, head_dim, window, scale,
+                         few, workspace, out, row_lens)
+        if not few:
+            return out
+        max_new, max_len = few, few_len
+    wanted = max_new * group
     columns = 4 if wanted <= 4 else 8 if wanted <= 8 else 16
     groups = -(-wanted // columns)
-    span = min(max_len, window + max_new - 1) if window > 0 else max_len
-    chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, max(1, span), window, _sms(q))
+    chunk, chunks = _kv4_chunks(rows, kv_heads, groups, columns, head_dim, (min(max_len, window + max_new - 1) if window > 0 else max_len) or 1, window, _sms(q))
     need, scratch = 0, None
     if chunks > 1:
         need = rows * kv_heads * groups * chunks * columns * (head_dim + 4)
         scratch = _kv4_scratch(need, workspace, q)
     rc = _entry("exl3_kv4_attn", "plpplpiippiiiiiiifiiipl")(
         _addr(q), pitch, _addr(out), _addr(pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], _addr(row_start),
-        _addr(row_pos0), rows, q.shape[0], max_new, heads, kv_heads, head_dim, window, scale, few, chunk, chunks, _addr(scratch), need, _raw_stream())
+        _addr(row_pos0), rows, T, max_new, heads, kv_heads, head_dim, window, scale, few, chunk, chunks, _addr(scratch), need, _raw_stream())
     if rc:
         _check(rc, "kv4_attn")
     return out
+
+
+def _kv4_scratch(floats: int, workspace, q: torch.Tensor) -> torch.Tensor:
+    return workspace.plain(floats) if workspace is not None else torch.empty(floats, dtype=torch.float32, device=q.device)
 
 
 def kv4_prompt_status() -> int:
