@@ -265,7 +265,13 @@ struct FaTile {
   int kept;        // pages from the sequence's start that are walked before it (kept first keys)
   int n_pages;     // pages to walk
   const int* bt;   // the sequence's page table
-  int mask_from;   // pages that reach beyond this position are masked: p_first, or (fp16) FA_HOLES where some page has to be hidden as a whole
+#ifdef EXL3_PREFILL_F16
+  int from;        // FA_HOLES where some page has to be hidden as a whole, else p_first
+  // pages that reach beyond this position are masked
+  __device__ inline int mask_from() const { return from; }
+#else
+  __device__ inline int mask_from() const { return p_first; }
+#endif
 };
 constexpr int FA_HOLES = INT32_MIN;
 __device__ inline FaRow fa_row(const FaOpts& opts, int b) {
@@ -321,7 +327,9 @@ __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride
   t.n_pages = t.kept + t.p_last / FA_BK - t.page_lo + 1;
   if (FA_F16) t.n_pages = max(t.n_pages, 1);              // (queries before position 0: one page, hidden from all)
   t.bt = block_table + (int64_t)b * bt_stride;
-  t.mask_from = FA_F16 && fa_has_holes(opts, b) ? FA_HOLES : t.p_first;
+#ifdef EXL3_PREFILL_F16
+  t.from = fa_has_holes(opts, b) ? FA_HOLES : t.p_first;
+#endif
   return t;
 }
 
@@ -698,7 +706,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       const bool p_free = f < 2 || fa_mbar_test(pv_done + st, ((f - 2) >> 1) & 1);
       const bool s_there = j + 1 < n_blocks && fa_mbar_test(s_full + (st ^ 1), ((f + 1) >> 1) & 1);
       const int key0 = (j < kept ? j : page_lo + j - kept) * FA_BK;
-      fa_adjust(sr, opts, head, key0, p, tw.mask_from, p_last, p_first + warp * 32, window, chunk, [&] { return missing(w, key0); });
+      fa_adjust(sr, opts, head, key0, p, tw.mask_from(), p_last, p_first + warp * 32, window, chunk, [&] { return missing(w, key0); });
       const float mx = fa_row_max(sr) * score_mul;           // scale > 0: max and scale commute
       // lazy rescale: move the reference maximum only when it is far behind
       const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
@@ -1171,7 +1179,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         // looked at early: see the kernel above
         const bool s_there = j + 1 < n_pages && fa_mbar_test(s_full + 2 * s + (sb ^ 1), ((f + 1) >> 1) & 1);
         const int key0 = (j < t.kept ? j : t.page_lo + j - t.kept) * FA_BK;
-        fa_adjust(sr, opts, head, key0, p, t.mask_from, t.p_last, t.p_first + q * 32, window, chunk, [&] {
+        fa_adjust(sr, opts, head, key0, p, t.mask_from(), t.p_last, t.p_first + q * 32, window, chunk, [&] {
           const int b = seq_of(item);
           return fa_page(block_table + (int64_t)b * bt_stride, fa_row(opts, b), opts, key0 / FA_BK) < 0;
         });

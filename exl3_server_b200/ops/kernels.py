@@ -2075,15 +2075,22 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
                 raise KernelLibraryError(f"kv4_attn: {tiles[2]} tiles, of which {t.numel()} are listed")
         # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000
         # keys beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 168 us and 5 MB this way).
-        few_len, most = max_len, min(max(1, KV4_FEW_COLUMNS // group), max_new - 1)
+        most, width = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1), block_table.shape[1]
         if row_lens is not None:
-            short = [(n, c + n) for c, n in row_lens if 0 < n <= most]
-            if short:
-                few, few_len = max(n for n, _ in short), max(k for _, k in short)
-        elif T < rows * max_new:
-            few = most
-        _kv4_attn_prompt(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, tiles, max_new, max_len, heads, kv_heads, head_dim, window, scale,
-                         few, workspace, out, row_lens)
+            few, few_len, row_pages, total = _kv4_rows(tuple(map(tuple, row_lens)), most, window, width)
+        else:
+            few, few_len, row_pages = most if T < rows * max_new else 0, max_len, min(width, -(-max_len // KV4_PAGE))
+            if window:
+                row_pages = min(row_pages, (window + max_new - 2) // KV4_PAGE + 2)
+            total = max(1, min(rows, T // (few + 1))) * row_pages
+        slots, stride, passes, room = _kv4_passes(T, rows, max(1, row_pages), max(1, total), tiles[2], heads, kv_heads, head_dim, KV4_PROMPT_BYTES)
+        scratch = _kv4_scratch(room // 4, workspace, q)
+        rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifiiiiiipl")(
+            _addr(q), pitch, T, _addr(out), _addr(pool), pages, _addr(block_table), block_table.stride(0), rows, width, _addr(row_start), _addr(row_pos0),
+            _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, few, max(1, row_pages), max(1, total), slots, stride, passes,
+            _addr(scratch), room, _raw_stream())
+        if rc:
+            _check(rc, "kv4_attn")
         if not few:
             return out
         max_new, max_len = few, few_len
@@ -2114,14 +2121,17 @@ def kv4_prompt_status() -> int:
 KV4_PROMPT_BYTES = 512 << 20      # scratch for fp16 copies of pages that a prompt step takes beyond what two of its longest rows need
 
 
-def _kv4_passes(row_pages: int, total: int, page_bytes: int) -> tuple:
-    """``(slots, stride, passes)`` for rows of up to ``row_pages`` pages each and ``total`` together: all at once where that fits into
-    ``KV4_PROMPT_BYTES`` (or two of the longest rows), else rows in turn: a row begins in the pass (pages before it) // stride."""
-    most = max(2 * row_pages, KV4_PROMPT_BYTES // page_bytes)
-    if total <= most:
-        return total, 1 << 30, 1
-    stride = most - row_pages + 1
-    return most, stride, (total - 1) // stride + 1
+@functools.lru_cache(maxsize=256)
+def _kv4_passes(T: int, rows: int, row_pages: int, total: int, n_tiles: int, heads: int, kv_heads: int, head_dim: int, most_bytes: int) -> tuple:
+    """``(slots, stride, passes, bytes of scratch)`` of the prompt form for rows of up to ``row_pages`` pages each and ``total`` together: all at once where
+    their copies fit into ``most_bytes`` (or two of the longest rows), else rows in turn: a row begins in the pass (pages before it) // stride."""
+    most = max(2 * row_pages, most_bytes // (4 * kv_heads * KV4_PAGE * head_dim))
+    slots, stride, passes = total, 1 << 30, 1
+    if total > most:
+        slots, stride = most, most - row_pages + 1
+        passes = (total - 1) // stride + 1
+    need = _long_entry("exl3_kv4_prompt_scratch", 10)(T, rows, row_pages, total, slots, passes, n_tiles, heads, kv_heads, head_dim)
+    return slots, stride, passes, need
 
 
 def _kv4_row_pages(ctx: int, new: int, window: int, width: int) -> int:
@@ -2130,29 +2140,14 @@ def _kv4_row_pages(ctx: int, new: int, window: int, width: int) -> int:
     return max(0, min(-(-(ctx + new) // KV4_PAGE), width) - lo) if new > 0 else 0
 
 
-def _kv4_attn_prompt(q, pitch, pool, pages, block_table, row_start, row_pos0, rows, tiles, max_new, max_len, heads, kv_heads, head_dim, window, scale, few,
-                     workspace, out, row_lens) -> None:
-    """Rows of more than ``few`` tokens: their pages and the queries in fp16 in scratch memory, and the tcgen05 attention over them
-    (attention_prefill_f16.cu)."""
-    T, width = q.shape[0], block_table.shape[1]
-    if row_lens is not None:
-        sizes = [_kv4_row_pages(c, n, window, width) for c, n in row_lens if n > few] or [1]
-        row_pages, total = max(sizes), sum(sizes)
-    else:
-        row_pages = min(width, -(-max_len // KV4_PAGE))
-        if window:
-            row_pages = min(row_pages, (window + max_new - 2) // KV4_PAGE + 2)
-        total = max(1, min(rows, T // (few + 1))) * row_pages
-    row_pages, total = max(1, row_pages), max(1, total)
-    slots, stride, passes = _kv4_passes(row_pages, total, 4 * kv_heads * KV4_PAGE * head_dim)
-    need = _long_entry("exl3_kv4_prompt_scratch", 10)(T, rows, row_pages, total, slots, passes, tiles[2], heads, kv_heads, head_dim)
-    scratch = _kv4_scratch(need // 4, workspace, q)
-    rc = _entry("exl3_kv4_prompt", "plipplpiiippppiiiiifiiiiiipl")(
-        _addr(q), pitch, T, _addr(out), _addr(pool), pages, _addr(block_table), block_table.stride(0), rows, width, _addr(row_start), _addr(row_pos0),
-        _addr(tiles[0]), _addr(tiles[1]), tiles[2], heads, kv_heads, head_dim, window, scale, few, row_pages, total, slots, stride, passes,
-        _addr(scratch), need, _raw_stream())
-    if rc:
-        _check(rc, "kv4_attn")
+@functools.lru_cache(maxsize=64)
+def _kv4_rows(row_lens: tuple, most: int, window: int, width: int) -> tuple:
+    """Of a step with prompts: the most tokens of a row of up to ``most`` (0: no such row) and the most keys of one, and the pages that the
+    other rows see, of one at most and together.  (Every layer of a step asks.)"""
+    short = [(n, c + n) for c, n in row_lens if 0 < n <= most]
+    few, few_len = (max(n for n, _ in short), max(k for _, k in short)) if short else (0, 0)
+    sizes = [_kv4_row_pages(c, n, window, width) for c, n in row_lens if n > few] or [1]
+    return few, few_len, max(sizes), sum(sizes)
 
 
 # ---- products in 8-bit floating point (fp8.cuh) ---------------------------------------------------------------

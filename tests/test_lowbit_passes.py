@@ -7,13 +7,17 @@ from exl3_server_b200.engine.batch import Workspace, pack_step
 from exl3_server_b200.ops import kernels as K
 
 
+def plan(row_pages, total, page_bytes):
+    return K._kv4_passes(1, 1, row_pages, total, 1, 1, 1, page_bytes // 256, K.KV4_PROMPT_BYTES)[:3]
+
+
 @pytest.mark.parametrize("seed", range(40))
 def test_every_pass_holds_its_rows(seed):
     rng = random.Random(seed)
     page_bytes = 4 * 64 * rng.choice([64, 128]) * rng.choice([1, 8, 36])
     pages = [rng.choice([0, 1, 4, rng.randint(1, 600)]) for _ in range(rng.randint(1, 200))]
     row_pages, total = max(1, max(pages)), max(1, sum(pages))
-    slots, stride, passes = K._kv4_passes(row_pages, total, page_bytes)
+    slots, stride, passes = plan(row_pages, total, page_bytes)
     used, before = {}, 0
     for n in pages:
         p = min(before // stride, passes - 1)
@@ -32,10 +36,10 @@ def test_scratch_of_one_long_prompt_among_short_ones():
     lens = [(0, 32768)] + [(0, 200)] * 63
     sizes = [K._kv4_row_pages(c, n, 0, 512) for c, n in lens]
     page_bytes = 4 * 36 * 64 * 64
-    slots, _, passes = K._kv4_passes(max(sizes), sum(sizes), page_bytes)
+    slots, _, passes = plan(max(sizes), sum(sizes), page_bytes)
     assert passes == 1 and slots == 512 + 63 * 4 and slots * page_bytes < 0.46e9
     many = [512] * 64
-    slots, _, passes = K._kv4_passes(512, sum(many), page_bytes)
+    slots, _, passes = plan(512, sum(many), page_bytes)
     assert passes > 1 and slots * page_bytes <= max(K.KV4_PROMPT_BYTES, 2 * 512 * page_bytes)
 
 
