@@ -286,7 +286,7 @@ class Rig:
         say(f"{name}: {self.layers} layers, cache of {cache_tokens} tokens, ready in {time.time() - t0:.1f}s")
         return self
 
-    def __init__(self, sizes_name: str, layers: int, cache_tokens: int, max_slots: int):
+    def __init__(self, sizes_name: str, layers: int, cache_tokens: int, max_slots: int, weight_type=None, cache_type=None):
         import torch
         import exl3_server_b200 as E
         from exl3_server_b200.config.presets import SIZES, sizes
@@ -305,7 +305,7 @@ class Rig:
         plan = build_plan(self.cfg)
         tensors = dict(random_tensors(plan_manifest(plan), seed=0, std=0.02, norm_std=None, dtype=torch.bfloat16,
                                       device=dev))
-        self.model = Model(plan, tensors, torch.bfloat16, dev)
+        self.model = Model(plan, tensors, torch.bfloat16, dev, weight_type=weight_type, cache_type=cache_type)
         del tensors
         self.engine = E.Engine(self.model, max_tokens=cache_tokens, max_slots=max_slots)
         self.gen = torch.Generator().manual_seed(1)
@@ -515,6 +515,8 @@ def main() -> int:
                     help="layer sizes; other than the default only with --only (a short JSON line)")
     ap.add_argument("--only", choices=["all", "decode", "prefill", "unequal", "designs"], default="all",
                     help="run one part only (for profiling small cases); prints a short JSON line")
+    ap.add_argument("--weight-type", choices=["fp8"], default=None, help="with --only decode, prefill or unequal: the layers' matrices in 8 bits")
+    ap.add_argument("--cache-type", choices=["int4"], default=None, help="with --only decode, prefill or unequal: keys and values in 4 bits")
     ap.add_argument("--design-sizes", choices=sorted(DESIGN_SIZES), default=None,
                     help="with --only designs: one size pair instead of all")
     ap.add_argument("--design-arch", choices=["both", "soporax", "tunavik", "potodra", "nibelix", "nikodra", "rigitar", "llama"], default="both",
@@ -530,6 +532,9 @@ def main() -> int:
         return 0
     if args.gpus != 1:
         print(f"bench.py: this library runs on one GPU; --gpus {args.gpus} is not supported")
+        return 2
+    if (args.weight_type or args.cache_type) and args.only not in ("decode", "prefill", "unequal"):
+        print("bench.py: --weight-type and --cache-type need --only decode, prefill or unequal")
         return 2
     if args.only == "designs":
         return designs(args)
@@ -548,28 +553,29 @@ def main() -> int:
     def room(batch, ctx):
         return (batch + 1) * ((ctx + page - 1) // page * page + page)
 
+    types = dict(weight_type=args.weight_type, cache_type=args.cache_type)
     # ---- one part only -----------------------------------------------------------------------------------------
     if args.only == "decode":
-        rig = Rig(args.sizes, args.layers, room(B, C), B + 1)
+        rig = Rig(args.sizes, args.layers, room(B, C), B + 1, **types)
         ms, launches, kv = rig.decode(B, C, Kst, W)
         gbs = (rig.model.weight_bytes() + kv) / (ms / Kst / 1e3) / 1e9
-        print(json.dumps({"only": "decode", "sizes": args.sizes, "batch": B, "context": C, "layers": rig.layers,
+        print(json.dumps({"only": "decode", "sizes": args.sizes, **types, "batch": B, "context": C, "layers": rig.layers,
                           "ms_per_step": ms / Kst, "tok_s": B * Kst / (ms / 1e3), "gb_s": gbs,
                           "hbm_frac": gbs / hbm_gbs, "gpu_launches": int(launches)}))
         return 0
     if args.only == "prefill":
-        rig = Rig(args.sizes, args.layers, room(1, args.prefill_tokens), 2)
+        rig = Rig(args.sizes, args.layers, room(1, args.prefill_tokens), 2, **types)
         ms = rig.prefill(args.prefill_tokens, repeats=max(1, Kst // 16))
         tf = rig.prefill_flops([args.prefill_tokens]) / (ms / 1e3) / 1e12
-        print(json.dumps({"only": "prefill", "sizes": args.sizes, "tokens": args.prefill_tokens, "layers": rig.layers,
+        print(json.dumps({"only": "prefill", "sizes": args.sizes, **types, "tokens": args.prefill_tokens, "layers": rig.layers,
                           "ms": ms, "tok_s": args.prefill_tokens / (ms / 1e3), "tflops": tf, "frac": tf / bf16_tf}))
         return 0
     if args.only == "unequal":
-        rig = Rig(args.sizes, args.layers, room(64, 2048 + 256 + 16), 65)
+        rig = Rig(args.sizes, args.layers, room(64, 2048 + 256 + 16), 65, **types)
         lens, pf, dec, kv = rig.unequal(64, 16, 2048, 256)
         tf = rig.prefill_flops(lens) / (pf / 1e3) / 1e12
         gbs = (rig.model.weight_bytes() + kv) / (dec / 1e3) / 1e9
-        print(json.dumps({"only": "unequal", "sizes": args.sizes, "prompts": 64, "tokens": sum(lens),
+        print(json.dumps({"only": "unequal", "sizes": args.sizes, **types, "prompts": 64, "tokens": sum(lens),
                           "layers": rig.layers, "prefill_ms": pf, "prefill_tok_s": sum(lens) / (pf / 1e3),
                           "prefill_tflops": tf, "prefill_frac": tf / bf16_tf, "decode_ms_per_step": dec,
                           "decode_tok_s": 64 / (dec / 1e3), "decode_gb_s": gbs, "decode_hbm_frac": gbs / hbm_gbs}))
