@@ -27,8 +27,9 @@
 //
 // Measured: 8 rows of 4,096 keys, 36 heads of 64 with keys of their own 28.8 us (94 MB, 3.3 TB/s); 64 rows of 130 to 8,000 keys, 32 heads of 128 on 8
 // 79.9 us (339 MB, 4.2 TB/s); one row of 131,071 keys of these 38.4 us (168 MB, 4.4 TB/s); one row of 128 keys, 16 heads of 64 on 2 3.9 us.
-// What bounds it is the instructions of a tile, some 650 for a warp, half of them integer ones (masks, byte permutes, minima and maxima) that a
-// scheduler takes every second cycle; more warps an SM, more stages of the ring or larger chunks change nothing.  What brought it here, for
+// No unit is full (64 rows: issue slots 0.63, ALU 0.53, tensor pipe 0.22, memory 0.65 of the copy rate, 14 warps an SM): a tile is some 650 instructions for a warp,
+// half of them integer ones (masks, byte permutes, minima and maxima), in phases that wait for one another (scores, one vote, exponentials, transposes,
+// products), and more warps an SM, more stages of the ring or larger chunks change nothing; two tiles at work at once in a warp were not tried.  What brought it here, for
 // the 64 rows: 127 us with every group's numbers multiplied in first, 98 with keys as e4m3, 87 with F in the reference, 81 with whole tiles
 // first, one vote a tile on the reference and two groups to an operand.  A block's beginning and end are some 4 us that few blocks an SM do not hide, hence the page numbers beside
 // the lengths (and chunks no smaller than a wave wants).  A join by a cluster through distributed shared memory takes 1 us less

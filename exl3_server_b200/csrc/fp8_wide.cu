@@ -7,7 +7,8 @@
 // What bounds such a kernel is therefore the way round: product, signal, tensor memory to registers, signal, next product.  It is kept
 // short: eight warps read an accumulator (lane = row, 128 float32 sums a thread, one sw a block of K), 64 columns at a time, the next ones on their way
 // while the last are added up (packed fma), and give it back before they have added up its end; waits suspend in hardware; the copies and the
-// products are issued by one thread each from end to end.  2,048 x 28,672, K 4,096 with the gate 228 us (2.1 PFLOP/s); what was measured on the
+// products are issued by one thread each from end to end.  2,048 x 28,672, K 4,096 with the gate 231 us in a short run (2.1 PFLOP/s) and 275 in a long one, which
+// meets the power cap (1.75; what follows is of short runs); what was measured on the
 // way: pairs of SMs on one tile 349 (a third less from L2, but the signals cross between SMs), two accumulators of 128 x 128 per block of K
 // 288 (the instruction reads x's rows again), without the sums 179, copies alone 125.
 //

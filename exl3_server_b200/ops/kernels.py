@@ -2074,7 +2074,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
             if t.numel() < tiles[2]:
                 raise KernelLibraryError(f"kv4_attn: {tiles[2]} tiles, of which {t.numel()} are listed")
         # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000
-        # keys beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 168 us and 5 MB this way).
+        # keys beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 154 us and 5 MB this way).
         most, width = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1), block_table.shape[1]
         if row_lens is not None:
             few, few_len, row_pages, total = _kv4_rows(tuple(map(tuple, row_lens)), most, window, width)
