@@ -25,7 +25,7 @@ static long long kv4_up16(long long n) { return (n + 15) / 16 * 16; }
 // and values by parts, and what undoes their factors.
 extern "C" long long exl3_kv4_prompt_scratch(int T, int rows, int row_pages, int total, int slots, int passes, int n_tiles, int nh, int nkv, int hd) {
   return 2 * (long long)slots * nkv * 64 * hd * 2 + kv4_up16((long long)T * nh * hd * 2) + kv4_up16((long long)T * nh * 4) + 16ll * rows +
-         16ll * passes + 16ll * total + kv4_up16(4ll * rows) + 2 * kv4_up16(4ll * n_tiles) + kv4_up16(8ll * rows * nkv) +
+         16ll * passes + 16ll * total + kv4_up16(4ll * rows) + 16ll * n_tiles + kv4_up16(8ll * rows * nkv) +
          kv4_up16(8ll * rows * nkv * c4_prompt_parts(row_pages));
 }
 
@@ -55,7 +55,7 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
   a.pool = static_cast<const unsigned char*>(pool); a.n_pages = (int)n_pages; a.nkv = nkv;
   a.block_table = block_table; a.bt_stride = bt_stride; a.width = width; a.rows = rows;
   a.row_start = row_start; a.row_pos0 = row_pos0; a.window = window; a.few = few; a.parts = c4_prompt_parts(row_pages);
-  a.tile_seq = tile_seq; a.tile_q0 = tile_q0; a.n_tiles = n_tiles;
+  a.tile_seq = tile_seq; a.tile_q0 = tile_q0; a.n_tiles = n_tiles; a.tile_queries = FA_BQ;
   a.row_pages = row_pages; a.total = total; a.stride = stride; a.passes = passes;
   a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.T = T; a.nh = nh;
   a.q_sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;        // (the attention takes positive scales)
@@ -67,17 +67,16 @@ extern "C" int exl3_kv4_prompt(const void* q, int64_t q_stride, int T, void* out
   a.pass = reinterpret_cast<PromptPass*>(take(16ll * passes));
   a.slot = reinterpret_cast<int4*>(take(16ll * total));
   a.pass_of = reinterpret_cast<int*>(take(4ll * rows));
-  a.seq_out = reinterpret_cast<int*>(take(4ll * n_tiles));
-  a.q0_out = reinterpret_cast<int*>(take(4ll * n_tiles));
+  a.tile = reinterpret_cast<PromptTile*>(take(16ll * n_tiles));
   a.undo = reinterpret_cast<float2*>(take(8ll * rows * nkv));
   a.tops = reinterpret_cast<float2*>(at);
   int rc = c4_prompt_plan(a, hd, stream);
   for (int p = 0; p < passes && !rc; ++p) {
     rc = c4_prompt_copies(a, hd, p, slots, stream);
     if (!rc)
-      rc = fa_run(a.q_out, (int64_t)nh * hd, T, out, a.k_out, a.v_out, (int64_t)slots * nkv * 64, block_table, bt_stride, row_start, row_pos0, a.seq_out,
-                  a.q0_out, n_tiles, nh, nkv, hd, 64, window, 0, 0, scale != 0.0f ? fabsf(scale) : 1.0f, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr,
-                  FaCopies{a.q_scale, a.undo, a.own, a.pass + p, passes == 1, (int)n_pages}, stream);
+      rc = fa_run(a.q_out, (int64_t)nh * hd, T, out, a.k_out, a.v_out, (int64_t)slots * nkv * 64, block_table, bt_stride, row_start, row_pos0, tile_seq,
+                  tile_q0, n_tiles, nh, nkv, hd, 64, window, 0, 0, scale != 0.0f ? fabsf(scale) : 1.0f, 0, 0, 0.0f, nullptr, nullptr, 0, nullptr,
+                  FaCopies{a.q_scale, a.undo, a.own, a.pass + p, a.tile, passes == 1, (int)n_pages}, stream);
   }
   return rc;
 }

@@ -49,18 +49,17 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <math.h>
+#include <type_traits>
 #ifdef EXL3_PREFILL_F16
 #include "cache4_rows.cuh"
 #else
-namespace exl3 { struct FaRow {}; struct PromptPass {}; }
+namespace exl3 { struct FaRow {}; struct PromptPass {}; struct PromptTile {}; }
 #endif
 
 #ifdef EXL3_PREFILL_F16
 #define EXL3_FA_NS prefill_f16
-#define EXL3_FA_LIST const int*                   // lists of tiles: a kernel's work here,
 #else
 #define EXL3_FA_NS prefill_bf16
-#define EXL3_FA_LIST const int* __restrict__      // the host's there
 #endif
 
 namespace exl3 {
@@ -214,8 +213,9 @@ struct FaCopies {
   const float* q_scale;        // what the scores of a (token, query head) are multiplied by beside the scale
   const float2* undo;          // per (row, kv head): what its products with keys (scores) and with values are multiplied by
   const FaRow* own;            // where the copies of the rows' pages are
-  const PromptPass* pass;      // the tiles of this launch, which
-  bool first;                  // begin the lists (known ahead of the pass where there is but one)
+  const PromptPass* pass;      // the part of the tiles that is this launch's; the host knows an upper bound of how many they are
+  const PromptTile* tiles;     // instead of the lists tile_seq and tile_q0
+  bool first;                  // that part begins the tiles (known ahead of the pass where there is but one)
   int table_pages;             // pages of the pool that the block table speaks of
 };
 // What a block needs to know of a tile of 128 queries.
@@ -234,11 +234,19 @@ struct FaOpts {
   const float* gate;           // a factor per (token, query head) on the output; null: none
   FaCopies copies;
 };
-// What the scores of row `row` of q, of the sequence b, are multiplied by (base-2 units); a positive number, so that a hidden score stays -inf.
-__device__ inline float fa_score_mul(const FaOpts& opts, float scale_log2, int64_t row, bool there, int nh, int head, int b, int nkv) {
+// fp16: what undoes the factors of a sequence's copies, asked for at a tile's start: what its end needs must not be a trip to memory there.
+__device__ inline float2 fa_undo(const FaOpts& opts, int b, int nkv, int g) {
+#ifdef EXL3_PREFILL_F16
+  return __ldcg(opts.copies.undo + (int64_t)b * nkv + g);
+#else
+  return {};
+#endif
+}
+// What the scores of row `row` of q are multiplied by (base-2 units); with fp16 a positive number, so that a hidden score stays -inf.
+__device__ inline float fa_score_mul(const FaOpts& opts, float scale_log2, int64_t row, bool there, int nh, int head, float2 undo) {
   const float mul = opts.cap_in > 0.0f ? opts.cap_log2 : scale_log2;
   if (!FA_F16) return mul;
-  const float f = there ? __ldcg(opts.copies.q_scale + row * nh + head) * __ldcg(opts.copies.undo + (int64_t)b * nkv + head / (nh / nkv)).x : 1.0f;
+  const float f = there ? __ldcg(opts.copies.q_scale + row * nh + head) * undo.x : 1.0f;
   return fminf(fmaxf(mul * f, 1.1754944e-38f), 3.4028235e38f);
 }
 // Whether a page of keys from key0 on holds a key with a bias for one of a warp's 32 queries from position p0 on.
@@ -266,14 +274,15 @@ struct FaTile {
   int n_pages;     // pages to walk
   const int* bt;   // the sequence's page table
 #ifdef EXL3_PREFILL_F16
-  int from;        // FA_HOLES where some page has to be hidden as a whole, else p_first
-  // pages that reach beyond this position are masked
-  __device__ inline int mask_from() const { return from; }
+  int b;           // the sequence
+  int some;        // whether some page has to be hidden as a whole
+  __device__ inline bool holes() const { return some != 0; }
+  __device__ inline int sequence() const { return b; }
 #else
-  __device__ inline int mask_from() const { return p_first; }
+  __device__ inline bool holes() const { return false; }
+  __device__ inline int sequence() const { return 0; }
 #endif
 };
-constexpr int FA_HOLES = INT32_MIN;
 __device__ inline FaRow fa_row(const FaOpts& opts, int b) {
 #ifdef EXL3_PREFILL_F16
   const int4 w = __ldcg(reinterpret_cast<const int4*>(opts.copies.own + b));
@@ -282,17 +291,29 @@ __device__ inline FaRow fa_row(const FaOpts& opts, int b) {
   return {};
 #endif
 }
-// fp16: the tiles of this launch, of which the host knows an upper bound only: moves the lists to their place and returns how many there are.
-template <typename List> __device__ inline int fa_tiles(const FaOpts& opts, int n_tiles, List& tile_seq, List& tile_q0) {
+// fp16: how many tiles this launch has, and where they begin (else all that the host lists).
+__device__ inline int fa_tiles(const FaOpts& opts, int n_tiles, int& tile0) {
 #ifdef EXL3_PREFILL_F16
   const int2 w = __ldcg(reinterpret_cast<const int2*>(&opts.copies.pass->tile0));
-  if (!opts.copies.first) {
-    tile_seq += w.x;
-    tile_q0 += w.x;
-  }
+  tile0 = opts.copies.first ? 0 : w.x;
   return w.y;
 #else
   return n_tiles;
+#endif
+}
+// fp16: a tile's sequence, first row, queries and first position (another kernel's work: through L2 only, see load_vec_cg).
+__device__ inline int4 fa_listed(const FaOpts& opts, int tile) {
+#ifdef EXL3_PREFILL_F16
+  return __ldcg(reinterpret_cast<const int4*>(opts.copies.tiles + tile));
+#else
+  return {};
+#endif
+}
+__device__ inline int fa_listed_sequence(const FaOpts& opts, int tile) {
+#ifdef EXL3_PREFILL_F16
+  return __ldcg(&opts.copies.tiles[tile].b);
+#else
+  return 0;
 #endif
 }
 __device__ inline bool fa_has_holes(const FaOpts& opts, int b) {
@@ -314,11 +335,19 @@ __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride
                                  const int* row_pos0, const int* tile_seq, const int* tile_q0, int window,
                                  int chunk, const FaOpts& opts) {
   FaTile t;
+#ifdef EXL3_PREFILL_F16
+  const int4 w = fa_listed(opts, tile);
+  const int b = w.x;
+  t.row0 = w.y;
+  t.rows = w.z;
+  t.p_first = w.w;
+#else
   const int b = tile_seq[tile], q0 = tile_q0[tile];
   const int n_new = row_start[b + 1] - row_start[b];
   t.row0 = row_start[b] + q0;
   t.rows = min(FA_BQ, n_new - q0);
   t.p_first = row_pos0[b] + q0;
+#endif
   t.p_last = t.p_first + t.rows - 1;
   int k_lo = (window > 0 && t.p_first - window + 1 > 0) ? t.p_first - window + 1 : 0;
   if (!FA_F16 && chunk > 0) k_lo = max(k_lo, t.p_first / chunk * chunk);    // the block of positions of the tile's first query
@@ -328,19 +357,27 @@ __device__ inline FaTile fa_tile(int tile, const int* block_table, int bt_stride
   if (FA_F16) t.n_pages = max(t.n_pages, 1);              // (queries before position 0: one page, hidden from all)
   t.bt = block_table + (int64_t)b * bt_stride;
 #ifdef EXL3_PREFILL_F16
-  t.from = fa_has_holes(opts, b) ? FA_HOLES : t.p_first;
+  t.b = b;
+  t.some = fa_has_holes(opts, b);
 #endif
   return t;
 }
 
 // ---- a row of 64 scores (thread = query row), for all kernels below ------------------------------------------------
-// Cap, distance biases and mask (fp16: the mask alone).  p0_warp: the position of the warp's first query.  missing() says whether nobody sees this
-// page; it is asked where mask_from is FA_HOLES, and looks up all it needs: more registers in the loop over pages made it a tenth slower.
-template <typename Missing>
-__device__ inline void fa_adjust(uint32_t (&sr)[2][32], const FaOpts& opts, int head, int key0, int p, int mask_from,
+// The loop over a tile's pages, for rows with pages to hide and for others: what hiding takes, a lookup in the block table and a test, took a tenth of the
+// time where both shared one.
+template <typename Pages> __device__ inline void fa_with_holes(bool holes, Pages& pages) {
+  if (FA_F16 && holes) pages(std::true_type());
+  else pages(std::false_type());
+}
+// Cap, distance biases and mask (fp16: the mask alone).  p0_warp: the position of the warp's first query.  HOLES: missing() says whether nobody sees this
+// page.
+template <bool HOLES, typename Missing>
+__device__ inline void fa_adjust(uint32_t (&sr)[2][32], const FaOpts& opts, int head, int key0, int p, int p_first,
                                  int p_last, int p0_warp, int window, int chunk, Missing missing) {
   if (FA_F16) chunk = 0;
-  const bool need_mask = (key0 + FA_BK - 1 > mask_from) || (window > 0 && key0 <= p_last - window) ||
+  const bool hidden = FA_F16 && HOLES && missing();
+  const bool need_mask = hidden || (key0 + FA_BK - 1 > p_first) || (window > 0 && key0 <= p_last - window) ||
                          (chunk > 0 && key0 < p_last / chunk * chunk);
   if (!FA_F16 && opts.cap_in > 0.0f) {                       // capped scores: tanh now, the cap with the scale below
 #pragma unroll
@@ -360,7 +397,7 @@ __device__ inline void fa_adjust(uint32_t (&sr)[2][32], const FaOpts& opts, int 
   if (need_mask) {                                           // without branches: one test per page decides about the page
     int lo_key = (window > 0) ? p - window : -1;             // keys <= lo_key are out of the window
     if (chunk > 0) lo_key = max(lo_key, p / chunk * chunk - 1);   // or before the query's block of positions
-    const int hi_key = FA_F16 && mask_from == FA_HOLES && missing() ? -1 : p;
+    const int hi_key = hidden ? -1 : p;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -454,8 +491,8 @@ __device__ inline void fa_rescale_slowly(uint32_t taddr, float corr) {
 }
 // What a row of O is multiplied by at the end.  A sink is a key of score 0 without a value: one more term in the sum, in
 // the units of the reference maximum.
-__device__ inline float fa_inverse(float l_run, float m_used, int sink, const FaOpts& opts, int head, int row, int nh, bool in, int b, int nkv) {
-  if (FA_F16) return l_run == 0.0f ? 0.0f : __ldcg(opts.copies.undo + (int64_t)b * nkv + head / (nh / nkv)).y / l_run;      // (0: a query that sees nothing)
+__device__ inline float fa_inverse(float l_run, float m_used, int sink, const FaOpts& opts, int head, int row, int nh, bool in, float2 undo) {
+  if (FA_F16) return l_run == 0.0f ? 0.0f : undo.y / l_run;  // (0: a query that sees nothing)
   float inv = 1.0f / (sink ? l_run + fa_exp2((opts.sink_vals ? __ldg(opts.sink_vals + head) * 1.4426950408889634f : 0.0f) - m_used) : l_run);
   if (opts.gate && in) inv *= __ldcg(opts.gate + (int64_t)row * nh + head);
   return inv;
@@ -492,8 +529,8 @@ __global__ void __launch_bounds__(FA_THREADS_MAIN, FA_HD == 64 ? 2 : 1)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out,
                        const int* __restrict__ block_table, int bt_stride, const int* __restrict__ row_start,
-                       const int* __restrict__ row_pos0, EXL3_FA_LIST tile_seq,
-                       EXL3_FA_LIST tile_q0, int n_tiles, int fold, int nh, int nkv, int window,
+                       const int* __restrict__ row_pos0, const int* __restrict__ tile_seq,
+                       const int* __restrict__ tile_q0, int n_tiles, int fold, int nh, int nkv, int window,
                        int chunk, int sink, float scale_log2, FaOpts opts) {
   extern __shared__ unsigned char fa_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fa_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -519,10 +556,11 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const int g = head / (nh / nkv);
   int other = n_tiles - 1 - (int)blockIdx.y;
   int n_own = (fold && other > (int)blockIdx.y) ? 2 : 1;
+  int tile0 = 0;                                    // fp16
   auto tile_of = [&](int w) {                       // the block's first (w = 0) or second tile
-    return fa_tile(w ? other : (int)blockIdx.y, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
+    return fa_tile((FA_F16 ? tile0 : 0) + (w ? other : (int)blockIdx.y), block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
   };
-  auto seq_of = [&](int w) { return !FA_F16 ? 0 : __ldcg(tile_seq + (w ? other : (int)blockIdx.y)); };
+  auto seq_of = [&](int w) { return fa_listed_sequence(opts, tile0 + (w ? other : (int)blockIdx.y)); };
   auto missing = [&](int w, int key0) {             // fp16: whether a page of that tile's sequence is not there
     const int b = seq_of(w);
     return fa_page(block_table + (int64_t)b * bt_stride, fa_row(opts, b), opts, key0 / FA_BK) < 0;
@@ -555,7 +593,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   pdl_trigger();
   pdl_wait();
   if (FA_F16) {
-    other = fa_tiles(opts, n_tiles, tile_seq, tile_q0) - 1 - (int)blockIdx.y;
+    other = fa_tiles(opts, n_tiles, tile0) - 1 - (int)blockIdx.y;
     n_own = fold ? (other > (int)blockIdx.y ? 2 : other == (int)blockIdx.y ? 1 : 0) : other >= 0 ? 1 : 0;
   }
   const uint32_t tmem_base = *tmem_slot;
@@ -573,7 +611,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // for there delayed S by more than it cost here).  Page numbers come 32 at a time, lane i holding the number of
     // page c0 + i of the block's walk, a batch ahead.
     const FaTile ta = tile_of(0), tb = n_own == 2 ? tile_of(1) : ta;
-    const FaRow owna = fa_row(opts, seq_of(0)), ownb = fa_row(opts, seq_of(n_own - 1));
+    const FaRow owna = fa_row(opts, ta.sequence()), ownb = fa_row(opts, tb.sequence());
     const int n0 = ta.n_pages;
     const int n_total = n0 + (n_own == 2 ? tb.n_pages : 0);   // the block's pages, numbered through both tiles
     if (lane == 0) {
@@ -680,7 +718,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int p_first = tw.p_first, p_last = tw.p_last, n_blocks = tw.n_pages, page_lo = tw.page_lo, rows = tw.rows;
     const int kept = tw.kept;
     const int p = p_first + r;                               // this row's position
-    const float score_mul = fa_score_mul(opts, scale_log2, tw.row0 + r, r < rows, nh, head, seq_of(w), nkv);
+    const float2 undo = fa_undo(opts, tw.sequence(), nkv, g);
+    const float score_mul = fa_score_mul(opts, scale_log2, tw.row0 + r, r < rows, nh, head, undo);
     float m_used = -INFINITY, l_run = 0.0f;
     // The row of S_f is asked for as soon as the row of P_(f-1) is on its way into tensor memory (the first of a
     // tile: here), so that the load's latency and the store's pass together.
@@ -694,6 +733,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       return true;
     };
     ok = ask_s(fb, false);
+    auto pages = [&](auto holes) {                           // (a loop of its own for rows with pages to hide: see fa_adjust)
     for (int j = 0; j < n_blocks && ok; ++j) {
       const int f = fb + j;
       const int st = f & 1;
@@ -706,7 +746,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       const bool p_free = f < 2 || fa_mbar_test(pv_done + st, ((f - 2) >> 1) & 1);
       const bool s_there = j + 1 < n_blocks && fa_mbar_test(s_full + (st ^ 1), ((f + 1) >> 1) & 1);
       const int key0 = (j < kept ? j : page_lo + j - kept) * FA_BK;
-      fa_adjust(sr, opts, head, key0, p, tw.mask_from(), p_last, p_first + warp * 32, window, chunk, [&] { return missing(w, key0); });
+      fa_adjust<decltype(holes)::value>(sr, opts, head, key0, p, p_first, p_last, p_first + warp * 32, window, chunk, [&] { return missing(w, key0); });
       const float mx = fa_row_max(sr) * score_mul;           // scale > 0: max and scale commute
       // lazy rescale: move the reference maximum only when it is far behind
       const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
@@ -733,13 +773,15 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       fa_fence_before();
       fa_mbar_arrive(p_full + st);
     }
+    };
+    fa_with_holes(tw.holes(), pages);
     if (ok) {
       // last product done -> O complete
       const int fl = fb + n_blocks - 1;
       ok = fa_mbar_wait(pv_done + (fl & 1), (fl >> 1) & 1);
       if (ok) {
         fa_fence_after();
-        const float inv = fa_inverse(l_run, m_used, sink, opts, head, tw.row0 + r, nh, r < rows, seq_of(w), nkv);
+        const float inv = fa_inverse(l_run, m_used, sink, opts, head, tw.row0 + r, nh, r < rows, undo);
         fa_store_row<FA_HD>(tmem_o + lane_addr, inv, out + ((int64_t)(tw.row0 + r) * nh + head) * FA_HD, r < rows);
         fa_fence_before();                                 // O is read: the next tile's first product may write it
       }
@@ -775,8 +817,8 @@ __global__ void __launch_bounds__(FA_THREADS, 4)
 attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out,
                         const int* __restrict__ block_table, int bt_stride, const int* __restrict__ row_start,
-                        const int* __restrict__ row_pos0, EXL3_FA_LIST tile_seq,
-                        EXL3_FA_LIST tile_q0, int nh, int nkv, int window, int chunk, int sink,
+                        const int* __restrict__ row_pos0, const int* __restrict__ tile_seq,
+                        const int* __restrict__ tile_q0, int nh, int nkv, int window, int chunk, int sink,
                         float scale_log2, FaOpts opts) {
   extern __shared__ unsigned char fa_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fa_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -795,26 +837,32 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x, tile = blockIdx.y;
-  if (FA_F16) {
-    pdl_wait();                                   // the list of tiles is the work of a kernel ahead
-    if (tile >= fa_tiles(opts, 0, tile_seq, tile_q0)) return;
-  }
+#ifdef EXL3_PREFILL_F16
+  pdl_wait();                                     // the tiles are the work of a kernel ahead
+  int tile0;
+  const int count = fa_tiles(opts, 0, tile0);
+  const int4 listed = fa_listed(opts, min(tile0 + tile, (int)gridDim.y - 1));         // (beside the count; a launch has a row of blocks for every tile)
+  if (tile >= count) return;
+  const int b = listed.x, rows = listed.z, p_first = listed.w;
+  auto row0 = [&] { return listed.y; };           // the tile's first row of q and out
+#else
   const int b = tile_seq[tile], q0 = tile_q0[tile];
   const int n_new = row_start[b + 1] - row_start[b];
   const int pos0 = row_pos0[b];
-  const int g = head / (nh / nkv);
   const int rows = min(FA_BQ, n_new - q0);
-  const int p_first = pos0 + q0, p_last = pos0 + q0 + rows - 1;
+  const int p_first = pos0 + q0;
+  auto row0 = [&] { return row_start[b] + q0; };
+#endif
+  const int g = head / (nh / nkv);
+  const int p_last = p_first + rows - 1;
   int k_lo = (window > 0 && p_first - window + 1 > 0) ? p_first - window + 1 : 0;
   if (!FA_F16 && chunk > 0) k_lo = max(k_lo, p_first / chunk * chunk);
   const int page_lo = k_lo / FA_BK, page_hi = p_last / FA_BK;
   const int kept = fa_kept_pages(window, opts.keep_first, page_lo);
   const int n_blocks = FA_F16 ? max(kept + page_hi - page_lo + 1, 1) : kept + page_hi - page_lo + 1;      // (as in fa_tile)
   const int* bt = block_table + (int64_t)b * bt_stride;
-  const int mask_from = FA_F16 && fa_has_holes(opts, b) ? FA_HOLES : p_first;
-  auto missing = [&](int key0) {                  // as in the kernel above
-    const int again = __ldcg(tile_seq + tile);
-    return fa_page(block_table + (int64_t)again * bt_stride, fa_row(opts, again), opts, key0 / FA_BK) < 0;
+  auto missing = [&](int key0) {                  // fp16: whether a page of the sequence is not there
+    return fa_page(bt, fa_row(opts, b), opts, key0 / FA_BK) < 0;
   };
 
   if (threadIdx.x == 0) {
@@ -844,7 +892,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     // ---- issuer: TMA and MMA -----------------------------------------------------------
     if (lane == 0) {
       fa_mbar_expect_tx(q_full, QB);
-      fa_tma_2d(sQ, &map_q, q_full, head * 64, row_start[b] + q0);
+      fa_tma_2d(sQ, &map_q, q_full, head * 64, row0());
     }
     auto load_kv = [&](int j) {
       const int st = j % F4_STAGES;
@@ -893,8 +941,11 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const int r = threadIdx.x;
     const int p = p_first + r;
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
-    const float score_mul = fa_score_mul(opts, scale_log2, row_start[b] + q0 + r, r < rows, nh, head, b, nkv);
+    const float2 undo = fa_undo(opts, b, nkv, g);
+    const float score_mul = fa_score_mul(opts, scale_log2, row0() + r, r < rows, nh, head, undo);
     float m_used = -INFINITY, l_run = 0.0f;
+    const bool some_missing = FA_F16 && fa_has_holes(opts, b);
+    auto pages = [&](auto holes) {
     for (int j = 0; j < n_blocks && ok; ++j) {
       if (!fa_mbar_wait(s_full, j & 1)) { ok = false; break; }
       fa_fence_after();
@@ -903,7 +954,7 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       fa_ld32(tmem_base + lane_addr + 32, sr[1]);
       fa_wait_ld();
       const int key0 = (j < kept ? j : page_lo + j - kept) * FA_BK;
-      fa_adjust(sr, opts, head, key0, p, mask_from, p_last, p_first + warp * 32, window, chunk, [&] { return missing(key0); });
+      fa_adjust<decltype(holes)::value>(sr, opts, head, key0, p, p_first, p_last, p_first + warp * 32, window, chunk, [&] { return missing(key0); });
       const float mx = fa_row_max(sr) * score_mul;
       const bool grow = mx > m_used + FA_RESCALE_STEP || (m_used == -INFINITY && mx > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
@@ -920,13 +971,15 @@ attn_prefill_tc4_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       fa_fence_before();
       fa_mbar_arrive_warp(p_full);
     }
+    };
+    fa_with_holes(some_missing, pages);
     if (ok) {
       const int jl = n_blocks - 1;
       ok = fa_mbar_wait(pv_done, jl & 1);
       if (ok) {
         fa_fence_after();
-        const float inv = fa_inverse(l_run, m_used, sink, opts, head, row_start[b] + q0 + r, nh, r < rows, FA_F16 ? __ldcg(tile_seq + tile) : 0, nkv);
-        __nv_bfloat16* dst = out + ((int64_t)(row_start[b] + q0 + r) * nh + head) * 64;
+        const float inv = fa_inverse(l_run, m_used, sink, opts, head, row0() + r, nh, r < rows, undo);
+        __nv_bfloat16* dst = out + ((int64_t)(row0() + r) * nh + head) * 64;
 #pragma unroll 1
         for (int c0 = 0; c0 < 64; c0 += 32) {
           uint32_t o[32];
@@ -987,8 +1040,8 @@ __global__ void __launch_bounds__(FP_THREADS, 1)
 attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                             const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out,
                             const int* __restrict__ block_table, int bt_stride, const int* __restrict__ row_start,
-                            const int* __restrict__ row_pos0, EXL3_FA_LIST tile_seq,
-                            EXL3_FA_LIST tile_q0, int n_tiles, int nh, int nkv, int window, int chunk, int sink,
+                            const int* __restrict__ row_pos0, const int* __restrict__ tile_seq,
+                            const int* __restrict__ tile_q0, int n_tiles, int nh, int nkv, int window, int chunk, int sink,
                             float scale_log2, FaOpts opts) {
   extern __shared__ unsigned char fa_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fa_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -1008,14 +1061,14 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_pairs = nh >> 1;
-  int n_items = n_tiles * n_pairs;
+  int n_items = n_tiles * n_pairs, tile0 = 0;     // tile0: fp16
   auto item_of = [&](int k) {                               // the block's k-th item; n_items or more: none
     return k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
   };
   auto tile_of = [&](int item) {
-    return fa_tile(item / n_pairs, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
+    return fa_tile((FA_F16 ? tile0 : 0) + item / n_pairs, block_table, bt_stride, row_start, row_pos0, tile_seq, tile_q0, window, chunk, opts);
   };
-  auto seq_of = [&](int item) { return !FA_F16 ? 0 : __ldcg(tile_seq + item / n_pairs); };
+  auto seq_of = [&](int item) { return fa_listed_sequence(opts, tile0 + item / n_pairs); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) { fa_mbar_init(q_full + i, 1); fa_mbar_init(q_free + i, 1); }
@@ -1034,7 +1087,7 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   // so far nothing was touched that another kernel writes; the next kernel in the stream may be set up meanwhile
   pdl_trigger();
   pdl_wait();
-  if (FA_F16) n_items = fa_tiles(opts, n_tiles, tile_seq, tile_q0) * n_pairs;
+  if (FA_F16) n_items = fa_tiles(opts, n_tiles, tile0) * n_pairs;
   const uint32_t tmem_base = *tmem_slot;                    // columns: S of head s at 128 s, O at 256 + 128 s
   bool ok = true;
 
@@ -1046,19 +1099,19 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     // first batch) ahead.
     int c = 0, k = 0, item = item_of(0);                    // c: pages asked for
     FaTile t = tile_of(item);
-    auto numbers = [&](const FaTile& u, int of, int j0) {
+    auto numbers = [&](const FaTile& u, int j0) {
       const int j = j0 + lane;
-      return j < u.n_pages ? fa_page(u.bt, fa_row(opts, seq_of(of)), opts, j < u.kept ? j : u.page_lo + j - u.kept) : 0;
+      return j < u.n_pages ? fa_page(u.bt, fa_row(opts, u.sequence()), opts, j < u.kept ? j : u.page_lo + j - u.kept) : 0;
     };
-    int pgs = numbers(t, item, 0);
+    int pgs = numbers(t, 0);
     while (ok) {
       const int next = item_of(k + 1);
       const FaTile tn = next < n_items ? tile_of(next) : t;
-      const int first_next = next < n_items ? numbers(tn, next, 0) : 0;
+      const int first_next = next < n_items ? numbers(tn, 0) : 0;
       const int hp = item % n_pairs, g = 2 * hp / (nh / nkv);
-      int ahead = numbers(t, item, 32);
+      int ahead = numbers(t, 32);
       for (int j = 0; j < t.n_pages; ++j, ++c) {
-        if ((j & 31) == 0 && j > 0) { pgs = ahead; ahead = numbers(t, item, j + 32); }
+        if ((j & 31) == 0 && j > 0) { pgs = ahead; ahead = numbers(t, j + 32); }
         const int st = c % FP_STAGES, pg = __shfl_sync(0xffffffffu, pgs, j & 31);
         if (c >= FP_STAGES && !fa_mbar_wait(kv_free + st, (c / FP_STAGES - 1) & 1)) { ok = false; break; }
         if (lane == 0) {
@@ -1162,7 +1215,8 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const FaTile tn = next < n_items ? tile_of(next) : t;  // asked for an item ahead
       const int head = 2 * (item % n_pairs) + s;
       const int p = t.p_first + r, n_pages = t.n_pages;
-      const float score_mul = fa_score_mul(opts, scale_log2, t.row0 + r, r < t.rows, nh, head, seq_of(item), nkv);
+      const float2 undo = fa_undo(opts, t.sequence(), nkv, head / (nh / nkv));
+      const float score_mul = fa_score_mul(opts, scale_log2, t.row0 + r, r < t.rows, nh, head, undo);
       float m_used = -INFINITY, l_run = 0.0f;
       uint32_t sr[2][32];
       auto ask_s = [&](int f, bool there) -> bool {         // there: the barrier is known to have flipped
@@ -1173,13 +1227,14 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         return true;
       };
       ok = ask_s(fb, false);
+      auto pages = [&](auto holes) {
       for (int j = 0; j < n_pages && ok; ++j) {
         const int f = fb + j, sb = f & 1;
         fa_wait_ld();
         // looked at early: see the kernel above
         const bool s_there = j + 1 < n_pages && fa_mbar_test(s_full + 2 * s + (sb ^ 1), ((f + 1) >> 1) & 1);
         const int key0 = (j < t.kept ? j : t.page_lo + j - t.kept) * FA_BK;
-        fa_adjust(sr, opts, head, key0, p, t.mask_from(), t.p_last, t.p_first + q * 32, window, chunk, [&] {
+        fa_adjust<decltype(holes)::value>(sr, opts, head, key0, p, t.p_first, t.p_last, t.p_first + q * 32, window, chunk, [&] {
           const int b = seq_of(item);
           return fa_page(block_table + (int64_t)b * bt_stride, fa_row(opts, b), opts, key0 / FA_BK) < 0;
         });
@@ -1206,13 +1261,15 @@ attn_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         fa_fence_before();
         fa_mbar_arrive_warp(p_full + 2 * s + sb);
       }
+      };
+      fa_with_holes(t.holes(), pages);
       if (ok) {
         const int fl = fb + n_pages - 1;                     // the last product done: O is complete
         ok = fa_mbar_wait(pv_done + 2 * s + (fl & 1), (fl >> 1) & 1);
         if (ok) {
           fa_fence_after();
           const bool in = r < t.rows;
-          const float inv = fa_inverse(l_run, m_used, sink, opts, head, t.row0 + r, nh, in, seq_of(item), nkv);
+          const float inv = fa_inverse(l_run, m_used, sink, opts, head, t.row0 + r, nh, in, undo);
           fa_store_row<128>(tmem_o, inv, out + ((int64_t)(t.row0 + r) * nh + head) * 128, in);
           fa_fence_before();                                 // O is read: the next item's first product may write it
         }

@@ -424,13 +424,16 @@ __device__ inline void c4_plan_tiles(const C4Prompt& a) {
     for (int t0 = 0; t0 < a.n_tiles; t0 += C4_THREADS) {
       const int t = t0 + threadIdx.x, row = t < a.n_tiles ? __ldcg(a.tile_seq + t) : -1, q0 = t < a.n_tiles ? __ldcg(a.tile_q0 + t) : 0;
       bool mine = row >= 0 && row < a.rows && (a.passes == 1 || __ldcg(a.pass_of + row) == p);
-      if (mine && a.few > 0) mine = __ldcg(a.row_start + row + 1) - __ldcg(a.row_start + row) > a.few;
+      int start = 0, n_new = 0, pos0 = 0;
+      if (mine) {
+        start = __ldcg(a.row_start + row);
+        n_new = __ldcg(a.row_start + row + 1) - start;
+        pos0 = __ldcg(a.row_pos0 + row);
+        mine = n_new > a.few;
+      }
       int all;
       const int at = out + c4_scan(mine ? 1 : 0, warp_sums, all);
-      if (mine) {
-        a.seq_out[at] = row;
-        a.q0_out[at] = q0;
-      }
+      if (mine) a.tile[at] = {row, start + q0, min(a.tile_queries, n_new - q0), pos0 + q0};
       out += all;
     }
     if (threadIdx.x == 0) { a.pass[p].tile0 = first; a.pass[p].tiles = out - first; }

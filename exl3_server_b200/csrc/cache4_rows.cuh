@@ -12,6 +12,9 @@ namespace exl3 {
 // for, and some page that the row's queries look for has none.
 struct FaRow { int lo, count, base, holes; };
 
+// A tile of queries: its sequence, its first row of q, its queries, the first one's position.
+struct PromptTile { int b, row0, rows, p_first; };
+
 // A pass: its slots among all rows' and its tiles in the list by passes.
 struct PromptPass { int slot0, slots, tile0, tiles; };
 
@@ -35,7 +38,7 @@ struct C4Prompt {
   int window, parts;
   int few;               // rows of up to so many new tokens are not taken here
   const int *tile_seq, *tile_q0;
-  int n_tiles;
+  int n_tiles, tile_queries;
   int row_pages, total;  // pages at most of a row, and of all rows
   int stride, passes;    // a row belongs to the pass (pages of the rows before it) / stride
   const __nv_bfloat16* q;
@@ -48,7 +51,7 @@ struct C4Prompt {
   int* pass_of;          // [rows]
   PromptPass* pass;      // [passes]
   int4* slot;            // [total]: row, page of the pool (-1: none), places of it that hold tokens, whether it is the first that the row sees
-  int *seq_out, *q0_out; // [n_tiles], by passes and within one in the given order
+  PromptTile* tile;      // [n_tiles], by passes and within one in the given order
   float2* tops;          // [rows][nkv][parts]: the largest |key| and |value| of a part of a row's pages
   float2* undo;          // [rows][nkv]: what the products of the copied keys and of the copied values are multiplied by
 };
