@@ -57,7 +57,7 @@ sys.path.insert(0, ROOT)
 
 FALLBACK_HBM_GBS = 6650.0
 FALLBACK_BF16_TFLOPS = 1590.0
-HEADLINE = "minicpm-2b"
+HEADLINE = "minicpm-2b"          # the sizes of the headline decode and prefill figures
 
 
 def peaks():

@@ -74,7 +74,7 @@ class StepBatch:
     host_slots: List[int] = field(default_factory=list)
     host_new: List[int] = field(default_factory=list)
     # (length before the step, new tokens) of each row, where the host knows them
-    row_lens: Optional[List[Tuple[int, int]]] = None
+    row_lens: Optional[Tuple[Tuple[int, int], ...]] = None
     # a second stream, in steps of one token per sequence: a block whose two sublayers do not depend on each other may run
     # one of them there (and must have joined it before it returns)
     side: Optional[Any] = None
@@ -145,4 +145,4 @@ def pack_step(slots: Sequence[int], starts: Sequence[int], tokens: Sequence[Sequ
         row_start=view(4), row_pos0=view(5), want_rows=view(6) if wanted else None, n_wanted=len(wanted),
         block_tables=bts, max_kv_len=max([s + c for s, c in zip(starts, counts)] + [0]),
         max_new=max(counts + [0]), workspace=workspace, tiles=tiles, tile_keys=tile_keys, host_slots=list(slots),
-        host_new=counts, row_lens=[(int(s), c) for s, c in zip(starts, counts)])
+        host_new=counts, row_lens=tuple((int(s), c) for s, c in zip(starts, counts)))

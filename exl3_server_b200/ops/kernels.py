@@ -2077,7 +2077,7 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
         # keys beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 154 us and 5 MB this way).
         most, width = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1), block_table.shape[1]
         if row_lens is not None:
-            few, few_len, row_pages, total = _kv4_rows(tuple(map(tuple, row_lens)), most, window, width)
+            few, few_len, row_pages, total = _kv4_rows(row_lens if type(row_lens) is tuple else tuple(map(tuple, row_lens)), most, window, width)
         else:
             few, few_len, row_pages = most if T < rows * max_new else 0, max_len, min(width, -(-max_len // KV4_PAGE))
             if window:

@@ -55,4 +55,4 @@ def test_pages_that_a_row_sees(ctx, new, window, width, want):
 
 def test_a_step_carries_its_rows_lengths():
     b = pack_step([0, 1], [5, 0], [[1, 2], [3]], [[], []], [[[0], [1]]], Workspace("cpu"), "cpu")
-    assert b.row_lens == [(5, 2), (0, 1)]
+    assert b.row_lens == ((5, 2), (0, 1))
