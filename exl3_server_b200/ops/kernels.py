@@ -1980,6 +1980,7 @@ def _kv4_walks(rows: int, tiles: int, heads: int, kv_heads: int, head_dim: int, 
     return walk < 10.0 + unpack + 0.75 * -(-span // KV4_PAGE) * max(1.0, tiles * heads / 190.0)
 
 
+KV4_BESIDE_US = 10.0        # what a launch for the few-token rows beside a step's prompts costs
 KV4_MAX_CHUNK = 128         # tiles of a chunk, and
 KV4_MAX_CHUNKS = 1024       # chunks of a row that the plan considers
 
@@ -2074,12 +2075,14 @@ def kv4_attn(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, row
             if t.numel() < tiles[2]:
                 raise KernelLibraryError(f"kv4_attn: {tiles[2]} tiles, of which {t.numel()} are listed")
         # Rows of a few tokens beside prompts (sequences that decode) walk all the same: their pages would be unpacked for a token or two (63 rows of 8,000
-        # keys beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 154 us and 5 MB this way).
+        # keys beside a prompt of 200, 32 heads of 128 on 8: 1,776 us and 2.1 GB of scratch, 154 us and 5 MB this way); unless that is so little that a launch of
+        # its own costs more (24 prompts of 16 to 2,040, 36 heads of 64: 541 us where the one of 16 walks, 530 where it does not).
         most, width = min(max(1, KV4_FEW_COLUMNS // group), max_new - 1), block_table.shape[1]
+        worth = int(KV4_BESIDE_US * 3e6 / (5.25 * kv_heads * head_dim))              # keys whose unpacking (3 TB/s) takes as long as the launch
         if row_lens is not None:
-            few, few_len, row_pages, total = _kv4_rows(row_lens if type(row_lens) is tuple else tuple(map(tuple, row_lens)), most, window, width)
+            few, few_len, row_pages, total = _kv4_rows(row_lens if type(row_lens) is tuple else tuple(map(tuple, row_lens)), most, worth, window, width)
         else:
-            few, few_len, row_pages = most if T < rows * max_new else 0, max_len, min(width, -(-max_len // KV4_PAGE))
+            few, few_len, row_pages = most if T < rows * max_new and rows * max_len >= worth else 0, max_len, min(width, -(-max_len // KV4_PAGE))
             if window:
                 row_pages = min(row_pages, (window + max_new - 2) // KV4_PAGE + 2)
             total = max(1, min(rows, T // (few + 1))) * row_pages
@@ -2141,11 +2144,13 @@ def _kv4_row_pages(ctx: int, new: int, window: int, width: int) -> int:
 
 
 @functools.lru_cache(maxsize=64)
-def _kv4_rows(row_lens: tuple, most: int, window: int, width: int) -> tuple:
-    """Of a step with prompts: the most tokens of a row of up to ``most`` (0: no such row) and the most keys of one, and the pages that the
-    other rows see, of one at most and together.  (Every layer of a step asks.)"""
+def _kv4_rows(row_lens: tuple, most: int, worth: int, window: int, width: int) -> tuple:
+    """Of a step with prompts: the most tokens of a row of up to ``most`` and the most keys of one (0 where these rows have fewer than ``worth`` keys
+    together: they go with the prompts), and the pages that the other rows see, of one at most and together.  (Every layer of a step asks.)"""
     short = [(n, c + n) for c, n in row_lens if 0 < n <= most]
-    few, few_len = (max(n for n, _ in short), max(k for _, k in short)) if short else (0, 0)
+    few, few_len = 0, 0
+    if short and sum(min(k, window + n) if window else k for n, k in short) >= worth:
+        few, few_len = max(n for n, _ in short), max(k for _, k in short)
     sizes = [_kv4_row_pages(c, n, window, width) for c, n in row_lens if n > few] or [1]
     return few, few_len, max(sizes), sum(sizes)
 

@@ -191,8 +191,10 @@ MIXED = [(700, 1), (0, 200), (1300, 1), (64, 1), (90, 150), (0, 1), (0, 0), (513
 @pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (16, 2, 64), (40, 1, 64), (8, 2, 128), (7, 1, 128)])
 @pytest.mark.parametrize("window", [0, 100])
 @pytest.mark.parametrize("known", [True, False])
-def test_single_tokens_beside_prompts(heads, kv_heads, d, window, known, monkeypatch):
+@pytest.mark.parametrize("beside", [True, False])
+def test_single_tokens_beside_prompts(heads, kv_heads, d, window, known, beside, monkeypatch):
     monkeypatch.setattr(K(), "_kv4_walks", lambda *a: False)
+    monkeypatch.setattr(K(), "KV4_BESIDE_US", 0.0 if beside else 1e9)
     c = Case(MIXED, heads, kv_heads, d, seed=29)
     out = c.run(window, row_lens=MIXED if known else None, out=torch.full_like(c.q, math.nan))
     c.check(out, window, only=(0, 1, 16, 149, 199))

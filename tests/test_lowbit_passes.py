@@ -56,3 +56,13 @@ def test_pages_that_a_row_sees(ctx, new, window, width, want):
 def test_a_step_carries_its_rows_lengths():
     b = pack_step([0, 1], [5, 0], [[1, 2], [3]], [[], []], [[[0], [1]]], Workspace("cpu"), "cpu")
     assert b.row_lens == ((5, 2), (0, 1))
+
+
+def test_which_rows_walk_beside_prompts():
+    """Rows of up to 4 tokens walk where they have enough keys together, and then up to the longest of them; the others' pages are counted."""
+    lens = ((8000, 1), (7000, 2), (0, 200), (100, 5), (5, 0))
+    assert K._kv4_rows(lens, 4, 15003, 0, 999) == (2, 8001, 4, 4 + 2)
+    assert K._kv4_rows(lens, 4, 15004, 0, 999) == (0, 0, 126, 126 + 110 + 4 + 2)
+    assert K._kv4_rows(lens, 4, 203, 100, 999) == (2, 8001, 4, 4 + 2)
+    assert K._kv4_rows(lens, 4, 204, 100, 999)[0] == 0
+    assert K._kv4_rows(((0, 200), (3, 0)), 4, 0, 0, 999) == (0, 0, 4, 4)
