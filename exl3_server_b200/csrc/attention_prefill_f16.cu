@@ -11,9 +11,9 @@
 // Three kernels a pass: the plan (where a row's copies go, which tiles are whose, the largest keys and values; once), the copies (and, once, the
 // queries), the attention.  Copies are made of the pages that a row's queries see and of nothing else, and of no more at a time than the caller gives room for.
 //
-// Measured: 3,900 new tokens behind 1,200, 32 heads of 128 on 8: 255 us of the GPU in a short run, 268 in a long one (201 GFLOP of causal work, 0.79 and
-// 0.75 PFLOP/s): 5 the plan, 30 the copies and the queries, the rest the attention, which is bound as it is for bfloat16, by the softmax's exponentials beside the
-// products.  One prompt of 200 tokens 14.6 us, 3 of them the plan behind the launch ahead.
+// Measured: 3,900 new tokens behind 1,200, 32 heads of 128 on 8: 253 us of the GPU in a short run, 270 in a long one (201 GFLOP of causal work, 0.79 and
+// 0.74 PFLOP/s): 5 the plan, 30 the copies and the queries, the rest the attention, which is bound as it is for bfloat16, by the softmax's exponentials beside the
+// products.  One prompt of 200 tokens 14.9 us, 3 of them the plan.
 #define EXL3_PREFILL_F16
 #include "attention_prefill_tc.cuh"
 
