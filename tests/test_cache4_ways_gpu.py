@@ -300,3 +300,22 @@ def test_queries_that_are_not_finite(way, value, d, new):
     q[0, d + 6] = value                                                 # head 1 of the first token
     out = c.run(q=q).view(new, 4, d)
     assert bool(out[0, 1].isnan().all()) and bool(out[0, [0, 2, 3]].isfinite().all()) and bool(out[1:].isfinite().all())
+
+
+def test_steps_in_a_row_in_one_workspace():
+    """Steps of other rows, lengths and head sizes, launched one behind the other into the same scratch memory: each as it is alone."""
+    from exl3_server_b200.engine.batch import Workspace
+    sets = [([(300, 200), (0, 130), (700, 17)], 8, 2, 128, 0), ([(0, 700)], 4, 4, 64, 0), ([(64, 300), (5, 150), (900, 1), (0, 140)], 8, 2, 128, 100),
+            ([(0, 140)] * 9, 16, 16, 64, 0), ([(20, 150), (0, 400)], 7, 1, 128, 0)]
+    cases = [(Case(rows, h, g, d, seed=40 + i), window, rows) for i, (rows, h, g, d, window) in enumerate(sets)]
+    cases[0][0].table[1, 0] = -1
+    want = []
+    for c, window, rows in cases:
+        want.append(c.run(window, workspace=Workspace(torch.device(DEV)), row_lens=rows))
+        torch.cuda.synchronize()
+    ws = Workspace(torch.device(DEV))
+    for turn in range(12):
+        order = [(3 * turn + i) % 5 for i in range(5)]
+        got = [(i, cases[i][0].run(cases[i][1], workspace=ws, row_lens=cases[i][2] if turn % 2 else None)) for i in order + order[::2]]
+        assert all(torch.equal(out, want[i]) for i, out in got), turn
+    K().check_status()
