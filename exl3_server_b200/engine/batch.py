@@ -37,6 +37,7 @@ class Workspace:
         if self._buf is None or self._buf.numel() < n:
             if self._buf is not None and self.keep_outgrown:
                 self._outgrown.append(self._buf)
+            self._buf = None                                  # (given back before the larger one is asked for)
             self._buf = torch.zeros(max(n, 1 << 16), dtype=torch.float32, device=self.device)
         return self._buf
 

@@ -319,3 +319,17 @@ def test_steps_in_a_row_in_one_workspace():
         got = [(i, cases[i][0].run(cases[i][1], workspace=ws, row_lens=cases[i][2] if turn % 2 else None)) for i in order + order[::2]]
         assert all(torch.equal(out, want[i]) for i, out in got), turn
     K().check_status()
+
+
+def test_a_workspace_grows_in_place_of_what_it_was():
+    """The smaller buffer is given back before the larger one is made, unless recorded graphs may hold its address."""
+    from exl3_server_b200.engine.batch import Workspace
+    n = 40 << 20
+    for keep in (False, True):
+        torch.cuda.empty_cache()
+        ws = Workspace(torch.device(DEV), keep_outgrown=keep)
+        first = ws.plain(n).data_ptr()
+        _, took = peak(lambda: ws.plain(2 * n) is None)
+        assert (took <= 4 * n + (1 << 20)) == (not keep), took      # from n floats to 2 n: n more, 2 n where both are held
+        assert not keep or ws._outgrown[0].data_ptr() + 4 * Workspace.COUNTERS == first
+        del ws
