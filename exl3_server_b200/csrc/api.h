@@ -504,4 +504,27 @@ int exl3_fp8_linear(const void* x, int64_t ldx, void* codes, float* sx, const vo
 // Codes left by bounded waits that ran out (0: none); cleared by the calls.
 int exl3_fp8_skinny_status();
 int exl3_fp8_wide_status();
+// Attention over lists of pages (attention_pages.cu) and over pages that rows share (attention_shared.cu), bfloat16, pools [pages, kv heads, 64, hd].  scratch:
+// exl3_attn_pages_scratch floats, the first 65,536 of them zero before the first call (they are zero after each).
+long long exl3_attn_pages_scratch(int sms, int T, int nh, int nkv, int hd, int n_groups);
+// Token t attends over the pages of its row that lists[t][kv head][count] names (its first min(count, tok_pos / 64 + 1) entries).
+int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table, int bt_stride,
+                    int bt_width, int bt_rows, const int* tok_pos, const int* tok_seq, int T, const int* lists, int count, int nh, int nkv, int hd, float scale,
+                    float* scratch, long long scratch_floats, cudaStream_t stream);
+// Causal attention of rows (tokens row_start[r] .. row_start[r + 1] - 1, at most max_new, at positions row_pos0[r] ...), where the rows of a group (groups [n_groups][3],
+// ascending: first row, rows, pages) have their first pages in common.
+int exl3_attn_shared(const void* q, int64_t q_stride, void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table, int bt_stride,
+                     int bt_width, const int* row_start, const int* row_pos0, int rows, int T, const int* groups, int n_groups, int max_new, int nh, int nkv, int hd,
+                     float scale, float* scratch, long long scratch_floats, cudaStream_t stream);
+// Codes left by bounded waits that ran out (0: none); cleared by the calls.
+int exl3_attn_pages_status();
+int exl3_attn_shared_status();
+// Bounds of pages in 8 bits and the choice of pages by them (page_select.cu): codes int8 [pages, kv heads, 2, hd], scales float32 [pages, kv heads].
+int exl3_page_bounds(const void* k_pool, int64_t n_pages, const int* block_table, int bt_stride, int bt_width, const int* row_start, const int* row_pos0, int rows,
+                     int max_new, int nkv, int hd, void* codes, float* scales, cudaStream_t stream);
+int exl3_page_bounds_load(const void* codes, const float* scales, int64_t n_pages, const int* pages, int n, int nkv, int hd, float* low, float* high,
+                          cudaStream_t stream);
+int exl3_page_select(const void* q, int64_t q_stride, const void* codes, const float* scales, int64_t n_pages, const int* block_table, int bt_stride, int bt_width,
+                     int bt_rows, const int* tok_pos, const int* tok_seq, int T, int nh, int nkv, int hd, int count, int first, int last, int* out,
+                     cudaStream_t stream);
 }

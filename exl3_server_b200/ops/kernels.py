@@ -1143,7 +1143,8 @@ def check_status() -> None:
                                      ("attn_decode", attn_decode_status),
                                      ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status),
                                      ("kv4_attn", kv4_attn_status), ("kv4_prompt", kv4_prompt_status), ("fp8_skinny", fp8_skinny_status),
-                                     ("fp8_wide", fp8_wide_status)) if fn()]
+                                     ("fp8_wide", fp8_wide_status), ("attn_pages", attn_pages_status),
+                                     ("attn_shared", attn_shared_status)) if fn()]
     if gave_up:
         raise KernelLibraryError("a bounded wait ran out in " + ", ".join(gave_up) +
                                  ": a copy or a tensor-core product did not complete in time")
@@ -2273,4 +2274,232 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Op
                                                      1 if gated else 0, 0 if not few else 1 if fixed_order else 2, _raw_stream())
     if rc:
         _check(rc, "fp8_linear")
+    return out
+
+
+# ---- attention over pages that rows share and over chosen pages (attention_pages.cu, attention_shared.cu, page_select.cu) -------------------
+
+PAGES_MAX_GROUPS = 256      # groups of rows of one call
+
+
+def attn_pages_status() -> int:
+    """0, or the code the attention over pages left when a bounded wait ran out (cleared by this call)."""
+    return int(library().exl3_attn_pages_status())
+
+
+def attn_shared_status() -> int:
+    """0, or the code the attention over shared pages left when a bounded wait ran out (cleared by this call)."""
+    return int(library().exl3_attn_shared_status())
+
+
+def _here(t: torch.Tensor, what: str) -> None:
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise KernelLibraryError(f"{what}: the tensors are on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """All tensors on the current device."""
+    _addr(first)
+    _here(first, what)
+    at = first.device
+    for t in others:
+        if t is not None and t.device != at:
+            raise KernelLibraryError(f"{what}: tensors on {at} and {t.device}")
+
+
+def _paged_pool(pool: torch.Tensor, name: str, kv_heads: int, head_dim: int, what: str) -> int:
+    """The pool's pages, after its checks."""
+    if pool.dtype is not torch.bfloat16 or pool.ndim != 4 or pool.shape[1:] != (kv_heads, 64, head_dim) or not pool.is_contiguous():
+        raise KernelLibraryError(f"{what}: {name} must be contiguous bfloat16 [pages, {kv_heads}, 64, {head_dim}], got {pool.dtype} {tuple(pool.shape)}")
+    return pool.shape[0]
+
+
+def _paged_q(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, what: str) -> None:
+    if head_dim not in (64, 128) or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise KernelLibraryError(f"{what}: heads of 64 or 128 in groups of one size, got {heads} heads on {kv_heads} of {head_dim}")
+    width = heads * head_dim
+    if q.dtype is not torch.bfloat16 or q.ndim != 2 or q.shape[1] != width or q.stride(1) != 1:
+        raise KernelLibraryError(f"{what}: q must be bfloat16 [tokens, {width}], got {q.dtype} {tuple(q.shape)}")
+
+
+def _paged_queries(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
+    """The output, after the queries' checks."""
+    _paged_q(q, heads, kv_heads, head_dim, what)
+    width = heads * head_dim
+    if out is None:
+        return q.new_empty((q.shape[0], width))
+    if out.dtype is not torch.bfloat16 or tuple(out.shape) != (q.shape[0], width) or not out.is_contiguous():
+        raise KernelLibraryError(f"{what}: out must be contiguous bfloat16 {(q.shape[0], width)}")
+    return out
+
+
+def _row_arrays(row_start: torch.Tensor, row_pos0: torch.Tensor, block_table: torch.Tensor, what: str) -> int:
+    """The rows, after the checks of their arrays."""
+    _int32(row_start, "row_start", what)
+    _int32(row_pos0, "row_pos0", what)
+    rows = row_pos0.numel()
+    if row_start.numel() != rows + 1:
+        raise KernelLibraryError(f"{what}: row_start has {row_start.numel()} entries for {rows} rows")
+    _table(block_table, rows, what)
+    return rows
+
+
+def _positive(scale: float, what: str) -> None:
+    if not 0.0 < scale < math.inf:
+        raise KernelLibraryError(f"{what}: the scale must be positive and finite, got {scale}")
+
+
+def _token_arrays(T: int, tok_pos: torch.Tensor, tok_seq: torch.Tensor, block_table: torch.Tensor, what: str) -> None:
+    _int32(tok_pos, "tok_pos", what)
+    _int32(tok_seq, "tok_seq", what)
+    if tok_pos.numel() < T or tok_seq.numel() < T:
+        raise KernelLibraryError(f"{what}: tok_pos has {tok_pos.numel()} and tok_seq {tok_seq.numel()} entries for {T} tokens")
+    _table(block_table, None, what)
+
+
+def _pages_scratch(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, groups: int, workspace) -> tuple:
+    need = _long_entry("exl3_attn_pages_scratch", 6)(_sms(q), q.shape[0], heads, kv_heads, head_dim, groups)
+    return need, workspace.floats(need) if workspace is not None else torch.zeros(need, dtype=torch.float32, device=q.device)
+
+
+def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, row_start: torch.Tensor, row_pos0: torch.Tensor,
+                groups: Optional[torch.Tensor], max_new: int, heads: int, kv_heads: int, head_dim: int, scale: float, workspace=None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention ``softmax(q K^T * scale) V`` of a step's new tokens over the paged bfloat16 cache, which already holds them, where rows share pages.  Row r has
+    tokens ``row_start[r] .. row_start[r + 1] - 1`` (at most ``max_new``) of ``q`` bfloat16 ``[T, heads * head_dim]`` at positions ``row_pos0[r] ...``.
+    ``groups``: int32 ``[n, 3]`` on the device, ascending: the rows ``first .. first + rows - 1`` have their first ``pages`` pages in common, which are read once for all of
+    them, from the first row's table (None: no groups).  Their tokens see all of these keys: positions from ``64 * pages - 1`` on.  Groups do not overlap (one that
+    begins before the one ahead of it ends is no group).  Pages that are not there are left out; a query that sees nothing gets zeros.
+    ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's)."""
+    out = _paged_queries(q, heads, kv_heads, head_dim, out, "attn_shared")
+    _positive(scale, "attn_shared")
+    pages = _paged_pool(k_pool, "k_pool", kv_heads, head_dim, "attn_shared")
+    if _paged_pool(v_pool, "v_pool", kv_heads, head_dim, "attn_shared") != pages:
+        raise KernelLibraryError("attn_shared: k_pool and v_pool have different numbers of pages")
+    rows = _row_arrays(row_start, row_pos0, block_table, "attn_shared")
+    n_groups = 0
+    if groups is not None:
+        _int32(groups, "groups", "attn_shared")
+        if groups.ndim != 2 or groups.shape[1] != 3 or groups.shape[0] > PAGES_MAX_GROUPS:
+            raise KernelLibraryError(f"attn_shared: groups must be int32 [up to {PAGES_MAX_GROUPS}, 3], got {tuple(groups.shape)}")
+        n_groups = groups.shape[0]
+    _same_device("attn_shared", q, k_pool, v_pool, block_table, row_start, row_pos0, groups, out)
+    T = q.shape[0]
+    if T == 0 or rows == 0:
+        return out
+    need, scratch = _pages_scratch(q, heads, kv_heads, head_dim, n_groups, workspace)
+    rc = _entry("exl3_attn_shared", "plppplpiippiipiiiiifpl")(
+        _addr(q), _pitch(q), _addr(out), _addr(k_pool), _addr(v_pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], _addr(row_start),
+        _addr(row_pos0), rows, T, _addr(groups), n_groups, max_new, heads, kv_heads, head_dim, scale, _addr(scratch), need, _raw_stream())
+    if rc:
+        _check(rc, "attn_shared")
+    return out
+
+
+def page_bounds_pool(pages: int, kv_heads: int, head_dim: int, device) -> tuple:
+    """Empty bounds for a pool of pages: codes int8 ``[pages, kv_heads, 2, head_dim]`` (smallest, largest) and scales float32 ``[pages, kv_heads]``."""
+    if head_dim not in (64, 128):
+        raise KernelLibraryError(f"bounds of pages: heads of 64 or 128, got {head_dim}")
+    return torch.zeros((pages, kv_heads, 2, head_dim), dtype=torch.int8, device=device), torch.zeros((pages, kv_heads), dtype=torch.float32, device=device)
+
+
+def _bounds_pool(codes: torch.Tensor, scales: torch.Tensor, what: str) -> tuple:
+    """Pages, kv heads and head size of the bounds, after their checks."""
+    if codes.dtype is not torch.int8 or codes.ndim != 4 or codes.shape[2] != 2 or codes.shape[3] not in (64, 128) or not codes.is_contiguous():
+        raise KernelLibraryError(f"{what}: codes must be contiguous int8 [pages, kv_heads, 2, 64 or 128], got {codes.dtype} {tuple(codes.shape)}")
+    pages, kv_heads, _, head_dim = codes.shape
+    if scales.dtype is not torch.float32 or tuple(scales.shape) != (pages, kv_heads) or not scales.is_contiguous():
+        raise KernelLibraryError(f"{what}: scales must be contiguous float32 {(pages, kv_heads)}, got {scales.dtype} {tuple(scales.shape)}")
+    return pages, kv_heads, head_dim
+
+
+def page_bounds(k_pool: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, row_start: torch.Tensor, row_pos0: torch.Tensor,
+                max_new: int) -> None:
+    """New bounds for the pages that hold a step's new tokens, whose keys are in the cache: the smallest and largest key of every feature over the page's tokens so far,
+    ``a = max |k|``, ``scale = a / 127``, ``code = rint(x * (127 / a))``.  Rows as in ``attn_shared``.  A page that holds a key that is not finite has
+    codes 0 and an infinite scale.  Pages that are not there are left out."""
+    pages, kv_heads, head_dim = _bounds_pool(codes, scales, "page_bounds")
+    if _paged_pool(k_pool, "k_pool", kv_heads, head_dim, "page_bounds") != pages:
+        raise KernelLibraryError(f"page_bounds: {k_pool.shape[0]} pages of keys, bounds of {pages}")
+    rows = _row_arrays(row_start, row_pos0, block_table, "page_bounds")
+    if max_new < 0:
+        raise KernelLibraryError(f"page_bounds: max_new {max_new}")
+    _same_device("page_bounds", k_pool, codes, scales, block_table, row_start, row_pos0)
+    if rows == 0 or max_new == 0:
+        return
+    rc = _entry("exl3_page_bounds", "plpiippiiiipp")(
+        _addr(k_pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], _addr(row_start), _addr(row_pos0), rows, max_new, kv_heads, head_dim,
+        _addr(codes), _addr(scales), _raw_stream())
+    if rc:
+        _check(rc, "page_bounds")
+
+
+def page_bounds_load(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Tensor):
+    """The bounds that the listed pages' codes stand for: smallest and largest, float32 ``[n, kv_heads, head_dim]`` each (zeros for a number that is no page's)."""
+    held, kv_heads, head_dim = _bounds_pool(codes, scales, "page_bounds_load")
+    _int32(pages, "pages", "page_bounds_load")
+    _same_device("page_bounds_load", codes, scales, pages)
+    n = pages.numel()
+    low = scales.new_empty((n, kv_heads, head_dim))
+    high = torch.empty_like(low)
+    rc = _entry("exl3_page_bounds_load", "pplpiiipp")(_addr(codes), _addr(scales), held, _addr(pages), n, kv_heads, head_dim, low.data_ptr(), high.data_ptr(), _raw_stream())
+    if rc:
+        _check(rc, "page_bounds_load")
+    return low, high
+
+
+def page_select(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, tok_pos: torch.Tensor, tok_seq: torch.Tensor, count: int,
+                heads: int, kv_heads: int, head_dim: int, first: int = 1, last: int = 1, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """For each token and key/value head up to ``count`` pages of the token's row (``tok_seq``) that hold positions up to its own (``tok_pos``): int32
+    ``[T, kv_heads, count]``, numbers of pages within the row in ascending order, -1 behind them.  The row's first ``first`` and last ``last`` pages up to the token's own are taken
+    first (the lowest of them where ``count`` is smaller), then those of the highest scores, of equal ones the lower page: an upper estimate of the largest ``q . k`` on the page
+    over the key/value head's query heads, ``max_h(n_h * (a_h / 127)) * scale`` with ``a_h = max |q_h|``, ``c_h = rint(q_h * (127 / a_h))`` and
+    ``n_h = sum_i max(c_hi * low_i, c_hi * high_i)`` over the page's codes (``page_bounds``).  A page whose keys are not finite comes before those that have a
+    score.  Pages that are not there are not taken.  For queries that are not finite some pages are taken."""
+    _paged_q(q, heads, kv_heads, head_dim, "page_select")
+    pages, held, size = _bounds_pool(codes, scales, "page_select")
+    if (held, size) != (kv_heads, head_dim):
+        raise KernelLibraryError(f"page_select: bounds of {held} key/value heads of {size}, not {kv_heads} of {head_dim}")
+    T = q.shape[0]
+    if count < 1 or first < 0 or last < 1:
+        raise KernelLibraryError(f"page_select: takes a count of 1 or more and at least the last page, got count {count}, first {first}, last {last}")
+    _token_arrays(T, tok_pos, tok_seq, block_table, "page_select")
+    if out is None:
+        out = tok_pos.new_empty((T, kv_heads, count))
+    elif out.dtype is not torch.int32 or tuple(out.shape) != (T, kv_heads, count) or not out.is_contiguous():
+        raise KernelLibraryError(f"page_select: out must be contiguous int32 {(T, kv_heads, count)}")
+    _same_device("page_select", q, codes, scales, block_table, tok_pos, tok_seq, out)
+    rc = _entry("exl3_page_select", "plpplpiiippiiiiiiip")(
+        _addr(q), _pitch(q), _addr(codes), _addr(scales), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0], _addr(tok_pos),
+        _addr(tok_seq), T, heads, kv_heads, head_dim, count, first, last, _addr(out), _raw_stream())
+    if rc:
+        _check(rc, "page_select")
+    return out
+
+
+def attn_pages(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, tok_pos: torch.Tensor, tok_seq: torch.Tensor, pages: torch.Tensor,
+               heads: int, kv_heads: int, head_dim: int, scale: float, workspace=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of each token over some pages of its row: ``softmax(q K^T * scale) V`` over the keys at positions up to its own (``tok_pos``) of the pages that ``pages`` int32
+    ``[T, kv_heads, count]`` lists for it and the key/value head, by their numbers within the row (``tok_seq``), in any order; ``page_select`` makes such lists.  The first
+    ``min(count, tok_pos // 64 + 1)`` entries are looked at (a token can see no more pages); entries that are negative or beyond the token's position, and pages
+    that are not there, are left out, one that is listed twice counts twice.  A query that sees nothing gets zeros."""
+    out = _paged_queries(q, heads, kv_heads, head_dim, out, "attn_pages")
+    _positive(scale, "attn_pages")
+    n_pages = _paged_pool(k_pool, "k_pool", kv_heads, head_dim, "attn_pages")
+    if _paged_pool(v_pool, "v_pool", kv_heads, head_dim, "attn_pages") != n_pages:
+        raise KernelLibraryError("attn_pages: k_pool and v_pool have different numbers of pages")
+    T = q.shape[0]
+    _token_arrays(T, tok_pos, tok_seq, block_table, "attn_pages")
+    _int32(pages, "pages", "attn_pages")
+    if pages.ndim != 3 or pages.shape[:2] != (T, kv_heads) or pages.shape[2] < 1:
+        raise KernelLibraryError(f"attn_pages: pages must be int32 [{T}, {kv_heads}, 1 or more], got {tuple(pages.shape)}")
+    _same_device("attn_pages", q, k_pool, v_pool, block_table, tok_pos, tok_seq, pages, out)
+    if T == 0:
+        return out
+    need, scratch = _pages_scratch(q, heads, kv_heads, head_dim, 0, workspace)
+    rc = _entry("exl3_attn_pages", "plppplpiiippipiiiifpl")(
+        _addr(q), _pitch(q), _addr(out), _addr(k_pool), _addr(v_pool), n_pages, _addr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0],
+        _addr(tok_pos), _addr(tok_seq), T, _addr(pages), pages.shape[2], heads, kv_heads, head_dim, scale, _addr(scratch), need, _raw_stream())
+    if rc:
+        _check(rc, "attn_pages")
     return out
