@@ -15,16 +15,15 @@
 
 namespace exl3 {
 
-constexpr int PG_WARPS = 4;                    // computing warps, and as many that ask for copies
-constexpr int PG_UNIT_BYTES = 16384;           // a unit: keys and values of a page (heads of 64) or of half a page (heads of 128)
-// A stage is always the same warps' (of the team's running count of units, n, warps n % lanes take unit n, in stage n % PG_STAGES): a warp that
-// waits for a stage has itself freed it before, so that the stage's barrier is never a phase behind what the warp asks for.
-constexpr int PG_STAGES = 8;
-static_assert(PG_STAGES % PG_WARPS == 0, "a stage is always the same warps'");
-constexpr int PG_MAX_COLS = 16 * PG_WARPS;     // queries of an item
-constexpr int PG_WINDOW = 1024;                // items of a launch
-constexpr int PG_MAX_WIDTH = 1 << 19;          // pages of a row: the units of a launch's items stay within 31 bits
-constexpr uint32_t PG_SMEM_RING = PG_STAGES * PG_UNIT_BYTES;
+constexpr int PG_WARPS = 8;                    // of a block, one block an SM
+constexpr int PG_STAGES = 3;                   // of a warp's ring
+constexpr int PG_UNIT_BYTES = 8192;            // a unit: keys and values of 32 tokens (heads of 64) or 16 (heads of 128)
+constexpr int PG_COLS = 16;                    // queries of an item
+constexpr int PG_WINDOW = 1024;                // rows of a launch
+constexpr int PG_MIN_UNITS = 4;                // of a warp's share, at least
+constexpr int PG_MAX_WIDTH = 1 << 19;          // pages of a row
+constexpr int PG_RING = PG_STAGES * PG_UNIT_BYTES;
+constexpr uint32_t PG_SMEM_RINGS = PG_WARPS * PG_RING;
 
 static __device__ int g_pg_error = 0;
 
@@ -41,8 +40,7 @@ struct PgArgs {
   const int* row_start;                        // rows
   const int* row_pos0;
   int rows, T, nh, nkv, G;
-  int item0;                                   // the first item of this launch
-  int groups_of_cols;                          // warps side by side on a unit, 16 queries each: 1, 2 or 4
+  int row0;                                    // the first row of this launch
   float scale_log2;
   int* counters;
   float* records;
@@ -50,7 +48,7 @@ struct PgArgs {
   const int* groups;
   int n_groups, ps_grid;
   int wait_first;                              // whether the kernel before must have ended
-  const float* ps_records;
+  float* own;                                  // rows of groups: their own pages' part goes here
 };
 
 __device__ inline void pg_ldsm(uint32_t (&r)[4], uint32_t addr) {
@@ -75,203 +73,205 @@ __device__ inline uint32_t pg_pack(float lo, float hi) {
 }
 // Whether one of a word's two bfloat16 is not finite.
 __device__ inline bool pg_odd(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
-// The form that a warp's threads may reach one after the other: code of one thread stands before most of these barriers.
-__device__ inline void pg_bar(int id, int threads) {
-  __syncwarp();
-  asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
 // Bounded, and one answer for the warp.
 __device__ inline bool pg_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tc5::mbar_wait(bar, parity)); }
 
 constexpr float PG_NEG = -INFINITY;
 
-template <int HD> struct PgSmem {
-  static constexpr int COLS = PG_MAX_COLS;
-  float acc[PG_WARPS][16][HD];                 // the warps' sums of an item, to be joined
-  float m[PG_WARPS][16], l[PG_WARPS][16];
-  uint64_t full[PG_STAGES], empty[PG_STAGES];
-  int key0[PG_STAGES];                         // a stage's first key (its place in the row); below 0: the page is not there
-  int cum[PG_WINDOW + 1];                      // units of the items before (per kv head)
-  int item_row[PG_WINDOW], item_block[PG_WINDOW];
-  int flag[PG_WARPS];
-  int n_items;
+// A warp's part of an item, at the start of its ring when the ring is done with: two of them at most, of the item that its share begins in and
+// of the one that it ends in.
+template <int HD> struct PgPart {
+  float m[PG_COLS], l[PG_COLS], acc[PG_COLS][HD];
+};
+struct PgSmem {
+  uint64_t full[PG_WARPS][PG_STAGES];
+  int64_t cum[PG_WINDOW + 1];                  // units of the rows before
+  int start[PG_WINDOW], n_new[PG_WINDOW], pos[PG_WINDOW], units[PG_WINDOW];
+  int64_t part_at[PG_WARPS][2];                // a part's item (the place of its first unit), -1: none
+  int64_t warp_sum[PG_WARPS];
+  int last[2];
   PsPlan plan;
 };
 
-// Items: the queries that walk the same pages: of a row (or of a listed token) and a kv head up to PG_MAX_COLS (token, query head) pairs.  The units of all
-// items, ordered by item and kv head, are cut into equal shares for teams of warps; a team's share may begin and end within an item, whose parts are then joined by the
-// team that is last to report (in the parts' order, so that results do not depend on which it was).
+// Items: up to PG_COLS queries (token, query head) of a row (or of a listed token) and key/value head, which walk the same pages.  The units of all items, ordered by row, head and
+// item, are cut into equal shares for the warps, which stream them through rings of their own, each asking for its own copies: nothing is waited for but
+// memory.  What a warp has whole it writes out; parts of items that shares cut are joined in shared memory at the end, and those that blocks cut by the block that
+// is the last to report, always in the order of the pages, so that results do not depend on which it was.
 template <int HD, bool LIST>
-__global__ void __launch_bounds__(2 * PG_WARPS * 32, 1)
+__global__ void __launch_bounds__(PG_WARPS * 32, 1)
 attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PgArgs a) {
-  constexpr int KS = HD == 64 ? 64 : 32;       // keys of a unit
+  constexpr int KS = HD == 64 ? 32 : 16;       // keys of a unit
   constexpr int UPP = PG_PAGE / KS;            // units of a page
   constexpr int NT = KS / 8;                   // tiles of 8 keys
   constexpr int KT = HD / 16;                  // pieces of 16 features
   constexpr int BOX = KS * 128;                // bytes of a box of 64 features
+  constexpr int HALF = PG_UNIT_BYTES / 2;      // keys, then values
+  static_assert(2 * sizeof(PgPart<HD>) <= PG_RING, "a warp's parts fit into its ring");
   extern __shared__ unsigned char pg_raw[];
-  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pg_raw) + 1023) & ~(uintptr_t)1023);
-  PgSmem<HD>& sm = *reinterpret_cast<PgSmem<HD>*>(ring + PG_SMEM_RING);
-  const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
-  const int ncg = a.groups_of_cols, cols = 16 * ncg;
+  unsigned char* rings = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pg_raw) + 1023) & ~(uintptr_t)1023);
+  PgSmem& sm = *reinterpret_cast<PgSmem*>(rings + PG_SMEM_RINGS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < PG_STAGES; ++s) { tc5::mbar_init(sm.full + s, 1); tc5::mbar_init(sm.empty + s, ncg); }
+    for (int w = 0; w < PG_WARPS; ++w)
+      for (int s = 0; s < PG_STAGES; ++s) tc5::mbar_init(&sm.full[w][s], 1);
     tc5::mbar_init_fence();
   }
-  // The kernel before is, with shared pages, the one that works on them: it let this one start when its own predecessors had ended, and what it
-  // writes is waited for where it is read.  Else everything is waited for here.
+  // The kernel before is, with shared pages, the one that works on them: it let this one start when its own predecessors had ended, and this one needs nothing of it.
+  // Else everything is waited for here.
   if (a.wait_first) pdl_wait();
   pdl_trigger();
-  if (a.n_groups > 0) ps_plan(sm.plan, a.groups, a.n_groups, a.row_start, a.rows, a.T, a.G, a.nkv, a.bt_width, a.ps_grid);
 
-  // ---- the items of this launch ------------------------------------------------------------------------------------------
-  const int most_keys = a.bt_width * PG_PAGE;
-  // a row's first token of q, its tokens, and the first one's position (one beyond the table sees all of it)
-  auto start_of = [&](int row) { return LIST ? row : min(max(__ldcg(a.row_start + row), 0), a.T); };
-  auto new_of = [&](int row, int start) { return LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start); };
-  auto pos_of = [&](int row) { return max(-most_keys, min(most_keys, __ldcg((LIST ? a.tok_pos : a.row_pos0) + row))); };
+  // ---- the rows of this launch -------------------------------------------------------------------------------------------
+  const int most_keys = a.bt_width * PG_PAGE, n_rows = min(a.rows - a.row0, PG_WINDOW);
+  for (int i = threadIdx.x; i < n_rows; i += PG_WARPS * 32) {
+    const int row = a.row0 + i;
+    // (a row beyond the table sees all of it)
+    sm.pos[i] = max(-most_keys, min(most_keys, __ldcg((LIST ? a.tok_pos : a.row_pos0) + row)));
+    const int start = LIST ? row : min(max(__ldcg(a.row_start + row), 0), a.T);
+    sm.start[i] = start;
+    sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
+  }
+  if (a.n_groups > 0) ps_plan(sm.plan, a.groups, a.n_groups, a.row_start, a.rows, a.T, a.G, a.nkv, a.bt_width, a.ps_grid);
+  else __syncthreads();
   auto group_of = [&](int row) {               // -1: none
-    if (a.n_groups == 0) return -1;
+    if (LIST || a.n_groups == 0) return -1;
     int lo = 0, hi = a.n_groups - 1;
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (sm.plan.row[mid] <= row) lo = mid; else hi = mid - 1; }
     return row >= sm.plan.row[lo] && row < sm.plan.row[lo] + sm.plan.rows[lo] && sm.plan.pages[lo] > 0 ? lo : -1;
   };
   auto shared_of = [&](int row) { const int j = group_of(row); return j < 0 ? 0 : sm.plan.pages[j]; };     // pages that the row shares
-  auto units_of = [&](int row, int block, int n_new) {
-    const int pos = pos_of(row);
-    if (LIST) return max(1, min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP);
-    const int end = min(pos + min(n_new, ((block + 1) * cols - 1) / a.G + 1), most_keys);      // keys that the item's last token sees
-    return max(1, (end + KS - 1) / KS - shared_of(row) * UPP);
-  };
-  if (wid == 0) {
-    // rows a stretch of 32 at a time; lane i has row r0 + i
-    int at = 0;                                // items before (of all rows)
-    const int n_rows = a.rows;
-    for (int r0 = 0; r0 < n_rows && at < a.item0 + PG_WINDOW; r0 += 32) {
-      const int row = r0 + lane;
-      int n_new = 0, nb = 0;
-      if (row < n_rows) {
-        n_new = new_of(row, start_of(row));
-        nb = (n_new * a.G + cols - 1) / cols;
+  auto blocks_of = [&](int i) { return (sm.n_new[i] * a.G + PG_COLS - 1) / PG_COLS; };                     // items of a row and head
+  {
+    int64_t run = 0;
+    for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
+      const int i = i0 + threadIdx.x;
+      int64_t mine = 0;
+      if (i < n_rows) {
+        const int pos = sm.pos[i];
+        int units;
+        if (LIST) units = min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP;
+        else units = (min(pos + sm.n_new[i], most_keys) + KS - 1) / KS - shared_of(a.row0 + i) * UPP;
+        sm.units[i] = max(units, 1);           // (one at least: every query gets an answer)
+        mine = (int64_t)max(units, 1) * blocks_of(i) * a.nkv;
       }
-      int incl = nb;
+      int64_t incl = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
-      const int total = __shfl_sync(0xffffffffu, incl, 31);
-      for (int b = 0; b < nb; ++b) {
-        const int i = at + incl - nb + b - a.item0;
-        if (i >= 0 && i < PG_WINDOW) { sm.item_row[i] = row; sm.item_block[i] = b; sm.cum[i + 1] = units_of(row, b, n_new); }
-      }
-      at += total;
+      for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+      if (lane == 31) sm.warp_sum[warp] = incl;
+      __syncthreads();
+      int64_t before = run;
+      for (int w = 0; w < PG_WARPS; ++w) { if (w < warp) before += sm.warp_sum[w]; run += sm.warp_sum[w]; }
+      if (i < n_rows) sm.cum[i + 1] = before + incl;
+      __syncthreads();
     }
-    const int n = max(0, min(at - a.item0, PG_WINDOW));
-    if (lane == 0) { sm.n_items = n; sm.cum[0] = 0; }
-    __syncwarp();
-    int run = 0;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      int incl = i < n ? sm.cum[i + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
-      if (i < n) sm.cum[i + 1] = run + incl;
-      run += __shfl_sync(0xffffffffu, incl, 31);
-    }
+    if (threadIdx.x == 0) sm.cum[0] = 0;
+    __syncthreads();
   }
-  __syncthreads();
-  const int n_items = sm.n_items;
-  if (n_items == 0) {
+  const int64_t total = sm.cum[n_rows];
+  const int n_blocks = (int)min((int64_t)gridDim.x, max((int64_t)1, total / (PG_WARPS * PG_MIN_UNITS)));
+  if (total == 0 || (int)blockIdx.x >= n_blocks) {
     if (!a.wait_first) pdl_wait();
     return;
   }
-
-  // ---- teams and shares ---------------------------------------------------------------------------------------------------
-  const int64_t total = (int64_t)sm.cum[n_items] * a.nkv;
-  constexpr int TS = PG_WARPS;                 // warps of a team
-  const int per_block = PG_WARPS / TS, stages = PG_STAGES / per_block;
-  const int warp = wid % PG_WARPS, team = warp / TS, tw = warp % TS;
-  const bool copier = wid >= PG_WARPS;
-  const int n_teams = (int)min((int64_t)gridDim.x * per_block, max((int64_t)1, total / 4));
-  const int my = blockIdx.x * per_block + team;
-  auto begin = [&](int t) { return total * t / n_teams; };
-  const int64_t i_lo = my < n_teams ? begin(my) : total, i_hi = my < n_teams ? begin(my + 1) : total;
-  auto item_of = [&](int64_t x) {
-    int lo = 0, hi = n_items - 1;
-    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if ((int64_t)sm.cum[mid] * a.nkv <= x) lo = mid; else hi = mid - 1; }
-    return lo;
+  auto begin = [&](int w) { return total * w / (n_blocks * PG_WARPS); };       // the first unit of a warp's share
+  const int64_t i_lo = begin(blockIdx.x * PG_WARPS + warp), i_hi = begin(blockIdx.x * PG_WARPS + warp + 1);
+  // The item at place x, and where in it.
+  struct Place { int i, g, b, u0, u1, units; int64_t base; };
+  auto place_of = [&](int64_t x, int64_t end) {
+    int lo = 0, hi = n_rows - 1;
+    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (sm.cum[mid] <= x) lo = mid; else hi = mid - 1; }
+    Place p;
+    p.i = lo;
+    p.units = sm.units[lo];
+    const int64_t r = x - sm.cum[lo];
+    const int item = (int)(r / p.units), nb = blocks_of(lo);
+    p.u0 = (int)(r - (int64_t)item * p.units);
+    p.u1 = (int)min((int64_t)p.units, p.u0 + (end - x));
+    p.g = item / nb;
+    p.b = item % nb;
+    p.base = x - p.u0;
+    return p;
   };
-  const int s0 = team * stages;                // the team's stages
-  bool ok = true;
-  if (copier) {
-    // ---- copies: a unit as soon as its stage is free; page numbers come 32 at a time ------------------------------------------
-    if (tw == 0) {
-      int n = 0;
-      for (int64_t x = i_lo; x < i_hi && ok;) {
-        const int it = item_of(x), units = sm.cum[it + 1] - sm.cum[it];
-        const int64_t r = x - (int64_t)sm.cum[it] * a.nkv;
-        const int g = (int)(r / units), u0 = (int)(r % units), u1 = (int)min((int64_t)units, u0 + (i_hi - x));
-        const int row = sm.item_row[it];
-        const int seq = LIST ? __ldcg(a.tok_seq + row) : row;
-        const bool known = seq >= 0 && seq < a.bt_rows;
-        const int* bt = a.block_table + (int64_t)seq * a.bt_stride;
-        const int* list = LIST ? a.lists + ((int64_t)row * a.nkv + g) * a.list_stride : nullptr;
-        const int shared = LIST ? 0 : shared_of(row);
-        for (int p0 = u0 / UPP; p0 * UPP < u1 && ok; p0 += 32) {
-          int logical = p0 + lane + shared;
-          if (LIST) logical = p0 + lane < a.count && (p0 + lane) * UPP < u1 ? __ldcg(list + p0 + lane) : -1;
-          int page = known && logical >= 0 && logical < a.bt_width ? __ldcg(bt + logical) : -1;
-          if (page >= a.n_pages) page = -1;
-          for (int u = max(u0, p0 * UPP); u < min(u1, (p0 + 32) * UPP) && ok; ++u, ++n) {
-            const int pg = __shfl_sync(0xffffffffu, page, u / UPP - p0), lg = __shfl_sync(0xffffffffu, logical, u / UPP - p0);
-            const int st = s0 + n % stages;
-            if (n >= stages && !pg_wait(sm.empty + st, (n / stages - 1) & 1)) { ok = false; break; }
-            if (lane == 0) {
-              sm.key0[st] = pg < 0 ? -1 : lg * PG_PAGE + (u % UPP) * KS;
-              if (pg < 0) {
-                tc5::mbar_arrive(sm.full + st);
-              } else {
-                tc5::mbar_expect_tx(sm.full + st, PG_UNIT_BYTES);
-                const int y = (int)(((int64_t)pg * a.nkv + g) * PG_PAGE) + (u % UPP) * KS;
-                unsigned char* dst = ring + st * PG_UNIT_BYTES;
-#pragma unroll
-                for (int b = 0; b < HD / 64; ++b) {
-                  tc5::tma_load_2d(dst + b * BOX, &map_k, sm.full + st, 64 * b, y);
-                  tc5::tma_load_2d(dst + PG_UNIT_BYTES / 2 + b * BOX, &map_v, sm.full + st, 64 * b, y);
-                }
-              }
-            }
-            __syncwarp();
-          }
-        }
-        x += u1 - u0;
-      }
-      // what was asked for must land before the block's shared memory goes away
-      if (!ok && lane == 0) atomicExch(&g_pg_error, 1);
-      for (int u = max(0, n - stages); u < n; ++u) pg_wait(sm.full + s0 + u % stages, (u / stages) & 1);
+
+  unsigned char* ring = rings + warp * PG_RING;
+  uint64_t* full = sm.full[warp];
+  // ---- copies: page numbers come 32 at a time, a batch ahead -----------------------------------------------------------------
+  int64_t ask_x = i_lo;                        // the next unit to ask for
+  Place ask = {};
+  int ask_u = 0, ask_n = 0, batch_p = 0;       // its number in the item; units asked for so far; the first page of the batch at hand
+  int page = 0, logical = 0, page_next = 0, logical_next = 0;
+  int key0s[PG_STAGES];                        // a stage's first key; below 0: its page is not there
+  auto fetch = [&](int p0, int& pg, int& lg) { // pages p0 + lane of the item
+    const int row = a.row0 + ask.i;
+    const int seq = LIST ? __ldcg(a.tok_seq + row) : row;
+    lg = p0 + lane + (LIST ? 0 : shared_of(row));
+    const bool in = (p0 + lane) * UPP < ask.units;
+    if (LIST) lg = in ? __ldcg(a.lists + ((int64_t)row * a.nkv + ask.g) * a.list_stride + p0 + lane) : -1;
+    pg = in && seq >= 0 && seq < a.bt_rows && lg >= 0 && lg < a.bt_width ? __ldcg(a.block_table + (int64_t)seq * a.bt_stride + lg) : -1;
+    if (pg >= a.n_pages) pg = -1;
+  };
+  auto ask_next = [&]() {
+    if (ask_x >= i_hi) return;
+    if (ask_x == i_lo || ask_u == ask.u1) {    // another item
+      ask = place_of(ask_x, i_hi);
+      ask_u = ask.u0;
+      batch_p = ask_u / UPP;
+      fetch(batch_p, page, logical);
+      fetch(batch_p + 32, page_next, logical_next);
+    } else if (ask_u / UPP - batch_p == 32) {
+      batch_p += 32;
+      page = page_next;
+      logical = logical_next;
+      fetch(batch_p + 32, page_next, logical_next);
     }
-  }
+    const int src = ask_u / UPP - batch_p;
+    const int pg = __shfl_sync(0xffffffffu, page, src), lg = __shfl_sync(0xffffffffu, logical, src);
+    const int st = ask_n % PG_STAGES;
+    const int key0 = pg < 0 ? -1 : lg * PG_PAGE + (ask_u % UPP) * KS;
+#pragma unroll
+    for (int s = 0; s < PG_STAGES; ++s)
+      if (s == st) key0s[s] = key0;
+    if (lane == 0 && pg >= 0) {
+      tc5::mbar_expect_tx(full + st, PG_UNIT_BYTES);
+      const int y = (pg * a.nkv + ask.g) * PG_PAGE + (ask_u % UPP) * KS;
+      unsigned char* dst = ring + st * PG_UNIT_BYTES;
+#pragma unroll
+      for (int x = 0; x < HD / 64; ++x) {
+        tc5::tma_load_2d(dst + x * BOX, &map_k, full + st, 64 * x, y);
+        tc5::tma_load_2d(dst + HALF + x * BOX, &map_v, full + st, 64 * x, y);
+      }
+    } else if (lane == 0) {
+      tc5::mbar_arrive(full + st);
+    }
+    ++ask_u;
+    ++ask_n;
+    ++ask_x;
+  };
+  for (int s = 0; s < PG_STAGES; ++s) ask_next();
 
   // ---- computing ------------------------------------------------------------------------------------------------------------
-  const int cg = tw % ncg, pl = tw / ncg, lanes_of_pages = TS / ncg;   // the warp's 16 queries, and its turn among the units
-  const int bar_id = 1 + team, bar_threads = TS * 32;
-  const uint32_t k_addr = tc5::smem_u32(ring), sw = lane & 7;
-  int n0 = 0;                                  // the team's units before this segment
-  for (int64_t x = copier ? i_hi : i_lo; x < i_hi; ) {
-    const int it = item_of(x), units = sm.cum[it + 1] - sm.cum[it];
-    const int64_t item_base = (int64_t)sm.cum[it] * a.nkv, r = x - item_base;
-    const int g = (int)(r / units), u0 = (int)(r % units), u1 = (int)min((int64_t)units, u0 + (i_hi - x));
-    const int row = sm.item_row[it], col0 = sm.item_block[it] * cols;
-    const int start = start_of(row), n_new = new_of(row, start), pos0 = pos_of(row);
-    const int n_cols = min(cols, n_new * a.G - col0);
-    // this thread's two queries: columns gl and gl + 8 of the warp's 16
+  const uint32_t ring_addr = tc5::smem_u32(ring), sw = lane & 7;
+  bool ok = true;
+  int n = 0;                                   // units done
+  if (lane == 0) sm.part_at[warp][0] = sm.part_at[warp][1] = -1;
+  float m_first[2], l_first[2];                // the first part's, until the ring is free
+  float m[2], l[2], o[HD / 8][4];
+  bool have_first = false;
+  float* const spill = a.records + ((int64_t)blockIdx.x * PG_WARPS + warp) * (PG_COLS * HD);   // (where the first part's sums wait meanwhile)
+  for (int64_t x = i_lo; x < i_hi;) {
+    const Place p = place_of(x, i_hi);
+    const int start = sm.start[p.i], n_new = sm.n_new[p.i], pos0 = sm.pos[p.i], col0 = p.b * PG_COLS;
+    const int n_cols = min(PG_COLS, n_new * a.G - col0);
+    // this thread's two queries: columns gl and gl + 8
     int limit[2];
     uint32_t qf[KT][4];
     {
       const __nv_bfloat16* src[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int c = min(col0 + cg * 16 + gl + 8 * e, n_new * a.G - 1), tok = c / a.G, h = c % a.G;
+        const int c = min(col0 + gl + 8 * e, n_new * a.G - 1), tok = c / a.G, h = c - tok * a.G;
         limit[e] = pos0 + tok;                 // the last key it sees
-        src[e] = a.q + (int64_t)(start + tok) * a.q_stride + (int64_t)(g * a.G + h) * HD;
+        src[e] = a.q + (int64_t)(start + tok) * a.q_stride + (int64_t)(p.g * a.G + h) * HD;
       }
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
@@ -280,16 +280,21 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           qf[k][e] = __ldcg(reinterpret_cast<const unsigned int*>(src[e & 1] + 16 * k + 8 * (e >> 1) + 2 * tl));
       }
     }
-    const int first_limit = pos0 + col0 / a.G, last_limit = pos0 + min((col0 + cols - 1) / a.G, n_new - 1);
-    float m[2] = {PG_NEG, PG_NEG}, l[2] = {0.0f, 0.0f}, o[HD / 8][4];
+    const int first_limit = pos0 + col0 / a.G, last_limit = pos0 + (col0 + n_cols - 1) / a.G;
+    m[0] = m[1] = PG_NEG;
+    l[0] = l[1] = 0.0f;
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    for (int i = (pl + lanes_of_pages - n0 % lanes_of_pages) % lanes_of_pages; i < u1 - u0; i += lanes_of_pages) {
-      const int n = n0 + i, st = s0 + n % stages;
-      if (ok) ok = pg_wait(sm.full + st, (n / stages) & 1);
-      const int key0 = sm.key0[st];
+    for (int u = p.u0; u < p.u1; ++u, ++n) {
+      const int st = n % PG_STAGES;
+      if (ok) ok = pg_wait(full + st, (n / PG_STAGES) & 1);
+      int key0 = key0s[0];
+#pragma unroll
+      for (int s = 1; s < PG_STAGES; ++s)
+        if (s == st) key0 = key0s[s];
       if (ok && key0 >= 0 && key0 <= last_limit) {
-        const uint32_t kb = k_addr + st * PG_UNIT_BYTES, vb = kb + PG_UNIT_BYTES / 2;
+        const unsigned char* vals = ring + st * PG_UNIT_BYTES + HALF;
+        const uint32_t kb = ring_addr + st * PG_UNIT_BYTES, vb = kb + HALF;
         // Values that a query does not see may be anything, and its probability of 0 would be multiplied with them.  Those that no query
         // of the item sees are taken as zeros; where one that some see is not finite, all that not everyone sees are added query by query.
         const bool edge = key0 + KS - 1 > first_limit;
@@ -299,7 +304,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int w = lane; w < KS * (HD / 8); w += 32) {
             const int key = w / (HD / 8), c = w % (HD / 8);
             if (key0 + key <= first_limit || key0 + key > last_limit) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(ring + st * PG_UNIT_BYTES + PG_UNIT_BYTES / 2 + (c / 8) * BOX + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+            const uint4 v = *reinterpret_cast<const uint4*>(vals + (c / 8) * BOX + key * 128 + (((c & 7) ^ (key & 7)) << 4));
             odd |= pg_odd(v.x) || pg_odd(v.y) || pg_odd(v.z) || pg_odd(v.w);
           }
           if (__any_sync(0xffffffffu, odd)) cut = first_limit;
@@ -354,14 +359,14 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int d = 0; d < HD / 8; ++d) { o[d][0] *= f[0]; o[d][1] *= f[0]; o[d][2] *= f[1]; o[d][3] *= f[1]; }
         }
         const float ref[2] = {m[0] == PG_NEG ? 0.0f : m[0], m[1] == PG_NEG ? 0.0f : m[1]};
-        uint32_t p[KS / 16][4];
+        uint32_t pr[KS / 16][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const float p0 = pg_exp2(s[j][0] - ref[0]), p1 = pg_exp2(s[j][1] - ref[0]), p2 = pg_exp2(s[j][2] - ref[1]), p3 = pg_exp2(s[j][3] - ref[1]);
           l[0] += p0 + p1;
           l[1] += p2 + p3;
-          p[j >> 1][2 * (j & 1)] = pg_pack(p0, p1);
-          p[j >> 1][2 * (j & 1) + 1] = pg_pack(p2, p3);
+          pr[j >> 1][2 * (j & 1)] = pg_pack(p0, p1);
+          pr[j >> 1][2 * (j & 1) + 1] = pg_pack(p2, p3);
         }
         auto values = [&](auto cutting) {
 #pragma unroll
@@ -376,8 +381,8 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int d2 = 0; d2 < KT; ++d2) {  // 16 features at a time
               uint32_t b[4];
               pg_ldsm_t(b, vb + (d2 >> 2) * BOX + (16 * k + (lane & 15)) * 128 + ((uint32_t)((2 * (d2 & 3) + (lane >> 4)) ^ sw) << 4));
-              pg_mma(o[2 * d2], p[k], b[0] & keep0, b[1] & keep1);
-              pg_mma(o[2 * d2 + 1], p[k], b[2] & keep0, b[3] & keep1);
+              pg_mma(o[2 * d2], pr[k], b[0] & keep0, b[1] & keep1);
+              pg_mma(o[2 * d2 + 1], pr[k], b[2] & keep0, b[3] & keep1);
             }
           }
         };
@@ -386,12 +391,12 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll 1
-            for (int u = 0; u < 8; ++u) {
-              const int key = 8 * j + u;
-              const uint32_t w0 = __shfl_sync(0xffffffffu, p[j >> 1][2 * (j & 1)], (lane & 28) + (u >> 1)), w1 = __shfl_sync(0xffffffffu, p[j >> 1][2 * (j & 1) + 1], (lane & 28) + (u >> 1));
+            for (int e = 0; e < 8; ++e) {
+              const int key = 8 * j + e;
+              const uint32_t w0 = __shfl_sync(0xffffffffu, pr[j >> 1][2 * (j & 1)], (lane & 28) + (e >> 1)), w1 = __shfl_sync(0xffffffffu, pr[j >> 1][2 * (j & 1) + 1], (lane & 28) + (e >> 1));
               if (key0 + key <= cut || key0 + key > last_limit) continue;
-              const float p0 = __uint_as_float(u & 1 ? w0 & 0xffff0000u : w0 << 16), p1 = __uint_as_float(u & 1 ? w1 & 0xffff0000u : w1 << 16);
-              const unsigned char* line = ring + st * PG_UNIT_BYTES + PG_UNIT_BYTES / 2 + key * 128 + 4 * tl;
+              const float p0 = __uint_as_float(e & 1 ? w0 & 0xffff0000u : w0 << 16), p1 = __uint_as_float(e & 1 ? w1 & 0xffff0000u : w1 << 16);
+              const unsigned char* line = vals + key * 128 + 4 * tl;
 #pragma unroll
               for (int d = 0; d < HD / 8; ++d) {
                 const uint32_t v = *reinterpret_cast<const uint32_t*>(line + (d >> 3) * BOX + (((d & 7) ^ (key & 7)) << 4));
@@ -402,116 +407,174 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
         }
       }
-      __syncwarp();
-      if (ok && lane == 0) tc5::mbar_arrive(sm.empty + st);            // (not after giving up: the copies end, too)
-      __syncwarp();
+      __syncwarp();                            // all lanes have read the stage
+      if (ok) ask_next();
     }
-    n0 += u1 - u0;
-    // ---- the team's sums, joined ------------------------------------------------------------------------------------------
+    x += p.u1 - p.u0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-      if (tl == 0) { sm.m[warp][gl + 8 * e] = m[e]; sm.l[warp][gl + 8 * e] = l[e]; }
     }
+    if (p.u0 == 0 && p.u1 == p.units) {
+      // ---- a whole item: out with it ------------------------------------------------------------------------------------------
+      const int grp = group_of(a.row0 + p.i);
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) {
-      *reinterpret_cast<float2*>(&sm.acc[warp][gl][8 * d + 2 * tl]) = make_float2(o[d][0], o[d][1]);
-      *reinterpret_cast<float2*>(&sm.acc[warp][gl + 8][8 * d + 2 * tl]) = make_float2(o[d][2], o[d][3]);
-    }
-    pg_bar(bar_id, bar_threads);
-    // the sum of column c and feature d over the team's warps of that column; tm and tsum: its maximum and sum
-    const int tid = tw * 32 + lane;
-    auto team_of = [&](int c, int d, float& tm, float& tsum) {
-      const int w0 = team * TS + c / 16, cc = c % 16;
-      tm = PG_NEG;
-      for (int i = 0; i < lanes_of_pages; ++i) tm = fmaxf(tm, sm.m[w0 + i * ncg][cc]);
-      const float safe = tm == PG_NEG ? 0.0f : tm;
-      float y = 0.0f;
-      tsum = 0.0f;
-      for (int i = 0; i < lanes_of_pages; ++i) {
-        const float f = pg_exp2(sm.m[w0 + i * ncg][cc] - safe);
-        tsum = fmaf(sm.l[w0 + i * ncg][cc], f, tsum);
-        y = fmaf(sm.acc[w0 + i * ncg][cc][d], f, y);
+      for (int e = 0; e < 2; ++e) {
+        const int c = gl + 8 * e;
+        if (c >= n_cols) continue;
+        const int tok = (col0 + c) / a.G, h = (col0 + c) - tok * a.G;
+        const int64_t th = (int64_t)(start + tok) * a.nh + p.g * a.G + h;
+        if (grp >= 0) {                        // its own pages' part, for the join with the shared ones'
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(a.own + th * HD + 8 * d + 2 * tl) = make_float2(o[d][2 * e], o[d][2 * e + 1]);
+          if (tl == 0) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * th) = make_float2(m[e], l[e]);
+        } else {
+          const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<uint32_t*>(a.out + th * HD + 8 * d + 2 * tl) = pg_pack(o[d][2 * e] * inv, o[d][2 * e + 1] * inv);
+        }
       }
-      return y;
+      __syncwarp();
+    } else if (x < i_hi) {
+      // ---- the first part, of an item that began in the share before: it waits until the ring is free ----------------------------------------
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) {
+        *reinterpret_cast<float2*>(spill + gl * HD + 8 * d + 2 * tl) = make_float2(o[d][0], o[d][1]);
+        *reinterpret_cast<float2*>(spill + (gl + 8) * HD + 8 * d + 2 * tl) = make_float2(o[d][2], o[d][3]);
+      }
+      m_first[0] = m[0]; m_first[1] = m[1]; l_first[0] = l[0]; l_first[1] = l[1];
+      have_first = true;
+      if (lane == 0) sm.part_at[warp][0] = p.base;
+    } else {
+      // ---- the last one -----------------------------------------------------------------------------------------------------------------
+      PgPart<HD>& part = reinterpret_cast<PgPart<HD>*>(ring)[1];
+      __syncwarp();
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) {
+        *reinterpret_cast<float2*>(&part.acc[gl][8 * d + 2 * tl]) = make_float2(o[d][0], o[d][1]);
+        *reinterpret_cast<float2*>(&part.acc[gl + 8][8 * d + 2 * tl]) = make_float2(o[d][2], o[d][3]);
+      }
+      if (tl == 0) { part.m[gl] = m[0]; part.m[gl + 8] = m[1]; part.l[gl] = l[0]; part.l[gl + 8] = l[1]; }
+      if (lane == 0) sm.part_at[warp][1] = p.base;
+    }
+  }
+  if (!ok) {                                   // what was asked for must land before the block's shared memory goes away
+    if (lane == 0) atomicExch(&g_pg_error, 1);
+    for (int u = max(0, ask_n - PG_STAGES); u < ask_n; ++u) pg_wait(full + u % PG_STAGES, (u / PG_STAGES) & 1);
+  }
+  if (have_first) {
+    PgPart<HD>& part = reinterpret_cast<PgPart<HD>*>(ring)[0];
+    __syncwarp();
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d) {         // (each thread its own)
+      *reinterpret_cast<float2*>(&part.acc[gl][8 * d + 2 * tl]) = *reinterpret_cast<const float2*>(spill + gl * HD + 8 * d + 2 * tl);
+      *reinterpret_cast<float2*>(&part.acc[gl + 8][8 * d + 2 * tl]) = *reinterpret_cast<const float2*>(spill + (gl + 8) * HD + 8 * d + 2 * tl);
+    }
+    if (tl == 0) { part.m[gl] = m_first[0]; part.m[gl + 8] = m_first[1]; part.l[gl] = l_first[0]; part.l[gl + 8] = l_first[1]; }
+  }
+  __syncthreads();
+
+  // ---- parts of items that shares cut, joined by all threads ------------------------------------------------------------------------------
+  auto parts = [&](int k) -> const PgPart<HD>& { return reinterpret_cast<const PgPart<HD>*>(rings + (k >> 1) * PG_RING)[k & 1]; };
+  constexpr int REC = PG_COLS * (HD + 2);
+  float* const records = a.records + (int64_t)gridDim.x * PG_WARPS * (PG_COLS * HD);
+  auto block_begin = [&](int b) { return begin(b * PG_WARPS); };
+  // a block's part of an item that began before the block, or with it, and the one that goes on in the next block
+  auto record = [&](int b, int64_t base) { return records + (2 * (int64_t)b + (block_begin(b) < base ? 1 : 0)) * REC; };
+  auto write = [&](const Place& p, int i, float mm, float ll, float y) {
+    const int c = p.b * PG_COLS + i / HD, tok = c / a.G, d = i % HD;
+    const int64_t th = (int64_t)(sm.start[p.i] + tok) * a.nh + p.g * a.G + c - tok * a.G;
+    if (group_of(a.row0 + p.i) >= 0) {
+      a.own[th * HD + d] = y;
+      if (d == 0) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * th) = make_float2(mm, ll);
+    } else {
+      a.out[th * HD + d] = __float2bfloat16_rn(ll == 0.0f ? 0.0f : y / ll);
+    }
+  };
+  int64_t edge_at[2] = {-1, -1};               // the items that go beyond the block: the first run's, the last run's
+  for (int k0 = 0; k0 < 2 * PG_WARPS;) {
+    const int64_t at = sm.part_at[k0 >> 1][k0 & 1];
+    int k1 = k0 + 1;
+    if (at < 0) { k0 = k1; continue; }
+    while (k1 < 2 * PG_WARPS && (sm.part_at[k1 >> 1][k1 & 1] == at || sm.part_at[k1 >> 1][k1 & 1] < 0)) ++k1;      // (a warp without a part there is between)
+    const Place p = place_of(at, at + 1);
+    const bool whole = at >= block_begin(blockIdx.x) && at + p.units <= block_begin(blockIdx.x + 1);
+    if (!whole) edge_at[at < block_begin(blockIdx.x) || at == block_begin(blockIdx.x) ? 0 : 1] = at;
+    const int n_cols = min(PG_COLS, sm.n_new[p.i] * a.G - p.b * PG_COLS);
+    for (int i = threadIdx.x; i < n_cols * HD; i += PG_WARPS * 32) {
+      const int c = i / HD, d = i % HD;
+      float mm = PG_NEG, ll = 0.0f, y = 0.0f;
+      for (int k = k0; k < k1; ++k)
+        if (sm.part_at[k >> 1][k & 1] == at) mm = fmaxf(mm, parts(k).m[c]);
+      const float safe = mm == PG_NEG ? 0.0f : mm;
+      for (int k = k0; k < k1; ++k) {
+        if (sm.part_at[k >> 1][k & 1] != at) continue;
+        const float f = pg_exp2(parts(k).m[c] - safe);
+        ll = fmaf(parts(k).l[c], f, ll);
+        y = fmaf(parts(k).acc[c][d], f, y);
+      }
+      if (whole) {
+        write(p, i, mm, ll, y);
+      } else {
+        float* r = record(blockIdx.x, at);
+        r[2 * PG_COLS + i] = y;
+        if (d == 0) { r[c] = mm; r[PG_COLS + c] = ll; }
+      }
+    }
+    k0 = k1;
+  }
+  // ---- items that blocks cut: the last of their blocks to report joins them ------------------------------------------------------------------
+  if (edge_at[0] >= 0 || edge_at[1] >= 0) {
+    auto block_of = [&](int64_t x) {
+      int b = (int)(x * n_blocks / total);
+      while (b > 0 && block_begin(b) > x) --b;
+      while (b + 1 < n_blocks && block_begin(b + 1) <= x) ++b;
+      return b;
     };
-    auto out_at = [&](int c, int d) {
-      const int cc = col0 + c;
-      return a.out + ((int64_t)(start + cc / a.G) * a.nh + g * a.G + cc % a.G) * HD + d;
-    };
-    // the shared pages' parts of a row's queries
-    const int grp = LIST ? -1 : group_of(row);
-    const int64_t base = item_base + (int64_t)g * units;
-    const bool whole = u0 == 0 && u1 == units;
-    const int64_t rec = (int64_t)cols * (HD + 2);
-    // a team's part of an item that began in the share before, or with this share, and the one that goes on in the next share
-    auto record = [&](int t) { return a.records + (2 * (int64_t)t + (begin(t) < base ? 1 : 0)) * rec; };
-    int ta = 0, tb = -1;                         // teams whose records are joined
-    if (!whole) {
-      float* dst = record(my);
-      for (int i = tid; i < n_cols * HD; i += TS * 32) {
-        float tm, ts;
-        const float y = team_of(i / HD, i % HD, tm, ts);
-        dst[2 * cols + i] = y;
-        if (i % HD == 0) { dst[i / HD] = tm; dst[cols + i / HD] = ts; }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      const int64_t at = edge_at[threadIdx.x];
+      bool last = false;
+      if (at >= 0) {
+        const int ba = block_of(at), bb = block_of(at + place_of(at, at + 1).units - 1);
+        last = atomicAdd(a.counters + ba, 1) == bb - ba;             // (of the items that begin in a block only one goes beyond it)
+        if (last) a.counters[ba] = 0;
       }
       __threadfence();
-      pg_bar(bar_id, bar_threads);
-      ta = (int)(base * n_teams / total), tb = (int)((base + units - 1) * n_teams / total);
-      while (ta > 0 && begin(ta) > base) --ta;
-      while (ta + 1 < n_teams && begin(ta + 1) <= base) ++ta;
-      while (tb > 0 && begin(tb) > base + units - 1) --tb;
-      while (tb + 1 < n_teams && begin(tb + 1) <= base + units - 1) ++tb;
-      if (tid == 0) {
-        int* counter = a.counters + it * a.nkv + g;
-        const bool last = atomicAdd(counter, 1) == tb - ta;
-        if (last) *counter = 0;
-        __threadfence();
-        sm.flag[team] = last;
-      }
-      pg_bar(bar_id, bar_threads);
+      sm.last[threadIdx.x] = last;
     }
-    if (whole || sm.flag[team]) {
-      if (grp >= 0) pdl_wait();
-      for (int i = tid; i < n_cols * HD; i += TS * 32) {
-        const int c = i / HD, d = i % HD;
+    __syncthreads();
+    for (int e = 0; e < 2; ++e) {
+      if (!sm.last[e]) continue;
+      const int64_t at = edge_at[e];
+      const Place p = place_of(at, at + 1);
+      const int ba = block_of(at), bb = block_of(at + p.units - 1);
+      const int n_cols = min(PG_COLS, sm.n_new[p.i] * a.G - p.b * PG_COLS);
+      for (int i = threadIdx.x; i < n_cols * HD; i += PG_WARPS * 32) {
+        const int c = i / HD;
         float mm = PG_NEG, ll = 0.0f, y = 0.0f;
-        if (whole) y = team_of(c, d, mm, ll);
-        auto add = [&](float m1, float l1, float y1) {
+#pragma unroll 8
+        for (int b = ba; b <= bb; ++b) {
+          const float* r = record(b, at);
+          const float m1 = __ldcg(r + c), l1 = __ldcg(r + PG_COLS + c), y1 = __ldcg(r + 2 * PG_COLS + i);
           const float top = fmaxf(mm, m1), safe = top == PG_NEG ? 0.0f : top;
           const float f0 = pg_exp2(mm - safe), f1 = pg_exp2(m1 - safe);
           ll = ll * f0 + l1 * f1;
           y = y * f0 + y1 * f1;
           mm = top;
-        };
-#pragma unroll 4
-        for (int t = ta; t <= tb; ++t) {
-          const float* p = record(t);
-          add(__ldcg(p + c), __ldcg(p + cols + c), __ldcg(p + 2 * cols + i));
         }
-        if (grp >= 0) {
-          const int query = (start + (col0 + c) / a.G - sm.plan.tok0[grp]) * a.G + (col0 + c) % a.G, tile = query / PS_TILE, qr = query % PS_TILE;
-          const int64_t first = sm.plan.work_before[grp] * a.nkv + ((int64_t)g * sm.plan.tiles(grp) + tile) * sm.plan.pages[grp];
-          const int ba = sm.plan.block_of(first), bb = sm.plan.block_of(first + sm.plan.pages[grp] - 1);
-#pragma unroll 4
-          for (int b = ba; b <= bb; ++b) {
-            const float* p = a.ps_records + ps_slot(sm.plan, a.nkv, grp, g, tile, b) * ps_record(HD);
-            add(__ldcg(p + qr), __ldcg(p + PS_TILE + qr), __ldcg(p + ps_value(qr, d)));
-          }
-        }
-        *out_at(c, d) = __float2bfloat16_rn(ll == 0.0f ? 0.0f : y / ll);
+        write(p, i, mm, ll, y);
       }
     }
-    pg_bar(bar_id, bar_threads);
-    x += u1 - u0;
   }
-  if (!ok && lane == 0) atomicExch(&g_pg_error, 2);
-  __syncthreads();
   if (!a.wait_first) pdl_wait();               // this kernel's end is then the shared pages' kernel's end, too
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
+
+constexpr int PG_SMEM = (int)(PG_SMEM_RINGS + sizeof(PgSmem) + 1024);
 
 int pg_sms(const char* what) {                 // of the current device, 0: an error
   static int known[64] = {};
@@ -519,30 +582,30 @@ int pg_sms(const char* what) {                 // of the current device, 0: an e
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("%s: no device", what); return 0; }
   if (known[dev]) return known[dev];
   cudaError_t e = cudaSuccess;
-  const int s64 = (int)(PG_SMEM_RING + sizeof(PgSmem<64>) + 1024), s128 = (int)(PG_SMEM_RING + sizeof(PgSmem<128>) + 1024);
-  for (auto f : {(const void*)attn_pages_kernel<64, false>, (const void*)attn_pages_kernel<64, true>})
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, s64);
-  for (auto f : {(const void*)attn_pages_kernel<128, false>, (const void*)attn_pages_kernel<128, true>})
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, s128);
+  for (auto f : {(const void*)attn_pages_kernel<64, false>, (const void*)attn_pages_kernel<64, true>, (const void*)attn_pages_kernel<128, false>, (const void*)attn_pages_kernel<128, true>})
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, PG_SMEM);
   if (e == cudaSuccess) e = attn_shared_prepare();
   int sms = 0;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess || sms < 1) { set_error("%s: cannot get %d bytes of shared memory: %s", what, s128, cudaGetErrorString(e)); return 0; }
+  if (e != cudaSuccess || sms < 1) { set_error("%s: cannot get %d bytes of shared memory: %s", what, PG_SMEM, cudaGetErrorString(e)); return 0; }
   return known[dev] = sms;
 }
 
-static int64_t pg_record_floats(int sms, int hd) { return 2ll * sms * PG_MAX_COLS * (hd + 2); }
-static int64_t ps_slots(int sms, int64_t T, int G, int nkv, int n_groups) { return n_groups ? sms + nkv * ((int64_t)T * G / PS_TILE + n_groups) : 0; }
+// Where the warps' first parts wait, and the blocks' parts.
+static int64_t pg_record_floats(int sms, int hd) { return (int64_t)sms * (PG_WARPS * PG_COLS * hd + 2 * PG_COLS * (hd + 2)); }
+// With groups: the plan, the parts of shared pages, the rows' own parts.
+constexpr int64_t PS_PLAN_FLOATS = (sizeof(PsPlan) + 63) / 64 * 16;
+static int64_t ps_slots(int sms, int64_t T, int G, int nkv, int n_groups) { return sms + nkv * (T * G / PS_TILE + n_groups); }
+static int64_t ps_floats(int sms, int64_t T, int G, int nkv, int hd, int n_groups) {
+  return n_groups ? PS_PLAN_FLOATS + ps_slots(sms, T, G, nkv, n_groups) * ps_record(hd) + ps_own(T, G * nkv, hd) : 0;
+}
 
-template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int most_cols, int sms, const char* what, cudaStream_t stream) {
-  a.groups_of_cols = most_cols <= 16 ? 1 : most_cols <= 32 ? 2 : 4;
-  const int cols = 16 * a.groups_of_cols;
-  const int64_t items = LIST ? (int64_t)a.rows * ceil_div(a.G, cols) : std::min((int64_t)a.T * a.G, (int64_t)a.T * a.G / cols + a.rows);
-  for (int64_t i0 = 0; i0 < items; i0 += PG_WINDOW) {
-    a.item0 = (int)i0;
-    a.wait_first = i0 > 0 || a.n_groups == 0;
-    if (hd == 64) launch_pdl(attn_pages_kernel<64, LIST>, dim3(sms), dim3(2 * PG_WARPS * 32), PG_SMEM_RING + sizeof(PgSmem<64>) + 1024, stream, map_k, map_v, a);
-    else launch_pdl(attn_pages_kernel<128, LIST>, dim3(sms), dim3(2 * PG_WARPS * 32), PG_SMEM_RING + sizeof(PgSmem<128>) + 1024, stream, map_k, map_v, a);
+template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int sms, const char* what, cudaStream_t stream) {
+  for (int r0 = 0; r0 < a.rows; r0 += PG_WINDOW) {
+    a.row0 = r0;
+    a.wait_first = r0 > 0 || a.n_groups == 0;
+    auto go = [&](auto kernel) { launch_pdl(kernel, dim3(sms), dim3(PG_WARPS * 32), PG_SMEM, stream, map_k, map_v, a); };
+    if (hd == 64) go(attn_pages_kernel<64, LIST>); else go(attn_pages_kernel<128, LIST>);
     const int rc = launch_status(what);
     if (rc) return rc;
   }
@@ -552,10 +615,10 @@ template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, co
 // What both entry points ask of their arguments, and the pools' maps.
 static int pg_check(const char* what, const void* q, int64_t q_stride, const void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table,
                     int bt_width, int rows, int T, int nh, int nkv, int hd, float scale, CUtensorMap* map_k, CUtensorMap* map_v) {
-  if (rows < 0 || T < 0 || nkv < 1 || nkv > PG_COUNTERS / PG_WINDOW || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || !(scale > 0.0f) || !isfinite(scale) || n_pages < 1 ||
-      (n_pages + 1) * nkv * PG_PAGE > INT32_MAX || bt_width < 1 || bt_width > PG_MAX_WIDTH || (int64_t)T * (nh / nkv) > INT32_MAX - PG_MAX_COLS) {
-    set_error("%s: needs heads of 64 or 128, at most %d key/value heads, a positive scale, tables of at most %d pages and pools of fewer than 2^31 tokens times key/value heads, got %d rows, %d tokens, %d "
-              "heads on %d of %d, scale %g, %lld pages, a table of %d", what, PG_COUNTERS / PG_WINDOW, PG_MAX_WIDTH, rows, T, nh, nkv, hd, (double)scale, (long long)n_pages, bt_width);
+  if (rows < 0 || T < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || !(scale > 0.0f) || !isfinite(scale) || n_pages < 1 ||
+      (n_pages + 1) * nkv * PG_PAGE > INT32_MAX || bt_width < 1 || bt_width > PG_MAX_WIDTH || (int64_t)T * (nh / nkv) > INT32_MAX - PG_COLS) {
+    set_error("%s: needs heads of 64 or 128, a positive scale, tables of at most %d pages and pools of fewer than 2^31 tokens times key/value heads, got %d rows, %d tokens, %d "
+              "heads on %d of %d, scale %g, %lld pages, a table of %d", what, PG_MAX_WIDTH, rows, T, nh, nkv, hd, (double)scale, (long long)n_pages, bt_width);
     return ERR_BAD_ARGUMENT;
   }
   if (!q || !out || !k_pool || !v_pool || !block_table) { set_error("%s: an array is missing", what); return ERR_BAD_ARGUMENT; }
@@ -563,7 +626,7 @@ static int pg_check(const char* what, const void* q, int64_t q_stride, const voi
     set_error("%s: q, its rows, out and the pools must be 16-byte aligned", what);
     return ERR_ALIGNMENT;
   }
-  const int box = hd == 64 ? 64 : 32;
+  const int box = hd == 64 ? 32 : 16;
   int rc = tc5::make_map_k64(map_k, k_pool, n_pages * nkv * PG_PAGE, hd, box, what);
   return rc ? rc : tc5::make_map_k64(map_v, v_pool, n_pages * nkv * PG_PAGE, hd, box, what);
 }
@@ -591,7 +654,7 @@ extern "C" int exl3_attn_pages_status() {
 // Floats of scratch that a call with these sizes wants; the first PG_COUNTERS must be zero before the first call and are zero after each.
 extern "C" long long exl3_attn_pages_scratch(int sms, int T, int nh, int nkv, int hd, int n_groups) {
   if (nkv < 1) return 0;
-  return PG_COUNTERS + pg_record_floats(sms, hd) + ps_slots(sms, T, nh / nkv, nkv, n_groups) * ps_record(hd);
+  return PG_COUNTERS + pg_record_floats(sms, hd) + ps_floats(sms, T, nh / nkv, nkv, hd, n_groups);
 }
 
 // Attention of each token over the pages that lists[token][kv head][count] names.
@@ -609,7 +672,7 @@ extern "C" int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, T, T, nh, nkv, scale, scratch);
   a.tok_pos = tok_pos; a.tok_seq = tok_seq; a.lists = lists; a.count = std::min(count, bt_width);
   a.list_stride = count; a.bt_rows = bt_rows;
-  return pg_launch<true>(a, map_k, map_v, hd, a.G, sms, "attn_pages", stream);
+  return pg_launch<true>(a, map_k, map_v, hd, sms, "attn_pages", stream);
 }
 
 // Causal attention of rows whose groups share their first pages (groups: int32 [n_groups, 3]: first row, rows, pages).
@@ -629,14 +692,16 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
   if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, nh, nkv, hd, n_groups)) { set_error("attn_shared: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, rows, T, nh, nkv, scale, scratch);
   a.row_start = row_start; a.row_pos0 = row_pos0; a.bt_rows = rows; a.groups = groups; a.n_groups = n_groups; a.ps_grid = sms;
-  float* ps = scratch + PG_COUNTERS + pg_record_floats(sms, hd);
-  a.ps_records = ps;
+  PsPlan* plan = reinterpret_cast<PsPlan*>(scratch + PG_COUNTERS + pg_record_floats(sms, hd));
+  float* parts = reinterpret_cast<float*>(plan) + PS_PLAN_FLOATS;
+  a.own = parts + (n_groups ? ps_slots(sms, T, a.G, nkv, n_groups) * ps_record(hd) : 0);
   if (n_groups) {
     PsArgs p = {};
     p.q = a.q; p.q_stride = q_stride; p.block_table = block_table; p.bt_stride = bt_stride; p.bt_width = bt_width; p.n_pages = (int)n_pages; p.row_start = row_start;
-    p.row_pos0 = row_pos0; p.rows = rows; p.T = T; p.nkv = nkv; p.G = a.G; p.groups = groups; p.n_groups = n_groups; p.scale_log2 = a.scale_log2; p.records = ps;
+    p.row_pos0 = row_pos0; p.rows = rows; p.T = T; p.nkv = nkv; p.G = a.G; p.groups = groups; p.n_groups = n_groups; p.scale_log2 = a.scale_log2; p.records = parts; p.plan = plan;
     rc = attn_shared_launch(p, k_pool, v_pool, hd, sms, stream);
     if (rc) return rc;
   }
-  return pg_launch<false>(a, map_k, map_v, hd, (int)std::min((int64_t)max_new * a.G, (int64_t)PG_MAX_COLS), sms, "attn_shared", stream);
+  rc = pg_launch<false>(a, map_k, map_v, hd, sms, "attn_shared", stream);
+  return rc || !n_groups ? rc : attn_shared_join(plan, parts, a.own, a.out, T, nh, nkv, hd, stream);
 }

@@ -98,10 +98,8 @@ __device__ inline PsPart ps_part(const PsPlan& p, int nkv, int64_t x, int64_t en
 __device__ inline int ps_slot(const PsPlan& p, int nkv, int j, int g, int tile, int b) {
   return b + p.tiles_before[j] * nkv + g * p.tiles(j) + tile;
 }
-// A record, in floats: the queries' maxima (base-2 units), their sums, their sums of values as [hd / 4][query][4], so that neighbouring
-// queries' stores are neighbours.
+// A record, in floats: the queries' maxima (base-2 units), their sums, their sums of values [query][hd].
 __host__ __device__ constexpr int64_t ps_record(int hd) { return (int64_t)PS_TILE * (hd + 2); }
-__device__ inline int ps_value(int query, int d) { return 2 * PS_TILE + ((d >> 2) * PS_TILE + query) * 4 + (d & 3); }
 
 // The kernel over the shared pages (attention_shared.cu): one record for every part of a tile that a block works on.
 struct PsArgs {
@@ -116,8 +114,12 @@ struct PsArgs {
   int n_groups;
   float scale_log2;
   float* records;
+  PsPlan* plan;                                // left for the join
 };
+// What the join of a query's parts needs beside the records: its row's own pages' part, sums of values [token][head][hd], then (maximum, sum) [token][head].
+__host__ __device__ constexpr int64_t ps_own(int64_t T, int nh, int hd) { return T * nh * (hd + 2); }
 cudaError_t attn_shared_prepare();             // once for a device
+int attn_shared_join(const PsPlan* plan, const float* records, const float* own, __nv_bfloat16* out, int T, int nh, int nkv, int hd, cudaStream_t stream);
 int attn_shared_launch(const PsArgs& a, const void* k_pool, const void* v_pool, int hd, int sms, cudaStream_t stream);
 
 }  // namespace exl3

@@ -108,6 +108,11 @@ __device__ inline void ps_exponentials(const uint32_t (&s)[32], float mul, float
     p[c] = ps_pack(e0, e1);
   }
 }
+// 32 bytes: a whole sector of a line, where each lane has a row of its own.
+__device__ inline void ps_store8(float* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 // This thread's row of O times f.
 template <int HD> __device__ inline void ps_rescale(uint32_t taddr, float f) {
 #pragma unroll
@@ -158,6 +163,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   pdl_wait();
   pdl_trigger();
   ps_plan(plan, a.groups, a.n_groups, a.row_start, a.rows, a.T, a.G, a.nkv, a.bt_width, gridDim.x);
+  if (blockIdx.x == 0)                         // (for the join)
+    for (int i = threadIdx.x; i < (int)(sizeof(PsPlan) / 4); i += PS_THREADS) reinterpret_cast<int*>(a.plan)[i] = reinterpret_cast<const int*>(&plan)[i];
   const uint32_t tmem = *tmem_slot;            // columns: scores of set s at 128 s, O at 256 + 128 s
   const int64_t lo = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x) : 0, hi = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x + 1) : 0;
   auto sets_of = [&](const PsPart& t) { return plan.queries[t.j] - t.tile * PS_TILE > 128 ? 2 : 1; };
@@ -348,8 +355,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         tmem_ld32(to + 32 * h, s0);
         if (in) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            *reinterpret_cast<uint4*>(rec + ps_value(qr, 32 * h + c)) = make_uint4(s0[c], s0[c + 1], s0[c + 2], s0[c + 3]);
+          for (int c = 0; c < 32; c += 8) ps_store8(rec + 2 * PS_TILE + (int64_t)qr * HD + 32 * h + c, s0 + c);
         }
       }
       __syncwarp();
@@ -361,6 +367,77 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   __syncthreads();
   fence_after();
   if (warp == 8) tmem_free<512>(tmem);
+}
+
+// Joins the parts of a query: a warp for each (token, head).  The parts of the shared pages are in the order of the pages, the own pages' part is the last, so
+// a result does not depend on which block was the first to end.
+constexpr int PJ_WARPS = 4;
+template <int HD>
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+attn_shared_join_kernel(const PsPlan* __restrict__ plan, const float* __restrict__ records, const float* __restrict__ own, __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
+  constexpr int V = HD / 32;                   // features a lane
+  __shared__ float s_w[PJ_WARPS][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t th = (int64_t)blockIdx.x * PJ_WARPS + warp;
+  pdl_trigger();
+  pdl_wait();
+  if (th >= (int64_t)T * nh) return;
+  const int tok = (int)(th / nh), head = (int)(th % nh), G = nh / nkv, g = head / G;
+  int lo = 0, hi = __ldcg(&plan->n) - 1;
+  while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (__ldcg(&plan->tok0[mid]) <= tok) lo = mid; else hi = mid - 1; }
+  const int query = (tok - __ldcg(&plan->tok0[lo])) * G + head % G, queries = __ldcg(&plan->queries[lo]), pages = __ldcg(&plan->pages[lo]);
+  if (query < 0 || query >= queries || pages == 0) return;             // in no group: its own pages' part was all
+  const int tile = query / PS_TILE, qr = query % PS_TILE, tiles = (queries + PS_TILE - 1) / PS_TILE, blocks = __ldcg(&plan->blocks);
+  const int64_t total = __ldcg(&plan->total), first = __ldcg(&plan->work_before[lo]) * nkv + ((int64_t)g * tiles + tile) * pages;
+  const int slot0 = __ldcg(&plan->tiles_before[lo]) * nkv + g * tiles + tile;
+  auto block_of = [&](int64_t x) {
+    int b = (int)(x * blocks / total);
+    while (b + 1 < blocks && total * (b + 1) / blocks <= x) ++b;
+    while (b > 0 && total * b / blocks > x) --b;
+    return b;
+  };
+  const int b0 = block_of(first), n = block_of(first + pages - 1) - b0 + 1;           // parts (at most as many as there are SMs)
+  const float* rec0 = records + (slot0 + b0) * ps_record(HD) + qr;
+  const float* mine = own + (int64_t)T * nh * HD + 2 * th;
+  float mm = -INFINITY;
+  for (int i = lane; i <= n; i += 32) mm = fmaxf(mm, __ldcg(i < n ? rec0 + i * ps_record(HD) : mine));
+  mm = warp_max(mm);
+  const float safe = mm == -INFINITY ? 0.0f : mm;
+  float l = 0.0f;
+  for (int i = lane; i <= n; i += 32) {
+    const float f = ps_exp2(__ldcg(i < n ? rec0 + i * ps_record(HD) : mine) - safe);
+    s_w[warp][i] = f;
+    l = fmaf(f, __ldcg(i < n ? rec0 + PS_TILE + i * ps_record(HD) : mine + 1), l);
+  }
+  l = warp_sum(l);
+  __syncwarp();
+  const float* y0 = rec0 - qr + 2 * PS_TILE + (int64_t)qr * HD + lane * V;
+  float y[V] = {};
+  auto add = [&](const float* p, float f) {
+    if (V == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+      y[0] = fmaf(f, v.x, y[0]); y[1] = fmaf(f, v.y, y[1]); y[V - 2] = fmaf(f, v.z, y[V - 2]); y[V - 1] = fmaf(f, v.w, y[V - 1]);
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
+      y[0] = fmaf(f, v.x, y[0]); y[1] = fmaf(f, v.y, y[1]);
+    }
+  };
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) add(y0 + i * ps_record(HD), s_w[warp][i]);
+  add(own + th * HD + lane * V, s_w[warp][n]);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint32_t w[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) w[i] = ps_pack(y[2 * i] * inv, y[2 * i + 1] * inv);
+  if (V == 4) *reinterpret_cast<uint2*>(out + th * HD + lane * V) = make_uint2(w[0], w[V / 2 - 1]);
+  else *reinterpret_cast<uint32_t*>(out + th * HD + lane * V) = w[0];
+}
+
+int attn_shared_join(const PsPlan* plan, const float* records, const float* own, __nv_bfloat16* out, int T, int nh, int nkv, int hd, cudaStream_t stream) {
+  const dim3 grid((unsigned)(((int64_t)T * nh + PJ_WARPS - 1) / PJ_WARPS)), block(PJ_WARPS * 32);
+  if (hd == 64) launch_pdl(attn_shared_join_kernel<64>, grid, block, 0, stream, plan, records, own, out, T, nh, nkv);
+  else launch_pdl(attn_shared_join_kernel<128>, grid, block, 0, stream, plan, records, own, out, T, nh, nkv);
+  return launch_status("attn_shared join");
 }
 
 cudaError_t attn_shared_prepare() {
