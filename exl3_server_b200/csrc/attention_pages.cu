@@ -15,15 +15,15 @@
 
 namespace exl3 {
 
-constexpr int PG_WARPS = 8;                    // of a block, one block an SM
+constexpr int PG_WARPS = 4;                    // of a block, one block an SM
 constexpr int PG_STAGES = 3;                   // of a warp's ring
-constexpr int PG_UNIT_BYTES = 8192;            // a unit: keys and values of 32 tokens (heads of 64) or 16 (heads of 128)
-constexpr int PG_COLS = 16;                    // queries of an item
+constexpr int PG_UNIT_BYTES = 16384;           // a unit: keys and values of 64 tokens (heads of 64) or 32 (heads of 128)
 constexpr int PG_WINDOW = 1024;                // rows of a launch
-constexpr int PG_MIN_UNITS = 4;                // of a warp's share, at least
+constexpr int PG_MIN_UNITS = 2;                // of a warp's share, at least
 constexpr int PG_MAX_WIDTH = 1 << 19;          // pages of a row
 constexpr int PG_RING = PG_STAGES * PG_UNIT_BYTES;
 constexpr uint32_t PG_SMEM_RINGS = PG_WARPS * PG_RING;
+constexpr int PG_MAX_COLS = 16;                // queries of an item
 
 static __device__ int g_pg_error = 0;
 
@@ -61,6 +61,12 @@ __device__ inline void pg_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// An 8 x 8 matrix of 16-bit elements, a pair to a lane, transposed across the warp.
+__device__ inline uint32_t pg_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ inline float pg_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -73,17 +79,40 @@ __device__ inline uint32_t pg_pack(float lo, float hi) {
 }
 // Whether one of a word's two bfloat16 is not finite.
 __device__ inline bool pg_odd(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
-// Bounded, and one answer for the warp.
-__device__ inline bool pg_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tc5::mbar_wait(bar, parity)); }
+template <int V> __device__ inline void pg_store(float* p, const float (&y)[V]) {
+  if (V == 4) *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[V - 2], y[V - 1]);
+  else *reinterpret_cast<float2*>(p) = make_float2(y[0], y[1]);
+}
+template <int V> __device__ inline void pg_load(const float* p, float (&y)[V]) {
+  if (V == 4) { const float4 v = __ldcg(reinterpret_cast<const float4*>(p)); y[0] = v.x; y[1] = v.y; y[V - 2] = v.z; y[V - 1] = v.w; }
+  else { const float2 v = __ldcg(reinterpret_cast<const float2*>(p)); y[0] = v.x; y[1] = v.y; }
+}
+// Bounded, and one answer for the warp.  The hardware may hold a look for a while.
+__device__ inline bool pg_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = tc5::smem_u32(bar);
+  uint32_t there = 0;
+  for (uint32_t i = 0; i < tc5::WAIT_LIMIT && !there; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(there) : "r"(addr), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, there);
+}
 
 constexpr float PG_NEG = -INFINITY;
 
 // A warp's part of an item, at the start of its ring when the ring is done with: two of them at most, of the item that its share begins in and
 // of the one that it ends in.
-template <int HD> struct PgPart {
-  float m[PG_COLS], l[PG_COLS], acc[PG_COLS][HD];
+template <int HD, int COLS> struct PgPart {
+  float m[COLS], l[COLS], acc[COLS][HD];
 };
+// An item, and where in it a share is.
+struct PgPlace { int i, g, b, u0, u1, units; int64_t base; };
+struct PgRun { PgPlace p; int k0, k1; bool whole, own; };
 struct PgSmem {
+  PgRun run[2 * PG_WARPS];
+  int n_runs, edge[2];
   uint64_t full[PG_WARPS][PG_STAGES];
   int64_t cum[PG_WINDOW + 1];                  // units of the rows before
   int start[PG_WINDOW], n_new[PG_WINDOW], pos[PG_WINDOW], units[PG_WINDOW];
@@ -93,20 +122,24 @@ struct PgSmem {
   PsPlan plan;
 };
 
-// Items: up to PG_COLS queries (token, query head) of a row (or of a listed token) and key/value head, which walk the same pages.  The units of all items, ordered by row, head and
+// Keys are the rows of the first product and queries its columns, S^T = K Q^T (8 columns an instruction; NC of them side by side), and the second is O^T = V^T P^T: half
+// the instructions that queries as 16 rows would take for up to 8 of them.
+//
+// Items: up to 8 NC queries (token, query head) of a row (or of a listed token) and key/value head, which walk the same pages.  The units of all items, ordered by row, head and
 // item, are cut into equal shares for the warps, which stream them through rings of their own, each asking for its own copies: nothing is waited for but
 // memory.  What a warp has whole it writes out; parts of items that shares cut are joined in shared memory at the end, and those that blocks cut by the block that
 // is the last to report, always in the order of the pages, so that results do not depend on which it was.
-template <int HD, bool LIST>
+template <int HD, int NC, bool LIST>
 __global__ void __launch_bounds__(PG_WARPS * 32, 1)
 attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PgArgs a) {
-  constexpr int KS = HD == 64 ? 32 : 16;       // keys of a unit
+  constexpr int COLS = 8 * NC;
+  constexpr int KS = HD == 64 ? 64 : 32;       // keys of a unit
   constexpr int UPP = PG_PAGE / KS;            // units of a page
-  constexpr int NT = KS / 8;                   // tiles of 8 keys
+  constexpr int MT = KS / 16;                  // tiles of 16 keys
   constexpr int KT = HD / 16;                  // pieces of 16 features
   constexpr int BOX = KS * 128;                // bytes of a box of 64 features
   constexpr int HALF = PG_UNIT_BYTES / 2;      // keys, then values
-  static_assert(2 * sizeof(PgPart<HD>) <= PG_RING, "a warp's parts fit into its ring");
+  static_assert(2 * sizeof(PgPart<HD, COLS>) <= PG_RING, "a warp's parts fit into its ring");
   extern __shared__ unsigned char pg_raw[];
   unsigned char* rings = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pg_raw) + 1023) & ~(uintptr_t)1023);
   PgSmem& sm = *reinterpret_cast<PgSmem*>(rings + PG_SMEM_RINGS);
@@ -140,7 +173,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     return row >= sm.plan.row[lo] && row < sm.plan.row[lo] + sm.plan.rows[lo] && sm.plan.pages[lo] > 0 ? lo : -1;
   };
   auto shared_of = [&](int row) { const int j = group_of(row); return j < 0 ? 0 : sm.plan.pages[j]; };     // pages that the row shares
-  auto blocks_of = [&](int i) { return (sm.n_new[i] * a.G + PG_COLS - 1) / PG_COLS; };                     // items of a row and head
+  auto blocks_of = [&](int i) { return (sm.n_new[i] * a.G + COLS - 1) / COLS; };                     // items of a row and head
   {
     int64_t run = 0;
     for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
@@ -175,12 +208,11 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
   auto begin = [&](int w) { return total * w / (n_blocks * PG_WARPS); };       // the first unit of a warp's share
   const int64_t i_lo = begin(blockIdx.x * PG_WARPS + warp), i_hi = begin(blockIdx.x * PG_WARPS + warp + 1);
-  // The item at place x, and where in it.
-  struct Place { int i, g, b, u0, u1, units; int64_t base; };
+  // The item at place x.
   auto place_of = [&](int64_t x, int64_t end) {
     int lo = 0, hi = n_rows - 1;
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (sm.cum[mid] <= x) lo = mid; else hi = mid - 1; }
-    Place p;
+    PgPlace p;
     p.i = lo;
     p.units = sm.units[lo];
     const int64_t r = x - sm.cum[lo];
@@ -197,7 +229,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   uint64_t* full = sm.full[warp];
   // ---- copies: page numbers come 32 at a time, a batch ahead -----------------------------------------------------------------
   int64_t ask_x = i_lo;                        // the next unit to ask for
-  Place ask = {};
+  PgPlace ask = {};
   int ask_u = 0, ask_n = 0, batch_p = 0;       // its number in the item; units asked for so far; the first page of the batch at hand
   int page = 0, logical = 0, page_next = 0, logical_next = 0;
   int key0s[PG_STAGES];                        // a stage's first key; below 0: its page is not there
@@ -250,51 +282,65 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   for (int s = 0; s < PG_STAGES; ++s) ask_next();
 
   // ---- computing ------------------------------------------------------------------------------------------------------------
-  const uint32_t ring_addr = tc5::smem_u32(ring), sw = lane & 7;
-  bool ok = true;
-  int n = 0;                                   // units done
-  if (lane == 0) sm.part_at[warp][0] = sm.part_at[warp][1] = -1;
-  float m_first[2], l_first[2];                // the first part's, until the ring is free
-  float m[2], l[2], o[HD / 8][4];
-  bool have_first = false;
-  float* const spill = a.records + ((int64_t)blockIdx.x * PG_WARPS + warp) * (PG_COLS * HD);   // (where the first part's sums wait meanwhile)
-  for (int64_t x = i_lo; x < i_hi;) {
-    const Place p = place_of(x, i_hi);
-    const int start = sm.start[p.i], n_new = sm.n_new[p.i], pos0 = sm.pos[p.i], col0 = p.b * PG_COLS;
-    const int n_cols = min(PG_COLS, n_new * a.G - col0);
-    // this thread's two queries: columns gl and gl + 8
-    int limit[2];
-    uint32_t qf[KT][4];
-    {
-      const __nv_bfloat16* src[2];
+  const uint32_t ring_addr = tc5::smem_u32(ring);
+  // ldmatrix: a row at 128 bytes, its 16-byte piece c at c ^ (row & 7)
+  const uint32_t k_row = ((lane & 7) + ((lane >> 3) & 1) * 8) * 128, v_row = ((lane & 7) + ((lane >> 4) & 1) * 8) * 128 + HALF;
+  uint32_t k_col[4], v_col[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = min(col0 + gl + 8 * e, n_new * a.G - 1), tok = c / a.G, h = c - tok * a.G;
-        limit[e] = pos0 + tok;                 // the last key it sees
-        src[e] = a.q + (int64_t)(start + tok) * a.q_stride + (int64_t)(p.g * a.G + h) * HD;
-      }
+  for (int j = 0; j < 4; ++j) {
+    k_col[j] = (uint32_t)(((2 * j + (lane >> 4)) ^ (lane & 7)) << 4);
+    v_col[j] = (uint32_t)(((2 * j + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+  }
+  bool ok = true;
+  int st = 0;                                  // the next unit's stage, and its phase
+  uint32_t phase = 0;
+  if (lane == 0) sm.part_at[warp][0] = sm.part_at[warp][1] = -1;
+  float m_first[NC][2], l_first[NC][2];        // the first part's, until the ring is free
+  float m[NC][2], l[NC][2], o[KT][NC][4];
+  bool have_first = false;
+  float* const spill = a.records + ((int64_t)blockIdx.x * PG_WARPS + warp) * (PG_MAX_COLS * HD);   // (where the first part's sums wait meanwhile)
+  // the item's query of column 8 nc + gl as the operand: features 16 k + 2 tl, + 1 and + 8, + 9
+  uint32_t qf[NC][KT][2];
+  auto load_q = [&](const PgPlace& p) {
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      const int c = min(p.b * COLS + 8 * nc + gl, sm.n_new[p.i] * a.G - 1), tok = c / a.G;
+      const __nv_bfloat16* src = a.q + (int64_t)(sm.start[p.i] + tok) * a.q_stride + (int64_t)(p.g * a.G + c - tok * a.G) * HD + 2 * tl;
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          qf[k][e] = __ldcg(reinterpret_cast<const unsigned int*>(src[e & 1] + 16 * k + 8 * (e >> 1) + 2 * tl));
+        qf[nc][k][0] = __ldcg(reinterpret_cast<const unsigned int*>(src + 16 * k));
+        qf[nc][k][1] = __ldcg(reinterpret_cast<const unsigned int*>(src + 16 * k + 8));
       }
     }
-    const int first_limit = pos0 + col0 / a.G, last_limit = pos0 + (col0 + n_cols - 1) / a.G;
-    m[0] = m[1] = PG_NEG;
-    l[0] = l[1] = 0.0f;
+  };
+  PgPlace p = {};
+  if (i_lo < i_hi) { p = place_of(i_lo, i_hi); load_q(p); }
+  for (int64_t x = i_lo; x < i_hi;) {
+    const int start = sm.start[p.i], n_new = sm.n_new[p.i], pos0 = sm.pos[p.i], col0 = p.b * COLS;
+    const int n_cols = min(COLS, n_new * a.G - col0);
+    int limit[NC][2];                          // the last keys that this thread's two queries of each 8 see: columns 2 tl, 2 tl + 1
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    for (int u = p.u0; u < p.u1; ++u, ++n) {
-      const int st = n % PG_STAGES;
-      if (ok) ok = pg_wait(full + st, (n / PG_STAGES) & 1);
+    for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        limit[nc][e] = pos0 + min(col0 + 8 * nc + 2 * tl + e, n_new * a.G - 1) / a.G;
+        m[nc][e] = PG_NEG;
+        l[nc][e] = 0.0f;
+      }
+    const int first_limit = pos0 + col0 / a.G, last_limit = pos0 + (col0 + n_cols - 1) / a.G;
+#pragma unroll
+    for (int i = 0; i < KT; ++i)
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) o[i][nc][0] = o[i][nc][1] = o[i][nc][2] = o[i][nc][3] = 0.0f;
+    for (int u = p.u0; u < p.u1; ++u) {
+      if (ok) ok = pg_wait(full + st, phase);
       int key0 = key0s[0];
 #pragma unroll
-      for (int s = 1; s < PG_STAGES; ++s)
-        if (s == st) key0 = key0s[s];
+      for (int i = 1; i < PG_STAGES; ++i)
+        if (i == st) key0 = key0s[i];
       if (ok && key0 >= 0 && key0 <= last_limit) {
+        const uint32_t unit = ring_addr + st * PG_UNIT_BYTES;
         const unsigned char* vals = ring + st * PG_UNIT_BYTES + HALF;
-        const uint32_t kb = ring_addr + st * PG_UNIT_BYTES, vb = kb + HALF;
         // Values that a query does not see may be anything, and its probability of 0 would be multiplied with them.  Those that no query
         // of the item sees are taken as zeros; where one that some see is not finite, all that not everyone sees are added query by query.
         const bool edge = key0 + KS - 1 > first_limit;
@@ -309,154 +355,203 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
           if (__any_sync(0xffffffffu, odd)) cut = first_limit;
         }
-        float s[NT][4];
+        float s[MT][NC][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int k2 = 0; k2 < KT / 2; ++k2) {  // 32 features at a time: lanes 0-7, 8-15, .. address the four pieces of 8 features
-          const uint32_t piece = (uint32_t)((4 * (k2 & 1) + (lane >> 3)) ^ sw) << 4;
+          for (int nc = 0; nc < NC; ++nc) s[t][nc][0] = s[t][nc][1] = s[t][nc][2] = s[t][nc][3] = 0.0f;
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            uint32_t b[4];
-            pg_ldsm(b, kb + (k2 >> 1) * BOX + (8 * j + (lane & 7)) * 128 + piece);
-            pg_mma(s[j], qf[2 * k2], b[0], b[1]);
-            pg_mma(s[j], qf[2 * k2 + 1], b[2], b[3]);
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            uint32_t kf[4];
+            pg_ldsm(kf, unit + (k >> 2) * BOX + 16 * t * 128 + k_row + k_col[k & 3]);
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) pg_mma(s[t][nc], kf, qf[nc][k][0], qf[nc][k][1]);
           }
-        }
-        float mx[2] = {PG_NEG, PG_NEG};
-        if (edge) {
+        // rows of a tile: keys gl and gl + 8; columns: queries 2 tl and 2 tl + 1
+        float mx[NC][2];
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+        for (int nc = 0; nc < NC; ++nc) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[j][e] = key0 + 8 * j + 2 * tl + (e & 1) > limit[e >> 1] ? PG_NEG : s[j][e] * a.scale_log2;
-        } else {
+          for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][e] *= a.scale_log2;
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-        }
-        const bool grows = mx[0] > m[0] || mx[1] > m[1];
-        if (__any_sync(0xffffffffu, grows)) {
-          float f[2];
+            for (int e = 0; e < 4; ++e) {
+              s[t][nc][e] *= a.scale_log2;
+              if (edge && key0 + 16 * t + gl + 8 * (e >> 1) > limit[nc][e & 1]) s[t][nc][e] = PG_NEG;
+            }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mn = fmaxf(m[e], mx[e]);
-            f[e] = m[e] == PG_NEG ? 0.0f : pg_exp2(m[e] - mn);
-            l[e] *= f[e];
-            m[e] = mn;
+            float v = fmaxf(s[0][nc][e], s[0][nc][2 + e]);
+#pragma unroll
+            for (int t = 1; t < MT; ++t) v = fmaxf(v, fmaxf(s[t][nc][e], s[t][nc][2 + e]));
+            mx[nc][e] = v;
           }
-#pragma unroll
-          for (int d = 0; d < HD / 8; ++d) { o[d][0] *= f[0]; o[d][1] *= f[0]; o[d][2] *= f[1]; o[d][3] *= f[1]; }
         }
-        const float ref[2] = {m[0] == PG_NEG ? 0.0f : m[0], m[1] == PG_NEG ? 0.0f : m[1]};
-        uint32_t pr[KS / 16][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float p0 = pg_exp2(s[j][0] - ref[0]), p1 = pg_exp2(s[j][1] - ref[0]), p2 = pg_exp2(s[j][2] - ref[1]), p3 = pg_exp2(s[j][3] - ref[1]);
-          l[0] += p0 + p1;
-          l[1] += p2 + p3;
-          pr[j >> 1][2 * (j & 1)] = pg_pack(p0, p1);
-          pr[j >> 1][2 * (j & 1) + 1] = pg_pack(p2, p3);
+        for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) mx[nc][e] = fmaxf(mx[nc][e], __shfl_xor_sync(0xffffffffu, mx[nc][e], d));
+        bool grows = false;
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) grows |= mx[nc][e] > m[nc][e];
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float mn = fmaxf(m[nc][e], mx[nc][e]), f = m[nc][e] == PG_NEG ? 0.0f : pg_exp2(m[nc][e] - mn);
+              l[nc][e] *= f;
+              m[nc][e] = mn;
+#pragma unroll
+              for (int i = 0; i < KT; ++i) { o[i][nc][e] *= f; o[i][nc][2 + e] *= f; }
+            }
+        }
+        // probabilities: packed by pairs of queries, turned into pairs of keys for the second product
+        uint32_t pr[MT][NC][2], pk[MT][NC][2];
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+          const float r0 = m[nc][0] == PG_NEG ? 0.0f : m[nc][0], r1 = m[nc][1] == PG_NEG ? 0.0f : m[nc][1];
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float p0 = pg_exp2(s[t][nc][2 * h] - r0), p1 = pg_exp2(s[t][nc][2 * h + 1] - r1);
+              l[nc][0] += p0;
+              l[nc][1] += p1;
+              pr[t][nc][h] = pg_pack(p0, p1);
+              pk[t][nc][h] = pg_transpose(pr[t][nc][h]);
+            }
         }
         auto values = [&](auto cutting) {
 #pragma unroll
-          for (int k = 0; k < KS / 16; ++k) {
-            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;         // of this lane's keys 16 k + 2 tl, + 1 and + 8, + 9
+          for (int t = 0; t < MT; ++t) {
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;         // of this lane's keys 16 t + 2 tl, + 1 and + 8, + 9
             if (decltype(cutting)::value) {
-              const int key = key0 + 16 * k + 2 * tl;
+              const int key = key0 + 16 * t + 2 * tl;
               keep0 = key + 1 <= cut ? 0xffffffffu : key <= cut ? 0xffffu : 0u;
               keep1 = key + 9 <= cut ? 0xffffffffu : key + 8 <= cut ? 0xffffu : 0u;
             }
 #pragma unroll
-            for (int d2 = 0; d2 < KT; ++d2) {  // 16 features at a time
-              uint32_t b[4];
-              pg_ldsm_t(b, vb + (d2 >> 2) * BOX + (16 * k + (lane & 15)) * 128 + ((uint32_t)((2 * (d2 & 3) + (lane >> 4)) ^ sw) << 4));
-              pg_mma(o[2 * d2], pr[k], b[0] & keep0, b[1] & keep1);
-              pg_mma(o[2 * d2 + 1], pr[k], b[2] & keep0, b[3] & keep1);
+            for (int i = 0; i < KT; ++i) {
+              uint32_t vf[4];
+              pg_ldsm_t(vf, unit + (i >> 2) * BOX + 16 * t * 128 + v_row + v_col[i & 3]);
+              if (decltype(cutting)::value) { vf[0] &= keep0; vf[1] &= keep0; vf[2] &= keep1; vf[3] &= keep1; }
+#pragma unroll
+              for (int nc = 0; nc < NC; ++nc) pg_mma(o[i][nc], vf, pk[t][nc][0], pk[t][nc][1]);
             }
           }
         };
         if (edge) values(std::true_type()); else values(std::false_type());
         if (cut < last_limit) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll 1
-            for (int e = 0; e < 8; ++e) {
-              const int key = 8 * j + e;
-              const uint32_t w0 = __shfl_sync(0xffffffffu, pr[j >> 1][2 * (j & 1)], (lane & 28) + (e >> 1)), w1 = __shfl_sync(0xffffffffu, pr[j >> 1][2 * (j & 1) + 1], (lane & 28) + (e >> 1));
-              if (key0 + key <= cut || key0 + key > last_limit) continue;
-              const float p0 = __uint_as_float(e & 1 ? w0 & 0xffff0000u : w0 << 16), p1 = __uint_as_float(e & 1 ? w1 & 0xffff0000u : w1 << 16);
-              const unsigned char* line = vals + key * 128 + 4 * tl;
+          for (int t = 0; t < MT; ++t)
 #pragma unroll
-              for (int d = 0; d < HD / 8; ++d) {
-                const uint32_t v = *reinterpret_cast<const uint32_t*>(line + (d >> 3) * BOX + (((d & 7) ^ (key & 7)) << 4));
-                const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xffff0000u);
-                if (key0 + key <= limit[0]) { o[d][0] = fmaf(p0, v0, o[d][0]); o[d][1] = fmaf(p0, v1, o[d][1]); }
-                if (key0 + key <= limit[1]) { o[d][2] = fmaf(p1, v0, o[d][2]); o[d][3] = fmaf(p1, v1, o[d][3]); }
+            for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+              for (int e = 0; e < 8; ++e) {
+                const int key = 16 * t + 8 * h + e;
+                uint32_t w[NC];
+#pragma unroll
+                for (int nc = 0; nc < NC; ++nc) w[nc] = __shfl_sync(0xffffffffu, pr[t][nc][h], 4 * e + tl);
+                if (key0 + key <= cut || key0 + key > last_limit) continue;
+                const unsigned char* line = vals + key * 128;
+#pragma unroll
+                for (int i = 0; i < KT; ++i)
+#pragma unroll
+                  for (int f = 0; f < 2; ++f) {          // feature 16 i + 8 f + gl
+                    const int c = 2 * i + f;
+                    const float v = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(line + (c >> 3) * BOX + (((c & 7) ^ (key & 7)) << 4) + 2 * gl));
+#pragma unroll
+                    for (int nc = 0; nc < NC; ++nc) {
+                      if (key0 + key <= limit[nc][0]) o[i][nc][2 * f] = fmaf(__uint_as_float(w[nc] << 16), v, o[i][nc][2 * f]);
+                      if (key0 + key <= limit[nc][1]) o[i][nc][2 * f + 1] = fmaf(__uint_as_float(w[nc] & 0xffff0000u), v, o[i][nc][2 * f + 1]);
+                    }
+                  }
               }
-            }
         }
       }
       __syncwarp();                            // all lanes have read the stage
       if (ok) ask_next();
+      if (++st == PG_STAGES) { st = 0; phase ^= 1; }
     }
     x += p.u1 - p.u0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    }
-    if (p.u0 == 0 && p.u1 == p.units) {
+    for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[nc][e] += __shfl_xor_sync(0xffffffffu, l[nc][e], d);
+    const PgPlace done = p;
+    if (x < i_hi) { p = place_of(x, i_hi); load_q(p); }        // (on its way while the sums go out)
+    // features 16 i + gl and + 8 of queries 2 tl, 2 tl + 1 to rows of hd floats
+    auto put = [&](auto row_of) {
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float* dst = row_of(8 * nc + 2 * tl + e);
+          if (dst == nullptr) continue;
+#pragma unroll
+          for (int i = 0; i < KT; ++i) { dst[16 * i + gl] = o[i][nc][e]; dst[16 * i + 8 + gl] = o[i][nc][2 + e]; }
+        }
+      __syncwarp();
+    };
+    auto query_of = [&](int c) {               // (token, head)
+      const int tok = (col0 + c) / a.G;
+      return (int64_t)(start + tok) * a.nh + done.g * a.G + (col0 + c) - tok * a.G;
+    };
+    if (done.u0 == 0 && done.u1 == done.units) {
       // ---- a whole item: out with it ------------------------------------------------------------------------------------------
-      const int grp = group_of(a.row0 + p.i);
+      if (group_of(a.row0 + done.i) >= 0) {    // its own pages' part, for the join with the shared ones'
+        put([&](int c) { return c < n_cols ? a.own + query_of(c) * HD : nullptr; });
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = gl + 8 * e;
-        if (c >= n_cols) continue;
-        const int tok = (col0 + c) / a.G, h = (col0 + c) - tok * a.G;
-        const int64_t th = (int64_t)(start + tok) * a.nh + p.g * a.G + h;
-        if (grp >= 0) {                        // its own pages' part, for the join with the shared ones'
+        for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-          for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(a.own + th * HD + 8 * d + 2 * tl) = make_float2(o[d][2 * e], o[d][2 * e + 1]);
-          if (tl == 0) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * th) = make_float2(m[e], l[e]);
-        } else {
-          const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+          for (int e = 0; e < 2; ++e) {
+            const int c = 8 * nc + 2 * tl + e;
+            if (gl == 0 && c < n_cols) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * query_of(c)) = make_float2(m[nc][e], l[nc][e]);
+          }
+      } else {
 #pragma unroll
-          for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<uint32_t*>(a.out + th * HD + 8 * d + 2 * tl) = pg_pack(o[d][2 * e] * inv, o[d][2 * e + 1] * inv);
+        for (int nc = 0; nc < NC; ++nc) {
+          const int c = 8 * nc + gl;           // (after the transposition)
+          const float i0 = l[nc][0] == 0.0f ? 0.0f : 1.0f / l[nc][0], i1 = l[nc][1] == 0.0f ? 0.0f : 1.0f / l[nc][1];
+          __nv_bfloat16* dst = a.out + query_of(min(c, n_cols - 1)) * HD + 2 * tl;
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              const uint32_t w = pg_transpose(pg_pack(o[i][nc][2 * f] * i0, o[i][nc][2 * f + 1] * i1));
+              if (c < n_cols) *reinterpret_cast<uint32_t*>(dst + 16 * i + 8 * f) = w;
+            }
         }
       }
       __syncwarp();
     } else if (x < i_hi) {
       // ---- the first part, of an item that began in the share before: it waits until the ring is free ----------------------------------------
+      put([&](int c) { return spill + c * HD; });
 #pragma unroll
-      for (int d = 0; d < HD / 8; ++d) {
-        *reinterpret_cast<float2*>(spill + gl * HD + 8 * d + 2 * tl) = make_float2(o[d][0], o[d][1]);
-        *reinterpret_cast<float2*>(spill + (gl + 8) * HD + 8 * d + 2 * tl) = make_float2(o[d][2], o[d][3]);
-      }
-      m_first[0] = m[0]; m_first[1] = m[1]; l_first[0] = l[0]; l_first[1] = l[1];
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { m_first[nc][e] = m[nc][e]; l_first[nc][e] = l[nc][e]; }
       have_first = true;
-      if (lane == 0) sm.part_at[warp][0] = p.base;
+      if (lane == 0) sm.part_at[warp][0] = done.base;
     } else {
       // ---- the last one -----------------------------------------------------------------------------------------------------------------
-      PgPart<HD>& part = reinterpret_cast<PgPart<HD>*>(ring)[1];
+      PgPart<HD, COLS>& part = reinterpret_cast<PgPart<HD, COLS>*>(ring)[1];
       __syncwarp();
+      put([&](int c) { return part.acc[c]; });
+      if (gl == 0)
 #pragma unroll
-      for (int d = 0; d < HD / 8; ++d) {
-        *reinterpret_cast<float2*>(&part.acc[gl][8 * d + 2 * tl]) = make_float2(o[d][0], o[d][1]);
-        *reinterpret_cast<float2*>(&part.acc[gl + 8][8 * d + 2 * tl]) = make_float2(o[d][2], o[d][3]);
-      }
-      if (tl == 0) { part.m[gl] = m[0]; part.m[gl + 8] = m[1]; part.l[gl] = l[0]; part.l[gl + 8] = l[1]; }
-      if (lane == 0) sm.part_at[warp][1] = p.base;
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) { part.m[8 * nc + 2 * tl + e] = m[nc][e]; part.l[8 * nc + 2 * tl + e] = l[nc][e]; }
+      if (lane == 0) sm.part_at[warp][1] = done.base;
     }
   }
   if (!ok) {                                   // what was asked for must land before the block's shared memory goes away
@@ -464,81 +559,101 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int u = max(0, ask_n - PG_STAGES); u < ask_n; ++u) pg_wait(full + u % PG_STAGES, (u / PG_STAGES) & 1);
   }
   if (have_first) {
-    PgPart<HD>& part = reinterpret_cast<PgPart<HD>*>(ring)[0];
+    PgPart<HD, COLS>& part = reinterpret_cast<PgPart<HD, COLS>*>(ring)[0];
     __syncwarp();
+    for (int i = lane; i < COLS * HD / 4; i += 32) reinterpret_cast<float4*>(part.acc[0])[i] = reinterpret_cast<const float4*>(spill)[i];
+    if (gl == 0)
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) {         // (each thread its own)
-      *reinterpret_cast<float2*>(&part.acc[gl][8 * d + 2 * tl]) = *reinterpret_cast<const float2*>(spill + gl * HD + 8 * d + 2 * tl);
-      *reinterpret_cast<float2*>(&part.acc[gl + 8][8 * d + 2 * tl]) = *reinterpret_cast<const float2*>(spill + (gl + 8) * HD + 8 * d + 2 * tl);
-    }
-    if (tl == 0) { part.m[gl] = m_first[0]; part.m[gl + 8] = m_first[1]; part.l[gl] = l_first[0]; part.l[gl + 8] = l_first[1]; }
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { part.m[8 * nc + 2 * tl + e] = m_first[nc][e]; part.l[8 * nc + 2 * tl + e] = l_first[nc][e]; }
   }
   __syncthreads();
 
-  // ---- parts of items that shares cut, joined by all threads ------------------------------------------------------------------------------
-  auto parts = [&](int k) -> const PgPart<HD>& { return reinterpret_cast<const PgPart<HD>*>(rings + (k >> 1) * PG_RING)[k & 1]; };
-  constexpr int REC = PG_COLS * (HD + 2);
-  float* const records = a.records + (int64_t)gridDim.x * PG_WARPS * (PG_COLS * HD);
+  // ---- parts of items that shares cut: runs of the warps' parts, a warp for a run's query, a lane for V features of it -----------------------------------
+  constexpr int V = HD / 32;
+  constexpr int REC = COLS * (HD + 2);
+  float* const records = a.records + (int64_t)gridDim.x * PG_WARPS * (PG_MAX_COLS * HD);
   auto block_begin = [&](int b) { return begin(b * PG_WARPS); };
+  auto block_of = [&](int64_t x) {
+    int b = (int)(x * n_blocks / total);
+    while (b > 0 && block_begin(b) > x) --b;
+    while (b + 1 < n_blocks && block_begin(b + 1) <= x) ++b;
+    return b;
+  };
   // a block's part of an item that began before the block, or with it, and the one that goes on in the next block
   auto record = [&](int b, int64_t base) { return records + (2 * (int64_t)b + (block_begin(b) < base ? 1 : 0)) * REC; };
-  auto write = [&](const Place& p, int i, float mm, float ll, float y) {
-    const int c = p.b * PG_COLS + i / HD, tok = c / a.G, d = i % HD;
-    const int64_t th = (int64_t)(sm.start[p.i] + tok) * a.nh + p.g * a.G + c - tok * a.G;
-    if (group_of(a.row0 + p.i) >= 0) {
-      a.own[th * HD + d] = y;
-      if (d == 0) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * th) = make_float2(mm, ll);
+  if (threadIdx.x == 0) {
+    int n = 0;
+    sm.edge[0] = sm.edge[1] = -1;
+    for (int k = 0; k < 2 * PG_WARPS; ++k) {
+      const int64_t at = sm.part_at[k >> 1][k & 1];
+      if (at < 0) continue;
+      if (n > 0 && sm.run[n - 1].p.base == at) { sm.run[n - 1].k1 = k + 1; continue; }
+      PgRun& r = sm.run[n++];
+      r.p = place_of(at, at + 1);
+      r.k0 = k;
+      r.k1 = k + 1;
+      r.whole = at >= block_begin(blockIdx.x) && at + r.p.units <= block_begin(blockIdx.x + 1);
+      r.own = group_of(a.row0 + r.p.i) >= 0;
+      if (!r.whole) sm.edge[at <= block_begin(blockIdx.x) ? 0 : 1] = n - 1;
+    }
+    sm.n_runs = n;
+  }
+  __syncthreads();
+  auto parts = [&](int k) -> const PgPart<HD, COLS>& { return reinterpret_cast<const PgPart<HD, COLS>*>(rings + (k >> 1) * PG_RING)[k & 1]; };
+  auto cols_of = [&](const PgPlace& p) { return min(COLS, sm.n_new[p.i] * a.G - p.b * COLS); };
+  // column c of a run's item, this lane's features
+  auto write = [&](const PgRun& r, int c, float mm, float ll, const float (&y)[V]) {
+    const int cc = r.p.b * COLS + c, tok = cc / a.G;
+    const int64_t th = (int64_t)(sm.start[r.p.i] + tok) * a.nh + r.p.g * a.G + cc - tok * a.G;
+    if (r.own) {
+      pg_store(a.own + th * HD + lane * V, y);
+      if (lane == 0) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * th) = make_float2(mm, ll);
     } else {
-      a.out[th * HD + d] = __float2bfloat16_rn(ll == 0.0f ? 0.0f : y / ll);
+      const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+      for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(a.out + th * HD + lane * V + i) = pg_pack(y[i] * inv, y[i + 1] * inv);
     }
   };
-  int64_t edge_at[2] = {-1, -1};               // the items that go beyond the block: the first run's, the last run's
-  for (int k0 = 0; k0 < 2 * PG_WARPS;) {
-    const int64_t at = sm.part_at[k0 >> 1][k0 & 1];
-    int k1 = k0 + 1;
-    if (at < 0) { k0 = k1; continue; }
-    while (k1 < 2 * PG_WARPS && (sm.part_at[k1 >> 1][k1 & 1] == at || sm.part_at[k1 >> 1][k1 & 1] < 0)) ++k1;      // (a warp without a part there is between)
-    const Place p = place_of(at, at + 1);
-    const bool whole = at >= block_begin(blockIdx.x) && at + p.units <= block_begin(blockIdx.x + 1);
-    if (!whole) edge_at[at < block_begin(blockIdx.x) || at == block_begin(blockIdx.x) ? 0 : 1] = at;
-    const int n_cols = min(PG_COLS, sm.n_new[p.i] * a.G - p.b * PG_COLS);
-    for (int i = threadIdx.x; i < n_cols * HD; i += PG_WARPS * 32) {
-      const int c = i / HD, d = i % HD;
-      float mm = PG_NEG, ll = 0.0f, y = 0.0f;
-      for (int k = k0; k < k1; ++k)
-        if (sm.part_at[k >> 1][k & 1] == at) mm = fmaxf(mm, parts(k).m[c]);
+  for (int k = 0; k < sm.n_runs; ++k) {
+    const PgRun& r = sm.run[k];
+    const int n_cols = cols_of(r.p);
+    float* const rec = record(blockIdx.x, r.p.base);
+    for (int c = warp; c < n_cols; c += PG_WARPS) {
+      float mm = PG_NEG, ll = 0.0f, y[V] = {};
+      for (int i = r.k0; i < r.k1; ++i)
+        if (sm.part_at[i >> 1][i & 1] >= 0) mm = fmaxf(mm, parts(i).m[c]);         // (a warp without a part there may be between)
       const float safe = mm == PG_NEG ? 0.0f : mm;
-      for (int k = k0; k < k1; ++k) {
-        if (sm.part_at[k >> 1][k & 1] != at) continue;
-        const float f = pg_exp2(parts(k).m[c] - safe);
-        ll = fmaf(parts(k).l[c], f, ll);
-        y = fmaf(parts(k).acc[c][d], f, y);
+      for (int i = r.k0; i < r.k1; ++i) {
+        if (sm.part_at[i >> 1][i & 1] < 0) continue;
+        const float f = pg_exp2(parts(i).m[c] - safe);
+        ll = fmaf(parts(i).l[c], f, ll);
+        const float* const acc = &parts(i).acc[c][lane * V];
+        float y1[V];
+        if (V == 4) { const float4 w = *reinterpret_cast<const float4*>(acc); y1[0] = w.x; y1[1] = w.y; y1[V - 2] = w.z; y1[V - 1] = w.w; }
+        else { const float2 w = *reinterpret_cast<const float2*>(acc); y1[0] = w.x; y1[1] = w.y; }
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = fmaf(y1[v], f, y[v]);
       }
-      if (whole) {
-        write(p, i, mm, ll, y);
+      if (r.whole) {
+        write(r, c, mm, ll, y);
       } else {
-        float* r = record(blockIdx.x, at);
-        r[2 * PG_COLS + i] = y;
-        if (d == 0) { r[c] = mm; r[PG_COLS + c] = ll; }
+        pg_store(rec + 2 * COLS + c * HD + lane * V, y);
+        if (lane == 0) { rec[c] = mm; rec[COLS + c] = ll; }
       }
     }
-    k0 = k1;
   }
   // ---- items that blocks cut: the last of their blocks to report joins them ------------------------------------------------------------------
-  if (edge_at[0] >= 0 || edge_at[1] >= 0) {
-    auto block_of = [&](int64_t x) {
-      int b = (int)(x * n_blocks / total);
-      while (b > 0 && block_begin(b) > x) --b;
-      while (b + 1 < n_blocks && block_begin(b + 1) <= x) ++b;
-      return b;
-    };
+  if (sm.edge[0] >= 0 || sm.edge[1] >= 0) {
     __threadfence();
     __syncthreads();
     if (threadIdx.x < 2) {
-      const int64_t at = edge_at[threadIdx.x];
+      const int k = sm.edge[threadIdx.x];
       bool last = false;
-      if (at >= 0) {
-        const int ba = block_of(at), bb = block_of(at + place_of(at, at + 1).units - 1);
+      if (k >= 0) {
+        const PgPlace& p = sm.run[k].p;
+        const int ba = block_of(p.base), bb = block_of(p.base + p.units - 1);
         last = atomicAdd(a.counters + ba, 1) == bb - ba;             // (of the items that begin in a block only one goes beyond it)
         if (last) a.counters[ba] = 0;
       }
@@ -548,24 +663,51 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __syncthreads();
     for (int e = 0; e < 2; ++e) {
       if (!sm.last[e]) continue;
-      const int64_t at = edge_at[e];
-      const Place p = place_of(at, at + 1);
-      const int ba = block_of(at), bb = block_of(at + p.units - 1);
-      const int n_cols = min(PG_COLS, sm.n_new[p.i] * a.G - p.b * PG_COLS);
-      for (int i = threadIdx.x; i < n_cols * HD; i += PG_WARPS * 32) {
-        const int c = i / HD;
-        float mm = PG_NEG, ll = 0.0f, y = 0.0f;
-#pragma unroll 8
-        for (int b = ba; b <= bb; ++b) {
-          const float* r = record(b, at);
-          const float m1 = __ldcg(r + c), l1 = __ldcg(r + PG_COLS + c), y1 = __ldcg(r + 2 * PG_COLS + i);
-          const float top = fmaxf(mm, m1), safe = top == PG_NEG ? 0.0f : top;
-          const float f0 = pg_exp2(mm - safe), f1 = pg_exp2(m1 - safe);
-          ll = ll * f0 + l1 * f1;
-          y = y * f0 + y1 * f1;
-          mm = top;
+      const PgRun& r = sm.run[sm.edge[e]];
+      const int ba = block_of(r.p.base), n = block_of(r.p.base + r.p.units - 1) - ba + 1, n_cols = cols_of(r.p);
+      // the records of blocks ba .. ba + n - 1: all but the first are their blocks' first
+      const float* const rec0 = record(ba, r.p.base);
+      auto rec = [&](int i) { return i == 0 ? rec0 : records + 2 * (int64_t)(ba + i) * REC; };
+      for (int c0 = warp; c0 < n_cols; c0 += 2 * PG_WARPS) {         // two queries at a time
+        float mm[2] = {PG_NEG, PG_NEG}, ll[2] = {0.0f, 0.0f}, y[2][V] = {};
+        for (int i0 = 0; i0 < n; i0 += 8) {
+          float m1[2][8], l1[2][8], y1[2][8][V];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = c0 + h * PG_WARPS;
+              const bool in = i0 + i < n && c < n_cols;
+              const float* q = rec(in ? i0 + i : 0) + (in ? c : 0);
+              m1[h][i] = in ? __ldcg(q) : PG_NEG;
+              l1[h][i] = in ? __ldcg(q + COLS) : 0.0f;
+              if (in) pg_load(rec(i0 + i) + 2 * COLS + c * HD + lane * V, y1[h][i]);
+              else
+#pragma unroll
+                for (int v = 0; v < V; ++v) y1[h][i][v] = 0.0f;
+            }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = mm[h];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, m1[h][i]);
+            const float safe = top == PG_NEG ? 0.0f : top, f0 = pg_exp2(mm[h] - safe);
+            ll[h] *= f0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) y[h][v] *= f0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float f = pg_exp2(m1[h][i] - safe);
+              ll[h] = fmaf(l1[h][i], f, ll[h]);
+#pragma unroll
+              for (int v = 0; v < V; ++v) y[h][v] = fmaf(y1[h][i][v], f, y[h][v]);
+            }
+            mm[h] = top;
+          }
         }
-        write(p, i, mm, ll, y);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (c0 + h * PG_WARPS < n_cols) write(r, c0 + h * PG_WARPS, mm[h], ll[h], y[h]);
       }
     }
   }
@@ -582,7 +724,9 @@ int pg_sms(const char* what) {                 // of the current device, 0: an e
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("%s: no device", what); return 0; }
   if (known[dev]) return known[dev];
   cudaError_t e = cudaSuccess;
-  for (auto f : {(const void*)attn_pages_kernel<64, false>, (const void*)attn_pages_kernel<64, true>, (const void*)attn_pages_kernel<128, false>, (const void*)attn_pages_kernel<128, true>})
+  for (auto f : {(const void*)attn_pages_kernel<64, 1, false>, (const void*)attn_pages_kernel<64, 1, true>, (const void*)attn_pages_kernel<128, 1, false>,
+                 (const void*)attn_pages_kernel<128, 1, true>, (const void*)attn_pages_kernel<64, 2, false>, (const void*)attn_pages_kernel<64, 2, true>,
+                 (const void*)attn_pages_kernel<128, 2, false>, (const void*)attn_pages_kernel<128, 2, true>})
     if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, PG_SMEM);
   if (e == cudaSuccess) e = attn_shared_prepare();
   int sms = 0;
@@ -592,7 +736,7 @@ int pg_sms(const char* what) {                 // of the current device, 0: an e
 }
 
 // Where the warps' first parts wait, and the blocks' parts.
-static int64_t pg_record_floats(int sms, int hd) { return (int64_t)sms * (PG_WARPS * PG_COLS * hd + 2 * PG_COLS * (hd + 2)); }
+static int64_t pg_record_floats(int sms, int hd) { return (int64_t)sms * (PG_WARPS * PG_MAX_COLS * hd + 2 * PG_MAX_COLS * (hd + 2)); }
 // With groups: the plan, the parts of shared pages, the rows' own parts.
 constexpr int64_t PS_PLAN_FLOATS = (sizeof(PsPlan) + 63) / 64 * 16;
 static int64_t ps_slots(int sms, int64_t T, int G, int nkv, int n_groups) { return sms + nkv * (T * G / PS_TILE + n_groups); }
@@ -600,12 +744,13 @@ static int64_t ps_floats(int sms, int64_t T, int G, int nkv, int hd, int n_group
   return n_groups ? PS_PLAN_FLOATS + ps_slots(sms, T, G, nkv, n_groups) * ps_record(hd) + ps_own(T, G * nkv, hd) : 0;
 }
 
-template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int sms, const char* what, cudaStream_t stream) {
+template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int most_cols, int sms, const char* what, cudaStream_t stream) {
   for (int r0 = 0; r0 < a.rows; r0 += PG_WINDOW) {
     a.row0 = r0;
     a.wait_first = r0 > 0 || a.n_groups == 0;
     auto go = [&](auto kernel) { launch_pdl(kernel, dim3(sms), dim3(PG_WARPS * 32), PG_SMEM, stream, map_k, map_v, a); };
-    if (hd == 64) go(attn_pages_kernel<64, LIST>); else go(attn_pages_kernel<128, LIST>);
+    if (most_cols <= 8) { if (hd == 64) go(attn_pages_kernel<64, 1, LIST>); else go(attn_pages_kernel<128, 1, LIST>); }
+    else { if (hd == 64) go(attn_pages_kernel<64, 2, LIST>); else go(attn_pages_kernel<128, 2, LIST>); }
     const int rc = launch_status(what);
     if (rc) return rc;
   }
@@ -616,7 +761,7 @@ template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, co
 static int pg_check(const char* what, const void* q, int64_t q_stride, const void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table,
                     int bt_width, int rows, int T, int nh, int nkv, int hd, float scale, CUtensorMap* map_k, CUtensorMap* map_v) {
   if (rows < 0 || T < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || !(scale > 0.0f) || !isfinite(scale) || n_pages < 1 ||
-      (n_pages + 1) * nkv * PG_PAGE > INT32_MAX || bt_width < 1 || bt_width > PG_MAX_WIDTH || (int64_t)T * (nh / nkv) > INT32_MAX - PG_COLS) {
+      (n_pages + 1) * nkv * PG_PAGE > INT32_MAX || bt_width < 1 || bt_width > PG_MAX_WIDTH || (int64_t)T * (nh / nkv) > INT32_MAX - PG_MAX_COLS) {
     set_error("%s: needs heads of 64 or 128, a positive scale, tables of at most %d pages and pools of fewer than 2^31 tokens times key/value heads, got %d rows, %d tokens, %d "
               "heads on %d of %d, scale %g, %lld pages, a table of %d", what, PG_MAX_WIDTH, rows, T, nh, nkv, hd, (double)scale, (long long)n_pages, bt_width);
     return ERR_BAD_ARGUMENT;
@@ -626,7 +771,7 @@ static int pg_check(const char* what, const void* q, int64_t q_stride, const voi
     set_error("%s: q, its rows, out and the pools must be 16-byte aligned", what);
     return ERR_ALIGNMENT;
   }
-  const int box = hd == 64 ? 32 : 16;
+  const int box = hd == 64 ? 64 : 32;
   int rc = tc5::make_map_k64(map_k, k_pool, n_pages * nkv * PG_PAGE, hd, box, what);
   return rc ? rc : tc5::make_map_k64(map_v, v_pool, n_pages * nkv * PG_PAGE, hd, box, what);
 }
@@ -672,7 +817,7 @@ extern "C" int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, T, T, nh, nkv, scale, scratch);
   a.tok_pos = tok_pos; a.tok_seq = tok_seq; a.lists = lists; a.count = std::min(count, bt_width);
   a.list_stride = count; a.bt_rows = bt_rows;
-  return pg_launch<true>(a, map_k, map_v, hd, sms, "attn_pages", stream);
+  return pg_launch<true>(a, map_k, map_v, hd, a.G, sms, "attn_pages", stream);
 }
 
 // Causal attention of rows whose groups share their first pages (groups: int32 [n_groups, 3]: first row, rows, pages).
@@ -702,6 +847,6 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
     rc = attn_shared_launch(p, k_pool, v_pool, hd, sms, stream);
     if (rc) return rc;
   }
-  rc = pg_launch<false>(a, map_k, map_v, hd, sms, "attn_shared", stream);
+  rc = pg_launch<false>(a, map_k, map_v, hd, (int)std::min((int64_t)max_new * a.G, (int64_t)PG_MAX_COLS), sms, "attn_shared", stream);
   return rc || !n_groups ? rc : attn_shared_join(plan, parts, a.own, a.out, T, nh, nkv, hd, stream);
 }
