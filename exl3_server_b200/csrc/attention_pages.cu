@@ -117,6 +117,7 @@ struct PgSmem {
   int64_t cum[PG_WINDOW + 1];                  // units of the rows before
   int start[PG_WINDOW], n_new[PG_WINDOW], pos[PG_WINDOW], units[PG_WINDOW];
   int64_t part_at[PG_WARPS][2];                // a part's item (the place of its first unit), -1: none
+  PgPlace part_of[PG_WARPS][2];
   int64_t warp_sum[PG_WARPS];
   int last[2];
   PsPlan plan;
@@ -206,7 +207,9 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (!a.wait_first) pdl_wait();
     return;
   }
-  auto begin = [&](int w) { return total * w / (n_blocks * PG_WARPS); };       // the first unit of a warp's share
+  const int n_shares = n_blocks * PG_WARPS;
+  const int64_t per = total / n_shares, rem = total - per * n_shares;
+  auto begin = [&](int w) { return per * w + min((int64_t)w, rem); };         // the first unit of a warp's share: they differ by one unit at most
   const int64_t i_lo = begin(blockIdx.x * PG_WARPS + warp), i_hi = begin(blockIdx.x * PG_WARPS + warp + 1);
   // The item at place x.
   auto place_of = [&](int64_t x, int64_t end) {
@@ -540,7 +543,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
         for (int e = 0; e < 2; ++e) { m_first[nc][e] = m[nc][e]; l_first[nc][e] = l[nc][e]; }
       have_first = true;
-      if (lane == 0) sm.part_at[warp][0] = done.base;
+      if (lane == 0) { sm.part_at[warp][0] = done.base; sm.part_of[warp][0] = done; }
     } else {
       // ---- the last one -----------------------------------------------------------------------------------------------------------------
       PgPart<HD, COLS>& part = reinterpret_cast<PgPart<HD, COLS>*>(ring)[1];
@@ -551,7 +554,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
           for (int e = 0; e < 2; ++e) { part.m[8 * nc + 2 * tl + e] = m[nc][e]; part.l[8 * nc + 2 * tl + e] = l[nc][e]; }
-      if (lane == 0) sm.part_at[warp][1] = done.base;
+      if (lane == 0) { sm.part_at[warp][1] = done.base; sm.part_of[warp][1] = done; }
     }
   }
   if (!ok) {                                   // what was asked for must land before the block's shared memory goes away
@@ -576,10 +579,8 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   float* const records = a.records + (int64_t)gridDim.x * PG_WARPS * (PG_MAX_COLS * HD);
   auto block_begin = [&](int b) { return begin(b * PG_WARPS); };
   auto block_of = [&](int64_t x) {
-    int b = (int)(x * n_blocks / total);
-    while (b > 0 && block_begin(b) > x) --b;
-    while (b + 1 < n_blocks && block_begin(b + 1) <= x) ++b;
-    return b;
+    const int64_t longer = rem * (per + 1);    // (units of the longer shares; per is 0 only where there is one block)
+    return (int)(x < longer ? x / (per + 1) : rem + (x - longer) / max(per, (int64_t)1)) / PG_WARPS;
   };
   // a block's part of an item that began before the block, or with it, and the one that goes on in the next block
   auto record = [&](int b, int64_t base) { return records + (2 * (int64_t)b + (block_begin(b) < base ? 1 : 0)) * REC; };
@@ -591,7 +592,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       if (at < 0) continue;
       if (n > 0 && sm.run[n - 1].p.base == at) { sm.run[n - 1].k1 = k + 1; continue; }
       PgRun& r = sm.run[n++];
-      r.p = place_of(at, at + 1);
+      r.p = sm.part_of[k >> 1][k & 1];
       r.k0 = k;
       r.k1 = k + 1;
       r.whole = at >= block_begin(blockIdx.x) && at + r.p.units <= block_begin(blockIdx.x + 1);

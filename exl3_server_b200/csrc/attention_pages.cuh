@@ -23,18 +23,14 @@ struct PsPlan {                                // in shared memory
   int n;                                       // groups
   int blocks;                                  // shares
   int64_t total;                               // pages of all tiles of all heads
+  int64_t per, rem;                            // a share has `per` pages, the first `rem` shares one more
   int tok0[PG_MAX_GROUPS], queries[PG_MAX_GROUPS], pages[PG_MAX_GROUPS], row[PG_MAX_GROUPS], rows[PG_MAX_GROUPS];
   int tiles_before[PG_MAX_GROUPS + 1];         // tiles of a head in the groups before
   int64_t work_before[PG_MAX_GROUPS + 1];      // pages of tiles of a head in the groups before
   __device__ int tiles(int j) const { return (queries[j] + PS_TILE - 1) / PS_TILE; }
-  __device__ int64_t begin(int block) const { return total * block / blocks; }
-  // the first share that holds place x of the list
-  __device__ int block_of(int64_t x) const {
-    int b = (int)(x * blocks / total);
-    while (b + 1 < blocks && begin(b + 1) <= x) ++b;
-    while (b > 0 && begin(b) > x) --b;
-    return b;
-  }
+  __device__ int64_t begin(int block) const { return per * block + min((int64_t)block, rem); }
+  // the share that holds place x of the list
+  __device__ int block_of(int64_t x) const { return x < rem * (per + 1) ? (int)(x / (per + 1)) : (int)(rem + (x - rem * (per + 1)) / per); }
 };
 
 // By all threads of a block (it ends with a barrier).  groups: int32 [n, 3], ascending; a group that begins before the one ahead of it ends
@@ -74,6 +70,8 @@ __device__ inline void ps_plan(PsPlan& p, const int* __restrict__ groups, int n,
     p.n = n;
     p.total = p.work_before[n] * nkv;
     p.blocks = (int)min((int64_t)grid, max((int64_t)1, p.total / PS_MIN_PAGES));
+    p.per = p.total / p.blocks;
+    p.rem = p.total - p.per * p.blocks;
   }
   __syncthreads();
 }
@@ -98,6 +96,7 @@ __device__ inline PsPart ps_part(const PsPlan& p, int nkv, int64_t x, int64_t en
 __device__ inline int ps_slot(const PsPlan& p, int nkv, int j, int g, int tile, int b) {
   return b + p.tiles_before[j] * nkv + g * p.tiles(j) + tile;
 }
+// A tile of up to 128 queries has a place for 256 all the same: the two halves of a block then take pages in turn, and leave a record's half each.
 // A record, in floats: the queries' maxima (base-2 units), their sums, their sums of values [query][hd].
 __host__ __device__ constexpr int64_t ps_record(int hd) { return (int64_t)PS_TILE * (hd + 2); }
 

@@ -73,8 +73,18 @@ __device__ inline float ps_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// Bounded, and one answer for the warp.
-__device__ inline bool ps_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// Bounded, and one answer for the warp.  The hardware may hold a look for a while.
+__device__ inline bool ps_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  uint32_t there = 0;
+  for (uint32_t i = 0; i < WAIT_LIMIT && !there; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(there) : "r"(addr), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, there);
+}
 // One arrival for the warp, when all its lanes are here.
 __device__ inline void ps_arrive_warp(uint64_t* bar) {
   __syncwarp();
@@ -167,7 +177,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     for (int i = threadIdx.x; i < (int)(sizeof(PsPlan) / 4); i += PS_THREADS) reinterpret_cast<int*>(a.plan)[i] = reinterpret_cast<const int*>(&plan)[i];
   const uint32_t tmem = *tmem_slot;            // columns: scores of set s at 128 s, O at 256 + 128 s
   const int64_t lo = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x) : 0, hi = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x + 1) : 0;
-  auto sets_of = [&](const PsPart& t) { return plan.queries[t.j] - t.tile * PS_TILE > 128 ? 2 : 1; };
+  // Tiles of more than 128 queries: both sets take every page, 128 queries each.  Smaller ones: the sets take the pages in turn, with the same queries.
+  auto both = [&](const PsPart& t) { return plan.queries[t.j] - t.tile * PS_TILE > 128; };
   bool ok = true;
 
   if (warp == 10) {
@@ -203,15 +214,15 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     int c = 0, f[2] = {0, 0}, k[2] = {0, 0};   // pages, pages of a set, parts of a set so far
     for (int64_t x = lo; x < hi && ok;) {
       const PsPart t = ps_part(plan, a.nkv, x, hi);
-      const int sets = sets_of(t);
+      const bool two = both(t);
       for (int p = t.p0; p < t.p1 && ok; ++p, ++c) {
         const int st = c % PS_STAGES;
         if (!ps_wait(kv_full + st, (c / PS_STAGES) & 1)) { ok = false; break; }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          if (s >= sets) break;
+          if (!two && ((p - t.p0) & 1) != s) continue;
           const int sb = f[s] & 1;
-          if (p == t.p0 && !ps_wait(q_full + s, k[s] & 1)) { ok = false; break; }
+          if (p == t.p0 + (two ? 0 : s) && !ps_wait(q_full + s, k[s] & 1)) { ok = false; break; }
           if (f[s] >= 2 && !ps_wait(pv_done + 2 * s + sb, ((f[s] >> 1) - 1) & 1)) { ok = false; break; }
           fence_after();
           if (lane == 0) {
@@ -227,8 +238,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           ++f[s];
         }
       }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) k[s] += s < sets;
+      ++k[0];
+      k[1] += two || t.p1 - t.p0 > 1;          // (a set without a page asks for no queries)
       x += t.p1 - t.p0;
     }
     if (!ok && lane == 0) atomicExch(&g_ps_error, 2);
@@ -237,22 +248,23 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     int c = 0, f[2] = {0, 0};
     for (int64_t x = lo; x < hi && ok;) {
       const PsPart t = ps_part(plan, a.nkv, x, hi);
-      const int sets = sets_of(t);
+      const bool two = both(t);
       for (int p = t.p0; p < t.p1 && ok; ++p, ++c) {
         const int st = c % PS_STAGES;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          if (s >= sets) break;
+          if (!two && ((p - t.p0) & 1) != s) continue;
           const int sb = f[s] & 1;
           if (!ps_wait(p_full + 2 * s + sb, (f[s] >> 1) & 1)) { ok = false; break; }
           fence_after();
           if (lane == 0) {
             const uint64_t db = ps_desc_v<HD>(smem_u32(sV + st * KVB));
+            const bool fresh = p == t.p0 + (two ? 0 : s);            // a part's first product starts O afresh
 #pragma unroll
-            for (int i = 0; i < PG_PAGE / 16; ++i)       // 16 keys: 8 columns of P, 16 rows of V; a part's first product starts O afresh
-              ps_mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 64 * sb + 8 * i, db + 128 * i, ps_idesc_pv(HD), (p > t.p0 || i > 0) ? 1u : 0u);
+            for (int i = 0; i < PG_PAGE / 16; ++i)                   // 16 keys: 8 columns of P, 16 rows of V
+              ps_mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 64 * sb + 8 * i, db + 128 * i, ps_idesc_pv(HD), (!fresh || i > 0) ? 1u : 0u);
             mma_commit(pv_done + 2 * s + sb);
-            if (s == sets - 1) mma_commit(kv_free + st);
+            if (!two || s == 1) mma_commit(kv_free + st);
           }
           __syncwarp();
           ++f[s];
@@ -270,8 +282,15 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     for (int64_t x = lo; x < hi && ok;) {
       const PsPart t = ps_part(plan, a.nkv, x, hi);
       x += t.p1 - t.p0;
-      if (s >= sets_of(t)) continue;
-      const int query = t.tile * PS_TILE + s * 128 + r;
+      const bool two = both(t);
+      const int step = two ? 1 : 2, first = t.p0 + (two ? 0 : s), qr = s * 128 + r;
+      const int query = t.tile * PS_TILE + (two ? qr : r);
+      float* rec = a.records + ps_slot(plan, a.nkv, t.j, t.g, t.tile, blockIdx.x) * ps_record(HD);
+      if (first >= t.p1) {                     // no page for this set
+        rec[qr] = -INFINITY;
+        rec[PS_TILE + qr] = 0.0f;
+        continue;
+      }
       const bool in = query < plan.queries[t.j];
       const int tok = plan.tok0[t.j] + (in ? query / a.G : 0), head = t.g * a.G + (in ? query % a.G : 0);
       // Q: this thread's row, into the operand's layout (the last S that read the place before is done)
@@ -297,12 +316,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const int sees = __reduce_min_sync(0xffffffffu, pos);              // all of the warp's queries see keys up to here
       float m_used = -INFINITY, l = 0.0f;
       uint32_t s0[32], s1[32];
-      for (int p = t.p0; p < t.p1; ++p, ++f) {
-        const int sb = f & 1;
-        if (!ps_wait(s_full + 2 * s + sb, (f >> 1) & 1)) { ok = false; break; }
+      auto ask = [&](int f) {                  // the scores of the set's page f: on their way
+        if (!ps_wait(s_full + 2 * s + (f & 1), (f >> 1) & 1)) return false;
         fence_after();
-        tmem_ld32_issue(ts + 64 * sb, s0);
-        tmem_ld32_issue(ts + 64 * sb + 32, s1);
+        tmem_ld32_issue(ts + 64 * (f & 1), s0);
+        tmem_ld32_issue(ts + 64 * (f & 1) + 32, s1);
+        return true;
+      };
+      ok = ask(f);
+      for (int p = first; p < t.p1 && ok; p += step, ++f) {
+        const int sb = f & 1;
         tmem_ld_wait(s0);
         tmem_ld_wait(s1);
         const int key0 = p * PG_PAGE;
@@ -320,7 +343,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (__any_sync(0xffffffffu, grow)) {
           const float m_new = grow ? mx : m_used;
           const float corr = m_used == -INFINITY ? 0.0f : ps_exp2(m_used - m_new);
-          if (p > t.p0) {
+          if (p > first) {
             if (!ps_wait(pv_done + 2 * s + (sb ^ 1), ((f - 1) >> 1) & 1)) { ok = false; break; }
             fence_after();
             ps_rescale<HD>(to, corr);
@@ -337,7 +360,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         float e0, e1;
         asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(sum[0]));
         l += e0 + e1;
-        ps_st32(ts + 64 * sb, pw);
+        ps_st32(ts + 64 * sb, pw);             // over the row's own scores
+        if (p + step < t.p1) ok = ask(f + 1);
         ps_wait_st();
         fence_before();
         ps_arrive_warp(p_full + 2 * s + sb);
@@ -346,8 +370,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       ok = ps_wait(pv_done + 2 * s + ((f - 1) & 1), ((f - 1) >> 1) & 1);
       if (!ok) break;
       fence_after();
-      float* rec = a.records + ps_slot(plan, a.nkv, t.j, t.g, t.tile, blockIdx.x) * ps_record(HD);
-      const int qr = s * 128 + r;
       if (in) { rec[qr] = m_used; rec[PS_TILE + qr] = l; }
 #pragma unroll
       for (int h = 0; h < HD / 32; ++h) {
@@ -361,6 +383,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       __syncwarp();
       fence_before();                          // O is read: the next part's first product may write it
     }
+    if (!ok) asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");         // a row of scores may still be on its way
     if (!ok && lane == 0) atomicExch(&g_ps_error, 4);
   }
   fence_before();
@@ -371,49 +394,64 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
 // Joins the parts of a query: a warp for each (token, head).  The parts of the shared pages are in the order of the pages, the own pages' part is the last, so
 // a result does not depend on which block was the first to end.
-constexpr int PJ_WARPS = 4;
+constexpr int PJ_WARPS = 4, PJ_PARTS = 512;               // two for every SM, at most
 template <int HD>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
 attn_shared_join_kernel(const PsPlan* __restrict__ plan, const float* __restrict__ records, const float* __restrict__ own, __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
   constexpr int V = HD / 32;                   // features a lane
-  __shared__ float s_w[PJ_WARPS][256];
+  __shared__ float s_w[PJ_WARPS][PJ_PARTS + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t th = (int64_t)blockIdx.x * PJ_WARPS + warp;
   pdl_trigger();
   pdl_wait();
   if (th >= (int64_t)T * nh) return;
-  const int tok = (int)(th / nh), head = (int)(th % nh), G = nh / nkv, g = head / G;
-  int lo = 0, hi = __ldcg(&plan->n) - 1;
-  while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (__ldcg(&plan->tok0[mid]) <= tok) lo = mid; else hi = mid - 1; }
-  const int query = (tok - __ldcg(&plan->tok0[lo])) * G + head % G, queries = __ldcg(&plan->queries[lo]), pages = __ldcg(&plan->pages[lo]);
-  if (query < 0 || query >= queries || pages == 0) return;             // in no group: its own pages' part was all
-  const int tile = query / PS_TILE, qr = query % PS_TILE, tiles = (queries + PS_TILE - 1) / PS_TILE, blocks = __ldcg(&plan->blocks);
-  const int64_t total = __ldcg(&plan->total), first = __ldcg(&plan->work_before[lo]) * nkv + ((int64_t)g * tiles + tile) * pages;
-  const int slot0 = __ldcg(&plan->tiles_before[lo]) * nkv + g * tiles + tile;
-  auto block_of = [&](int64_t x) {
-    int b = (int)(x * blocks / total);
-    while (b + 1 < blocks && total * (b + 1) / blocks <= x) ++b;
-    while (b > 0 && total * b / blocks > x) --b;
-    return b;
-  };
-  const int b0 = block_of(first), n = block_of(first + pages - 1) - b0 + 1;           // parts (at most as many as there are SMs)
-  const float* rec0 = records + (slot0 + b0) * ps_record(HD) + qr;
+  const int tok = (int)(th / nh), head = (int)(th - (int64_t)tok * nh), G = nh / nkv, g = head / G;
+  // the token's group: the last that begins at or before it; lanes side by side, all of a group's numbers at once
+  const int n_groups = __ldcg(&plan->n), blocks_per = (int)min(__ldcg(&plan->per), (int64_t)INT32_MAX);
+  const int64_t rem = __ldcg(&plan->rem), per = blocks_per;
+  int tok0 = -1, queries = 0, pages = 0, tiles_before = 0;
+  int64_t work_before = 0;
+  for (int j0 = 0; j0 < n_groups; j0 += 32) {
+    const int j = min(j0 + lane, n_groups - 1);
+    const int t0 = __ldcg(&plan->tok0[j]), q0 = __ldcg(&plan->queries[j]), p0 = __ldcg(&plan->pages[j]), b0 = __ldcg(&plan->tiles_before[j]);
+    const int64_t w0 = __ldcg(&plan->work_before[j]);
+    const unsigned here = __ballot_sync(0xffffffffu, j0 + lane < n_groups && t0 <= tok && q0 > 0);
+    if (here) {
+      const int src = 31 - __clz(here);
+      tok0 = __shfl_sync(0xffffffffu, t0, src);
+      queries = __shfl_sync(0xffffffffu, q0, src);
+      pages = __shfl_sync(0xffffffffu, p0, src);
+      tiles_before = __shfl_sync(0xffffffffu, b0, src);
+      work_before = __shfl_sync(0xffffffffu, w0, src);
+    }
+  }
+  const int query = (tok - tok0) * G + head - g * G;
+  if (tok0 < 0 || query >= queries || pages == 0) return;              // in no group: its own pages' part was all
+  const int tile = query / PS_TILE, tiles = (queries + PS_TILE - 1) / PS_TILE;
+  const int64_t first = work_before * nkv + ((int64_t)g * tiles + tile) * pages, longer = rem * (per + 1);
+  auto block_of = [&](int64_t x) { return x < longer ? (int)(x / (per + 1)) : (int)(rem + (x - longer) / per); };
+  const int b0 = block_of(first), halves = queries - tile * PS_TILE > 128 ? 1 : 2;
+  const int n = (block_of(first + pages - 1) - b0 + 1) * halves;       // parts: at most two for every SM
+  const float* rec0 = records + (tiles_before * nkv + g * tiles + tile + b0) * ps_record(HD);
+  const int qr = query - tile * PS_TILE;
+  auto rec = [&](int i) { return rec0 + (i / halves) * ps_record(HD); };
+  auto row = [&](int i) { return qr + (halves == 2 ? (i & 1) * 128 : 0); };
   const float* mine = own + (int64_t)T * nh * HD + 2 * th;
   float mm = -INFINITY;
-  for (int i = lane; i <= n; i += 32) mm = fmaxf(mm, __ldcg(i < n ? rec0 + i * ps_record(HD) : mine));
+  for (int i = lane; i <= n; i += 32) mm = fmaxf(mm, i < n ? __ldcg(rec(i) + row(i)) : __ldcg(mine));
   mm = warp_max(mm);
   const float safe = mm == -INFINITY ? 0.0f : mm;
   float l = 0.0f;
   for (int i = lane; i <= n; i += 32) {
-    const float f = ps_exp2(__ldcg(i < n ? rec0 + i * ps_record(HD) : mine) - safe);
+    const float f = ps_exp2((i < n ? __ldcg(rec(i) + row(i)) : __ldcg(mine)) - safe);
     s_w[warp][i] = f;
-    l = fmaf(f, __ldcg(i < n ? rec0 + PS_TILE + i * ps_record(HD) : mine + 1), l);
+    l = fmaf(f, i < n ? __ldcg(rec(i) + PS_TILE + row(i)) : __ldcg(mine + 1), l);
   }
   l = warp_sum(l);
   __syncwarp();
-  const float* y0 = rec0 - qr + 2 * PS_TILE + (int64_t)qr * HD + lane * V;
   float y[V] = {};
   auto add = [&](const float* p, float f) {
+    if (f == 0.0f) return;                     // (a part without a key leaves no sums)
     if (V == 4) {
       const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
       y[0] = fmaf(f, v.x, y[0]); y[1] = fmaf(f, v.y, y[1]); y[V - 2] = fmaf(f, v.z, y[V - 2]); y[V - 1] = fmaf(f, v.w, y[V - 1]);
@@ -423,7 +461,7 @@ attn_shared_join_kernel(const PsPlan* __restrict__ plan, const float* __restrict
     }
   };
 #pragma unroll 8
-  for (int i = 0; i < n; ++i) add(y0 + i * ps_record(HD), s_w[warp][i]);
+  for (int i = 0; i < n; ++i) add(rec(i) + 2 * PS_TILE + (int64_t)row(i) * HD + lane * V, s_w[warp][i]);
   add(own + th * HD + lane * V, s_w[warp][n]);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint32_t w[V / 2];

@@ -10,6 +10,7 @@
 // chosen follows from the definition, not from how a kernel adds up.
 #include "api.h"
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 #include <math.h>
 
@@ -146,12 +147,13 @@ struct SelArgs {
   const int* tok_pos;
   const int* tok_seq;
   int nkv, G, count, first, last;
+  int cluster;                                   // blocks of an item: 1, 2, 4 or 8
   int* out;
 };
 
-// A block for each (token, kv head).  Pages are the rows of the matrix instruction, query heads its columns.  A lane's 16 bytes of
-// a page's codes are four of the instruction's operand words; the query's codes are laid out alike, so that the order of features within the
-// product is the memory's.
+// A cluster of blocks (one for many items) for each (token, kv head): each scores a stretch of the row's pages and puts the scores into the first one's shared memory, which
+// chooses.  Pages are the rows of the matrix instruction, query heads its columns.  A lane's 16 bytes of a page's codes are four of the instruction's operand words; the
+// query's codes are laid out alike, so that the order of features within the product is the memory's.  A warp's page numbers are asked for two steps ahead, codes one.
 template <int HD>
 __global__ void __launch_bounds__(SEL_THREADS)
 page_select_kernel(const SelArgs a) {
@@ -161,15 +163,44 @@ page_select_kernel(const SelArgs a) {
   int8_t* s_q = reinterpret_cast<int8_t*>(sel_raw);                             // [8 ng][2][HD] codes below and above zero
   float* s_scale = reinterpret_cast<float*>(s_q + ng * 8 * 2 * HD);           // [8 ng]
   uint32_t* s_key = reinterpret_cast<uint32_t*>(s_scale + ng * 8);            // [pages of the row]
-  __shared__ int s_count[2][SEL_WARPS];
-  __shared__ int s_base[SEL_WARPS + 1], s_equal[SEL_WARPS + 1];
+  __shared__ int4 s_count[2][SEL_WARPS];
+  __shared__ int s_base[SEL_WARPS], s_equal[SEL_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
-  const int t = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv;
+  const int C = a.cluster, rank = C > 1 ? (int)tc5::cluster_rank() : 0, item = blockIdx.x / C;
+  const int t = item / a.nkv, g = item - t * a.nkv;
+  if (C > 1) tc5::cluster_arrive_all();          // (the first block must have begun before its memory is written)
   pdl_trigger();
   pdl_wait();
   const int pos = __ldcg(a.tok_pos + t), seq = __ldcg(a.tok_seq + t);
   const int there = seq < 0 || seq >= a.bt_rows || pos < 0 ? 0 : min(pos / PB_PAGE + 1, a.bt_width);   // pages that the token may see
   const int* bt = a.block_table + (int64_t)max(seq, 0) * a.bt_stride;
+  const int per = ((there + C - 1) / C + 15) / 16 * 16, p_lo = min(rank * per, there), p_hi = min(p_lo + per, there);
+  constexpr int STEP = SEL_WARPS * 16;
+  struct Pages { int at[2]; };                   // pages gl and gl + 8 of a step; -1: not there
+  auto numbers = [&](int p0) {
+    Pages n;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int p = p0 + gl + 8 * e;
+      n.at[e] = p < p_hi ? __ldcg(bt + p) : -1;
+      if (n.at[e] >= a.n_pages) n.at[e] = -1;
+    }
+    return n;
+  };
+  struct Codes { uint4 w[2][L]; float scale[2]; };
+  auto codes = [&](const Pages& n) {
+    Codes c;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t at = (int64_t)max(n.at[e], 0) * a.nkv + g;
+#pragma unroll
+      for (int i = 0; i < L; ++i) c.w[e][i] = __ldcg(reinterpret_cast<const uint4*>(a.codes + at * 2 * HD + 64 * i + 16 * tl));
+      c.scale[e] = __ldcg(a.scales + at);
+    }
+    return c;
+  };
+  int p0 = p_lo + warp * 16;
+  Pages n0 = numbers(p0), n1 = numbers(p0 + STEP);
 
   for (int h = warp; h < 8 * ng; h += SEL_WARPS) {
     float x[HD / 32], m = 0.0f;
@@ -192,26 +223,15 @@ page_select_kernel(const SelArgs a) {
     }
     if (lane == 0) s_scale[h] = h < a.G ? __fdiv_rn(m, 127.0f) : -1.0f;
   }
+  Codes now = codes(n0);
+  if (C > 1) tc5::cluster_wait_all();
   __syncthreads();
 
   // ---- scores ------------------------------------------------------------------------------------------------------------------
-  for (int p0 = warp * 16; p0 < there; p0 += SEL_WARPS * 16) {
-    int64_t at[2];
-    bool held[2];
-    uint4 w[2][L];
-    float scale[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int p = p0 + gl + 8 * e, page = p < there ? __ldcg(bt + p) : -1;
-      held[e] = page >= 0 && page < a.n_pages;
-      at[e] = (int64_t)(held[e] ? page : 0) * a.nkv + g;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int i = 0; i < L; ++i) w[e][i] = __ldcg(reinterpret_cast<const uint4*>(a.codes + at[e] * 2 * HD + 64 * i + 16 * tl));
-      scale[e] = __ldcg(a.scales + at[e]);
-    }
+  const uint32_t keys = C > 1 ? tc5::cluster_addr(s_key, 0) : tc5::smem_u32(s_key);
+  for (; p0 < p_hi; p0 += STEP) {
+    const Codes next = codes(n1);                // (past the end: page 0's, not used)
+    const Pages n2 = numbers(p0 + 2 * STEP);
     float best[2] = {-INFINITY, -INFINITY};
     __syncwarp();
     for (int n = 0; n < ng; ++n) {
@@ -219,8 +239,8 @@ page_select_kernel(const SelArgs a) {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
         const uint4 b = *reinterpret_cast<const uint4*>(s_q + (n * 8 + gl) * 2 * HD + 64 * i + 16 * tl);
-        sel_mma(c, w[0][i].x, w[1][i].x, w[0][i].y, w[1][i].y, b.x, b.y);
-        sel_mma(c, w[0][i].z, w[1][i].z, w[0][i].w, w[1][i].w, b.z, b.w);
+        sel_mma(c, now.w[0][i].x, now.w[1][i].x, now.w[0][i].y, now.w[1][i].y, b.x, b.y);
+        sel_mma(c, now.w[0][i].z, now.w[1][i].z, now.w[0][i].w, now.w[1][i].w, b.z, b.w);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -233,59 +253,80 @@ page_select_kernel(const SelArgs a) {
       best[e] = fmaxf(best[e], __shfl_xor_sync(0xffffffffu, best[e], 1));
       best[e] = fmaxf(best[e], __shfl_xor_sync(0xffffffffu, best[e], 2));
       const int p = p0 + gl + 8 * e;
-      if (tl == 0 && p < there)
-        s_key[p] = !held[e] ? 0u : p < a.first || p >= there - a.last ? SEL_MUST : isinf(scale[e]) ? SEL_ODD : sel_key(__fmul_rn(best[e], scale[e]));
+      if (tl == 0 && p < p_hi) {
+        const uint32_t key = n0.at[e] < 0 ? 0u : p < a.first || p >= there - a.last ? SEL_MUST : isinf(now.scale[e]) ? SEL_ODD : sel_key(__fmul_rn(best[e], now.scale[e]));
+        if (C > 1) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(keys + 4 * p), "r"(key) : "memory");
+        else s_key[p] = key;
+      }
     }
+    now = next;
+    n0 = n1;
+    n1 = n2;
   }
-  __syncthreads();
-
-  // ---- the k-th largest place: the largest bound that k keys reach, bit by bit -------------------------------------------------------
-  int turn = 0;
-  auto reach = [&](uint32_t bound) {             // keys of at least `bound`
-    int n = 0;
-    for (int p = threadIdx.x; p < there; p += SEL_THREADS) n += s_key[p] >= bound;
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) s_count[turn][warp] = n;
+  if (C > 1) {
+    tc5::cluster_sync_all();
+    if (rank != 0) return;
+  } else {
     __syncthreads();
-    n = 0;
+  }
+
+  // ---- the k-th largest place: the largest bound that k keys reach, two bits at a time -----------------------------------------------
+  int turn = 0;
+  auto reach = [&](uint32_t b1, uint32_t b2, uint32_t b3) {            // keys of at least each bound (at most 32,768: two to a word)
+    int n12 = 0, n3 = 0;
+    for (int p = threadIdx.x; p < there; p += SEL_THREADS) {
+      const uint32_t key = s_key[p];
+      n12 += (key >= b1) + ((key >= b2) << 16);
+      n3 += key >= b3;
+    }
+    n12 = __reduce_add_sync(0xffffffffu, n12);   // (a warp has 4,096 of them at most)
+    n3 = __reduce_add_sync(0xffffffffu, n3);
+    if (lane == 0) s_count[turn][warp] = make_int4(n12 & 0xffff, n12 >> 16, n3, 0);
+    __syncthreads();
+    int4 n = s_count[turn][0];
 #pragma unroll
-    for (int i = 0; i < SEL_WARPS; ++i) n += s_count[turn][i];
+    for (int i = 1; i < SEL_WARPS; ++i) { const int4 m = s_count[turn][i]; n.x += m.x; n.y += m.y; n.z += m.z; }
     turn ^= 1;
     return n;
   };
-  const int held = reach(1u), k = min(a.count, held);
+  const int held = reach(1u, 1u, 1u).x, k = min(a.count, held);
   uint32_t bound = 0u;
+  int want = 0;                                  // of the keys at the bound
   if (k < held) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t next = bound | (1u << bit);
-      if (reach(next) >= k) bound = next;
+    int at_least = held;                         // keys that reach the bound
+    for (int bit = 30; bit >= 0 && at_least > k; bit -= 2) {
+      const uint32_t b1 = bound | 1u << bit, b2 = bound | 2u << bit, b3 = bound | 3u << bit;
+      const int4 n = reach(b1, b2, b3);
+      if (n.z >= k) { bound = b3; at_least = n.z; }
+      else if (n.y >= k) { bound = b2; at_least = n.y; }
+      else if (n.x >= k) { bound = b1; at_least = n.x; }
     }
-  } else {
-    bound = 1u;
+    if (at_least == k) bound -= 1;               // all that reach it, and none below
+    else want = k - reach(bound + 1, bound + 1, bound + 1).x;          // (more than k reach the highest place: only if all of them must be chosen)
+    if (at_least != k && bound == 0xffffffffu) want = k;
   }
-  const int above = bound == 0xffffffffu ? 0 : reach(bound + 1);
   // ---- the chosen pages in order: all above the bound, and the first of those at it ---------------------------------------------------
   // a warp has a stretch of pages: first its numbers, then its places
-  const int per = (there + SEL_THREADS - 1) / SEL_THREADS * 32, from = min(warp * per, there), to = min(from + per, there);
+  const int stretch = (there + SEL_THREADS - 1) / SEL_THREADS * 32, from = min(warp * stretch, there), to = min(from + stretch, there);
   int n_above = 0, n_equal = 0;
-  for (int p0 = from; p0 < to; p0 += 32) {
-    const uint32_t key = p0 + lane < to ? s_key[p0 + lane] : 0u;
+  for (int q0 = from; q0 < to; q0 += 32) {
+    const uint32_t key = q0 + lane < to ? s_key[q0 + lane] : 0u;
     n_above += __popc(__ballot_sync(0xffffffffu, key > bound));
-    n_equal += __popc(__ballot_sync(0xffffffffu, key == bound));
+    n_equal += __popc(__ballot_sync(0xffffffffu, q0 + lane < to && key == bound));
   }
   if (lane == 0) { s_base[warp] = n_above; s_equal[warp] = n_equal; }
   __syncthreads();
   int at = 0, equal = 0;
   for (int i = 0; i < warp; ++i) { at += s_base[i]; equal += s_equal[i]; }
-  const int want = k - above;                    // of those at the bound
   at += min(equal, want);
-  int* out = a.out + (int64_t)blockIdx.x * a.count;
-  for (int p0 = from; p0 < to; p0 += 32) {
-    const uint32_t key = p0 + lane < to ? s_key[p0 + lane] : 0u;
-    const uint32_t below = (1u << lane) - 1, eq = __ballot_sync(0xffffffffu, key == bound);
-    const bool take = key > bound || (key == bound && equal + __popc(eq & below) < want);
+  int* out = a.out + (int64_t)item * a.count;
+  for (int q0 = from; q0 < to; q0 += 32) {
+    const bool in = q0 + lane < to;
+    const uint32_t key = in ? s_key[q0 + lane] : 0u;
+    const uint32_t below = (1u << lane) - 1, eq = __ballot_sync(0xffffffffu, in && key == bound);
+    const bool take = key > bound || (in && key == bound && equal + __popc(eq & below) < want);
     const uint32_t took = __ballot_sync(0xffffffffu, take);
-    if (take) out[at + __popc(took & below)] = p0 + lane;
+    if (take) out[at + __popc(took & below)] = q0 + lane;
     at += __popc(took);
     equal += __popc(eq);
   }
@@ -305,12 +346,12 @@ extern "C" int exl3_page_bounds(const void* k_pool, int64_t n_pages, const int* 
     return ERR_BAD_ARGUMENT;
   }
   if (!aligned16(k_pool) || !aligned16(codes)) { set_error("page_bounds: the pools must be 16-byte aligned"); return ERR_ALIGNMENT; }
-  const int most = min(bt_width, (max_new - 1) / PB_PAGE + 2);      // pages that max_new tokens can touch
+  const int most = min(bt_width, max_new == 1 ? 1 : (max_new - 2) / PB_PAGE + 2);        // pages that max_new tokens can touch
   const int64_t blocks = ((int64_t)rows * most * nkv + PB_WARPS - 1) / PB_WARPS;
   if (blocks > INT32_MAX) { set_error("page_bounds: too many pages for one launch"); return ERR_UNSUPPORTED; }
   auto go = [&](auto kernel) {
     launch_pdl(kernel, dim3((unsigned)blocks), dim3(PB_WARPS * 32), 0, stream, static_cast<const __nv_bfloat16*>(k_pool), n_pages, block_table, bt_stride, bt_width, row_start,
-               row_pos0, rows, max_new == 1 ? 1 : most, nkv, static_cast<int8_t*>(codes), scales);
+               row_pos0, rows, most, nkv, static_cast<int8_t*>(codes), scales);
   };
   if (hd == 64) go(page_bounds_kernel<64>); else go(page_bounds_kernel<128>);
   return launch_status("page_bounds");
@@ -330,26 +371,34 @@ extern "C" int exl3_page_select(const void* q, int64_t q_stride, const void* cod
                                 cudaStream_t stream) {
   if (T == 0) return 0;
   if (T < 0 || nkv < 1 || nh < nkv || nh % nkv || nh / nkv > SEL_MAX_HEADS || (hd != 64 && hd != 128) || n_pages < 1 || bt_width < 1 || bt_width > SEL_MAX_PAGES || count < 1 ||
-      first < 0 || last < 1 || (int64_t)T * nkv > INT32_MAX || !q || !codes || !scales || !block_table || !tok_pos || !tok_seq || !out) {
+      first < 0 || last < 1 || (int64_t)T * nkv > INT32_MAX / 8 || !q || !codes || !scales || !block_table || !tok_pos || !tok_seq || !out) {
     set_error("page_select: needs heads of 64 or 128, at most %d query heads a key/value head, rows of at most %d pages, a count of 1 or more, and at least the last page, got %d "
               "heads on %d of %d, %d pages, count %d, first %d, last %d", SEL_MAX_HEADS, SEL_MAX_PAGES, nh, nkv, hd, bt_width, count, first, last);
     return ERR_BAD_ARGUMENT;
   }
   if (!aligned16(q) || q_stride % 8 || !aligned16(codes)) { set_error("page_select: q, its rows and the codes must be 16-byte aligned"); return ERR_ALIGNMENT; }
-  static bool configured[64] = {};
+  static int sms[64] = {};
   int dev = 0;
-  cudaGetDevice(&dev);
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("page_select: no device"); return ERR_UNSUPPORTED; }
   const int ng = ceil_div(nh / nkv, 8);
-  const size_t most = (size_t)(SEL_MAX_HEADS / 8) * 8 * (2 * 128 + 4) + (size_t)SEL_MAX_PAGES * 4, smem = (size_t)ng * 8 * (2 * hd + 4) + (size_t)bt_width * 4;
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
+  const size_t most = (size_t)SEL_MAX_HEADS * (2 * 128 + 4) + (size_t)SEL_MAX_PAGES * 4, smem = (size_t)ng * 8 * (2 * hd + 4) + (size_t)bt_width * 4;
+  if (!sms[dev]) {
     cudaError_t e = cudaFuncSetAttribute(page_select_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(page_select_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    int n = 0;
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) { set_error("page_select: cannot get %zu bytes of shared memory: %s", most, cudaGetErrorString(e)); return (int)e; }
-    if (dev >= 0 && dev < 64) configured[dev] = true;
+    sms[dev] = n;
   }
   SelArgs a = {static_cast<const __nv_bfloat16*>(q), q_stride, static_cast<const int8_t*>(codes), scales, n_pages, block_table, bt_stride, bt_width, bt_rows, tok_pos, tok_seq,
-               nkv, nh / nkv, count, first, last, out};
-  if (hd == 64) launch_pdl(page_select_kernel<64>, dim3((unsigned)(T * nkv)), dim3(SEL_THREADS), smem, stream, a);
-  else launch_pdl(page_select_kernel<128>, dim3((unsigned)(T * nkv)), dim3(SEL_THREADS), smem, stream, a);
+               nkv, nh / nkv, count, first, last, 1, out};
+  // several blocks an item while that leaves SMs idle, each with 256 pages or more
+  while (a.cluster < 8 && (int64_t)T * nkv * a.cluster * 2 <= sms[dev] && bt_width >= 512 * a.cluster) a.cluster *= 2;
+  auto go = [&](auto kernel) {
+    const dim3 grid((unsigned)(T * nkv * a.cluster));
+    if (a.cluster > 1) launch_pdl_clusters(kernel, grid, dim3(SEL_THREADS), (unsigned)a.cluster, smem, stream, a);
+    else launch_pdl(kernel, grid, dim3(SEL_THREADS), smem, stream, a);
+  };
+  if (hd == 64) go(page_select_kernel<64>); else go(page_select_kernel<128>);
   return launch_status("page_select");
 }
