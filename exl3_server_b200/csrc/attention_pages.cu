@@ -46,7 +46,9 @@ struct PgArgs {
   float* records;
   // the shared pages' parts
   const int* groups;
-  int n_groups, ps_grid;
+  int n_groups;
+  int many;                                    // whether rows of more than PS_MANY queries are another kernel's work
+  int tiles;                                   // whether the kernel before works on shared pages, or on rows of many queries
   int wait_first;                              // whether the kernel before must have ended
   float* own;                                  // rows of groups: their own pages' part goes here
 };
@@ -120,7 +122,7 @@ struct PgSmem {
   PgPlace part_of[PG_WARPS][2];
   int64_t warp_sum[PG_WARPS];
   int last[2];
-  PsPlan plan;
+  PgGroups groups;
 };
 
 // Keys are the rows of the first product and queries its columns, S^T = K Q^T (8 columns an instruction; NC of them side by side), and the second is O^T = V^T P^T: half
@@ -165,16 +167,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     sm.start[i] = start;
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
   }
-  if (a.n_groups > 0) ps_plan(sm.plan, a.groups, a.n_groups, a.row_start, a.rows, a.T, a.G, a.nkv, a.bt_width, a.ps_grid);
-  else __syncthreads();
-  auto group_of = [&](int row) {               // -1: none
-    if (LIST || a.n_groups == 0) return -1;
-    int lo = 0, hi = a.n_groups - 1;
-    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (sm.plan.row[mid] <= row) lo = mid; else hi = mid - 1; }
-    return row >= sm.plan.row[lo] && row < sm.plan.row[lo] + sm.plan.rows[lo] && sm.plan.pages[lo] > 0 ? lo : -1;
+  pg_groups(sm.groups, a.groups, LIST ? 0 : a.n_groups, a.rows, a.bt_width);
+  auto group_of = [&](int row) { return LIST ? -1 : sm.groups.of(row); };
+  auto shared_of = [&](int row) { const int j = group_of(row); return j < 0 ? 0 : sm.groups.pages[j]; };   // pages that the row shares
+  auto blocks_of = [&](int i) {                // items of a row and head
+    const int queries = sm.n_new[i] * a.G;
+    return !LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS;
   };
-  auto shared_of = [&](int row) { const int j = group_of(row); return j < 0 ? 0 : sm.plan.pages[j]; };     // pages that the row shares
-  auto blocks_of = [&](int i) { return (sm.n_new[i] * a.G + COLS - 1) / COLS; };                     // items of a row and head
   {
     int64_t run = 0;
     for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
@@ -738,17 +737,31 @@ int pg_sms(const char* what) {                 // of the current device, 0: an e
 
 // Where the warps' first parts wait, and the blocks' parts.
 static int64_t pg_record_floats(int sms, int hd) { return (int64_t)sms * (PG_WARPS * PG_MAX_COLS * hd + 2 * PG_MAX_COLS * (hd + 2)); }
-// With groups: the plan, the parts of shared pages, the rows' own parts.
-constexpr int64_t PS_PLAN_FLOATS = (sizeof(PsPlan) + 63) / 64 * 16;
-static int64_t ps_slots(int sms, int64_t T, int G, int nkv, int n_groups) { return sms + nkv * (T * G / PS_TILE + n_groups); }
-static int64_t ps_floats(int sms, int64_t T, int G, int nkv, int hd, int n_groups) {
-  return n_groups ? PS_PLAN_FLOATS + ps_slots(sms, T, G, nkv, n_groups) * ps_record(hd) + ps_own(T, G * nkv, hd) : 0;
+// With tiles: the plan, the tiles, the tokens, the tiles' parts, the rows' own parts.
+struct PsSpace { int64_t plan, tiles, tokens, records, own, end; };            // floats from the start of this part of the scratch memory
+static PsSpace ps_space(int sms, int64_t T, int G, int nkv, int hd, int tiles) {
+  PsSpace s = {};
+  auto after = [](int64_t at, int64_t n) { return (at + n + 15) / 16 * 16; };
+  s.tiles = after(0, sizeof(PsPlan) / 4);
+  s.tokens = after(s.tiles, 4 * (int64_t)tiles);
+  s.records = after(s.tokens, 4 * T);
+  s.own = after(s.records, ps_slots(sms, nkv, tiles) * ps_record(hd));
+  s.end = after(s.own, ps_own(T, G * nkv, hd));
+  return s;
+}
+// Whether rows of many tokens are the tensor cores' work, and the most tiles there can be (0: no call of that kernel).
+static bool ps_many(int64_t T, int G, int rows, int n_groups, int max_new) {
+  return (int64_t)max_new * G > PS_MANY && rows <= PS_MAX_ROWS && ps_most_tiles(T, G, n_groups, rows) <= PS_MAX_TILES;
+}
+static int64_t ps_tiles_of(int64_t T, int G, int rows, int n_groups, int max_new) {
+  if (ps_many(T, G, rows, n_groups, max_new)) return ps_most_tiles(T, G, n_groups, rows);
+  return n_groups ? T * G / PS_TILE + n_groups : 0;
 }
 
 template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int most_cols, int sms, const char* what, cudaStream_t stream) {
   for (int r0 = 0; r0 < a.rows; r0 += PG_WINDOW) {
     a.row0 = r0;
-    a.wait_first = r0 > 0 || a.n_groups == 0;
+    a.wait_first = r0 > 0 || !a.tiles;
     auto go = [&](auto kernel) { launch_pdl(kernel, dim3(sms), dim3(PG_WARPS * 32), PG_SMEM, stream, map_k, map_v, a); };
     if (most_cols <= 8) { if (hd == 64) go(attn_pages_kernel<64, 1, LIST>); else go(attn_pages_kernel<128, 1, LIST>); }
     else { if (hd == 64) go(attn_pages_kernel<64, 2, LIST>); else go(attn_pages_kernel<128, 2, LIST>); }
@@ -797,10 +810,11 @@ extern "C" int exl3_attn_pages_status() {
   return v;
 }
 
-// Floats of scratch that a call with these sizes wants; the first PG_COUNTERS must be zero before the first call and are zero after each.
-extern "C" long long exl3_attn_pages_scratch(int sms, int T, int nh, int nkv, int hd, int n_groups) {
+// Floats of scratch that a call with these sizes wants (lists: no groups, max_new 0); the first PG_COUNTERS must be zero before the first call and are zero after each.
+extern "C" long long exl3_attn_pages_scratch(int sms, int T, int rows, int nh, int nkv, int hd, int n_groups, int max_new) {
   if (nkv < 1) return 0;
-  return PG_COUNTERS + pg_record_floats(sms, hd) + ps_floats(sms, T, nh / nkv, nkv, hd, n_groups);
+  const int64_t tiles = max_new ? ps_tiles_of(T, nh / nkv, rows, n_groups, max_new) : 0;
+  return PG_COUNTERS + pg_record_floats(sms, hd) + (tiles ? ps_space(sms, T, nh / nkv, nkv, hd, (int)std::min<int64_t>(tiles, PS_MAX_TILES)).end : 0);
 }
 
 // Attention of each token over the pages that lists[token][kv head][count] names.
@@ -814,7 +828,7 @@ extern "C" int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const
   if (!tok_pos || !tok_seq || !lists || count < 1) { set_error("attn_pages: an array is missing, or lists of %d pages", count); return ERR_BAD_ARGUMENT; }
   const int sms = pg_sms("attn_pages");
   if (!sms) return ERR_UNSUPPORTED;
-  if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, nh, nkv, hd, 0)) { set_error("attn_pages: scratch too small"); return ERR_SCRATCH; }
+  if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, T, nh, nkv, hd, 0, 0)) { set_error("attn_pages: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, T, T, nh, nkv, scale, scratch);
   a.tok_pos = tok_pos; a.tok_seq = tok_seq; a.lists = lists; a.count = std::min(count, bt_width);
   a.list_stride = count; a.bt_rows = bt_rows;
@@ -835,19 +849,28 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
   }
   const int sms = pg_sms("attn_shared");
   if (!sms) return ERR_UNSUPPORTED;
-  if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, nh, nkv, hd, n_groups)) { set_error("attn_shared: scratch too small"); return ERR_SCRATCH; }
+  if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, rows, nh, nkv, hd, n_groups, max_new)) { set_error("attn_shared: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, rows, T, nh, nkv, scale, scratch);
-  a.row_start = row_start; a.row_pos0 = row_pos0; a.bt_rows = rows; a.groups = groups; a.n_groups = n_groups; a.ps_grid = sms;
-  PsPlan* plan = reinterpret_cast<PsPlan*>(scratch + PG_COUNTERS + pg_record_floats(sms, hd));
-  float* parts = reinterpret_cast<float*>(plan) + PS_PLAN_FLOATS;
-  a.own = parts + (n_groups ? ps_slots(sms, T, a.G, nkv, n_groups) * ps_record(hd) : 0);
-  if (n_groups) {
-    PsArgs p = {};
+  a.row_start = row_start; a.row_pos0 = row_pos0; a.bt_rows = rows; a.groups = groups; a.n_groups = n_groups;
+  const int64_t tiles = ps_tiles_of(T, a.G, rows, n_groups, max_new);
+  if (tiles > PS_MAX_TILES) {
+    set_error("attn_shared: %d tokens of %d query heads a key/value head are more than %d tiles of %d queries with %d groups: in one call at most that", T, a.G, PS_MAX_TILES, PS_TILE, n_groups);
+    return ERR_UNSUPPORTED;
+  }
+  a.tiles = tiles > 0;
+  a.many = ps_many(T, a.G, rows, n_groups, max_new);
+  PsArgs p = {};
+  if (tiles) {
+    float* at = scratch + PG_COUNTERS + pg_record_floats(sms, hd);
+    const PsSpace s = ps_space(sms, T, a.G, nkv, hd, (int)tiles);
     p.q = a.q; p.q_stride = q_stride; p.block_table = block_table; p.bt_stride = bt_stride; p.bt_width = bt_width; p.n_pages = (int)n_pages; p.row_start = row_start;
-    p.row_pos0 = row_pos0; p.rows = rows; p.T = T; p.nkv = nkv; p.G = a.G; p.groups = groups; p.n_groups = n_groups; p.scale_log2 = a.scale_log2; p.records = parts; p.plan = plan;
+    p.row_pos0 = row_pos0; p.rows = rows; p.T = T; p.nkv = nkv; p.G = a.G; p.groups = groups; p.n_groups = n_groups; p.many = a.many; p.scale_log2 = a.scale_log2;
+    p.plan = reinterpret_cast<PsPlan*>(at + s.plan); p.tiles = reinterpret_cast<int*>(at + s.tiles); p.tokens = reinterpret_cast<PsToken*>(at + s.tokens);
+    p.records = at + s.records;
+    a.own = at + s.own;
     rc = attn_shared_launch(p, k_pool, v_pool, hd, sms, stream);
     if (rc) return rc;
   }
   rc = pg_launch<false>(a, map_k, map_v, hd, (int)std::min((int64_t)max_new * a.G, (int64_t)PG_MAX_COLS), sms, "attn_shared", stream);
-  return rc || !n_groups ? rc : attn_shared_join(plan, parts, a.own, a.out, T, nh, nkv, hd, stream);
+  return rc || !tiles ? rc : attn_shared_join(p, a.own, a.out, hd, stream);
 }

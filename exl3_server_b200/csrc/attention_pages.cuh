@@ -1,4 +1,4 @@
-// What the attention over shared and over chosen pages have in common: the arguments, and how the shared pages' work is cut.
+// What the attention over shared and over chosen pages have in common: the caller's groups, and how the tensor cores' part of the work is cut.
 #pragma once
 
 #include "common.cuh"
@@ -9,98 +9,75 @@ constexpr int PG_PAGE = 64;                    // tokens of a page
 constexpr int PG_MAX_GROUPS = 256;             // groups of rows that share pages, in one call
 constexpr int PG_COUNTERS = 65536;             // ints at the start of the scratch memory: zero between launches
 
-// A group's entry in the caller's list: rows first .. first + rows - 1 have their first `pages` pages in common.
-struct PgGroup { int first, rows, pages; };
-
-// ---- the shared pages' work ---------------------------------------------------------------------------------------------
-// A group's queries of a key/value head are (token of the group, query head) in this order, cut into tiles of PS_TILE.  The work is the list of
-// (group, kv head, tile, page) in this order, cut into equal shares for the blocks: a share ends in the middle of a tile's pages, and
-// the parts are joined by whoever finishes the queries.  Both kernels work out the same cut from the groups.
-constexpr int PS_TILE = 256;
-constexpr int PS_MIN_PAGES = 4;                // pages of a share, at least: every part more is joined again
-
-struct PsPlan {                                // in shared memory
-  int n;                                       // groups
-  int blocks;                                  // shares
-  int64_t total;                               // pages of all tiles of all heads
-  int64_t per, rem;                            // a share has `per` pages, the first `rem` shares one more
-  int tok0[PG_MAX_GROUPS], queries[PG_MAX_GROUPS], pages[PG_MAX_GROUPS], row[PG_MAX_GROUPS], rows[PG_MAX_GROUPS];
-  int tiles_before[PG_MAX_GROUPS + 1];         // tiles of a head in the groups before
-  int64_t work_before[PG_MAX_GROUPS + 1];      // pages of tiles of a head in the groups before
-  __device__ int tiles(int j) const { return (queries[j] + PS_TILE - 1) / PS_TILE; }
-  __device__ int64_t begin(int block) const { return per * block + min((int64_t)block, rem); }
-  // the share that holds place x of the list
-  __device__ int block_of(int64_t x) const { return x < rem * (per + 1) ? (int)(x / (per + 1)) : (int)(rem + (x - rem * (per + 1)) / per); }
+// ---- the groups -------------------------------------------------------------------------------------------------------------
+// The caller's list, int32 [n, 3]: first row, rows, pages that they have in common; ascending.  A group that begins before the one ahead of it ends has no rows.
+struct PgGroups {                              // in shared memory
+  int first[PG_MAX_GROUPS], rows[PG_MAX_GROUPS], pages[PG_MAX_GROUPS];
+  int n;
+  // a row's group, -1: none
+  __device__ int of(int row) const {
+    if (n == 0) return -1;
+    int lo = 0, hi = n - 1;
+    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (first[mid] <= row) lo = mid; else hi = mid - 1; }
+    return row >= first[lo] && row < first[lo] + rows[lo] && pages[lo] > 0 ? lo : -1;
+  }
 };
-
-// By all threads of a block (it ends with a barrier).  groups: int32 [n, 3], ascending; a group that begins before the one ahead of it ends
-// has no rows.
-__device__ inline void ps_plan(PsPlan& p, const int* __restrict__ groups, int n, const int* __restrict__ row_start, int rows, int T, int G, int nkv,
-                               int bt_width, int grid) {
+// By all threads of a block; ends with a barrier.
+__device__ inline void pg_groups(PgGroups& g, const int* __restrict__ list, int n, int rows, int bt_width) {
   for (int j = threadIdx.x; j < n; j += blockDim.x) {
-    p.row[j] = __ldcg(groups + 3 * j);
-    p.rows[j] = __ldcg(groups + 3 * j + 1);
-    p.pages[j] = min(max(__ldcg(groups + 3 * j + 2), 0), bt_width);
+    g.first[j] = __ldcg(list + 3 * j);
+    g.rows[j] = __ldcg(list + 3 * j + 1);
+    g.pages[j] = min(max(__ldcg(list + 3 * j + 2), 0), bt_width);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     int end = 0;
     for (int j = 0; j < n; ++j) {
-      const int first = p.row[j];
+      const int first = g.first[j];
       const bool apart = first >= end && first < rows;
-      p.row[j] = apart ? first : end;
-      p.rows[j] = apart ? min(max(p.rows[j], 0), rows - first) : 0;
-      end = p.row[j] + p.rows[j];
+      g.first[j] = apart ? first : end;
+      g.rows[j] = apart ? min(max(g.rows[j], 0), rows - first) : 0;
+      end = g.first[j] + g.rows[j];
     }
-  }
-  __syncthreads();
-  for (int j = threadIdx.x; j < n; j += blockDim.x) {
-    const int a = min(max(__ldcg(row_start + p.row[j]), 0), T), b = min(max(__ldcg(row_start + p.row[j] + p.rows[j]), a), T);
-    p.tok0[j] = a;
-    p.queries[j] = (b - a) * G;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    p.tiles_before[0] = 0;
-    p.work_before[0] = 0;
-    for (int j = 0; j < n; ++j) {
-      p.tiles_before[j + 1] = p.tiles_before[j] + p.tiles(j);
-      p.work_before[j + 1] = p.work_before[j] + (int64_t)p.tiles(j) * p.pages[j];
-    }
-    p.n = n;
-    p.total = p.work_before[n] * nkv;
-    p.blocks = (int)min((int64_t)grid, max((int64_t)1, p.total / PS_MIN_PAGES));
-    p.per = p.total / p.blocks;
-    p.rem = p.total - p.per * p.blocks;
+    g.n = n;
   }
   __syncthreads();
 }
-// A part of the list that one block works on.
-struct PsPart {
-  int j, g, tile, p0, p1;                      // group, kv head, tile, pages
-};
-__device__ inline PsPart ps_part(const PsPlan& p, int nkv, int64_t x, int64_t end) {
-  int lo = 0, hi = p.n - 1;
-  while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (p.work_before[mid] * nkv <= x) lo = mid; else hi = mid - 1; }
-  PsPart t;
-  const int64_t r = x - p.work_before[lo] * nkv;
-  const int64_t ht = r / p.pages[lo];
-  t.j = lo;
-  t.g = (int)(ht / p.tiles(lo));
-  t.tile = (int)(ht % p.tiles(lo));
-  t.p0 = (int)(r % p.pages[lo]);
-  t.p1 = (int)min((int64_t)p.pages[lo], t.p0 + (end - x));
-  return t;
-}
-// Where a part of tile `tile` of group j and kv head g, worked on by block b, leaves its record: blocks and tiles both ascend along the list.
-__device__ inline int ps_slot(const PsPlan& p, int nkv, int j, int g, int tile, int b) {
-  return b + p.tiles_before[j] * nkv + g * p.tiles(j) + tile;
-}
-// A tile of up to 128 queries has a place for 256 all the same: the two halves of a block then take pages in turn, and leave a record's half each.
-// A record, in floats: the queries' maxima (base-2 units), their sums, their sums of values [query][hd].
-__host__ __device__ constexpr int64_t ps_record(int hd) { return (int64_t)PS_TILE * (hd + 2); }
 
-// The kernel over the shared pages (attention_shared.cu): one record for every part of a tile that a block works on.
+// ---- the tensor cores' work -----------------------------------------------------------------------------------------------------
+// Tiles of up to PS_TILE queries (token, query head of a key/value head): of a group's tokens over the pages that its rows share, and of a row of many new
+// tokens over its own pages.  The work is the list of (kv head, tile, page) in this order, cut into equal shares for the blocks: a share ends in the middle of a
+// tile's pages, and the parts are joined by another kernel.
+constexpr int PS_TILE = 256;
+constexpr int PS_MAX_TILES = 768;              // of a key/value head
+constexpr int PS_MAX_ROWS = 1024;              // rows up to which rows of many tokens have tiles of their own
+constexpr int PS_MANY = 64;                    // queries of a row and key/value head from which its own pages are the tensor cores' work
+constexpr int PS_MIN_PAGES = 4;                // pages of a share, at least: every part more is joined again
+
+struct PsPlan {                                // the head of the list, in scratch memory for the join
+  int n_tiles;
+  int blocks;                                  // shares
+  int64_t total, per, rem;                     // pages of all; a share has `per` of them, the first `rem` shares one more
+  __device__ int64_t begin(int block) const { return per * block + min((int64_t)block, rem); }
+  // the share that holds place x
+  __device__ int block_of(int64_t x) const { return x < rem * (per + 1) ? (int)(x / (per + 1)) : (int)(rem + (x - rem * (per + 1)) / per); }
+};
+// What the join needs of a token: its group's tiles and its row's own, each as the first tile's number (-1: none) and the token that this begins with.
+struct PsToken { int shared_tile, shared_tok, own_tile, own_tok; };
+
+// A part of a tile that one block works on leaves its record at the slot block + place of the tile in the list: both ascend along it.
+__host__ __device__ constexpr int64_t ps_slots(int blocks, int nkv, int tiles) { return blocks + (int64_t)nkv * tiles; }
+// Tiles of a key/value head that a call may have, at most.
+__host__ __device__ constexpr int64_t ps_most_tiles(int64_t T, int G, int groups, int64_t rows) {
+  return T * G / PS_TILE + groups + (rows < T * G / (PS_MANY + 1) ? rows : T * G / (PS_MANY + 1)) + (T * G > PS_MANY ? T * G / PS_TILE : 0);
+}
+// A record, in floats: the queries' maxima (base-2 units), their sums, their sums of values [query][hd].  A tile of up to 128 queries has a place for 256 all the
+// same: the two halves of a block then take its pages in turn, and leave a record's half each.
+__host__ __device__ constexpr int64_t ps_record(int hd) { return (int64_t)PS_TILE * (hd + 2); }
+// What the join needs beside: a row's own pages' part where it is not the tensor cores', sums of values [token][head][hd], then (maximum, sum) [token][head].
+__host__ __device__ constexpr int64_t ps_own(int64_t T, int nh, int hd) { return T * nh * (hd + 2); }
+
+// The kernel over these tiles (attention_shared.cu).
 struct PsArgs {
   const __nv_bfloat16* q;
   int64_t q_stride;
@@ -111,14 +88,15 @@ struct PsArgs {
   int rows, T, nkv, G;
   const int* groups;
   int n_groups;
+  int many;                                    // whether rows of more than PS_MANY queries have tiles of their own
   float scale_log2;
   float* records;
-  PsPlan* plan;                                // left for the join
+  PsPlan* plan;
+  PsToken* tokens;
+  int* tiles;                                  // for the join: per tile its place among all pages of a head, its pages and its queries [tiles][4]
 };
-// What the join of a query's parts needs beside the records: its row's own pages' part, sums of values [token][head][hd], then (maximum, sum) [token][head].
-__host__ __device__ constexpr int64_t ps_own(int64_t T, int nh, int hd) { return T * nh * (hd + 2); }
 cudaError_t attn_shared_prepare();             // once for a device
-int attn_shared_join(const PsPlan* plan, const float* records, const float* own, __nv_bfloat16* out, int T, int nh, int nkv, int hd, cudaStream_t stream);
 int attn_shared_launch(const PsArgs& a, const void* k_pool, const void* v_pool, int hd, int sms, cudaStream_t stream);
+int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int hd, cudaStream_t stream);
 
 }  // namespace exl3

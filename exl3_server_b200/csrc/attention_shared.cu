@@ -1,14 +1,15 @@
-// Attention over the pages that the rows of a group share, on the 5th-generation tensor cores (bfloat16, heads of 64 or 128, pages of 64 keys): the keys of a page
-// are read once for up to PS_TILE queries (token of the group, query head of the key/value head), whatever rows they belong to.
+// Attention of many queries over the same pages on the 5th-generation tensor cores (bfloat16, heads of 64 or 128, pages of 64 keys): the pages that the rows of a group
+// share, whose keys are read once for up to PS_TILE queries (token, query head of the key/value head) of whatever rows, and a row's own pages where it brings many tokens.
 //
-//   m = max_j s_j,  l = sum_j 2^(s_j - m),  y = sum_j 2^(s_j - m) V[j]    over the part's pages, s_j = (q . K[j]) * scale * log2 e
+//   m = max_j s_j,  l = sum_j 2^(s_j - m),  y = sum_j 2^(s_j - m) V[j]    over a part's pages, s_j = (q . K[j]) * scale * log2 e
 //
-// A part's (m, l, y) of every query goes to a record in float32; attention_pages.cu joins the records of a query with its own pages' part.
+// A part's (m, l, y) of every query goes to a record in float32; a second kernel joins the records of a query, with the part that attention_pages.cu worked out of its
+// row's own pages.
 //
 // Two sets of 128 queries stand side by side in a block, each with four softmax warps (thread = query = row of tensor memory), and take turns with
 // the tensor core: S = Q K^T into one of two buffers of 64 columns, P over the columns of its own S, O += P V.  The maximum that the exponentials are
 // taken against moves only when a row's true maximum has grown by more than 2^8, so that O is rescaled rarely.  Blocks are persistent, one an SM,
-// and take equal shares of the list of pages (attention_pages.cuh), whatever the groups' sizes.
+// and take equal shares of the list of pages (attention_pages.cuh), whatever the tiles' sizes.
 //
 // Every wait is bounded: a kernel that gives up leaves a code (exl3_attn_shared_status), frees its tensor memory and ends.
 #include "api.h"
@@ -21,14 +22,36 @@ namespace exl3 {
 
 using namespace tc5;
 
-constexpr int PS_STAGES = 4, PS_THREADS = 352;
+constexpr int PS_THREADS = 352;
 constexpr float PS_RESCALE_STEP = 8.0f;        // base-2 units
 constexpr uint32_t PS_BOX = PG_PAGE * 128;     // bytes of 64 features of a page
 static __device__ int g_ps_error = 0;
 
 __host__ __device__ constexpr uint32_t ps_q_bytes(int hd) { return 128 * hd * 2; }
 __host__ __device__ constexpr uint32_t ps_page_bytes(int hd) { return PG_PAGE * hd * 2; }
-__host__ __device__ constexpr uint32_t ps_smem(int hd) { return 2 * ps_q_bytes(hd) + 2 * PS_STAGES * ps_page_bytes(hd) + 256 + (uint32_t)sizeof(PsPlan) + 1024; }
+// Queries and pages share this much: two sets of queries and 4 pages of heads of 128 (10 of 64), or one set and 5 (11).
+__host__ __device__ constexpr uint32_t ps_ring(int hd) { return 196608; }
+__host__ __device__ constexpr int ps_stages(int hd, bool one) { return (int)((ps_ring(hd) - (one ? 1 : 2) * ps_q_bytes(hd)) / (2 * ps_page_bytes(hd))); }
+constexpr int PS_MAX_STAGES = 11;
+
+// The list of tiles, in shared memory.
+struct PsTiles {
+  PsPlan plan;
+  int cum[PS_MAX_TILES + 1];                   // pages of the tiles before
+  int tok0[PS_MAX_TILES], query0[PS_MAX_TILES], queries[PS_MAX_TILES], row[PS_MAX_TILES], page0[PS_MAX_TILES];
+  PgGroups groups;
+  int group_tile[PG_MAX_GROUPS], group_tok[PG_MAX_GROUPS], group_seen[PG_MAX_GROUPS];  // first tile, first token, the first token's position of the row that has the lowest
+  int row_tile[PS_MAX_ROWS];                   // a row's own first tile, -1: none
+  int warp_sum[PS_THREADS / 32];
+  int small;                                   // no tile has more than 128 queries
+  int odd_key[2][2][128];                      // per set, in turns, and feature: the first key whose value is not finite among those that not all of the tile's queries see
+  int odd[2][2];
+};
+struct PsBars {
+  uint64_t q_full[2], q_free, kv_full[PS_MAX_STAGES], kv_free[PS_MAX_STAGES], s_full[4], p_full[4], pv_done[4];
+  uint32_t tmem_slot;
+};
+__host__ __device__ constexpr uint32_t ps_smem(int hd) { return ps_ring(hd) + (uint32_t)sizeof(PsTiles) + (uint32_t)sizeof(PsBars) + 1024; }
 
 // S: M = 128, N = 64, both operands K-major; P V: N = the head's features, V as it lies (keys down, features across).
 constexpr uint32_t PS_IDESC_S = idesc_bf16(128, 64);
@@ -137,6 +160,98 @@ template <int HD> __device__ inline void ps_rescale(uint32_t taddr, float f) {
   fence_before();
 }
 
+// The list of tiles; by all threads of a block, ends with a barrier.  The same in every block.
+__device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
+  pg_groups(t.groups, a.groups, a.n_groups, a.rows, a.bt_width);
+  for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS) {
+    const int r0 = t.groups.first[j], r1 = r0 + t.groups.rows[j];
+    const int s0 = min(max(__ldcg(a.row_start + r0), 0), a.T), s1 = min(max(__ldcg(a.row_start + r1), s0), a.T);
+    t.group_tok[j] = s0;
+    t.group_tile[j] = t.groups.pages[j] > 0 ? (s1 - s0) * a.G : 0;     // (queries, for now)
+    t.group_seen[j] = INT32_MAX;
+  }
+  // rows of many tokens: their queries, for now, and what of the shared pages a group's rows see
+  const int n_rows = a.many ? a.rows : 0;
+  __syncthreads();
+  for (int r = threadIdx.x; r < a.rows; r += PS_THREADS) {
+    const int s0 = min(max(__ldcg(a.row_start + r), 0), a.T), s1 = min(__ldcg(a.row_start + r + 1), a.T), j = t.groups.of(r);
+    if (j >= 0 && s1 > s0) atomicMin(&t.group_seen[j], __ldcg(a.row_pos0 + r));
+    if (r < n_rows) t.row_tile[r] = s1 > s0 && (int64_t)(s1 - s0) * a.G > PS_MANY ? (s1 - s0) * a.G : 0;
+  }
+  __syncthreads();
+  // places: groups, then rows, a thread each, in rounds of the block
+  int n_tiles = 0, small = 1;
+  for (int i0 = 0; i0 < a.n_groups + n_rows; i0 += PS_THREADS) {
+    const int i = i0 + threadIdx.x;
+    const bool group = i < a.n_groups;
+    const int queries = group ? t.group_tile[i] : i - a.n_groups < n_rows ? t.row_tile[i - a.n_groups] : 0;
+    const int mine = (queries + PS_TILE - 1) / PS_TILE, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+    if (lane == 31) t.warp_sum[warp] = incl;
+    small &= __syncthreads_and(queries <= 128);
+    int at = n_tiles + incl - mine;
+    for (int w = 0; w < PS_THREADS / 32; ++w) { if (w < warp) at += t.warp_sum[w]; n_tiles += t.warp_sum[w]; }
+    if (i < a.n_groups + n_rows) {
+      const int row = group ? t.groups.first[i] : i - a.n_groups;
+      const int own = group ? -1 : t.groups.of(row), page0 = own >= 0 ? t.groups.pages[own] : 0;
+      const int tok0 = group ? t.group_tok[i] : queries ? min(max(__ldcg(a.row_start + row), 0), a.T) : 0;
+      const int pos0 = group || !queries ? 0 : min(__ldcg(a.row_pos0 + row), a.bt_width * PG_PAGE);
+      for (int k = 0; k < mine && at + k < PS_MAX_TILES; ++k) {
+        const int q0 = k * PS_TILE, n = min(PS_TILE, queries - q0), last = pos0 + (q0 + n - 1) / a.G;
+        t.tok0[at + k] = tok0;
+        t.query0[at + k] = q0;
+        t.queries[at + k] = n;
+        t.row[at + k] = group ? row : -1 - row;          // (below 0: the row's own pages, which its queries do not see alike)
+        t.page0[at + k] = page0;
+        // (one page at least: a query that sees nothing of its own has a part all the same)
+        t.cum[at + k + 1] = group ? t.groups.pages[i] : max(1, min(a.bt_width, (max(last, 0) + PG_PAGE) / PG_PAGE) - page0);
+      }
+      if (group) t.group_tile[i] = mine ? at : -1;
+      else t.row_tile[row] = mine ? at : -1;
+    }
+    __syncthreads();
+  }
+  n_tiles = min(n_tiles, PS_MAX_TILES);
+  if (threadIdx.x < 32) {                      // running sums, a warp
+    int run = 0;
+    for (int i0 = 0; i0 < n_tiles; i0 += 32) {
+      const int i = i0 + threadIdx.x;
+      int incl = i < n_tiles ? t.cum[i + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if ((int)threadIdx.x >= o) incl += v; }
+      if (i < n_tiles) t.cum[i + 1] = run + incl;
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (threadIdx.x == 0) {
+      PsPlan& p = t.plan;
+      t.cum[0] = 0;
+      t.small = small;
+      p.n_tiles = n_tiles;
+      p.total = (int64_t)run * a.nkv;
+      p.blocks = (int)min((int64_t)gridDim.x, max((int64_t)1, p.total / PS_MIN_PAGES));
+      p.per = p.total / p.blocks;
+      p.rem = p.total - p.per * p.blocks;
+    }
+  }
+  __syncthreads();
+}
+// A part of the list that one block works on.
+struct PsPart { int g, tile, p0, p1; };        // kv head, tile, pages of the tile
+__device__ inline PsPart ps_part(const PsTiles& t, int64_t x, int64_t end) {
+  const int all = t.cum[t.plan.n_tiles];
+  PsPart p;
+  p.g = (int)(t.plan.total <= INT32_MAX ? (uint32_t)x / (uint32_t)all : x / all);
+  const int r = (int)(x - (int64_t)p.g * all);
+  int lo = 0, hi = t.plan.n_tiles - 1;
+  while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (t.cum[mid] <= r) lo = mid; else hi = mid - 1; }
+  p.tile = lo;
+  p.p0 = r - t.cum[lo];
+  p.p1 = (int)min((int64_t)(t.cum[lo + 1] - t.cum[lo]), p.p0 + (end - x));
+  return p;
+}
+
 // warps 0-3, 4-7: softmax of the first and the second 128 queries; warp 8: S; warp 9: O; warp 10: copies of pages.
 template <int HD>
 __global__ void __launch_bounds__(PS_THREADS, 1)
@@ -145,54 +260,79 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   constexpr int BOXES = HD / 64;
   extern __shared__ unsigned char ps_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ps_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* sQ = base;                    // [2 sets][boxes][128][64]
-  unsigned char* sK = sQ + 2 * QB;             // [stages][boxes][64][64]
-  unsigned char* sV = sK + PS_STAGES * KVB;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + PS_STAGES * KVB);
-  uint64_t* q_full = bars;                     // [2 sets] Q is there
-  uint64_t* kv_full = q_full + 2;              // [stages] a page's keys and values are there
-  uint64_t* kv_free = kv_full + PS_STAGES;     // [stages] the products that read it are done
-  uint64_t* s_full = kv_free + PS_STAGES;      // [2 sets][2] scores
-  uint64_t* p_full = s_full + 4;               // [2 sets][2] probabilities, by four warps
-  uint64_t* pv_done = p_full + 4;              // [2 sets][2] O += P V
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
-  PsPlan& plan = *reinterpret_cast<PsPlan*>(reinterpret_cast<unsigned char*>(bars) + 256);
+  PsBars& bars = *reinterpret_cast<PsBars*>(base + ps_ring(HD));
+  PsTiles& tiles = *reinterpret_cast<PsTiles*>(base + ps_ring(HD) + sizeof(PsBars));
+  uint64_t *q_full = bars.q_full, *kv_full = bars.kv_full, *kv_free = bars.kv_free, *s_full = bars.s_full, *p_full = bars.p_full, *pv_done = bars.pv_done;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(q_full + i, 4);
-    for (int i = 0; i < PS_STAGES; ++i) { mbar_init(kv_full + i, 1); mbar_init(kv_free + i, 1); }
+    mbar_init(&bars.q_free, 1);
+    for (int i = 0; i < PS_MAX_STAGES; ++i) { mbar_init(kv_full + i, 1); mbar_init(kv_free + i, 1); }
     for (int i = 0; i < 4; ++i) { mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(pv_done + i, 1); }
     mbar_init_fence();
   }
-  if (warp == 8) tmem_alloc<512>(tmem_slot);
+  if (warp == 8) tmem_alloc<512>(&bars.tmem_slot);
   fence_before();
   __syncthreads();
   fence_after();
   // The kernel that walks the rows' own pages may start when all that it reads beside the records is there: after this.
   pdl_wait();
   pdl_trigger();
-  ps_plan(plan, a.groups, a.n_groups, a.row_start, a.rows, a.T, a.G, a.nkv, a.bt_width, gridDim.x);
-  if (blockIdx.x == 0)                         // (for the join)
-    for (int i = threadIdx.x; i < (int)(sizeof(PsPlan) / 4); i += PS_THREADS) reinterpret_cast<int*>(a.plan)[i] = reinterpret_cast<const int*>(&plan)[i];
-  const uint32_t tmem = *tmem_slot;            // columns: scores of set s at 128 s, O at 256 + 128 s
+  ps_tiles(tiles, a);
+  const PsPlan& plan = tiles.plan;
+  // for the join: the plan, the tiles, and every token's
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *a.plan = plan;
+    for (int i = threadIdx.x; i < plan.n_tiles; i += PS_THREADS)
+      reinterpret_cast<int4*>(a.tiles)[i] = make_int4(tiles.cum[i], tiles.cum[i + 1] - tiles.cum[i], tiles.queries[i], tiles.cum[plan.n_tiles]);
+  }
+  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const int s0 = min(max(__ldcg(a.row_start + r), 0), a.T), s1 = min(__ldcg(a.row_start + r + 1), a.T), j = tiles.groups.of(r);
+    PsToken w;
+    w.shared_tile = j >= 0 ? tiles.group_tile[j] : -1;
+    w.shared_tok = j >= 0 ? tiles.group_tok[j] : 0;
+    w.own_tile = a.many ? tiles.row_tile[r] : -1;
+    w.own_tok = s0;
+    for (int i = s0 + threadIdx.x; i < s1; i += PS_THREADS) reinterpret_cast<int4*>(a.tokens)[i] = make_int4(w.shared_tile, w.shared_tok, w.own_tile, w.own_tok);
+  }
+  {                                            // (tokens of no row)
+    const int t0 = min(max(__ldcg(a.row_start), 0), a.T), t1 = min(max(__ldcg(a.row_start + a.rows), 0), a.T);
+    for (int i = blockIdx.x * PS_THREADS + threadIdx.x; i < a.T; i += gridDim.x * PS_THREADS)
+      if (i < t0 || i >= t1) reinterpret_cast<int4*>(a.tokens)[i] = make_int4(-1, 0, -1, 0);
+  }
+  const uint32_t tmem = bars.tmem_slot;        // columns: scores of set s at 128 s, O at 256 + 128 s
   const int64_t lo = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x) : 0, hi = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x + 1) : 0;
-  // Tiles of more than 128 queries: both sets take every page, 128 queries each.  Smaller ones: the sets take the pages in turn, with the same queries.
-  auto both = [&](const PsPart& t) { return plan.queries[t.j] - t.tile * PS_TILE > 128; };
+  // Tiles of more than 128 queries: both sets take every page, 128 queries each.  Smaller ones: the sets take the pages in turn, with the same queries, and where there
+  // are only such tiles one copy of them, which leaves room for more pages: a page's stage is taken for a copy's way and two pages' softmax, and with 4 stages
+  // a page took 0.86 us.
+  auto both = [&](const PsPart& t) { return tiles.queries[t.tile] > 128; };
+  const bool one = tiles.small != 0;
+  const int stages = ps_stages(HD, one);
+  unsigned char* const sQ = base;              // [1 or 2 sets][boxes][128][64]
+  unsigned char* const sK = sQ + (one ? 1 : 2) * QB;       // [stages][boxes][64][64]
+  unsigned char* const sV = sK + stages * KVB;
+  const uint32_t second_q = one ? 0 : QB;
   bool ok = true;
 
   if (warp == 10) {
-    // ---- copies; page numbers come 32 at a time -------------------------------------------------------------------------
-    int c = 0;
+    // ---- copies; page numbers come 32 at a time, a batch ahead ------------------------------------------------------------------
+    int c = 0, st = 0;
+    uint32_t phase = 1;                        // of the stage's being free again
     for (int64_t x = lo; x < hi && ok;) {
-      const PsPart t = ps_part(plan, a.nkv, x, hi);
-      const int* bt = a.block_table + (int64_t)plan.row[t.j] * a.bt_stride;
+      const PsPart t = ps_part(tiles, x, hi);
+      const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile];
+      const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
+      auto numbers = [&](int p) {              // beyond the pool: zeros, hidden by the softmax
+        const int n = p + lane < t.p1 && p_off + p + lane < a.bt_width ? __ldcg(bt + p + lane) : a.n_pages;
+        return n < 0 || n > a.n_pages ? a.n_pages : n;
+      };
+      int page = numbers(t.p0);
       for (int p = t.p0; p < t.p1 && ok; p += 32) {
-        int page = p + lane < t.p1 ? __ldcg(bt + p + lane) : 0;
-        if (page < 0 || page > a.n_pages) page = a.n_pages;            // beyond the pool: zeros, hidden by the softmax
+        const int ahead = numbers(p + 32);
         for (int i = 0; i < min(32, t.p1 - p); ++i, ++c) {
-          const int st = c % PS_STAGES, y = (__shfl_sync(0xffffffffu, page, i) * a.nkv + t.g) * PG_PAGE;
-          if (c >= PS_STAGES && !ps_wait(kv_free + st, (c / PS_STAGES - 1) & 1)) { ok = false; break; }
+          const int y = (__shfl_sync(0xffffffffu, page, i) * a.nkv + t.g) * PG_PAGE;
+          if (c >= stages && !ps_wait(kv_free + st, phase)) { ok = false; break; }
           if (lane == 0) {
             mbar_expect_tx(kv_full + st, 2 * KVB);
 #pragma unroll
@@ -202,22 +342,24 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             }
           }
           __syncwarp();
+          if (++st == stages) { st = 0; phase ^= 1; }
         }
+        page = ahead;
       }
       x += t.p1 - t.p0;
     }
     // what was asked for must land before the block's shared memory goes away
     if (!ok && lane == 0) atomicExch(&g_ps_error, 1);
-    for (int u = max(0, c - PS_STAGES); u < c; ++u) ps_wait(kv_full + u % PS_STAGES, (u / PS_STAGES) & 1);
+    for (int u = max(0, c - stages); u < c; ++u) ps_wait(kv_full + u % stages, (u / stages) & 1);
   } else if (warp == 8) {
     // ---- S = Q K^T, up to two pages ahead of the softmax -------------------------------------------------------------------
-    int c = 0, f[2] = {0, 0}, k[2] = {0, 0};   // pages, pages of a set, parts of a set so far
+    int st = 0, f[2] = {0, 0}, k[2] = {0, 0};  // pages of a set, parts of a set so far
+    uint32_t phase = 0;
     for (int64_t x = lo; x < hi && ok;) {
-      const PsPart t = ps_part(plan, a.nkv, x, hi);
+      const PsPart t = ps_part(tiles, x, hi);
       const bool two = both(t);
-      for (int p = t.p0; p < t.p1 && ok; ++p, ++c) {
-        const int st = c % PS_STAGES;
-        if (!ps_wait(kv_full + st, (c / PS_STAGES) & 1)) { ok = false; break; }
+      for (int p = t.p0; p < t.p1 && ok; ++p) {
+        if (!ps_wait(kv_full + st, phase)) { ok = false; break; }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (!two && ((p - t.p0) & 1) != s) continue;
@@ -228,15 +370,17 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           if (lane == 0) {
 #pragma unroll
             for (int b = 0; b < BOXES; ++b) {
-              const uint64_t da = smem_desc_k128(smem_u32(sQ + s * QB + b * 128 * 128)), db = smem_desc_k128(smem_u32(sK + st * KVB + b * PS_BOX));
+              const uint64_t da = smem_desc_k128(smem_u32(sQ + s * second_q + b * 128 * 128)), db = smem_desc_k128(smem_u32(sK + st * KVB + b * PS_BOX));
 #pragma unroll
               for (int i = 0; i < 4; ++i) mma_ss(tmem + 128 * s + 64 * sb, da + 2 * i, db + 2 * i, PS_IDESC_S, (b | i) > 0);
             }
             mma_commit(s_full + 2 * s + sb);
+            if (one && p == t.p1 - 1) mma_commit(&bars.q_free);        // (the sets share the queries' place)
           }
           __syncwarp();
           ++f[s];
         }
+        if (++st == stages) { st = 0; phase ^= 1; }
       }
       ++k[0];
       k[1] += two || t.p1 - t.p0 > 1;          // (a set without a page asks for no queries)
@@ -245,12 +389,49 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     if (!ok && lane == 0) atomicExch(&g_ps_error, 2);
   } else if (warp == 9) {
     // ---- O += P V ----------------------------------------------------------------------------------------------------------------
-    int c = 0, f[2] = {0, 0};
+    int st = 0, f[2] = {0, 0}, k[2] = {0, 0};
+    uint32_t phase = 0;
     for (int64_t x = lo; x < hi && ok;) {
-      const PsPart t = ps_part(plan, a.nkv, x, hi);
+      const PsPart t = ps_part(tiles, x, hi);
       const bool two = both(t);
-      for (int p = t.p0; p < t.p1 && ok; ++p, ++c) {
-        const int st = c % PS_STAGES;
+      const int row = tiles.row[t.tile], q0 = tiles.query0[t.tile];
+      // a row's own pages: the last keys that the tile's first and last queries see
+      const int own_pos = row < 0 ? min(__ldcg(a.row_pos0 - 1 - row), a.bt_width * PG_PAGE) : 0;
+      const int first_limit = row < 0 ? own_pos + q0 / a.G : INT32_MAX, last_limit = own_pos + (q0 + tiles.queries[t.tile] - 1) / a.G;
+      for (int p = t.p0; p < t.p1 && ok; ++p) {
+        const int key0 = (tiles.page0[t.tile] + p) * PG_PAGE;
+        if (row < 0 && key0 + PG_PAGE - 1 > first_limit) {
+          // Values that not all queries see: a probability of 0 is multiplied with them all the same, so those that are not finite become zeros here, and the softmax
+          // threads are told from which key on a feature is not finite (when they are known to have begun the part: they have handed over P).
+          if (!ps_wait(kv_full + st, phase)) { ok = false; break; }
+          for (int s = 0; s < 2; ++s)
+            if ((two || ((p - t.p0) & 1) == s) && !ps_wait(p_full + 2 * s + (f[s] & 1), (f[s] >> 1) & 1)) { ok = false; break; }
+          if (!ok) break;
+          for (int w = lane; w < PG_PAGE * (HD / 8); w += 32) {
+            const int key = w / (HD / 8), c = w % (HD / 8);
+            if (key0 + key <= first_limit) continue;
+            uint4* at = reinterpret_cast<uint4*>(sV + st * KVB + (c >> 3) * PS_BOX + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+            uint4 v = *at;
+            uint32_t* word = reinterpret_cast<uint32_t*>(&v);
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t bits = e & 1 ? 0x7f800000u : 0x7f80u;
+              if ((word[e >> 1] & bits) != bits) continue;
+              word[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+              any = true;
+              if (key0 + key <= last_limit) {
+                const int set = two ? -1 : (p - t.p0) & 1;
+                for (int s = 0; s < 2; ++s)
+                  if (set < 0 || set == s) { atomicMin(&tiles.odd_key[s][k[s] & 1][8 * c + e], key0 + key); tiles.odd[s][k[s] & 1] = 1; }
+              }
+            }
+            if (any) *at = v;
+          }
+          fence_smem_to_tma();
+          __threadfence_block();
+          __syncwarp();
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (!two && ((p - t.p0) & 1) != s) continue;
@@ -269,7 +450,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           __syncwarp();
           ++f[s];
         }
+        if (++st == stages) { st = 0; phase ^= 1; }
       }
+      ++k[0];
+      k[1] += two || t.p1 - t.p0 > 1;
       x += t.p1 - t.p0;
     }
     if (!ok && lane == 0) atomicExch(&g_ps_error, 3);
@@ -278,22 +462,27 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + 128 * s, to = tmem + lanes + 256 + 128 * s;
-    int f = 0;
-    for (int64_t x = lo; x < hi && ok;) {
-      const PsPart t = ps_part(plan, a.nkv, x, hi);
+    int f = 0, parts = 0, mine = 0;            // the set's pages so far, all parts, the set's
+    for (int64_t x = lo; x < hi && ok; ++parts) {
+      const PsPart t = ps_part(tiles, x, hi);
       x += t.p1 - t.p0;
+      if (one && parts > 0 && !ps_wait(&bars.q_free, (parts - 1) & 1)) { ok = false; break; }        // (every part's, whether the set has pages of it or not)
       const bool two = both(t);
       const int step = two ? 1 : 2, first = t.p0 + (two ? 0 : s), qr = s * 128 + r;
-      const int query = t.tile * PS_TILE + (two ? qr : r);
-      float* rec = a.records + ps_slot(plan, a.nkv, t.j, t.g, t.tile, blockIdx.x) * ps_record(HD);
+      const int in_tile = two ? qr : r;
+      float* rec = a.records + (blockIdx.x + (int64_t)t.g * plan.n_tiles + t.tile) * ps_record(HD);
       if (first >= t.p1) {                     // no page for this set
         rec[qr] = -INFINITY;
         rec[PS_TILE + qr] = 0.0f;
         continue;
       }
-      const bool in = query < plan.queries[t.j];
-      const int tok = plan.tok0[t.j] + (in ? query / a.G : 0), head = t.g * a.G + (in ? query % a.G : 0);
+      const bool in = in_tile < tiles.queries[t.tile];
+      const int query = tiles.query0[t.tile] + (in ? in_tile : 0), step_tok = query / a.G;
+      const int tok = tiles.tok0[t.tile] + step_tok, head = t.g * a.G + query - step_tok * a.G;
       // Q: this thread's row, into the operand's layout (the last S that read the place before is done)
+      const int turn = mine++ & 1;
+      if (r < 32) for (int d = r; d < HD; d += 32) tiles.odd_key[s][turn][d] = INT32_MAX;
+      if (r == 0) tiles.odd[s][turn] = 0;
       {
         const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.q_stride + (int64_t)head * HD);
         uint4 w[HD / 8];
@@ -301,18 +490,28 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int i = 0; i < HD / 8; ++i) w[i] = in ? __ldcg(src + i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i)
-          *reinterpret_cast<uint4*>(sQ + s * QB + (i >> 3) * 128 * 128 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = w[i];
+          *reinterpret_cast<uint4*>(sQ + s * second_q + (i >> 3) * 128 * 128 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = w[i];
         fence_smem_to_tma();
         ps_arrive_warp(q_full + s);
       }
-      // the first key that this query does not see, and whether some page of the part is not there
-      int row_lo = plan.row[t.j], row_hi = plan.row[t.j] + plan.rows[t.j] - 1;
-      while (row_lo < row_hi) { const int mid = (row_lo + row_hi + 1) >> 1; if (__ldcg(a.row_start + mid) <= tok) row_lo = mid; else row_hi = mid - 1; }
-      const int pos = min(__ldcg(a.row_pos0 + row_lo), a.bt_width * PG_PAGE) + tok - __ldcg(a.row_start + row_lo);
-      const int* bt = a.block_table + (int64_t)plan.row[t.j] * a.bt_stride;
-      bool odd = false;
-      for (int p = t.p0 + lane; p < t.p1; p += 32) { const int page = __ldcg(bt + p); odd |= page < 0 || page >= a.n_pages; }
-      odd = __any_sync(0xffffffffu, odd);
+      // the last key that this query sees, and whether some page of the part is not there
+      const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile];
+      int pos;
+      if (row < 0) {
+        pos = min(__ldcg(a.row_pos0 - 1 - row), a.bt_width * PG_PAGE) + step_tok;
+      } else {                                 // (shared pages, seen by all as a rule)
+        const int j = tiles.groups.of(row);
+        pos = INT32_MAX;
+        if (tiles.group_seen[j] < (p_off + t.p1) * PG_PAGE - 1) {
+          int row_lo = row, row_hi = row + tiles.groups.rows[j] - 1;
+          while (row_lo < row_hi) { const int mid = (row_lo + row_hi + 1) >> 1; if (__ldcg(a.row_start + mid) <= tok) row_lo = mid; else row_hi = mid - 1; }
+          pos = min(__ldcg(a.row_pos0 + row_lo), a.bt_width * PG_PAGE) + tok - __ldcg(a.row_start + row_lo);
+        }
+      }
+      const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
+      bool holes = false;
+      for (int p = t.p0 + lane; p < t.p1; p += 32) { const int page = p_off + p < a.bt_width ? __ldcg(bt + p) : -1; holes |= page < 0 || page >= a.n_pages; }
+      holes = __any_sync(0xffffffffu, holes);
       const int sees = __reduce_min_sync(0xffffffffu, pos);              // all of the warp's queries see keys up to here
       float m_used = -INFINITY, l = 0.0f;
       uint32_t s0[32], s1[32];
@@ -328,10 +527,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int sb = f & 1;
         tmem_ld_wait(s0);
         tmem_ld_wait(s1);
-        const int key0 = p * PG_PAGE;
-        if (key0 + PG_PAGE - 1 > sees || odd) {
+        const int key0 = (p_off + p) * PG_PAGE;
+        if (key0 + PG_PAGE - 1 > sees || holes) {
           int last = pos;
-          if (odd) { const int page = __ldcg(bt + p); if (page < 0 || page >= a.n_pages) last = -1; }
+          if (holes) { const int page = p_off + p < a.bt_width ? __ldcg(bt + p) : -1; if (page < 0 || page >= a.n_pages) last = -1; }
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             if (key0 + c > last) s0[c] = 0xff800000u;
@@ -371,10 +570,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       if (!ok) break;
       fence_after();
       if (in) { rec[qr] = m_used; rec[PS_TILE + qr] = l; }
+      const bool odd = tiles.odd[s][turn] != 0;          // (written before the product that has ended)
 #pragma unroll
       for (int h = 0; h < HD / 32; ++h) {
         __syncwarp();
         tmem_ld32(to + 32 * h, s0);
+        if (odd) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (tiles.odd_key[s][turn][32 * h + c] <= pos) s0[c] = 0x7fc00000u;
+        }
         if (in) {
 #pragma unroll
           for (int c = 0; c < 32; c += 8) ps_store8(rec + 2 * PS_TILE + (int64_t)qr * HD + 32 * h + c, s0 + c);
@@ -392,89 +597,122 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   if (warp == 8) tmem_free<512>(tmem);
 }
 
-// Joins the parts of a query: a warp for each (token, head).  The parts of the shared pages are in the order of the pages, the own pages' part is the last, so
-// a result does not depend on which block was the first to end.
-constexpr int PJ_WARPS = 4, PJ_PARTS = 512;               // two for every SM, at most
-template <int HD>
+// Joins the parts of a query: PJ_WARPS / SPLIT (token, head) pairs a block, SPLIT warps each.  The parts of the shared pages come first, in the order of the pages, those of the
+// row's own pages last, so a result does not depend on which block was the first to end.
+constexpr int PJ_WARPS = 4;
+constexpr int PJ_PARTS = 1024;                 // four for every SM, at most
+template <int HD, int SPLIT>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
-attn_shared_join_kernel(const PsPlan* __restrict__ plan, const float* __restrict__ records, const float* __restrict__ own, __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
-  constexpr int V = HD / 32;                   // features a lane
-  __shared__ float s_w[PJ_WARPS][PJ_PARTS + 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t th = (int64_t)blockIdx.x * PJ_WARPS + warp;
+attn_shared_join_kernel(const PsPlan* __restrict__ plan, const int4* __restrict__ tiles, const int4* __restrict__ tokens, const float* __restrict__ records,
+                        const float* __restrict__ own, __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
+  constexpr int V = HD / 32, PAIRS = PJ_WARPS / SPLIT;       // features a lane; pairs a block
+  __shared__ float s_w[PAIRS][PJ_PARTS + 1];
+  __shared__ float s_y[SPLIT > 1 ? PJ_WARPS : 1][SPLIT > 1 ? HD : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pair = warp / SPLIT, w0 = warp % SPLIT;
+  const int64_t th = (int64_t)blockIdx.x * PAIRS + pair;
   pdl_trigger();
   pdl_wait();
-  if (th >= (int64_t)T * nh) return;
-  const int tok = (int)(th / nh), head = (int)(th - (int64_t)tok * nh), G = nh / nkv, g = head / G;
-  // the token's group: the last that begins at or before it; lanes side by side, all of a group's numbers at once
-  const int n_groups = __ldcg(&plan->n), blocks_per = (int)min(__ldcg(&plan->per), (int64_t)INT32_MAX);
-  const int64_t rem = __ldcg(&plan->rem), per = blocks_per;
-  int tok0 = -1, queries = 0, pages = 0, tiles_before = 0;
-  int64_t work_before = 0;
-  for (int j0 = 0; j0 < n_groups; j0 += 32) {
-    const int j = min(j0 + lane, n_groups - 1);
-    const int t0 = __ldcg(&plan->tok0[j]), q0 = __ldcg(&plan->queries[j]), p0 = __ldcg(&plan->pages[j]), b0 = __ldcg(&plan->tiles_before[j]);
-    const int64_t w0 = __ldcg(&plan->work_before[j]);
-    const unsigned here = __ballot_sync(0xffffffffu, j0 + lane < n_groups && t0 <= tok && q0 > 0);
-    if (here) {
-      const int src = 31 - __clz(here);
-      tok0 = __shfl_sync(0xffffffffu, t0, src);
-      queries = __shfl_sync(0xffffffffu, q0, src);
-      pages = __shfl_sync(0xffffffffu, p0, src);
-      tiles_before = __shfl_sync(0xffffffffu, b0, src);
-      work_before = __shfl_sync(0xffffffffu, w0, src);
-    }
-  }
-  const int query = (tok - tok0) * G + head - g * G;
-  if (tok0 < 0 || query >= queries || pages == 0) return;              // in no group: its own pages' part was all
-  const int tile = query / PS_TILE, tiles = (queries + PS_TILE - 1) / PS_TILE;
-  const int64_t first = work_before * nkv + ((int64_t)g * tiles + tile) * pages, longer = rem * (per + 1);
-  auto block_of = [&](int64_t x) { return x < longer ? (int)(x / (per + 1)) : (int)(rem + (x - longer) / per); };
-  const int b0 = block_of(first), halves = queries - tile * PS_TILE > 128 ? 1 : 2;
-  const int n = (block_of(first + pages - 1) - b0 + 1) * halves;       // parts: at most two for every SM
-  const float* rec0 = records + (tiles_before * nkv + g * tiles + tile + b0) * ps_record(HD);
-  const int qr = query - tile * PS_TILE;
-  auto rec = [&](int i) { return rec0 + (i / halves) * ps_record(HD); };
-  auto row = [&](int i) { return qr + (halves == 2 ? (i & 1) * 128 : 0); };
-  const float* mine = own + (int64_t)T * nh * HD + 2 * th;
-  float mm = -INFINITY;
-  for (int i = lane; i <= n; i += 32) mm = fmaxf(mm, i < n ? __ldcg(rec(i) + row(i)) : __ldcg(mine));
-  mm = warp_max(mm);
-  const float safe = mm == -INFINITY ? 0.0f : mm;
-  float l = 0.0f;
-  for (int i = lane; i <= n; i += 32) {
-    const float f = ps_exp2((i < n ? __ldcg(rec(i) + row(i)) : __ldcg(mine)) - safe);
-    s_w[warp][i] = f;
-    l = fmaf(f, i < n ? __ldcg(rec(i) + PS_TILE + row(i)) : __ldcg(mine + 1), l);
-  }
-  l = warp_sum(l);
-  __syncwarp();
-  float y[V] = {};
-  auto add = [&](const float* p, float f) {
-    if (f == 0.0f) return;                     // (a part without a key leaves no sums)
-    if (V == 4) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
-      y[0] = fmaf(f, v.x, y[0]); y[1] = fmaf(f, v.y, y[1]); y[V - 2] = fmaf(f, v.z, y[V - 2]); y[V - 1] = fmaf(f, v.w, y[V - 1]);
-    } else {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
-      y[0] = fmaf(f, v.x, y[0]); y[1] = fmaf(f, v.y, y[1]);
-    }
+  const bool there = th < (int64_t)T * nh;
+  if (SPLIT == 1 && !there) return;
+  const int tok = there ? (int)(th / nh) : 0, head = there ? (int)(th - (int64_t)tok * nh) : 0, G = nh / nkv, g = head / G, h = head - g * G;
+  const int4 w = __ldcg(tokens + tok);         // (shared tile, its first token, own tile, its first token)
+  const int n_tiles = __ldcg(&plan->n_tiles);
+  const int64_t per = __ldcg(&plan->per), rem = __ldcg(&plan->rem), longer = rem * (per + 1);
+  auto share_of = [&](int64_t x) {
+    if (longer + per * 1024 <= INT32_MAX && x <= INT32_MAX)              // (as a rule)
+      return x < longer ? (int)((uint32_t)x / (uint32_t)(per + 1)) : (int)rem + (int)((uint32_t)(x - longer) / (uint32_t)per);
+    return x < longer ? (int)(x / (per + 1)) : (int)(rem + (x - longer) / per);
   };
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) add(rec(i) + 2 * PS_TILE + (int64_t)row(i) * HD + lane * V, s_w[warp][i]);
-  add(own + th * HD + lane * V, s_w[warp][n]);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint32_t w[V / 2];
+  // a source: the parts of one tile
+  struct Source { const float* at; int n, halves, row; };     // its first record, its parts, and the query's place in a record
+  auto source = [&](int tile0, int tok0) {
+    Source s = {records, 0, 1, 0};
+    const int query = (tok - tok0) * G + h, tile = tile0 + query / PS_TILE;
+    if (tile0 < 0 || query < 0 || tile >= n_tiles) return s;
+    const int4 t = __ldcg(tiles + tile);
+    const int64_t first = (int64_t)g * t.w + t.x;
+    const int b0 = share_of(first);
+    s.halves = t.z > 128 ? 1 : 2;
+    s.n = (share_of(first + t.y - 1) - b0 + 1) * s.halves;
+    s.row = query % PS_TILE;
+    s.at = records + (b0 + (int64_t)g * n_tiles + tile) * ps_record(HD);
+    return s;
+  };
+  const bool any = there && (w.x >= 0 || w.z >= 0);          // else its own pages' part was all
+  if (SPLIT == 1 && !any) return;
+  const Source s0 = source(any ? w.x : -1, w.y), s1 = source(any ? w.z : -1, w.w);
+  const int n01 = s0.n + s1.n, n = any ? n01 + (w.z < 0 ? 1 : 0) : 0;    // (no tile for the row's own pages: the walk's part)
+  const float* mine = own + (int64_t)T * nh * HD + 2 * th;
+  // part i: its record, and the query's place in it; the walk's part is the last
+  auto part = [&](int i, int& row) {
+    const bool second = i >= s0.n;
+    const int k = second ? i - s0.n : i, halves = second ? s1.halves : s0.halves;
+    row = (second ? s1.row : s0.row) + (halves == 2 ? (k & 1) * 128 : 0);
+    return (second ? s1.at : s0.at) + (halves == 2 ? k >> 1 : k) * ps_record(HD);
+  };
+  float mm = -INFINITY, l = 0.0f;
+  for (int i = lane; i < n; i += 32) {
+    int row = 0;
+    const float* p = i < n01 ? part(i, row) : mine;
+    const float m1 = __ldcg(p + row), l1 = __ldcg(p + row + (i < n01 ? PS_TILE : 1)), top = fmaxf(mm, m1), safe = top == -INFINITY ? 0.0f : top;
+    l = l * ps_exp2(mm - safe) + l1 * ps_exp2(m1 - safe);
+    mm = top;
+    if (w0 == 0) s_w[pair][i] = m1;
+  }
+  const float top = warp_max(mm), safe = top == -INFINITY ? 0.0f : top;
+  l = warp_sum(l * ps_exp2(mm - safe));
+  if (SPLIT > 1) __syncthreads(); else __syncwarp();
+  float y[V] = {};
+  constexpr int BATCH = 8;
+  for (int i0 = w0; i0 < n; i0 += SPLIT * BATCH) {
+    float v[BATCH][V], f[BATCH];
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) w[i] = ps_pack(y[2 * i] * inv, y[2 * i + 1] * inv);
-  if (V == 4) *reinterpret_cast<uint2*>(out + th * HD + lane * V) = make_uint2(w[0], w[V / 2 - 1]);
-  else *reinterpret_cast<uint32_t*>(out + th * HD + lane * V) = w[0];
+    for (int b = 0; b < BATCH; ++b) {
+      const int i = i0 + b * SPLIT;
+      f[b] = 0.0f;
+      if (i < n) {
+        int row = 0;
+        const float* p = i < n01 ? part(i, row) + 2 * PS_TILE : own + th * HD;
+        p += row * HD;
+        f[b] = ps_exp2(s_w[pair][i] - safe);
+        if (V == 4) { const float4 x = __ldcg(reinterpret_cast<const float4*>(p + lane * V)); v[b][0] = x.x; v[b][1] = x.y; v[b][V - 2] = x.z; v[b][V - 1] = x.w; }
+        else { const float2 x = __ldcg(reinterpret_cast<const float2*>(p + lane * V)); v[b][0] = x.x; v[b][1] = x.y; }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (f[b] != 0.0f) y[e] = fmaf(f[b], v[b][e], y[e]);          // (a part without a key leaves no sums)
+  }
+  if (SPLIT > 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_y[warp][lane * V + e] = y[e];
+    __syncthreads();
+    if (w0 != 0 || !any) return;
+#pragma unroll
+    for (int k = 1; k < SPLIT; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] += s_y[warp + k][lane * V + e];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint32_t o[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) o[i] = ps_pack(y[2 * i] * inv, y[2 * i + 1] * inv);
+  if (V == 4) *reinterpret_cast<uint2*>(out + th * HD + lane * V) = make_uint2(o[0], o[V / 2 - 1]);
+  else *reinterpret_cast<uint32_t*>(out + th * HD + lane * V) = o[0];
 }
 
-int attn_shared_join(const PsPlan* plan, const float* records, const float* own, __nv_bfloat16* out, int T, int nh, int nkv, int hd, cudaStream_t stream) {
-  const dim3 grid((unsigned)(((int64_t)T * nh + PJ_WARPS - 1) / PJ_WARPS)), block(PJ_WARPS * 32);
-  if (hd == 64) launch_pdl(attn_shared_join_kernel<64>, grid, block, 0, stream, plan, records, own, out, T, nh, nkv);
-  else launch_pdl(attn_shared_join_kernel<128>, grid, block, 0, stream, plan, records, own, out, T, nh, nkv);
+int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int hd, cudaStream_t stream) {
+  // few queries: a block each, since a query of a few may have hundreds of parts
+  const int64_t pairs = (int64_t)a.T * a.nkv * a.G;
+  const bool few = pairs <= 4096;
+  auto go = [&](auto kernel, int per_block) {
+    launch_pdl(kernel, dim3((unsigned)((pairs + per_block - 1) / per_block)), dim3(PJ_WARPS * 32), 0, stream, (const PsPlan*)a.plan, reinterpret_cast<const int4*>(a.tiles),
+               reinterpret_cast<const int4*>(a.tokens), (const float*)a.records, own, out, a.T, a.nkv * a.G, a.nkv);
+  };
+  if (hd == 64) { if (few) go(attn_shared_join_kernel<64, PJ_WARPS>, 1); else go(attn_shared_join_kernel<64, 1>, PJ_WARPS); }
+  else { if (few) go(attn_shared_join_kernel<128, PJ_WARPS>, 1); else go(attn_shared_join_kernel<128, 1>, PJ_WARPS); }
   return launch_status("attn_shared join");
 }
 

@@ -2357,8 +2357,8 @@ def _token_arrays(T: int, tok_pos: torch.Tensor, tok_seq: torch.Tensor, block_ta
     _table(block_table, None, what)
 
 
-def _pages_scratch(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, groups: int, workspace) -> tuple:
-    need = _long_entry("exl3_attn_pages_scratch", 6)(_sms(q), q.shape[0], heads, kv_heads, head_dim, groups)
+def _pages_scratch(q: torch.Tensor, rows: int, heads: int, kv_heads: int, head_dim: int, groups: int, max_new: int, workspace) -> tuple:
+    need = _long_entry("exl3_attn_pages_scratch", 8)(_sms(q), q.shape[0], rows, heads, kv_heads, head_dim, groups, max_new)
     return need, workspace.floats(need) if workspace is not None else torch.zeros(need, dtype=torch.float32, device=q.device)
 
 
@@ -2387,7 +2387,7 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
     T = q.shape[0]
     if T == 0 or rows == 0:
         return out
-    need, scratch = _pages_scratch(q, heads, kv_heads, head_dim, n_groups, workspace)
+    need, scratch = _pages_scratch(q, rows, heads, kv_heads, head_dim, n_groups, max_new, workspace)
     rc = _entry("exl3_attn_shared", "plppplpiippiipiiiiifpl")(
         _addr(q), _pitch(q), _addr(out), _addr(k_pool), _addr(v_pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], _addr(row_start),
         _addr(row_pos0), rows, T, _addr(groups), n_groups, max_new, heads, kv_heads, head_dim, scale, _addr(scratch), need, _raw_stream())
@@ -2496,7 +2496,7 @@ def attn_pages(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, bloc
     _same_device("attn_pages", q, k_pool, v_pool, block_table, tok_pos, tok_seq, pages, out)
     if T == 0:
         return out
-    need, scratch = _pages_scratch(q, heads, kv_heads, head_dim, 0, workspace)
+    need, scratch = _pages_scratch(q, T, heads, kv_heads, head_dim, 0, 0, workspace)
     rc = _entry("exl3_attn_pages", "plppplpiiippipiiiifpl")(
         _addr(q), _pitch(q), _addr(out), _addr(k_pool), _addr(v_pool), n_pages, _addr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0],
         _addr(tok_pos), _addr(tok_seq), T, _addr(pages), pages.shape[2], heads, kv_heads, head_dim, scale, _addr(scratch), need, _raw_stream())

@@ -92,6 +92,36 @@ def test_long_prefix_and_many_blocks():
     assert P.off(run_shared(case, ws=workspace()), want, size) <= 1.0
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (8, 2, 128), (6, 6, 128), (16, 1, 64), (5, 1, 128)])
+@pytest.mark.parametrize("rows,groups", [
+    ([(0, 200)], []),                                       # a prompt
+    ([(3, 130), (700, 65), (10, 1), (0, 300)], []),         # prompts beside a token, behind contexts
+    ([(200, 150), (192, 70), (193, 2), (50, 129)], [(3, 3)]),                # behind shared pages, beside drafts
+    ([(64, 17), (64, 16), (64, 33), (64, 1)], [(4, 1)]),
+    ([(128, 400), (128, 3)], [(1, 2)]),
+])
+def test_rows_of_many_tokens(heads, kv_heads, d, rows, groups):
+    case = Paged(rows, heads, kv_heads, d, share=share(groups, len(rows) - sum(n for n, _ in groups)), seed=d + len(rows))
+    want, size = P.shared(case, d ** -0.5)
+    assert P.off(run_shared(case, ws=workspace()), want, size) <= 1.0
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (8, 2, 128)])
+def test_values_of_later_tokens_of_a_prompt(heads, kv_heads, d):
+    """A prompt's tokens 70 and 100 have values that are not finite: those before them stay as they are, the others' features are not finite."""
+    case = Paged([(40, 140), (20, 100)], heads, kv_heads, d, seed=26)
+    want, size = P.shared(case, d ** -0.5)
+    for at, feature, value in ((110, 3, math.nan), (140, 7, math.inf)):
+        case.v[int(case.table[0, at // PAGE]), :, at % PAGE, feature] = value
+    got = run_shared(case, ws=workspace()).cpu().view(-1, heads, d)
+    w, s = want.view(-1, heads, d), size.view(-1, heads, d)
+    for t in range(240):
+        bad = {f for at, f in ((110, 3), (140, 7)) if t < 140 and 40 + t >= at}
+        rest = [i for i in range(d) if i not in bad]
+        assert P.off(got[t][:, rest], w[t][:, rest], s[t][:, rest]) <= 1.0, t
+        assert all(not bool(torch.isfinite(got[t][:, f]).any()) for f in bad), t
+
+
 # ---- bounds and the choice ----------------------------------------------------------------------------------------------------------
 
 def make_bounds(case):
