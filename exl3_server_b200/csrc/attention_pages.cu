@@ -586,6 +586,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   if (threadIdx.x == 0) {
     int n = 0;
     sm.edge[0] = sm.edge[1] = -1;
+#pragma unroll 1
     for (int k = 0; k < 2 * PG_WARPS; ++k) {
       const int64_t at = sm.part_at[k >> 1][k & 1];
       if (at < 0) continue;
@@ -616,15 +617,19 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(a.out + th * HD + lane * V + i) = pg_pack(y[i] * inv, y[i + 1] * inv);
     }
   };
+#pragma unroll 1
   for (int k = 0; k < sm.n_runs; ++k) {
     const PgRun& r = sm.run[k];
     const int n_cols = cols_of(r.p);
     float* const rec = record(blockIdx.x, r.p.base);
+#pragma unroll 1
     for (int c = warp; c < n_cols; c += PG_WARPS) {
       float mm = PG_NEG, ll = 0.0f, y[V] = {};
+#pragma unroll 1
       for (int i = r.k0; i < r.k1; ++i)
         if (sm.part_at[i >> 1][i & 1] >= 0) mm = fmaxf(mm, parts(i).m[c]);         // (a warp without a part there may be between)
       const float safe = mm == PG_NEG ? 0.0f : mm;
+#pragma unroll 1
       for (int i = r.k0; i < r.k1; ++i) {
         if (sm.part_at[i >> 1][i & 1] < 0) continue;
         const float f = pg_exp2(parts(i).m[c] - safe);
@@ -661,6 +666,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       sm.last[threadIdx.x] = last;
     }
     __syncthreads();
+#pragma unroll 1
     for (int e = 0; e < 2; ++e) {
       if (!sm.last[e]) continue;
       const PgRun& r = sm.run[sm.edge[e]];
@@ -668,46 +674,35 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       // the records of blocks ba .. ba + n - 1: all but the first are their blocks' first
       const float* const rec0 = record(ba, r.p.base);
       auto rec = [&](int i) { return i == 0 ? rec0 : records + 2 * (int64_t)(ba + i) * REC; };
-      for (int c0 = warp; c0 < n_cols; c0 += 2 * PG_WARPS) {         // two queries at a time
-        float mm[2] = {PG_NEG, PG_NEG}, ll[2] = {0.0f, 0.0f}, y[2][V] = {};
-        for (int i0 = 0; i0 < n; i0 += 8) {
-          float m1[2][8], l1[2][8], y1[2][8][V];
+      // (this code runs once: short, since its way into the SM costs more than its loads)
+#pragma unroll 1
+      for (int c = warp; c < n_cols; c += PG_WARPS) {
+        float mm = PG_NEG, ll = 0.0f, y[V] = {};
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += 4) {
+          float m1[4], l1[4], y1[4][V];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int c = c0 + h * PG_WARPS;
-              const bool in = i0 + i < n && c < n_cols;
-              const float* q = rec(in ? i0 + i : 0) + (in ? c : 0);
-              m1[h][i] = in ? __ldcg(q) : PG_NEG;
-              l1[h][i] = in ? __ldcg(q + COLS) : 0.0f;
-              if (in) pg_load(rec(i0 + i) + 2 * COLS + c * HD + lane * V, y1[h][i]);
-              else
-#pragma unroll
-                for (int v = 0; v < V; ++v) y1[h][i][v] = 0.0f;
-            }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float top = mm[h];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, m1[h][i]);
-            const float safe = top == PG_NEG ? 0.0f : top, f0 = pg_exp2(mm[h] - safe);
-            ll[h] *= f0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) y[h][v] *= f0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float f = pg_exp2(m1[h][i] - safe);
-              ll[h] = fmaf(l1[h][i], f, ll[h]);
-#pragma unroll
-              for (int v = 0; v < V; ++v) y[h][v] = fmaf(y1[h][i][v], f, y[h][v]);
-            }
-            mm[h] = top;
+          for (int i = 0; i < 4; ++i) {
+            const bool in = i0 + i < n;
+            const float* q = rec(in ? i0 + i : 0);
+            m1[i] = in ? __ldcg(q + c) : PG_NEG;
+            l1[i] = __ldcg(q + COLS + c);
+            pg_load(q + 2 * COLS + c * HD + lane * V, y1[i]);
           }
-        }
+          const float top = fmaxf(fmaxf(fmaxf(m1[0], m1[1]), fmaxf(m1[2], m1[3])), mm), safe = top == PG_NEG ? 0.0f : top, f0 = pg_exp2(mm - safe);
+          ll *= f0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (c0 + h * PG_WARPS < n_cols) write(r, c0 + h * PG_WARPS, mm[h], ll[h], y[h]);
+          for (int v = 0; v < V; ++v) y[v] *= f0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float f = i0 + i < n ? pg_exp2(m1[i] - safe) : 0.0f;
+            ll += i0 + i < n ? l1[i] * f : 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) y[v] += i0 + i < n ? y1[i][v] * f : 0.0f;
+          }
+          mm = top;
+        }
+        write(r, c, mm, ll, y);
       }
     }
   }

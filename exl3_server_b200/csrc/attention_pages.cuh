@@ -46,18 +46,19 @@ __device__ inline void pg_groups(PgGroups& g, const int* __restrict__ list, int 
 
 // ---- the tensor cores' work -----------------------------------------------------------------------------------------------------
 // Tiles of up to PS_TILE queries (token, query head of a key/value head): of a group's tokens over the pages that its rows share, and of a row of many new
-// tokens over its own pages.  The work is the list of (kv head, tile, page) in this order, cut into equal shares for the blocks: a share ends in the middle of a
-// tile's pages, and the parts are joined by another kernel.
+// tokens over its own pages.  The work is the list of (kv head, tile, PS_SETUP places and the tile's pages) in this order, cut into equal shares for the blocks: a
+// share ends in the middle of a tile's pages, and the parts are joined by another kernel.
 constexpr int PS_TILE = 256;
-constexpr int PS_MAX_TILES = 768;              // of a key/value head
+constexpr int PS_MAX_TILES = 512;              // of a key/value head
 constexpr int PS_MAX_ROWS = 1024;              // rows up to which rows of many tokens have tiles of their own
 constexpr int PS_MANY = 64;                    // queries of a row and key/value head from which its own pages are the tensor cores' work
-constexpr int PS_MIN_PAGES = 4;                // pages of a share, at least: every part more is joined again
+constexpr int PS_MIN_PAGES = 4;                // places of a share, at least: every part more is joined again
+constexpr int PS_SETUP = 3;                    // places of the list that a tile has beside its pages': what its queries' way in and its sums' way out cost, in pages
 
 struct PsPlan {                                // the head of the list, in scratch memory for the join
   int n_tiles;
   int blocks;                                  // shares
-  int64_t total, per, rem;                     // pages of all; a share has `per` of them, the first `rem` shares one more
+  int64_t total, per, rem;                     // places of the list; a share has `per` of them, the first `rem` shares one more
   __device__ int64_t begin(int block) const { return per * block + min((int64_t)block, rem); }
   // the share that holds place x
   __device__ int block_of(int64_t x) const { return x < rem * (per + 1) ? (int)(x / (per + 1)) : (int)(rem + (x - rem * (per + 1)) / per); }
@@ -93,7 +94,7 @@ struct PsArgs {
   float* records;
   PsPlan* plan;
   PsToken* tokens;
-  int* tiles;                                  // for the join: per tile its place among all pages of a head, its pages and its queries [tiles][4]
+  int* tiles;                                  // for the join: per tile its place in a head's list, its pages, its queries, and the head's places [tiles][4]
 };
 cudaError_t attn_shared_prepare();             // once for a device
 int attn_shared_launch(const PsArgs& a, const void* k_pool, const void* v_pool, int hd, int sms, cudaStream_t stream);

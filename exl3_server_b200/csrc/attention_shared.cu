@@ -37,21 +37,23 @@ constexpr int PS_MAX_STAGES = 11;
 // The list of tiles, in shared memory.
 struct PsTiles {
   PsPlan plan;
-  int cum[PS_MAX_TILES + 1];                   // pages of the tiles before
+  int cum[PS_MAX_TILES + 1];                   // places of the tiles before
+  int start[PS_MAX_ROWS + 1], pos[PS_MAX_ROWS];          // the rows' first tokens and their positions, where there are no more rows than that
   int tok0[PS_MAX_TILES], query0[PS_MAX_TILES], queries[PS_MAX_TILES], row[PS_MAX_TILES], page0[PS_MAX_TILES];
   PgGroups groups;
   int group_tile[PG_MAX_GROUPS], group_tok[PG_MAX_GROUPS], group_seen[PG_MAX_GROUPS];  // first tile, first token, the first token's position of the row that has the lowest
   int row_tile[PS_MAX_ROWS];                   // a row's own first tile, -1: none
   int warp_sum[PS_THREADS / 32];
   int small;                                   // no tile has more than 128 queries
-  int odd_key[2][2][128];                      // per set, in turns, and feature: the first key whose value is not finite among those that not all of the tile's queries see
-  int odd[2][2];
+  int odd_key[2][3][128];                      // per set, in turns (a warp may be two parts behind another), and feature: the first key whose value is not finite among those that not all of the tile's queries see
+  int odd[2][3];
 };
 struct PsBars {
   uint64_t q_full[2], q_free, kv_full[PS_MAX_STAGES], kv_free[PS_MAX_STAGES], s_full[4], p_full[4], pv_done[4];
   uint32_t tmem_slot;
 };
 __host__ __device__ constexpr uint32_t ps_smem(int hd) { return ps_ring(hd) + (uint32_t)sizeof(PsTiles) + (uint32_t)sizeof(PsBars) + 1024; }
+static_assert(ps_smem(128) <= 232448, "what a block may have");
 
 // S: M = 128, N = 64, both operands K-major; P V: N = the head's features, V as it lies (keys down, features across).
 constexpr uint32_t PS_IDESC_S = idesc_bf16(128, 64);
@@ -162,10 +164,18 @@ template <int HD> __device__ inline void ps_rescale(uint32_t taddr, float f) {
 
 // The list of tiles; by all threads of a block, ends with a barrier.  The same in every block.
 __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
+  const bool held = a.rows <= PS_MAX_ROWS;     // the rows' arrays are here
+  const int most = a.bt_width * PG_PAGE;       // (a row beyond the table sees all of it)
+  auto start_of = [&](int r) { return held ? t.start[r] : min(max(__ldcg(a.row_start + r), 0), a.T); };
+  auto pos_of = [&](int r) { return held ? t.pos[r] : min(__ldcg(a.row_pos0 + r), most); };
+  if (held)
+    for (int r = threadIdx.x; r <= a.rows; r += PS_THREADS) {
+      t.start[r] = min(max(__ldcg(a.row_start + r), 0), a.T);
+      if (r < a.rows) t.pos[r] = min(__ldcg(a.row_pos0 + r), most);
+    }
   pg_groups(t.groups, a.groups, a.n_groups, a.rows, a.bt_width);
   for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS) {
-    const int r0 = t.groups.first[j], r1 = r0 + t.groups.rows[j];
-    const int s0 = min(max(__ldcg(a.row_start + r0), 0), a.T), s1 = min(max(__ldcg(a.row_start + r1), s0), a.T);
+    const int r0 = t.groups.first[j], s0 = start_of(r0), s1 = max(start_of(r0 + t.groups.rows[j]), s0);
     t.group_tok[j] = s0;
     t.group_tile[j] = t.groups.pages[j] > 0 ? (s1 - s0) * a.G : 0;     // (queries, for now)
     t.group_seen[j] = INT32_MAX;
@@ -174,8 +184,8 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   const int n_rows = a.many ? a.rows : 0;
   __syncthreads();
   for (int r = threadIdx.x; r < a.rows; r += PS_THREADS) {
-    const int s0 = min(max(__ldcg(a.row_start + r), 0), a.T), s1 = min(__ldcg(a.row_start + r + 1), a.T), j = t.groups.of(r);
-    if (j >= 0 && s1 > s0) atomicMin(&t.group_seen[j], __ldcg(a.row_pos0 + r));
+    const int s0 = start_of(r), s1 = start_of(r + 1), j = t.groups.of(r);
+    if (j >= 0 && s1 > s0) atomicMin(&t.group_seen[j], pos_of(r));
     if (r < n_rows) t.row_tile[r] = s1 > s0 && (int64_t)(s1 - s0) * a.G > PS_MANY ? (s1 - s0) * a.G : 0;
   }
   __syncthreads();
@@ -196,8 +206,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
     if (i < a.n_groups + n_rows) {
       const int row = group ? t.groups.first[i] : i - a.n_groups;
       const int own = group ? -1 : t.groups.of(row), page0 = own >= 0 ? t.groups.pages[own] : 0;
-      const int tok0 = group ? t.group_tok[i] : queries ? min(max(__ldcg(a.row_start + row), 0), a.T) : 0;
-      const int pos0 = group || !queries ? 0 : min(__ldcg(a.row_pos0 + row), a.bt_width * PG_PAGE);
+      const int tok0 = group ? t.group_tok[i] : start_of(row), pos0 = group ? 0 : pos_of(row);
       for (int k = 0; k < mine && at + k < PS_MAX_TILES; ++k) {
         const int q0 = k * PS_TILE, n = min(PS_TILE, queries - q0), last = pos0 + (q0 + n - 1) / a.G;
         t.tok0[at + k] = tok0;
@@ -206,7 +215,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
         t.row[at + k] = group ? row : -1 - row;          // (below 0: the row's own pages, which its queries do not see alike)
         t.page0[at + k] = page0;
         // (one page at least: a query that sees nothing of its own has a part all the same)
-        t.cum[at + k + 1] = group ? t.groups.pages[i] : max(1, min(a.bt_width, (max(last, 0) + PG_PAGE) / PG_PAGE) - page0);
+        t.cum[at + k + 1] = PS_SETUP + (group ? t.groups.pages[i] : max(1, min(a.bt_width, (max(last, 0) + PG_PAGE) / PG_PAGE) - page0));
       }
       if (group) t.group_tile[i] = mine ? at : -1;
       else t.row_tile[row] = mine ? at : -1;
@@ -238,7 +247,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   __syncthreads();
 }
 // A part of the list that one block works on.
-struct PsPart { int g, tile, p0, p1; };        // kv head, tile, pages of the tile
+struct PsPart { int g, tile, p0, p1, places; };          // kv head, tile, pages of the tile (none where a share has the tile's first places only), places of the list
 __device__ inline PsPart ps_part(const PsTiles& t, int64_t x, int64_t end) {
   const int all = t.cum[t.plan.n_tiles];
   PsPart p;
@@ -247,8 +256,10 @@ __device__ inline PsPart ps_part(const PsTiles& t, int64_t x, int64_t end) {
   int lo = 0, hi = t.plan.n_tiles - 1;
   while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (t.cum[mid] <= r) lo = mid; else hi = mid - 1; }
   p.tile = lo;
-  p.p0 = r - t.cum[lo];
-  p.p1 = (int)min((int64_t)(t.cum[lo + 1] - t.cum[lo]), p.p0 + (end - x));
+  const int at = r - t.cum[lo];
+  p.places = (int)min((int64_t)(t.cum[lo + 1] - r), end - x);
+  p.p0 = max(0, at - PS_SETUP);
+  p.p1 = max(0, at + p.places - PS_SETUP);
   return p;
 }
 
@@ -281,26 +292,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   pdl_trigger();
   ps_tiles(tiles, a);
   const PsPlan& plan = tiles.plan;
-  // for the join: the plan, the tiles, and every token's
-  if (blockIdx.x == 0) {
-    if (threadIdx.x == 0) *a.plan = plan;
-    for (int i = threadIdx.x; i < plan.n_tiles; i += PS_THREADS)
-      reinterpret_cast<int4*>(a.tiles)[i] = make_int4(tiles.cum[i], tiles.cum[i + 1] - tiles.cum[i], tiles.queries[i], tiles.cum[plan.n_tiles]);
-  }
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const int s0 = min(max(__ldcg(a.row_start + r), 0), a.T), s1 = min(__ldcg(a.row_start + r + 1), a.T), j = tiles.groups.of(r);
-    PsToken w;
-    w.shared_tile = j >= 0 ? tiles.group_tile[j] : -1;
-    w.shared_tok = j >= 0 ? tiles.group_tok[j] : 0;
-    w.own_tile = a.many ? tiles.row_tile[r] : -1;
-    w.own_tok = s0;
-    for (int i = s0 + threadIdx.x; i < s1; i += PS_THREADS) reinterpret_cast<int4*>(a.tokens)[i] = make_int4(w.shared_tile, w.shared_tok, w.own_tile, w.own_tok);
-  }
-  {                                            // (tokens of no row)
-    const int t0 = min(max(__ldcg(a.row_start), 0), a.T), t1 = min(max(__ldcg(a.row_start + a.rows), 0), a.T);
-    for (int i = blockIdx.x * PS_THREADS + threadIdx.x; i < a.T; i += gridDim.x * PS_THREADS)
-      if (i < t0 || i >= t1) reinterpret_cast<int4*>(a.tokens)[i] = make_int4(-1, 0, -1, 0);
-  }
   const uint32_t tmem = bars.tmem_slot;        // columns: scores of set s at 128 s, O at 256 + 128 s
   const int64_t lo = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x) : 0, hi = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x + 1) : 0;
   // Tiles of more than 128 queries: both sets take every page, 128 queries each.  Smaller ones: the sets take the pages in turn, with the same queries, and where there
@@ -346,7 +337,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         page = ahead;
       }
-      x += t.p1 - t.p0;
+      x += t.places;
     }
     // what was asked for must land before the block's shared memory goes away
     if (!ok && lane == 0) atomicExch(&g_ps_error, 1);
@@ -382,12 +373,27 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         if (++st == stages) { st = 0; phase ^= 1; }
       }
-      ++k[0];
-      k[1] += two || t.p1 - t.p0 > 1;          // (a set without a page asks for no queries)
-      x += t.p1 - t.p0;
+      k[0] += t.p1 > t.p0;
+      k[1] += t.p1 - t.p0 > (two ? 0 : 1);     // (a set without a page asks for no queries)
+      x += t.places;
     }
     if (!ok && lane == 0) atomicExch(&g_ps_error, 2);
   } else if (warp == 9) {
+    // ---- for the join, while the first scores are on their way: the plan, the tiles, and every token's -------------------------------
+    if (blockIdx.x == 0) {
+      if (lane == 0) *a.plan = plan;
+      for (int i = lane; i < plan.n_tiles; i += 32)
+        reinterpret_cast<int4*>(a.tiles)[i] = make_int4(tiles.cum[i] + PS_SETUP, tiles.cum[i + 1] - tiles.cum[i] - PS_SETUP, tiles.queries[i], tiles.cum[plan.n_tiles]);
+    }
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+      const int s0 = min(max(__ldcg(a.row_start + r), 0), a.T), s1 = min(__ldcg(a.row_start + r + 1), a.T), j = tiles.groups.of(r);
+      const int4 w = make_int4(j >= 0 ? tiles.group_tile[j] : -1, j >= 0 ? tiles.group_tok[j] : 0, a.many ? tiles.row_tile[r] : -1, s0);       // a PsToken
+      for (int i = s0 + lane; i < s1; i += 32) reinterpret_cast<int4*>(a.tokens)[i] = w;
+    }
+    {                                          // (tokens of no row)
+      const int t0 = min(max(__ldcg(a.row_start), 0), a.T), t1 = max(t0, min(max(__ldcg(a.row_start + a.rows), 0), a.T));
+      for (int i = blockIdx.x * 32 + lane; i < t0 + a.T - t1; i += gridDim.x * 32) reinterpret_cast<int4*>(a.tokens)[i < t0 ? i : t1 + i - t0] = make_int4(-1, 0, -1, 0);
+    }
     // ---- O += P V ----------------------------------------------------------------------------------------------------------------
     int st = 0, f[2] = {0, 0}, k[2] = {0, 0};
     uint32_t phase = 0;
@@ -423,7 +429,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               if (key0 + key <= last_limit) {
                 const int set = two ? -1 : (p - t.p0) & 1;
                 for (int s = 0; s < 2; ++s)
-                  if (set < 0 || set == s) { atomicMin(&tiles.odd_key[s][k[s] & 1][8 * c + e], key0 + key); tiles.odd[s][k[s] & 1] = 1; }
+                  if (set < 0 || set == s) { atomicMin(&tiles.odd_key[s][k[s] % 3][8 * c + e], key0 + key); tiles.odd[s][k[s] % 3] = 1; }
               }
             }
             if (any) *at = v;
@@ -452,9 +458,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         if (++st == stages) { st = 0; phase ^= 1; }
       }
-      ++k[0];
-      k[1] += two || t.p1 - t.p0 > 1;
-      x += t.p1 - t.p0;
+      k[0] += t.p1 > t.p0;
+      k[1] += t.p1 - t.p0 > (two ? 0 : 1);
+      x += t.places;
     }
     if (!ok && lane == 0) atomicExch(&g_ps_error, 3);
   } else {
@@ -462,50 +468,65 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + 128 * s, to = tmem + lanes + 256 + 128 * s;
-    int f = 0, parts = 0, mine = 0;            // the set's pages so far, all parts, the set's
-    for (int64_t x = lo; x < hi && ok; ++parts) {
-      const PsPart t = ps_part(tiles, x, hi);
-      x += t.p1 - t.p0;
-      if (one && parts > 0 && !ps_wait(&bars.q_free, (parts - 1) & 1)) { ok = false; break; }        // (every part's, whether the set has pages of it or not)
-      const bool two = both(t);
-      const int step = two ? 1 : 2, first = t.p0 + (two ? 0 : s), qr = s * 128 + r;
-      const int in_tile = two ? qr : r;
-      float* rec = a.records + (blockIdx.x + (int64_t)t.g * plan.n_tiles + t.tile) * ps_record(HD);
-      if (first >= t.p1) {                     // no page for this set
-        rec[qr] = -INFINITY;
-        rec[PS_TILE + qr] = 0.0f;
-        continue;
+    int f = 0, parts = 0, mine = 0;            // the set's pages so far, all parts with pages, the set's
+    // The set's next part from place x on, and its queries on their way into the operand's layout: beside the last sums of the part before.
+    struct Mine { PsPart t; bool two, in; int first, qr, step_tok, turn; int64_t slot; };
+    auto enter = [&](int64_t& x, Mine& m) {
+      for (;;) {
+        if (x >= hi) return false;
+        m.t = ps_part(tiles, x, hi);
+        x += m.t.places;
+        if (m.t.p1 == m.t.p0) continue;
+        if (one && parts > 0 && !ps_wait(&bars.q_free, (parts - 1) & 1)) { ok = false; return false; }     // (every part's, whether the set has pages of it or not)
+        ++parts;
+        m.two = both(m.t);
+        m.first = m.t.p0 + (m.two ? 0 : s);
+        m.qr = s * 128 + r;
+        m.slot = blockIdx.x + (int64_t)m.t.g * plan.n_tiles + m.t.tile;
+        if (m.first < m.t.p1) break;
+        float* rec = a.records + m.slot * ps_record(HD);       // no page for this set
+        rec[m.qr] = -INFINITY;
+        rec[PS_TILE + m.qr] = 0.0f;
       }
-      const bool in = in_tile < tiles.queries[t.tile];
-      const int query = tiles.query0[t.tile] + (in ? in_tile : 0), step_tok = query / a.G;
-      const int tok = tiles.tok0[t.tile] + step_tok, head = t.g * a.G + query - step_tok * a.G;
-      // Q: this thread's row, into the operand's layout (the last S that read the place before is done)
-      const int turn = mine++ & 1;
-      if (r < 32) for (int d = r; d < HD; d += 32) tiles.odd_key[s][turn][d] = INT32_MAX;
-      if (r == 0) tiles.odd[s][turn] = 0;
-      {
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.q_stride + (int64_t)head * HD);
-        uint4 w[HD / 8];
+      const int in_tile = m.two ? m.qr : r;
+      m.in = in_tile < tiles.queries[m.t.tile];
+      const int query = tiles.query0[m.t.tile] + (m.in ? in_tile : 0);
+      m.step_tok = query / a.G;
+      m.turn = mine++ % 3;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)(tiles.tok0[m.t.tile] + m.step_tok) * a.q_stride + (int64_t)(m.t.g * a.G + query - m.step_tok * a.G) * HD);
+      uint4 w[HD / 8];
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i) w[i] = in ? __ldcg(src + i) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < HD / 8; ++i) w[i] = m.in ? __ldcg(src + i) : make_uint4(0, 0, 0, 0);
+      if (r < 32) for (int d = r; d < HD; d += 32) tiles.odd_key[s][m.turn][d] = INT32_MAX;
+      if (r == 0) tiles.odd[s][m.turn] = 0;
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i)
-          *reinterpret_cast<uint4*>(sQ + s * second_q + (i >> 3) * 128 * 128 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = w[i];
-        fence_smem_to_tma();
-        ps_arrive_warp(q_full + s);
-      }
+      for (int i = 0; i < HD / 8; ++i)         // (the last S that read the place before is done)
+        *reinterpret_cast<uint4*>(sQ + s * second_q + (i >> 3) * 128 * 128 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = w[i];
+      fence_smem_to_tma();
+      ps_arrive_warp(q_full + s);
+      return true;
+    };
+    int64_t x = lo;
+    Mine now;
+    bool more = enter(x, now);
+    while (more && ok) {
+      const PsPart t = now.t;
+      const bool in = now.in;
+      const int step = now.two ? 1 : 2, first = now.first, qr = now.qr, turn = now.turn, step_tok = now.step_tok;
+      float* const rec = a.records + now.slot * ps_record(HD);
       // the last key that this query sees, and whether some page of the part is not there
-      const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile];
+      const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile], most = a.bt_width * PG_PAGE;
       int pos;
       if (row < 0) {
-        pos = min(__ldcg(a.row_pos0 - 1 - row), a.bt_width * PG_PAGE) + step_tok;
+        pos = (a.rows <= PS_MAX_ROWS ? tiles.pos[-1 - row] : min(__ldcg(a.row_pos0 - 1 - row), most)) + step_tok;
       } else {                                 // (shared pages, seen by all as a rule)
         const int j = tiles.groups.of(row);
         pos = INT32_MAX;
         if (tiles.group_seen[j] < (p_off + t.p1) * PG_PAGE - 1) {
+          const int tok = tiles.tok0[t.tile] + step_tok;
           int row_lo = row, row_hi = row + tiles.groups.rows[j] - 1;
           while (row_lo < row_hi) { const int mid = (row_lo + row_hi + 1) >> 1; if (__ldcg(a.row_start + mid) <= tok) row_lo = mid; else row_hi = mid - 1; }
-          pos = min(__ldcg(a.row_pos0 + row_lo), a.bt_width * PG_PAGE) + tok - __ldcg(a.row_start + row_lo);
+          pos = min(__ldcg(a.row_pos0 + row_lo), most) + tok - __ldcg(a.row_start + row_lo);
         }
       }
       const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
@@ -565,6 +586,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         fence_before();
         ps_arrive_warp(p_full + 2 * s + sb);
       }
+      if (!ok) break;
+      more = enter(x, now);
       if (!ok) break;
       ok = ps_wait(pv_done + 2 * s + ((f - 1) & 1), ((f - 1) >> 1) & 1);
       if (!ok) break;
