@@ -53,7 +53,7 @@ constexpr int PS_MAX_TILES = 512;              // of a key/value head
 constexpr int PS_MAX_ROWS = 1024;              // rows up to which rows of many tokens have tiles of their own
 constexpr int PS_MANY = 64;                    // queries of a row and key/value head from which its own pages are the tensor cores' work
 constexpr int PS_MIN_PAGES = 4;                // places of a share, at least: every part more is joined again
-constexpr int PS_SETUP = 3;                    // places of the list that a tile has beside its pages': what its queries' way in and its sums' way out cost, in pages
+constexpr int PS_SETUP = 4;                    // places of the list that a tile has beside its pages': what its queries' way in and its sums' way out cost, in pages
 
 struct PsPlan {                                // the head of the list, in scratch memory for the join
   int n_tiles;

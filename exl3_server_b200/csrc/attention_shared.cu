@@ -110,6 +110,8 @@ __device__ inline bool ps_wait(uint64_t* bar, uint32_t parity) {
         : "=r"(there) : "r"(addr), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, there);
 }
+// Whether one of a word's two bfloat16 is not finite.
+__device__ inline bool ps_odd(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 // One arrival for the warp, when all its lanes are here.
 __device__ inline void ps_arrive_warp(uint64_t* bar) {
   __syncwarp();
@@ -417,22 +419,18 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             const int key = w / (HD / 8), c = w % (HD / 8);
             if (key0 + key <= first_limit) continue;
             uint4* at = reinterpret_cast<uint4*>(sV + st * KVB + (c >> 3) * PS_BOX + key * 128 + (((c & 7) ^ (key & 7)) << 4));
-            uint4 v = *at;
-            uint32_t* word = reinterpret_cast<uint32_t*>(&v);
-            bool any = false;
-#pragma unroll
+            const uint4 v = *at;
+            if (!(ps_odd(v.x) || ps_odd(v.y) || ps_odd(v.z) || ps_odd(v.w))) continue;
+            __nv_bfloat16* each = reinterpret_cast<__nv_bfloat16*>(at);
+            const int set = two ? -1 : (p - t.p0) & 1;
+#pragma unroll 1
             for (int e = 0; e < 8; ++e) {
-              const uint32_t bits = e & 1 ? 0x7f800000u : 0x7f80u;
-              if ((word[e >> 1] & bits) != bits) continue;
-              word[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
-              any = true;
-              if (key0 + key <= last_limit) {
-                const int set = two ? -1 : (p - t.p0) & 1;
-                for (int s = 0; s < 2; ++s)
-                  if (set < 0 || set == s) { atomicMin(&tiles.odd_key[s][k[s] % 3][8 * c + e], key0 + key); tiles.odd[s][k[s] % 3] = 1; }
-              }
+              if (isfinite(__bfloat162float(each[e]))) continue;
+              each[e] = __float2bfloat16(0.0f);
+              if (key0 + key > last_limit) continue;
+              for (int s = 0; s < 2; ++s)
+                if (set < 0 || set == s) { atomicMin(&tiles.odd_key[s][k[s] % 3][8 * c + e], key0 + key); tiles.odd[s][k[s] % 3] = 1; }
             }
-            if (any) *at = v;
           }
           fence_smem_to_tma();
           __threadfence_block();
@@ -470,7 +468,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const uint32_t ts = tmem + lanes + 128 * s, to = tmem + lanes + 256 + 128 * s;
     int f = 0, parts = 0, mine = 0;            // the set's pages so far, all parts with pages, the set's
     // The set's next part from place x on, and its queries on their way into the operand's layout: beside the last sums of the part before.
-    struct Mine { PsPart t; bool two, in; int first, qr, step_tok, turn; int64_t slot; };
+    // pos: the last key that this query sees; sees: all of the warp's queries see keys up to here; holes: some page of the part is not there.
+    struct Mine { PsPart t; bool two, in, holes; int first, qr, pos, sees, turn; int64_t slot; };
     auto enter = [&](int64_t& x, Mine& m) {
       for (;;) {
         if (x >= hi) return false;
@@ -490,18 +489,39 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       }
       const int in_tile = m.two ? m.qr : r;
       m.in = in_tile < tiles.queries[m.t.tile];
-      const int query = tiles.query0[m.t.tile] + (m.in ? in_tile : 0);
-      m.step_tok = query / a.G;
+      const PsPart& t = m.t;
+      const int query = tiles.query0[t.tile] + (m.in ? in_tile : 0), step_tok = query / a.G, tok = tiles.tok0[t.tile] + step_tok;
       m.turn = mine++ % 3;
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)(tiles.tok0[m.t.tile] + m.step_tok) * a.q_stride + (int64_t)(m.t.g * a.G + query - m.step_tok * a.G) * HD);
-      uint4 w[HD / 8];
+      // the warp's 32 queries, rows of the operand (the last S that read the place is done): several of them an instruction, 16 bytes a lane
+      constexpr int LANES = HD / 8, EACH = 32 / LANES;
+      const int64_t from = m.in ? (int64_t)tok * a.q_stride + (int64_t)(t.g * a.G + query - step_tok * a.G) * HD : -1;
+      uint4 w[LANES];
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i) w[i] = m.in ? __ldcg(src + i) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < LANES; ++i) {
+        const int64_t at = __shfl_sync(0xffffffffu, from, EACH * i + lane / LANES);
+        w[i] = at >= 0 ? __ldcg(reinterpret_cast<const uint4*>(a.q + at) + lane % LANES) : make_uint4(0, 0, 0, 0);
+      }
+      const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile], most = a.bt_width * PG_PAGE;
+      const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
+      bool holes = false;
+      for (int p = t.p0 + lane; p < t.p1; p += 32) { const int page = p_off + p < a.bt_width ? __ldcg(bt + p) : -1; holes |= page < 0 || page >= a.n_pages; }
+      m.pos = INT32_MAX;                       // (shared pages, seen by all as a rule)
+      if (row < 0) {
+        m.pos = (a.rows <= PS_MAX_ROWS ? tiles.pos[-1 - row] : min(__ldcg(a.row_pos0 - 1 - row), most)) + step_tok;
+      } else if (tiles.group_seen[tiles.groups.of(row)] < (p_off + t.p1) * PG_PAGE - 1) {
+        int row_lo = row, row_hi = row + tiles.groups.rows[tiles.groups.of(row)] - 1;
+        while (row_lo < row_hi) { const int mid = (row_lo + row_hi + 1) >> 1; if (__ldcg(a.row_start + mid) <= tok) row_lo = mid; else row_hi = mid - 1; }
+        m.pos = min(__ldcg(a.row_pos0 + row_lo), most) + tok - __ldcg(a.row_start + row_lo);
+      }
       if (r < 32) for (int d = r; d < HD; d += 32) tiles.odd_key[s][m.turn][d] = INT32_MAX;
       if (r == 0) tiles.odd[s][m.turn] = 0;
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i)         // (the last S that read the place before is done)
-        *reinterpret_cast<uint4*>(sQ + s * second_q + (i >> 3) * 128 * 128 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = w[i];
+      for (int i = 0; i < LANES; ++i) {
+        const int c = lane % LANES, rr = (warp & 3) * 32 + EACH * i + lane / LANES;
+        *reinterpret_cast<uint4*>(sQ + s * second_q + (c >> 3) * 128 * 128 + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = w[i];
+      }
+      m.holes = __any_sync(0xffffffffu, holes);
+      m.sees = __reduce_min_sync(0xffffffffu, m.pos);
       fence_smem_to_tma();
       ps_arrive_warp(q_full + s);
       return true;
@@ -512,28 +532,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     while (more && ok) {
       const PsPart t = now.t;
       const bool in = now.in;
-      const int step = now.two ? 1 : 2, first = now.first, qr = now.qr, turn = now.turn, step_tok = now.step_tok;
+      const bool holes = now.holes;
+      const int step = now.two ? 1 : 2, first = now.first, qr = now.qr, turn = now.turn, pos = now.pos, sees = now.sees, p_off = tiles.page0[t.tile];
       float* const rec = a.records + now.slot * ps_record(HD);
-      // the last key that this query sees, and whether some page of the part is not there
-      const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile], most = a.bt_width * PG_PAGE;
-      int pos;
-      if (row < 0) {
-        pos = (a.rows <= PS_MAX_ROWS ? tiles.pos[-1 - row] : min(__ldcg(a.row_pos0 - 1 - row), most)) + step_tok;
-      } else {                                 // (shared pages, seen by all as a rule)
-        const int j = tiles.groups.of(row);
-        pos = INT32_MAX;
-        if (tiles.group_seen[j] < (p_off + t.p1) * PG_PAGE - 1) {
-          const int tok = tiles.tok0[t.tile] + step_tok;
-          int row_lo = row, row_hi = row + tiles.groups.rows[j] - 1;
-          while (row_lo < row_hi) { const int mid = (row_lo + row_hi + 1) >> 1; if (__ldcg(a.row_start + mid) <= tok) row_lo = mid; else row_hi = mid - 1; }
-          pos = min(__ldcg(a.row_pos0 + row_lo), most) + tok - __ldcg(a.row_start + row_lo);
-        }
-      }
-      const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
-      bool holes = false;
-      for (int p = t.p0 + lane; p < t.p1; p += 32) { const int page = p_off + p < a.bt_width ? __ldcg(bt + p) : -1; holes |= page < 0 || page >= a.n_pages; }
-      holes = __any_sync(0xffffffffu, holes);
-      const int sees = __reduce_min_sync(0xffffffffu, pos);              // all of the warp's queries see keys up to here
       float m_used = -INFINITY, l = 0.0f;
       uint32_t s0[32], s1[32];
       auto ask = [&](int f) {                  // the scores of the set's page f: on their way
@@ -551,7 +552,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int key0 = (p_off + p) * PG_PAGE;
         if (key0 + PG_PAGE - 1 > sees || holes) {
           int last = pos;
-          if (holes) { const int page = p_off + p < a.bt_width ? __ldcg(bt + p) : -1; if (page < 0 || page >= a.n_pages) last = -1; }
+          if (holes) {
+            const int row = tiles.row[t.tile], page = p_off + p < a.bt_width ? __ldcg(a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off + p) : -1;
+            if (page < 0 || page >= a.n_pages) last = -1;
+          }
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             if (key0 + c > last) s0[c] = 0xff800000u;
