@@ -40,7 +40,7 @@ struct PgArgs {
   const int* row_start;                        // rows
   const int* row_pos0;
   int rows, T, nh, nkv, G;
-  int row0;                                    // the first row of this launch
+  int row0, window;                            // the first row of this launch, and how many it takes
   float scale_log2;
   int* counters;
   float* records;
@@ -86,6 +86,10 @@ template <int V> __device__ inline void pg_store(float* p, const float (&y)[V]) 
   else *reinterpret_cast<float2*>(p) = make_float2(y[0], y[1]);
 }
 template <int V> __device__ inline void pg_load(const float* p, float (&y)[V]) {
+  if (V == 4) { const float4 v = *reinterpret_cast<const float4*>(p); y[0] = v.x; y[1] = v.y; y[V - 2] = v.z; y[V - 1] = v.w; }
+  else { const float2 v = *reinterpret_cast<const float2*>(p); y[0] = v.x; y[1] = v.y; }
+}
+template <int V> __device__ inline void pg_load_cg(const float* p, float (&y)[V]) {
   if (V == 4) { const float4 v = __ldcg(reinterpret_cast<const float4*>(p)); y[0] = v.x; y[1] = v.y; y[V - 2] = v.z; y[V - 1] = v.w; }
   else { const float2 v = __ldcg(reinterpret_cast<const float2*>(p)); y[0] = v.x; y[1] = v.y; }
 }
@@ -110,18 +114,19 @@ template <int HD, int COLS> struct PgPart {
   float m[COLS], l[COLS], acc[COLS][HD];
 };
 // An item, and where in it a share is.
-struct PgPlace { int i, g, b, u0, u1, units; int64_t base; };
+struct PgPlace { int i, g, b, u0, u1, units, base; };
 struct PgRun { PgPlace p; int k0, k1; bool whole, own; };
-struct PgSmem {
+template <int HD> struct PgSmem {
+  uint64_t full[PG_WARPS][PG_STAGES];
   PgRun run[2 * PG_WARPS];
   int n_runs, edge[2];
-  uint64_t full[PG_WARPS][PG_STAGES];
-  int64_t cum[PG_WINDOW + 1];                  // units of the rows before
+  int cum[PG_WINDOW + 1];                      // units of the rows before
   int start[PG_WINDOW], n_new[PG_WINDOW], pos[PG_WINDOW], units[PG_WINDOW];
-  int64_t part_at[PG_WARPS][2];                // a part's item (the place of its first unit), -1: none
-  PgPlace part_of[PG_WARPS][2];
-  int64_t warp_sum[PG_WARPS];
+  int shared[PG_WINDOW];                       // the pages that the row shares, -1: it is in no group
+  PgPlace part_of[PG_WARPS][2];                // the warps' parts' items; units 0: none
+  int warp_sum[PG_WARPS];
   int last[2];
+  int odd_key[PG_WARPS][HD];                   // per feature the first key whose value is not finite among those that not all of an item's queries see
   PgGroups groups;
 };
 
@@ -132,6 +137,8 @@ struct PgSmem {
 // item, are cut into equal shares for the warps, which stream them through rings of their own, each asking for its own copies: nothing is waited for but
 // memory.  What a warp has whole it writes out; parts of items that shares cut are joined in shared memory at the end, and those that blocks cut by the block that
 // is the last to report, always in the order of the pages, so that results do not depend on which it was.
+//
+// The memory's queue is full while the units stream, and code that is met for the first time then comes in at its end, as does anything else: what runs once is kept short.
 template <int HD, int NC, bool LIST>
 __global__ void __launch_bounds__(PG_WARPS * 32, 1)
 attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PgArgs a) {
@@ -142,23 +149,23 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   constexpr int KT = HD / 16;                  // pieces of 16 features
   constexpr int BOX = KS * 128;                // bytes of a box of 64 features
   constexpr int HALF = PG_UNIT_BYTES / 2;      // keys, then values
-  static_assert(2 * sizeof(PgPart<HD, COLS>) <= PG_RING, "a warp's parts fit into its ring");
+  constexpr int V = HD / 32;                   // features a lane, where a warp has a row of them
+  using Part = PgPart<HD, COLS>;
+  static_assert(2 * sizeof(Part) <= PG_RING, "a warp's parts fit into its ring");
   extern __shared__ unsigned char pg_raw[];
   unsigned char* rings = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pg_raw) + 1023) & ~(uintptr_t)1023);
-  PgSmem& sm = *reinterpret_cast<PgSmem*>(rings + PG_SMEM_RINGS);
+  PgSmem<HD>& sm = *reinterpret_cast<PgSmem<HD>*>(rings + PG_SMEM_RINGS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < PG_WARPS; ++w)
-      for (int s = 0; s < PG_STAGES; ++s) tc5::mbar_init(&sm.full[w][s], 1);
-    tc5::mbar_init_fence();
-  }
+  if (threadIdx.x < PG_WARPS * PG_STAGES) tc5::mbar_init(&sm.full[0][0] + threadIdx.x, 1);
+  if (threadIdx.x < 32) tc5::mbar_init_fence();
   // The kernel before is, with shared pages, the one that works on them: it let this one start when its own predecessors had ended, and this one needs nothing of it.
   // Else everything is waited for here.
   if (a.wait_first) pdl_wait();
   pdl_trigger();
 
   // ---- the rows of this launch -------------------------------------------------------------------------------------------
-  const int most_keys = a.bt_width * PG_PAGE, n_rows = min(a.rows - a.row0, PG_WINDOW);
+  const int most_keys = a.bt_width * PG_PAGE, n_rows = min(a.rows - a.row0, a.window);
+#pragma unroll 1
   for (int i = threadIdx.x; i < n_rows; i += PG_WARPS * 32) {
     const int row = a.row0 + i;
     // (a row beyond the table sees all of it)
@@ -167,120 +174,109 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     sm.start[i] = start;
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
   }
-  pg_groups(sm.groups, a.groups, LIST ? 0 : a.n_groups, a.rows, a.bt_width);
-  auto group_of = [&](int row) { return LIST ? -1 : sm.groups.of(row); };
-  auto shared_of = [&](int row) { const int j = group_of(row); return j < 0 ? 0 : sm.groups.pages[j]; };   // pages that the row shares
-  auto blocks_of = [&](int i) {                // items of a row and head
-    const int queries = sm.n_new[i] * a.G;
-    return !LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS;
-  };
-  {
-    int64_t run = 0;
-    for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
-      const int i = i0 + threadIdx.x;
-      int64_t mine = 0;
-      if (i < n_rows) {
-        const int pos = sm.pos[i];
-        int units;
-        if (LIST) units = min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP;
-        else units = (min(pos + sm.n_new[i], most_keys) + KS - 1) / KS - shared_of(a.row0 + i) * UPP;
-        sm.units[i] = max(units, 1);           // (one at least: every query gets an answer)
-        mine = (int64_t)max(units, 1) * blocks_of(i) * a.nkv;
-      }
-      int64_t incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
-      if (lane == 31) sm.warp_sum[warp] = incl;
-      __syncthreads();
-      int64_t before = run;
-      for (int w = 0; w < PG_WARPS; ++w) { if (w < warp) before += sm.warp_sum[w]; run += sm.warp_sum[w]; }
-      if (i < n_rows) sm.cum[i + 1] = before + incl;
-      __syncthreads();
+  if (LIST) __syncthreads();
+  else pg_groups(sm.groups, a.groups, a.n_groups, a.rows, a.bt_width);
+  int total = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
+    const int i = i0 + threadIdx.x;
+    int mine = 0;
+    if (i < n_rows) {
+      const int pos = sm.pos[i], queries = sm.n_new[i] * a.G, j = LIST ? -1 : sm.groups.of(a.row0 + i), shared = j < 0 ? -1 : sm.groups.pages[j];
+      const int units = LIST ? min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP : (min(pos + sm.n_new[i], most_keys) + KS - 1) / KS - max(shared, 0) * UPP;
+      sm.shared[i] = shared;
+      sm.units[i] = max(units, 1);             // (one at least: every query gets an answer)
+      mine = !LIST && a.many && queries > PS_MANY ? 0 : max(units, 1) * ((queries + COLS - 1) / COLS) * a.nkv;
     }
-    if (threadIdx.x == 0) sm.cum[0] = 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+    if (lane == 31) sm.warp_sum[warp] = incl;
+    __syncthreads();
+    int before = total;
+#pragma unroll
+    for (int w = 0; w < PG_WARPS; ++w) { if (w < warp) before += sm.warp_sum[w]; total += sm.warp_sum[w]; }
+    if (i < n_rows) sm.cum[i + 1] = before + incl;
     __syncthreads();
   }
-  const int64_t total = sm.cum[n_rows];
-  const int n_blocks = (int)min((int64_t)gridDim.x, max((int64_t)1, total / (PG_WARPS * PG_MIN_UNITS)));
+  if (threadIdx.x == 0) sm.cum[0] = 0;
+  __syncthreads();
+  const int n_blocks = min((int)gridDim.x, max(1, total / (PG_WARPS * PG_MIN_UNITS))), n_shares = n_blocks * PG_WARPS;
   if (total == 0 || (int)blockIdx.x >= n_blocks) {
     if (!a.wait_first) pdl_wait();
     return;
   }
-  const int n_shares = n_blocks * PG_WARPS;
-  const int64_t per = total / n_shares, rem = total - per * n_shares;
-  auto begin = [&](int w) { return per * w + min((int64_t)w, rem); };         // the first unit of a warp's share: they differ by one unit at most
-  const int64_t i_lo = begin(blockIdx.x * PG_WARPS + warp), i_hi = begin(blockIdx.x * PG_WARPS + warp + 1);
+  const int per = total / n_shares, rem = total - per * n_shares;
+  auto begin = [&](int w) { return per * w + min(w, rem); };           // the first unit of a warp's share: they differ by one unit at most
+  const int i_lo = begin(blockIdx.x * PG_WARPS + warp), i_hi = begin(blockIdx.x * PG_WARPS + warp + 1);
   // The item at place x.
-  auto place_of = [&](int64_t x, int64_t end) {
+  auto place_of = [&](int x) {
     int lo = 0, hi = n_rows - 1;
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (sm.cum[mid] <= x) lo = mid; else hi = mid - 1; }
     PgPlace p;
     p.i = lo;
     p.units = sm.units[lo];
-    const int64_t r = x - sm.cum[lo];
-    const int item = (int)(r / p.units), nb = blocks_of(lo);
-    p.u0 = (int)(r - (int64_t)item * p.units);
-    p.u1 = (int)min((int64_t)p.units, p.u0 + (end - x));
+    const int r = x - sm.cum[lo], item = r / p.units, nb = (sm.n_new[lo] * a.G + COLS - 1) / COLS;
+    p.u0 = r - item * p.units;
+    p.u1 = min(p.units, p.u0 + i_hi - x);
     p.g = item / nb;
-    p.b = item % nb;
+    p.b = item - p.g * nb;
     p.base = x - p.u0;
     return p;
   };
 
-  unsigned char* ring = rings + warp * PG_RING;
-  uint64_t* full = sm.full[warp];
+  unsigned char* const ring = rings + warp * PG_RING;
+  uint64_t* const full = sm.full[warp];
   // ---- copies: page numbers come 32 at a time, a batch ahead -----------------------------------------------------------------
-  int64_t ask_x = i_lo;                        // the next unit to ask for
+  int ask_x = i_lo, ask_st = 0;                // the next unit to ask for, and its stage
   PgPlace ask = {};
-  int ask_u = 0, ask_n = 0, batch_p = 0;       // its number in the item; units asked for so far; the first page of the batch at hand
+  int ask_u = 0, batch_p = 0;                  // its number in the item; the first page of the batch at hand
   int page = 0, logical = 0, page_next = 0, logical_next = 0;
   int key0s[PG_STAGES];                        // a stage's first key; below 0: its page is not there
-  auto fetch = [&](int p0, int& pg, int& lg) { // pages p0 + lane of the item
-    const int row = a.row0 + ask.i;
-    const int seq = LIST ? __ldcg(a.tok_seq + row) : row;
-    lg = p0 + lane + (LIST ? 0 : shared_of(row));
-    const bool in = (p0 + lane) * UPP < ask.units;
-    if (LIST) lg = in ? __ldcg(a.lists + ((int64_t)row * a.nkv + ask.g) * a.list_stride + p0 + lane) : -1;
-    pg = in && seq >= 0 && seq < a.bt_rows && lg >= 0 && lg < a.bt_width ? __ldcg(a.block_table + (int64_t)seq * a.bt_stride + lg) : -1;
-    if (pg >= a.n_pages) pg = -1;
-  };
   auto ask_next = [&]() {
     if (ask_x >= i_hi) return;
-    if (ask_x == i_lo || ask_u == ask.u1) {    // another item
-      ask = place_of(ask_x, i_hi);
+    int batches = 0;                           // to ask for: two for another item
+    if (ask_u == ask.u1) {
+      ask = place_of(ask_x);
       ask_u = ask.u0;
       batch_p = ask_u / UPP;
-      fetch(batch_p, page, logical);
-      fetch(batch_p + 32, page_next, logical_next);
+      batches = 2;
     } else if (ask_u / UPP - batch_p == 32) {
       batch_p += 32;
+      batches = 1;
+    }
+#pragma unroll 1
+    for (; batches > 0; --batches) {
       page = page_next;
       logical = logical_next;
-      fetch(batch_p + 32, page_next, logical_next);
+      const int p = batch_p + (batches == 2 ? 0 : 32) + lane, row = a.row0 + ask.i, seq = LIST ? __ldcg(a.tok_seq + row) : row;
+      const bool in = p * UPP < ask.units && seq >= 0 && seq < a.bt_rows;
+      logical_next = LIST ? in ? __ldcg(a.lists + ((int64_t)row * a.nkv + ask.g) * a.list_stride + p) : -1 : p + max(sm.shared[ask.i], 0);
+      page_next = in && logical_next >= 0 && logical_next < a.bt_width ? __ldcg(a.block_table + (int64_t)seq * a.bt_stride + logical_next) : -1;
+      if (page_next >= a.n_pages) page_next = -1;
     }
-    const int src = ask_u / UPP - batch_p;
-    const int pg = __shfl_sync(0xffffffffu, page, src), lg = __shfl_sync(0xffffffffu, logical, src);
-    const int st = ask_n % PG_STAGES;
+    const int src = ask_u / UPP - batch_p, pg = __shfl_sync(0xffffffffu, page, src), lg = __shfl_sync(0xffffffffu, logical, src);
     const int key0 = pg < 0 ? -1 : lg * PG_PAGE + (ask_u % UPP) * KS;
 #pragma unroll
     for (int s = 0; s < PG_STAGES; ++s)
-      if (s == st) key0s[s] = key0;
+      if (s == ask_st) key0s[s] = key0;
     if (lane == 0 && pg >= 0) {
-      tc5::mbar_expect_tx(full + st, PG_UNIT_BYTES);
+      tc5::mbar_expect_tx(full + ask_st, PG_UNIT_BYTES);
       const int y = (pg * a.nkv + ask.g) * PG_PAGE + (ask_u % UPP) * KS;
-      unsigned char* dst = ring + st * PG_UNIT_BYTES;
+      unsigned char* dst = ring + ask_st * PG_UNIT_BYTES;
 #pragma unroll
       for (int x = 0; x < HD / 64; ++x) {
-        tc5::tma_load_2d(dst + x * BOX, &map_k, full + st, 64 * x, y);
-        tc5::tma_load_2d(dst + HALF + x * BOX, &map_v, full + st, 64 * x, y);
+        tc5::tma_load_2d(dst + x * BOX, &map_k, full + ask_st, 64 * x, y);
+        tc5::tma_load_2d(dst + HALF + x * BOX, &map_v, full + ask_st, 64 * x, y);
       }
     } else if (lane == 0) {
-      tc5::mbar_arrive(full + st);
+      tc5::mbar_arrive(full + ask_st);
     }
+    if (++ask_st == PG_STAGES) ask_st = 0;
     ++ask_u;
-    ++ask_n;
     ++ask_x;
   };
+#pragma unroll 1
   for (int s = 0; s < PG_STAGES; ++s) ask_next();
 
   // ---- computing ------------------------------------------------------------------------------------------------------------
@@ -296,30 +292,100 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   bool ok = true;
   int st = 0;                                  // the next unit's stage, and its phase
   uint32_t phase = 0;
-  if (lane == 0) sm.part_at[warp][0] = sm.part_at[warp][1] = -1;
-  float m_first[NC][2], l_first[NC][2];        // the first part's, until the ring is free
+  if (lane < 2) sm.part_of[warp][lane].units = 0;
   float m[NC][2], l[NC][2], o[KT][NC][4];
-  bool have_first = false;
+  float m_first[NC][2], l_first[NC][2];        // the first part's, until the ring is free
+  bool have_first = false, odd = false;
   float* const spill = a.records + ((int64_t)blockIdx.x * PG_WARPS + warp) * (PG_MAX_COLS * HD);   // (where the first part's sums wait meanwhile)
-  // the item's query of column 8 nc + gl as the operand: features 16 k + 2 tl, + 1 and + 8, + 9
-  uint32_t qf[NC][KT][2];
-  auto load_q = [&](const PgPlace& p) {
+  uint32_t qf[NC][KT][2];                      // the query of column 8 nc + gl as the operand: features 16 k + 2 tl, + 1 and + 8, + 9
+  PgPlace p = {};
+  int x = i_lo;
+  for (bool begun = false;; begun = true) {
+    // the next item's queries on their way, then the sums of the one that is done
+    const PgPlace done = p;
+    const bool more = x < i_hi;
+    if (more) {
+      p = place_of(x);
 #pragma unroll
-    for (int nc = 0; nc < NC; ++nc) {
-      const int c = min(p.b * COLS + 8 * nc + gl, sm.n_new[p.i] * a.G - 1), tok = c / a.G;
-      const __nv_bfloat16* src = a.q + (int64_t)(sm.start[p.i] + tok) * a.q_stride + (int64_t)(p.g * a.G + c - tok * a.G) * HD + 2 * tl;
+      for (int nc = 0; nc < NC; ++nc) {
+        const int c = min(p.b * COLS + 8 * nc + gl, sm.n_new[p.i] * a.G - 1), tok = c / a.G;
+        const __nv_bfloat16* src = a.q + (int64_t)(sm.start[p.i] + tok) * a.q_stride + (int64_t)(p.g * a.G + c - tok * a.G) * HD + 2 * tl;
 #pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        qf[nc][k][0] = __ldcg(reinterpret_cast<const unsigned int*>(src + 16 * k));
-        qf[nc][k][1] = __ldcg(reinterpret_cast<const unsigned int*>(src + 16 * k + 8));
+        for (int k = 0; k < KT; ++k) {
+          qf[nc][k][0] = __ldcg(reinterpret_cast<const unsigned int*>(src + 16 * k));
+          qf[nc][k][1] = __ldcg(reinterpret_cast<const unsigned int*>(src + 16 * k + 8));
+        }
       }
     }
-  };
-  PgPlace p = {};
-  if (i_lo < i_hi) { p = place_of(i_lo, i_hi); load_q(p); }
-  for (int64_t x = i_lo; x < i_hi;) {
-    const int start = sm.start[p.i], n_new = sm.n_new[p.i], pos0 = sm.pos[p.i], col0 = p.b * COLS;
-    const int n_cols = min(COLS, n_new * a.G - col0);
+    if (begun) {
+      const int col0 = done.b * COLS, n_cols = min(COLS, sm.n_new[done.i] * a.G - col0);
+      auto query_of = [&](int c) {             // (token, head)
+        const int tok = (col0 + c) / a.G;
+        return (int64_t)(sm.start[done.i] + tok) * a.nh + done.g * a.G + (col0 + c) - tok * a.G;
+      };
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[nc][e] += __shfl_xor_sync(0xffffffffu, l[nc][e], d);
+        }
+      if (odd) {                               // features whose values are not finite are not, for those who see them
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (sm.odd_key[warp][16 * i + 8 * (e >> 1) + gl] <= sm.pos[done.i] + min(col0 + 8 * nc + 2 * tl + (e & 1), col0 + n_cols - 1) / a.G) o[i][nc][e] = __int_as_float(0x7fc00000);
+      }
+      const bool whole = done.u0 == 0 && done.u1 == done.units;
+      if (whole && sm.shared[done.i] < 0) {
+        // ---- a whole item: out with it ----------------------------------------------------------------------------------------
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+          const int c = 8 * nc + gl;           // (after the transposition)
+          const float i0 = l[nc][0] == 0.0f ? 0.0f : 1.0f / l[nc][0], i1 = l[nc][1] == 0.0f ? 0.0f : 1.0f / l[nc][1];
+          __nv_bfloat16* dst = a.out + query_of(min(c, n_cols - 1)) * HD + 2 * tl;
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              const uint32_t w = pg_transpose(pg_pack(o[i][nc][2 * f] * i0, o[i][nc][2 * f + 1] * i1));
+              if (c < n_cols) *reinterpret_cast<uint32_t*>(dst + 16 * i + 8 * f) = w;
+            }
+        }
+      } else {
+        // ---- rows of hd floats: the own pages' part of a row that shares pages; or a part of an item, the first one (of an item that began in the share before) where
+        // it can wait until the ring is free, the last one in the ring --------------------------------------------------------------------------
+        const bool first = !whole && more;
+        Part& part = reinterpret_cast<Part*>(ring)[1];
+        __syncwarp();
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = 8 * nc + 2 * tl + e;
+            float* const dst = whole ? a.own + query_of(min(c, n_cols - 1)) * HD : first ? spill + c * HD : part.acc[c];
+            if (!whole || c < n_cols) {
+#pragma unroll
+              for (int i = 0; i < KT; ++i) { dst[16 * i + gl] = o[i][nc][e]; dst[16 * i + 8 + gl] = o[i][nc][2 + e]; }
+              if (gl == 0) {
+                if (whole) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * query_of(c)) = make_float2(m[nc][e], l[nc][e]);
+                else if (!first) { part.m[c] = m[nc][e]; part.l[c] = l[nc][e]; }
+              }
+            }
+            if (first) { m_first[nc][e] = m[nc][e]; l_first[nc][e] = l[nc][e]; }
+          }
+        have_first |= first;
+        if (!whole && lane == 0) sm.part_of[warp][first ? 0 : 1] = done;
+        __syncwarp();
+      }
+    }
+    if (!more) break;
+    // ---- the item's units ---------------------------------------------------------------------------------------------------------------
+    const int n_new = sm.n_new[p.i], pos0 = sm.pos[p.i], col0 = p.b * COLS;
     int limit[NC][2];                          // the last keys that this thread's two queries of each 8 see: columns 2 tl, 2 tl + 1
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
@@ -329,11 +395,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         m[nc][e] = PG_NEG;
         l[nc][e] = 0.0f;
       }
-    const int first_limit = pos0 + col0 / a.G, last_limit = pos0 + (col0 + n_cols - 1) / a.G;
+    const int first_limit = pos0 + col0 / a.G, last_limit = pos0 + min(col0 + COLS - 1, n_new * a.G - 1) / a.G;
 #pragma unroll
     for (int i = 0; i < KT; ++i)
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) o[i][nc][0] = o[i][nc][1] = o[i][nc][2] = o[i][nc][3] = 0.0f;
+    odd = false;
+#pragma unroll 1
     for (int u = p.u0; u < p.u1; ++u) {
       if (ok) ok = pg_wait(full + st, phase);
       int key0 = key0s[0];
@@ -342,20 +410,35 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         if (i == st) key0 = key0s[i];
       if (ok && key0 >= 0 && key0 <= last_limit) {
         const uint32_t unit = ring_addr + st * PG_UNIT_BYTES;
-        const unsigned char* vals = ring + st * PG_UNIT_BYTES + HALF;
-        // Values that a query does not see may be anything, and its probability of 0 would be multiplied with them.  Those that no query
-        // of the item sees are taken as zeros; where one that some see is not finite, all that not everyone sees are added query by query.
         const bool edge = key0 + KS - 1 > first_limit;
-        int cut = last_limit;                  // the last key whose values the products take
-        if (edge && first_limit < last_limit) {
-          bool odd = false;
-          for (int w = lane; w < KS * (HD / 8); w += 32) {
+        if (edge) {
+          // Values that not all queries see may be anything, and a probability of 0 is multiplied with them all the same: those that are not finite become zeros, and where
+          // some queries see them it is noted from which key on the feature is not finite.
+          unsigned char* vals = ring + st * PG_UNIT_BYTES + HALF;
+          bool any = false;
+#pragma unroll 4
+          for (int w = max(first_limit + 1 - key0, 0) * (HD / 8) + lane; w < KS * (HD / 8); w += 32) {
             const int key = w / (HD / 8), c = w % (HD / 8);
-            if (key0 + key <= first_limit || key0 + key > last_limit) continue;
             const uint4 v = *reinterpret_cast<const uint4*>(vals + (c / 8) * BOX + key * 128 + (((c & 7) ^ (key & 7)) << 4));
-            odd |= pg_odd(v.x) || pg_odd(v.y) || pg_odd(v.z) || pg_odd(v.w);
+            any |= pg_odd(v.x) || pg_odd(v.y) || pg_odd(v.z) || pg_odd(v.w);
           }
-          if (__any_sync(0xffffffffu, odd)) cut = first_limit;
+          if (__any_sync(0xffffffffu, any)) {
+            if (!odd)
+#pragma unroll 1
+              for (int d = lane; d < HD; d += 32) sm.odd_key[warp][d] = INT32_MAX;
+            odd = true;
+            __syncwarp();
+#pragma unroll 1
+            for (int w = max(first_limit + 1 - key0, 0) * HD + lane; w < KS * HD; w += 32) {
+              const int key = w / HD, d = w % HD;
+              __nv_bfloat16* v = reinterpret_cast<__nv_bfloat16*>(vals + (d / 64) * BOX + key * 128 + ((((d / 8) & 7) ^ (key & 7)) << 4)) + d % 8;
+              if (isfinite(__bfloat162float(*v))) continue;
+              *v = __float2bfloat16(0.0f);
+              if (key0 + key <= last_limit) atomicMin(&sm.odd_key[warp][d], key0 + key);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
         }
         float s[MT][NC][4];
 #pragma unroll
@@ -414,7 +497,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
         }
         // probabilities: packed by pairs of queries, turned into pairs of keys for the second product
-        uint32_t pr[MT][NC][2], pk[MT][NC][2];
+        uint32_t pk[MT][NC][2];
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
           const float r0 = m[nc][0] == PG_NEG ? 0.0f : m[nc][0], r1 = m[nc][1] == PG_NEG ? 0.0f : m[nc][1];
@@ -425,144 +508,35 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               const float p0 = pg_exp2(s[t][nc][2 * h] - r0), p1 = pg_exp2(s[t][nc][2 * h + 1] - r1);
               l[nc][0] += p0;
               l[nc][1] += p1;
-              pr[t][nc][h] = pg_pack(p0, p1);
-              pk[t][nc][h] = pg_transpose(pr[t][nc][h]);
+              pk[t][nc][h] = pg_transpose(pg_pack(p0, p1));
             }
         }
-        auto values = [&](auto cutting) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;         // of this lane's keys 16 t + 2 tl, + 1 and + 8, + 9
-            if (decltype(cutting)::value) {
-              const int key = key0 + 16 * t + 2 * tl;
-              keep0 = key + 1 <= cut ? 0xffffffffu : key <= cut ? 0xffffu : 0u;
-              keep1 = key + 9 <= cut ? 0xffffffffu : key + 8 <= cut ? 0xffffu : 0u;
-            }
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int i = 0; i < KT; ++i) {
-              uint32_t vf[4];
-              pg_ldsm_t(vf, unit + (i >> 2) * BOX + 16 * t * 128 + v_row + v_col[i & 3]);
-              if (decltype(cutting)::value) { vf[0] &= keep0; vf[1] &= keep0; vf[2] &= keep1; vf[3] &= keep1; }
+          for (int i = 0; i < KT; ++i) {
+            uint32_t vf[4];
+            pg_ldsm_t(vf, unit + (i >> 2) * BOX + 16 * t * 128 + v_row + v_col[i & 3]);
 #pragma unroll
-              for (int nc = 0; nc < NC; ++nc) pg_mma(o[i][nc], vf, pk[t][nc][0], pk[t][nc][1]);
-            }
+            for (int nc = 0; nc < NC; ++nc) pg_mma(o[i][nc], vf, pk[t][nc][0], pk[t][nc][1]);
           }
-        };
-        if (edge) values(std::true_type()); else values(std::false_type());
-        if (cut < last_limit) {
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-              for (int e = 0; e < 8; ++e) {
-                const int key = 16 * t + 8 * h + e;
-                uint32_t w[NC];
-#pragma unroll
-                for (int nc = 0; nc < NC; ++nc) w[nc] = __shfl_sync(0xffffffffu, pr[t][nc][h], 4 * e + tl);
-                if (key0 + key <= cut || key0 + key > last_limit) continue;
-                const unsigned char* line = vals + key * 128;
-#pragma unroll
-                for (int i = 0; i < KT; ++i)
-#pragma unroll
-                  for (int f = 0; f < 2; ++f) {          // feature 16 i + 8 f + gl
-                    const int c = 2 * i + f;
-                    const float v = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(line + (c >> 3) * BOX + (((c & 7) ^ (key & 7)) << 4) + 2 * gl));
-#pragma unroll
-                    for (int nc = 0; nc < NC; ++nc) {
-                      if (key0 + key <= limit[nc][0]) o[i][nc][2 * f] = fmaf(__uint_as_float(w[nc] << 16), v, o[i][nc][2 * f]);
-                      if (key0 + key <= limit[nc][1]) o[i][nc][2 * f + 1] = fmaf(__uint_as_float(w[nc] & 0xffff0000u), v, o[i][nc][2 * f + 1]);
-                    }
-                  }
-              }
-        }
       }
       __syncwarp();                            // all lanes have read the stage
       if (ok) ask_next();
       if (++st == PG_STAGES) { st = 0; phase ^= 1; }
     }
     x += p.u1 - p.u0;
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1)
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) l[nc][e] += __shfl_xor_sync(0xffffffffu, l[nc][e], d);
-    const PgPlace done = p;
-    if (x < i_hi) { p = place_of(x, i_hi); load_q(p); }        // (on its way while the sums go out)
-    // features 16 i + gl and + 8 of queries 2 tl, 2 tl + 1 to rows of hd floats
-    auto put = [&](auto row_of) {
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float* dst = row_of(8 * nc + 2 * tl + e);
-          if (dst == nullptr) continue;
-#pragma unroll
-          for (int i = 0; i < KT; ++i) { dst[16 * i + gl] = o[i][nc][e]; dst[16 * i + 8 + gl] = o[i][nc][2 + e]; }
-        }
-      __syncwarp();
-    };
-    auto query_of = [&](int c) {               // (token, head)
-      const int tok = (col0 + c) / a.G;
-      return (int64_t)(start + tok) * a.nh + done.g * a.G + (col0 + c) - tok * a.G;
-    };
-    if (done.u0 == 0 && done.u1 == done.units) {
-      // ---- a whole item: out with it ------------------------------------------------------------------------------------------
-      if (group_of(a.row0 + done.i) >= 0) {    // its own pages' part, for the join with the shared ones'
-        put([&](int c) { return c < n_cols ? a.own + query_of(c) * HD : nullptr; });
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = 8 * nc + 2 * tl + e;
-            if (gl == 0 && c < n_cols) *reinterpret_cast<float2*>(a.own + (int64_t)a.T * a.nh * HD + 2 * query_of(c)) = make_float2(m[nc][e], l[nc][e]);
-          }
-      } else {
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc) {
-          const int c = 8 * nc + gl;           // (after the transposition)
-          const float i0 = l[nc][0] == 0.0f ? 0.0f : 1.0f / l[nc][0], i1 = l[nc][1] == 0.0f ? 0.0f : 1.0f / l[nc][1];
-          __nv_bfloat16* dst = a.out + query_of(min(c, n_cols - 1)) * HD + 2 * tl;
-#pragma unroll
-          for (int i = 0; i < KT; ++i)
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-              const uint32_t w = pg_transpose(pg_pack(o[i][nc][2 * f] * i0, o[i][nc][2 * f + 1] * i1));
-              if (c < n_cols) *reinterpret_cast<uint32_t*>(dst + 16 * i + 8 * f) = w;
-            }
-        }
-      }
-      __syncwarp();
-    } else if (x < i_hi) {
-      // ---- the first part, of an item that began in the share before: it waits until the ring is free ----------------------------------------
-      put([&](int c) { return spill + c * HD; });
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) { m_first[nc][e] = m[nc][e]; l_first[nc][e] = l[nc][e]; }
-      have_first = true;
-      if (lane == 0) { sm.part_at[warp][0] = done.base; sm.part_of[warp][0] = done; }
-    } else {
-      // ---- the last one -----------------------------------------------------------------------------------------------------------------
-      PgPart<HD, COLS>& part = reinterpret_cast<PgPart<HD, COLS>*>(ring)[1];
-      __syncwarp();
-      put([&](int c) { return part.acc[c]; });
-      if (gl == 0)
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) { part.m[8 * nc + 2 * tl + e] = m[nc][e]; part.l[8 * nc + 2 * tl + e] = l[nc][e]; }
-      if (lane == 0) { sm.part_at[warp][1] = done.base; sm.part_of[warp][1] = done; }
-    }
   }
   if (!ok) {                                   // what was asked for must land before the block's shared memory goes away
     if (lane == 0) atomicExch(&g_pg_error, 1);
-    for (int u = max(0, ask_n - PG_STAGES); u < ask_n; ++u) pg_wait(full + u % PG_STAGES, (u / PG_STAGES) & 1);
+    const int asked = ask_x - i_lo;
+#pragma unroll 1
+    for (int u = max(0, asked - PG_STAGES); u < asked; ++u) pg_wait(full + u % PG_STAGES, (u / PG_STAGES) & 1);
   }
   if (have_first) {
-    PgPart<HD, COLS>& part = reinterpret_cast<PgPart<HD, COLS>*>(ring)[0];
+    Part& part = reinterpret_cast<Part*>(ring)[0];
     __syncwarp();
+#pragma unroll 4
     for (int i = lane; i < COLS * HD / 4; i += 32) reinterpret_cast<float4*>(part.acc[0])[i] = reinterpret_cast<const float4*>(spill)[i];
     if (gl == 0)
 #pragma unroll
@@ -573,37 +547,35 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   __syncthreads();
 
   // ---- parts of items that shares cut: runs of the warps' parts, a warp for a run's query, a lane for V features of it -----------------------------------
-  constexpr int V = HD / 32;
   constexpr int REC = COLS * (HD + 2);
   float* const records = a.records + (int64_t)gridDim.x * PG_WARPS * (PG_MAX_COLS * HD);
-  auto block_begin = [&](int b) { return begin(b * PG_WARPS); };
-  auto block_of = [&](int64_t x) {
-    const int64_t longer = rem * (per + 1);    // (units of the longer shares; per is 0 only where there is one block)
-    return (int)(x < longer ? x / (per + 1) : rem + (x - longer) / max(per, (int64_t)1)) / PG_WARPS;
+  const int block_lo = begin(blockIdx.x * PG_WARPS), block_hi = begin((blockIdx.x + 1) * PG_WARPS);
+  auto block_of = [&](int at) {                // (per is 0 only where there is one block)
+    const int longer = rem * (per + 1);        // units of the longer shares
+    return (at < longer ? at / (per + 1) : rem + (at - longer) / max(per, 1)) / PG_WARPS;
   };
-  // a block's part of an item that began before the block, or with it, and the one that goes on in the next block
-  auto record = [&](int b, int64_t base) { return records + (2 * (int64_t)b + (block_begin(b) < base ? 1 : 0)) * REC; };
   if (threadIdx.x == 0) {
-    int n = 0;
+    int n = 0, last = -1;
     sm.edge[0] = sm.edge[1] = -1;
 #pragma unroll 1
     for (int k = 0; k < 2 * PG_WARPS; ++k) {
-      const int64_t at = sm.part_at[k >> 1][k & 1];
-      if (at < 0) continue;
-      if (n > 0 && sm.run[n - 1].p.base == at) { sm.run[n - 1].k1 = k + 1; continue; }
-      PgRun& r = sm.run[n++];
-      r.p = sm.part_of[k >> 1][k & 1];
-      r.k0 = k;
-      r.k1 = k + 1;
-      r.whole = at >= block_begin(blockIdx.x) && at + r.p.units <= block_begin(blockIdx.x + 1);
-      r.own = group_of(a.row0 + r.p.i) >= 0;
-      if (!r.whole) sm.edge[at <= block_begin(blockIdx.x) ? 0 : 1] = n - 1;
+      const PgPlace& q = sm.part_of[0][k];     // (of the warps one behind the other)
+      if (q.units == 0) continue;
+      if (q.base != last) {
+        PgRun& r = sm.run[n];
+        r.p = q;
+        r.k0 = k;
+        r.whole = q.base >= block_lo && q.base + q.units <= block_hi;
+        r.own = sm.shared[q.i] >= 0;
+        if (!r.whole) sm.edge[q.base <= block_lo ? 0 : 1] = n;
+        last = q.base;
+        ++n;
+      }
+      sm.run[n - 1].k1 = k + 1;
     }
     sm.n_runs = n;
   }
   __syncthreads();
-  auto parts = [&](int k) -> const PgPart<HD, COLS>& { return reinterpret_cast<const PgPart<HD, COLS>*>(rings + (k >> 1) * PG_RING)[k & 1]; };
-  auto cols_of = [&](const PgPlace& p) { return min(COLS, sm.n_new[p.i] * a.G - p.b * COLS); };
   // column c of a run's item, this lane's features
   auto write = [&](const PgRun& r, int c, float mm, float ll, const float (&y)[V]) {
     const int cc = r.p.b * COLS + c, tok = cc / a.G;
@@ -617,29 +589,30 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(a.out + th * HD + lane * V + i) = pg_pack(y[i] * inv, y[i + 1] * inv);
     }
   };
+  // a running sum, and a part more
+  auto add = [&](float& mm, float& ll, float (&y)[V], float m1, float l1, const float (&y1)[V]) {
+    const float top = fmaxf(mm, m1), safe = top == PG_NEG ? 0.0f : top, f0 = pg_exp2(mm - safe), f1 = pg_exp2(m1 - safe);
+    ll = ll * f0 + l1 * f1;
+#pragma unroll
+    for (int v = 0; v < V; ++v) y[v] = y[v] * f0 + y1[v] * f1;
+    mm = top;
+  };
 #pragma unroll 1
   for (int k = 0; k < sm.n_runs; ++k) {
     const PgRun& r = sm.run[k];
-    const int n_cols = cols_of(r.p);
-    float* const rec = record(blockIdx.x, r.p.base);
+    const int n_cols = min(COLS, sm.n_new[r.p.i] * a.G - r.p.b * COLS);
+    // a block's record of an item that began before the block, or with it, and of the one that goes on in the next block
+    float* const rec = records + (2 * blockIdx.x + (block_lo < r.p.base ? 1 : 0)) * REC;
 #pragma unroll 1
     for (int c = warp; c < n_cols; c += PG_WARPS) {
       float mm = PG_NEG, ll = 0.0f, y[V] = {};
 #pragma unroll 1
-      for (int i = r.k0; i < r.k1; ++i)
-        if (sm.part_at[i >> 1][i & 1] >= 0) mm = fmaxf(mm, parts(i).m[c]);         // (a warp without a part there may be between)
-      const float safe = mm == PG_NEG ? 0.0f : mm;
-#pragma unroll 1
       for (int i = r.k0; i < r.k1; ++i) {
-        if (sm.part_at[i >> 1][i & 1] < 0) continue;
-        const float f = pg_exp2(parts(i).m[c] - safe);
-        ll = fmaf(parts(i).l[c], f, ll);
-        const float* const acc = &parts(i).acc[c][lane * V];
+        if (sm.part_of[0][i].units == 0) continue;         // (a warp without a part there may be between)
+        const Part& part = reinterpret_cast<const Part*>(rings + (i >> 1) * PG_RING)[i & 1];
         float y1[V];
-        if (V == 4) { const float4 w = *reinterpret_cast<const float4*>(acc); y1[0] = w.x; y1[1] = w.y; y1[V - 2] = w.z; y1[V - 1] = w.w; }
-        else { const float2 w = *reinterpret_cast<const float2*>(acc); y1[0] = w.x; y1[1] = w.y; }
-#pragma unroll
-        for (int v = 0; v < V; ++v) y[v] = fmaf(y1[v], f, y[v]);
+        pg_load(&part.acc[c][lane * V], y1);
+        add(mm, ll, y, part.m[c], part.l[c], y1);
       }
       if (r.whole) {
         write(r, c, mm, ll, y);
@@ -657,8 +630,8 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       const int k = sm.edge[threadIdx.x];
       bool last = false;
       if (k >= 0) {
-        const PgPlace& p = sm.run[k].p;
-        const int ba = block_of(p.base), bb = block_of(p.base + p.units - 1);
+        const PgPlace& q = sm.run[k].p;
+        const int ba = block_of(q.base), bb = block_of(q.base + q.units - 1);
         last = atomicAdd(a.counters + ba, 1) == bb - ba;             // (of the items that begin in a block only one goes beyond it)
         if (last) a.counters[ba] = 0;
       }
@@ -670,11 +643,9 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int e = 0; e < 2; ++e) {
       if (!sm.last[e]) continue;
       const PgRun& r = sm.run[sm.edge[e]];
-      const int ba = block_of(r.p.base), n = block_of(r.p.base + r.p.units - 1) - ba + 1, n_cols = cols_of(r.p);
+      const int ba = block_of(r.p.base), n = block_of(r.p.base + r.p.units - 1) - ba + 1, n_cols = min(COLS, sm.n_new[r.p.i] * a.G - r.p.b * COLS);
       // the records of blocks ba .. ba + n - 1: all but the first are their blocks' first
-      const float* const rec0 = record(ba, r.p.base);
-      auto rec = [&](int i) { return i == 0 ? rec0 : records + 2 * (int64_t)(ba + i) * REC; };
-      // (this code runs once: short, since its way into the SM costs more than its loads)
+      const float* const rec0 = records + (2 * ba + (begin(ba * PG_WARPS) < r.p.base ? 1 : 0)) * REC;
 #pragma unroll 1
       for (int c = warp; c < n_cols; c += PG_WARPS) {
         float mm = PG_NEG, ll = 0.0f, y[V] = {};
@@ -683,24 +654,14 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           float m1[4], l1[4], y1[4][V];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool in = i0 + i < n;
-            const float* q = rec(in ? i0 + i : 0);
-            m1[i] = in ? __ldcg(q + c) : PG_NEG;
+            const float* q = i0 + i > 0 && i0 + i < n ? records + 2 * (ba + i0 + i) * REC : rec0;
+            m1[i] = __ldcg(q + c);
             l1[i] = __ldcg(q + COLS + c);
-            pg_load(q + 2 * COLS + c * HD + lane * V, y1[i]);
+            pg_load_cg(q + 2 * COLS + c * HD + lane * V, y1[i]);
           }
-          const float top = fmaxf(fmaxf(fmaxf(m1[0], m1[1]), fmaxf(m1[2], m1[3])), mm), safe = top == PG_NEG ? 0.0f : top, f0 = pg_exp2(mm - safe);
-          ll *= f0;
 #pragma unroll
-          for (int v = 0; v < V; ++v) y[v] *= f0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float f = i0 + i < n ? pg_exp2(m1[i] - safe) : 0.0f;
-            ll += i0 + i < n ? l1[i] * f : 0.0f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) y[v] += i0 + i < n ? y1[i][v] * f : 0.0f;
-          }
-          mm = top;
+          for (int i = 0; i < 4; ++i)
+            if (i0 + i < n) add(mm, ll, y, m1[i], l1[i], y1[i]);
         }
         write(r, c, mm, ll, y);
       }
@@ -711,7 +672,8 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 
-constexpr int PG_SMEM = (int)(PG_SMEM_RINGS + sizeof(PgSmem) + 1024);
+constexpr int PG_SMEM = (int)(PG_SMEM_RINGS + sizeof(PgSmem<128>) + 1024);
+static_assert(PG_SMEM <= 232448, "what a block may have");
 
 int pg_sms(const char* what) {                 // of the current device, 0: an error
   static int known[64] = {};
@@ -753,12 +715,17 @@ static int64_t ps_tiles_of(int64_t T, int G, int rows, int n_groups, int max_new
   return n_groups ? T * G / PS_TILE + n_groups : 0;
 }
 
-template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int most_cols, int sms, const char* what, cudaStream_t stream) {
-  for (int r0 = 0; r0 < a.rows; r0 += PG_WINDOW) {
+template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int max_new, int sms, const char* what, cudaStream_t stream) {
+  // as many rows a launch as have fewer than 2^31 units together
+  const int cols = (int64_t)max_new * a.G <= 8 ? 8 : 16;
+  const int64_t queries = a.many ? PS_MANY : (int64_t)max_new * a.G, row = (int64_t)(LIST ? a.count : a.bt_width) * (hd / 64) * a.nkv * ((queries + cols - 1) / cols);
+  a.window = (int)std::min<int64_t>(PG_WINDOW, INT32_MAX / row);
+  if (a.window < 1) { set_error("%s: a row of %d pages with %lld queries of %d key/value heads is too long", what, a.bt_width, (long long)queries, a.nkv); return ERR_UNSUPPORTED; }
+  for (int r0 = 0; r0 < a.rows; r0 += a.window) {
     a.row0 = r0;
     a.wait_first = r0 > 0 || !a.tiles;
     auto go = [&](auto kernel) { launch_pdl(kernel, dim3(sms), dim3(PG_WARPS * 32), PG_SMEM, stream, map_k, map_v, a); };
-    if (most_cols <= 8) { if (hd == 64) go(attn_pages_kernel<64, 1, LIST>); else go(attn_pages_kernel<128, 1, LIST>); }
+    if (cols == 8) { if (hd == 64) go(attn_pages_kernel<64, 1, LIST>); else go(attn_pages_kernel<128, 1, LIST>); }
     else { if (hd == 64) go(attn_pages_kernel<64, 2, LIST>); else go(attn_pages_kernel<128, 2, LIST>); }
     const int rc = launch_status(what);
     if (rc) return rc;
@@ -769,7 +736,7 @@ template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, co
 // What both entry points ask of their arguments, and the pools' maps.
 static int pg_check(const char* what, const void* q, int64_t q_stride, const void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table,
                     int bt_width, int rows, int T, int nh, int nkv, int hd, float scale, CUtensorMap* map_k, CUtensorMap* map_v) {
-  if (rows < 0 || T < 0 || nkv < 1 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || !(scale > 0.0f) || !isfinite(scale) || n_pages < 1 ||
+  if (rows < 0 || T < 0 || nkv < 1 || nkv > 4096 || nh < nkv || nh % nkv || (hd != 64 && hd != 128) || !(scale > 0.0f) || !isfinite(scale) || n_pages < 1 ||
       (n_pages + 1) * nkv * PG_PAGE > INT32_MAX || bt_width < 1 || bt_width > PG_MAX_WIDTH || (int64_t)T * (nh / nkv) > INT32_MAX - PG_MAX_COLS) {
     set_error("%s: needs heads of 64 or 128, a positive scale, tables of at most %d pages and pools of fewer than 2^31 tokens times key/value heads, got %d rows, %d tokens, %d "
               "heads on %d of %d, scale %g, %lld pages, a table of %d", what, PG_MAX_WIDTH, rows, T, nh, nkv, hd, (double)scale, (long long)n_pages, bt_width);
@@ -827,7 +794,7 @@ extern "C" int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, T, T, nh, nkv, scale, scratch);
   a.tok_pos = tok_pos; a.tok_seq = tok_seq; a.lists = lists; a.count = std::min(count, bt_width);
   a.list_stride = count; a.bt_rows = bt_rows;
-  return pg_launch<true>(a, map_k, map_v, hd, a.G, sms, "attn_pages", stream);
+  return pg_launch<true>(a, map_k, map_v, hd, 1, sms, "attn_pages", stream);
 }
 
 // Causal attention of rows whose groups share their first pages (groups: int32 [n_groups, 3]: first row, rows, pages).
@@ -866,6 +833,6 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
     rc = attn_shared_launch(p, k_pool, v_pool, hd, sms, stream);
     if (rc) return rc;
   }
-  rc = pg_launch<false>(a, map_k, map_v, hd, (int)std::min((int64_t)max_new * a.G, (int64_t)PG_MAX_COLS), sms, "attn_shared", stream);
+  rc = pg_launch<false>(a, map_k, map_v, hd, max_new, sms, "attn_shared", stream);
   return rc || !tiles ? rc : attn_shared_join(p, a.own, a.out, hd, stream);
 }
