@@ -128,6 +128,8 @@ template <int HD> struct PgSmem {
   int last[2];
   int odd_key[PG_WARPS][HD];                   // per feature the first key whose value is not finite among those that not all of an item's queries see
   PgGroups groups;
+  int group_queries[PG_MAX_GROUPS];
+  unsigned long long cost;                     // of the groups' tiles
 };
 
 // Keys are the rows of the first product and queries its columns, S^T = K Q^T (8 columns an instruction; NC of them side by side), and the second is O^T = V^T P^T: half
@@ -174,24 +176,29 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     sm.start[i] = start;
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
   }
+  if (!LIST && a.n_groups > 0) for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32) sm.group_queries[j] = 0;
+  if (threadIdx.x == 0) sm.cost = 0;
   if (LIST) __syncthreads();
   else pg_groups(sm.groups, a.groups, a.n_groups, a.rows, a.bt_width);
-  int total = 0;
+  int total = 0, items = 0;
 #pragma unroll 1
   for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
     const int i = i0 + threadIdx.x;
-    int mine = 0;
+    int mine = 0, blocks = 0;
     if (i < n_rows) {
       const int pos = sm.pos[i], queries = sm.n_new[i] * a.G, j = LIST ? -1 : sm.groups.of(a.row0 + i), shared = j < 0 ? -1 : sm.groups.pages[j];
       const int units = LIST ? min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP : (min(pos + sm.n_new[i], most_keys) + KS - 1) / KS - max(shared, 0) * UPP;
       sm.shared[i] = shared;
       sm.units[i] = max(units, 1);             // (one at least: every query gets an answer)
-      mine = !LIST && a.many && queries > PS_MANY ? 0 : max(units, 1) * ((queries + COLS - 1) / COLS) * a.nkv;
+      blocks = !LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS;
+      mine = max(units, 1) * blocks * a.nkv;
+      if (j >= 0) atomicAdd(&sm.group_queries[j], queries);
     }
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
     if (lane == 31) sm.warp_sum[warp] = incl;
+    items += __reduce_add_sync(0xffffffffu, blocks);                  // (a warp's, over its rounds)
     __syncthreads();
     int before = total;
 #pragma unroll
@@ -200,8 +207,21 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __syncthreads();
   }
   if (threadIdx.x == 0) sm.cum[0] = 0;
+  if (lane == 0) sm.warp_sum[warp] = items;
+  const bool beside = !LIST && a.n_groups > 0 && !a.many && a.rows <= a.window;     // the other kernel leaves this one some of the SMs
+  if (beside)
+    for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32)
+      if (sm.groups.pages[j] > 0 && sm.group_queries[j] > 0) atomicAdd(&sm.cost, (unsigned long long)ps_cost(sm.group_queries[j], sm.groups.pages[j]));
   __syncthreads();
-  const int n_blocks = min((int)gridDim.x, max(1, total / (PG_WARPS * PG_MIN_UNITS))), n_shares = n_blocks * PG_WARPS;
+  int sms = gridDim.x;
+  if (beside && sm.cost > 0) {
+    items = 0;
+#pragma unroll
+    for (int w = 0; w < PG_WARPS; ++w) items += sm.warp_sum[w];
+    sms -= ps_sms((int64_t)sm.cost * a.nkv, (int64_t)total * PG_COST_UNIT + (int64_t)items * a.nkv * PG_COST_ITEM, total, gridDim.x);
+    if (sms < 1) sms = gridDim.x;
+  }
+  const int n_blocks = min(sms, max(1, total / (PG_WARPS * PG_MIN_UNITS))), n_shares = n_blocks * PG_WARPS;
   if (total == 0 || (int)blockIdx.x >= n_blocks) {
     if (!a.wait_first) pdl_wait();
     return;
@@ -694,13 +714,12 @@ int pg_sms(const char* what) {                 // of the current device, 0: an e
 
 // Where the warps' first parts wait, and the blocks' parts.
 static int64_t pg_record_floats(int sms, int hd) { return (int64_t)sms * (PG_WARPS * PG_MAX_COLS * hd + 2 * PG_MAX_COLS * (hd + 2)); }
-// With tiles: the plan, the tiles, the tokens, the tiles' parts, the rows' own parts.
-struct PsSpace { int64_t plan, tiles, tokens, records, own, end; };            // floats from the start of this part of the scratch memory
+// With tiles: their parts' places, the tokens, the tiles' parts, the rows' own parts.
+struct PsSpace { int64_t parts, tokens, records, own, end; };                  // floats from the start of this part of the scratch memory
 static PsSpace ps_space(int sms, int64_t T, int G, int nkv, int hd, int tiles) {
   PsSpace s = {};
   auto after = [](int64_t at, int64_t n) { return (at + n + 15) / 16 * 16; };
-  s.tiles = after(0, sizeof(PsPlan) / 4);
-  s.tokens = after(s.tiles, 4 * (int64_t)tiles);
+  s.tokens = after(0, 4 * (int64_t)tiles * nkv);
   s.records = after(s.tokens, 4 * T);
   s.own = after(s.records, ps_slots(sms, nkv, tiles) * ps_record(hd));
   s.end = after(s.own, ps_own(T, G * nkv, hd));
@@ -715,12 +734,17 @@ static int64_t ps_tiles_of(int64_t T, int G, int rows, int n_groups, int max_new
   return n_groups ? T * G / PS_TILE + n_groups : 0;
 }
 
+static int pg_cols(int max_new, int G) { return (int64_t)max_new * G <= 8 ? 8 : 16; }
+// As many rows a launch as have fewer than 2^31 units together.
+static int pg_window(const PgArgs& a, int hd, int max_new, bool list) {
+  const int cols = pg_cols(max_new, a.G);
+  const int64_t queries = a.many ? PS_MANY : (int64_t)max_new * a.G, row = (int64_t)(list ? a.count : a.bt_width) * (hd / 64) * a.nkv * ((queries + cols - 1) / cols);
+  return (int)std::min<int64_t>(PG_WINDOW, INT32_MAX / row);
+}
 template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int max_new, int sms, const char* what, cudaStream_t stream) {
-  // as many rows a launch as have fewer than 2^31 units together
-  const int cols = (int64_t)max_new * a.G <= 8 ? 8 : 16;
-  const int64_t queries = a.many ? PS_MANY : (int64_t)max_new * a.G, row = (int64_t)(LIST ? a.count : a.bt_width) * (hd / 64) * a.nkv * ((queries + cols - 1) / cols);
-  a.window = (int)std::min<int64_t>(PG_WINDOW, INT32_MAX / row);
-  if (a.window < 1) { set_error("%s: a row of %d pages with %lld queries of %d key/value heads is too long", what, a.bt_width, (long long)queries, a.nkv); return ERR_UNSUPPORTED; }
+  const int cols = pg_cols(max_new, a.G);
+  a.window = pg_window(a, hd, max_new, LIST);
+  if (a.window < 1) { set_error("%s: rows of %d pages and %d tokens of %d query heads on %d are too long", what, a.bt_width, max_new, a.nh, a.nkv); return ERR_UNSUPPORTED; }
   for (int r0 = 0; r0 < a.rows; r0 += a.window) {
     a.row0 = r0;
     a.wait_first = r0 > 0 || !a.tiles;
@@ -827,7 +851,8 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
     const PsSpace s = ps_space(sms, T, a.G, nkv, hd, (int)tiles);
     p.q = a.q; p.q_stride = q_stride; p.block_table = block_table; p.bt_stride = bt_stride; p.bt_width = bt_width; p.n_pages = (int)n_pages; p.row_start = row_start;
     p.row_pos0 = row_pos0; p.rows = rows; p.T = T; p.nkv = nkv; p.G = a.G; p.groups = groups; p.n_groups = n_groups; p.many = a.many; p.scale_log2 = a.scale_log2;
-    p.plan = reinterpret_cast<PsPlan*>(at + s.plan); p.tiles = reinterpret_cast<int*>(at + s.tiles); p.tokens = reinterpret_cast<PsToken*>(at + s.tokens);
+    p.parts = reinterpret_cast<int*>(at + s.parts); p.most_tiles = (int)tiles; p.sms = sms; p.tokens = reinterpret_cast<PsToken*>(at + s.tokens);
+    p.cols = pg_cols(max_new, a.G); p.window = pg_window(a, hd, max_new, false); p.hd = hd;
     p.records = at + s.records;
     a.own = at + s.own;
     rc = attn_shared_launch(p, k_pool, v_pool, hd, sms, stream);

@@ -55,7 +55,25 @@ constexpr int PS_MANY = 64;                    // queries of a row and key/value
 constexpr int PS_MIN_PAGES = 4;                // places of a share, at least: every part more is joined again
 constexpr int PS_SETUP = 4;                    // places of the list that a tile has beside its pages': what its queries' way in and its sums' way out cost, in pages
 
-struct PsPlan {                                // the head of the list, in scratch memory for the join
+// Both kernels run side by side where there is work for both: the tensor cores' takes some of the SMs and leaves the others to the walk, whose streams of pages fill the memory's queue
+// from fewer SMs than there are (a batch of 64 behind 4,096 shared keys, 32 heads of 128 on 8, 30 to 2,000 keys of their own: one after the other 117 us).  Both work out how many, in units of
+// 10 ns of an SM: `tiles` for the tiles' pages (120 for two sets of queries, 60 for one), `walk` for the rows' own units of 16 KB (28, and 100 for an item); and the time that
+// the memory takes for these (16 KB in 2.5 ns).
+__host__ __device__ inline int ps_sms(int64_t tiles, int64_t walk, int64_t units, int sms) {
+  if (tiles == 0 || walk == 0) return sms;
+  int64_t n = (tiles * sms + (tiles + walk) / 2) / (tiles + walk);
+  const int64_t memory = units / 4;            // 10 ns
+  if (memory > 0 && tiles / memory + 1 < n) n = tiles / memory + 1;
+  return (int)(n < 1 ? 1 : n > sms - 1 ? sms - 1 : n);
+}
+constexpr int64_t PS_COST_TWO = 120, PS_COST_ONE = 60, PG_COST_UNIT = 28, PG_COST_ITEM = 100;
+
+// A group's tiles of a key/value head, in the units of ps_sms.
+__device__ inline int64_t ps_cost(int queries, int pages) {
+  return (int64_t)((queries + PS_TILE - 1) / PS_TILE) * (pages + PS_SETUP) * (queries > 128 ? PS_COST_TWO : PS_COST_ONE);
+}
+
+struct PsPlan {                                // the head of the list
   int n_tiles;
   int blocks;                                  // shares
   int64_t total, per, rem;                     // places of the list; a share has `per` of them, the first `rem` shares one more
@@ -86,15 +104,16 @@ struct PsArgs {
   int bt_stride, bt_width, n_pages;
   const int* row_start;
   const int* row_pos0;
-  int rows, T, nkv, G;
+  int rows, T, nkv, G, hd;
   const int* groups;
   int n_groups;
   int many;                                    // whether rows of more than PS_MANY queries have tiles of their own
+  int cols, window;                            // queries of an item of the walk, rows of a launch of it
   float scale_log2;
   float* records;
-  PsPlan* plan;
   PsToken* tokens;
-  int* tiles;                                  // for the join: per tile its place in a head's list, its pages, its queries, and the head's places [tiles][4]
+  int* parts;                                  // for the join: per kv head and tile its first part's slot, its parts, the halves of a record (1 or 2) [kv heads][most tiles][4]
+  int most_tiles, sms;
 };
 cudaError_t attn_shared_prepare();             // once for a device
 int attn_shared_launch(const PsArgs& a, const void* k_pool, const void* v_pool, int hd, int sms, cudaStream_t stream);

@@ -45,6 +45,8 @@ struct PsTiles {
   int row_tile[PS_MAX_ROWS];                   // a row's own first tile, -1: none
   int warp_sum[PS_THREADS / 32];
   int small;                                   // no tile has more than 128 queries
+  int sms;                                     // for this kernel
+  unsigned long long units, items, cost;       // of the walk, and the tiles'
   int odd_key[2][3][128];                      // per set, in turns (a warp may be two parts behind another), and feature: the first key whose value is not finite among those that not all of the tile's queries see
   int odd[2][3];
 };
@@ -184,13 +186,26 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   }
   // rows of many tokens: their queries, for now, and what of the shared pages a group's rows see
   const int n_rows = a.many ? a.rows : 0;
+  if (threadIdx.x == 0) t.units = t.items = t.cost = 0;
   __syncthreads();
+  int64_t units = 0, items = 0;
+  const int ks = a.hd == 64 ? 64 : 32;
   for (int r = threadIdx.x; r < a.rows; r += PS_THREADS) {
     const int s0 = start_of(r), s1 = start_of(r + 1), j = t.groups.of(r);
     if (j >= 0 && s1 > s0) atomicMin(&t.group_seen[j], pos_of(r));
+    if (s1 > s0) {                             // (as the walk does)
+      const int blocks = ((s1 - s0) * a.G + a.cols - 1) / a.cols;
+      units += (int64_t)max(1, (min(max(pos_of(r), -most) + s1 - s0, most) + ks - 1) / ks - (j >= 0 ? t.groups.pages[j] : 0) * (PG_PAGE / ks)) * blocks;
+      items += blocks;
+    }
     if (r < n_rows) t.row_tile[r] = s1 > s0 && (int64_t)(s1 - s0) * a.G > PS_MANY ? (s1 - s0) * a.G : 0;
   }
   __syncthreads();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { units += __shfl_xor_sync(0xffffffffu, units, o); items += __shfl_xor_sync(0xffffffffu, items, o); }
+  if ((threadIdx.x & 31) == 0 && items) { atomicAdd(&t.units, (unsigned long long)units); atomicAdd(&t.items, (unsigned long long)items); }
+  for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS)
+    if (t.group_tile[j]) atomicAdd(&t.cost, (unsigned long long)ps_cost(t.group_tile[j], t.groups.pages[j]));
   // places: groups, then rows, a thread each, in rounds of the block
   int n_tiles = 0, small = 1;
   for (int i0 = 0; i0 < a.n_groups + n_rows; i0 += PS_THREADS) {
@@ -239,9 +254,11 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
       PsPlan& p = t.plan;
       t.cum[0] = 0;
       t.small = small;
+      // (beside rows of many tokens the walk has little to do, and of more rows than a launch of it takes it knows no more than these)
+      t.sms = a.many || a.rows > a.window ? (int)gridDim.x : ps_sms(t.cost * a.nkv, (t.units * PG_COST_UNIT + t.items * PG_COST_ITEM) * a.nkv, t.units * a.nkv, gridDim.x);
       p.n_tiles = n_tiles;
       p.total = (int64_t)run * a.nkv;
-      p.blocks = (int)min((int64_t)gridDim.x, max((int64_t)1, p.total / PS_MIN_PAGES));
+      p.blocks = (int)min((int64_t)t.sms, max((int64_t)1, p.total / PS_MIN_PAGES));
       p.per = p.total / p.blocks;
       p.rem = p.total - p.per * p.blocks;
     }
@@ -381,11 +398,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     }
     if (!ok && lane == 0) atomicExch(&g_ps_error, 2);
   } else if (warp == 9) {
-    // ---- for the join, while the first scores are on their way: the plan, the tiles, and every token's -------------------------------
-    if (blockIdx.x == 0) {
-      if (lane == 0) *a.plan = plan;
-      for (int i = lane; i < plan.n_tiles; i += 32)
-        reinterpret_cast<int4*>(a.tiles)[i] = make_int4(tiles.cum[i] + PS_SETUP, tiles.cum[i + 1] - tiles.cum[i] - PS_SETUP, tiles.queries[i], tiles.cum[plan.n_tiles]);
+    // ---- for the join, while the first scores are on their way: the tiles' parts, and every token's tiles -------------------------------
+    for (int i = blockIdx.x * 32 + lane; i < plan.n_tiles * a.nkv; i += gridDim.x * 32) {
+      const int g = i / plan.n_tiles, tile = i - g * plan.n_tiles;
+      const int64_t first = (int64_t)g * tiles.cum[plan.n_tiles] + tiles.cum[tile] + PS_SETUP, last = first + tiles.cum[tile + 1] - tiles.cum[tile] - PS_SETUP - 1;
+      const int b0 = plan.block_of(first), halves = tiles.queries[tile] > 128 ? 1 : 2;
+      reinterpret_cast<int4*>(a.parts)[(int64_t)g * a.most_tiles + tile] = make_int4(b0 + i, (plan.block_of(last) - b0 + 1) * halves, halves, 0);
     }
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
       const int s0 = min(max(__ldcg(a.row_start + r), 0), a.T), s1 = min(__ldcg(a.row_start + r + 1), a.T), j = tiles.groups.of(r);
@@ -630,8 +648,8 @@ constexpr int PJ_WARPS = 4;
 constexpr int PJ_PARTS = 1024;                 // four for every SM, at most
 template <int HD, int SPLIT>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
-attn_shared_join_kernel(const PsPlan* __restrict__ plan, const int4* __restrict__ tiles, const int4* __restrict__ tokens, const float* __restrict__ records,
-                        const float* __restrict__ own, __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
+attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slots, const int4* __restrict__ tokens, const float* __restrict__ records, const float* __restrict__ own,
+                        __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
   constexpr int V = HD / 32, PAIRS = PJ_WARPS / SPLIT;       // features a lane; pairs a block
   __shared__ float s_w[PAIRS][PJ_PARTS + 1];
   __shared__ float s_y[SPLIT > 1 ? PJ_WARPS : 1][SPLIT > 1 ? HD : 1];
@@ -643,26 +661,19 @@ attn_shared_join_kernel(const PsPlan* __restrict__ plan, const int4* __restrict_
   if (SPLIT == 1 && !there) return;
   const int tok = there ? (int)(th / nh) : 0, head = there ? (int)(th - (int64_t)tok * nh) : 0, G = nh / nkv, g = head / G, h = head - g * G;
   const int4 w = __ldcg(tokens + tok);         // (shared tile, its first token, own tile, its first token)
-  const int n_tiles = __ldcg(&plan->n_tiles);
-  const int64_t per = __ldcg(&plan->per), rem = __ldcg(&plan->rem), longer = rem * (per + 1);
-  auto share_of = [&](int64_t x) {
-    if (longer + per * 1024 <= INT32_MAX && x <= INT32_MAX)              // (as a rule)
-      return x < longer ? (int)((uint32_t)x / (uint32_t)(per + 1)) : (int)rem + (int)((uint32_t)(x - longer) / (uint32_t)per);
-    return x < longer ? (int)(x / (per + 1)) : (int)(rem + (x - longer) / per);
-  };
   // a source: the parts of one tile
   struct Source { const float* at; int n, halves, row; };     // its first record, its parts, and the query's place in a record
   auto source = [&](int tile0, int tok0) {
     Source s = {records, 0, 1, 0};
     const int query = (tok - tok0) * G + h, tile = tile0 + query / PS_TILE;
-    if (tile0 < 0 || query < 0 || tile >= n_tiles) return s;
-    const int4 t = __ldcg(tiles + tile);
-    const int64_t first = (int64_t)g * t.w + t.x;
-    const int b0 = share_of(first);
-    s.halves = t.z > 128 ? 1 : 2;
-    s.n = (share_of(first + t.y - 1) - b0 + 1) * s.halves;
+    if (tile0 < 0 || query < 0 || tile >= most_tiles) return s;
+    const int4 t = __ldcg(parts + (int64_t)g * most_tiles + tile);
+    // (rows that are not one behind the other leave tokens without a tile: nothing beyond the records is read for them)
+    if (t.x < 0 || t.y < 1 || t.y >= PJ_PARTS / 2 || t.z < 1 || t.z > 2 || t.x + t.y / t.z > slots) return s;
+    s.n = t.y;
+    s.halves = t.z;
     s.row = query % PS_TILE;
-    s.at = records + (b0 + (int64_t)g * n_tiles + tile) * ps_record(HD);
+    s.at = records + t.x * ps_record(HD);
     return s;
   };
   const bool any = there && (w.x >= 0 || w.z >= 0);          // else its own pages' part was all
@@ -735,7 +746,7 @@ int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int 
   const int64_t pairs = (int64_t)a.T * a.nkv * a.G;
   const bool few = pairs <= 4096;
   auto go = [&](auto kernel, int per_block) {
-    launch_pdl(kernel, dim3((unsigned)((pairs + per_block - 1) / per_block)), dim3(PJ_WARPS * 32), 0, stream, (const PsPlan*)a.plan, reinterpret_cast<const int4*>(a.tiles),
+    launch_pdl(kernel, dim3((unsigned)((pairs + per_block - 1) / per_block)), dim3(PJ_WARPS * 32), 0, stream, reinterpret_cast<const int4*>(a.parts), a.most_tiles, (int)ps_slots(a.sms, a.nkv, a.most_tiles),
                reinterpret_cast<const int4*>(a.tokens), (const float*)a.records, own, out, a.T, a.nkv * a.G, a.nkv);
   };
   if (hd == 64) { if (few) go(attn_shared_join_kernel<64, PJ_WARPS>, 1); else go(attn_shared_join_kernel<64, 1>, PJ_WARPS); }
