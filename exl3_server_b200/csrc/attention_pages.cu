@@ -15,11 +15,11 @@
 
 namespace exl3 {
 
-constexpr int PG_WARPS = 4;                    // of a block, one block an SM
+constexpr int PG_WARPS = 8;                    // of a block, one block an SM: two a scheduler, whose chains of one unit's steps overlap
 constexpr int PG_STAGES = 3;                   // of a warp's ring
-constexpr int PG_UNIT_BYTES = 16384;           // a unit: keys and values of 64 tokens (heads of 64) or 32 (heads of 128)
+constexpr int PG_UNIT_BYTES = 8192;            // a unit: keys and values of 32 tokens (heads of 64) or 16 (heads of 128)
 constexpr int PG_WINDOW = 1024;                // rows of a launch
-constexpr int PG_MIN_UNITS = 2;                // of a warp's share, at least
+constexpr int PG_MIN_UNITS = 4;                // places of a warp's share, at least
 constexpr int PG_MAX_WIDTH = 1 << 19;          // pages of a row
 constexpr int PG_RING = PG_STAGES * PG_UNIT_BYTES;
 constexpr uint32_t PG_SMEM_RINGS = PG_WARPS * PG_RING;
@@ -114,13 +114,14 @@ template <int HD, int COLS> struct PgPart {
   float m[COLS], l[COLS], acc[COLS][HD];
 };
 // An item, and where in it a share is.
-struct PgPlace { int i, g, b, u0, u1, units, base; };
+// (base: the place of its first unit; places: of the share's)
+struct PgPlace { int i, g, b, u0, u1, units, base, places; };
 struct PgRun { PgPlace p; int k0, k1; bool whole, own; };
 template <int HD> struct PgSmem {
   uint64_t full[PG_WARPS][PG_STAGES];
   PgRun run[2 * PG_WARPS];
   int n_runs, edge[2];
-  int cum[PG_WINDOW + 1];                      // units of the rows before
+  int cum[PG_WINDOW + 1];                      // places of the rows before
   int start[PG_WINDOW], n_new[PG_WINDOW], pos[PG_WINDOW], units[PG_WINDOW];
   int shared[PG_WINDOW];                       // the pages that the row shares, -1: it is in no group
   PgPlace part_of[PG_WARPS][2];                // the warps' parts' items; units 0: none
@@ -135,8 +136,8 @@ template <int HD> struct PgSmem {
 // Keys are the rows of the first product and queries its columns, S^T = K Q^T (8 columns an instruction; NC of them side by side), and the second is O^T = V^T P^T: half
 // the instructions that queries as 16 rows would take for up to 8 of them.
 //
-// Items: up to 8 NC queries (token, query head) of a row (or of a listed token) and key/value head, which walk the same pages.  The units of all items, ordered by row, head and
-// item, are cut into equal shares for the warps, which stream them through rings of their own, each asking for its own copies: nothing is waited for but
+// Items: up to 8 NC queries (token, query head) of a row (or of a listed token) and key/value head, which walk the same pages.  The list of all items, ordered by row, head and
+// item, with PG_SETUP places and one for each unit, is cut into equal shares for the warps, which stream them through rings of their own, each asking for its own copies: nothing is waited for but
 // memory.  What a warp has whole it writes out; parts of items that shares cut are joined in shared memory at the end, and those that blocks cut by the block that
 // is the last to report, always in the order of the pages, so that results do not depend on which it was.
 //
@@ -145,7 +146,7 @@ template <int HD, int NC, bool LIST>
 __global__ void __launch_bounds__(PG_WARPS * 32, 1)
 attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PgArgs a) {
   constexpr int COLS = 8 * NC;
-  constexpr int KS = HD == 64 ? 64 : 32;       // keys of a unit
+  constexpr int KS = HD == 64 ? 32 : 16;       // keys of a unit
   constexpr int UPP = PG_PAGE / KS;            // units of a page
   constexpr int MT = KS / 16;                  // tiles of 16 keys
   constexpr int KT = HD / 16;                  // pieces of 16 features
@@ -180,7 +181,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   if (threadIdx.x == 0) sm.cost = 0;
   if (LIST) __syncthreads();
   else pg_groups(sm.groups, a.groups, a.n_groups, a.rows, a.bt_width);
-  int total = 0, items = 0;
+  int total = 0;
 #pragma unroll 1
   for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
     const int i = i0 + threadIdx.x;
@@ -191,14 +192,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       sm.shared[i] = shared;
       sm.units[i] = max(units, 1);             // (one at least: every query gets an answer)
       blocks = !LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS;
-      mine = max(units, 1) * blocks * a.nkv;
+      mine = (max(units, 1) + PG_SETUP) * blocks * a.nkv;
       if (j >= 0) atomicAdd(&sm.group_queries[j], queries);
     }
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
     if (lane == 31) sm.warp_sum[warp] = incl;
-    items += __reduce_add_sync(0xffffffffu, blocks);                  // (a warp's, over its rounds)
     __syncthreads();
     int before = total;
 #pragma unroll
@@ -207,7 +207,6 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __syncthreads();
   }
   if (threadIdx.x == 0) sm.cum[0] = 0;
-  if (lane == 0) sm.warp_sum[warp] = items;
   const bool beside = !LIST && a.n_groups > 0 && !a.many && a.rows <= a.window;     // the other kernel leaves this one some of the SMs
   if (beside)
     for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32)
@@ -215,10 +214,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   __syncthreads();
   int sms = gridDim.x;
   if (beside && sm.cost > 0) {
-    items = 0;
-#pragma unroll
-    for (int w = 0; w < PG_WARPS; ++w) items += sm.warp_sum[w];
-    sms -= ps_sms((int64_t)sm.cost * a.nkv, (int64_t)total * PG_COST_UNIT + (int64_t)items * a.nkv * PG_COST_ITEM, total, gridDim.x);
+    sms -= ps_sms((int64_t)sm.cost * a.nkv, total, gridDim.x);
     if (sms < 1) sms = gridDim.x;
   }
   const int n_blocks = min(sms, max(1, total / (PG_WARPS * PG_MIN_UNITS))), n_shares = n_blocks * PG_WARPS;
@@ -236,29 +232,33 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     PgPlace p;
     p.i = lo;
     p.units = sm.units[lo];
-    const int r = x - sm.cum[lo], item = r / p.units, nb = (sm.n_new[lo] * a.G + COLS - 1) / COLS;
-    p.u0 = r - item * p.units;
-    p.u1 = min(p.units, p.u0 + i_hi - x);
+    const int all = p.units + PG_SETUP, r = x - sm.cum[lo], item = r / all, nb = (sm.n_new[lo] * a.G + COLS - 1) / COLS, at = r - item * all;
+    p.places = min(all - at, i_hi - x);
+    p.u0 = max(at - PG_SETUP, 0);
+    p.u1 = max(at + p.places - PG_SETUP, 0);   // (none where the share has the item's first places only)
     p.g = item / nb;
     p.b = item - p.g * nb;
-    p.base = x - p.u0;
+    p.base = x - at + PG_SETUP;
     return p;
   };
 
   unsigned char* const ring = rings + warp * PG_RING;
   uint64_t* const full = sm.full[warp];
   // ---- copies: page numbers come 32 at a time, a batch ahead -----------------------------------------------------------------
-  int ask_x = i_lo, ask_st = 0;                // the next unit to ask for, and its stage
+  int ask_x = i_lo, ask_n = 0, ask_st = 0;     // the next item to ask for; units asked for, and the next one's stage
   PgPlace ask = {};
   int ask_u = 0, batch_p = 0;                  // its number in the item; the first page of the batch at hand
   int page = 0, logical = 0, page_next = 0, logical_next = 0;
   int key0s[PG_STAGES];                        // a stage's first key; below 0: its page is not there
   auto ask_next = [&]() {
-    if (ask_x >= i_hi) return;
     int batches = 0;                           // to ask for: two for another item
     if (ask_u == ask.u1) {
-      ask = place_of(ask_x);
-      ask_u = ask.u0;
+      do {
+        if (ask_x >= i_hi) return;
+        ask = place_of(ask_x);
+        ask_x += ask.places;
+        ask_u = ask.u0;
+      } while (ask.u1 == ask.u0);
       batch_p = ask_u / UPP;
       batches = 2;
     } else if (ask_u / UPP - batch_p == 32) {
@@ -294,7 +294,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
     if (++ask_st == PG_STAGES) ask_st = 0;
     ++ask_u;
-    ++ask_x;
+    ++ask_n;
   };
 #pragma unroll 1
   for (int s = 0; s < PG_STAGES; ++s) ask_next();
@@ -323,9 +323,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   for (bool begun = false;; begun = true) {
     // the next item's queries on their way, then the sums of the one that is done
     const PgPlace done = p;
-    const bool more = x < i_hi;
-    if (more) {
+    bool more = false;
+    while (!more && x < i_hi) {
       p = place_of(x);
+      x += p.places;
+      more = p.u1 > p.u0;
+    }
+    if (more) {
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
         const int c = min(p.b * COLS + 8 * nc + gl, sm.n_new[p.i] * a.G - 1), tok = c / a.G;
@@ -545,13 +549,11 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       if (ok) ask_next();
       if (++st == PG_STAGES) { st = 0; phase ^= 1; }
     }
-    x += p.u1 - p.u0;
   }
   if (!ok) {                                   // what was asked for must land before the block's shared memory goes away
     if (lane == 0) atomicExch(&g_pg_error, 1);
-    const int asked = ask_x - i_lo;
 #pragma unroll 1
-    for (int u = max(0, asked - PG_STAGES); u < asked; ++u) pg_wait(full + u % PG_STAGES, (u / PG_STAGES) & 1);
+    for (int u = max(0, ask_n - PG_STAGES); u < ask_n; ++u) pg_wait(full + u % PG_STAGES, (u / PG_STAGES) & 1);
   }
   if (have_first) {
     Part& part = reinterpret_cast<Part*>(ring)[0];
@@ -738,7 +740,7 @@ static int pg_cols(int max_new, int G) { return (int64_t)max_new * G <= 8 ? 8 : 
 // As many rows a launch as have fewer than 2^31 units together.
 static int pg_window(const PgArgs& a, int hd, int max_new, bool list) {
   const int cols = pg_cols(max_new, a.G);
-  const int64_t queries = a.many ? PS_MANY : (int64_t)max_new * a.G, row = (int64_t)(list ? a.count : a.bt_width) * (hd / 64) * a.nkv * ((queries + cols - 1) / cols);
+  const int64_t queries = a.many ? PS_MANY : (int64_t)max_new * a.G, row = ((int64_t)(list ? a.count : a.bt_width) * (hd / 32) + PG_SETUP) * a.nkv * ((queries + cols - 1) / cols);
   return (int)std::min<int64_t>(PG_WINDOW, INT32_MAX / row);
 }
 template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, const CUtensorMap& map_v, int hd, int max_new, int sms, const char* what, cudaStream_t stream) {
@@ -771,7 +773,7 @@ static int pg_check(const char* what, const void* q, int64_t q_stride, const voi
     set_error("%s: q, its rows, out and the pools must be 16-byte aligned", what);
     return ERR_ALIGNMENT;
   }
-  const int box = hd == 64 ? 64 : 32;
+  const int box = hd == 64 ? 32 : 16;
   int rc = tc5::make_map_k64(map_k, k_pool, n_pages * nkv * PG_PAGE, hd, box, what);
   return rc ? rc : tc5::make_map_k64(map_v, v_pool, n_pages * nkv * PG_PAGE, hd, box, what);
 }

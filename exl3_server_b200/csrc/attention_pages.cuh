@@ -55,18 +55,21 @@ constexpr int PS_MANY = 64;                    // queries of a row and key/value
 constexpr int PS_MIN_PAGES = 4;                // places of a share, at least: every part more is joined again
 constexpr int PS_SETUP = 4;                    // places of the list that a tile has beside its pages': what its queries' way in and its sums' way out cost, in pages
 
+// The rows' own pages, and chosen pages, are walked in units of 8 KB; an item of that work (the queries that walk the same pages) has as many places in its list beside its units', for
+// its queries' way in and its sums' way out.
+constexpr int PG_SETUP = 3;
+
 // Both kernels run side by side where there is work for both: the tensor cores' takes some of the SMs and leaves the others to the walk, whose streams of pages fill the memory's queue
 // from fewer SMs than there are (a batch of 64 behind 4,096 shared keys, 32 heads of 128 on 8, 30 to 2,000 keys of their own: one after the other 117 us).  Both work out how many, in units of
-// 10 ns of an SM: `tiles` for the tiles' pages (120 for two sets of queries, 60 for one), `walk` for the rows' own units of 16 KB (28, and 100 for an item); and the time that
-// the memory takes for these (16 KB in 2.5 ns).
-__host__ __device__ inline int ps_sms(int64_t tiles, int64_t walk, int64_t units, int sms) {
-  if (tiles == 0 || walk == 0) return sms;
+// 10 ns of an SM: `tiles` for the tiles' pages (120 for two sets of queries, 60 for one), PG_COST for a place of the walk; and the time that the memory takes for these (8 KB in 1.25 ns).
+constexpr int64_t PS_COST_TWO = 120, PS_COST_ONE = 60, PG_COST = 13;
+__host__ __device__ inline int ps_sms(int64_t tiles, int64_t places, int sms) {
+  if (tiles == 0 || places == 0) return sms;
+  const int64_t walk = places * PG_COST, memory = places / 8;
   int64_t n = (tiles * sms + (tiles + walk) / 2) / (tiles + walk);
-  const int64_t memory = units / 4;            // 10 ns
   if (memory > 0 && tiles / memory + 1 < n) n = tiles / memory + 1;
   return (int)(n < 1 ? 1 : n > sms - 1 ? sms - 1 : n);
 }
-constexpr int64_t PS_COST_TWO = 120, PS_COST_ONE = 60, PG_COST_UNIT = 28, PG_COST_ITEM = 100;
 
 // A group's tiles of a key/value head, in the units of ps_sms.
 __device__ inline int64_t ps_cost(int queries, int pages) {

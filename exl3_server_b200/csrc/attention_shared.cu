@@ -46,7 +46,7 @@ struct PsTiles {
   int warp_sum[PS_THREADS / 32];
   int small;                                   // no tile has more than 128 queries
   int sms;                                     // for this kernel
-  unsigned long long units, items, cost;       // of the walk, and the tiles'
+  unsigned long long places, cost;             // of the walk, and the tiles'
   int odd_key[2][3][128];                      // per set, in turns (a warp may be two parts behind another), and feature: the first key whose value is not finite among those that not all of the tile's queries see
   int odd[2][3];
 };
@@ -186,24 +186,23 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   }
   // rows of many tokens: their queries, for now, and what of the shared pages a group's rows see
   const int n_rows = a.many ? a.rows : 0;
-  if (threadIdx.x == 0) t.units = t.items = t.cost = 0;
+  if (threadIdx.x == 0) t.places = t.cost = 0;
   __syncthreads();
-  int64_t units = 0, items = 0;
-  const int ks = a.hd == 64 ? 64 : 32;
+  int64_t places = 0;
+  const int ks = a.hd == 64 ? 32 : 16;
   for (int r = threadIdx.x; r < a.rows; r += PS_THREADS) {
     const int s0 = start_of(r), s1 = start_of(r + 1), j = t.groups.of(r);
     if (j >= 0 && s1 > s0) atomicMin(&t.group_seen[j], pos_of(r));
     if (s1 > s0) {                             // (as the walk does)
       const int blocks = ((s1 - s0) * a.G + a.cols - 1) / a.cols;
-      units += (int64_t)max(1, (min(max(pos_of(r), -most) + s1 - s0, most) + ks - 1) / ks - (j >= 0 ? t.groups.pages[j] : 0) * (PG_PAGE / ks)) * blocks;
-      items += blocks;
+      places += (int64_t)(PG_SETUP + max(1, (min(max(pos_of(r), -most) + s1 - s0, most) + ks - 1) / ks - (j >= 0 ? t.groups.pages[j] : 0) * (PG_PAGE / ks))) * blocks;
     }
     if (r < n_rows) t.row_tile[r] = s1 > s0 && (int64_t)(s1 - s0) * a.G > PS_MANY ? (s1 - s0) * a.G : 0;
   }
   __syncthreads();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) { units += __shfl_xor_sync(0xffffffffu, units, o); items += __shfl_xor_sync(0xffffffffu, items, o); }
-  if ((threadIdx.x & 31) == 0 && items) { atomicAdd(&t.units, (unsigned long long)units); atomicAdd(&t.items, (unsigned long long)items); }
+  for (int o = 16; o > 0; o >>= 1) places += __shfl_xor_sync(0xffffffffu, places, o);
+  if ((threadIdx.x & 31) == 0 && places) atomicAdd(&t.places, (unsigned long long)places);
   for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS)
     if (t.group_tile[j]) atomicAdd(&t.cost, (unsigned long long)ps_cost(t.group_tile[j], t.groups.pages[j]));
   // places: groups, then rows, a thread each, in rounds of the block
@@ -255,7 +254,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
       t.cum[0] = 0;
       t.small = small;
       // (beside rows of many tokens the walk has little to do, and of more rows than a launch of it takes it knows no more than these)
-      t.sms = a.many || a.rows > a.window ? (int)gridDim.x : ps_sms(t.cost * a.nkv, (t.units * PG_COST_UNIT + t.items * PG_COST_ITEM) * a.nkv, t.units * a.nkv, gridDim.x);
+      t.sms = a.many || a.rows > a.window ? (int)gridDim.x : ps_sms(t.cost * a.nkv, t.places * a.nkv, gridDim.x);
       p.n_tiles = n_tiles;
       p.total = (int64_t)run * a.nkv;
       p.blocks = (int)min((int64_t)t.sms, max((int64_t)1, p.total / PS_MIN_PAGES));
