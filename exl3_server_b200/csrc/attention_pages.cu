@@ -97,6 +97,7 @@ template <int V> __device__ inline void pg_load_cg(const float* p, float (&y)[V]
 __device__ inline bool pg_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = tc5::smem_u32(bar);
   uint32_t there = 0;
+#pragma unroll 1
   for (uint32_t i = 0; i < tc5::WAIT_LIMIT && !there; ++i)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -209,6 +210,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   if (threadIdx.x == 0) sm.cum[0] = 0;
   const bool beside = !LIST && a.n_groups > 0 && !a.many && a.rows <= a.window;     // the other kernel leaves this one some of the SMs
   if (beside)
+#pragma unroll 1
     for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32)
       if (sm.groups.pages[j] > 0 && sm.group_queries[j] > 0) atomicAdd(&sm.cost, (unsigned long long)ps_cost(sm.group_queries[j], sm.groups.pages[j]));
   __syncthreads();
@@ -228,6 +230,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   // The item at place x.
   auto place_of = [&](int x) {
     int lo = 0, hi = n_rows - 1;
+#pragma unroll 1
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (sm.cum[mid] <= x) lo = mid; else hi = mid - 1; }
     PgPlace p;
     p.i = lo;
@@ -296,9 +299,6 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     ++ask_u;
     ++ask_n;
   };
-#pragma unroll 1
-  for (int s = 0; s < PG_STAGES; ++s) ask_next();
-
   // ---- computing ------------------------------------------------------------------------------------------------------------
   const uint32_t ring_addr = tc5::smem_u32(ring);
   // ldmatrix: a row at 128 bytes, its 16-byte piece c at c ^ (row & 7)
@@ -319,11 +319,18 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   float* const spill = a.records + ((int64_t)blockIdx.x * PG_WARPS + warp) * (PG_MAX_COLS * HD);   // (where the first part's sums wait meanwhile)
   uint32_t qf[NC][KT][2];                      // the query of column 8 nc + gl as the operand: features 16 k + 2 tl, + 1 and + 8, + 9
   PgPlace p = {};
-  int x = i_lo;
-  for (bool begun = false;; begun = true) {
+  int x = i_lo, u = 0, first_limit = 0, last_limit = 0;
+  int limit[NC][2] = {};                       // the last keys that this thread's two queries of each 8 see: columns 2 tl, 2 tl + 1
+  bool begun = false;
+  // (one loop for the first copies, the items and their units: the code of each stands here once)
+#pragma unroll 1
+  for (int step = -PG_STAGES;; ++step) {
+    if (step >= 0) {
+    if (u == p.u1) {
     // the next item's queries on their way, then the sums of the one that is done
     const PgPlace done = p;
     bool more = false;
+#pragma unroll 1
     while (!more && x < i_hi) {
       p = place_of(x);
       x += p.places;
@@ -409,8 +416,8 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
     if (!more) break;
     // ---- the item's units ---------------------------------------------------------------------------------------------------------------
+    begun = true;
     const int n_new = sm.n_new[p.i], pos0 = sm.pos[p.i], col0 = p.b * COLS;
-    int limit[NC][2];                          // the last keys that this thread's two queries of each 8 see: columns 2 tl, 2 tl + 1
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
@@ -419,14 +426,16 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         m[nc][e] = PG_NEG;
         l[nc][e] = 0.0f;
       }
-    const int first_limit = pos0 + col0 / a.G, last_limit = pos0 + min(col0 + COLS - 1, n_new * a.G - 1) / a.G;
+    first_limit = pos0 + col0 / a.G;
+    last_limit = pos0 + min(col0 + COLS - 1, n_new * a.G - 1) / a.G;
 #pragma unroll
     for (int i = 0; i < KT; ++i)
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) o[i][nc][0] = o[i][nc][1] = o[i][nc][2] = o[i][nc][3] = 0.0f;
     odd = false;
-#pragma unroll 1
-    for (int u = p.u0; u < p.u1; ++u) {
+    u = p.u0;
+    }
+    {
       if (ok) ok = pg_wait(full + st, phase);
       int key0 = key0s[0];
 #pragma unroll
@@ -546,9 +555,11 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
       }
       __syncwarp();                            // all lanes have read the stage
-      if (ok) ask_next();
+      ++u;
       if (++st == PG_STAGES) { st = 0; phase ^= 1; }
     }
+    }
+    if (ok) ask_next();
   }
   if (!ok) {                                   // what was asked for must land before the block's shared memory goes away
     if (lane == 0) atomicExch(&g_pg_error, 1);
@@ -841,8 +852,9 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, rows, T, nh, nkv, scale, scratch);
   a.row_start = row_start; a.row_pos0 = row_pos0; a.bt_rows = rows; a.groups = groups; a.n_groups = n_groups;
   const int64_t tiles = ps_tiles_of(T, a.G, rows, n_groups, max_new);
-  if (tiles > PS_MAX_TILES) {
-    set_error("attn_shared: %d tokens of %d query heads a key/value head are more than %d tiles of %d queries with %d groups: in one call at most that", T, a.G, PS_MAX_TILES, PS_TILE, n_groups);
+  if (tiles > PS_MAX_TILES || tiles * (bt_width + PS_SETUP) * nkv > INT32_MAX) {
+    set_error("attn_shared: %d tokens of %d query heads a key/value head with %d groups are more than %d tiles of %d queries, or tables of %d pages too wide for them", T, a.G, n_groups,
+              PS_MAX_TILES, PS_TILE, bt_width);
     return ERR_UNSUPPORTED;
   }
   a.tiles = tiles > 0;

@@ -18,12 +18,14 @@ struct PgGroups {                              // in shared memory
   __device__ int of(int row) const {
     if (n == 0) return -1;
     int lo = 0, hi = n - 1;
+#pragma unroll 1
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (first[mid] <= row) lo = mid; else hi = mid - 1; }
     return row >= first[lo] && row < first[lo] + rows[lo] && pages[lo] > 0 ? lo : -1;
   }
 };
 // By all threads of a block; ends with a barrier.
 __device__ inline void pg_groups(PgGroups& g, const int* __restrict__ list, int n, int rows, int bt_width) {
+#pragma unroll 1
   for (int j = threadIdx.x; j < n; j += blockDim.x) {
     g.first[j] = __ldcg(list + 3 * j);
     g.rows[j] = __ldcg(list + 3 * j + 1);
@@ -32,6 +34,7 @@ __device__ inline void pg_groups(PgGroups& g, const int* __restrict__ list, int 
   __syncthreads();
   if (threadIdx.x == 0) {
     int end = 0;
+#pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int first = g.first[j];
       const bool apart = first >= end && first < rows;
@@ -61,8 +64,8 @@ constexpr int PG_SETUP = 3;
 
 // Both kernels run side by side where there is work for both: the tensor cores' takes some of the SMs and leaves the others to the walk, whose streams of pages fill the memory's queue
 // from fewer SMs than there are (a batch of 64 behind 4,096 shared keys, 32 heads of 128 on 8, 30 to 2,000 keys of their own: one after the other 117 us).  Both work out how many, in units of
-// 10 ns of an SM: `tiles` for the tiles' pages (120 for two sets of queries, 60 for one), PG_COST for a place of the walk; and the time that the memory takes for these (8 KB in 1.25 ns).
-constexpr int64_t PS_COST_TWO = 120, PS_COST_ONE = 60, PG_COST = 13;
+// 10 ns of an SM: `tiles` for the tiles' pages (180 for two sets of queries, 60 for one), PG_COST for a place of the walk; and the time that the memory takes for these (8 KB in 1.25 ns).
+constexpr int64_t PS_COST_TWO = 180, PS_COST_ONE = 60, PG_COST = 16;
 __host__ __device__ inline int ps_sms(int64_t tiles, int64_t places, int sms) {
   if (tiles == 0 || places == 0) return sms;
   const int64_t walk = places * PG_COST, memory = places / 8;
@@ -79,10 +82,10 @@ __device__ inline int64_t ps_cost(int queries, int pages) {
 struct PsPlan {                                // the head of the list
   int n_tiles;
   int blocks;                                  // shares
-  int64_t total, per, rem;                     // places of the list; a share has `per` of them, the first `rem` shares one more
-  __device__ int64_t begin(int block) const { return per * block + min((int64_t)block, rem); }
+  int total, per, rem;                         // places of the list; a share has `per` of them, the first `rem` shares one more
+  __device__ int begin(int block) const { return per * block + min(block, rem); }
   // the share that holds place x
-  __device__ int block_of(int64_t x) const { return x < rem * (per + 1) ? (int)(x / (per + 1)) : (int)(rem + (x - rem * (per + 1)) / per); }
+  __device__ int block_of(int x) const { return x < rem * (per + 1) ? x / (per + 1) : rem + (x - rem * (per + 1)) / per; }
 };
 // What the join needs of a token: its group's tiles and its row's own, each as the first tile's number (-1: none) and the token that this begins with.
 struct PsToken { int shared_tile, shared_tok, own_tile, own_tok; };

@@ -104,6 +104,7 @@ __device__ inline float ps_max3(float a, float b, float c) {
 __device__ inline bool ps_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
   uint32_t there = 0;
+#pragma unroll 1
   for (uint32_t i = 0; i < WAIT_LIMIT && !there; ++i)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -173,11 +174,13 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   auto start_of = [&](int r) { return held ? t.start[r] : min(max(__ldcg(a.row_start + r), 0), a.T); };
   auto pos_of = [&](int r) { return held ? t.pos[r] : min(__ldcg(a.row_pos0 + r), most); };
   if (held)
+#pragma unroll 1
     for (int r = threadIdx.x; r <= a.rows; r += PS_THREADS) {
       t.start[r] = min(max(__ldcg(a.row_start + r), 0), a.T);
       if (r < a.rows) t.pos[r] = min(__ldcg(a.row_pos0 + r), most);
     }
   pg_groups(t.groups, a.groups, a.n_groups, a.rows, a.bt_width);
+#pragma unroll 1
   for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS) {
     const int r0 = t.groups.first[j], s0 = start_of(r0), s1 = max(start_of(r0 + t.groups.rows[j]), s0);
     t.group_tok[j] = s0;
@@ -190,6 +193,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   __syncthreads();
   int64_t places = 0;
   const int ks = a.hd == 64 ? 32 : 16;
+#pragma unroll 1
   for (int r = threadIdx.x; r < a.rows; r += PS_THREADS) {
     const int s0 = start_of(r), s1 = start_of(r + 1), j = t.groups.of(r);
     if (j >= 0 && s1 > s0) atomicMin(&t.group_seen[j], pos_of(r));
@@ -203,10 +207,12 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) places += __shfl_xor_sync(0xffffffffu, places, o);
   if ((threadIdx.x & 31) == 0 && places) atomicAdd(&t.places, (unsigned long long)places);
+#pragma unroll 1
   for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS)
     if (t.group_tile[j]) atomicAdd(&t.cost, (unsigned long long)ps_cost(t.group_tile[j], t.groups.pages[j]));
   // places: groups, then rows, a thread each, in rounds of the block
   int n_tiles = 0, small = 1;
+#pragma unroll 1
   for (int i0 = 0; i0 < a.n_groups + n_rows; i0 += PS_THREADS) {
     const int i = i0 + threadIdx.x;
     const bool group = i < a.n_groups;
@@ -218,11 +224,13 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
     if (lane == 31) t.warp_sum[warp] = incl;
     small &= __syncthreads_and(queries <= 128);
     int at = n_tiles + incl - mine;
+#pragma unroll 1
     for (int w = 0; w < PS_THREADS / 32; ++w) { if (w < warp) at += t.warp_sum[w]; n_tiles += t.warp_sum[w]; }
     if (i < a.n_groups + n_rows) {
       const int row = group ? t.groups.first[i] : i - a.n_groups;
       const int own = group ? -1 : t.groups.of(row), page0 = own >= 0 ? t.groups.pages[own] : 0;
       const int tok0 = group ? t.group_tok[i] : start_of(row), pos0 = group ? 0 : pos_of(row);
+#pragma unroll 1
       for (int k = 0; k < mine && at + k < PS_MAX_TILES; ++k) {
         const int q0 = k * PS_TILE, n = min(PS_TILE, queries - q0), last = pos0 + (q0 + n - 1) / a.G;
         t.tok0[at + k] = tok0;
@@ -241,6 +249,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   n_tiles = min(n_tiles, PS_MAX_TILES);
   if (threadIdx.x < 32) {                      // running sums, a warp
     int run = 0;
+#pragma unroll 1
     for (int i0 = 0; i0 < n_tiles; i0 += 32) {
       const int i = i0 + threadIdx.x;
       int incl = i < n_tiles ? t.cum[i + 1] : 0;
@@ -256,8 +265,8 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
       // (beside rows of many tokens the walk has little to do, and of more rows than a launch of it takes it knows no more than these)
       t.sms = a.many || a.rows > a.window ? (int)gridDim.x : ps_sms(t.cost * a.nkv, t.places * a.nkv, gridDim.x);
       p.n_tiles = n_tiles;
-      p.total = (int64_t)run * a.nkv;
-      p.blocks = (int)min((int64_t)t.sms, max((int64_t)1, p.total / PS_MIN_PAGES));
+      p.total = run * a.nkv;                   // (the host has seen that it stays within 31 bits)
+      p.blocks = min(t.sms, max(1, p.total / PS_MIN_PAGES));
       p.per = p.total / p.blocks;
       p.rem = p.total - p.per * p.blocks;
     }
@@ -266,16 +275,17 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
 }
 // A part of the list that one block works on.
 struct PsPart { int g, tile, p0, p1, places; };          // kv head, tile, pages of the tile (none where a share has the tile's first places only), places of the list
-__device__ inline PsPart ps_part(const PsTiles& t, int64_t x, int64_t end) {
+__device__ inline PsPart ps_part(const PsTiles& t, int x, int end) {
   const int all = t.cum[t.plan.n_tiles];
   PsPart p;
-  p.g = (int)(t.plan.total <= INT32_MAX ? (uint32_t)x / (uint32_t)all : x / all);
-  const int r = (int)(x - (int64_t)p.g * all);
+  p.g = x / all;
+  const int r = x - p.g * all;
   int lo = 0, hi = t.plan.n_tiles - 1;
+#pragma unroll 1
   while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (t.cum[mid] <= r) lo = mid; else hi = mid - 1; }
   p.tile = lo;
   const int at = r - t.cum[lo];
-  p.places = (int)min((int64_t)(t.cum[lo + 1] - r), end - x);
+  p.places = min(t.cum[lo + 1] - r, end - x);
   p.p0 = max(0, at - PS_SETUP);
   p.p1 = max(0, at + p.places - PS_SETUP);
   return p;
@@ -295,9 +305,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) mbar_init(q_full + i, 4);
     mbar_init(&bars.q_free, 1);
+#pragma unroll 1
     for (int i = 0; i < PS_MAX_STAGES; ++i) { mbar_init(kv_full + i, 1); mbar_init(kv_free + i, 1); }
+#pragma unroll 1
     for (int i = 0; i < 4; ++i) { mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(pv_done + i, 1); }
     mbar_init_fence();
   }
@@ -311,7 +324,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   ps_tiles(tiles, a);
   const PsPlan& plan = tiles.plan;
   const uint32_t tmem = bars.tmem_slot;        // columns: scores of set s at 128 s, O at 256 + 128 s
-  const int64_t lo = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x) : 0, hi = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x + 1) : 0;
+  const int lo = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x) : 0, hi = (int)blockIdx.x < plan.blocks ? plan.begin(blockIdx.x + 1) : 0;
   // Tiles of more than 128 queries: both sets take every page, 128 queries each.  Smaller ones: the sets take the pages in turn, with the same queries, and where there
   // are only such tiles one copy of them, which leaves room for more pages: a page's stage is taken for a copy's way and two pages' softmax, and with 4 stages
   // a page took 0.86 us.
@@ -328,7 +341,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     // ---- copies; page numbers come 32 at a time, a batch ahead ------------------------------------------------------------------
     int c = 0, st = 0;
     uint32_t phase = 1;                        // of the stage's being free again
-    for (int64_t x = lo; x < hi && ok;) {
+#pragma unroll 1
+    for (int x = lo; x < hi && ok;) {
       const PsPart t = ps_part(tiles, x, hi);
       const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile];
       const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
@@ -337,8 +351,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         return n < 0 || n > a.n_pages ? a.n_pages : n;
       };
       int page = numbers(t.p0);
+#pragma unroll 1
       for (int p = t.p0; p < t.p1 && ok; p += 32) {
         const int ahead = numbers(p + 32);
+#pragma unroll 1
         for (int i = 0; i < min(32, t.p1 - p); ++i, ++c) {
           const int y = (__shfl_sync(0xffffffffu, page, i) * a.nkv + t.g) * PG_PAGE;
           if (c >= stages && !ps_wait(kv_free + st, phase)) { ok = false; break; }
@@ -359,14 +375,17 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     }
     // what was asked for must land before the block's shared memory goes away
     if (!ok && lane == 0) atomicExch(&g_ps_error, 1);
+#pragma unroll 1
     for (int u = max(0, c - stages); u < c; ++u) ps_wait(kv_full + u % stages, (u / stages) & 1);
   } else if (warp == 8) {
     // ---- S = Q K^T, up to two pages ahead of the softmax -------------------------------------------------------------------
     int st = 0, f[2] = {0, 0}, k[2] = {0, 0};  // pages of a set, parts of a set so far
     uint32_t phase = 0;
-    for (int64_t x = lo; x < hi && ok;) {
+#pragma unroll 1
+    for (int x = lo; x < hi && ok;) {
       const PsPart t = ps_part(tiles, x, hi);
       const bool two = both(t);
+#pragma unroll 1
       for (int p = t.p0; p < t.p1 && ok; ++p) {
         if (!ps_wait(kv_full + st, phase)) { ok = false; break; }
 #pragma unroll
@@ -398,40 +417,48 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     if (!ok && lane == 0) atomicExch(&g_ps_error, 2);
   } else if (warp == 9) {
     // ---- for the join, while the first scores are on their way: the tiles' parts, and every token's tiles -------------------------------
+#pragma unroll 1
     for (int i = blockIdx.x * 32 + lane; i < plan.n_tiles * a.nkv; i += gridDim.x * 32) {
       const int g = i / plan.n_tiles, tile = i - g * plan.n_tiles;
-      const int64_t first = (int64_t)g * tiles.cum[plan.n_tiles] + tiles.cum[tile] + PS_SETUP, last = first + tiles.cum[tile + 1] - tiles.cum[tile] - PS_SETUP - 1;
+      const int first = g * tiles.cum[plan.n_tiles] + tiles.cum[tile] + PS_SETUP, last = first + tiles.cum[tile + 1] - tiles.cum[tile] - PS_SETUP - 1;
       const int b0 = plan.block_of(first), halves = tiles.queries[tile] > 128 ? 1 : 2;
       reinterpret_cast<int4*>(a.parts)[(int64_t)g * a.most_tiles + tile] = make_int4(b0 + i, (plan.block_of(last) - b0 + 1) * halves, halves, 0);
     }
+#pragma unroll 1
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
       const int s0 = min(max(__ldcg(a.row_start + r), 0), a.T), s1 = min(__ldcg(a.row_start + r + 1), a.T), j = tiles.groups.of(r);
       const int4 w = make_int4(j >= 0 ? tiles.group_tile[j] : -1, j >= 0 ? tiles.group_tok[j] : 0, a.many ? tiles.row_tile[r] : -1, s0);       // a PsToken
+#pragma unroll 1
       for (int i = s0 + lane; i < s1; i += 32) reinterpret_cast<int4*>(a.tokens)[i] = w;
     }
     {                                          // (tokens of no row)
       const int t0 = min(max(__ldcg(a.row_start), 0), a.T), t1 = max(t0, min(max(__ldcg(a.row_start + a.rows), 0), a.T));
+#pragma unroll 1
       for (int i = blockIdx.x * 32 + lane; i < t0 + a.T - t1; i += gridDim.x * 32) reinterpret_cast<int4*>(a.tokens)[i < t0 ? i : t1 + i - t0] = make_int4(-1, 0, -1, 0);
     }
     // ---- O += P V ----------------------------------------------------------------------------------------------------------------
     int st = 0, f[2] = {0, 0}, k[2] = {0, 0};
     uint32_t phase = 0;
-    for (int64_t x = lo; x < hi && ok;) {
+#pragma unroll 1
+    for (int x = lo; x < hi && ok;) {
       const PsPart t = ps_part(tiles, x, hi);
       const bool two = both(t);
       const int row = tiles.row[t.tile], q0 = tiles.query0[t.tile];
       // a row's own pages: the last keys that the tile's first and last queries see
       const int own_pos = row < 0 ? min(__ldcg(a.row_pos0 - 1 - row), a.bt_width * PG_PAGE) : 0;
       const int first_limit = row < 0 ? own_pos + q0 / a.G : INT32_MAX, last_limit = own_pos + (q0 + tiles.queries[t.tile] - 1) / a.G;
+#pragma unroll 1
       for (int p = t.p0; p < t.p1 && ok; ++p) {
         const int key0 = (tiles.page0[t.tile] + p) * PG_PAGE;
         if (row < 0 && key0 + PG_PAGE - 1 > first_limit) {
           // Values that not all queries see: a probability of 0 is multiplied with them all the same, so those that are not finite become zeros here, and the softmax
           // threads are told from which key on a feature is not finite (when they are known to have begun the part: they have handed over P).
           if (!ps_wait(kv_full + st, phase)) { ok = false; break; }
+#pragma unroll 1
           for (int s = 0; s < 2; ++s)
             if ((two || ((p - t.p0) & 1) == s) && !ps_wait(p_full + 2 * s + (f[s] & 1), (f[s] >> 1) & 1)) { ok = false; break; }
           if (!ok) break;
+#pragma unroll 1
           for (int w = lane; w < PG_PAGE * (HD / 8); w += 32) {
             const int key = w / (HD / 8), c = w % (HD / 8);
             if (key0 + key <= first_limit) continue;
@@ -445,6 +472,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               if (isfinite(__bfloat162float(each[e]))) continue;
               each[e] = __float2bfloat16(0.0f);
               if (key0 + key > last_limit) continue;
+#pragma unroll 1
               for (int s = 0; s < 2; ++s)
                 if (set < 0 || set == s) { atomicMin(&tiles.odd_key[s][k[s] % 3][8 * c + e], key0 + key); tiles.odd[s][k[s] % 3] = 1; }
             }
@@ -487,13 +515,22 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     // The set's next part from place x on, and its queries on their way into the operand's layout: beside the last sums of the part before.
     // pos: the last key that this query sees; sees: all of the warp's queries see keys up to here; holes: some page of the part is not there.
     struct Mine { PsPart t; bool two, in, holes; int first, qr, pos, sees, turn; int64_t slot; };
-    auto enter = [&](int64_t& x, Mine& m) {
-      for (;;) {
-        if (x >= hi) return false;
+    int x = lo;
+    bool more = true;
+    float m_used = -INFINITY, l = 0.0f;
+    uint32_t s0[32], s1[32];
+    Mine m = {};
+#pragma unroll 1
+    for (bool begun = false;; begun = true) {
+      const Mine now = m;                      // the part whose last sums are on their way
+#pragma unroll 1
+      while (more) {                           // the next one
+        more = x < hi;
+        if (!more) break;
         m.t = ps_part(tiles, x, hi);
         x += m.t.places;
         if (m.t.p1 == m.t.p0) continue;
-        if (one && parts > 0 && !ps_wait(&bars.q_free, (parts - 1) & 1)) { ok = false; return false; }     // (every part's, whether the set has pages of it or not)
+        if (one && parts > 0 && !ps_wait(&bars.q_free, (parts - 1) & 1)) { ok = false; break; }            // (every part's, whether the set has pages of it or not)
         ++parts;
         m.two = both(m.t);
         m.first = m.t.p0 + (m.two ? 0 : s);
@@ -504,56 +541,76 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         rec[m.qr] = -INFINITY;
         rec[PS_TILE + m.qr] = 0.0f;
       }
-      const int in_tile = m.two ? m.qr : r;
-      m.in = in_tile < tiles.queries[m.t.tile];
-      const PsPart& t = m.t;
-      const int query = tiles.query0[t.tile] + (m.in ? in_tile : 0), step_tok = query / a.G, tok = tiles.tok0[t.tile] + step_tok;
-      m.turn = mine++ % 3;
-      // the warp's 32 queries, rows of the operand (the last S that read the place is done): several of them an instruction, 16 bytes a lane
-      constexpr int LANES = HD / 8, EACH = 32 / LANES;
-      const int64_t from = m.in ? (int64_t)tok * a.q_stride + (int64_t)(t.g * a.G + query - step_tok * a.G) * HD : -1;
-      uint4 w[LANES];
+      if (!ok) break;
+      if (more) {
+        const int in_tile = m.two ? m.qr : r;
+        m.in = in_tile < tiles.queries[m.t.tile];
+        const PsPart& t = m.t;
+        const int query = tiles.query0[t.tile] + (m.in ? in_tile : 0), step_tok = query / a.G, tok = tiles.tok0[t.tile] + step_tok;
+        m.turn = mine++ % 3;
+        // the warp's 32 queries, rows of the operand (the last S that read the place is done): several of them an instruction, 16 bytes a lane
+        constexpr int LANES = HD / 8, EACH = 32 / LANES;
+        const int64_t from = m.in ? (int64_t)tok * a.q_stride + (int64_t)(t.g * a.G + query - step_tok * a.G) * HD : -1;
+        uint4 w[LANES];
 #pragma unroll
-      for (int i = 0; i < LANES; ++i) {
-        const int64_t at = __shfl_sync(0xffffffffu, from, EACH * i + lane / LANES);
-        w[i] = at >= 0 ? __ldcg(reinterpret_cast<const uint4*>(a.q + at) + lane % LANES) : make_uint4(0, 0, 0, 0);
-      }
-      const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile], most = a.bt_width * PG_PAGE;
-      const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
-      bool holes = false;
-      for (int p = t.p0 + lane; p < t.p1; p += 32) { const int page = p_off + p < a.bt_width ? __ldcg(bt + p) : -1; holes |= page < 0 || page >= a.n_pages; }
-      m.pos = INT32_MAX;                       // (shared pages, seen by all as a rule)
-      if (row < 0) {
-        m.pos = (a.rows <= PS_MAX_ROWS ? tiles.pos[-1 - row] : min(__ldcg(a.row_pos0 - 1 - row), most)) + step_tok;
-      } else if (tiles.group_seen[tiles.groups.of(row)] < (p_off + t.p1) * PG_PAGE - 1) {
-        int row_lo = row, row_hi = row + tiles.groups.rows[tiles.groups.of(row)] - 1;
-        while (row_lo < row_hi) { const int mid = (row_lo + row_hi + 1) >> 1; if (__ldcg(a.row_start + mid) <= tok) row_lo = mid; else row_hi = mid - 1; }
-        m.pos = min(__ldcg(a.row_pos0 + row_lo), most) + tok - __ldcg(a.row_start + row_lo);
-      }
-      if (r < 32) for (int d = r; d < HD; d += 32) tiles.odd_key[s][m.turn][d] = INT32_MAX;
-      if (r == 0) tiles.odd[s][m.turn] = 0;
+        for (int i = 0; i < LANES; ++i) {
+          const int64_t at = __shfl_sync(0xffffffffu, from, EACH * i + lane / LANES);
+          w[i] = at >= 0 ? __ldcg(reinterpret_cast<const uint4*>(a.q + at) + lane % LANES) : make_uint4(0, 0, 0, 0);
+        }
+        const int row = tiles.row[t.tile], p_off = tiles.page0[t.tile], most = a.bt_width * PG_PAGE;
+        const int* bt = a.block_table + (int64_t)(row < 0 ? -1 - row : row) * a.bt_stride + p_off;
+        bool holes = false;
+#pragma unroll 1
+        for (int p = t.p0 + lane; p < t.p1; p += 32) { const int page = p_off + p < a.bt_width ? __ldcg(bt + p) : -1; holes |= page < 0 || page >= a.n_pages; }
+        m.pos = INT32_MAX;                       // (shared pages, seen by all as a rule)
+        if (row < 0) {
+          m.pos = (a.rows <= PS_MAX_ROWS ? tiles.pos[-1 - row] : min(__ldcg(a.row_pos0 - 1 - row), most)) + step_tok;
+        } else if (tiles.group_seen[tiles.groups.of(row)] < (p_off + t.p1) * PG_PAGE - 1) {
+          int row_lo = row, row_hi = row + tiles.groups.rows[tiles.groups.of(row)] - 1;
+#pragma unroll 1
+          while (row_lo < row_hi) { const int mid = (row_lo + row_hi + 1) >> 1; if (__ldcg(a.row_start + mid) <= tok) row_lo = mid; else row_hi = mid - 1; }
+          m.pos = min(__ldcg(a.row_pos0 + row_lo), most) + tok - __ldcg(a.row_start + row_lo);
+        }
+        if (r < 32) for (int d = r; d < HD; d += 32) tiles.odd_key[s][m.turn][d] = INT32_MAX;
+        if (r == 0) tiles.odd[s][m.turn] = 0;
 #pragma unroll
-      for (int i = 0; i < LANES; ++i) {
-        const int c = lane % LANES, rr = (warp & 3) * 32 + EACH * i + lane / LANES;
-        *reinterpret_cast<uint4*>(sQ + s * second_q + (c >> 3) * 128 * 128 + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = w[i];
+        for (int i = 0; i < LANES; ++i) {
+          const int c = lane % LANES, rr = (warp & 3) * 32 + EACH * i + lane / LANES;
+          *reinterpret_cast<uint4*>(sQ + s * second_q + (c >> 3) * 128 * 128 + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = w[i];
+        }
+        m.holes = __any_sync(0xffffffffu, holes);
+        m.sees = __reduce_min_sync(0xffffffffu, m.pos);
+        fence_smem_to_tma();
+        ps_arrive_warp(q_full + s);
       }
-      m.holes = __any_sync(0xffffffffu, holes);
-      m.sees = __reduce_min_sync(0xffffffffu, m.pos);
-      fence_smem_to_tma();
-      ps_arrive_warp(q_full + s);
-      return true;
-    };
-    int64_t x = lo;
-    Mine now;
-    bool more = enter(x, now);
-    while (more && ok) {
-      const PsPart t = now.t;
-      const bool in = now.in;
-      const bool holes = now.holes;
-      const int step = now.two ? 1 : 2, first = now.first, qr = now.qr, turn = now.turn, pos = now.pos, sees = now.sees, p_off = tiles.page0[t.tile];
-      float* const rec = a.records + now.slot * ps_record(HD);
-      float m_used = -INFINITY, l = 0.0f;
-      uint32_t s0[32], s1[32];
+      if (begun) {
+        ok = ps_wait(pv_done + 2 * s + ((f - 1) & 1), ((f - 1) >> 1) & 1);
+        if (!ok) break;
+        fence_after();
+        float* const rec = a.records + now.slot * ps_record(HD), *const sums = rec + 2 * PS_TILE + (int64_t)now.qr * HD;
+        if (now.in) { rec[now.qr] = m_used; rec[PS_TILE + now.qr] = l; }
+#pragma unroll 1
+        for (int h = 0; h < HD / 32; ++h) {
+          __syncwarp();
+          tmem_ld32(to + 32 * h, s0);
+          if (now.in) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) ps_store8(sums + 32 * h + c, s0 + c);
+          }
+        }
+        if (tiles.odd[s][now.turn] != 0 && now.in)           // (written before the product that has ended)
+#pragma unroll 1
+          for (int d = 0; d < HD; ++d)
+            if (tiles.odd_key[s][now.turn][d] <= now.pos) sums[d] = __int_as_float(0x7fc00000);
+        __syncwarp();
+        fence_before();                        // O is read: the next part's first product may write it
+      }
+      if (!more) break;
+      const PsPart t = m.t;
+      const bool holes = m.holes;
+      const int step = m.two ? 1 : 2, first = m.first, pos = m.pos, sees = m.sees, p_off = tiles.page0[t.tile];
+      m_used = -INFINITY;
+      l = 0.0f;
       auto ask = [&](int f) {                  // the scores of the set's page f: on their way
         if (!ps_wait(s_full + 2 * s + (f & 1), (f >> 1) & 1)) return false;
         fence_after();
@@ -562,6 +619,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         return true;
       };
       ok = ask(f);
+#pragma unroll 1
       for (int p = first; p < t.p1 && ok; p += step, ++f) {
         const int sb = f & 1;
         tmem_ld_wait(s0);
@@ -608,29 +666,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         ps_arrive_warp(p_full + 2 * s + sb);
       }
       if (!ok) break;
-      more = enter(x, now);
-      if (!ok) break;
-      ok = ps_wait(pv_done + 2 * s + ((f - 1) & 1), ((f - 1) >> 1) & 1);
-      if (!ok) break;
-      fence_after();
-      if (in) { rec[qr] = m_used; rec[PS_TILE + qr] = l; }
-      const bool odd = tiles.odd[s][turn] != 0;          // (written before the product that has ended)
-#pragma unroll
-      for (int h = 0; h < HD / 32; ++h) {
-        __syncwarp();
-        tmem_ld32(to + 32 * h, s0);
-        if (odd) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (tiles.odd_key[s][turn][32 * h + c] <= pos) s0[c] = 0x7fc00000u;
-        }
-        if (in) {
-#pragma unroll
-          for (int c = 0; c < 32; c += 8) ps_store8(rec + 2 * PS_TILE + (int64_t)qr * HD + 32 * h + c, s0 + c);
-        }
-      }
-      __syncwarp();
-      fence_before();                          // O is read: the next part's first product may write it
     }
     if (!ok) asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");         // a row of scores may still be on its way
     if (!ok && lane == 0) atomicExch(&g_ps_error, 4);
@@ -688,6 +723,7 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
     return (second ? s1.at : s0.at) + (halves == 2 ? k >> 1 : k) * ps_record(HD);
   };
   float mm = -INFINITY, l = 0.0f;
+#pragma unroll 1
   for (int i = lane; i < n; i += 32) {
     int row = 0;
     const float* p = i < n01 ? part(i, row) : mine;
@@ -701,6 +737,7 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
   if (SPLIT > 1) __syncthreads(); else __syncwarp();
   float y[V] = {};
   constexpr int BATCH = 8;
+#pragma unroll 1
   for (int i0 = w0; i0 < n; i0 += SPLIT * BATCH) {
     float v[BATCH][V], f[BATCH];
 #pragma unroll

@@ -120,7 +120,7 @@ __global__ void page_bounds_load_kernel(const int8_t* __restrict__ codes, const 
 
 // ---- the choice -----------------------------------------------------------------------------------------------------------------
 
-constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32;
+constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_BLOCKS = 4;          // (of an SM, at least)
 constexpr int SEL_MAX_HEADS = 128;             // query heads of a key/value head
 constexpr int SEL_MAX_PAGES = 32768;           // pages of a row
 
@@ -153,9 +153,9 @@ struct SelArgs {
 
 // A cluster of blocks (one for many items) for each (token, kv head): each scores a stretch of the row's pages and puts the scores into the first one's shared memory, which
 // chooses.  Pages are the rows of the matrix instruction, query heads its columns.  A lane's 16 bytes of a page's codes are four of the instruction's operand words; the
-// query's codes are laid out alike, so that the order of features within the product is the memory's.  A warp's page numbers are asked for two steps ahead, codes one.
+// query's codes are laid out alike, so that the order of features within the product is the memory's.  A warp's page numbers are asked for a step ahead.
 template <int HD>
-__global__ void __launch_bounds__(SEL_THREADS)
+__global__ void __launch_bounds__(SEL_THREADS, SEL_BLOCKS)
 page_select_kernel(const SelArgs a) {
   constexpr int L = 2 * HD / 64;                 // 16-byte pieces a lane has of a page
   extern __shared__ uint4 sel_raw[];
@@ -200,7 +200,7 @@ page_select_kernel(const SelArgs a) {
     return c;
   };
   int p0 = p_lo + warp * 16;
-  Pages n0 = numbers(p0), n1 = numbers(p0 + STEP);
+  Pages n0 = numbers(p0);
 
   for (int h = warp; h < 8 * ng; h += SEL_WARPS) {
     float x[HD / 32], m = 0.0f;
@@ -223,15 +223,14 @@ page_select_kernel(const SelArgs a) {
     }
     if (lane == 0) s_scale[h] = h < a.G ? __fdiv_rn(m, 127.0f) : -1.0f;
   }
-  Codes now = codes(n0);
   if (C > 1) tc5::cluster_wait_all();
   __syncthreads();
 
   // ---- scores ------------------------------------------------------------------------------------------------------------------
   const uint32_t keys = C > 1 ? tc5::cluster_addr(s_key, 0) : tc5::smem_u32(s_key);
   for (; p0 < p_hi; p0 += STEP) {
-    const Codes next = codes(n1);                // (past the end: page 0's, not used)
-    const Pages n2 = numbers(p0 + 2 * STEP);
+    const Codes now = codes(n0);
+    const Pages n1 = numbers(p0 + STEP);
     float best[2] = {-INFINITY, -INFINITY};
     __syncwarp();
     for (int n = 0; n < ng; ++n) {
@@ -259,9 +258,7 @@ page_select_kernel(const SelArgs a) {
         else s_key[p] = key;
       }
     }
-    now = next;
     n0 = n1;
-    n1 = n2;
   }
   if (C > 1) {
     tc5::cluster_sync_all();
