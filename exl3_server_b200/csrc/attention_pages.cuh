@@ -56,7 +56,7 @@ constexpr int PS_MAX_TILES = 512;              // of a key/value head
 constexpr int PS_MAX_ROWS = 1024;              // rows up to which rows of many tokens have tiles of their own
 constexpr int PS_MANY = 64;                    // queries of a row and key/value head from which its own pages are the tensor cores' work
 constexpr int PS_MIN_PAGES = 4;                // places of a share, at least: every part more is joined again
-constexpr int PS_SETUP = 4;                    // places of the list that a tile has beside its pages': what its queries' way in and its sums' way out cost, in pages
+constexpr int PS_SETUP = 6;                    // places of the list that a tile has beside its pages': what its queries' way in and its sums' way out cost, in pages
 
 // The rows' own pages, and chosen pages, are walked in units of 8 KB; an item of that work (the queries that walk the same pages) has as many places in its list beside its units', for
 // its queries' way in and its sums' way out.

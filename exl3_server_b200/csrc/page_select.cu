@@ -120,7 +120,8 @@ __global__ void page_bounds_load_kernel(const int8_t* __restrict__ codes, const 
 
 // ---- the choice -----------------------------------------------------------------------------------------------------------------
 
-constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32, SEL_BLOCKS = 4;          // (of an SM, at least)
+constexpr int SEL_THREADS = 256, SEL_WARPS = SEL_THREADS / 32;
+constexpr int SEL_LANE = 16;                   // keys of a lane where one warp searches
 constexpr int SEL_MAX_HEADS = 128;             // query heads of a key/value head
 constexpr int SEL_MAX_PAGES = 32768;           // pages of a row
 
@@ -153,9 +154,9 @@ struct SelArgs {
 
 // A cluster of blocks (one for many items) for each (token, kv head): each scores a stretch of the row's pages and puts the scores into the first one's shared memory, which
 // chooses.  Pages are the rows of the matrix instruction, query heads its columns.  A lane's 16 bytes of a page's codes are four of the instruction's operand words; the
-// query's codes are laid out alike, so that the order of features within the product is the memory's.  A warp's page numbers are asked for a step ahead.
+// query's codes are laid out alike, so that the order of features within the product is the memory's.  A warp's page numbers are asked for two steps ahead, codes one.
 template <int HD>
-__global__ void __launch_bounds__(SEL_THREADS, SEL_BLOCKS)
+__global__ void __launch_bounds__(SEL_THREADS)
 page_select_kernel(const SelArgs a) {
   constexpr int L = 2 * HD / 64;                 // 16-byte pieces a lane has of a page
   extern __shared__ uint4 sel_raw[];
@@ -165,6 +166,7 @@ page_select_kernel(const SelArgs a) {
   uint32_t* s_key = reinterpret_cast<uint32_t*>(s_scale + ng * 8);            // [pages of the row]
   __shared__ int4 s_count[2][SEL_WARPS];
   __shared__ int s_base[SEL_WARPS], s_equal[SEL_WARPS];
+  __shared__ int3 s_found;                       // the bound, how many of the keys at it are taken, and how many pages in all
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, tl = lane & 3;
   const int C = a.cluster, rank = C > 1 ? (int)tc5::cluster_rank() : 0, item = blockIdx.x / C;
   const int t = item / a.nkv, g = item - t * a.nkv;
@@ -200,7 +202,7 @@ page_select_kernel(const SelArgs a) {
     return c;
   };
   int p0 = p_lo + warp * 16;
-  Pages n0 = numbers(p0);
+  Pages n0 = numbers(p0), n1 = numbers(p0 + STEP);
 
   for (int h = warp; h < 8 * ng; h += SEL_WARPS) {
     float x[HD / 32], m = 0.0f;
@@ -223,14 +225,15 @@ page_select_kernel(const SelArgs a) {
     }
     if (lane == 0) s_scale[h] = h < a.G ? __fdiv_rn(m, 127.0f) : -1.0f;
   }
+  Codes now = codes(n0);
   if (C > 1) tc5::cluster_wait_all();
   __syncthreads();
 
   // ---- scores ------------------------------------------------------------------------------------------------------------------
   const uint32_t keys = C > 1 ? tc5::cluster_addr(s_key, 0) : tc5::smem_u32(s_key);
   for (; p0 < p_hi; p0 += STEP) {
-    const Codes now = codes(n0);
-    const Pages n1 = numbers(p0 + STEP);
+    const Codes next = codes(n1);                // (past the end: page 0's, not used)
+    const Pages n2 = numbers(p0 + 2 * STEP);
     float best[2] = {-INFINITY, -INFINITY};
     __syncwarp();
     for (int n = 0; n < ng; ++n) {
@@ -258,7 +261,9 @@ page_select_kernel(const SelArgs a) {
         else s_key[p] = key;
       }
     }
+    now = next;
     n0 = n1;
+    n1 = n2;
   }
   if (C > 1) {
     tc5::cluster_sync_all();
@@ -267,41 +272,78 @@ page_select_kernel(const SelArgs a) {
     __syncthreads();
   }
 
-  // ---- the k-th largest place: the largest bound that k keys reach, two bits at a time -----------------------------------------------
-  int turn = 0;
-  auto reach = [&](uint32_t b1, uint32_t b2, uint32_t b3) {            // keys of at least each bound (at most 32,768: two to a word)
-    int n12 = 0, n3 = 0;
-    for (int p = threadIdx.x; p < there; p += SEL_THREADS) {
-      const uint32_t key = s_key[p];
-      n12 += (key >= b1) + ((key >= b2) << 16);
-      n3 += key >= b3;
-    }
-    n12 = __reduce_add_sync(0xffffffffu, n12);   // (a warp has 4,096 of them at most)
-    n3 = __reduce_add_sync(0xffffffffu, n3);
-    if (lane == 0) s_count[turn][warp] = make_int4(n12 & 0xffff, n12 >> 16, n3, 0);
-    __syncthreads();
-    int4 n = s_count[turn][0];
-#pragma unroll
-    for (int i = 1; i < SEL_WARPS; ++i) { const int4 m = s_count[turn][i]; n.x += m.x; n.y += m.y; n.z += m.z; }
-    turn ^= 1;
-    return n;
-  };
-  const int held = reach(1u, 1u, 1u).x, k = min(a.count, held);
-  uint32_t bound = 0u;
-  int want = 0;                                  // of the keys at the bound
-  if (k < held) {
+  // ---- the k-th largest place: the largest bound that k keys reach, two bits at a time.  counts(b1, b2, b3): keys of at least each bound -----------------------------
+  auto search = [&](auto counts, int held, int k, uint32_t& bound, int& want) {
+    bound = 0u;
+    want = 0;                                    // of the keys at the bound
+    if (k >= held) return;                       // (all that are there)
     int at_least = held;                         // keys that reach the bound
+#pragma unroll 1
     for (int bit = 30; bit >= 0 && at_least > k; bit -= 2) {
       const uint32_t b1 = bound | 1u << bit, b2 = bound | 2u << bit, b3 = bound | 3u << bit;
-      const int4 n = reach(b1, b2, b3);
+      const int3 n = counts(b1, b2, b3);
       if (n.z >= k) { bound = b3; at_least = n.z; }
       else if (n.y >= k) { bound = b2; at_least = n.y; }
       else if (n.x >= k) { bound = b1; at_least = n.x; }
     }
-    if (at_least == k) bound -= 1;               // all that reach it, and none below
-    else want = k - reach(bound + 1, bound + 1, bound + 1).x;          // (more than k reach the highest place: only if all of them must be chosen)
-    if (at_least != k && bound == 0xffffffffu) want = k;
+    if (at_least == k) { bound -= 1; return; }   // all that reach it, and none below
+    want = bound == 0xffffffffu ? k : k - counts(bound + 1, bound + 1, bound + 1).x;   // (more than k reach the highest place: only if all of them must be chosen)
+  };
+  if (there <= 32 * SEL_LANE) {
+    // few pages: one warp, their keys in registers, no barrier a step (470 pages: 4.4 us -> 1)
+    if (warp == 0) {
+      uint32_t key[SEL_LANE];
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < SEL_LANE; ++i) {
+        key[i] = 32 * i + lane < there ? s_key[32 * i + lane] : 0u;
+        n += key[i] > 0u;
+      }
+      n = __reduce_add_sync(0xffffffffu, n);
+      uint32_t b;
+      int w;
+      search([&](uint32_t b1, uint32_t b2, uint32_t b3) {
+        int n12 = 0, n3 = 0;
+#pragma unroll
+        for (int i = 0; i < SEL_LANE; ++i) {
+          n12 += (key[i] >= b1) + ((key[i] >= b2) << 16);
+          n3 += key[i] >= b3;
+        }
+        n12 = __reduce_add_sync(0xffffffffu, n12);
+        n3 = __reduce_add_sync(0xffffffffu, n3);
+        return make_int3(n12 & 0xffff, n12 >> 16, n3);
+      }, n, min(a.count, n), b, w);
+      if (lane == 0) s_found = make_int3((int)b, w, min(a.count, n));
+    }
+    __syncthreads();
+  } else {
+    int turn = 0;
+    auto reach = [&](uint32_t b1, uint32_t b2, uint32_t b3) {          // (at most 32,768 pages: two counts to a word)
+      int n12 = 0, n3 = 0;
+      for (int p = threadIdx.x; p < there; p += SEL_THREADS) {
+        const uint32_t key = s_key[p];
+        n12 += (key >= b1) + ((key >= b2) << 16);
+        n3 += key >= b3;
+      }
+      n12 = __reduce_add_sync(0xffffffffu, n12);
+      n3 = __reduce_add_sync(0xffffffffu, n3);
+      if (lane == 0) s_count[turn][warp] = make_int4(n12 & 0xffff, n12 >> 16, n3, 0);
+      __syncthreads();
+      int3 n = make_int3(0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < SEL_WARPS; ++i) { const int4 m = s_count[turn][i]; n.x += m.x; n.y += m.y; n.z += m.z; }
+      turn ^= 1;
+      return n;
+    };
+    const int held = reach(1u, 1u, 1u).x;
+    uint32_t b;
+    int w;
+    search(reach, held, min(a.count, held), b, w);
+    if (threadIdx.x == 0) s_found = make_int3((int)b, w, min(a.count, held));
+    __syncthreads();
   }
+  const uint32_t bound = (uint32_t)s_found.x;
+  const int want = s_found.y, k = s_found.z;
   // ---- the chosen pages in order: all above the bound, and the first of those at it ---------------------------------------------------
   // a warp has a stretch of pages: first its numbers, then its places
   const int stretch = (there + SEL_THREADS - 1) / SEL_THREADS * 32, from = min(warp * stretch, there), to = min(from + stretch, there);
