@@ -2292,44 +2292,46 @@ def attn_shared_status() -> int:
     return int(library().exl3_attn_shared_status())
 
 
-def _here(t: torch.Tensor, what: str) -> None:
-    if t.get_device() != torch._C._cuda_getDevice():
-        raise KernelLibraryError(f"{what}: the tensors are on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-
-
-def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    """All tensors on the current device."""
-    _addr(first)
-    _here(first, what)
-    at = first.device
-    for t in others:
-        if t is not None and t.device != at:
-            raise KernelLibraryError(f"{what}: tensors on {at} and {t.device}")
+def _on_this_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All of them on the current CUDA device."""
+    here = -1
+    for t in tensors:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at != here or at < 0:
+            _addr(t)
+            here = torch._C._cuda_getDevice()
+            if at != here:
+                raise KernelLibraryError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
 
 
 def _paged_pool(pool: torch.Tensor, name: str, kv_heads: int, head_dim: int, what: str) -> int:
     """The pool's pages, after its checks."""
-    if pool.dtype is not torch.bfloat16 or pool.ndim != 4 or pool.shape[1:] != (kv_heads, 64, head_dim) or not pool.is_contiguous():
-        raise KernelLibraryError(f"{what}: {name} must be contiguous bfloat16 [pages, {kv_heads}, 64, {head_dim}], got {pool.dtype} {tuple(pool.shape)}")
-    return pool.shape[0]
+    shape = pool.shape
+    if pool.dtype is not torch.bfloat16 or len(shape) != 4 or shape[1] != kv_heads or shape[2] != 64 or shape[3] != head_dim or not pool.is_contiguous():
+        raise KernelLibraryError(f"{what}: {name} must be contiguous bfloat16 [pages, {kv_heads}, 64, {head_dim}], got {pool.dtype} {tuple(shape)}")
+    return shape[0]
 
 
-def _paged_q(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, what: str) -> None:
+def _paged_q(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, what: str) -> tuple:
+    """Tokens, and elements from one to the next, after the queries' checks."""
     if head_dim not in (64, 128) or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise KernelLibraryError(f"{what}: heads of 64 or 128 in groups of one size, got {heads} heads on {kv_heads} of {head_dim}")
-    width = heads * head_dim
-    if q.dtype is not torch.bfloat16 or q.ndim != 2 or q.shape[1] != width or q.stride(1) != 1:
-        raise KernelLibraryError(f"{what}: q must be bfloat16 [tokens, {width}], got {q.dtype} {tuple(q.shape)}")
+    shape, width = q.shape, heads * head_dim
+    if q.dtype is torch.bfloat16 and len(shape) == 2 and shape[1] == width:
+        if q.is_contiguous():
+            return shape[0], width
+        if q.stride(1) == 1:
+            return shape[0], _pitch(q)
+    raise KernelLibraryError(f"{what}: q must be bfloat16 [tokens, {width}], got {q.dtype} {tuple(shape)}")
 
 
-def _paged_queries(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
-    """The output, after the queries' checks."""
-    _paged_q(q, heads, kv_heads, head_dim, what)
-    width = heads * head_dim
+def _paged_out(out: Optional[torch.Tensor], q: torch.Tensor, T: int, width: int, what: str) -> torch.Tensor:
     if out is None:
-        return q.new_empty((q.shape[0], width))
-    if out.dtype is not torch.bfloat16 or tuple(out.shape) != (q.shape[0], width) or not out.is_contiguous():
-        raise KernelLibraryError(f"{what}: out must be contiguous bfloat16 {(q.shape[0], width)}")
+        return q.new_empty((T, width))
+    if out.dtype is not torch.bfloat16 or out.shape != (T, width) or not out.is_contiguous():
+        raise KernelLibraryError(f"{what}: out must be contiguous bfloat16 {(T, width)}")
     return out
 
 
@@ -2357,9 +2359,14 @@ def _token_arrays(T: int, tok_pos: torch.Tensor, tok_seq: torch.Tensor, block_ta
     _table(block_table, None, what)
 
 
-def _pages_scratch(q: torch.Tensor, rows: int, heads: int, kv_heads: int, head_dim: int, groups: int, max_new: int, workspace) -> tuple:
-    need = _long_entry("exl3_attn_pages_scratch", 8)(_sms(q), q.shape[0], rows, heads, kv_heads, head_dim, groups, max_new)
-    return need, workspace.floats(need) if workspace is not None else torch.zeros(need, dtype=torch.float32, device=q.device)
+@functools.lru_cache(maxsize=4096)
+def _pages_floats(sms: int, T: int, rows: int, heads: int, kv_heads: int, head_dim: int, groups: int, max_new: int) -> int:
+    return _long_entry("exl3_attn_pages_scratch", 8)(sms, T, rows, heads, kv_heads, head_dim, groups, max_new)
+
+
+def _pages_scratch(need: int, q: torch.Tensor, workspace) -> int:
+    """Address of scratch memory whose counters are zero."""
+    return (workspace.floats(need) if workspace is not None else torch.zeros(need, dtype=torch.float32, device=q.device)).data_ptr()
 
 
 def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, row_start: torch.Tensor, row_pos0: torch.Tensor,
@@ -2371,7 +2378,7 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
     them, from the first row's table (None: no groups).  Their tokens see all of these keys: positions from ``64 * pages - 1`` on.  Groups do not overlap (one that
     begins before the one ahead of it ends is no group).  Pages that are not there are left out; a query that sees nothing gets zeros.
     ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's)."""
-    out = _paged_queries(q, heads, kv_heads, head_dim, out, "attn_shared")
+    T, pitch = _paged_q(q, heads, kv_heads, head_dim, "attn_shared")
     _positive(scale, "attn_shared")
     pages = _paged_pool(k_pool, "k_pool", kv_heads, head_dim, "attn_shared")
     if _paged_pool(v_pool, "v_pool", kv_heads, head_dim, "attn_shared") != pages:
@@ -2383,14 +2390,15 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
         if groups.ndim != 2 or groups.shape[1] != 3 or groups.shape[0] > PAGES_MAX_GROUPS:
             raise KernelLibraryError(f"attn_shared: groups must be int32 [up to {PAGES_MAX_GROUPS}, 3], got {tuple(groups.shape)}")
         n_groups = groups.shape[0]
-    _same_device("attn_shared", q, k_pool, v_pool, block_table, row_start, row_pos0, groups, out)
-    T = q.shape[0]
+    out = _paged_out(out, q, T, heads * head_dim, "attn_shared")
+    _on_this_device("attn_shared", q, k_pool, v_pool, block_table, row_start, row_pos0, groups, out)
     if T == 0 or rows == 0:
         return out
-    need, scratch = _pages_scratch(q, rows, heads, kv_heads, head_dim, n_groups, max_new, workspace)
+    need = _pages_floats(_sms(q), T, rows, heads, kv_heads, head_dim, n_groups, max_new)
+    scratch = _pages_scratch(need, q, workspace)
     rc = _entry("exl3_attn_shared", "plppplpiippiipiiiiifpl")(
-        _addr(q), _pitch(q), _addr(out), _addr(k_pool), _addr(v_pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], _addr(row_start),
-        _addr(row_pos0), rows, T, _addr(groups), n_groups, max_new, heads, kv_heads, head_dim, scale, _addr(scratch), need, _raw_stream())
+        q.data_ptr(), pitch, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        row_start.data_ptr(), row_pos0.data_ptr(), rows, T, groups.data_ptr() if n_groups else 0, n_groups, max_new, heads, kv_heads, head_dim, scale, scratch, need, _raw_stream())
     if rc:
         _check(rc, "attn_shared")
     return out
@@ -2424,7 +2432,7 @@ def page_bounds(k_pool: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     rows = _row_arrays(row_start, row_pos0, block_table, "page_bounds")
     if max_new < 0:
         raise KernelLibraryError(f"page_bounds: max_new {max_new}")
-    _same_device("page_bounds", k_pool, codes, scales, block_table, row_start, row_pos0)
+    _on_this_device("page_bounds", k_pool, codes, scales, block_table, row_start, row_pos0)
     if rows == 0 or max_new == 0:
         return
     rc = _entry("exl3_page_bounds", "plpiippiiiipp")(
@@ -2438,7 +2446,7 @@ def page_bounds_load(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Ten
     """The bounds that the listed pages' codes stand for: smallest and largest, float32 ``[n, kv_heads, head_dim]`` each (zeros for a number that is no page's)."""
     held, kv_heads, head_dim = _bounds_pool(codes, scales, "page_bounds_load")
     _int32(pages, "pages", "page_bounds_load")
-    _same_device("page_bounds_load", codes, scales, pages)
+    _on_this_device("page_bounds_load", codes, scales, pages)
     n = pages.numel()
     low = scales.new_empty((n, kv_heads, head_dim))
     high = torch.empty_like(low)
@@ -2456,11 +2464,10 @@ def page_select(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bloc
     over the key/value head's query heads, ``max_h(n_h * (a_h / 127)) * scale`` with ``a_h = max |q_h|``, ``c_h = rint(q_h * (127 / a_h))`` and
     ``n_h = sum_i max(c_hi * low_i, c_hi * high_i)`` over the page's codes (``page_bounds``).  A page whose keys are not finite comes before those that have a
     score.  Pages that are not there are not taken.  For queries that are not finite some pages are taken."""
-    _paged_q(q, heads, kv_heads, head_dim, "page_select")
+    T, pitch = _paged_q(q, heads, kv_heads, head_dim, "page_select")
     pages, held, size = _bounds_pool(codes, scales, "page_select")
     if (held, size) != (kv_heads, head_dim):
         raise KernelLibraryError(f"page_select: bounds of {held} key/value heads of {size}, not {kv_heads} of {head_dim}")
-    T = q.shape[0]
     if count < 1 or first < 0 or last < 1:
         raise KernelLibraryError(f"page_select: takes a count of 1 or more and at least the last page, got count {count}, first {first}, last {last}")
     _token_arrays(T, tok_pos, tok_seq, block_table, "page_select")
@@ -2468,9 +2475,9 @@ def page_select(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bloc
         out = tok_pos.new_empty((T, kv_heads, count))
     elif out.dtype is not torch.int32 or tuple(out.shape) != (T, kv_heads, count) or not out.is_contiguous():
         raise KernelLibraryError(f"page_select: out must be contiguous int32 {(T, kv_heads, count)}")
-    _same_device("page_select", q, codes, scales, block_table, tok_pos, tok_seq, out)
+    _on_this_device("page_select", q, codes, scales, block_table, tok_pos, tok_seq, out)
     rc = _entry("exl3_page_select", "plpplpiiippiiiiiiip")(
-        _addr(q), _pitch(q), _addr(codes), _addr(scales), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0], _addr(tok_pos),
+        _addr(q), pitch, _addr(codes), _addr(scales), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0], _addr(tok_pos),
         _addr(tok_seq), T, heads, kv_heads, head_dim, count, first, last, _addr(out), _raw_stream())
     if rc:
         _check(rc, "page_select")
@@ -2483,23 +2490,25 @@ def attn_pages(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, bloc
     ``[T, kv_heads, count]`` lists for it and the key/value head, by their numbers within the row (``tok_seq``), in any order; ``page_select`` makes such lists.  The first
     ``min(count, tok_pos // 64 + 1)`` entries are looked at (a token can see no more pages); entries that are negative or beyond the token's position, and pages
     that are not there, are left out, one that is listed twice counts twice.  A query that sees nothing gets zeros."""
-    out = _paged_queries(q, heads, kv_heads, head_dim, out, "attn_pages")
+    T, pitch = _paged_q(q, heads, kv_heads, head_dim, "attn_pages")
     _positive(scale, "attn_pages")
     n_pages = _paged_pool(k_pool, "k_pool", kv_heads, head_dim, "attn_pages")
     if _paged_pool(v_pool, "v_pool", kv_heads, head_dim, "attn_pages") != n_pages:
         raise KernelLibraryError("attn_pages: k_pool and v_pool have different numbers of pages")
-    T = q.shape[0]
     _token_arrays(T, tok_pos, tok_seq, block_table, "attn_pages")
     _int32(pages, "pages", "attn_pages")
-    if pages.ndim != 3 or pages.shape[:2] != (T, kv_heads) or pages.shape[2] < 1:
-        raise KernelLibraryError(f"attn_pages: pages must be int32 [{T}, {kv_heads}, 1 or more], got {tuple(pages.shape)}")
-    _same_device("attn_pages", q, k_pool, v_pool, block_table, tok_pos, tok_seq, pages, out)
+    shape = pages.shape
+    if len(shape) != 3 or shape[0] != T or shape[1] != kv_heads or shape[2] < 1:
+        raise KernelLibraryError(f"attn_pages: pages must be int32 [{T}, {kv_heads}, 1 or more], got {tuple(shape)}")
+    out = _paged_out(out, q, T, heads * head_dim, "attn_pages")
+    _on_this_device("attn_pages", q, k_pool, v_pool, block_table, tok_pos, tok_seq, pages, out)
     if T == 0:
         return out
-    need, scratch = _pages_scratch(q, T, heads, kv_heads, head_dim, 0, 0, workspace)
+    need = _pages_floats(_sms(q), T, T, heads, kv_heads, head_dim, 0, 0)
+    scratch = _pages_scratch(need, q, workspace)
     rc = _entry("exl3_attn_pages", "plppplpiiippipiiiifpl")(
-        _addr(q), _pitch(q), _addr(out), _addr(k_pool), _addr(v_pool), n_pages, _addr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0],
-        _addr(tok_pos), _addr(tok_seq), T, _addr(pages), pages.shape[2], heads, kv_heads, head_dim, scale, _addr(scratch), need, _raw_stream())
+        q.data_ptr(), pitch, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], block_table.shape[0],
+        tok_pos.data_ptr(), tok_seq.data_ptr(), T, pages.data_ptr(), shape[2], heads, kv_heads, head_dim, scale, scratch, need, _raw_stream())
     if rc:
         _check(rc, "attn_pages")
     return out
