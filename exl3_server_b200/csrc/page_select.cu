@@ -53,15 +53,19 @@ page_bounds_kernel(const __nv_bfloat16* __restrict__ k_pool, int64_t n_pages, co
   const int page = __ldcg(block_table + (int64_t)row * bt_stride + logical);
   if (page < 0 || page >= n_pages) return;
   const int filled = (int)min((int64_t)PB_PAGE, end - logical * PB_PAGE);
-  const uint4* src = reinterpret_cast<const uint4*>(k_pool + ((int64_t)page * nkv + g) * PB_PAGE * HD) + lane;
+  const uint4* src = reinterpret_cast<const uint4*>(k_pool + ((int64_t)page * nkv + g) * PB_PAGE * HD) + lane % CH;
   uint32_t mn[4], mx[4], odd = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) { mn[i] = 0x7f807f80u; mx[i] = 0xff80ff80u; }
-#pragma unroll 16
-  for (int t = 0; t < PB_PAGE / TOK; ++t) {
-    if (t * TOK + lane / CH < filled) {
-      const uint4 w = __ldcg(src + t * 32);
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  // Sixteen loads in flight a lane; behind the last token it is read again, which changes no bound.
+#pragma unroll 1
+  for (int t0 = 0; t0 < PB_PAGE / TOK && t0 * TOK < filled; t0 += 16) {
+    uint4 w[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) w[t] = __ldcg(src + min((t0 + t) * TOK + lane / CH, filled - 1) * CH);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      const uint32_t x[4] = {w[t].x, w[t].y, w[t].z, w[t].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         mn[i] = pb_min2(mn[i], x[i]);
