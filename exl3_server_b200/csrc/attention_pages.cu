@@ -20,6 +20,7 @@ constexpr int PG_STAGES = 3;                   // of a warp's ring
 constexpr int PG_UNIT_BYTES = 8192;            // a unit: keys and values of 32 tokens (heads of 64) or 16 (heads of 128)
 constexpr int PG_WINDOW = 1024;                // rows of a launch
 constexpr int PG_MIN_UNITS = 4;                // places of a warp's share, at least
+constexpr int PG_ALONE = 4;                    // units by which a share may be longer so that blocks cut no item
 constexpr int PG_MAX_WIDTH = 1 << 19;          // pages of a row
 constexpr int PG_RING = PG_STAGES * PG_UNIT_BYTES;
 constexpr uint32_t PG_SMEM_RINGS = PG_WARPS * PG_RING;
@@ -126,8 +127,8 @@ template <int HD> struct PgSmem {
   int start[PG_WINDOW], n_new[PG_WINDOW], pos[PG_WINDOW], units[PG_WINDOW];
   int shared[PG_WINDOW];                       // the pages that the row shares, -1: it is in no group
   PgPlace part_of[PG_WARPS][2];                // the warps' parts' items; units 0: none
-  int warp_sum[PG_WARPS];
-  int last[2];
+  unsigned long long warp_sum[PG_WARPS];
+  int last[2], most;                           // (most: units of the longest row)
   int odd_key[PG_WARPS][HD];                   // per feature the first key whose value is not finite among those that not all of an item's queries see
   PgGroups groups;
   int group_queries[PG_MAX_GROUPS];
@@ -179,34 +180,37 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
   }
   if (!LIST && a.n_groups > 0) for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32) sm.group_queries[j] = 0;
-  if (threadIdx.x == 0) sm.cost = 0;
+  if (threadIdx.x == 0) { sm.cost = 0; sm.most = 0; }
   if (LIST) __syncthreads();
   else pg_groups(sm.groups, a.groups, a.n_groups, a.rows, a.bt_width);
-  int total = 0;
+  unsigned long long totals = 0, upto = 0;     // items << 32 | places: of all rows, and of those up to this thread's last one
 #pragma unroll 1
   for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
     const int i = i0 + threadIdx.x;
-    int mine = 0, blocks = 0;
+    int blocks = 0, units = 0;
     if (i < n_rows) {
       const int pos = sm.pos[i], queries = sm.n_new[i] * a.G, j = LIST ? -1 : sm.groups.of(a.row0 + i), shared = j < 0 ? -1 : sm.groups.pages[j];
-      const int units = LIST ? min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP : (min(pos + sm.n_new[i], most_keys) + KS - 1) / KS - max(shared, 0) * UPP;
+      units = LIST ? min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP : (min(pos + sm.n_new[i], most_keys) + KS - 1) / KS - max(shared, 0) * UPP;
+      units = max(units, 1);                   // (one at least: every query gets an answer)
       sm.shared[i] = shared;
-      sm.units[i] = max(units, 1);             // (one at least: every query gets an answer)
-      blocks = !LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS;
-      mine = (max(units, 1) + PG_SETUP) * blocks * a.nkv;
+      sm.units[i] = units;
+      blocks = (!LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS) * a.nkv;
       if (j >= 0) atomicAdd(&sm.group_queries[j], queries);
     }
-    int incl = mine;
+    const int longest = __reduce_max_sync(0xffffffffu, blocks ? units : 0);
+    if (lane == 0) atomicMax(&sm.most, longest);
+    unsigned long long incl = (unsigned long long)blocks << 32 | (unsigned int)((units + PG_SETUP) * blocks);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+    for (int o = 1; o < 32; o <<= 1) { const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
     if (lane == 31) sm.warp_sum[warp] = incl;
     __syncthreads();
-    int before = total;
+    upto = totals + incl;
 #pragma unroll
-    for (int w = 0; w < PG_WARPS; ++w) { if (w < warp) before += sm.warp_sum[w]; total += sm.warp_sum[w]; }
-    if (i < n_rows) sm.cum[i + 1] = before + incl;
+    for (int w = 0; w < PG_WARPS; ++w) { if (w < warp) upto += sm.warp_sum[w]; totals += sm.warp_sum[w]; }
+    if (i < n_rows) sm.cum[i + 1] = (int)(unsigned int)upto;
     __syncthreads();
   }
+  int total = (int)(unsigned int)totals;
   if (threadIdx.x == 0) sm.cum[0] = 0;
   const bool beside = !LIST && a.n_groups > 0 && !a.many && a.rows <= a.window;     // the other kernel leaves this one some of the SMs
   if (beside)
@@ -219,7 +223,18 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     sms -= ps_sms((int64_t)sm.cost * a.nkv, total, gridDim.x);
     if (sms < 1) sms = gridDim.x;
   }
-  const int n_blocks = min(sms, max(1, total / (PG_WARPS * PG_MIN_UNITS))), n_shares = n_blocks * PG_WARPS;
+  int n_blocks = min(sms, max(1, total / (PG_WARPS * PG_MIN_UNITS))), setup = PG_SETUP, padded = 0;
+  // Few items get a block each, padded to one length, where that makes no share much longer than equal shares are: no item is cut by blocks then, and no share has two items.
+  const int items = (int)(totals >> 32), each = (sm.most + PG_WARPS - 1) / PG_WARPS;
+  if (items > 0 && items <= sms && n_rows <= PG_WARPS * 32 && each <= total / (n_blocks * PG_WARPS) + PG_ALONE) {
+    n_blocks = items;
+    setup = 0;
+    padded = PG_WARPS * each;
+    total = items * padded;
+    if ((int)threadIdx.x < n_rows) sm.cum[threadIdx.x + 1] = (int)(upto >> 32) * padded;
+    __syncthreads();
+  }
+  const int n_shares = n_blocks * PG_WARPS;
   if (total == 0 || (int)blockIdx.x >= n_blocks) {
     if (!a.wait_first) pdl_wait();
     return;
@@ -235,13 +250,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     PgPlace p;
     p.i = lo;
     p.units = sm.units[lo];
-    const int all = p.units + PG_SETUP, r = x - sm.cum[lo], item = r / all, nb = (sm.n_new[lo] * a.G + COLS - 1) / COLS, at = r - item * all;
+    const int all = padded ? padded : p.units + PG_SETUP, r = x - sm.cum[lo], item = r / all, nb = (sm.n_new[lo] * a.G + COLS - 1) / COLS, at = r - item * all;
     p.places = min(all - at, i_hi - x);
-    p.u0 = max(at - PG_SETUP, 0);
-    p.u1 = max(at + p.places - PG_SETUP, 0);   // (none where the share has the item's first places only)
+    p.u0 = min(max(at - setup, 0), p.units);   // (no units where the share has the item's first places only, or the padding)
+    p.u1 = min(max(at + p.places - setup, 0), p.units);
     p.g = item / nb;
     p.b = item - p.g * nb;
-    p.base = x - at + PG_SETUP;
+    p.base = x - at + setup;
     return p;
   };
 
@@ -587,26 +602,26 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int longer = rem * (per + 1);        // units of the longer shares
     return (at < longer ? at / (per + 1) : rem + (at - longer) / max(per, 1)) / PG_WARPS;
   };
-  if (threadIdx.x == 0) {
-    int n = 0, last = -1;
-    sm.edge[0] = sm.edge[1] = -1;
-#pragma unroll 1
-    for (int k = 0; k < 2 * PG_WARPS; ++k) {
-      const PgPlace& q = sm.part_of[0][k];     // (of the warps one behind the other)
-      if (q.units == 0) continue;
-      if (q.base != last) {
-        PgRun& r = sm.run[n];
-        r.p = q;
-        r.k0 = k;
-        r.whole = q.base >= block_lo && q.base + q.units <= block_hi;
-        r.own = sm.shared[q.i] >= 0;
-        if (!r.whole) sm.edge[q.base <= block_lo ? 0 : 1] = n;
-        last = q.base;
-        ++n;
-      }
-      sm.run[n - 1].k1 = k + 1;
+  if (warp == 0) {                             // a lane for each of the warps' parts, which stand one behind the other
+    const PgPlace& q = sm.part_of[0][lane % (2 * PG_WARPS)];
+    const bool there = lane < 2 * PG_WARPS && q.units != 0;
+    const uint32_t below = (1u << lane) - 1, before = __ballot_sync(0xffffffffu, there) & below;
+    const int base = q.base, base_before = __shfl_sync(0xffffffffu, base, before ? 31 - __clz(before) : 0);
+    const bool begins = there && (!before || base_before != base), whole = base >= block_lo && base + q.units <= block_hi;
+    const uint32_t all = __ballot_sync(0xffffffffu, begins), after = all & ~below & ~(1u << lane);
+    const int n = __popc(all & below);
+    if (lane < 2) sm.edge[lane] = -1;
+    __syncwarp();
+    if (begins) {
+      PgRun& r = sm.run[n];
+      r.p = q;
+      r.k0 = lane;
+      r.k1 = after ? __ffs(after) - 1 : 2 * PG_WARPS;
+      r.whole = whole;
+      r.own = sm.shared[q.i] >= 0;
+      if (!whole) sm.edge[base <= block_lo ? 0 : 1] = n;
     }
-    sm.n_runs = n;
+    if (lane == 0) sm.n_runs = __popc(all);
   }
   __syncthreads();
   // column c of a run's item, this lane's features
@@ -770,6 +785,15 @@ template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, co
   return 0;
 }
 
+// Whether a call reads so little that its rows had better read the shared pages each for itself: two launches less, and no join.  Both sides over 2 to 32 rows of 2 to 64
+// shared pages and five layouts of heads, graph time: up to 100 MB of units all of them are faster alone (8 rows of 8 pages, 32 heads on 8 of 128, 21 MB: 16.7 against 27.4 us; 32 rows
+// of 8 pages, 84 MB: 22.8 against 28.7), at 140 to 160 MB they meet (29.2 against 29.1, 27.5 against 28.4, 31.4 against 29.5).  The tables' width stands for the rows' lengths,
+// which only the GPU knows.
+static bool pg_alone(int rows, int bt_width, int max_new, int G, int nkv, int hd) {
+  const double units = (double)rows * (((int64_t)max_new * G + PG_MAX_COLS - 1) / PG_MAX_COLS) * bt_width * nkv;
+  return units * PG_PAGE * hd * 4 <= 128e6;
+}
+
 // What both entry points ask of their arguments, and the pools' maps.
 static int pg_check(const char* what, const void* q, int64_t q_stride, const void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table,
                     int bt_width, int rows, int T, int nh, int nkv, int hd, float scale, CUtensorMap* map_k, CUtensorMap* map_v) {
@@ -851,6 +875,7 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
   if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, rows, nh, nkv, hd, n_groups, max_new)) { set_error("attn_shared: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, rows, T, nh, nkv, scale, scratch);
   a.row_start = row_start; a.row_pos0 = row_pos0; a.bt_rows = rows; a.groups = groups; a.n_groups = n_groups;
+  if (n_groups && pg_alone(rows, bt_width, max_new, a.G, nkv, hd)) a.n_groups = n_groups = 0;
   const int64_t tiles = ps_tiles_of(T, a.G, rows, n_groups, max_new);
   if (tiles > PS_MAX_TILES || tiles * (bt_width + PS_SETUP) * nkv > INT32_MAX) {
     set_error("attn_shared: %d tokens of %d query heads a key/value head with %d groups are more than %d tiles of %d queries, or tables of %d pages too wide for them", T, a.G, n_groups,
