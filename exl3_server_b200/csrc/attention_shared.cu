@@ -680,19 +680,19 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // row's own pages last, so a result does not depend on which block was the first to end.
 constexpr int PJ_WARPS = 4;
 constexpr int PJ_PARTS = 1024;                 // four for every SM, at most
-template <int HD, int SPLIT>
+template <int HD, int SPLIT, int LANES>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
 attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slots, const int4* __restrict__ tokens, const float* __restrict__ records, const float* __restrict__ own,
                         __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
-  constexpr int V = HD / 32, PAIRS = PJ_WARPS / SPLIT;       // features a lane; pairs a block
-  __shared__ float s_w[PAIRS][PJ_PARTS + 1];
+  static_assert(LANES == 32 || SPLIT == 1, "a pair has some of a warp's lanes, or some warps");
+  constexpr int V = HD / LANES, W = V < 4 ? V : 4, PAIRS = PJ_WARPS * 32 / (SPLIT * LANES);      // features a lane, side by side; pairs a block
+  __shared__ float s_w[SPLIT > 1 ? PAIRS : 1][SPLIT > 1 ? PJ_PARTS + 1 : 1];
   __shared__ float s_y[SPLIT > 1 ? PJ_WARPS : 1][SPLIT > 1 ? HD : 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pair = warp / SPLIT, w0 = warp % SPLIT;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x % LANES, pair = threadIdx.x / (SPLIT * LANES), w0 = warp % SPLIT;
   const int64_t th = (int64_t)blockIdx.x * PAIRS + pair;
   pdl_trigger();
   pdl_wait();
   const bool there = th < (int64_t)T * nh;
-  if (SPLIT == 1 && !there) return;
   const int tok = there ? (int)(th / nh) : 0, head = there ? (int)(th - (int64_t)tok * nh) : 0, G = nh / nkv, g = head / G, h = head - g * G;
   const int4 w = __ldcg(tokens + tok);         // (shared tile, its first token, own tile, its first token)
   // a source: the parts of one tile
@@ -711,7 +711,6 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
     return s;
   };
   const bool any = there && (w.x >= 0 || w.z >= 0);          // else its own pages' part was all
-  if (SPLIT == 1 && !any) return;
   const Source s0 = source(any ? w.x : -1, w.y), s1 = source(any ? w.z : -1, w.w);
   const int n01 = s0.n + s1.n, n = any ? n01 + (w.z < 0 ? 1 : 0) : 0;    // (no tile for the row's own pages: the walk's part)
   const float* mine = own + (int64_t)T * nh * HD + 2 * th;
@@ -724,19 +723,24 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
   };
   float mm = -INFINITY, l = 0.0f;
 #pragma unroll 1
-  for (int i = lane; i < n; i += 32) {
+  for (int i = lane; i < n; i += LANES) {
     int row = 0;
     const float* p = i < n01 ? part(i, row) : mine;
     const float m1 = __ldcg(p + row), l1 = __ldcg(p + row + (i < n01 ? PS_TILE : 1)), top = fmaxf(mm, m1), safe = top == -INFINITY ? 0.0f : top;
     l = l * ps_exp2(mm - safe) + l1 * ps_exp2(m1 - safe);
     mm = top;
-    if (w0 == 0) s_w[pair][i] = m1;
+    if (SPLIT > 1 && w0 == 0) s_w[pair][i] = m1;
   }
-  const float top = warp_max(mm), safe = top == -INFINITY ? 0.0f : top;
-  l = warp_sum(l * ps_exp2(mm - safe));
-  if (SPLIT > 1) __syncthreads(); else __syncwarp();
+  float top = mm;
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float safe = top == -INFINITY ? 0.0f : top;
+  l *= ps_exp2(mm - safe);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (SPLIT > 1) __syncthreads();
   float y[V] = {};
-  constexpr int BATCH = 8;
+  constexpr int BATCH = LANES == 32 ? 8 : 2;
 #pragma unroll 1
   for (int i0 = w0; i0 < n; i0 += SPLIT * BATCH) {
     float v[BATCH][V], f[BATCH];
@@ -746,13 +750,19 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
       f[b] = 0.0f;
       if (i < n) {
         int row = 0;
-        const float* p = i < n01 ? part(i, row) + 2 * PS_TILE : own + th * HD;
-        p += row * HD;
-        f[b] = ps_exp2(s_w[pair][i] - safe);
-        if (V == 4) { const float4 x = __ldcg(reinterpret_cast<const float4*>(p + lane * V)); v[b][0] = x.x; v[b][1] = x.y; v[b][V - 2] = x.z; v[b][V - 1] = x.w; }
-        else { const float2 x = __ldcg(reinterpret_cast<const float2*>(p + lane * V)); v[b][0] = x.x; v[b][1] = x.y; }
+        const float* p = i < n01 ? part(i, row) : mine;
+        f[b] = SPLIT > 1 ? s_w[pair][i] : __ldcg(p + row);
+        p = i < n01 ? p + 2 * PS_TILE + row * HD : own + th * HD;
+#pragma unroll
+        for (int e = 0; e < V; e += W) {
+          const float* const at = p + (e * LANES + lane * W);
+          if (W == 4) { const float4 x = __ldcg(reinterpret_cast<const float4*>(at)); v[b][e] = x.x; v[b][e + 1] = x.y; v[b][e + W - 2] = x.z; v[b][e + W - 1] = x.w; }
+          else { const float2 x = __ldcg(reinterpret_cast<const float2*>(at)); v[b][e] = x.x; v[b][e + 1] = x.y; }
+        }
       }
     }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) f[b] = i0 + b * SPLIT < n ? ps_exp2(f[b] - safe) : 0.0f;
 #pragma unroll
     for (int b = 0; b < BATCH; ++b)
 #pragma unroll
@@ -763,18 +773,20 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
 #pragma unroll
     for (int e = 0; e < V; ++e) s_y[warp][lane * V + e] = y[e];
     __syncthreads();
-    if (w0 != 0 || !any) return;
+    if (w0 != 0) return;
 #pragma unroll
     for (int k = 1; k < SPLIT; ++k)
 #pragma unroll
       for (int e = 0; e < V; ++e) y[e] += s_y[warp + k][lane * V + e];
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint32_t o[V / 2];
+  if (!any) return;
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) o[i] = ps_pack(y[2 * i] * inv, y[2 * i + 1] * inv);
-  if (V == 4) *reinterpret_cast<uint2*>(out + th * HD + lane * V) = make_uint2(o[0], o[V / 2 - 1]);
-  else *reinterpret_cast<uint32_t*>(out + th * HD + lane * V) = o[0];
+  for (int e = 0; e < V; e += W) {
+    __nv_bfloat16* const to = out + th * HD + e * LANES + lane * W;
+    if (W == 4) *reinterpret_cast<uint2*>(to) = make_uint2(ps_pack(y[e] * inv, y[e + 1] * inv), ps_pack(y[e + W - 2] * inv, y[e + W - 1] * inv));
+    else *reinterpret_cast<uint32_t*>(to) = ps_pack(y[e] * inv, y[e + 1] * inv);
+  }
 }
 
 int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int hd, cudaStream_t stream) {
@@ -785,8 +797,8 @@ int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int 
     launch_pdl(kernel, dim3((unsigned)((pairs + per_block - 1) / per_block)), dim3(PJ_WARPS * 32), 0, stream, reinterpret_cast<const int4*>(a.parts), a.most_tiles, (int)ps_slots(a.sms, a.nkv, a.most_tiles),
                reinterpret_cast<const int4*>(a.tokens), (const float*)a.records, own, out, a.T, a.nkv * a.G, a.nkv);
   };
-  if (hd == 64) { if (few) go(attn_shared_join_kernel<64, PJ_WARPS>, 1); else go(attn_shared_join_kernel<64, 1>, PJ_WARPS); }
-  else { if (few) go(attn_shared_join_kernel<128, PJ_WARPS>, 1); else go(attn_shared_join_kernel<128, 1>, PJ_WARPS); }
+  if (hd == 64) { if (few) go(attn_shared_join_kernel<64, PJ_WARPS, 32>, 1); else go(attn_shared_join_kernel<64, 1, 8>, PJ_WARPS * 4); }
+  else { if (few) go(attn_shared_join_kernel<128, PJ_WARPS, 32>, 1); else go(attn_shared_join_kernel<128, 1, 8>, PJ_WARPS * 4); }
   return launch_status("attn_shared join");
 }
 

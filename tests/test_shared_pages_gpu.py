@@ -102,7 +102,7 @@ def test_long_prefix_and_many_blocks():
     assert P.off(run_shared(case, ws=workspace()), want, size) <= 1.0
 
 
-@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (8, 2, 128), (6, 6, 128), (16, 1, 64), (5, 1, 128)])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (8, 2, 128), (6, 6, 128), (16, 1, 64), (5, 1, 128), (16, 2, 128)])
 @pytest.mark.parametrize("rows,groups", [
     ([(0, 200)], []),                                       # a prompt
     ([(3, 130), (700, 65), (10, 1), (0, 300)], []),         # prompts beside a token, behind contexts
