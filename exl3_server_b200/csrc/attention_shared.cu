@@ -70,8 +70,22 @@ __device__ inline void ps_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t db, 
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// D (+)= A B^T, both in shared memory.
+__device__ inline void ps_mma_ss(uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// One lane of a whole warp, always the same one.
+__device__ inline bool ps_elect() {
+  uint32_t it;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(it));
+  return it != 0;
 }
 __device__ inline void ps_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -395,12 +409,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           if (p == t.p0 + (two ? 0 : s) && !ps_wait(q_full + s, k[s] & 1)) { ok = false; break; }
           if (f[s] >= 2 && !ps_wait(pv_done + 2 * s + sb, ((f[s] >> 1) - 1) & 1)) { ok = false; break; }
           fence_after();
-          if (lane == 0) {
+          if (ps_elect()) {
 #pragma unroll
             for (int b = 0; b < BOXES; ++b) {
               const uint64_t da = smem_desc_k128(smem_u32(sQ + s * second_q + b * 128 * 128)), db = smem_desc_k128(smem_u32(sK + st * KVB + b * PS_BOX));
 #pragma unroll
-              for (int i = 0; i < 4; ++i) mma_ss(tmem + 128 * s + 64 * sb, da + 2 * i, db + 2 * i, PS_IDESC_S, (b | i) > 0);
+              for (int i = 0; i < 4; ++i) ps_mma_ss(tmem + 128 * s + 64 * sb, da + 2 * i, db + 2 * i, PS_IDESC_S, (b | i) > 0);
             }
             mma_commit(s_full + 2 * s + sb);
             if (one && p == t.p1 - 1) mma_commit(&bars.q_free);        // (the sets share the queries' place)
@@ -487,7 +501,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           const int sb = f[s] & 1;
           if (!ps_wait(p_full + 2 * s + sb, (f[s] >> 1) & 1)) { ok = false; break; }
           fence_after();
-          if (lane == 0) {
+          if (ps_elect()) {
             const uint64_t db = ps_desc_v<HD>(smem_u32(sV + st * KVB));
             const bool fresh = p == t.p0 + (two ? 0 : s);            // a part's first product starts O afresh
 #pragma unroll
