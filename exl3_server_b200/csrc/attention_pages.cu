@@ -220,7 +220,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   __syncthreads();
   int sms = gridDim.x;
   if (beside && sm.cost > 0) {
-    sms -= ps_sms((int64_t)sm.cost * a.nkv, total, gridDim.x);
+    sms -= ps_sms((int64_t)sm.cost * a.nkv, total, COLS, gridDim.x);
     if (sms < 1) sms = gridDim.x;
   }
   int n_blocks = min(sms, max(1, total / (PG_WARPS * PG_MIN_UNITS))), setup = PG_SETUP, padded = 0;

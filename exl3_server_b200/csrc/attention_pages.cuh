@@ -63,13 +63,19 @@ constexpr int PS_SETUP = 6;                    // places of the list that a tile
 constexpr int PG_SETUP = 3;
 
 // Both kernels run side by side where there is work for both: the tensor cores' takes some of the SMs and leaves the others to the walk, whose streams of pages fill the memory's queue
-// from fewer SMs than there are (a batch of 64 behind 4,096 shared keys, 32 heads of 128 on 8, 30 to 2,000 keys of their own: one after the other 117 us).  Both work out how many, in units of
-// 10 ns of an SM: `tiles` for the tiles' pages (180 for two sets of queries, 60 for one), PG_COST for a place of the walk; and the time that the memory takes for these (8 KB in 1.25 ns).
-constexpr int64_t PS_COST_TWO = 180, PS_COST_ONE = 60, PG_COST = 16;
-__host__ __device__ inline int ps_sms(int64_t tiles, int64_t places, int sms) {
+// from fewer SMs than there are (a batch of 64 behind 4,096 shared keys, 32 heads of 128 on 8, 30 to 2,000 keys of their own: one after the other 117 us, side by side 80).  Both work out
+// how many, in units of 10 ns of an SM: `tiles` for the tiles' pages (180 for two sets of queries, 60 for one), PG_COST for a place of the walk (8 queries an item, PG_COST_16: 16), PG_START
+// for what the walk takes however many SMs it has; and the time that the memory takes for its units (8 KB in 1.25 ns).  16 rows of up to 500 keys behind 2,048 pages, 32 heads on 2:
+// without PG_START and with 16 for all the walk had 2 SMs and the call took 102 us, now 69.5; 48 rows in 5 groups 50 and 46; 24 or 40 for PG_COST_16: 76.7 or 69.6, 48.1 or 47.9.
+constexpr int64_t PS_COST_TWO = 180, PS_COST_ONE = 60, PG_COST = 16, PG_COST_16 = 32, PG_START = 400;
+__host__ __device__ inline int ps_sms(int64_t tiles, int64_t places, int cols, int sms) {
   if (tiles == 0 || places == 0) return sms;
-  const int64_t walk = places * PG_COST, memory = places / 8;
-  int64_t n = (tiles * sms + (tiles + walk) / 2) / (tiles + walk);
+  const int64_t walk = places * (cols == 8 ? PG_COST : PG_COST_16), memory = places / 8;
+  // the fewest SMs from which on the tiles are not the slower side, or one less
+  auto slower = [&](int64_t n) { return tiles * (sms - n) > (walk + PG_START * (sms - n)) * n; };
+  int64_t n = 1, hi = sms - 1;
+  while (n < hi) { const int64_t mid = (n + hi) >> 1; if (slower(mid)) n = mid + 1; else hi = mid; }
+  if (n > 1 && tiles * (sms - n) < (walk + PG_START * (sms - n)) * (n - 1)) --n;
   if (memory > 0 && tiles / memory + 1 < n) n = tiles / memory + 1;
   return (int)(n < 1 ? 1 : n > sms - 1 ? sms - 1 : n);
 }

@@ -277,7 +277,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
       t.cum[0] = 0;
       t.small = small;
       // (beside rows of many tokens the walk has little to do, and of more rows than a launch of it takes it knows no more than these)
-      t.sms = a.many || a.rows > a.window ? (int)gridDim.x : ps_sms(t.cost * a.nkv, t.places * a.nkv, gridDim.x);
+      t.sms = a.many || a.rows > a.window ? (int)gridDim.x : ps_sms(t.cost * a.nkv, t.places * a.nkv, a.cols, gridDim.x);
       p.n_tiles = n_tiles;
       p.total = run * a.nkv;                   // (the host has seen that it stays within 31 bits)
       p.blocks = min(t.sms, max(1, p.total / PS_MIN_PAGES));
