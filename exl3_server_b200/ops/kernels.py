@@ -2436,8 +2436,8 @@ def page_bounds(k_pool: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     if rows == 0 or max_new == 0:
         return
     rc = _entry("exl3_page_bounds", "plpiippiiiipp")(
-        _addr(k_pool), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], _addr(row_start), _addr(row_pos0), rows, max_new, kv_heads, head_dim,
-        _addr(codes), _addr(scales), _raw_stream())
+        k_pool.data_ptr(), pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], row_start.data_ptr(), row_pos0.data_ptr(), rows, max_new, kv_heads, head_dim,
+        codes.data_ptr(), scales.data_ptr(), _raw_stream())
     if rc:
         _check(rc, "page_bounds")
 
@@ -2450,7 +2450,7 @@ def page_bounds_load(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Ten
     n = pages.numel()
     low = scales.new_empty((n, kv_heads, head_dim))
     high = torch.empty_like(low)
-    rc = _entry("exl3_page_bounds_load", "pplpiiipp")(_addr(codes), _addr(scales), held, _addr(pages), n, kv_heads, head_dim, low.data_ptr(), high.data_ptr(), _raw_stream())
+    rc = _entry("exl3_page_bounds_load", "pplpiiipp")(codes.data_ptr(), scales.data_ptr(), held, pages.data_ptr(), n, kv_heads, head_dim, low.data_ptr(), high.data_ptr(), _raw_stream())
     if rc:
         _check(rc, "page_bounds_load")
     return low, high
@@ -2477,8 +2477,8 @@ def page_select(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bloc
         raise KernelLibraryError(f"page_select: out must be contiguous int32 {(T, kv_heads, count)}")
     _on_this_device("page_select", q, codes, scales, block_table, tok_pos, tok_seq, out)
     rc = _entry("exl3_page_select", "plpplpiiippiiiiiiip")(
-        _addr(q), pitch, _addr(codes), _addr(scales), pages, _addr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0], _addr(tok_pos),
-        _addr(tok_seq), T, heads, kv_heads, head_dim, count, first, last, _addr(out), _raw_stream())
+        q.data_ptr(), pitch, codes.data_ptr(), scales.data_ptr(), pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], block_table.shape[0], tok_pos.data_ptr(),
+        tok_seq.data_ptr(), T, heads, kv_heads, head_dim, count, first, last, out.data_ptr(), _raw_stream())
     if rc:
         _check(rc, "page_select")
     return out
