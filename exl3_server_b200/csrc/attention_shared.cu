@@ -407,6 +407,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll 1
       for (int p = t.p0; p < t.p1 && ok; ++p) {
         if (!ps_wait(kv_full + st, phase)) { ok = false; break; }
+        if (one && t.p1 - t.p0 == 1 && !ps_wait(q_full + 1, k[1] & 1)) { ok = false; break; }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (!two && ((p - t.p0) & 1) != s) continue;
@@ -430,7 +431,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (++st == stages) { st = 0; phase ^= 1; }
       }
       k[0] += t.p1 > t.p0;
-      k[1] += t.p1 - t.p0 > (two ? 0 : 1);     // (a set without a page asks for no queries)
+      k[1] += t.p1 - t.p0 > (two || one ? 0 : 1);              // (a set without a page asks for no queries; where the sets share them it says so)
       x += t.places;
     }
     if (!ok && lane == 0) atomicExch(&g_ps_error, 2);
@@ -559,6 +560,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         float* rec = a.records + m.slot * ps_record(HD);       // no page for this set
         rec[m.qr] = -INFINITY;
         rec[PS_TILE + m.qr] = 0.0f;
+        if (one) ps_arrive_warp(q_full + s);                   // (it asks for nothing, but no part may be two ahead of a set)
       }
       if (!ok) break;
       if (more) {

@@ -2366,7 +2366,12 @@ def _pages_floats(sms: int, T: int, rows: int, heads: int, kv_heads: int, head_d
 
 def _pages_scratch(need: int, q: torch.Tensor, workspace) -> int:
     """Address of scratch memory whose counters are zero."""
-    return (workspace.floats(need) if workspace is not None else torch.zeros(need, dtype=torch.float32, device=q.device)).data_ptr()
+    if workspace is None:
+        return torch.zeros(need, dtype=torch.float32, device=q.device).data_ptr()
+    t = workspace.floats(need)
+    if t.get_device() != q.get_device():
+        raise KernelLibraryError(f"the workspace is on {t.device}, the tensors on {q.device}")
+    return t.data_ptr()
 
 
 def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, row_start: torch.Tensor, row_pos0: torch.Tensor,
