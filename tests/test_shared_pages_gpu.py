@@ -452,3 +452,59 @@ def test_on_another_stream():
         got = K().attn_shared(q, k, v, table, start, pos0, None, 3, 8, 2, 64, scale=0.125, workspace=ws)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+def test_two_graphs_over_one_workspace():
+    """Recorded one by one, replayed in turn: what one leaves in the scratch memory is nothing to the other."""
+    ws = workspace()
+    ws.reserve(1 << 22)
+    a = Paged([(40 * PAGE + 5 * i, 1) for i in range(6)], 8, 2, 128, share=share([(6, 40)]), seed=31)
+    b = Paged([(900, 2), (64, 1), (5 * PAGE, 1)], 4, 4, 64, share=share([(1, 5)], 2), seed=32)
+    lists = torch.tensor([[[p for p in (0, 3, 9, -1)]] * 2] * 6, dtype=torch.int32, device=DEV)
+    graphs = []
+    for case in (a, b):
+        q, k, v, table = case.q.to(DEV), case.k.to(DEV), case.v.to(DEV), wide(case, case.table.to(DEV))
+        start, pos0, groups, pos, seq = ints(case.start), ints(case.pos0), ints(case.groups).view(-1, 3), ints(case.tok_pos), ints(case.tok_seq)
+
+        def step(case=case, q=q, k=k, v=v, table=table, start=start, pos0=pos0, groups=groups, pos=pos, seq=seq):
+            y = K().attn_shared(q, k, v, table, start, pos0, groups, case.max_new, case.h, case.g, case.d, scale=0.1, workspace=ws)
+            return y, K().attn_pages(q, k, v, table, pos, seq, lists, 8, 2, 128, scale=0.1, workspace=ws) if case is a else y
+
+        want = [t.clone() for t in step()]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, got, want, step))
+    for _ in range(3):
+        for graph, got, _, _ in graphs:
+            for t in got:
+                t.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        K().check_status()
+        assert all(torch.equal(x, y) for _, got, want, _ in graphs for x, y in zip(got, want))
+
+
+def test_two_streams_at_once():
+    """Two calls at a time, each with a workspace of its own, over one cache."""
+    case = Paged([(70 * PAGE + 3 * i, 1) for i in range(12)], 16, 2, 64, share=share([(12, 70)]), seed=33)
+    want = run_shared(case)
+    q, k, v, table = case.q.to(DEV), case.k.to(DEV), case.v.to(DEV), wide(case, case.table.to(DEV))
+    start, pos0, groups = ints(case.start), ints(case.pos0), ints(case.groups)
+    streams, spaces = [torch.cuda.Stream() for _ in range(2)], [workspace() for _ in range(2)]
+    for ws in spaces:
+        ws.reserve(1 << 22)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for s, ws in zip(streams, spaces):
+            with torch.cuda.stream(s):
+                got.append(K().attn_shared(q, k, v, table, start, pos0, groups, 1, 16, 2, 64, scale=0.125, workspace=ws))
+    torch.cuda.synchronize()
+    K().check_status()
+    assert all(torch.equal(y, want) for y in got)
