@@ -53,6 +53,7 @@ struct PgArgs {
   int many;                                    // whether rows of more than PS_MANY queries are another kernel's work
   int tiles;                                   // whether the kernel before works on shared pages, or on rows of many queries
   int wait_first;                              // whether the kernel before must have ended
+  int* late;                                   // where the blocks with work are counted (plus 1) for those that begin when the kernel before leaves them an SM; 0: not yet, null: no such
   float* own;                                  // rows of groups: their own pages' part goes here
 };
 
@@ -130,7 +131,7 @@ template <int HD> struct PgSmem {
   int shared[PG_WINDOW];                       // the pages that the row shares, -1: it is in no group
   PgPlace part_of[PG_WARPS][2];                // the warps' parts' items; units 0: none
   unsigned long long warp_sum[PG_WARPS];
-  int last[2], most;                           // (most: units of the longest row)
+  int last[2], most, late;                           // (most: units of the longest row)
   int odd_key[PG_WARPS][HD];                   // per feature the first key whose value is not finite among those that not all of an item's queries see
   PgGroups groups;
   int group_queries[PG_MAX_GROUPS];
@@ -170,6 +171,8 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   if (a.wait_first) pdl_wait();
   pdl_trigger();
 
+  const int late = !LIST && a.late && threadIdx.x == 0 ? __ldcg(a.late) : 0;
+  const int3 asked = !LIST ? pg_group_asked(a.groups, a.n_groups) : make_int3(0, 0, 0);
   // ---- the rows of this launch -------------------------------------------------------------------------------------------
   const int most_keys = a.bt_width * PG_PAGE, n_rows = min(a.rows - a.row0, a.window);
 #pragma unroll 1
@@ -182,9 +185,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
   }
   if (!LIST && a.n_groups > 0) for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32) sm.group_queries[j] = 0;
-  if (threadIdx.x == 0) { sm.cost = 0; sm.most = 0; }
+  if (threadIdx.x == 0) { sm.cost = 0; sm.most = 0; sm.late = late; }
   if (LIST) __syncthreads();
-  else pg_groups(sm.groups, a.groups, a.n_groups, a.rows, a.bt_width);
+  else pg_groups(sm.groups, asked, a.n_groups, a.rows, a.bt_width);
+  if (!LIST && sm.late > 0 && (int)blockIdx.x >= sm.late - 1) {      // (no work came to it before)
+    if (!a.wait_first) pdl_wait();
+    return;
+  }
   unsigned long long totals = 0, upto = 0;     // items << 32 | places: of all rows, and of those up to this thread's last one
 #pragma unroll 1
   for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
@@ -236,6 +243,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if ((int)threadIdx.x < n_rows) sm.cum[threadIdx.x + 1] = (int)(upto >> 32) * padded;
     __syncthreads();
   }
+  if (!LIST && a.late && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.late, (total ? n_blocks : 0) + 1);
   const int n_shares = n_blocks * PG_WARPS;
   if (total == 0 || (int)blockIdx.x >= n_blocks) {
     if (!a.wait_first) pdl_wait();
@@ -896,9 +904,10 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
     p.cols = pg_cols(max_new, a.G); p.window = pg_window(a, hd, max_new, false); p.hd = hd;
     p.records = at + s.records;
     a.own = at + s.own;
+    if (rows <= p.window) a.late = a.counters + PG_COUNTERS - 1;
     rc = attn_shared_launch(p, k_pool, v_pool, hd, sms, stream);
     if (rc) return rc;
   }
   rc = pg_launch<false>(a, map_k, map_v, hd, max_new, sms, "attn_shared", stream);
-  return rc || !tiles ? rc : attn_shared_join(p, a.own, a.out, hd, stream);
+  return rc || !tiles ? rc : attn_shared_join(p, a.own, a.out, a.counters + PG_COUNTERS - 1, hd, stream);
 }

@@ -23,13 +23,18 @@ struct PgGroups {                              // in shared memory
     return row >= first[lo] && row < first[lo] + rows[lo] && pages[lo] > 0 ? lo : -1;
   }
 };
+static_assert(PG_MAX_GROUPS <= 256, "a thread of a block for each");
+// This thread's group of the list, on its way beside whatever else is asked for.
+__device__ inline int3 pg_group_asked(const int* __restrict__ list, int n) {
+  const int* const at = list + 3 * threadIdx.x;
+  return (int)threadIdx.x < n ? make_int3(__ldcg(at), __ldcg(at + 1), __ldcg(at + 2)) : make_int3(0, 0, 0);
+}
 // By all threads of a block; ends with a barrier.
-__device__ inline void pg_groups(PgGroups& g, const int* __restrict__ list, int n, int rows, int bt_width) {
-#pragma unroll 1
-  for (int j = threadIdx.x; j < n; j += blockDim.x) {
-    g.first[j] = __ldcg(list + 3 * j);
-    g.rows[j] = __ldcg(list + 3 * j + 1);
-    g.pages[j] = min(max(__ldcg(list + 3 * j + 2), 0), bt_width);
+__device__ inline void pg_groups(PgGroups& g, int3 asked, int n, int rows, int bt_width) {
+  if ((int)threadIdx.x < n) {
+    g.first[threadIdx.x] = asked.x;
+    g.rows[threadIdx.x] = asked.y;
+    g.pages[threadIdx.x] = min(max(asked.z, 0), bt_width);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -129,6 +134,6 @@ struct PsArgs {
 };
 cudaError_t attn_shared_prepare();             // once for a device
 int attn_shared_launch(const PsArgs& a, const void* k_pool, const void* v_pool, int hd, int sms, cudaStream_t stream);
-int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int hd, cudaStream_t stream);
+int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int* late, int hd, cudaStream_t stream);
 
 }  // namespace exl3

@@ -192,13 +192,14 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
   const int most = a.bt_width * PG_PAGE;       // (a row beyond the table sees all of it)
   auto start_of = [&](int r) { return held ? t.start[r] : min(max(__ldcg(a.row_start + r), 0), a.T); };
   auto pos_of = [&](int r) { return held ? t.pos[r] : min(__ldcg(a.row_pos0 + r), most); };
+  const int3 asked = pg_group_asked(a.groups, a.n_groups);
   if (held)
 #pragma unroll 1
     for (int r = threadIdx.x; r <= a.rows; r += PS_THREADS) {
       t.start[r] = min(max(__ldcg(a.row_start + r), 0), a.T);
       if (r < a.rows) t.pos[r] = min(__ldcg(a.row_pos0 + r), most);
     }
-  pg_groups(t.groups, a.groups, a.n_groups, a.rows, a.bt_width);
+  pg_groups(t.groups, asked, a.n_groups, a.rows, a.bt_width);
 #pragma unroll 1
   for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS) {
     const int r0 = t.groups.first[j], s0 = start_of(r0), s1 = max(start_of(r0 + t.groups.rows[j]), s0);
@@ -705,7 +706,7 @@ constexpr int PJ_PARTS = 1024;                 // four for every SM, at most
 template <int HD, int SPLIT, int LANES>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
 attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slots, const int4* __restrict__ tokens, const float* __restrict__ records, const float* __restrict__ own,
-                        __nv_bfloat16* __restrict__ out, int T, int nh, int nkv) {
+                        __nv_bfloat16* __restrict__ out, int T, int nh, int nkv, int* late) {
   static_assert(LANES == 32 || SPLIT == 1, "a pair has some of a warp's lanes, or some warps");
   constexpr int V = HD / LANES, W = V < 4 ? V : 4, PAIRS = PJ_WARPS * 32 / (SPLIT * LANES);      // features a lane, side by side; pairs a block
   __shared__ float s_w[SPLIT > 1 ? PAIRS : 1][SPLIT > 1 ? PJ_PARTS + 1 : 1];
@@ -715,6 +716,7 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
   pdl_trigger();
   pdl_wait();
   const bool there = th < (int64_t)T * nh;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *late = 0;         // (the walk has ended)
   const int tok = there ? (int)(th / nh) : 0, head = there ? (int)(th - (int64_t)tok * nh) : 0, G = nh / nkv, g = head / G, h = head - g * G;
   const int4 w = __ldcg(tokens + tok);         // (shared tile, its first token, own tile, its first token)
   // a source: the parts of one tile
@@ -811,13 +813,13 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
   }
 }
 
-int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int hd, cudaStream_t stream) {
+int attn_shared_join(const PsArgs& a, const float* own, __nv_bfloat16* out, int* late, int hd, cudaStream_t stream) {
   // few queries: a block each, since a query of a few may have hundreds of parts
   const int64_t pairs = (int64_t)a.T * a.nkv * a.G;
   const bool few = pairs <= 4096;
   auto go = [&](auto kernel, int per_block) {
     launch_pdl(kernel, dim3((unsigned)((pairs + per_block - 1) / per_block)), dim3(PJ_WARPS * 32), 0, stream, reinterpret_cast<const int4*>(a.parts), a.most_tiles, (int)ps_slots(a.sms, a.nkv, a.most_tiles),
-               reinterpret_cast<const int4*>(a.tokens), (const float*)a.records, own, out, a.T, a.nkv * a.G, a.nkv);
+               reinterpret_cast<const int4*>(a.tokens), (const float*)a.records, own, out, a.T, a.nkv * a.G, a.nkv, late);
   };
   if (hd == 64) { if (few) go(attn_shared_join_kernel<64, PJ_WARPS, 32>, 1); else go(attn_shared_join_kernel<64, 1, 8>, PJ_WARPS * 4); }
   else { if (few) go(attn_shared_join_kernel<128, PJ_WARPS, 32>, 1); else go(attn_shared_join_kernel<128, 1, 8>, PJ_WARPS * 4); }
