@@ -2292,18 +2292,15 @@ def attn_shared_status() -> int:
     return int(library().exl3_attn_shared_status())
 
 
-def _on_this_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+def _on_this_device(what: str, *tensors: torch.Tensor) -> None:
     """All of them on the current CUDA device."""
-    here = -1
+    here = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        at = t.get_device()
-        if at != here or at < 0:
-            _addr(t)
-            here = torch._C._cuda_getDevice()
-            if at != here:
-                raise KernelLibraryError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+        if t.get_device() != here:
+            raise KernelLibraryError(f"{what}: tensors on {tensors[0].device} and on {t.device}")
+    _addr(tensors[0])
+    if here != torch._C._cuda_getDevice():
+        raise KernelLibraryError(f"{what}: the tensors are on {tensors[0].device}, the current device is another")
 
 
 def _paged_pool(pool: torch.Tensor, name: str, kv_heads: int, head_dim: int, what: str) -> int:
@@ -2329,7 +2326,7 @@ def _paged_q(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, what: st
 
 def _paged_out(out: Optional[torch.Tensor], q: torch.Tensor, T: int, width: int, what: str) -> torch.Tensor:
     if out is None:
-        return q.new_empty((T, width))
+        return q.new_empty(T, width)
     if out.dtype is not torch.bfloat16 or out.shape != (T, width) or not out.is_contiguous():
         raise KernelLibraryError(f"{what}: out must be contiguous bfloat16 {(T, width)}")
     return out
@@ -2352,8 +2349,9 @@ def _positive(scale: float, what: str) -> None:
 
 
 def _token_arrays(T: int, tok_pos: torch.Tensor, tok_seq: torch.Tensor, block_table: torch.Tensor, what: str) -> None:
-    _int32(tok_pos, "tok_pos", what)
-    _int32(tok_seq, "tok_seq", what)
+    if tok_pos.dtype is not torch.int32 or tok_seq.dtype is not torch.int32 or not tok_pos.is_contiguous() or not tok_seq.is_contiguous():
+        _int32(tok_pos, "tok_pos", what)
+        _int32(tok_seq, "tok_seq", what)
     if tok_pos.numel() < T or tok_seq.numel() < T:
         raise KernelLibraryError(f"{what}: tok_pos has {tok_pos.numel()} and tok_seq {tok_seq.numel()} entries for {T} tokens")
     _table(block_table, None, what)
@@ -2396,7 +2394,7 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
             raise KernelLibraryError(f"attn_shared: groups must be int32 [up to {PAGES_MAX_GROUPS}, 3], got {tuple(groups.shape)}")
         n_groups = groups.shape[0]
     out = _paged_out(out, q, T, heads * head_dim, "attn_shared")
-    _on_this_device("attn_shared", q, k_pool, v_pool, block_table, row_start, row_pos0, groups, out)
+    _on_this_device("attn_shared", q, k_pool, v_pool, block_table, row_start, row_pos0, q if groups is None else groups, out)
     if T == 0 or rows == 0:
         return out
     need = _pages_floats(_sms(q), T, rows, heads, kv_heads, head_dim, n_groups, max_new)
@@ -2453,8 +2451,7 @@ def page_bounds_load(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Ten
     _int32(pages, "pages", "page_bounds_load")
     _on_this_device("page_bounds_load", codes, scales, pages)
     n = pages.numel()
-    low = scales.new_empty((n, kv_heads, head_dim))
-    high = torch.empty_like(low)
+    low, high = scales.new_empty(n, kv_heads, head_dim), scales.new_empty(n, kv_heads, head_dim)
     rc = _entry("exl3_page_bounds_load", "pplpiiipp")(codes.data_ptr(), scales.data_ptr(), held, pages.data_ptr(), n, kv_heads, head_dim, low.data_ptr(), high.data_ptr(), _raw_stream())
     if rc:
         _check(rc, "page_bounds_load")
@@ -2477,7 +2474,7 @@ def page_select(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bloc
         raise KernelLibraryError(f"page_select: takes a count of 1 or more and at least the last page, got count {count}, first {first}, last {last}")
     _token_arrays(T, tok_pos, tok_seq, block_table, "page_select")
     if out is None:
-        out = tok_pos.new_empty((T, kv_heads, count))
+        out = tok_pos.new_empty(T, kv_heads, count)
     elif out.dtype is not torch.int32 or tuple(out.shape) != (T, kv_heads, count) or not out.is_contiguous():
         raise KernelLibraryError(f"page_select: out must be contiguous int32 {(T, kv_heads, count)}")
     _on_this_device("page_select", q, codes, scales, block_table, tok_pos, tok_seq, out)
