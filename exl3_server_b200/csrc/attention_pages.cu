@@ -131,7 +131,7 @@ template <int HD> struct PgSmem {
   int shared[PG_WINDOW];                       // the pages that the row shares, -1: it is in no group
   PgPlace part_of[PG_WARPS][2];                // the warps' parts' items; units 0: none
   unsigned long long warp_sum[PG_WARPS];
-  int last[2], most, late;                           // (most: units of the longest row)
+  int last[2], most, late, rows_end;                           // (most: units of the longest row)
   int odd_key[PG_WARPS][HD];                   // per feature the first key whose value is not finite among those that not all of an item's queries see
   PgGroups groups;
   int group_queries[PG_MAX_GROUPS];
@@ -171,6 +171,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   if (a.wait_first) pdl_wait();
   pdl_trigger();
 
+  const int rows_end = !LIST && threadIdx.x == 0 ? min(max(__ldcg(a.row_start + a.rows), 0), a.T) : 0;
   const int late = !LIST && a.late && threadIdx.x == 0 ? __ldcg(a.late) : 0;
   const int3 asked = !LIST ? pg_group_asked(a.groups, a.n_groups) : make_int3(0, 0, 0);
   // ---- the rows of this launch -------------------------------------------------------------------------------------------
@@ -184,13 +185,28 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     sm.start[i] = start;
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
   }
-  if (!LIST && a.n_groups > 0) for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32) sm.group_queries[j] = 0;
-  if (threadIdx.x == 0) { sm.cost = 0; sm.most = 0; sm.late = late; }
+  int* const group_alone = &sm.odd_key[0][0];  // (before the units need the place)
+  if (!LIST && a.n_groups > 0) for (int j = threadIdx.x; j < a.n_groups; j += PG_WARPS * 32) { sm.group_queries[j] = 0; group_alone[j] = 0; }
+  if (threadIdx.x == 0) { sm.cost = 0; sm.most = 0; sm.late = late; sm.rows_end = rows_end; }
   if (LIST) __syncthreads();
   else pg_groups(sm.groups, asked, a.n_groups, a.rows, a.bt_width);
   if (!LIST && sm.late > 0 && (int)blockIdx.x >= sm.late - 1) {      // (no work came to it before)
     if (!a.wait_first) pdl_wait();
     return;
+  }
+  if (!LIST && a.many && a.n_groups > 0) {     // groups that are worth it, as the tensor cores' kernel finds them, of all rows
+    auto start_of = [&](int r) { return r == a.rows ? sm.rows_end : a.rows <= a.window ? sm.start[r] : min(max(__ldcg(a.row_start + r), 0), a.T); };
+#pragma unroll 1
+    for (int r = threadIdx.x; r < a.rows; r += PG_WARPS * 32) {
+      const int n = max(start_of(r + 1) - start_of(r), 0) * a.G, j = sm.groups.of(r);
+      if (j >= 0 && n > 0) atomicAdd(&group_alone[j], ps_alone(n, COLS, HD));
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < a.n_groups) {
+      const int r0 = sm.groups.first[threadIdx.x], s0 = start_of(r0), s1 = max(start_of(r0 + sm.groups.rows[threadIdx.x]), s0);
+      if (!ps_worth((s1 - s0) * a.G, sm.groups.pages[threadIdx.x], group_alone[threadIdx.x])) sm.groups.pages[threadIdx.x] = 0;
+    }
+    __syncthreads();
   }
   unsigned long long totals = 0, upto = 0;     // items << 32 | places: of all rows, and of those up to this thread's last one
 #pragma unroll 1
@@ -730,6 +746,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 
+static_assert(sizeof(PgSmem<64>::odd_key) >= PG_MAX_GROUPS * sizeof(int), "the groups' sums lie there first");
 constexpr int PG_SMEM = (int)(PG_SMEM_RINGS + sizeof(PgSmem<128>) + 1024);
 static_assert(PG_SMEM <= 232448, "what a block may have");
 

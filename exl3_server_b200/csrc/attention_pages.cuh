@@ -90,6 +90,18 @@ __device__ inline int64_t ps_cost(int queries, int pages) {
   return (int64_t)((queries + PS_TILE - 1) / PS_TILE) * (pages + PS_SETUP) * (queries > 128 ? PS_COST_TWO : PS_COST_ONE);
 }
 
+// Where rows have many tokens: whether a group's tiles cost less than its rows reading the pages each for itself, in 10 ns of an SM.  Tiles: a page 1.1 us for two sets of queries, 0.52 for one; a group's way in
+// and out PS_SETUP pages, and 0.04 us a query to join.  Rows: tiles of their own where they have many queries, else the walk.  37 prompts of 41 to 252 tokens
+// behind one page, 36 heads of 64: 219 us when they shared it, 167; 62 of 99 to 128 tokens behind 16 to 19 pages in three groups 399 and 353; 24 of 16 to 120 behind
+// 94 pages, 32 heads of 128 on 8, share them: 220 and 260.  (Steps of few tokens a row are not asked: the pass over the rows costs 1 us, and short ones leave groups alone anyhow.)
+__device__ inline int64_t ps_tile_cost(int queries) { return (int64_t)(queries / PS_TILE) * 110 + (queries % PS_TILE > 128 ? 110 : queries % PS_TILE > 0 ? 52 : 0); }
+__device__ inline int ps_alone(int queries, int cols, int hd) {                    // a page, for a row's queries
+  return queries > PS_MANY ? (int)ps_tile_cost(queries) : (queries + cols - 1) / cols * (hd == 64 ? 2 : 4) * (int)(cols == 8 ? PG_COST : PG_COST_16);
+}
+__device__ inline bool ps_worth(int queries, int pages, int alone) {               // alone: of all of the group's rows
+  return pages > 0 && ps_tile_cost(queries) * (pages + PS_SETUP) + 4 * (int64_t)queries < (int64_t)alone * pages;
+}
+
 struct PsPlan {                                // the head of the list
   int n_tiles;
   int blocks;                                  // shares

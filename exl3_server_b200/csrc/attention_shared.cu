@@ -199,10 +199,22 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
       t.start[r] = min(max(__ldcg(a.row_start + r), 0), a.T);
       if (r < a.rows) t.pos[r] = min(__ldcg(a.row_pos0 + r), most);
     }
+  static_assert(sizeof(t.odd_key) >= PG_MAX_GROUPS * sizeof(int), "the groups' sums lie there first");
+  int* const group_alone = &t.odd_key[0][0][0];
+  if ((int)threadIdx.x < a.n_groups) group_alone[threadIdx.x] = 0;
   pg_groups(t.groups, asked, a.n_groups, a.rows, a.bt_width);
+  if (a.many && a.n_groups > 0) {
+#pragma unroll 1
+    for (int r = threadIdx.x; r < a.rows; r += PS_THREADS) {
+      const int n = max(start_of(r + 1) - start_of(r), 0) * a.G, j = t.groups.of(r);
+      if (j >= 0 && n > 0) atomicAdd(&group_alone[j], ps_alone(n, a.cols, a.hd));
+    }
+    __syncthreads();
+  }
 #pragma unroll 1
   for (int j = threadIdx.x; j < a.n_groups; j += PS_THREADS) {
     const int r0 = t.groups.first[j], s0 = start_of(r0), s1 = max(start_of(r0 + t.groups.rows[j]), s0);
+    if (a.many && !ps_worth((s1 - s0) * a.G, t.groups.pages[j], group_alone[j])) t.groups.pages[j] = 0;
     t.group_tok[j] = s0;
     t.group_tile[j] = t.groups.pages[j] > 0 ? (s1 - s0) * a.G : 0;     // (queries, for now)
     t.group_seen[j] = INT32_MAX;

@@ -2377,8 +2377,8 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention ``softmax(q K^T * scale) V`` of a step's new tokens over the paged bfloat16 cache, which already holds them, where rows share pages.  Row r has
     tokens ``row_start[r] .. row_start[r + 1] - 1`` (at most ``max_new``) of ``q`` bfloat16 ``[T, heads * head_dim]`` at positions ``row_pos0[r] ...``.
-    ``groups``: int32 ``[n, 3]`` on the device, ascending: the rows ``first .. first + rows - 1`` have their first ``pages`` pages in common, which are read once for all of
-    them, from the first row's table (None: no groups).  Their tokens see all of these keys: positions from ``64 * pages - 1`` on.  Groups do not overlap (one that
+    ``groups``: int32 ``[n, 3]`` on the device, ascending: the rows ``first .. first + rows - 1`` have their first ``pages`` pages in common, the same in each one's table,
+    which are read once for all of them where that is the faster way (None: no groups).  Their tokens see all of these keys: positions from ``64 * pages - 1`` on.  Groups do not overlap (one that
     begins before the one ahead of it ends is no group).  Pages that are not there are left out; a query that sees nothing gets zeros.
     ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's)."""
     T, pitch = _paged_q(q, heads, kv_heads, head_dim, "attn_shared")

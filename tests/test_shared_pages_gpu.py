@@ -100,7 +100,7 @@ def test_more_queries_than_a_tile(heads, kv_heads, d, n, new):
 @pytest.mark.parametrize("pages", [[1], [1, 1, 2, 1, 3]])
 def test_many_groups_of_few_pages(heads, kv_heads, d, pages):
     """A block has several tiles one behind the other, of which only one of its two sets of queries has a page."""
-    shares = [(j, pages[j % len(pages)]) for j in range(100) for _ in range(2)]
+    shares = [(j, pages[j % len(pages)]) for j in range(60) for _ in range(16)]
     case = Paged([(p * PAGE + r % 7, 1) for r, (_, p) in enumerate(shares)], heads, kv_heads, d, share=shares, seed=8)
     want, size = P.shared(case, d ** -0.5)
     assert P.off(run_shared(case, ws=workspace()), want, size) <= 1.0
@@ -109,7 +109,7 @@ def test_many_groups_of_few_pages(heads, kv_heads, d, pages):
 @pytest.mark.parametrize("heads,kv_heads,d", [(16, 8, 64), (8, 8, 128)])
 def test_many_groups_of_few_pages_beside_a_large_one(heads, kv_heads, d):
     """The same, where the two sets have places of their own for their queries."""
-    shares = [(j, 1) for j in range(90) for _ in range(2)] + [(99, 2)] * 140
+    shares = [(j, 1) for j in range(50) for _ in range(16)] + [(99, 2)] * 140
     case = Paged([(s[1] * PAGE + r % 7, 1) for r, s in enumerate(shares)], heads, kv_heads, d, share=shares, seed=9)
     want, size = P.shared(case, d ** -0.5)
     assert P.off(run_shared(case, ws=workspace()), want, size) <= 1.0
