@@ -71,7 +71,7 @@ constexpr int PG_SETUP = 3;
 // from fewer SMs than there are (a batch of 64 behind 4,096 shared keys, 32 heads of 128 on 8, 30 to 2,000 keys of their own: one after the other 117 us, side by side 80).  Both work out
 // how many, in units of 10 ns of an SM: `tiles` for the tiles' pages (180 for two sets of queries, 60 for one), PG_COST for a place of the walk (8 queries an item, PG_COST_16: 16), PG_START
 // for what the walk takes however many SMs it has; and the time that the memory takes for its units (8 KB in 1.25 ns).  16 rows of up to 500 keys behind 2,048 pages, 32 heads on 2:
-// without PG_START and with 16 for all the walk had 2 SMs and the call took 102 us, now 69.5; 48 rows in 5 groups 50 and 46; 24 or 40 for PG_COST_16: 76.7 or 69.6, 48.1 or 47.9.
+// without PG_START and with 16 for all the walk had 2 SMs and the call took 102 us, with them 69.5; 48 rows in 5 groups 50 and 46; 24 or 40 for PG_COST_16: 76.7 or 69.6, 48.1 or 47.9.
 constexpr int64_t PS_COST_TWO = 180, PS_COST_ONE = 60, PG_COST = 16, PG_COST_16 = 32, PG_START = 400;
 __host__ __device__ inline int ps_sms(int64_t tiles, int64_t places, int cols, int sms) {
   if (tiles == 0 || places == 0) return sms;
