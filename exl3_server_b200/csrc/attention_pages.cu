@@ -131,7 +131,8 @@ template <int HD> struct PgSmem {
   int shared[PG_WINDOW];                       // the pages that the row shares, -1: it is in no group
   PgPlace part_of[PG_WARPS][2];                // the warps' parts' items; units 0: none
   unsigned long long warp_sum[PG_WARPS];
-  int last[2], most, late, rows_end;                           // (most: units of the longest row)
+  int last[2], late;
+  int most, rows_end;                          // units of the longest row; the token behind the last row
   int odd_key[PG_WARPS][HD];                   // per feature the first key whose value is not finite among those that not all of an item's queries see
   PgGroups groups;
   int group_queries[PG_MAX_GROUPS];
@@ -190,7 +191,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   if (threadIdx.x == 0) { sm.cost = 0; sm.most = 0; sm.late = late; sm.rows_end = rows_end; }
   if (LIST) __syncthreads();
   else pg_groups(sm.groups, asked, a.n_groups, a.rows, a.bt_width);
-  if (!LIST && sm.late > 0 && (int)blockIdx.x >= sm.late - 1) {      // (no work came to it before)
+  if (!LIST && sm.late > 0 && (int)blockIdx.x >= sm.late - 1) {      // (began late: the blocks that have work are others)
     if (!a.wait_first) pdl_wait();
     return;
   }
