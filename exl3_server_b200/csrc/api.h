@@ -505,8 +505,10 @@ int exl3_fp8_linear(const void* x, int64_t ldx, void* codes, float* sx, const vo
 int exl3_fp8_skinny_status();
 int exl3_fp8_wide_status();
 // Attention over lists of pages (attention_pages.cu) and over pages that rows share (attention_shared.cu), bfloat16, pools [pages, kv heads, 64, hd].  scratch:
-// exl3_attn_pages_scratch floats, the first 65,536 of them zero before the first call (they are zero after each).
-long long exl3_attn_pages_scratch(int sms, int T, int rows, int nh, int nkv, int hd, int n_groups, int max_new);
+// exl3_attn_pages_scratch or exl3_attn_shared_scratch floats, the first 65,536 of them zero before the first call (they are zero after each).
+// chosen (may be null): the groups that are used, whether rows of many tokens have tiles of their own, the most tiles of a key/value head.
+long long exl3_attn_pages_scratch(int sms, int hd);
+long long exl3_attn_shared_scratch(int sms, int T, int rows, int nh, int nkv, int hd, int n_groups, int max_new, int bt_width, int* chosen);
 // Token t attends over the pages of its row that lists[t][kv head][count] names (its first min(count, tok_pos / 64 + 1) entries).
 int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table, int bt_stride,
                     int bt_width, int bt_rows, const int* tok_pos, const int* tok_seq, int T, const int* lists, int count, int nh, int nkv, int hd, float scale,

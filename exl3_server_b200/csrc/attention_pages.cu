@@ -781,15 +781,6 @@ static PsSpace ps_space(int sms, int64_t T, int G, int nkv, int hd, int tiles) {
   s.end = after(s.own, ps_own(T, G * nkv, hd));
   return s;
 }
-// Whether rows of many tokens are the tensor cores' work, and the most tiles there can be (0: no call of that kernel).
-static bool ps_many(int64_t T, int G, int rows, int n_groups, int max_new) {
-  return (int64_t)max_new * G > PS_MANY && rows <= PS_MAX_ROWS && ps_most_tiles(T, G, n_groups, rows) <= PS_MAX_TILES;
-}
-static int64_t ps_tiles_of(int64_t T, int G, int rows, int n_groups, int max_new) {
-  if (ps_many(T, G, rows, n_groups, max_new)) return ps_most_tiles(T, G, n_groups, rows);
-  return n_groups ? T * G / PS_TILE + n_groups : 0;
-}
-
 static int pg_cols(int max_new, int G) { return (int64_t)max_new * G <= 8 ? 8 : 16; }
 // As many rows a launch as have fewer than 2^31 units together.
 static int pg_window(const PgArgs& a, int hd, int max_new, bool list) {
@@ -820,6 +811,25 @@ template <bool LIST> static int pg_launch(PgArgs a, const CUtensorMap& map_k, co
 static bool pg_alone(int rows, int bt_width, int max_new, int G, int nkv, int hd) {
   const double units = (double)rows * (((int64_t)max_new * G + PG_MAX_COLS - 1) / PG_MAX_COLS) * bt_width * nkv;
   return units * PG_PAGE * hd * 4 <= 128e6;
+}
+
+// What a call works with: the one place where that is settled, so that the scratch memory is asked for, checked and laid out for the same tiles.  (Fewer groups can mean more tiles:
+// without their tiles rows of many tokens may have tiles of their own.)
+struct PsChoice {
+  int groups;                                  // the caller's, or 0 where they are left alone
+  bool many;                                   // whether rows of many tokens are the tensor cores' work
+  int64_t tiles;                               // of a key/value head, at most; 0: no call of that kernel
+};
+static PsChoice ps_choose(int64_t T, int G, int rows, int n_groups, int max_new, int bt_width, int nkv, int hd) {
+  PsChoice c = {n_groups && pg_alone(rows, bt_width, max_new, G, nkv, hd) ? 0 : n_groups, false, 0};
+  const int64_t most = ps_most_tiles(T, G, c.groups, rows);
+  c.many = (int64_t)max_new * G > PS_MANY && rows <= PS_MAX_ROWS && most <= PS_MAX_TILES;
+  c.tiles = c.many ? most : c.groups ? T * G / PS_TILE + c.groups : 0;
+  return c;
+}
+// Floats of scratch for it.
+static int64_t ps_floats(const PsChoice& c, int sms, int64_t T, int G, int nkv, int hd) {
+  return PG_COUNTERS + pg_record_floats(sms, hd) + (c.tiles ? ps_space(sms, T, G, nkv, hd, (int)std::min<int64_t>(c.tiles, PS_MAX_TILES)).end : 0);
 }
 
 // What both entry points ask of their arguments, and the pools' maps.
@@ -861,11 +871,14 @@ extern "C" int exl3_attn_pages_status() {
   return v;
 }
 
-// Floats of scratch that a call with these sizes wants (lists: no groups, max_new 0); the first PG_COUNTERS must be zero before the first call and are zero after each.
-extern "C" long long exl3_attn_pages_scratch(int sms, int T, int rows, int nh, int nkv, int hd, int n_groups, int max_new) {
-  if (nkv < 1) return 0;
-  const int64_t tiles = max_new ? ps_tiles_of(T, nh / nkv, rows, n_groups, max_new) : 0;
-  return PG_COUNTERS + pg_record_floats(sms, hd) + (tiles ? ps_space(sms, T, nh / nkv, nkv, hd, (int)std::min<int64_t>(tiles, PS_MAX_TILES)).end : 0);
+// Floats of scratch that a call over lists wants; the first PG_COUNTERS must be zero before the first call and are zero after each.
+extern "C" long long exl3_attn_pages_scratch(int sms, int hd) { return PG_COUNTERS + pg_record_floats(sms, hd); }
+// The same for a call over rows; chosen (may be null): the groups that are used, whether rows of many tokens have tiles of their own, the most tiles of a key/value head.
+extern "C" long long exl3_attn_shared_scratch(int sms, int T, int rows, int nh, int nkv, int hd, int n_groups, int max_new, int bt_width, int* chosen) {
+  if (nkv < 1 || nh < nkv) return 0;
+  const PsChoice c = ps_choose(T, nh / nkv, rows, n_groups, max_new, bt_width, nkv, hd);
+  if (chosen) { chosen[0] = c.groups; chosen[1] = c.many; chosen[2] = (int)std::min<int64_t>(c.tiles, INT32_MAX); }
+  return ps_floats(c, sms, T, nh / nkv, nkv, hd);
 }
 
 // Attention of each token over the pages that lists[token][kv head][count] names.
@@ -879,7 +892,7 @@ extern "C" int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const
   if (!tok_pos || !tok_seq || !lists || count < 1) { set_error("attn_pages: an array is missing, or lists of %d pages", count); return ERR_BAD_ARGUMENT; }
   const int sms = pg_sms("attn_pages");
   if (!sms) return ERR_UNSUPPORTED;
-  if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, T, nh, nkv, hd, 0, 0)) { set_error("attn_pages: scratch too small"); return ERR_SCRATCH; }
+  if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, hd)) { set_error("attn_pages: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, T, T, nh, nkv, scale, scratch);
   a.tok_pos = tok_pos; a.tok_seq = tok_seq; a.lists = lists; a.count = std::min(count, bt_width);
   a.list_stride = count; a.bt_rows = bt_rows;
@@ -900,18 +913,19 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
   }
   const int sms = pg_sms("attn_shared");
   if (!sms) return ERR_UNSUPPORTED;
-  if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, T, rows, nh, nkv, hd, n_groups, max_new)) { set_error("attn_shared: scratch too small"); return ERR_SCRATCH; }
+  const PsChoice c = ps_choose(T, nh / nkv, rows, n_groups, max_new, bt_width, nkv, hd);
+  const int64_t tiles = c.tiles;
+  n_groups = c.groups;
+  if (!scratch || scratch_floats < ps_floats(c, sms, T, nh / nkv, nkv, hd)) { set_error("attn_shared: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, rows, T, nh, nkv, scale, scratch);
   a.row_start = row_start; a.row_pos0 = row_pos0; a.bt_rows = rows; a.groups = groups; a.n_groups = n_groups;
-  if (n_groups && pg_alone(rows, bt_width, max_new, a.G, nkv, hd)) a.n_groups = n_groups = 0;
-  const int64_t tiles = ps_tiles_of(T, a.G, rows, n_groups, max_new);
   if (tiles > PS_MAX_TILES || tiles * (bt_width + PS_SETUP) * nkv > INT32_MAX) {
     set_error("attn_shared: %d tokens of %d query heads a key/value head with %d groups are more than %d tiles of %d queries, or tables of %d pages too wide for them", T, a.G, n_groups,
               PS_MAX_TILES, PS_TILE, bt_width);
     return ERR_UNSUPPORTED;
   }
   a.tiles = tiles > 0;
-  a.many = ps_many(T, a.G, rows, n_groups, max_new);
+  a.many = c.many;
   PsArgs p = {};
   if (tiles) {
     float* at = scratch + PG_COUNTERS + pg_record_floats(sms, hd);

@@ -2357,9 +2357,21 @@ def _token_arrays(T: int, tok_pos: torch.Tensor, tok_seq: torch.Tensor, block_ta
     _table(block_table, None, what)
 
 
+@functools.lru_cache(maxsize=64)
+def _pages_floats(sms: int, head_dim: int) -> int:
+    return _long_entry("exl3_attn_pages_scratch", 2)(sms, head_dim)
+
+
 @functools.lru_cache(maxsize=4096)
-def _pages_floats(sms: int, T: int, rows: int, heads: int, kv_heads: int, head_dim: int, groups: int, max_new: int) -> int:
-    return _long_entry("exl3_attn_pages_scratch", 8)(sms, T, rows, heads, kv_heads, head_dim, groups, max_new)
+def _shared_plan(sms: int, T: int, rows: int, heads: int, kv_heads: int, head_dim: int, groups: int, max_new: int, width: int) -> tuple:
+    """Floats of scratch that ``attn_shared`` wants, and what it works with: the groups that are used, whether rows of many tokens have tiles of their own, and the most tiles of a
+    key/value head."""
+    fn = library().exl3_attn_shared_scratch
+    fn.argtypes = [_c_int] * 9 + [_c_void_p]
+    fn.restype = ctypes.c_longlong
+    chosen = (_c_int * 3)()
+    need = fn(sms, T, rows, heads, kv_heads, head_dim, groups, max_new, width, ctypes.addressof(chosen))
+    return need, chosen[0], bool(chosen[1]), chosen[2]
 
 
 def _pages_scratch(need: int, q: torch.Tensor, workspace) -> int:
@@ -2397,7 +2409,7 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
     _on_this_device("attn_shared", q, k_pool, v_pool, block_table, row_start, row_pos0, q if groups is None else groups, out)
     if T == 0 or rows == 0:
         return out
-    need = _pages_floats(_sms(q), T, rows, heads, kv_heads, head_dim, n_groups, max_new)
+    need = _shared_plan(_sms(q), T, rows, heads, kv_heads, head_dim, n_groups, max_new, block_table.shape[1])[0]
     scratch = _pages_scratch(need, q, workspace)
     rc = _entry("exl3_attn_shared", "plppplpiippiipiiiiifpl")(
         q.data_ptr(), pitch, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
@@ -2506,7 +2518,7 @@ def attn_pages(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, bloc
     _on_this_device("attn_pages", q, k_pool, v_pool, block_table, tok_pos, tok_seq, pages, out)
     if T == 0:
         return out
-    need = _pages_floats(_sms(q), T, T, heads, kv_heads, head_dim, 0, 0)
+    need = _pages_floats(_sms(q), head_dim)
     scratch = _pages_scratch(need, q, workspace)
     rc = _entry("exl3_attn_pages", "plppplpiiippipiiiifpl")(
         q.data_ptr(), pitch, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], block_table.shape[0],

@@ -1,0 +1,45 @@
+"""Calls of attention over shared and over chosen pages that the tests of their results do not make: at the limits of what the kernels take, with arrays that are laid out otherwise, and what
+they write into beside the output."""
+import math
+
+import pytest
+import torch
+
+import plain_pages as P
+import test_shared_pages_gpu as base
+from plain_pages import PAGE, Paged
+from test_shared_pages_gpu import DEV, K, ints, run_shared, share, wide, workspace
+
+pytestmark = pytest.mark.gpu
+
+
+class Guarded:
+    """A workspace whose buffer ends where the call's scratch memory does, with a pattern behind it."""
+
+    GUARD = 16 << 20      # floats
+
+    def __init__(self):
+        self.buf, self.asked = None, 0
+
+    def floats(self, n):
+        self.asked = n
+        self.buf = torch.zeros(n + self.GUARD, dtype=torch.float32, device=DEV)
+        self.buf[n:] = 7.0
+        return self.buf[:n]
+
+    def untouched(self):
+        return bool((self.buf[self.asked:] == 7.0).all()) and bool((self.buf[:65536].view(torch.int32) == 0).all())
+
+
+# ---- scratch memory -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,new,heads,kv_heads,groups", [(300, 5, 16, 1, 32), (300, 10, 8, 1, 30)])
+def test_groups_that_are_left_alone_write_no_further_than_their_scratch(rows, new, heads, kv_heads, groups):
+    """Without its groups each row has a tile, with them there are too many: the scratch memory is that of the call that is made."""
+    cuts = [rows * i // groups for i in range(groups + 1)]
+    case = Paged([(PAGE, new)] * rows, heads, kv_heads, 64, share=share([(b - a, 1) for a, b in zip(cuts, cuts[1:])]), seed=40)
+    ws = Guarded()
+    want, size = P.shared(case, 0.125)
+    got = run_shared(case, ws=ws, little=True)
+    assert ws.untouched()
+    assert P.off(got, want, size) <= 1.0

@@ -1,0 +1,63 @@
+"""What a call of attention over shared pages settles before anything is launched: its scratch memory against what its kernels write into it, worked out here.  On the CPU."""
+import random
+
+import pytest
+
+from exl3_server_b200.ops import kernels as K
+
+SMS = 148
+
+
+def tiles_made(news, groups, heads_per, many):
+    """Tiles of a key/value head that a step's kernel makes: of each group's queries, and of each row's own where rows of many tokens have tiles."""
+    first = 0
+    tiles = 0
+    for n in groups:
+        tiles += -(-sum(news[first:first + n]) * heads_per // 256)
+        first += n
+    return tiles + (sum(-(-n * heads_per // 256) for n in news if n * heads_per > 64) if many else 0)
+
+
+def floats_written(tiles, T, heads, kv_heads, d):
+    """The counters, the walk's records, the tiles' places and parts, the tokens' and the rows' own parts, each at least as far as it is written."""
+    walk = SMS * (8 * 16 * d + 2 * 16 * (d + 2))
+    return 65536 + walk + 4 * kv_heads * tiles + 4 * T + (SMS - 1 + kv_heads * tiles) * 256 * (d + 2) + T * heads * (d + 2)
+
+
+def check(news, groups, heads, kv_heads, d, width):
+    T = sum(news)
+    need, used, many, most = K._shared_plan(SMS, T, len(news), heads, kv_heads, d, len(groups), max(news), width)
+    assert used in (0, len(groups))
+    tiles = tiles_made(news, groups if used else [], heads // kv_heads, many)
+    assert tiles <= most
+    if 0 < most <= 512:
+        assert need >= floats_written(tiles, T, heads, kv_heads, d), (need, used, many, most)
+    return used, many, most
+
+
+@pytest.mark.parametrize("rows,new,heads,kv_heads,groups,width", [
+    (300, 5, 16, 1, 32, 1), (300, 5, 16, 1, 32, 4), (300, 10, 8, 1, 30, 2), (300, 16, 20, 4, 32, 1), (300, 16, 20, 4, 100, 1)])
+def test_groups_that_are_left_alone(rows, new, heads, kv_heads, groups, width):
+    """Without its groups such a call gives each row a tile of its own, and with them not: its scratch memory has to be that of the tiles it has."""
+    cuts = [rows * i // groups for i in range(groups + 1)]
+    used, many, most = check([new] * rows, [b - a for a, b in zip(cuts, cuts[1:])], heads, kv_heads, 64, width)
+    assert used == 0 and many and most >= rows
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_scratch_holds_what_is_written(seed):
+    """Rows, groups and tables on both sides of the limits."""
+    rng = random.Random(seed)
+    seen = set()
+    for _ in range(1500):
+        heads, kv_heads, d = rng.choice([(16, 2, 64), (16, 1, 64), (8, 1, 64), (20, 4, 64), (36, 36, 64), (32, 8, 128), (32, 1, 128), (7, 1, 128), (128, 1, 128)])
+        rows = int(2 ** rng.uniform(0, 10.2))
+        high = int(2 ** rng.uniform(0, min(13, 17.5 - rng.uniform(0, 1) * rows.bit_length())))
+        news = [rng.randint(0, max(high, 1)) for _ in range(rows)]
+        news[rng.randrange(rows)] = max(high, 1)
+        left, groups = rows, []
+        while left and len(groups) < 256 and rng.random() < 0.97:
+            groups.append(min(left, rng.choice([1, 2, 3, 10, 40])))
+            left -= groups[-1]
+        seen.add(check(news, groups, heads, kv_heads, d, int(2 ** rng.uniform(0, 9)))[:2])
+    assert len({many for _, many in seen}) == 2
