@@ -278,7 +278,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
     }
     __syncthreads();
   }
-  n_tiles = min(n_tiles, PS_MAX_TILES);
+  n_tiles = min(n_tiles, a.most_tiles);        // (rows that are not one behind the other could make more than there are places for)
   if (threadIdx.x < 32) {                      // running sums, a warp
     int run = 0;
 #pragma unroll 1

@@ -43,3 +43,21 @@ def test_groups_that_are_left_alone_write_no_further_than_their_scratch(rows, ne
     got = run_shared(case, ws=ws, little=True)
     assert ws.untouched()
     assert P.off(got, want, size) <= 1.0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("groups", [[], [[6 * j, 6, 1] for j in range(33)]])
+def test_rows_that_are_not_one_behind_the_other(d, groups):
+    """Rows that all claim the same tokens make more tiles than the tokens can: no result is defined, and nothing is written but the output and the scratch memory."""
+    k, case = K(), Paged([(3 * PAGE, 100)], 16, 1, d, seed=41)
+    T, rows = 100, 200
+    out = torch.full((T + 64, 16 * d), 7.0, dtype=torch.bfloat16, device=DEV)
+    table = wide(case, case.table.to(DEV)).expand(rows, -1)
+    start = ints([0, T] * (rows // 2) + [0])
+    ws = Guarded()
+    k.attn_shared(case.q.to(DEV), case.k.to(DEV), case.v.to(DEV), table, start, ints([3 * PAGE] * rows), ints(groups).view(-1, 3), 100, 16, 1, d, scale=0.1, workspace=ws, out=out[:T])
+    torch.cuda.synchronize()
+    k.check_status()
+    assert ws.untouched() and bool((out[T:] == 7.0).all())
+    want, size = P.shared(case, 0.1)
+    assert P.off(run_shared(case, scale=0.1), want, size) <= 1.0
