@@ -2374,14 +2374,14 @@ def _shared_plan(sms: int, T: int, rows: int, heads: int, kv_heads: int, head_di
     return need, chosen[0], bool(chosen[1]), chosen[2]
 
 
-def _pages_scratch(need: int, q: torch.Tensor, workspace) -> int:
-    """Address of scratch memory whose counters are zero."""
+def _pages_scratch(need: int, q: torch.Tensor, workspace) -> torch.Tensor:
+    """Scratch memory whose counters are zero.  (To be held until the kernels are in the stream: what is freed before may be given to another thread's tensor.)"""
     if workspace is None:
-        return torch.zeros(need, dtype=torch.float32, device=q.device).data_ptr()
+        return torch.zeros(need, dtype=torch.float32, device=q.device)
     t = workspace.floats(need)
     if t.get_device() != q.get_device():
         raise KernelLibraryError(f"the workspace is on {t.device}, the tensors on {q.device}")
-    return t.data_ptr()
+    return t
 
 
 def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, row_start: torch.Tensor, row_pos0: torch.Tensor,
@@ -2413,7 +2413,7 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
     scratch = _pages_scratch(need, q, workspace)
     rc = _entry("exl3_attn_shared", "plppplpiippiipiiiiifpl")(
         q.data_ptr(), pitch, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        row_start.data_ptr(), row_pos0.data_ptr(), rows, T, groups.data_ptr() if n_groups else 0, n_groups, max_new, heads, kv_heads, head_dim, scale, scratch, need, _raw_stream())
+        row_start.data_ptr(), row_pos0.data_ptr(), rows, T, groups.data_ptr() if n_groups else 0, n_groups, max_new, heads, kv_heads, head_dim, scale, scratch.data_ptr(), need, _raw_stream())
     if rc:
         _check(rc, "attn_shared")
     return out
@@ -2522,7 +2522,7 @@ def attn_pages(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, bloc
     scratch = _pages_scratch(need, q, workspace)
     rc = _entry("exl3_attn_pages", "plppplpiiippipiiiifpl")(
         q.data_ptr(), pitch, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], block_table.shape[0],
-        tok_pos.data_ptr(), tok_seq.data_ptr(), T, pages.data_ptr(), shape[2], heads, kv_heads, head_dim, scale, scratch, need, _raw_stream())
+        tok_pos.data_ptr(), tok_seq.data_ptr(), T, pages.data_ptr(), shape[2], heads, kv_heads, head_dim, scale, scratch.data_ptr(), need, _raw_stream())
     if rc:
         _check(rc, "attn_pages")
     return out

@@ -1,7 +1,9 @@
 """What a call of attention over shared pages settles before anything is launched: its scratch memory against what its kernels write into it, worked out here.  On the CPU."""
 import random
+import weakref
 
 import pytest
+import torch
 
 from exl3_server_b200.ops import kernels as K
 
@@ -61,3 +63,34 @@ def test_scratch_holds_what_is_written(seed):
             left -= groups[-1]
         seen.add(check(news, groups, heads, kv_heads, d, int(2 ** rng.uniform(0, 9)))[:2])
     assert len({many for _, many in seen}) == 2
+
+
+@pytest.mark.parametrize("lists", [False, True])
+def test_scratch_memory_lives_until_the_launch(lists, monkeypatch):
+    """Without a workspace: memory that is free when the kernels go into the stream may be another thread's by then."""
+    made, alive = [], []
+    zeros = torch.zeros
+
+    def note(*a, **kw):
+        t = zeros(*a, **kw)
+        made.append(weakref.ref(t))
+        return t
+
+    def entry(name, args):
+        def call(*values):
+            alive.append([r() is not None and r().data_ptr() in values for r in made])
+            return 0
+        return call
+
+    q, pool, table = zeros(3, 256).bfloat16(), zeros(4, 2, 64, 64).bfloat16(), zeros(2, 2, dtype=torch.int32)
+    row_start, pos0, pos, seq, pages = (torch.tensor(v, dtype=torch.int32) for v in ([0, 1, 3], [5, 70], [5, 70, 71], [0, 1, 1], [[[0], [0]]] * 3))
+    monkeypatch.setattr(K, "_entry", entry)
+    monkeypatch.setattr(K, "_on_this_device", lambda *a: None)
+    monkeypatch.setattr(K, "_raw_stream", lambda: 0)
+    monkeypatch.setattr(K, "_sms", lambda t: SMS)
+    monkeypatch.setattr(K.torch, "zeros", note)
+    if lists:
+        K.attn_pages(q, pool, pool, table, pos, seq, pages, 4, 2, 64, scale=0.1)
+    else:
+        K.attn_shared(q, pool, pool, table, row_start, pos0, None, 2, 4, 2, 64, scale=0.1)
+    assert alive == [[True]]
