@@ -518,7 +518,7 @@ int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const void* k_po
 int exl3_attn_shared(const void* q, int64_t q_stride, void* out, const void* k_pool, const void* v_pool, int64_t n_pages, const int* block_table, int bt_stride,
                      int bt_width, const int* row_start, const int* row_pos0, int rows, int T, const int* groups, int n_groups, int max_new, int nh, int nkv, int hd,
                      float scale, float* scratch, long long scratch_floats, cudaStream_t stream);
-// Codes left by bounded waits that ran out (0: none); cleared by the calls.
+// Codes left by bounded waits that ran out (0: none; attn_pages 2: rows of more tokens than max_new, too many to count); cleared by the calls.
 int exl3_attn_pages_status();
 int exl3_attn_shared_status();
 // Bounds of pages in 8 bits and the choice of pages by them (page_select.cu): codes int8 [pages, kv heads, 2, hd], scales float32 [pages, kv heads].

@@ -27,6 +27,8 @@ constexpr int PG_MAX_WIDTH = 1 << 19;          // pages of a row
 constexpr int PG_RING = PG_STAGES * PG_UNIT_BYTES;
 constexpr uint32_t PG_SMEM_RINGS = PG_WARPS * PG_RING;
 constexpr int PG_MAX_COLS = 16;                // queries of an item
+constexpr int PG_ITEMS = 42;                   // bits of a sum of places
+static_assert(PG_WINDOW <= 1024, "sums of 2^31 places and 2,048 items a row");
 
 static __device__ int g_pg_error = 0;
 
@@ -209,23 +211,27 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
     __syncthreads();
   }
-  unsigned long long totals = 0, upto = 0;     // items << 32 | places: of all rows, and of those up to this thread's last one
+  // items << PG_ITEMS | places: of all rows, and of those up to this thread's last one.  A row counts no more than 2,048 of the first (items matter where there are fewer than SMs) and
+  // 2^31 of the second, so that neither sum passes its bits.
+  unsigned long long totals = 0, upto = 0;
+  constexpr unsigned long long PLACES = (1ull << PG_ITEMS) - 1;
 #pragma unroll 1
   for (int i0 = 0; i0 < n_rows; i0 += PG_WARPS * 32) {
     const int i = i0 + threadIdx.x;
-    int blocks = 0, units = 0;
+    int units = 0;
+    int64_t blocks = 0;
     if (i < n_rows) {
       const int pos = sm.pos[i], queries = sm.n_new[i] * a.G, j = LIST ? -1 : sm.groups.of(a.row0 + i), shared = j < 0 ? -1 : sm.groups.pages[j];
       units = LIST ? min(a.count, pos < 0 ? 0 : pos / PG_PAGE + 1) * UPP : (min(pos + sm.n_new[i], most_keys) + KS - 1) / KS - max(shared, 0) * UPP;
       units = max(units, 1);                   // (one at least: every query gets an answer)
       sm.shared[i] = shared;
       sm.units[i] = units;
-      blocks = (!LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS) * a.nkv;
+      blocks = (int64_t)(!LIST && a.many && queries > PS_MANY ? 0 : (queries + COLS - 1) / COLS) * a.nkv;
       if (j >= 0) atomicAdd(&sm.group_queries[j], queries);
     }
     const int longest = __reduce_max_sync(0xffffffffu, blocks ? units : 0);
     if (lane == 0) atomicMax(&sm.most, longest);
-    unsigned long long incl = (unsigned long long)blocks << 32 | (unsigned int)((units + PG_SETUP) * blocks);
+    unsigned long long incl = (unsigned long long)min(blocks, (int64_t)2048) << PG_ITEMS | (unsigned long long)min((units + PG_SETUP) * blocks, (int64_t)1 << 31);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
     if (lane == 31) sm.warp_sum[warp] = incl;
@@ -233,10 +239,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     upto = totals + incl;
 #pragma unroll
     for (int w = 0; w < PG_WARPS; ++w) { if (w < warp) upto += sm.warp_sum[w]; totals += sm.warp_sum[w]; }
-    if (i < n_rows) sm.cum[i + 1] = (int)(unsigned int)upto;
+    if (i < n_rows) sm.cum[i + 1] = (int)(upto & PLACES);
     __syncthreads();
   }
-  int total = (int)(unsigned int)totals;
+  // The host has seen that rows of up to max_new tokens have fewer than 2^31 places; more tokens than that may have more: nothing is done for them, and the status says so.
+  const bool too_many = (totals & PLACES) > INT32_MAX;
+  if (too_many && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(&g_pg_error, 2);
+  int total = too_many ? 0 : (int)(totals & PLACES);
   if (threadIdx.x == 0) sm.cum[0] = 0;
   const bool beside = !LIST && a.n_groups > 0 && !a.many && a.rows <= a.window;     // the other kernel leaves this one some of the SMs
   if (beside)
@@ -251,13 +260,13 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
   int n_blocks = min(sms, max(1, total / (PG_WARPS * PG_MIN_UNITS))), setup = PG_SETUP, padded = 0;
   // Few items get a block each, padded to one length, where that makes no share much longer than equal shares are: no item is cut by blocks then, and no share has two items.
-  const int items = (int)(totals >> 32), each = (sm.most + PG_WARPS - 1) / PG_WARPS;
+  const int items = (int)(totals >> PG_ITEMS), each = (sm.most + PG_WARPS - 1) / PG_WARPS;
   if (items > 0 && items <= sms && n_rows <= PG_WARPS * 32 && each <= total / (n_blocks * PG_WARPS) + PG_ALONE) {
     n_blocks = items;
     setup = 0;
     padded = PG_WARPS * each;
     total = items * padded;
-    if ((int)threadIdx.x < n_rows) sm.cum[threadIdx.x + 1] = (int)(upto >> 32) * padded;
+    if ((int)threadIdx.x < n_rows) sm.cum[threadIdx.x + 1] = (int)(upto >> PG_ITEMS) * padded;
     __syncthreads();
   }
   if (!LIST && a.late && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.late, (total ? n_blocks : 0) + 1);

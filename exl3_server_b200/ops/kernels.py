@@ -1137,17 +1137,22 @@ def check_status() -> None:
     """Raises if a kernel with bounded waits (the tcgen05 GEMMs and attention, the TMA decode attention) gave up
     on one since the last call: its results are then not to be trusted.  Reads their flags from the device, so
     it waits for the work launched so far; call it where the host waits anyway."""
-    gave_up = [name for name, fn in (("gemm_tc", gemm_tc_status), ("gemm_skinny", gemm_skinny_status),
-                                     ("gemm_pair", gemm_pair_status),
-                                     ("attn_prefill_tc", attn_prefill_tc_status),
-                                     ("attn_decode", attn_decode_status),
-                                     ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status),
-                                     ("kv4_attn", kv4_attn_status), ("kv4_prompt", kv4_prompt_status), ("fp8_skinny", fp8_skinny_status),
-                                     ("fp8_wide", fp8_wide_status), ("attn_pages", attn_pages_status),
-                                     ("attn_shared", attn_shared_status)) if fn()]
+    codes = [(name, fn()) for name, fn in (("gemm_tc", gemm_tc_status), ("gemm_skinny", gemm_skinny_status),
+                                           ("gemm_pair", gemm_pair_status),
+                                           ("attn_prefill_tc", attn_prefill_tc_status),
+                                           ("attn_decode", attn_decode_status),
+                                           ("attn_latent", attn_latent_status), ("moe_gemm_tc", moe_tc_status),
+                                           ("kv4_attn", kv4_attn_status), ("kv4_prompt", kv4_prompt_status),
+                                           ("fp8_skinny", fp8_skinny_status),
+                                           ("fp8_wide", fp8_wide_status), ("attn_pages", attn_pages_status),
+                                           ("attn_shared", attn_shared_status))]
+    uncounted = ("attn_pages", 2) in codes
+    gave_up = [name for name, code in codes if code and not (uncounted and name == "attn_pages")]
     if gave_up:
         raise KernelLibraryError("a bounded wait ran out in " + ", ".join(gave_up) +
                                  ": a copy or a tensor-core product did not complete in time")
+    if uncounted:
+        raise KernelLibraryError("attn_shared: rows brought more tokens than max_new says, more than can be counted: nothing was done for their own pages")
 
 
 def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2283,7 +2288,7 @@ PAGES_MAX_GROUPS = 256      # groups of rows of one call
 
 
 def attn_pages_status() -> int:
-    """0, or the code the attention over pages left when a bounded wait ran out (cleared by this call)."""
+    """0, or the code the attention over pages left (cleared by this call): 1 when a bounded wait ran out, 2 when rows of more tokens than ``max_new`` were too many to count."""
     return int(library().exl3_attn_pages_status())
 
 

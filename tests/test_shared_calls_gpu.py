@@ -61,3 +61,25 @@ def test_rows_that_are_not_one_behind_the_other(d, groups):
     assert ws.untouched() and bool((out[T:] == 7.0).all())
     want, size = P.shared(case, 0.1)
     assert P.off(run_shared(case, scale=0.1), want, size) <= 1.0
+
+
+@pytest.mark.parametrize("news", [[1100], [600, 600]])
+def test_rows_of_more_tokens_than_said_that_cannot_be_counted(news):
+    """Rows bring hundreds of tokens where the call says one each, behind so many pages that their units pass 31 bits (a token's eight queries are an item of
+    more than 2^21 - 125 units: 1,025 of them are too many): the status says so, and nothing is written."""
+    k, width, T = K(), 1 << 19, sum(news)
+    pool = torch.zeros(1, 1, PAGE, 128, dtype=torch.bfloat16, device=DEV)
+    q, out = torch.zeros(T, 1024, dtype=torch.bfloat16, device=DEV), torch.full((T, 1024), 7.0, dtype=torch.bfloat16, device=DEV)
+    table = torch.full((len(news), width), -1, dtype=torch.int32, device=DEV)
+    start, pos0 = ints([sum(news[:i]) for i in range(len(news) + 1)]), ints([width * PAGE - 2000] * len(news))
+    ws = Guarded()
+    k.attn_shared(q, pool, pool, table, start, pos0, None, 1, 8, 1, 128, scale=0.1, workspace=ws, out=out)
+    torch.cuda.synchronize()
+    with pytest.raises(K().KernelLibraryError, match="more tokens than max_new"):
+        k.check_status()
+    assert bool((out == 7.0).all()) and ws.untouched()
+    k.check_status()
+    case = Paged([(100, 3)], 8, 1, 128, seed=42)            # (fewer than that are answered)
+    want, size = P.shared(case, 0.1)
+    case.max_new = 1
+    assert P.off(run_shared(case, groups=None, scale=0.1), want, size) <= 1.0
