@@ -829,16 +829,20 @@ struct PsChoice {
   bool many;                                   // whether rows of many tokens are the tensor cores' work
   int64_t tiles;                               // of a key/value head, at most; 0: no call of that kernel
 };
+// Groups are what may be shared, not what must be: where their tiles are more than the list holds, the rows read for themselves.
 static PsChoice ps_choose(int64_t T, int G, int rows, int n_groups, int max_new, int bt_width, int nkv, int hd) {
-  PsChoice c = {n_groups && pg_alone(rows, bt_width, max_new, G, nkv, hd) ? 0 : n_groups, false, 0};
-  const int64_t most = ps_most_tiles(T, G, c.groups, rows);
-  c.many = (int64_t)max_new * G > PS_MANY && rows <= PS_MAX_ROWS && most <= PS_MAX_TILES;
-  c.tiles = c.many ? most : c.groups ? T * G / PS_TILE + c.groups : 0;
-  return c;
+  auto fits = [&](int64_t tiles) { return tiles <= PS_MAX_TILES && tiles * (bt_width + PS_SETUP) * nkv <= INT32_MAX; };
+  const bool many = (int64_t)max_new * G > PS_MANY && rows <= PS_MAX_ROWS;
+  const int groups = n_groups && pg_alone(rows, bt_width, max_new, G, nkv, hd) ? 0 : n_groups;
+  const int64_t both = ps_most_tiles(T, G, groups, rows), shared = T * G / PS_TILE + groups, own = ps_most_tiles(T, G, 0, rows);
+  if (many && fits(both)) return {groups, true, both};
+  if (groups && fits(shared)) return {groups, false, shared};
+  if (many && fits(own)) return {0, true, own};
+  return {0, false, 0};
 }
 // Floats of scratch for it.
 static int64_t ps_floats(const PsChoice& c, int sms, int64_t T, int G, int nkv, int hd) {
-  return PG_COUNTERS + pg_record_floats(sms, hd) + (c.tiles ? ps_space(sms, T, G, nkv, hd, (int)std::min<int64_t>(c.tiles, PS_MAX_TILES)).end : 0);
+  return PG_COUNTERS + pg_record_floats(sms, hd) + (c.tiles ? ps_space(sms, T, G, nkv, hd, (int)c.tiles).end : 0);
 }
 
 // What both entry points ask of their arguments, and the pools' maps.
@@ -886,7 +890,7 @@ extern "C" long long exl3_attn_pages_scratch(int sms, int hd) { return PG_COUNTE
 extern "C" long long exl3_attn_shared_scratch(int sms, int T, int rows, int nh, int nkv, int hd, int n_groups, int max_new, int bt_width, int* chosen) {
   if (nkv < 1 || nh < nkv) return 0;
   const PsChoice c = ps_choose(T, nh / nkv, rows, n_groups, max_new, bt_width, nkv, hd);
-  if (chosen) { chosen[0] = c.groups; chosen[1] = c.many; chosen[2] = (int)std::min<int64_t>(c.tiles, INT32_MAX); }
+  if (chosen) { chosen[0] = c.groups; chosen[1] = c.many; chosen[2] = (int)c.tiles; }
   return ps_floats(c, sms, T, nh / nkv, nkv, hd);
 }
 
@@ -928,11 +932,6 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
   if (!scratch || scratch_floats < ps_floats(c, sms, T, nh / nkv, nkv, hd)) { set_error("attn_shared: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, rows, T, nh, nkv, scale, scratch);
   a.row_start = row_start; a.row_pos0 = row_pos0; a.bt_rows = rows; a.groups = groups; a.n_groups = n_groups;
-  if (tiles > PS_MAX_TILES || tiles * (bt_width + PS_SETUP) * nkv > INT32_MAX) {
-    set_error("attn_shared: %d tokens of %d query heads a key/value head with %d groups are more than %d tiles of %d queries, or tables of %d pages too wide for them", T, a.G, n_groups,
-              PS_MAX_TILES, PS_TILE, bt_width);
-    return ERR_UNSUPPORTED;
-  }
   a.tiles = tiles > 0;
   a.many = c.many;
   PsArgs p = {};

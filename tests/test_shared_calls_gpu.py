@@ -83,3 +83,19 @@ def test_rows_of_more_tokens_than_said_that_cannot_be_counted(news):
     want, size = P.shared(case, 0.1)
     case.max_new = 1
     assert P.off(run_shared(case, groups=None, scale=0.1), want, size) <= 1.0
+
+
+# ---- the limits of the tensor cores' list of tiles -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("prompts,new", [(20, 50), (22, 50)])
+def test_groups_on_both_sides_of_the_most_tiles(prompts, new):
+    """1,000 tokens of 128 heads are 500 tiles and 4 groups; 1,100 are 550, which is too many: the rows then read for themselves."""
+    shares = share([(prompts // 4, 1 + j) for j in range(4)], prompts - prompts // 4 * 4)
+    case = Paged([((s[1] * PAGE if s else 0) + r % 9, new) for r, s in enumerate(shares)], 128, 1, 64, share=shares, seed=43)
+    want, size = P.shared(case, 0.125)
+    table = torch.cat([case.table, torch.full((prompts, 20 - case.table.shape[1]), -1, dtype=torch.int32)], 1)
+    used, _, tiles = K()._shared_plan(148, prompts * new, prompts, 128, 1, 64, 4, new, 20)[1:]
+    assert (used, tiles) == ((4, 504) if prompts == 20 else (0, 0))
+    case.table = table
+    got = run_shared(case, ws=workspace(), little=True)
+    assert P.off(got, want, size) <= 1.0

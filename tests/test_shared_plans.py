@@ -31,8 +31,8 @@ def check(news, groups, heads, kv_heads, d, width):
     need, used, many, most = K._shared_plan(SMS, T, len(news), heads, kv_heads, d, len(groups), max(news), width)
     assert used in (0, len(groups))
     tiles = tiles_made(news, groups if used else [], heads // kv_heads, many)
-    assert tiles <= most
-    if 0 < most <= 512:
+    assert tiles <= most <= 512
+    if most:
         assert need >= floats_written(tiles, T, heads, kv_heads, d), (need, used, many, most)
     return used, many, most
 
@@ -44,6 +44,20 @@ def test_groups_that_are_left_alone(rows, new, heads, kv_heads, groups, width):
     cuts = [rows * i // groups for i in range(groups + 1)]
     used, many, most = check([new] * rows, [b - a for a, b in zip(cuts, cuts[1:])], heads, kv_heads, 64, width)
     assert used == 0 and many and most >= rows
+
+
+@pytest.mark.parametrize("news,heads,kv_heads,d,groups,width,want", [
+    ([98] * 62, 32, 1, 128, [20, 20, 22], 18, (0, False)),              # 759 tiles and more of the groups alone
+    ([8192], 32, 2, 128, [1], 400, (0, False)),                         # 512 and one
+    ([5, 8180], 32, 2, 128, [1], 400, (1, False)),                      # 512
+    ([1] * 512, 128, 1, 128, [2] * 256, 300, (256, False)),             # 512
+    ([1] * 514, 128, 1, 128, [2] * 256, 300, (0, False)),               # 513
+    ([1] * 64, 32, 8, 128, [64], 1 << 19, (1, False)),
+    ([1] * 64, 16384, 4096, 128, [64], 1 << 19, (0, False)),            # 2 tiles of 4,096 heads and 2^19 pages: more than 31 bits hold
+])
+def test_groups_are_never_why_a_call_is_refused(news, heads, kv_heads, d, groups, width, want):
+    """They say what may be read once: where their tiles are too many, rows read for themselves."""
+    assert check(news, groups, heads, kv_heads, d, width)[:2] == want
 
 
 @pytest.mark.parametrize("seed", range(8))
