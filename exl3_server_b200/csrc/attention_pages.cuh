@@ -115,9 +115,9 @@ struct PsToken { int shared_tile, shared_tok, own_tile, own_tok; };
 
 // A part of a tile that one block works on leaves its record at the slot block + place of the tile in the list: both ascend along it.
 __host__ __device__ constexpr int64_t ps_slots(int blocks, int nkv, int tiles) { return blocks + (int64_t)nkv * tiles; }
-// Tiles of a key/value head that a call may have, at most.
+// Tiles of a key/value head that a call may have, at most, where rows of many tokens have tiles of their own: the groups', and a row's own for each PS_TILE queries or part of them.
 __host__ __device__ constexpr int64_t ps_most_tiles(int64_t T, int G, int groups, int64_t rows) {
-  return T * G / PS_TILE + groups + (rows < T * G / (PS_MANY + 1) ? rows : T * G / (PS_MANY + 1)) + (T * G > PS_MANY ? T * G / PS_TILE : 0);
+  return (groups ? T * G / PS_TILE + groups : 0) + (rows < T * G / (PS_MANY + 1) ? rows : T * G / (PS_MANY + 1)) + (T * G > PS_MANY ? T * G / PS_TILE : 0);
 }
 // A record, in floats: the queries' maxima (base-2 units), their sums, their sums of values [query][hd].  A tile of up to 128 queries has a place for 256 all the
 // same: the two halves of a block then take its pages in turn, and leave a record's half each.

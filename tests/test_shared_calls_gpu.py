@@ -99,3 +99,13 @@ def test_groups_on_both_sides_of_the_most_tiles(prompts, new):
     case.table = table
     got = run_shared(case, ws=workspace(), little=True)
     assert P.off(got, want, size) <= 1.0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,tiles", [(600, 302), (1020, 512), (1022, 0)])
+def test_prompts_on_both_sides_of_the_most_tiles(new, tiles, d):
+    """128 heads: two tokens a tile, and one tile more for each row.  Beyond 512 of a key/value head the prompts' queries walk."""
+    case = Paged([(70, new - 3), (9, 3)], 128, 1, d, seed=44)
+    assert K()._shared_plan(148, new, 2, 128, 1, d, 0, new - 3, case.table.shape[1])[3] == tiles
+    want, size = P.shared(case, d ** -0.5)
+    assert P.off(run_shared(case, groups=None, ws=workspace()), want, size) <= 1.0

@@ -60,6 +60,15 @@ def test_groups_are_never_why_a_call_is_refused(news, heads, kv_heads, d, groups
     assert check(news, groups, heads, kv_heads, d, width)[:2] == want
 
 
+@pytest.mark.parametrize("news,heads,kv_heads,groups,want", [
+    ([8191], 64, 8, [], (True, 256)), ([8192], 64, 8, [], (True, 257)), ([4096], 32, 2, [], (True, 257)), ([8150], 32, 2, [], (True, 510)),
+    ([8176], 32, 2, [], (True, 512)), ([8192], 32, 2, [], (False, 0)),
+    ([100] * 60, 32, 2, [], (True, 435)), ([100] * 60, 32, 2, [60], (False, 376)),             # (a group's tiles are counted beside the rows')
+])
+def test_prompts_have_tiles_up_to_what_the_list_holds(news, heads, kv_heads, groups, want):
+    assert check(news, groups, heads, kv_heads, 64, 300)[1:] == want
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_scratch_holds_what_is_written(seed):
     """Rows, groups and tables on both sides of the limits."""
