@@ -889,7 +889,7 @@ extern "C" long long exl3_attn_pages_scratch(int sms, int hd) { return PG_COUNTE
 // The same for a call over rows; chosen (may be null): the groups that are used, whether rows of many tokens have tiles of their own, the most tiles of a key/value head.
 extern "C" long long exl3_attn_shared_scratch(int sms, int T, int rows, int nh, int nkv, int hd, int n_groups, int max_new, int bt_width, int* chosen) {
   if (nkv < 1 || nh < nkv) return 0;
-  const PsChoice c = ps_choose(T, nh / nkv, rows, n_groups, max_new, bt_width, nkv, hd);
+  const PsChoice c = ps_choose(T, nh / nkv, rows, n_groups, std::min(max_new, T), bt_width, nkv, hd);
   if (chosen) { chosen[0] = c.groups; chosen[1] = c.many; chosen[2] = (int)c.tiles; }
   return ps_floats(c, sms, T, nh / nkv, nkv, hd);
 }
@@ -926,6 +926,7 @@ extern "C" int exl3_attn_shared(const void* q, int64_t q_stride, void* out, cons
   }
   const int sms = pg_sms("attn_shared");
   if (!sms) return ERR_UNSUPPORTED;
+  max_new = std::min(max_new, T);              // (no row brings more)
   const PsChoice c = ps_choose(T, nh / nkv, rows, n_groups, max_new, bt_width, nkv, hd);
   const int64_t tiles = c.tiles;
   n_groups = c.groups;

@@ -109,3 +109,11 @@ def test_prompts_on_both_sides_of_the_most_tiles(new, tiles, d):
     assert K()._shared_plan(148, new, 2, 128, 1, d, 0, new - 3, case.table.shape[1])[3] == tiles
     want, size = P.shared(case, d ** -0.5)
     assert P.off(run_shared(case, groups=None, ws=workspace()), want, size) <= 1.0
+
+
+def test_more_new_tokens_allowed_than_there_are():
+    """``max_new`` says how many tokens a row may bring, not how many there are."""
+    case = Paged([(r % 90, 1) for r in range(1100)], 8, 1, 64, seed=45)
+    want, size = P.shared(case, 0.125)
+    case.max_new = 1 << 30
+    assert P.off(run_shared(case, groups=None, ws=workspace()), want, size) <= 1.0

@@ -117,3 +117,10 @@ def test_scratch_memory_lives_until_the_launch(lists, monkeypatch):
     else:
         K.attn_shared(q, pool, pool, table, row_start, pos0, None, 2, 4, 2, 64, scale=0.1)
     assert alive == [[True]]
+
+
+@pytest.mark.parametrize("rows,heads,groups,width", [(4, 8, 1, 20), (30, 2, 0, 20), (64, 8, 1, 200), (1500, 8, 3, 200)])
+def test_no_row_brings_more_than_all_tokens(rows, heads, groups, width):
+    """``max_new`` is a bound: one far above the tokens that there are changes nothing."""
+    plans = {K._shared_plan(SMS, rows, rows, heads, 1, 64, groups, most, width) for most in (rows, 1 << 24, 2 ** 31 - 1)}
+    assert len(plans) == 1
