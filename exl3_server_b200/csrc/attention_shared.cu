@@ -783,7 +783,7 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       const int i = i0 + b * SPLIT;
-      f[b] = 0.0f;
+      f[b] = -INFINITY;
       if (i < n) {
         int row = 0;
         const float* p = i < n01 ? part(i, row) : mine;
@@ -798,12 +798,13 @@ attn_shared_join_kernel(const int4* __restrict__ parts, int most_tiles, int slot
       }
     }
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) f[b] = i0 + b * SPLIT < n ? ps_exp2(f[b] - safe) : 0.0f;
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b)
+    for (int b = 0; b < BATCH; ++b) {
+      const bool seen = f[b] > -INFINITY;                            // (a part without a key leaves no sums)
+      const float w = ps_exp2(f[b] - safe);                          // (0 for one far below the others: its sums that are not finite are not, all the same)
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (f[b] != 0.0f) y[e] = fmaf(f[b], v[b][e], y[e]);          // (a part without a key leaves no sums)
+        if (seen) y[e] = fmaf(w, v[b][e], y[e]);
+    }
   }
   if (SPLIT > 1) {
 #pragma unroll

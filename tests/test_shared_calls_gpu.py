@@ -117,3 +117,29 @@ def test_more_new_tokens_allowed_than_there_are():
     want, size = P.shared(case, 0.125)
     case.max_new = 1 << 30
     assert P.off(run_shared(case, groups=None, ws=workspace()), want, size) <= 1.0
+
+
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("high", ["shared", "own"])
+def test_values_that_are_not_finite_behind_keys_of_no_weight(high, d, rows):
+    """The rows' own keys are so far below the shared ones (or these below them) that their weight rounds to zero: a value that is not finite is seen all the same, as where rows
+    read for themselves.  Few and many queries, which are joined differently."""
+    case = Paged([(4 * PAGE + 3, 1)] * rows, 8, 1, d, share=share([(rows, 4)]), seed=46)
+    shared, own = case.table[0, :4].long(), case.table[:, 4].long()
+    case.q.fill_(1.0)
+    case.k[:] = 4.0 if high == "own" else -4.0
+    case.k[shared] = -4.0 if high == "own" else 4.0
+    case.v[:] = torch.randn(case.v.shape, generator=torch.Generator().manual_seed(1)).bfloat16()
+    want, size = P.shared(case, 0.5)                        # scores of d * 2 and -d * 2: weights of e^-256 and less
+    if high == "own":
+        case.v[shared[1], :, 9, 5] = math.nan
+        case.v[shared[2], :, 60, 7] = math.inf
+    else:
+        case.v[own, :, 1, 5] = math.nan
+        case.v[own, :, 3, 7] = math.inf
+    rest = [i for i in range(d) if i not in (5, 7)]
+    for groups in ("own", None):
+        got = run_shared(case, groups=groups, scale=0.5, ws=workspace()).view(rows, 8, d)
+        assert not bool(torch.isfinite(got[..., [5, 7]]).any()), groups
+        assert P.off(got[..., rest], want.view(rows, 8, d)[..., rest], size.view(rows, 8, d)[..., rest]) <= 1.0
