@@ -41,7 +41,7 @@ struct PgArgs {
   const int* tok_pos;                          // lists: position and row of each token
   const int* tok_seq;
   const int* lists;                            // [tokens, kv heads, count]: pages of the row
-  int count, list_stride;                      // entries that are looked at, and that a list has
+  int count;                                   // entries of a list
   const int* row_start;                        // rows
   const int* row_pos0;
   int rows, T, nh, nkv, G;
@@ -182,8 +182,8 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll 1
   for (int i = threadIdx.x; i < n_rows; i += PG_WARPS * 32) {
     const int row = a.row0 + i;
-    // (a row beyond the table sees all of it)
-    sm.pos[i] = max(-most_keys, min(most_keys, __ldcg((LIST ? a.tok_pos : a.row_pos0) + row)));
+    // (a row beyond the table sees all of it; a listed token's position says how many entries are looked at, too)
+    sm.pos[i] = LIST ? __ldcg(a.tok_pos + row) : max(-most_keys, min(most_keys, __ldcg(a.row_pos0 + row)));
     const int start = LIST ? row : min(max(__ldcg(a.row_start + row), 0), a.T);
     sm.start[i] = start;
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);
@@ -325,7 +325,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       logical = logical_next;
       const int p = batch_p + (batches == 2 ? 0 : 32) + lane, row = a.row0 + ask.i, seq = LIST ? __ldcg(a.tok_seq + row) : row;
       const bool in = p * UPP < ask.units && seq >= 0 && seq < a.bt_rows;
-      logical_next = LIST ? in ? __ldcg(a.lists + ((int64_t)row * a.nkv + ask.g) * a.list_stride + p) : -1 : p + max(sm.shared[ask.i], 0);
+      logical_next = LIST ? in ? __ldcg(a.lists + ((int64_t)row * a.nkv + ask.g) * a.count + p) : -1 : p + max(sm.shared[ask.i], 0);
       page_next = in && logical_next >= 0 && logical_next < a.bt_width ? __ldcg(a.block_table + (int64_t)seq * a.bt_stride + logical_next) : -1;
       if (page_next >= a.n_pages) page_next = -1;
     }
@@ -907,8 +907,7 @@ extern "C" int exl3_attn_pages(const void* q, int64_t q_stride, void* out, const
   if (!sms) return ERR_UNSUPPORTED;
   if (!scratch || scratch_floats < exl3_attn_pages_scratch(sms, hd)) { set_error("attn_pages: scratch too small"); return ERR_SCRATCH; }
   PgArgs a = pg_args(q, q_stride, out, n_pages, block_table, bt_stride, bt_width, T, T, nh, nkv, scale, scratch);
-  a.tok_pos = tok_pos; a.tok_seq = tok_seq; a.lists = lists; a.count = std::min(count, bt_width);
-  a.list_stride = count; a.bt_rows = bt_rows;
+  a.tok_pos = tok_pos; a.tok_seq = tok_seq; a.lists = lists; a.count = count; a.bt_rows = bt_rows;
   return pg_launch<true>(a, map_k, map_v, hd, 1, sms, "attn_pages", stream);
 }
 

@@ -143,3 +143,21 @@ def test_values_that_are_not_finite_behind_keys_of_no_weight(high, d, rows):
         got = run_shared(case, groups=groups, scale=0.5, ws=workspace()).view(rows, 8, d)
         assert not bool(torch.isfinite(got[..., [5, 7]]).any()), groups
         assert P.off(got[..., rest], want.view(rows, 8, d)[..., rest], size.view(rows, 8, d)[..., rest]) <= 1.0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_lists_of_tokens_beyond_the_table(d):
+    """As many entries are looked at as the token's position has pages, however wide the table is; pages beyond the table are not there."""
+    case = Paged([(200, 1), (3000, 1), (130, 1)], 4, 2, d, seed=47)
+    case.table = case.table[:, :4].contiguous()
+    case.tok_pos[0] = case.pos0[0] = 1 << 30
+    lists = [[[-1, 9, -1, 4, 5, 1, 0], [-1, -1, -1, -1, -1, -1, 3]], [[50, 46, 40, 30, 2, 3, 1], [-1] * 5 + [0, 0]], [[-1, -1, 2, 1, 0, 0, 0], [7, 0, 1, 2, 2, 2, 2]]]
+    case.k[case.table[0].long()] = torch.randn(4, 2, PAGE, d, generator=torch.Generator().manual_seed(2)).bfloat16()      # (the whole of row 0's pages is seen)
+    case.v[case.table[0].long()] = torch.randn(4, 2, PAGE, d, generator=torch.Generator().manual_seed(3)).bfloat16()
+    flat = Paged([(255, 1), (255, 1), (130, 1)], 4, 2, d, seed=47)      # the same rows, as far as the table goes
+    flat.table, flat.k, flat.v, flat.q = case.table, case.k, case.v, case.q
+    looked = [[[p if 0 <= p < 4 else -1 for p in entries] for entries in token] for token in lists]
+    # (the plain form looks at as many entries as pages up to its position: the ones that count, first)
+    looked[0], looked[1] = ([sorted(entries, key=lambda p: p < 0) for entries in looked[t]] for t in (0, 1))
+    want, size = P.listed(flat, looked, d ** -0.5)
+    assert P.off(base.run_listed(case, ints(lists), ws=workspace()), want, size) <= 1.0
