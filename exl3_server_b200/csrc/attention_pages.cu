@@ -183,7 +183,7 @@ attn_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   for (int i = threadIdx.x; i < n_rows; i += PG_WARPS * 32) {
     const int row = a.row0 + i;
     // (a row beyond the table sees all of it; a listed token's position says how many entries are looked at, too)
-    sm.pos[i] = LIST ? __ldcg(a.tok_pos + row) : max(-most_keys, min(most_keys, __ldcg(a.row_pos0 + row)));
+    sm.pos[i] = LIST ? __ldcg(a.tok_pos + row) : max(PG_LOWEST, min(most_keys, __ldcg(a.row_pos0 + row)));
     const int start = LIST ? row : min(max(__ldcg(a.row_start + row), 0), a.T);
     sm.start[i] = start;
     sm.n_new[i] = LIST ? 1 : max(0, min(__ldcg(a.row_start + row + 1), a.T) - start);

@@ -7,6 +7,7 @@ namespace exl3 {
 
 constexpr int PG_PAGE = 64;                    // tokens of a page
 constexpr int PG_MAX_GROUPS = 256;             // groups of rows that share pages, in one call
+constexpr int PG_LOWEST = -(1 << 30);          // positions below count as this one: its sums with keys and tokens stay within 32 bits
 constexpr int PG_COUNTERS = 65536;             // ints at the start of the scratch memory: zero between launches
 
 // ---- the groups -------------------------------------------------------------------------------------------------------------

@@ -231,7 +231,7 @@ __device__ inline void ps_tiles(PsTiles& t, const PsArgs& a) {
     if (j >= 0 && s1 > s0) atomicMin(&t.group_seen[j], pos_of(r));
     if (s1 > s0) {                             // (as the walk does)
       const int blocks = ((s1 - s0) * a.G + a.cols - 1) / a.cols;
-      places += (int64_t)(PG_SETUP + max(1, (min(max(pos_of(r), -most) + s1 - s0, most) + ks - 1) / ks - (j >= 0 ? t.groups.pages[j] : 0) * (PG_PAGE / ks))) * blocks;
+      places += (int64_t)(PG_SETUP + max(1, (min(max(pos_of(r), PG_LOWEST) + s1 - s0, most) + ks - 1) / ks - (j >= 0 ? t.groups.pages[j] : 0) * (PG_PAGE / ks))) * blocks;
     }
     if (r < n_rows) t.row_tile[r] = s1 > s0 && (int64_t)(s1 - s0) * a.G > PS_MANY ? (s1 - s0) * a.G : 0;
   }

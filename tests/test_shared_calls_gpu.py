@@ -161,3 +161,15 @@ def test_lists_of_tokens_beyond_the_table(d):
     looked[0], looked[1] = ([sorted(entries, key=lambda p: p < 0) for entries in looked[t]] for t in (0, 1))
     want, size = P.listed(flat, looked, d ** -0.5)
     assert P.off(base.run_listed(case, ints(lists), ws=workspace()), want, size) <= 1.0
+
+
+@pytest.mark.parametrize("others", [0, 1100])
+def test_positions_far_before_everything(others):
+    """A row that begins further below position 0 than its table is long, walked (beside more rows than have tiles) and in tiles: its later tokens see what they see."""
+    case = Paged([(0, 100)] + [(0, 0)] * others, 1, 1, 64, seed=48)
+    case.table = case.table[:, :1].contiguous()
+    case.pos0[0] = -70
+    case.tok_pos = list(range(-70, 30))
+    want, size = P.shared(case, 0.125)
+    got = run_shared(case, groups=None)
+    assert P.off(got, want, size) <= 1.0 and bool((got[:70] == 0).all())
