@@ -407,6 +407,7 @@ extern "C" int exl3_page_bounds_load(const void* codes, const float* scales, int
                                      cudaStream_t stream) {
   if (n == 0) return 0;
   if (n < 0 || nkv < 1 || (hd != 64 && hd != 128) || n_pages < 1 || !codes || !scales || !pages || !low || !high) { set_error("page_bounds_load: bad sizes or a missing array"); return ERR_BAD_ARGUMENT; }
+  if (!aligned16(codes) || !aligned16(low) || !aligned16(high)) { set_error("page_bounds_load: the codes and the bounds must be 16-byte aligned"); return ERR_ALIGNMENT; }
   const int64_t total = (int64_t)n * nkv * hd;
   launch_pdl(page_bounds_load_kernel, dim3((unsigned)((total / 4 + 255) / 256)), dim3(256), 0, stream, static_cast<const int8_t*>(codes), scales, n_pages, pages, total, nkv, hd, low, high);
   return launch_status("page_bounds_load");

@@ -124,3 +124,19 @@ def test_no_row_brings_more_than_all_tokens(rows, heads, groups, width):
     """``max_new`` is a bound: one far above the tokens that there are changes nothing."""
     plans = {K._shared_plan(SMS, rows, rows, heads, 1, 64, groups, most, width) for most in (rows, 1 << 24, 2 ** 31 - 1)}
     assert len(plans) == 1
+
+
+@pytest.mark.parametrize("off", [1, 4])
+def test_codes_of_bounds_that_are_not_aligned(off):
+    """Refused by all that read or write them, before anything is launched."""
+    flat = torch.zeros(4 * 2 * 2 * 64 + 16, dtype=torch.int8)
+    codes = flat[(-flat.data_ptr()) % 16 + off:].data_ptr()
+    x = torch.zeros(4096, dtype=torch.float32)
+    p = x.data_ptr() + (-x.data_ptr()) % 16
+    for call in (
+        lambda: K._entry("exl3_page_bounds_load", "pplpiiipp")(codes, p, 4, p, 1, 2, 64, p, p, 0),
+        lambda: K._entry("exl3_page_bounds", "plpiippiiiipp")(p, 4, p, 2, 2, p, p, 1, 1, 2, 64, codes, p, 0),
+        lambda: K._entry("exl3_page_select", "plpplpiiippiiiiiiip")(p, 256, codes, p, 4, p, 2, 2, 1, p, p, 1, 4, 2, 64, 1, 1, 1, p, 0),
+    ):
+        with pytest.raises(K.KernelLibraryError, match="aligned"):
+            K._check(call(), "bounds")
