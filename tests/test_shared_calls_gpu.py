@@ -173,3 +173,76 @@ def test_positions_far_before_everything(others):
     want, size = P.shared(case, 0.125)
     got = run_shared(case, groups=None)
     assert P.off(got, want, size) <= 1.0 and bool((got[:70] == 0).all())
+
+
+# ---- arrays that are laid out otherwise -------------------------------------------------------------------------------------------------
+
+def cut(x, left=8, right=24):
+    """The same matrix as part of a wider one."""
+    whole = torch.full((x.shape[0], left + x.shape[1] + right), math.nan if x.is_floating_point() else -7, dtype=x.dtype, device=DEV)
+    whole[:, left:left + x.shape[1]] = x.to(DEV)
+    return whole[:, left:left + x.shape[1]]
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (16, 2, 128), (32, 1, 128)])
+@pytest.mark.parametrize("rows,groups", [
+    ([(5 * PAGE + 3, 1), (5 * PAGE, 1), (5 * PAGE + 99, 1), (7, 1)], [(3, 5)]),
+    ([(PAGE, 90), (PAGE + 70, 130), (300, 2)], [(2, 1)]),
+    ([(20, 150), (0, 1)], []),
+])
+def test_shared_with_strided_queries_and_tables(heads, kv_heads, d, rows, groups):
+    case = Paged(rows, heads, kv_heads, d, share=share(groups, len(rows) - sum(n for n, _ in groups)), seed=50)
+    want, size = P.shared(case, d ** -0.5)
+    table = cut(wide(case, case.table.to(DEV)), 3, 5)
+    assert not table.is_contiguous()
+    got = K().attn_shared(cut(case.q), case.k.to(DEV), case.v.to(DEV), table, ints(case.start), ints(case.pos0), ints(case.groups).view(-1, 3), case.max_new, heads, kv_heads, d,
+                          scale=d ** -0.5, workspace=workspace())
+    torch.cuda.synchronize()
+    K().check_status()
+    assert P.off(got, want, size) <= 1.0
+
+
+@pytest.mark.parametrize("width", [0, 600, 32768])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (16, 2, 128)])
+def test_choice_with_strided_queries_and_wide_tables(heads, kv_heads, d, width):
+    """Bounds, choice and attention over a table that is part of a wider one, and as wide as a recorded step's may be."""
+    k, case = K(), Paged([(1500, 1), (90, 2), (0, 1)], heads, kv_heads, d, seed=51)
+    table = case.table.to(DEV)
+    if width:
+        table = torch.cat([table, torch.full((3, width - table.shape[1]), -1, dtype=torch.int32, device=DEV)], 1)
+    table = cut(table, 3, 5)
+    codes, scales = k.page_bounds_pool(case.k.shape[0], kv_heads, d, DEV)
+    lens = [c + n for c, n in case.rows]
+    k.page_bounds(case.k.to(DEV), codes, scales, table, ints([sum(lens[:i]) for i in range(4)]), ints([0] * 3), max(lens))
+    pages = k.page_select(cut(case.q), codes, scales, table, ints(case.tok_pos), ints(case.tok_seq), 5, heads, kv_heads, d, first=1, last=2)
+    want = [P.choose(case, codes.cpu(), scales.cpu(), t, 5, 1, 2) for t in range(4)]
+    assert pages.tolist() == want
+    y = k.attn_pages(cut(case.q), case.k.to(DEV), case.v.to(DEV), table, ints(case.tok_pos), ints(case.tok_seq), pages, heads, kv_heads, d, scale=0.1, workspace=workspace())
+    torch.cuda.synchronize()
+    k.check_status()
+    right, size = P.listed(case, want, 0.1)
+    assert P.off(y, right, size) <= 1.0
+
+
+# ---- more rows than a launch of the walk takes ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new", [1, 3, 33])
+def test_groups_among_more_rows_than_a_launch_takes(new):
+    """1,200 rows: groups in the first launch, across both and in the second; a row of many tokens has no tile of its own then."""
+    groups = share([(300, 2), (400, 1)], 100) + [(9, 1)] * 350 + [None] * 50
+    case = Paged([((s[1] * PAGE if s else 0) + r % 9, new if r % 400 == 7 else 1 + r % min(new, 3)) for r, s in enumerate(groups)], 4, 2, 64, share=groups, seed=52)
+    want, size = P.shared(case, 0.125)
+    assert P.off(run_shared(case, ws=workspace()), want, size) <= 1.0
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_tables_so_wide_that_a_launch_takes_few_rows(new):
+    """Rows of 2^18 pages for 16 heads of 128: 127 of one token fill 31 bits of units."""
+    shares = share([(150, 3)], 20)
+    case = Paged([((s[1] * PAGE if s else 0) + r % 9, new if r % 60 == 0 else 1) for r, s in enumerate(shares)], 16, 16, 128, share=shares, seed=53)
+    want, size = P.shared(case, 0.1)
+    table = case.table
+    case.table = torch.full((len(shares), 1 << 18), -1, dtype=torch.int32)
+    case.table[:, :table.shape[1]] = table
+    for groups in ("own", None):
+        assert P.off(run_shared(case, groups=groups, ws=workspace(), scale=0.1, little=True), want, size) <= 1.0
