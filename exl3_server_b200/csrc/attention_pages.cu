@@ -4,6 +4,7 @@
 //   s[j] = (q . K[j]) * scale  over the keys of the listed pages at positions <= pos;   out = sum_j softmax(s)[j] V[j]
 //
 // One pass with running maximum and sum (float32; probabilities are rounded to bfloat16 for the second product, as in the other attention kernels here).
+// Which queries walk, which have tiles and how much scratch memory that takes is settled in one place (ps_choose).
 // Bound by memory: a key and a value are read once, for all query heads of their head and all tokens of the item (64 tokens, 64 chosen pages each of 32 heads of 128 on 8: 1.04 GB
 // in 184 us, 5.7 TB/s).  Mean blocks end at 137 us of these and the last at 168: equal shares of bytes are not equal times for all SMs.  Few and short rows take what
 // a chain of dependent reads takes, row, page number, page, softmax: 8 to 15 us.

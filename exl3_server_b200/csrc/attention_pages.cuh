@@ -70,8 +70,9 @@ constexpr int PG_SETUP = 3;
 
 // Both kernels run side by side where there is work for both: the tensor cores' takes some of the SMs and leaves the others to the walk, whose streams of pages fill the memory's queue
 // from fewer SMs than there are (a batch of 64 behind 4,096 shared keys, 32 heads of 128 on 8, 30 to 2,000 keys of their own: one after the other 117 us, side by side 80).  Both work out
-// how many, in units of 10 ns of an SM: `tiles` for the tiles' pages (180 for two sets of queries, 60 for one), PG_COST for a place of the walk (8 queries an item, PG_COST_16: 16), PG_START
-// for what the walk takes however many SMs it has; and the time that the memory takes for its units (8 KB in 1.25 ns).  16 rows of up to 500 keys behind 2,048 pages, 32 heads on 2:
+// how many, in units of about 10 ns of an SM: `tiles` for the tiles' pages (180 for two sets of queries, 60 for one), PG_COST for a place of the walk (8 queries an item, PG_COST_16: 16), PG_START
+// for what the walk takes however many SMs it has; and the time that the memory takes for its units (8 KB in 1.25 ns).  These are weights that were fitted to the three batches named here, with
+// heads of 64 and 128 alike, and not costs: a tile's page by itself takes 110 and 52 (ps_tile_cost).  16 rows of up to 500 keys behind 2,048 pages, 32 heads on 2:
 // without PG_START and with 16 for all the walk had 2 SMs and the call took 102 us, with them 69.5; 48 rows in 5 groups 50 and 46; 24 or 40 for PG_COST_16: 76.7 or 69.6, 48.1 or 47.9.
 constexpr int64_t PS_COST_TWO = 180, PS_COST_ONE = 60, PG_COST = 16, PG_COST_16 = 32, PG_START = 400;
 __host__ __device__ inline int ps_sms(int64_t tiles, int64_t places, int cols, int sms) {
@@ -92,9 +93,9 @@ __device__ inline int64_t ps_cost(int queries, int pages) {
 }
 
 // Where rows have many tokens: whether a group's tiles cost less than its rows reading the pages each for itself, in 10 ns of an SM.  Tiles: a page 1.1 us for two sets of queries, 0.52 for one; a group's way in
-// and out PS_SETUP pages, and 0.04 us a query to join.  Rows: tiles of their own where they have many queries, else the walk.  37 prompts of 41 to 252 tokens
-// behind one page, 36 heads of 64: 219 us when they shared it, 167; 62 of 99 to 128 tokens behind 16 to 19 pages in three groups 399 and 353; 24 of 16 to 120 behind
-// 94 pages, 32 heads of 128 on 8, share them: 220 and 260.  (Steps of few tokens a row are not asked: the pass over the rows costs 1 us, and short ones leave groups alone anyhow.)
+// and out PS_SETUP pages, and 0.04 us a query to join.  Rows: tiles of their own where they have many queries, else the walk.  Both sides measured, shared and each for itself: 37 prompts of 41 to
+// 252 tokens behind one page, 36 heads of 64, 216 and 171 us; 62 of 99 to 128 tokens behind 16 to 19 pages in three groups, 36 heads of 64, 404 and 335 (8 heads of 128: 157 and 130); 24 of 16 to
+// 120 behind 94 pages, 32 heads of 128 on 8, 224 and 266: only these share.  (Steps of few tokens a row are not asked: the pass over the rows costs 1 us, and short ones leave groups alone anyhow.)
 __device__ inline int64_t ps_tile_cost(int queries) { return (int64_t)(queries / PS_TILE) * 110 + (queries % PS_TILE > 128 ? 110 : queries % PS_TILE > 0 ? 52 : 0); }
 __device__ inline int ps_alone(int queries, int cols, int hd) {                    // a page, for a row's queries
   return queries > PS_MANY ? (int)ps_tile_cost(queries) : (queries + cols - 1) / cols * (hd == 64 ? 2 : 4) * (int)(cols == 8 ? PG_COST : PG_COST_16);

@@ -34,8 +34,9 @@ __device__ inline float pb_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ inline float pb_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ inline int pb_code(float x, float inv) { return (int)fminf(fmaxf(rintf(__fmul_rn(x, inv)), -127.0f), 127.0f); }
 
-// A warp for each (page that got new keys, key/value head): one read of the page.  Bound by memory where there are many (8,192 tokens of 36 heads of 64, 38 MB: with the load of these
-// bounds 16 us, 19 when the loads were conditional and so one after the other), else by the chain row, page number, page (64 rows' last pages and their load: 8.2 us).
+// A warp for each (page that got new keys, key/value head): one read of the page.  Where there are many it is bound by the bytes that a warp has on their way (8,192 tokens of 36 heads of 64, 38 MB: with
+// the load of these bounds 16 us, 0.4 of the copy rate; 19 when the loads were conditional and so one after the other), else by the chain row, page number, page (64 rows' last pages and their
+// load: 8.2 us).
 template <int HD>
 __global__ void __launch_bounds__(PB_WARPS * 32)
 page_bounds_kernel(const __nv_bfloat16* __restrict__ k_pool, int64_t n_pages, const int* __restrict__ block_table, int bt_stride, int bt_width,
@@ -58,7 +59,8 @@ page_bounds_kernel(const __nv_bfloat16* __restrict__ k_pool, int64_t n_pages, co
   uint32_t mn[4], mx[4], odd = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) { mn[i] = 0x7f807f80u; mx[i] = 0xff80ff80u; }
-  // Sixteen loads in flight a lane; behind the last token it is read again, which changes no bound.
+  // Loads that depend on no condition, so that several of a lane are on their way at once: as many as 33 registers (heads of 128; 34 of 64) hold, far fewer than the sixteen of a round.  Behind the
+  // last token it is read again, which changes no bound.
 #pragma unroll 1
   for (int t0 = 0; t0 < PB_PAGE / TOK && t0 * TOK < filled; t0 += 16) {
     uint4 w[16];

@@ -2397,6 +2397,8 @@ def attn_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, blo
     ``groups``: int32 ``[n, 3]`` on the device, ascending: the rows ``first .. first + rows - 1`` have their first ``pages`` pages in common, the same in each one's table,
     which are read once for all of them where that is the faster way (None: no groups).  Their tokens see all of these keys: positions from ``64 * pages - 1`` on.  Groups do not overlap (one that
     begins before the one ahead of it ends is no group).  Pages that are not there are left out; a query that sees nothing gets zeros.
+    Groups, and rows of more than 64 queries a key/value head, are worked on in up to 512 tiles of 256 queries a key/value head; where that is too few, or there are more than
+    1,024 rows (for the rows' own pages), rows read their pages for every 16 queries again.
     ``workspace``: an ``engine.batch.Workspace`` that the scratch memory comes from (None: torch's)."""
     T, pitch = _paged_q(q, heads, kv_heads, head_dim, "attn_shared")
     _positive(scale, "attn_shared")
