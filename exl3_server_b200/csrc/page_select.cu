@@ -59,7 +59,7 @@ page_bounds_kernel(const __nv_bfloat16* __restrict__ k_pool, int64_t n_pages, co
   uint32_t mn[4], mx[4], odd = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) { mn[i] = 0x7f807f80u; mx[i] = 0xff80ff80u; }
-  // Loads that depend on no condition, so that several of a lane are on their way at once: as many as 33 registers (heads of 128; 34 of 64) hold, far fewer than the sixteen of a round.  Behind the
+  // Loads that depend on no condition, so that several of a lane are on their way at once: as many as 33 registers (heads of 128; 34 of 64) hold, far fewer than the sixteen asked for.  Behind the
   // last token it is read again, which changes no bound.
 #pragma unroll 1
   for (int t0 = 0; t0 < PB_PAGE / TOK && t0 * TOK < filled; t0 += 16) {
